@@ -43,6 +43,7 @@ extern "C" {
 #define PKV_DEVERR_WAIT_TIMEOUT 2
 #define PKV_DEVERR_BAD_SLOT 3
 #define PKV_DEVERR_SEQ_TOO_LONG 4 /* seq_len beyond the block-table width */
+#define PKV_DEVERR_BAD_POSITION 5 /* position outside the rotary table */
 
 /* Element types of floating-point KV inputs. */
 #define PKV_DTYPE_F32 0
@@ -281,6 +282,67 @@ int pkv_write_to_cache(const void *key, const void *value, int32_t dtype,
                        int64_t num_blocks, int32_t block_size,
                        int32_t num_kv_heads, int32_t head_dim, void *workspace,
                        size_t workspace_bytes, void *stream);
+
+/*
+ * Per-head RMS norm and rotary position of queries and keys in one pass:
+ *   n = x / sqrt(mean(x^2) + eps) * weight     (left out when both weights
+ *                                               are NULL)
+ *   a' = a cos - b sin, b' = b cos + a sin     over the first rotary_dim
+ * channels of each head, pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) when
+ * `interleaved`; later channels are not rotated.  q [num_tokens, num_heads,
+ * head_dim] and k [num_tokens, num_kv_heads, head_dim] (PKV_DTYPE_*) have
+ * their own token and head strides, in elements, and contiguous channels;
+ * q_out and k_out are contiguous and do not overlap the inputs.  rotary is
+ * float32 [num_positions, rotary_dim]: rotary_dim / 2 cosines, then as many
+ * sines.  positions int64 [num_tokens]; a position outside the table records
+ * PKV_DEVERR_BAD_POSITION and its token's rows become zero.  The weights
+ * [head_dim] are float32 when weights_f32, else of the inputs' type.  The
+ * arithmetic is in 32 bits, rounded once to the output.  num_kv_heads may be
+ * 0 (k unused).  head_dim <= 256, rotary_dim even and <= head_dim.
+ */
+int pkv_qk_norm_rope(const void *q, const void *k, int32_t dtype, void *q_out,
+                     void *k_out, const int64_t *positions,
+                     const float *rotary, const void *q_weight,
+                     const void *k_weight, int32_t weights_f32, float eps,
+                     int64_t num_tokens, int32_t num_heads,
+                     int32_t num_kv_heads, int32_t head_dim,
+                     int32_t rotary_dim, int64_t num_positions,
+                     int32_t interleaved, int64_t q_token_stride,
+                     int64_t q_head_stride, int64_t k_token_stride,
+                     int64_t k_head_stride, void *stream);
+
+/*
+ * Appends keys and values to the vLLM-shaped cache kv_cache int8 [2,
+ * num_blocks, block_size, num_kv_heads, head_dim] / scale_cache fp32 [2,
+ * num_blocks, num_kv_heads], keeping the earlier tokens of a started page
+ * readable (pkv_write_to_cache replaces a page's scale by that of the
+ * call's tokens).  Keys are rotated on the way (as pkv_qk_norm_rope, each
+ * 32-bit product and sum rounded) when positions and rotary are given.  Per
+ * (page, head, K or V) with new tokens:
+ *   step  = absmax(new values) / 127     (0 when that is 0 or NaN)
+ *   scale = step, or 1 when step is 0    if the call writes offset 0: a page
+ *                                        begun by this call
+ *         = max(old scale, step)         otherwise
+ *   codes at offsets below the lowest one written become
+ *   rint(code * (old scale / scale)) where the scale grew; new codes are
+ *   rint(value / scale), clamped to [-127, 127]; other codes stay.
+ * slot_mapping int64 [num_tokens] holds block * block_size + offset; slot -1
+ * is padding and skipped; other slots outside the cache record
+ * PKV_DEVERR_BAD_SLOT and are skipped.  Of equal slots the last token
+ * counts.  key and value have token and head strides, in elements.
+ * block_size <= 64, head_dim <= 256.
+ */
+size_t pkv_append_kv_workspace_size(int64_t num_tokens, int64_t num_blocks);
+int pkv_append_kv(const void *key, const void *value, int32_t dtype,
+                  int8_t *kv_cache, float *scale_cache,
+                  const int64_t *slot_mapping, const int64_t *positions,
+                  const float *rotary, int64_t num_tokens, int64_t num_blocks,
+                  int32_t block_size, int32_t num_kv_heads, int32_t head_dim,
+                  int32_t rotary_dim, int64_t num_positions,
+                  int32_t interleaved, int64_t k_token_stride,
+                  int64_t k_head_stride, int64_t v_token_stride,
+                  int64_t v_head_stride, void *workspace,
+                  size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -368,4 +368,112 @@ int pkv_write_to_cache(const void* key, const void* value, int32_t dtype, int8_t
                                     workspace, workspace_bytes, as_stream(stream));
 }
 
+static int check_rotary(int32_t head_dim, int32_t rotary_dim, int64_t num_positions) {
+  if (head_dim <= 0 || head_dim > 256)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "head_dim must be 1 to 256");
+  if (rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 2 != 0)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "rotary_dim must be even and at most head_dim");
+  if (num_positions < 0) return fail(PKV_ERR_INVALID_ARGUMENT, "negative num_positions");
+  return PKV_OK;
+}
+
+int pkv_qk_norm_rope(const void* q, const void* k, int32_t dtype, void* q_out, void* k_out,
+                     const int64_t* positions, const float* rotary, const void* q_weight,
+                     const void* k_weight, int32_t weights_f32, float eps, int64_t num_tokens,
+                     int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                     int32_t rotary_dim, int64_t num_positions, int32_t interleaved,
+                     int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
+                     int64_t k_head_stride, void* stream) {
+  clear_error();
+  if (num_tokens < 0 || num_heads < 0 || num_kv_heads < 0)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "invalid qk_norm_rope shape");
+  if (dtype < 0 || dtype > 2)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "q/k must be float32, float16 or bfloat16");
+  int rc = check_rotary(head_dim, rotary_dim, num_positions);
+  if (rc != PKV_OK) return rc;
+  if (num_tokens > 0 && ((num_heads > 0 && (!q || !q_out)) || (num_kv_heads > 0 && (!k || !k_out)) ||
+                         !positions || (rotary_dim > 0 && !rotary)))
+    return fail(PKV_ERR_INVALID_ARGUMENT, "null input or output pointer");
+  const bool norm = q_weight != nullptr || k_weight != nullptr;
+  if (norm && ((num_heads > 0 && !q_weight) || (num_kv_heads > 0 && !k_weight)))
+    return fail(PKV_ERR_INVALID_ARGUMENT, "q_weight and k_weight go together");
+  if (num_tokens * ((int64_t)num_heads + num_kv_heads) > 0x7fffffffLL)
+    return fail(PKV_ERR_UNSUPPORTED, "more than 2^31 - 1 rows in one call");
+  pkv::QkNormRopeArgs a;
+  a.q = q;
+  a.k = num_kv_heads > 0 ? k : q;
+  a.q_out = q_out;
+  a.k_out = num_kv_heads > 0 ? k_out : q_out;
+  a.dtype = dtype;
+  a.q_token_stride = q_token_stride;
+  a.q_head_stride = q_head_stride;
+  a.k_token_stride = num_kv_heads > 0 ? k_token_stride : 0;
+  a.k_head_stride = num_kv_heads > 0 ? k_head_stride : 0;
+  a.positions = positions;
+  a.table = rotary;
+  a.q_weight = q_weight ? q_weight : k_weight;
+  a.k_weight = k_weight ? k_weight : q_weight;
+  a.weight_f32 = weights_f32 != 0;
+  a.tokens = num_tokens;
+  a.table_rows = num_positions;
+  a.heads = num_heads;
+  a.kv_heads = num_kv_heads;
+  a.dim = head_dim;
+  a.rot = rotary_dim;
+  a.eps = eps;
+  a.interleaved = interleaved != 0;
+  return pkv::launch_qk_norm_rope(a, as_stream(stream));
+}
+
+size_t pkv_append_kv_workspace_size(int64_t num_tokens, int64_t num_blocks) {
+  if (num_tokens <= 0 || num_blocks <= 0) return 0;
+  return pkv::append_kv_workspace_size(num_tokens, num_blocks);
+}
+
+int pkv_append_kv(const void* key, const void* value, int32_t dtype, int8_t* kv_cache,
+                  float* scale_cache, const int64_t* slot_mapping, const int64_t* positions,
+                  const float* rotary, int64_t num_tokens, int64_t num_blocks, int32_t block_size,
+                  int32_t num_kv_heads, int32_t head_dim, int32_t rotary_dim,
+                  int64_t num_positions, int32_t interleaved, int64_t k_token_stride,
+                  int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                  void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  if (num_tokens < 0 || num_blocks < 0 || num_kv_heads <= 0)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "invalid append_kv shape");
+  if (block_size <= 0 || block_size > 64)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "supports block_size <= 64");
+  if (dtype < 0 || dtype > 2)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "key/value must be float32, float16 or bfloat16");
+  const int rc = check_rotary(head_dim, positions ? rotary_dim : 0, num_positions);
+  if (rc != PKV_OK) return rc;
+  if (num_tokens > 0 && (positions == nullptr) != (rotary == nullptr))
+    return fail(PKV_ERR_INVALID_ARGUMENT, "positions and rotary go together");
+  if (num_tokens > 0 && (!key || !value || !kv_cache || !scale_cache || !slot_mapping))
+    return fail(PKV_ERR_INVALID_ARGUMENT, "null input or output pointer");
+  if (num_tokens > 0x7ffffffeLL || num_blocks > 0x7ffffffeLL)
+    return fail(PKV_ERR_UNSUPPORTED, "more than 2^31 - 2 tokens or blocks");
+  pkv::AppendKvArgs a;
+  a.key = key;
+  a.value = value;
+  a.dtype = dtype;
+  a.k_token_stride = k_token_stride;
+  a.k_head_stride = k_head_stride;
+  a.v_token_stride = v_token_stride;
+  a.v_head_stride = v_head_stride;
+  a.cache = kv_cache;
+  a.scales = scale_cache;
+  a.slots = slot_mapping;
+  a.positions = positions;
+  a.table = rotary;
+  a.tokens = num_tokens;
+  a.blocks = num_blocks;
+  a.table_rows = num_positions;
+  a.block_size = block_size;
+  a.kv_heads = num_kv_heads;
+  a.dim = head_dim;
+  a.rot = rotary_dim;
+  a.interleaved = interleaved != 0;
+  return pkv::launch_append_kv(a, workspace, workspace_bytes, as_stream(stream));
+}
+
 }  // extern "C"

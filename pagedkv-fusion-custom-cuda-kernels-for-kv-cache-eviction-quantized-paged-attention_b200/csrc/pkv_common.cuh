@@ -27,6 +27,7 @@ enum DeviceError : int {
   kDevWaitTimeout = 2,    // a bounded barrier wait gave up
   kDevBadSlot = 3,        // slot_mapping entry outside the cache
   kDevSeqTooLong = 4,     // seq_len needs more pages than the block table has
+  kDevBadPosition = 5,    // position outside the rotary table
 };
 
 // Pages a decode split may read for a sequence: ceil(L / bs), clamped to the

@@ -44,6 +44,44 @@ int launch_write_to_cache(const void* key, const void* value, int dtype, int8_t*
                           void* workspace, size_t workspace_bytes, cudaStream_t stream);
 size_t write_to_cache_workspace_size(int64_t num_tokens, int num_kv_heads);
 
+// ---- rotary.cu ------------------------------------------------------------
+struct QkNormRopeArgs {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  int dtype;  // 0 fp32, 1 fp16, 2 bf16
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;  // elements
+  const int64_t* positions;
+  const float* table;  // [table_rows, rot]: cos | sin
+  const void* q_weight;  // nullable with k_weight: no norm
+  const void* k_weight;
+  bool weight_f32;
+  int64_t tokens, table_rows;
+  int heads, kv_heads, dim, rot;
+  float eps;
+  bool interleaved;
+};
+int launch_qk_norm_rope(const QkNormRopeArgs& a, cudaStream_t stream);
+
+struct AppendKvArgs {
+  const void* key;
+  const void* value;
+  int dtype;
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;  // elements
+  int8_t* cache;
+  float* scales;
+  const int64_t* slots;
+  const int64_t* positions;  // nullable: no rotation
+  const float* table;
+  int64_t tokens, blocks, table_rows;
+  int block_size, kv_heads, dim, rot;
+  bool interleaved;
+};
+size_t append_kv_workspace_size(int64_t tokens, int64_t blocks);
+int launch_append_kv(const AppendKvArgs& a, void* workspace, size_t workspace_bytes,
+                     cudaStream_t stream);
+
 // ---- eviction.cu ----------------------------------------------------------
 int launch_eviction_scores(const float* recency, const float* frequency, const float* attn,
                            const uint8_t* valid, float* scores, int64_t num_blocks,

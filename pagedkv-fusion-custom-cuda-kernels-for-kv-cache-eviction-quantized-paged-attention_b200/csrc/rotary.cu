@@ -1,0 +1,767 @@
+// Rotary positions: per-head RMS norm + rotation of queries and keys in one
+// pass (qk_norm_rope), and the append of keys and values to the INT8 paged
+// cache with the rotation applied on the way (append_kv).
+//
+// The rotation of one pair (a, b) at position p with table entry (c, s):
+//   a' = a c - b s,   b' = b c + a s
+// in 32 bits with each product and sum rounded on its own, so that the INT8
+// codes of append_kv have one defined value.  Pairs are (i, i + R/2) (half
+// layout) or (2i, 2i + 1) (interleaved); channels from R on pass unchanged.
+// The table is float32 [P, R]: R/2 cosines, then R/2 sines per position.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <string>
+
+#include "pkv_common.cuh"
+#include "pkv_internal.h"
+#include "quantize_math.cuh"
+
+namespace pkv {
+namespace {
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+
+__device__ __forceinline__ float rot_first(float a, float b, float c, float s) {
+  return __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
+}
+__device__ __forceinline__ float rot_second(float a, float b, float c, float s) {
+  return __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
+}
+
+// N consecutive values of T as 32-bit words (N * sizeof(T) = 4, 8 or 16
+// bytes, or a single value), loaded and stored in one access.
+template <typename T, int N>
+struct alignas(N * sizeof(T)) Chunk {
+  T e[N];
+};
+
+template <typename T, int N>
+__device__ __forceinline__ Chunk<T, N> load_chunk(const T* p) {
+  Chunk<T, N> c;
+  if constexpr (N * sizeof(T) == 16) {
+    *reinterpret_cast<uint4*>(c.e) = *reinterpret_cast<const uint4*>(p);
+  } else if constexpr (N * sizeof(T) == 8) {
+    *reinterpret_cast<uint2*>(c.e) = *reinterpret_cast<const uint2*>(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) c.e[i] = p[i];
+  }
+  return c;
+}
+
+// ---------------------------------------------------------------------------
+// qk_norm_rope
+// ---------------------------------------------------------------------------
+
+template <typename T>
+struct QkArgs {
+  const T* q;
+  const T* k;
+  T* q_out;
+  T* k_out;
+  int64_t q_tok, q_head, k_tok, k_head;  // input strides in elements
+  const int64_t* positions;
+  const float* table;
+  const void* q_weight;  // both null: no norm
+  const void* k_weight;
+  bool weight_f32;  // weights in float32, else in T
+  int64_t tokens;
+  int heads, kv_heads, dim, rot;
+  int64_t table_rows;
+  float eps;
+};
+
+// A group of LPR lanes (a power of two) owns RPG rows (token, head) of one
+// token; lane l holds chunks l and (NC = 2) l + LPR of VEC channels, one
+// 16-byte access each.  The partners of the half layout are R/2 channels
+// away, in another lane: their raw words come by shuffle, so a row is read
+// once.  The table entries of a lane are the same for all its rows.
+// What bounds it: HBM (a row is read and written once); RPG = 4 keeps four
+// independent loads in flight and reads the table a quarter as often.
+template <typename T, int VEC, int LPR, int NC, int RPG, bool NORM, bool INTER>
+__global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkArgs<T> a, int* err) {
+  const int rows = a.heads + a.kv_heads;
+  const int per_token = (rows + RPG - 1) / RPG;
+  const int lane = threadIdx.x & 31, gl = lane & (LPR - 1), g0 = lane - gl;
+  const int64_t group = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const int64_t token = group / per_token;
+  const int sub = (int)(group - token * per_token);
+  const bool live = token < a.tokens;  // every lane stays for the shuffles
+  const int chunks = a.dim / VEC, half = a.rot / 2;
+  int64_t pos = live ? a.positions[token] : 0;
+  const bool bad = pos < 0 || pos >= a.table_rows;
+  if (bad) {
+    if (gl == 0) record_error(err, kDevBadPosition);
+    pos = 0;
+  }
+  const float* row = a.table + pos * a.rot;
+
+  alignas(16) float cs[NC][VEC], sn[NC][VEC];
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int d = (gl + i * LPR) * VEC;
+    if (live && d < a.rot) {
+      if constexpr (INTER) {
+        const int p = d / 2;
+#pragma unroll
+        for (int e = 0; e < VEC / 2; ++e) {
+          cs[i][e] = p + e < half ? row[p + e] : 1.0f;
+          sn[i][e] = p + e < half ? row[half + p + e] : 0.0f;
+        }
+      } else {
+        const int p = d < half ? d : d - half;
+#pragma unroll
+        for (int e = 0; e < VEC; e += 4) {
+          *reinterpret_cast<float4*>(&cs[i][e]) = *reinterpret_cast<const float4*>(row + p + e);
+          *reinterpret_cast<float4*>(&sn[i][e]) =
+              *reinterpret_cast<const float4*>(row + half + p + e);
+        }
+      }
+    }
+  }
+
+  Chunk<T, VEC> x[RPG][NC];
+#pragma unroll
+  for (int r = 0; r < RPG; ++r) {
+    const int h = sub + r * per_token;
+    if (live && h < rows) {
+      const T* src = h < a.heads ? a.q + token * a.q_tok + (int64_t)h * a.q_head
+                                 : a.k + token * a.k_tok + (int64_t)(h - a.heads) * a.k_head;
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        if (gl + i * LPR < chunks) x[r][i] = load_chunk<T, VEC>(src + (gl + i * LPR) * VEC);
+    }
+  }
+
+#pragma unroll
+  for (int r = 0; r < RPG; ++r) {
+    const int h = sub + r * per_token;
+    const bool on = live && h < rows;
+    if (RPG > 1 && !__any_sync(0xffffffffu, on)) break;
+    const bool is_q = h < a.heads;
+    float rstd = 1.0f;
+    const void* w = is_q ? a.q_weight : a.k_weight;
+    if constexpr (NORM) {
+      float ss = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        if (on && gl + i * LPR < chunks)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const float v = to_f32<T>(x[r][i].e[e]);
+            ss = fmaf(v, v, ss);
+          }
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      rstd = rsqrtf(ss / (float)a.dim + a.eps);
+    }
+    auto weight = [&](int d) {
+      if constexpr (!NORM) {
+        return 1.0f;
+      } else {
+        return a.weight_f32 ? static_cast<const float*>(w)[d]
+                            : to_f32<T>(static_cast<const T*>(w)[d]);
+      }
+    };
+    T* dst = is_q ? a.q_out + (token * a.heads + h) * (int64_t)a.dim
+                  : a.k_out + (token * a.kv_heads + (h - a.heads)) * (int64_t)a.dim;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = gl + i * LPR, d = c * VEC;
+      Chunk<T, VEC> other;
+      if constexpr (!INTER) {
+        // the partner chunk of a rotated chunk, from whichever lane and slot
+        // holds it (every lane of the warp takes part in the shuffles)
+        const int pc = d < half ? c + half / VEC : c - half / VEC;
+        constexpr int W = VEC * sizeof(T) / 4;
+        uint32_t* o32 = reinterpret_cast<uint32_t*>(other.e);
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+          const uint32_t* v32 = reinterpret_cast<const uint32_t*>(x[r][j].e);
+#pragma unroll
+          for (int u = 0; u < W; ++u) {
+            const uint32_t v = __shfl_sync(0xffffffffu, v32[u], g0 + (pc & (LPR - 1)));
+            if (NC == 1 || pc / LPR == j) o32[u] = v;
+          }
+        }
+      }
+      if (!on || c >= chunks) continue;
+      float y[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        y[e] = to_f32<T>(x[r][i].e[e]);
+        if constexpr (NORM) y[e] = y[e] * rstd * weight(d + e);
+      }
+      if (d < a.rot) {
+        if constexpr (INTER) {
+#pragma unroll
+          for (int e = 0; e < VEC; e += 2) {
+            const float p = y[e], q = y[e + 1];
+            if (d + e < a.rot) {
+              y[e] = rot_first(p, q, cs[i][e / 2], sn[i][e / 2]);
+              y[e + 1] = rot_second(p, q, cs[i][e / 2], sn[i][e / 2]);
+            }
+          }
+        } else {
+          const int pd = d < half ? d + half : d - half;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            float p = to_f32<T>(other.e[e]);
+            if constexpr (NORM) p = p * rstd * weight(pd + e);
+            y[e] = d < half ? rot_first(y[e], p, cs[i][e], sn[i][e])
+                            : rot_second(p, y[e], cs[i][e], sn[i][e]);
+          }
+        }
+      }
+      Chunk<T, VEC> out;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) out.e[e] = from_f32<T>(bad ? 0.0f : y[e]);
+      if constexpr (VEC * sizeof(T) == 16)
+        *reinterpret_cast<uint4*>(dst + d) = *reinterpret_cast<const uint4*>(out.e);
+    }
+  }
+}
+
+// Any head_dim, rotary width, alignment and stride: one warp per row, one
+// value per access, the partner value read from memory again.
+template <typename T, bool NORM>
+__global__ void __launch_bounds__(256)
+    qk_norm_rope_scalar_kernel(QkArgs<T> a, bool interleaved, int* err) {
+  const int rows = a.heads + a.kv_heads;
+  const int lane = threadIdx.x & 31;
+  const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int64_t token = unit / rows;
+  if (token >= a.tokens) return;  // whole warps
+  const int h = (int)(unit - token * rows);
+  const bool is_q = h < a.heads;
+  const int half = a.rot / 2;
+  const int64_t pos = a.positions[token];
+  const bool bad = pos < 0 || pos >= a.table_rows;
+  if (bad && lane == 0) record_error(err, kDevBadPosition);
+  const float* row = a.table + (bad ? 0 : pos) * a.rot;
+  const T* src = is_q ? a.q + token * a.q_tok + (int64_t)h * a.q_head
+                      : a.k + token * a.k_tok + (int64_t)(h - a.heads) * a.k_head;
+  T* dst = is_q ? a.q_out + (token * a.heads + h) * (int64_t)a.dim
+                : a.k_out + (token * a.kv_heads + (h - a.heads)) * (int64_t)a.dim;
+  const void* w = is_q ? a.q_weight : a.k_weight;
+  float rstd = 1.0f;
+  if constexpr (NORM) {
+    float ss = 0.0f;
+    for (int d = lane; d < a.dim; d += 32) {
+      const float v = to_f32<T>(src[d]);
+      ss = fmaf(v, v, ss);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    rstd = rsqrtf(ss / (float)a.dim + a.eps);
+  }
+  auto value = [&](int d) {
+    const float v = to_f32<T>(src[d]);
+    if constexpr (!NORM) {
+      return v;
+    } else {
+      return v * rstd * (a.weight_f32 ? static_cast<const float*>(w)[d]
+                                      : to_f32<T>(static_cast<const T*>(w)[d]));
+    }
+  };
+  for (int d = lane; d < a.dim; d += 32) {
+    float y = value(d);
+    if (d < a.rot) {
+      const bool first = interleaved ? (d & 1) == 0 : d < half;
+      const int i = interleaved ? d / 2 : (first ? d : d - half);
+      const float p = value(interleaved ? d ^ 1 : (first ? d + half : d - half));
+      y = first ? rot_first(y, p, row[i], row[half + i]) : rot_second(p, y, row[i], row[half + i]);
+    }
+    dst[d] = from_f32<T>(bad ? 0.0f : y);
+  }
+}
+
+template <typename T, int VEC, int LPR, int NC, bool NORM, bool INTER>
+void launch_qk_rows(const QkArgs<T>& a, cudaStream_t stream) {
+  const int rows = a.heads + a.kv_heads;
+  constexpr int kGroups = 256 / LPR;
+  // Few rows: one row per group, so that the call spreads over the SMs.
+  if (a.tokens * rows <= 148LL * 4 * kGroups) {
+    const int64_t groups = a.tokens * rows;
+    qk_norm_rope_kernel<T, VEC, LPR, NC, 1, NORM, INTER>
+        <<<(unsigned)((groups + kGroups - 1) / kGroups), 256, 0, stream>>>(a, device_error_word());
+  } else {
+    const int64_t groups = a.tokens * ((rows + 3) / 4);
+    qk_norm_rope_kernel<T, VEC, LPR, NC, 4, NORM, INTER>
+        <<<(unsigned)((groups + kGroups - 1) / kGroups), 256, 0, stream>>>(a, device_error_word());
+  }
+}
+
+template <typename T, bool NORM, bool INTER>
+bool launch_qk_vec(const QkArgs<T>& a, cudaStream_t stream) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int chunks = a.dim / VEC;
+  if (chunks <= 4) launch_qk_rows<T, VEC, 4, 1, NORM, INTER>(a, stream);
+  else if (chunks <= 8) launch_qk_rows<T, VEC, 8, 1, NORM, INTER>(a, stream);
+  else if (chunks <= 16) launch_qk_rows<T, VEC, 16, 1, NORM, INTER>(a, stream);
+  else if (chunks <= 32) launch_qk_rows<T, VEC, 32, 1, NORM, INTER>(a, stream);
+  else if (chunks <= 64) launch_qk_rows<T, VEC, 32, 2, NORM, INTER>(a, stream);
+  else return false;
+  return true;
+}
+
+template <typename T>
+int launch_qk_t(const QkNormRopeArgs& p, cudaStream_t stream) {
+  QkArgs<T> a;
+  a.q = static_cast<const T*>(p.q);
+  a.k = static_cast<const T*>(p.k);
+  a.q_out = static_cast<T*>(p.q_out);
+  a.k_out = static_cast<T*>(p.k_out);
+  a.q_tok = p.q_token_stride;
+  a.q_head = p.q_head_stride;
+  a.k_tok = p.k_token_stride;
+  a.k_head = p.k_head_stride;
+  a.positions = p.positions;
+  a.table = p.table;
+  a.q_weight = p.q_weight;
+  a.k_weight = p.k_weight;
+  a.weight_f32 = p.weight_f32;
+  a.tokens = p.tokens;
+  a.heads = p.heads;
+  a.kv_heads = p.kv_heads;
+  a.dim = p.dim;
+  a.rot = p.rot;
+  a.table_rows = p.table_rows;
+  a.eps = p.eps;
+  const bool norm = p.q_weight != nullptr;
+  constexpr int VEC = 16 / sizeof(T);
+  auto aligned = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };
+  const bool strides = a.q_tok % VEC == 0 && a.q_head % VEC == 0 && a.k_tok % VEC == 0 &&
+                       a.k_head % VEC == 0;
+  const bool rot_ok = p.interleaved ? a.rot % 2 == 0 : (a.rot % 8 == 0 && (a.rot / 2) % VEC == 0);
+  const bool vec = a.dim % VEC == 0 && strides && rot_ok && aligned(a.q) && aligned(a.k) &&
+                   aligned(a.q_out) && aligned(a.k_out) && aligned(a.table);
+  if (vec) {
+    const bool done = norm ? (p.interleaved ? launch_qk_vec<T, true, true>(a, stream)
+                                            : launch_qk_vec<T, true, false>(a, stream))
+                           : (p.interleaved ? launch_qk_vec<T, false, true>(a, stream)
+                                            : launch_qk_vec<T, false, false>(a, stream));
+    if (done) return kOk;
+  }
+  const int64_t units = a.tokens * (a.heads + a.kv_heads);
+  const unsigned grid = (unsigned)((units + 7) / 8);
+  if (norm)
+    qk_norm_rope_scalar_kernel<T, true><<<grid, 256, 0, stream>>>(a, p.interleaved,
+                                                                  device_error_word());
+  else
+    qk_norm_rope_scalar_kernel<T, false><<<grid, 256, 0, stream>>>(a, p.interleaved,
+                                                                   device_error_word());
+  return kOk;
+}
+
+// ---------------------------------------------------------------------------
+// append_kv
+// ---------------------------------------------------------------------------
+//
+// A work unit is (page touched by the call, K or V): the call's tokens in
+// that page set its scale together.  Up to kAppendScan tokens every CTA finds
+// its page's tokens by scanning the slots itself (one launch); above that, an
+// index kernel first chains the runs of consecutive tokens per page.
+
+constexpr int kAppendThreads = 256;
+constexpr int kAppendWarps = kAppendThreads / 32;
+constexpr int kAppendMaxPage = 64;  // largest block_size
+constexpr int kAppendHold = 16;     // tokens of a head kept in registers
+
+template <typename T>
+struct AppendArgs {
+  const T* key;
+  const T* value;
+  int64_t k_tok, k_head, v_tok, v_head;
+  int8_t* cache;
+  float* scales;
+  const int64_t* slots;
+  const int64_t* positions;  // null: no rotation
+  const float* table;
+  int64_t tokens, blocks, table_rows;
+  int bs, kv_heads, dim, rot;
+  bool interleaved;
+};
+
+// Slot of token t, or -1 where the token is not to be written: the padding
+// slot -1, a slot outside the cache, a position outside the table.
+template <typename T>
+__device__ __forceinline__ int64_t append_slot(const AppendArgs<T>& a, int64_t t, int* err) {
+  const int64_t slot = a.slots[t];
+  if (slot == -1) return -1;
+  if (slot < 0 || slot >= a.blocks * a.bs) {
+    record_error(err, kDevBadSlot);
+    return -1;
+  }
+  if (a.positions != nullptr) {
+    const int64_t p = a.positions[t];
+    if (p < 0 || p >= a.table_rows) {
+      record_error(err, kDevBadPosition);
+      return -1;
+    }
+  }
+  return slot;
+}
+
+// Chunk c (VEC channels) of token t's head h, rotated when it is a key.
+template <typename T, int VEC, int NC>
+__device__ __forceinline__ void append_load(const AppendArgs<T>& a, bool is_key, int64_t t, int h,
+                                            int c, bool on, float (&y)[VEC]) {
+  const T* src = is_key ? a.key + t * a.k_tok + (int64_t)h * a.k_head
+                        : a.value + t * a.v_tok + (int64_t)h * a.v_head;
+  Chunk<T, VEC> x;
+  if (on) x = load_chunk<T, VEC>(src + c * VEC);
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) y[e] = on ? to_f32<T>(x.e[e]) : 0.0f;
+  if (!is_key || a.positions == nullptr) return;  // uniform for the CTA
+  const int half = a.rot / 2, d = c * VEC;
+  const float* row = a.table + a.positions[t] * a.rot;
+  if (a.interleaved && VEC > 1) {
+#pragma unroll
+    for (int e = 0; e + 1 < VEC; e += 2) {
+      if (on && d + e < a.rot) {
+        const float cc = row[(d + e) / 2], ss = row[half + (d + e) / 2];
+        const float p = y[e], q = y[e + 1];
+        y[e] = rot_first(p, q, cc, ss);
+        y[e + 1] = rot_second(p, q, cc, ss);
+      }
+    }
+    return;
+  }
+  const bool first = a.interleaved ? (d & 1) == 0 : d < half;
+  Chunk<T, VEC> o;
+  if (VEC > 1 && NC == 1) {  // the partner chunk is another lane's
+    constexpr int W = VEC * sizeof(T) / 4 > 0 ? VEC * sizeof(T) / 4 : 1;
+    const int pc = first ? c + half / VEC : c - half / VEC;
+    const uint32_t* v32 = reinterpret_cast<const uint32_t*>(x.e);
+    uint32_t* o32 = reinterpret_cast<uint32_t*>(o.e);
+#pragma unroll
+    for (int u = 0; u < W; ++u) o32[u] = __shfl_sync(0xffffffffu, v32[u], pc & 31);
+  } else if (on && d < a.rot) {
+    const int pd = a.interleaved ? d ^ 1 : (first ? d + half : d - half);
+    o = load_chunk<T, VEC>(src + pd);
+  }
+  if (!on || d >= a.rot) return;
+  const int i = a.interleaved ? d / 2 : (first ? d : d - half);
+  alignas(16) float cc[VEC], ss[VEC];
+  if constexpr (VEC == 4) {
+    *reinterpret_cast<float4*>(cc) = *reinterpret_cast<const float4*>(row + i);
+    *reinterpret_cast<float4*>(ss) = *reinterpret_cast<const float4*>(row + half + i);
+  } else {
+    cc[0] = row[i];
+    ss[0] = row[half + i];
+  }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    const float p = to_f32<T>(o.e[e]);
+    y[e] = first ? rot_first(y[e], p, cc[e], ss[e]) : rot_second(p, y[e], cc[e], ss[e]);
+  }
+}
+
+// One page, K or V.  s_tok[offset] is the call's token for that offset or -1.
+// A warp owns a head: absmax of the new values, the page's scale, the earlier
+// codes moved to a larger scale, the new codes.  Up to kAppendHold tokens of
+// up to 128 channels stay in registers between the two steps (one read of the
+// inputs); more are read again (from L2).
+template <typename T, int VEC, int NC>
+__device__ void append_page(const AppendArgs<T>& a, int64_t page, bool is_key, const int* s_tok,
+                            int* s_list) {
+  __shared__ int s_meta[2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (warp == 0) {  // compact list of (offset, token), ascending offsets
+    int n = 0, lowest = a.bs;
+    for (int b = 0; b < a.bs; b += 32) {
+      const int off = b + lane;
+      const int t = off < a.bs ? s_tok[off] : -1;
+      const unsigned m = __ballot_sync(0xffffffffu, t >= 0);
+      if (t >= 0) {
+        const int at = n + __popc(m & ((1u << lane) - 1u));
+        s_list[2 * at] = off;
+        s_list[2 * at + 1] = t;
+      }
+      if (m != 0 && lowest == a.bs) lowest = b + __ffs(m) - 1;
+      n += __popc(m);
+    }
+    if (lane == 0) {
+      s_meta[0] = n;
+      s_meta[1] = lowest;
+    }
+  }
+  __syncthreads();
+  const int n = s_meta[0], lowest = s_meta[1];
+  const int chunks = a.dim / VEC;
+  const int64_t tok_stride = (int64_t)a.kv_heads * a.dim;
+  int8_t* page_base = a.cache + (is_key ? 0 : a.blocks * a.bs * tok_stride) +
+                      page * a.bs * tok_stride;
+  float* scale_base = a.scales + (is_key ? 0 : a.blocks * a.kv_heads) + page * a.kv_heads;
+  constexpr bool kHold = NC == 1 && VEC == 4;
+  for (int h = warp; h < a.kv_heads; h += kAppendWarps) {
+    float held[kHold ? kAppendHold : 1][VEC];
+    uint32_t m = 0u;
+    auto fold = [&](const float (&y)[VEC]) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) m = max(m, __float_as_uint(y[e]) & 0x7fffffffu);
+    };
+    const bool hold = kHold && n <= kAppendHold;
+    if (hold) {
+#pragma unroll
+      for (int i = 0; i < (kHold ? kAppendHold : 1); ++i)
+        if (i < n) {
+          append_load<T, VEC, NC>(a, is_key, s_list[2 * i + 1], h, lane, lane < chunks, held[i]);
+          fold(held[i]);
+        }
+    } else {
+      for (int i = 0; i < n; ++i)
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+          float y[VEC];
+          append_load<T, VEC, NC>(a, is_key, s_list[2 * i + 1], h, lane + 32 * j,
+                                  lane + 32 * j < chunks, y);
+          fold(y);
+        }
+    }
+    m = __reduce_max_sync(0xffffffffu, m);  // NaN bits exceed +inf: NaN wins
+    const float amax = __uint_as_float(m);
+    const float step = amax > 0.0f ? __fdiv_rn(amax, 127.0f) : 0.0f;
+    float old = 0.0f;
+    if (lowest > 0) old = scale_base[h];
+    const bool grow = step > old;
+    const float sc = lowest == 0 ? (step > 0.0f ? step : 1.0f) : (grow ? step : old);
+    __syncwarp();  // every lane has the old scale
+    if (lane == 0) scale_base[h] = sc;
+    if (lowest > 0 && grow) {
+      const float ratio = __fdiv_rn(old, sc);
+      for (int off = 0; off < lowest; ++off) {
+        int8_t* row = page_base + off * tok_stride + (int64_t)h * a.dim;
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+          const int c = lane + 32 * j;
+          if (c < chunks) {
+            if constexpr (VEC == 4) {
+              const uint32_t w = *reinterpret_cast<const uint32_t*>(row + 4 * c);
+              uint32_t r = 0u;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float v = (float)(int8_t)(w >> (8 * e));
+                r |= (uint32_t)(__float2int_rn(__fmul_rn(v, ratio)) & 255) << (8 * e);
+              }
+              *reinterpret_cast<uint32_t*>(row + 4 * c) = r;
+            } else {
+              row[c] = (int8_t)__float2int_rn(__fmul_rn((float)row[c], ratio));
+            }
+          }
+        }
+      }
+    }
+    const float rcp = __frcp_rn(sc);
+    const bool fast = isfinite(amax) && !isinf(rcp);
+    auto store = [&](int off, int c, const float (&y)[VEC]) {
+      int8_t* dst = page_base + off * tok_stride + (int64_t)h * a.dim + c * VEC;
+      if constexpr (VEC == 4)
+        *reinterpret_cast<uint32_t*>(dst) = quantize_word(y, sc, rcp, fast);
+      else
+        *dst = (int8_t)quantize_one(y[0], sc);
+    };
+    if (hold) {
+#pragma unroll
+      for (int i = 0; i < (kHold ? kAppendHold : 1); ++i)
+        if (i < n && lane < chunks) store(s_list[2 * i], lane, held[i]);
+    } else {
+      for (int i = 0; i < n; ++i)
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+          const int c = lane + 32 * j;
+          float y[VEC];
+          append_load<T, VEC, NC>(a, is_key, s_list[2 * i + 1], h, c, c < chunks, y);
+          if (c < chunks) store(s_list[2 * i], c, y);
+        }
+    }
+  }
+}
+
+// Up to kAppendScan tokens: CTA (t, K/V) handles the page of token t if no
+// earlier token of the call is in that page.
+template <typename T, int VEC, int NC>
+__global__ void __launch_bounds__(kAppendThreads) append_scan_kernel(AppendArgs<T> a, int* err) {
+  __shared__ int s_tok[kAppendMaxPage], s_list[2 * kAppendMaxPage];
+  __shared__ int s_taken;
+  const int64_t t = blockIdx.x >> 1;
+  const bool is_key = (blockIdx.x & 1) == 0;
+  const int64_t slot = append_slot(a, t, err);
+  if (slot < 0) return;  // whole CTA
+  const int64_t page = slot / a.bs;
+  for (int i = threadIdx.x; i < a.bs; i += kAppendThreads) s_tok[i] = -1;
+  if (threadIdx.x == 0) s_taken = 0;
+  __syncthreads();
+  for (int64_t u = threadIdx.x; u < a.tokens; u += kAppendThreads) {
+    const int64_t su = append_slot(a, u, err);
+    if (su < 0 || su / a.bs != page) continue;
+    if (u < t) s_taken = 1;
+    atomicMax(&s_tok[su % a.bs], (int)u);  // of equal slots the last token counts
+  }
+  __syncthreads();
+  if (s_taken) return;  // whole CTA
+  append_page<T, VEC, NC>(a, page, is_key, s_tok, s_list);
+}
+
+// Index of larger calls.  A run head (a token whose predecessor is not in the
+// same page) pushes itself on its page's list: head[page] = last pushed + 1
+// (0: none), next[t] = the one before.  The first to push lists the page.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    append_index_kernel(AppendArgs<T> a, int* head, int* next, int* pages, int* count, int* err) {
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t >= a.tokens) return;
+  const int64_t slot = append_slot(a, t, err);
+  if (slot < 0) return;
+  const int64_t page = slot / a.bs;
+  if (t > 0) {
+    const int64_t before = append_slot(a, t - 1, err);
+    if (before >= 0 && before / a.bs == page) return;
+  }
+  const int prev = atomicExch(&head[page], (int)t + 1);
+  next[t] = prev;
+  if (prev == 0) pages[atomicAdd(count, 1)] = (int)page;
+}
+
+template <typename T, int VEC, int NC>
+__global__ void __launch_bounds__(kAppendThreads)
+    append_pages_kernel(AppendArgs<T> a, const int* head, const int* next, const int* pages,
+                        const int* count, int* err) {
+  __shared__ int s_tok[kAppendMaxPage], s_list[2 * kAppendMaxPage];
+  const int units = 2 * *count;
+  for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    const int64_t page = pages[u >> 1];
+    __syncthreads();  // the previous unit is done with s_tok and s_list
+    for (int i = threadIdx.x; i < a.bs; i += kAppendThreads) s_tok[i] = -1;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      for (int link = head[page]; link != 0; link = next[link - 1]) {
+        for (int64_t t0 = link - 1; t0 < a.tokens; t0 += 32) {
+          const int64_t t = t0 + threadIdx.x;
+          const int64_t slot = t < a.tokens ? append_slot(a, t, err) : -1;
+          const bool in = slot >= 0 && slot / a.bs == page;
+          // the run ends at the first token of another page
+          const unsigned out = __ballot_sync(0xffffffffu, !in);
+          const int len = out == 0 ? 32 : __ffs(out) - 1;
+          if ((int)threadIdx.x < len) atomicMax(&s_tok[slot % a.bs], (int)t);
+          if (len < 32) break;
+        }
+      }
+    }
+    __syncthreads();
+    append_page<T, VEC, NC>(a, page, (u & 1) == 0, s_tok, s_list);
+  }
+}
+
+// Largest call that scans its slots in every CTA.
+constexpr int64_t kAppendScan = 512;
+
+template <typename T, int VEC, int NC>
+void launch_append_n(const AppendArgs<T>& a, int* ws, cudaStream_t stream) {
+  int* err = device_error_word();
+  if (a.tokens <= kAppendScan) {
+    append_scan_kernel<T, VEC, NC><<<(unsigned)(2 * a.tokens), kAppendThreads, 0, stream>>>(a, err);
+    return;
+  }
+  int* head = ws;
+  int* count = ws + a.blocks;
+  int* next = count + 1;
+  int* pages = next + a.tokens;
+  cudaMemsetAsync(head, 0, (size_t)(a.blocks + 1) * sizeof(int), stream);
+  append_index_kernel<T><<<(unsigned)((a.tokens + 255) / 256), 256, 0, stream>>>(a, head, next,
+                                                                                 pages, count, err);
+  const int64_t ctas = std::min<int64_t>(2 * a.tokens, 8LL * 148);
+  append_pages_kernel<T, VEC, NC>
+      <<<(unsigned)ctas, kAppendThreads, 0, stream>>>(a, head, next, pages, count, err);
+}
+
+template <typename T>
+int launch_append_t(const AppendKvArgs& p, int* ws, cudaStream_t stream) {
+  AppendArgs<T> a;
+  a.key = static_cast<const T*>(p.key);
+  a.value = static_cast<const T*>(p.value);
+  a.k_tok = p.k_token_stride;
+  a.k_head = p.k_head_stride;
+  a.v_tok = p.v_token_stride;
+  a.v_head = p.v_head_stride;
+  a.cache = p.cache;
+  a.scales = p.scales;
+  a.slots = p.slots;
+  a.positions = p.positions;
+  a.table = p.table;
+  a.tokens = p.tokens;
+  a.blocks = p.blocks;
+  a.table_rows = p.table_rows;
+  a.bs = p.block_size;
+  a.kv_heads = p.kv_heads;
+  a.dim = p.dim;
+  a.rot = p.positions != nullptr ? p.rot : 0;
+  a.interleaved = p.interleaved;
+  auto aligned = [](const void* x, int n) { return reinterpret_cast<uintptr_t>(x) % n == 0; };
+  const bool vec = a.dim % 4 == 0 && a.k_tok % 4 == 0 && a.k_head % 4 == 0 && a.v_tok % 4 == 0 &&
+                   a.v_head % 4 == 0 && aligned(a.key, 4 * sizeof(T)) &&
+                   aligned(a.value, 4 * sizeof(T)) && aligned(a.cache, 4) &&
+                   (a.rot == 0 || a.interleaved || (a.rot % 8 == 0 && aligned(a.table, 16)));
+  if (vec && a.dim <= 128) launch_append_n<T, 4, 1>(a, ws, stream);
+  else if (vec) launch_append_n<T, 4, 2>(a, ws, stream);
+  else launch_append_n<T, 1, 8>(a, ws, stream);
+  return kOk;
+}
+
+int launched(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) return kOk;
+  set_error(std::string(what) + " launch failed: " + cudaGetErrorString(e));
+  return kCudaError;
+}
+
+}  // namespace
+
+int launch_qk_norm_rope(const QkNormRopeArgs& a, cudaStream_t stream) {
+  if (a.tokens == 0 || a.heads + a.kv_heads == 0) return kOk;
+  switch (a.dtype) {
+    case 0: launch_qk_t<float>(a, stream); break;
+    case 1: launch_qk_t<__half>(a, stream); break;
+    case 2: launch_qk_t<__nv_bfloat16>(a, stream); break;
+    default: set_error("unknown dtype code"); return kInvalidArgument;
+  }
+  return launched("qk_norm_rope");
+}
+
+size_t append_kv_workspace_size(int64_t tokens, int64_t blocks) {
+  if (tokens <= kAppendScan) return 0;
+  return (size_t)(blocks + 1 + 2 * tokens) * sizeof(int);
+}
+
+int launch_append_kv(const AppendKvArgs& a, void* workspace, size_t workspace_bytes,
+                     cudaStream_t stream) {
+  if (a.tokens == 0) return kOk;
+  if (append_kv_workspace_size(a.tokens, a.blocks) > workspace_bytes ||
+      (a.tokens > kAppendScan && workspace == nullptr)) {
+    set_error("workspace too small for append_kv");
+    return kWorkspace;
+  }
+  int* ws = static_cast<int*>(workspace);
+  switch (a.dtype) {
+    case 0: launch_append_t<float>(a, ws, stream); break;
+    case 1: launch_append_t<__half>(a, ws, stream); break;
+    case 2: launch_append_t<__nv_bfloat16>(a, ws, stream); break;
+    default: set_error("unknown dtype code"); return kInvalidArgument;
+  }
+  return launched("append_kv");
+}
+
+}  // namespace pkv

@@ -14,6 +14,7 @@ this module fails with ``ImportError`` when that library has not been built.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as ct
 from pathlib import Path
 
@@ -81,6 +82,14 @@ _wtc_ws = _sig("pkv_write_to_cache_workspace_size", [_I64, _I32], _SZ)
 _wtc = _sig("pkv_write_to_cache",
             [_P, _P, _I32, _P, _P, _P, _I64, _I64, _I32, _I32, _I32, _P, _SZ, _P])
 
+_rope = _sig("pkv_qk_norm_rope",
+             [_P, _P, _I32, _P, _P, _P, _P, _P, _P, _I32, _F, _I64, _I32, _I32, _I32, _I32, _I64,
+              _I32, _I64, _I64, _I64, _I64, _P])
+_append_ws = _sig("pkv_append_kv_workspace_size", [_I64, _I64], _SZ)
+_append = _sig("pkv_append_kv",
+               [_P, _P, _I32, _P, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _I32, _I32, _I64, _I32,
+                _I64, _I64, _I64, _I64, _P, _SZ, _P])
+
 LIBRARY_PATH = str(_LIB_PATH)
 _DTYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
@@ -107,6 +116,34 @@ def _require(cond: bool, msg: str):
 def _stream(t: torch.Tensor) -> int:
     """Raw cudaStream_t of the current stream on ``t``'s device."""
     return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def _on_device(t: torch.Tensor):
+    """Makes ``t``'s device the current one where it is not already."""
+    if t.device.index == torch.cuda.current_device():
+        return _SAME_DEVICE
+    return torch.cuda.device(t.device)
+
+
+def _check_inputs(*tensors):
+    """CUDA tensors of one device, none of which wants a gradient: the
+    operators that call this have no backward pass and must not drop one."""
+    first = tensors[0]
+    for t in tensors:
+        if t is None:
+            continue
+        _require(t.is_cuda, "all inputs must be CUDA tensors")
+        _require(t.device == first.device, "all inputs must be on one device")
+        _require(not (t.requires_grad and torch.is_grad_enabled()),
+                 "inputs that require grad: this operator has no backward pass")
+
+
+def _channels_last(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself where its last dimension is contiguous, else a copy."""
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
 def _workspace(nbytes: int, device) -> tuple[torch.Tensor | None, int]:
@@ -456,3 +493,94 @@ def write_to_cache(key, value, kv_cache_int8, scale_cache, slot_mapping, block_s
     _check(_wtc(kc.data_ptr(), vc.data_ptr(), _DTYPE_CODE[kc.dtype], kv_cache_int8.data_ptr(),
                 scale_cache.data_ptr(), sm.data_ptr(), nt, NB, bs, Hkv, D, wp,
                 0 if ws is None else ws.numel(), _stream(kc)))
+
+
+def _check_rotary(rotary, positions, num_tokens: int, head_dim: int):
+    _require(rotary.dtype == torch.float32 and rotary.dim() == 2 and rotary.shape[1] % 2 == 0
+             and rotary.shape[1] <= head_dim,
+             "rotary must be a float32 [num_positions, rotary_dim] table, rotary_dim even and at "
+             "most head_dim")
+    _require(positions.dtype in (torch.int64, torch.int32) and positions.dim() == 1
+             and positions.shape[0] == num_tokens, "positions must be int64 or int32 [num_tokens]")
+    return rotary.contiguous(), positions.to(torch.int64).contiguous()
+
+
+def qk_norm_rope(q, k, positions, rotary, q_weight=None, k_weight=None, eps=1e-6,
+                 interleaved=False):
+    """Per-head RMS norm (with weights) and rotary position of ``q``
+    ``[T, H, D]`` and ``k`` ``[T, Hkv, D]`` (or None) in one launch."""
+    _check_inputs(q, k, positions, rotary, q_weight, k_weight)
+    _require(q.dim() == 3 and q.dtype in _DTYPE_CODE,
+             "q must be [num_tokens, num_heads, head_dim] float32, float16 or bfloat16")
+    T, H, D = q.shape
+    _require(0 < D <= 256, "head_dim must be 1 to 256")
+    Hkv = 0
+    if k is not None:
+        _require(k.dim() == 3 and k.dtype == q.dtype and k.shape[0] == T and k.shape[2] == D,
+                 "k must be [num_tokens, num_kv_heads, head_dim] of q's type")
+        Hkv = k.shape[1]
+    table, pos = _check_rotary(rotary, positions, T, D)
+    _require((q_weight is None) == (k_weight is None) or k is None,
+             "q_weight and k_weight go together")
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    for w in weights:
+        _require(w.dim() == 1 and w.shape[0] == D and w.dtype in (q.dtype, torch.float32)
+                 and w.dtype == weights[0].dtype,
+                 "weights must be [head_dim], both float32 or of q's type")
+    weights = [w.contiguous() for w in weights]
+    qc = _channels_last(q)
+    kc = None if k is None else _channels_last(k)
+    q_out = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
+    k_out = None if k is None else torch.empty((T, Hkv, D), dtype=q.dtype, device=q.device)
+    with _on_device(q):
+        _check(_rope(qc.data_ptr(), kc.data_ptr() if Hkv else None, _DTYPE_CODE[q.dtype],
+                     q_out.data_ptr(), k_out.data_ptr() if Hkv else None, pos.data_ptr(),
+                     table.data_ptr(), weights[0].data_ptr() if weights else None,
+                     weights[-1].data_ptr() if weights else None,
+                     1 if weights and weights[0].dtype == torch.float32 else 0, float(eps), T, H,
+                     Hkv, D, table.shape[1], table.shape[0], 1 if interleaved else 0,
+                     qc.stride(0), qc.stride(1), kc.stride(0) if Hkv else 0,
+                     kc.stride(1) if Hkv else 0, _stream(q)))
+    return q_out, k_out
+
+
+def append_kv(key, value, kv_cache_int8, scale_cache, slot_mapping, block_size: int,
+              positions=None, rotary=None, interleaved=False):
+    """Rotate, quantize and append new tokens to the [2, NB, bs, Hkv, D]
+    cache in place, keeping the pages' earlier tokens readable."""
+    _check_inputs(key, value, kv_cache_int8, scale_cache, slot_mapping, positions, rotary)
+    _require(key.dim() == 3 and key.dtype in _DTYPE_CODE and value.dtype == key.dtype
+             and value.shape == key.shape,
+             "key/value must be [num_tokens, Hkv, D] of one float32/float16/bfloat16 dtype")
+    _require(kv_cache_int8.dtype == torch.int8 and kv_cache_int8.dim() == 5
+             and kv_cache_int8.shape[0] == 2, "kv_cache_int8 must be int8 [2, NB, bs, Hkv, D]")
+    _require(kv_cache_int8.is_contiguous() and scale_cache.is_contiguous(),
+             "caches must be contiguous (they are written in place)")
+    _, NB, bs, Hkv, D = kv_cache_int8.shape
+    T = key.shape[0]
+    _require(int(block_size) == bs, "block_size must match the cache")
+    _require(0 < bs <= 64, "supports block_size <= 64")
+    _require(0 < D <= 256, "head_dim must be 1 to 256")
+    _require(tuple(key.shape[1:]) == (Hkv, D), "key/value must be [num_tokens, Hkv, D]")
+    _require(scale_cache.dtype == torch.float32 and tuple(scale_cache.shape) == (2, NB, Hkv),
+             "scale_cache must be float32 [2, NB, Hkv]")
+    _require(slot_mapping.dtype in (torch.int64, torch.int32) and slot_mapping.dim() == 1
+             and slot_mapping.shape[0] == T, "slot_mapping must be int64 or int32 [num_tokens]")
+    _require((positions is None) == (rotary is None), "positions and rotary go together")
+    pos = table = None
+    if rotary is not None:
+        table, pos = _check_rotary(rotary, positions, T, D)
+        if table.shape[1] == 0:  # nothing to rotate
+            table = pos = None
+    kc, vc = _channels_last(key), _channels_last(value)
+    slots = slot_mapping.to(torch.int64).contiguous()
+    with _on_device(key):
+        ws, wp = _workspace(_append_ws(T, NB), key.device)
+        _check(_append(kc.data_ptr(), vc.data_ptr(), _DTYPE_CODE[key.dtype],
+                       kv_cache_int8.data_ptr(), scale_cache.data_ptr(), slots.data_ptr(),
+                       None if pos is None else pos.data_ptr(),
+                       None if table is None else table.data_ptr(), T, NB, bs, Hkv, D,
+                       0 if table is None else table.shape[1],
+                       0 if table is None else table.shape[0], 1 if interleaved else 0,
+                       kc.stride(0), kc.stride(1), vc.stride(0), vc.stride(1), wp,
+                       0 if ws is None else ws.numel(), _stream(key)))

@@ -18,6 +18,7 @@ call raises ``RuntimeError``.
 
 from __future__ import annotations
 
+import math
 from typing import Any
 
 import numpy as np
@@ -39,6 +40,9 @@ __all__ = [
     "attention_stats",
     "quant_paged_attention",
     "DecodePlan",
+    "rotary_table",
+    "qk_norm_rope",
+    "append_kv",
 ]
 
 
@@ -270,3 +274,109 @@ class DecodePlan:
         """Replays the capture on the current stream; returns ``out``."""
         self._graph.replay()
         return self.out
+
+
+# ---------------------------------------------------------------------------
+# Rotary positions and the cache append
+# ---------------------------------------------------------------------------
+
+def rotary_table(max_positions: int, rotary_dim: int, base: float = 10000.0, scaling: str = "none",
+                 factor: float = 1.0, original_positions: int = 0, beta_fast: float = 32.0,
+                 beta_slow: float = 1.0, device=None) -> torch.Tensor:
+    """Cosines and sines of every position, float32 ``[max_positions,
+    rotary_dim]`` (``rotary_dim / 2`` cosines, then the sines), the table that
+    :func:`qk_norm_rope` and :func:`append_kv` read.  Angles are taken in 64
+    bits, so far positions keep their precision.
+
+    Pair i turns by ``base ** (-2 i / rotary_dim)`` per position.  ``scaling``
+    stretches a model trained on ``original_positions`` by ``factor``:
+
+    * ``"linear"``: every frequency divided by ``factor``;
+    * ``"ntk"``: ``base`` raised to ``base * factor ** (r / (r - 2))``, which
+      keeps the fastest pair and divides the slowest by ``factor``;
+    * ``"yarn"``: pairs that turn more than ``beta_fast`` times within
+      ``original_positions`` are kept, those below ``beta_slow`` turns are
+      divided by ``factor``, a linear ramp between; cosines and sines are
+      multiplied by ``0.1 ln(factor) + 1``.
+    """
+    if max_positions < 0 or rotary_dim < 0 or rotary_dim % 2:
+        raise ValueError("max_positions must be non-negative and rotary_dim even")
+    if not (base > 0 and factor > 0):
+        raise ValueError("base and factor must be positive")
+    if device is None:
+        device = torch.device("cuda", torch.cuda.current_device()) if torch.cuda.is_available() \
+            else torch.device("cpu")
+    i = torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device)
+    magnitude = 1.0
+    if scaling == "ntk":
+        if rotary_dim <= 2:
+            raise ValueError("ntk scaling needs rotary_dim > 2")
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    freq = base ** (-i / rotary_dim) if rotary_dim else i
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "yarn":
+        if original_positions <= 0 or not beta_fast > beta_slow > 0:
+            raise ValueError("yarn scaling needs original_positions > 0 and beta_fast > beta_slow")
+        if factor < 1:
+            raise ValueError("yarn scaling needs factor >= 1")
+
+        def pair_of(turns):  # the (fractional) pair that turns so often in original_positions
+            return rotary_dim * math.log(original_positions / (turns * 2 * math.pi)) / \
+                (2 * math.log(base))
+
+        low = max(math.floor(pair_of(beta_fast)), 0)
+        high = min(math.ceil(pair_of(beta_slow)), rotary_dim - 1)
+        ramp = ((i / 2 - low) / max(high - low, 1e-3)).clamp(0, 1)  # 0: kept, 1: divided
+        freq = freq * (1 - ramp) + freq / factor * ramp
+        magnitude = 0.1 * math.log(factor) + 1.0
+    elif scaling not in ("none", "ntk"):
+        raise ValueError(f"unknown scaling {scaling!r}: none, linear, ntk or yarn")
+    angle = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] * freq
+    return (torch.cat([angle.cos(), angle.sin()], dim=1) * magnitude).float()
+
+
+def qk_norm_rope(q, k, positions, rotary, q_weight=None, k_weight=None, eps: float = 1e-6,
+                 interleaved: bool = False):
+    """Per-head RMS norm and rotary position of queries and keys, one pass.
+
+    ``q`` ``[T, H, D]`` and ``k`` ``[T, Hkv, D]`` (float32, float16 or
+    bfloat16; ``k`` may be None) may be strided views of one projection's
+    output.  With ``q_weight`` / ``k_weight`` ``[D]`` (float32 or of ``q``'s
+    type) each head is divided by ``sqrt(mean(x^2) + eps)`` and multiplied by
+    its weight first.  The first ``rotary.shape[1]`` channels are rotated by
+    ``rotary[positions]`` (:func:`rotary_table`), as pairs ``(i, i + R/2)`` or,
+    ``interleaved``, ``(2i, 2i + 1)``.  Returns new contiguous ``(q, k)``.
+    The arithmetic is in 32 bits, rounded once.  A position outside the table
+    gives rows of zeros and ``PKV_DEVERR_BAD_POSITION``.  No backward pass.
+    """
+    C = _lib()
+    given = [t for t in (q, k, positions, rotary, q_weight, k_weight) if t is not None]
+    if _all_cuda(*given):
+        return C.qk_norm_rope(q, k, positions, rotary, q_weight, k_weight, eps, interleaved)
+    st = _Staging(*given)
+    q2, k2, p2, r2, qw, kw = (None if t is None else st.to_device(t)
+                              for t in (q, k, positions, rotary, q_weight, k_weight))
+    qo, ko = C.qk_norm_rope(q2, k2, p2, r2, qw, kw, eps, interleaved)
+    return st.back(qo), None if ko is None else st.back(ko)
+
+
+def append_kv(key, value, kv_cache_int8, scale_cache, slot_mapping, block_size: int,
+              positions=None, rotary=None, interleaved: bool = False) -> None:
+    """Appends new tokens to the paged INT8 cache in place: rotation of the
+    keys (with ``positions`` and ``rotary``, as :func:`qk_norm_rope`),
+    quantization and scatter in one pass on the current stream.
+
+    ``key`` / ``value`` ``[T, Hkv, D]`` (float32, float16 or bfloat16, strided
+    views allowed); ``kv_cache_int8`` ``[2, NB, bs, Hkv, D]`` and
+    ``scale_cache`` ``[2, NB, Hkv]``; ``slot_mapping`` ``[T]`` with
+    ``block * bs + offset``, -1 for padding.  A page whose offset 0 is written
+    begins anew with the scale of its new tokens.  Otherwise the tokens below
+    the lowest written offset stay: where the new tokens need a larger scale,
+    their codes are moved to it, so a page filled token by token decodes as
+    one filled at once, up to the rounding of each move (``write_to_cache``
+    replaces the scale and leaves the codes).  Of equal slots the last token
+    counts.  The caches must be CUDA tensors.  No backward pass.
+    """
+    _lib().append_kv(key, value, kv_cache_int8, scale_cache, slot_mapping, block_size, positions,
+                     rotary, interleaved)
