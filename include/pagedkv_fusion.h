@@ -44,6 +44,7 @@ extern "C" {
 #define PKV_DEVERR_BAD_SLOT 3
 #define PKV_DEVERR_SEQ_TOO_LONG 4 /* seq_len beyond the block-table width */
 #define PKV_DEVERR_BAD_POSITION 5 /* position outside the rotary table */
+#define PKV_DEVERR_BAD_SEQLENS 6  /* cu_seqlens not ascending within the tensor */
 
 /* Element types of floating-point KV inputs. */
 #define PKV_DTYPE_F32 0
@@ -343,6 +344,36 @@ int pkv_append_kv(const void *key, const void *value, int32_t dtype,
                   int64_t k_head_stride, int64_t v_token_stride,
                   int64_t v_head_stride, void *workspace,
                   size_t workspace_bytes, void *stream);
+
+/*
+ * Attention over packed prompts: out[i, h, :] = softmax(sm_scale * q[i, h] .
+ * K^T) V over the keys of token i's sequence, GQA as in decode, fp32
+ * accumulation and softmax, probabilities rounded to the inputs' type for
+ * the second product.  q, out [total_q, num_heads, head_dim], k, v [total_k,
+ * num_kv_heads, head_dim] (PKV_DTYPE_F16 or PKV_DTYPE_BF16); sequence s is
+ * rows cu_seqlens_q[s] .. cu_seqlens_q[s + 1] of q and cu_seqlens_k[s] ..
+ * cu_seqlens_k[s + 1] of k and v (int32 [num_seqs + 1]).  Under `causal`,
+ * token i of a sequence of Lq tokens and Lk keys sees keys j <= i + Lk - Lq
+ * (a chunk of a longer prompt is a sequence with more keys than tokens).
+ * Rows that see no key, and rows of q behind the last sequence, become zero,
+ * with lse -inf; lse (nullable, float32 [total_q, num_heads]) is the natural
+ * logarithm of the softmax denominator.  Values of keys that a row does not
+ * see, NaN and infinities included, do not reach it.  Token and head strides
+ * are in elements, multiples of 8, pointers 16-byte aligned, channels
+ * contiguous, out contiguous.  head_dim a multiple of 8 up to 128, at most
+ * 128 query heads per KV head, sm_scale > 0.  cu_seqlens that do not ascend
+ * within the tensors record PKV_DEVERR_BAD_SEQLENS and are clamped.
+ */
+int pkv_prefill_attention(const void *q, const void *k, const void *v,
+                          int32_t dtype, void *out, float *lse,
+                          const int32_t *cu_seqlens_q,
+                          const int32_t *cu_seqlens_k, int32_t num_seqs,
+                          int64_t total_q, int64_t total_k, int32_t num_heads,
+                          int32_t num_kv_heads, int32_t head_dim,
+                          int64_t q_token_stride, int64_t q_head_stride,
+                          int64_t k_token_stride, int64_t k_head_stride,
+                          int64_t v_token_stride, int64_t v_head_stride,
+                          float sm_scale, int32_t causal, void *stream);
 
 #ifdef __cplusplus
 }

@@ -476,4 +476,64 @@ int pkv_append_kv(const void* key, const void* value, int32_t dtype, int8_t* kv_
   return pkv::launch_append_kv(a, workspace, workspace_bytes, as_stream(stream));
 }
 
+int pkv_prefill_attention(const void* q, const void* k, const void* v, int32_t dtype, void* out,
+                          float* lse, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                          int32_t num_seqs, int64_t total_q, int64_t total_k, int32_t num_heads,
+                          int32_t num_kv_heads, int32_t head_dim, int64_t q_token_stride,
+                          int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,
+                          int64_t v_token_stride, int64_t v_head_stride, float sm_scale,
+                          int32_t causal, void* stream) {
+  clear_error();
+  if (num_seqs < 0 || total_q < 0 || total_k < 0 || num_heads <= 0 || num_kv_heads <= 0)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "invalid prefill shape");
+  if (dtype != PKV_DTYPE_F16 && dtype != PKV_DTYPE_BF16)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "q/k/v must be float16 or bfloat16");
+  if (head_dim <= 0 || head_dim > 128 || head_dim % 8 != 0)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "supports head_dim % 8 == 0, <= 128");
+  if (num_heads % num_kv_heads != 0)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "GQA requires num_heads % num_kv_heads == 0");
+  if (num_heads / num_kv_heads > 128)
+    return fail(PKV_ERR_UNSUPPORTED, "more than 128 query heads per KV head");
+  if (!(sm_scale > 0.0f) || sm_scale > 3.0e38f)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "sm_scale must be positive and finite");
+  if (total_q > 0x7fffffffLL - 256 || total_k > 0x7fffffffLL - 256 ||
+      (total_q + num_seqs + 1) * (int64_t)num_kv_heads > 0x7fffffffLL)
+    return fail(PKV_ERR_UNSUPPORTED, "too many rows for one call");
+  if (total_q == 0) return PKV_OK;
+  if (!q || !out || !cu_seqlens_q || !cu_seqlens_k || (total_k > 0 && (!k || !v)))
+    return fail(PKV_ERR_INVALID_ARGUMENT, "null input or output pointer");
+  const int64_t strides[6] = {q_token_stride, q_head_stride, k_token_stride,
+                              k_head_stride,  v_token_stride, v_head_stride};
+  for (int i = 0; i < 6; ++i)
+    if ((strides[i] <= 0 || strides[i] % 8 != 0) && (i < 2 || total_k > 0))
+      return fail(PKV_ERR_INVALID_ARGUMENT, "strides must be positive multiples of 8 elements");
+  if (reinterpret_cast<uintptr_t>(q) % 16 != 0 || reinterpret_cast<uintptr_t>(k) % 16 != 0 ||
+      reinterpret_cast<uintptr_t>(v) % 16 != 0 || reinterpret_cast<uintptr_t>(out) % 16 != 0)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "q, k, v and out must be 16-byte aligned");
+  pkv::PrefillArgs a;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.out = out;
+  a.lse = lse;
+  a.dtype = dtype;
+  a.cu_q = cu_seqlens_q;
+  a.cu_k = cu_seqlens_k;
+  a.num_seqs = num_seqs;
+  a.heads = num_heads;
+  a.kv_heads = num_kv_heads;
+  a.dim = head_dim;
+  a.total_q = total_q;
+  a.total_k = total_k;
+  a.q_token_stride = q_token_stride;
+  a.q_head_stride = q_head_stride;
+  a.k_token_stride = k_token_stride;
+  a.k_head_stride = k_head_stride;
+  a.v_token_stride = v_token_stride;
+  a.v_head_stride = v_head_stride;
+  a.sm_scale = sm_scale;
+  a.causal = causal != 0;
+  return pkv::launch_prefill(a, as_stream(stream));
+}
+
 }  // extern "C"

@@ -82,6 +82,25 @@ size_t append_kv_workspace_size(int64_t tokens, int64_t blocks);
 int launch_append_kv(const AppendKvArgs& a, void* workspace, size_t workspace_bytes,
                      cudaStream_t stream);
 
+// ---- prefill.cu -----------------------------------------------------------
+struct PrefillArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  float* lse;  // nullable
+  int dtype;   // 1 fp16, 2 bf16
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  int num_seqs, heads, kv_heads, dim;
+  int64_t total_q, total_k;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride,
+      v_head_stride;  // elements, multiples of 8
+  float sm_scale;
+  bool causal;
+};
+int launch_prefill(const PrefillArgs& a, cudaStream_t stream);
+
 // ---- eviction.cu ----------------------------------------------------------
 int launch_eviction_scores(const float* recency, const float* frequency, const float* attn,
                            const uint8_t* valid, float* scores, int64_t num_blocks,

@@ -1,0 +1,619 @@
+// Attention over packed prompts: out[i] = sum_j softmax_j(scale q_i . k_j) v_j
+// over the keys j of token i's sequence, causal from the sequences' ends
+// (j <= i + Lk - Lq), grouped heads, fp16 or bf16 with fp32 accumulators.
+//
+// One CTA owns two row tiles of 128 rows of one KV head.  A row is a (token,
+// query head of the group) pair, so the G heads of a group share every K / V
+// tile that is loaded.  Keys come in tiles of 128 tokens; per row tile
+//   S = Q K^T    tcgen05 kind::f16, 128 x 128, K-major A and B from shared
+//                memory, S in 128 columns of tensor memory;
+//   P = exp2(scale log2e (S - m)), one thread per row, written back over S as
+//                16-bit values;
+//   O += P V     A = P from tensor memory, B = the V tile read MN-major.
+// The two row tiles alternate: while the softmax warps of one turn S into P,
+// the tensor cores work for the other.
+//
+// The running maximum m is moved only when a tile's maximum exceeds it by
+// more than 2^8 (the exponentials then stay below 2^8, exact enough in fp32
+// sums and 16-bit P); O is rescaled in tensor memory by its softmax warps
+// then, which is safe because S(j) is complete only after P V (j - 1).
+//
+// Masked places hold no influence: masked scores become -inf by selection,
+// and in tiles that contain masked keys the V rows are cleaned first (two
+// warps, off the critical path): rows past the sequence become zero, and
+// where causal masking hides a key from some rows, its non-finite values are
+// taken out of the product and added, in the epilogue, to the rows that see
+// it.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <mutex>
+#include <string>
+#include <type_traits>
+
+#include "pkv_common.cuh"
+#include "pkv_internal.h"
+
+namespace pkv {
+namespace {
+
+constexpr int kRows = 128;      // rows of a row tile (MMA M)
+constexpr int kKeys = 128;      // keys of a tile (MMA N of Q K^T, K of P V)
+constexpr int kPreThreads = 384;  // softmax A, softmax B, load, MMA, 2 cleaning warps
+constexpr int kLoadWarp = 8, kMmaWarp = 9, kCleanWarp = 10;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kLazy = 8.0f;   // log2 growth of a row maximum that moves it
+constexpr int kMaskedTiles = 4; // tiles with masked keys per CTA: 256 tokens span at most 3
+
+template <int DP>
+struct PreCfg {
+  static constexpr int kChunks = DP / 64;               // 128-byte column chunks
+  static constexpr int kTileBytes = kKeys * DP * 2;     // a K, V or Q tile
+  static constexpr int kStages = DP == 128 ? 5 : 8;     // K / V ring
+  static constexpr int kOffQ = 0;                       // two Q tiles
+  static constexpr int kOffKV = 2 * kTileBytes;
+  static constexpr int kOffBar = kOffKV + kStages * kTileBytes;
+  static constexpr int kBars = 2 * kStages + 8 + kMaskedTiles + 1;
+  static constexpr int kOffMisc = kOffBar + kBars * 8;
+  static constexpr int kSmemBytes = kOffMisc + 64 + kMaskedTiles * 16 + 1024;
+  static constexpr int kSCol = 0;                       // S / P of the two tiles
+  static constexpr int kOCol = 256;
+};
+
+struct PreParams {
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  void* out;
+  float* lse;   // nullable
+  const void* v;
+  int64_t v_tok, v_head;
+  int num_seqs, total_q, total_k;
+  int heads, kv_heads, group, dim, tile_tokens;
+  float scale_log2, scale;
+  int causal;
+};
+
+struct PreWork {
+  int q0, lq, k0, lk;  // the sequence's rows in the packed tensors
+  int t0;              // first token (in the sequence) of row tile 0
+};
+
+// Sequence and token range of pair `pair` (of 2 * tile_tokens tokens).  Pairs
+// are numbered sequence by sequence, the last pair of a sequence first: under
+// a causal mask it is the longest, and long work should start early.  The rows
+// behind the last sequence form one more sequence without keys (zeros).
+// One warp; false when `pair` is past the end.
+__device__ bool find_work(const PreParams& p, int pair, PreWork& w, int* err) {
+  const int lane = threadIdx.x & 31;
+  const int span = 2 * p.tile_tokens;
+  int base = 0;
+  for (int s0 = 0; s0 <= p.num_seqs; s0 += 32) {
+    const int s = s0 + lane;
+    int q0 = 0, q1 = 0;
+    if (s < p.num_seqs) {
+      const int a = p.cu_q[s], b = p.cu_q[s + 1];
+      q0 = min(max(a, 0), p.total_q);
+      q1 = min(max(b, q0), p.total_q);
+      const int ka = p.cu_k[s], kb = p.cu_k[s + 1];
+      if (pair == 0 && (a != q0 || b != q1 || ka < 0 || kb < ka || kb > p.total_k))
+        record_error(err, kDevBadSeqlens);
+    } else if (s == p.num_seqs) {
+      q0 = min(max(p.cu_q[s], 0), p.total_q);
+      q1 = p.total_q;
+    }
+    const int n = (q1 - q0 + span - 1) / span;
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    const int total = __shfl_sync(0xffffffffu, incl, 31);
+    if (pair < base + total) {
+      const unsigned m = __ballot_sync(0xffffffffu, pair < base + incl);
+      const int src = __ffs(m) - 1;
+      const int local = pair - base - (__shfl_sync(0xffffffffu, incl, src) -
+                                       __shfl_sync(0xffffffffu, n, src));
+      w.q0 = __shfl_sync(0xffffffffu, q0, src);
+      w.lq = __shfl_sync(0xffffffffu, q1, src) - w.q0;
+      w.t0 = (__shfl_sync(0xffffffffu, n, src) - 1 - local) * span;
+      const int seq = s0 + src;
+      w.k0 = 0;
+      w.lk = 0;
+      if (seq < p.num_seqs) {
+        w.k0 = min(max(p.cu_k[seq], 0), p.total_k);
+        w.lk = min(max(p.cu_k[seq + 1], w.k0), p.total_k) - w.k0;
+      }
+      return true;
+    }
+    base += total;
+  }
+  return false;
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float widen(__half v) { return __half2float(v); }
+
+// Whether either 16-bit float of a word is infinite or NaN (all exponent bits set).
+__device__ __forceinline__ uint32_t nonfinite_mask(uint32_t w, __nv_bfloat16) {
+  return ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) |
+         ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+}
+__device__ __forceinline__ uint32_t nonfinite_mask(uint32_t w, __half) {
+  return ((w & 0x7c00u) == 0x7c00u ? 0xffffu : 0u) |
+         ((w & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u);
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kPreThreads, 1)
+    prefill_kernel(const __grid_constant__ CUtensorMap map_q,
+                   const __grid_constant__ CUtensorMap map_k,
+                   const __grid_constant__ CUtensorMap map_v, const PreParams p, int* err) {
+  using C = PreCfg<DP>;
+  constexpr int kBf16 = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* kv_empty = kv_full + C::kStages;
+  uint64_t* q_full = kv_empty + C::kStages;  // per row tile, as the next three
+  uint64_t* s_full = q_full + 2;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_full = p_full + 2;
+  uint64_t* raw_full = o_full + 2;  // V tiles with masked keys, before they are cleaned
+  uint64_t* mma_done = raw_full + kMaskedTiles;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
+  int* s_work = reinterpret_cast<int*>(smem + C::kOffMisc + 16);
+  uint32_t* s_flags = reinterpret_cast<uint32_t*>(smem + C::kOffMisc + 64);  // [tile][4]
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int kvh = blockIdx.x % p.kv_heads;
+  if (warp == 0) {
+    PreWork w = {0, 0, 0, 0, 0};
+    const bool any = find_work(p, blockIdx.x / p.kv_heads, w, err);
+    if (lane == 0) {
+      s_work[0] = any;
+      s_work[1] = w.q0;
+      s_work[2] = w.lq;
+      s_work[3] = w.k0;
+      s_work[4] = w.lk;
+      s_work[5] = w.t0;
+    }
+  }
+  if (tid == 32) {
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&o_full[i], 1);
+    }
+    for (int i = 0; i < kMaskedTiles; ++i) mbar_init(&raw_full[i], 1);
+    mbar_init(mma_done, 1);
+    mbar_fence_init();
+  }
+  if (warp == kMmaWarp) tmem_alloc(s_tmem, 512);
+  if (warp == kCleanWarp && lane < kMaskedTiles * 4) s_flags[lane] = 0u;
+  tmem_fence_before_sync();
+  __syncthreads();
+  tmem_fence_after_sync();
+  const uint32_t tmem = *s_tmem;
+
+  if (s_work[0]) {
+    const int q0 = s_work[1], lq = s_work[2], k0 = s_work[3], lk = s_work[4], t0 = s_work[5];
+    const int shift = lk - lq;  // key of token i under the causal mask: i + shift
+    // key tiles of each row tile: up to the last key that its last token sees
+    int n_tiles[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int first = t0 + x * p.tile_tokens;
+      const int last = min(first + p.tile_tokens, lq) - 1;
+      int keys = first < lq ? (p.causal ? min(max(last + shift + 1, 0), lk) : lk) : 0;
+      n_tiles[x] = (keys + kKeys - 1) / kKeys;
+    }
+    const int n = max(n_tiles[0], n_tiles[1]);
+    // tiles from here on hold keys that some row does not see
+    const int first_masked =
+        p.causal ? min(max(t0 + shift + 1, 0), lk) / kKeys : lk / kKeys;
+
+    if (warp == kLoadWarp) {
+      // ---- loads: the Q tiles, then K and V tiles in turn ----------------------
+      if (lane == 0 && n > 0) {
+        const uint64_t keep = l2_policy_evict_first();
+        for (int x = 0; x < 2; ++x) {
+          if (n_tiles[x] == 0) continue;
+          mbar_arrive_expect_tx(&q_full[x],
+                                (uint32_t)(C::kChunks * p.tile_tokens * p.group * 128));
+          for (int c = 0; c < C::kChunks; ++c)
+            tma_load_3d(smem + C::kOffQ + x * C::kTileBytes + c * kRows * 128, &map_q, &q_full[x],
+                        c * 64, kvh * p.group, q0 + t0 + x * p.tile_tokens, keep);
+        }
+        uint64_t hold;
+        asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(hold));
+        int i = 0;
+        bool ok = true;
+        for (int j = 0; j < n && ok; ++j) {
+          for (int kind = 0; kind < 2; ++kind, ++i) {
+            const int st = i % C::kStages;
+            if (!mbar_wait_bounded(&kv_empty[st], ((uint32_t)(i / C::kStages) & 1u) ^ 1u, err)) {
+              record_error(err, kDevWaitTimeout);
+              ok = false;
+              break;
+            }
+            // a V tile with masked keys goes through the cleaning warps, which
+            // complete kv_full in the load's place
+            uint64_t* bar =
+                kind == 1 && j >= first_masked ? &raw_full[j - first_masked] : &kv_full[st];
+            mbar_arrive_expect_tx(bar, C::kTileBytes);
+            for (int c = 0; c < C::kChunks; ++c)
+              tma_load_3d(smem + C::kOffKV + st * C::kTileBytes + c * kKeys * 128,
+                          kind ? &map_v : &map_k, bar, c * 64, kvh, k0 + j * kKeys, hold);
+          }
+        }
+        drain_ring(kv_full, C::kStages, i);  // no copy outlives the CTA
+        for (int f = 0; 2 * (first_masked + f) + 1 < i; ++f) mbar_drain(&raw_full[f], 0);
+        for (int x = 0; x < 2; ++x)
+          if (n_tiles[x] > 0) mbar_drain(&q_full[x], 0);
+      }
+    } else if (warp == kMmaWarp) {
+      // ---- MMA issue -------------------------------------------------------------
+      if (lane == 0 && n > 0) {
+        constexpr uint32_t kIdQK = umma_f16_idesc(kBf16, 0, kRows, kKeys);
+        constexpr uint32_t kIdPV = umma_f16_idesc(kBf16, 1, kRows, DP);
+        const uint32_t qa = smem_u32(smem + C::kOffQ), kv = smem_u32(smem + C::kOffKV);
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+          if (ok && !mbar_wait_bounded(bar, parity, err)) {
+            record_error(err, kDevWaitTimeout);
+            ok = false;
+          }
+          tmem_fence_after_sync();
+        };
+        auto stage_of = [&](int i) { return kv + (uint32_t)(i % C::kStages) * C::kTileBytes; };
+        auto wait_load = [&](int i) {
+          wait(&kv_full[i % C::kStages], (uint32_t)(i / C::kStages) & 1u);
+        };
+        // a stage is released only if a later load reuses it
+        auto release = [&](int i) {
+          if (i + C::kStages < 2 * n) umma_commit(&kv_empty[i % C::kStages]);
+        };
+        auto qk = [&](int x, int j) {
+          const uint32_t b = stage_of(2 * j), a = qa + (uint32_t)x * C::kTileBytes;
+#pragma unroll
+          for (int kk = 0; kk < DP / 16; ++kk) {
+            const uint32_t off = (uint32_t)(kk / 4) * (kKeys * 128) + (uint32_t)(kk % 4) * 32;
+            umma_f16(tmem + C::kSCol + x * 128, umma_sw128_desc(a + off, 16, 1024),
+                     umma_sw128_desc(b + off, 16, 1024), kIdQK, kk > 0);
+          }
+          umma_commit(&s_full[x]);
+        };
+        auto pv = [&](int x, int j) {
+          const uint32_t b = stage_of(2 * j + 1);
+#pragma unroll
+          for (int kk = 0; kk < kKeys / 16; ++kk)
+            umma_f16_ta(tmem + C::kOCol + x * 128, tmem + C::kSCol + x * 128 + kk * 8,
+                        umma_sw128_desc(b + kk * 2048, kKeys * 128, 1024), kIdPV,
+                        (j > 0 || kk > 0) ? 1u : 0u);
+          if (j == n_tiles[x] - 1) umma_commit(&o_full[x]);
+        };
+        wait_load(0);
+        for (int x = 0; x < 2; ++x)
+          if (n_tiles[x] > 0) {
+            wait(&q_full[x], 0);
+            if (ok) qk(x, 0);
+          }
+        release(0);
+        for (int j = 0; j < n && ok; ++j) {
+          wait_load(2 * j + 1);
+          for (int x = 0; x < 2; ++x) {
+            if (j >= n_tiles[x]) continue;
+            wait(&p_full[x], (uint32_t)j & 1u);
+            if (!ok) break;
+            pv(x, j);
+            if (x == 1 || n_tiles[1] <= j) release(2 * j + 1);
+            if (j + 1 < n_tiles[x]) {
+              wait_load(2 * j + 2);
+              if (!ok) break;
+              qk(x, j + 1);
+            }
+          }
+          if (j + 1 < n) release(2 * j + 2);
+        }
+        umma_commit(mma_done);
+        mbar_drain(mma_done, 0);  // every MMA is done before tensor memory is freed
+      }
+    } else if (warp >= kCleanWarp) {
+      // ---- V tiles with masked keys ----------------------------------------------
+      const int t64 = tid - kCleanWarp * 32;
+      bool ok = true;
+      for (int j = first_masked; j < n; ++j) {
+        const int i = 2 * j + 1;
+        if (ok && !mbar_wait_bounded(&raw_full[j - first_masked], 0, err)) {
+          record_error(err, kDevWaitTimeout);
+          ok = false;
+        }
+        if (ok) {
+          uint8_t* tile = smem + C::kOffKV + (i % C::kStages) * C::kTileBytes;
+          const int valid = min(lk - j * kKeys, kKeys);
+          for (int r = t64; r < C::kChunks * kKeys; r += 64) {  // a 128-byte row per thread
+            const int key = r % kKeys;
+            uint4* row = reinterpret_cast<uint4*>(tile + r * 128);
+            bool flagged = false;
+#pragma unroll 4
+            for (int u = 0; u < 8; ++u) {
+              if (key >= valid) {
+                row[u] = make_uint4(0, 0, 0, 0);
+                continue;
+              }
+              uint4 w = row[u];
+              const uint32_t a = nonfinite_mask(w.x, T()), b = nonfinite_mask(w.y, T()),
+                             c = nonfinite_mask(w.z, T()), d = nonfinite_mask(w.w, T());
+              if (a | b | c | d) {
+                row[u] = make_uint4(w.x & ~a, w.y & ~b, w.z & ~c, w.w & ~d);
+                flagged = true;
+              }
+            }
+            if (flagged) atomicOr(&s_flags[(j - first_masked) * 4 + key / 32], 1u << (key & 31));
+          }
+          fence_proxy_async_smem();  // an MMA operand
+        }
+        named_barrier(1, 64);
+        if (t64 == 0) mbar_arrive(&kv_full[i % C::kStages]);
+      }
+    } else if (warp < 8) {
+      // ---- softmax and epilogue: thread = row ---------------------------------------
+      const int x = warp >> 2;
+      const int row = tid & 127;
+      const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+      const uint32_t s_addr = tmem + lanes + C::kSCol + x * 128;
+      const uint32_t o_addr = tmem + lanes + C::kOCol + x * 128;
+      const int tok = t0 + x * p.tile_tokens + row / p.group;  // in the sequence
+      const bool valid = row < p.tile_tokens * p.group && tok < lq;
+      // keys below `limit` are seen
+      const int limit = valid ? (p.causal ? min(tok + shift + 1, lk) : lk) : 0;
+      float m = -INFINITY, l = 0.0f;
+      const int nt = n_tiles[x];
+      bool ok = true;
+      for (int j = 0; j < nt; ++j) {
+        if (ok && !mbar_wait_bounded(&s_full[x], (uint32_t)j & 1u, err)) {
+          record_error(err, kDevWaitTimeout);
+          ok = false;
+        }
+        __syncwarp();
+        tmem_fence_after_sync();
+        float s[kKeys];
+        {
+          uint32_t(&u)[kKeys] = reinterpret_cast<uint32_t(&)[kKeys]>(s);
+#pragma unroll
+          for (int c = 0; c < kKeys; c += 32)
+            tmem_load<32>(s_addr + c, reinterpret_cast<uint32_t(&)[32]>(u[c]));
+          tmem_wait_load();
+        }
+        const int seen = limit - j * kKeys;  // columns below this are seen
+        if (j >= first_masked) {
+#pragma unroll
+          for (int c = 0; c < kKeys; ++c) s[c] = c < seen ? s[c] : -INFINITY;
+        }
+        float t = s[0];
+#pragma unroll
+        for (int c = 1; c < kKeys; ++c) t = fmaxf(t, s[c]);
+        // move the maximum where it grew by more than 2^kLazy (or from -inf);
+        // each row by its own scores, so that its bits do not depend on others
+        const bool move =
+            valid && t > m && (m == -INFINITY || (t - m) * p.scale_log2 > kLazy);
+        if (__any_sync(0xffffffffu, move)) {
+          const float alpha = move ? exp2_approx((m - t) * p.scale_log2) : 1.0f;
+          if (move) m = t;
+          l *= alpha;
+          if (j > 0) {
+#pragma unroll
+            for (int c = 0; c < DP; c += 32) {
+              uint32_t o[32];
+              tmem_load<32>(o_addr + c, o);
+              tmem_wait_load();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_store<32>(o_addr + c, o);
+            }
+          }
+        }
+        const float ms = m == -INFINITY ? 0.0f : m * p.scale_log2;
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < kKeys; c += 32) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float a = exp2_approx(fmaf(s[c + e], p.scale_log2, -ms));
+            const float b = exp2_approx(fmaf(s[c + e + 1], p.scale_log2, -ms));
+            sum[e & 2] += a;
+            sum[(e & 2) + 1] += b;
+            pk[e / 2] = pack2(a, b, T());
+          }
+          tmem_store<16>(s_addr + c / 2, pk);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_store();
+        tmem_fence_before_sync();
+        mbar_arrive(&p_full[x]);
+      }
+      if (nt > 0) {
+        if (ok && !mbar_wait_bounded(&o_full[x], 0, err)) record_error(err, kDevWaitTimeout);
+        __syncwarp();
+        tmem_fence_after_sync();
+      }
+      const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+      uint32_t flags = 0u;
+      for (int f = 0; f < kMaskedTiles * 4; ++f) flags |= s_flags[f];
+      const int64_t out_row = ((int64_t)(q0 + tok) * p.heads + kvh * p.group + row % p.group);
+      T* out = static_cast<T*>(p.out) + out_row * p.dim;
+#pragma unroll
+      for (int c = 0; c < DP; c += 32) {
+        uint32_t o[32];
+        if (nt > 0) {
+          tmem_load<32>(o_addr + c, o);
+          tmem_wait_load();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0u;
+        }
+        if (!valid) continue;
+        float f[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) f[e] = l == 0.0f ? 0.0f : __uint_as_float(o[e]) * inv;
+        if (flags != 0u) {  // non-finite values of keys that this row sees
+          for (int k = 0; k < kMaskedTiles * kKeys; ++k) {
+            const int key = first_masked * kKeys + k;
+            if (!(s_flags[k / 32] >> (k & 31) & 1u) || key >= limit) continue;
+            const T* vr = static_cast<const T*>(p.v) + (int64_t)(k0 + key) * p.v_tok +
+                          (int64_t)kvh * p.v_head + c;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float v = c + e < p.dim ? widen(vr[e]) : 0.0f;
+              if (!isfinite(v)) f[e] += v;
+            }
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e += 8)
+          if (c + e < p.dim)
+            *reinterpret_cast<uint4*>(out + c + e) =
+                make_uint4(pack2(f[e], f[e + 1], T()), pack2(f[e + 2], f[e + 3], T()),
+                           pack2(f[e + 4], f[e + 5], T()), pack2(f[e + 6], f[e + 7], T()));
+      }
+      if (valid && p.lse != nullptr)
+        p.lse[out_row] = l == 0.0f ? -INFINITY : fmaf(m, p.scale, logf(l));
+    }
+  }
+  tmem_fence_before_sync();
+  __syncthreads();
+  if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
+}
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(p);
+  });
+  return fn;
+}
+
+// [tokens, heads, dim] with token and head strides (elements, multiples of
+// 8) as (channel, head, token); boxes of 64 channels x box_heads x box_tokens.
+// Channels past `dim` and tokens past the end load as zero.
+bool make_map(CUtensorMap* map, const void* base, int bf16, int dim, int heads, int64_t tokens,
+              int64_t tok_stride, int64_t head_stride, int box_heads, int box_tokens) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)tokens};
+  cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)tok_stride * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r =
+      fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+         const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS;
+}
+
+template <typename T, int DP>
+int launch_prefill_t(const PrefillArgs& a, cudaStream_t stream) {
+  using C = PreCfg<DP>;
+  const int bf16 = a.dtype == 2;
+  PreParams p;
+  p.cu_q = a.cu_q;
+  p.cu_k = a.cu_k;
+  p.out = a.out;
+  p.lse = a.lse;
+  p.v = a.v;
+  p.v_tok = a.v_token_stride;
+  p.v_head = a.v_head_stride;
+  p.num_seqs = a.num_seqs;
+  p.total_q = (int)a.total_q;
+  p.total_k = (int)a.total_k;
+  p.heads = a.heads;
+  p.kv_heads = a.kv_heads;
+  p.group = a.heads / a.kv_heads;
+  p.dim = a.dim;
+  p.tile_tokens = kRows / p.group;
+  p.scale = a.sm_scale;
+  p.scale_log2 = a.sm_scale * kLog2e;
+  p.causal = a.causal ? 1 : 0;
+  CUtensorMap mq, mk, mv;
+  // without keys the key maps are never used, but a map needs memory
+  const bool none = a.total_k == 0;
+  if (!make_map(&mq, a.q, bf16, a.dim, a.heads, a.total_q, a.q_token_stride, a.q_head_stride,
+                p.group, p.tile_tokens) ||
+      !make_map(&mk, none ? a.q : a.k, bf16, a.dim, none ? a.heads : a.kv_heads,
+                none ? a.total_q : a.total_k, none ? a.q_token_stride : a.k_token_stride,
+                none ? a.q_head_stride : a.k_head_stride, 1, kKeys) ||
+      !make_map(&mv, none ? a.q : a.v, bf16, a.dim, none ? a.heads : a.kv_heads,
+                none ? a.total_q : a.total_k, none ? a.q_token_stride : a.v_token_stride,
+                none ? a.q_head_stride : a.v_head_stride, 1, kKeys)) {
+    set_error("cuTensorMapEncodeTiled failed for q, k or v");
+    return kCudaError;
+  }
+  auto kern = prefill_kernel<T, DP>;
+  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+  // pairs of row tiles: at most this many over all sequences (and the rest)
+  const int span = 2 * p.tile_tokens;
+  const int64_t pairs = a.total_q / span + std::min<int64_t>(a.num_seqs + 1, a.total_q);
+  kern<<<(unsigned)(pairs * a.kv_heads), kPreThreads, C::kSmemBytes, stream>>>(
+      mq, mk, mv, p, device_error_word());
+  return kOk;
+}
+
+}  // namespace
+
+int launch_prefill(const PrefillArgs& a, cudaStream_t stream) {
+  if (a.total_q == 0) return kOk;
+  int rc;
+  if (a.dtype == 1)
+    rc = a.dim <= 64 ? launch_prefill_t<__half, 64>(a, stream)
+                     : launch_prefill_t<__half, 128>(a, stream);
+  else
+    rc = a.dim <= 64 ? launch_prefill_t<__nv_bfloat16, 64>(a, stream)
+                     : launch_prefill_t<__nv_bfloat16, 128>(a, stream);
+  if (rc != kOk) return rc;
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) {
+    set_error(std::string("prefill launch failed: ") + cudaGetErrorString(e));
+    return kCudaError;
+  }
+  return kOk;
+}
+
+}  // namespace pkv

@@ -90,6 +90,10 @@ _append = _sig("pkv_append_kv",
                [_P, _P, _I32, _P, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _I32, _I32, _I64, _I32,
                 _I64, _I64, _I64, _I64, _P, _SZ, _P])
 
+_prefill = _sig("pkv_prefill_attention",
+                [_P, _P, _P, _I32, _P, _P, _P, _P, _I32, _I64, _I64, _I32, _I32, _I32, _I64, _I64,
+                 _I64, _I64, _I64, _I64, _F, _I32, _P])
+
 LIBRARY_PATH = str(_LIB_PATH)
 _DTYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
@@ -584,3 +588,42 @@ def append_kv(key, value, kv_cache_int8, scale_cache, slot_mapping, block_size: 
                        0 if table is None else table.shape[0], 1 if interleaved else 0,
                        kc.stride(0), kc.stride(1), vc.stride(0), vc.stride(1), wp,
                        0 if ws is None else ws.numel(), _stream(key)))
+
+
+def _tma_rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` ``[tokens, heads, D]`` itself where tiles can be copied from it
+    (contiguous channels, strides of 16 bytes, 16-byte aligned), else a copy."""
+    if t.numel() == 0 or (t.stride(2) == 1 and t.stride(0) > 0 and t.stride(1) > 0
+                          and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0
+                          and t.data_ptr() % 16 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def prefill_attention(q, k, v, cu_seqlens, sm_scale, cu_seqlens_k=None, causal=True,
+                      return_lse=False):
+    """Attention over packed prompts, ``[total_q, H, D]`` (and, with
+    ``return_lse``, the float32 ``[total_q, H]`` log denominators)."""
+    _check_inputs(q, k, v, cu_seqlens, cu_seqlens_k)
+    _require(q.dim() == 3 and q.dtype in (torch.float16, torch.bfloat16),
+             "q must be [total_q, num_heads, head_dim] float16 or bfloat16")
+    Tq, H, D = q.shape
+    _require(k.dim() == 3 and k.dtype == q.dtype and k.shape[2] == D and v.dtype == q.dtype
+             and v.shape == k.shape, "k and v must be [total_k, num_kv_heads, head_dim] of q's type")
+    Tk, Hkv, _ = k.shape
+    cq = cu_seqlens
+    ck = cu_seqlens if cu_seqlens_k is None else cu_seqlens_k
+    for c in (cq, ck):
+        _require(c.dtype == torch.int32 and c.dim() == 1 and c.shape[0] == cq.shape[0]
+                 and c.shape[0] > 0, "cu_seqlens must be int32 [num_seqs + 1]")
+    cq, ck = cq.contiguous(), ck.contiguous()
+    qc, kc, vc = _tma_rows(q), _tma_rows(k), _tma_rows(v)
+    out = torch.empty((Tq, H, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((Tq, H), dtype=torch.float32, device=q.device) if return_lse else None
+    with _on_device(q):
+        _check(_prefill(qc.data_ptr(), kc.data_ptr(), vc.data_ptr(), _DTYPE_CODE[q.dtype],
+                        out.data_ptr(), None if lse is None else lse.data_ptr(), cq.data_ptr(),
+                        ck.data_ptr(), cq.shape[0] - 1, Tq, Tk, H, Hkv, D, qc.stride(0),
+                        qc.stride(1), kc.stride(0), kc.stride(1), vc.stride(0), vc.stride(1),
+                        float(sm_scale), 1 if causal else 0, _stream(q)))
+    return (out, lse) if return_lse else out

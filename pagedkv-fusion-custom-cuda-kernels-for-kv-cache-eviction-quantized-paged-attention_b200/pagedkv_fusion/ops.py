@@ -43,6 +43,7 @@ __all__ = [
     "rotary_table",
     "qk_norm_rope",
     "append_kv",
+    "prefill_attention",
 ]
 
 
@@ -380,3 +381,37 @@ def append_kv(key, value, kv_cache_int8, scale_cache, slot_mapping, block_size: 
     """
     _lib().append_kv(key, value, kv_cache_int8, scale_cache, slot_mapping, block_size, positions,
                      rotary, interleaved)
+
+
+# ---------------------------------------------------------------------------
+# Prompt attention
+# ---------------------------------------------------------------------------
+
+def prefill_attention(q, k, v, cu_seqlens, sm_scale: float, cu_seqlens_k=None,
+                      causal: bool = True, return_lse: bool = False):
+    """Attention over packed prompts of different lengths, grouped heads.
+
+    ``q`` ``[total_q, H, D]``, ``k`` / ``v`` ``[total_k, Hkv, D]`` (float16 or
+    bfloat16, D a multiple of 8 up to 128; strided views with contiguous
+    channels are read in place); ``cu_seqlens`` int32 ``[num_seqs + 1]``, the
+    sequences' first rows and the end.  ``cu_seqlens_k`` (default:
+    ``cu_seqlens``) gives the keys' rows where a sequence has more keys than
+    tokens, as a chunk of a longer prompt has: with ``causal``, token i of Lq
+    sees keys ``j <= i + Lk - Lq``.  ``sm_scale`` > 0.
+
+    Returns ``[total_q, H, D]`` in the inputs' type, and with ``return_lse``
+    also the float32 ``[total_q, H]`` logarithms of the softmax denominators.
+    Rows that see no key, and rows behind the last sequence, are zero (lse
+    -inf).  What a row does not see does not reach it, whatever its value.
+    No backward pass.
+    """
+    C = _lib()
+    given = [t for t in (q, k, v, cu_seqlens, cu_seqlens_k) if t is not None]
+    if _all_cuda(*given):
+        return C.prefill_attention(q, k, v, cu_seqlens, sm_scale, cu_seqlens_k, causal, return_lse)
+    st = _Staging(*given)
+    got = C.prefill_attention(st.to_device(q), st.to_device(k), st.to_device(v),
+                              st.to_device(cu_seqlens, torch.int32), sm_scale,
+                              None if cu_seqlens_k is None else
+                              st.to_device(cu_seqlens_k, torch.int32), causal, return_lse)
+    return tuple(st.back(t) for t in got) if return_lse else st.back(got)

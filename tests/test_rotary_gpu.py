@@ -400,11 +400,10 @@ def test_refusals(cuda):
         (lambda: ops.qk_norm_rope(q, q, pos, torch.cat([table, table], 1)), "rotary"),
         (lambda: ops.qk_norm_rope(q, q, pos, table, w, None), "go together"),
         (lambda: ops.qk_norm_rope(q, q, pos, table, w, w.half()), "weights"),
-        (lambda: ops.qk_norm_rope(q.requires_grad_(), q, pos, table), "backward"),
+        (lambda: ops.qk_norm_rope(q.clone().requires_grad_(), q, pos, table), "backward"),
     ]:
         with pytest.raises(RuntimeError, match=msg):
             call()
-        q = q.detach()
     cache = torch.zeros(2, 2, 16, 2, 64, dtype=torch.int8, device="cuda")
     scales = torch.ones(2, 2, 2, device="cuda")
     args = [q, q, cache, scales, pos, 16]
