@@ -375,6 +375,34 @@ int pkv_prefill_attention(const void *q, const void *k, const void *v,
                           int64_t v_token_stride, int64_t v_head_stride,
                           float sm_scale, int32_t causal, void *stream);
 
+/*
+ * Decode-step attention for a batch that shares a prefix: as
+ * pkv_quant_paged_attention over the tokens [prefix | own tokens] of each
+ * sequence, where the prefix_len[0] tokens of the prefix are reached through
+ * prefix_table (int32 [prefix_blocks], pages shared by every sequence, the
+ * last one possibly partial) and the sequence's own seq_lens[s] tokens through
+ * block_tables[s].  The prefix's pages are read once for the batch.  A
+ * sequence without any token yields zeros.  A prefix_len beyond the table
+ * records PKV_DEVERR_SEQ_TOO_LONG and is cut to it; tokens on a page outside
+ * the cache record PKV_DEVERR_BAD_BLOCK_ID and are not attended.  Envelope:
+ * head_dim % 32 == 0 and <= 128, block_size <= 64, num_heads % num_kv_heads
+ * == 0; q, out and the caches 16-byte aligned.  prefix_blocks and
+ * max_blocks_per_seq may be 0.  The workspace holds the partial results and
+ * needs no initialisation.
+ */
+size_t pkv_shared_prefix_attention_workspace_size(
+    int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+    int32_t block_size, int64_t num_blocks, int32_t prefix_blocks,
+    int32_t max_blocks_per_seq);
+int pkv_shared_prefix_attention(
+    const float *q, const int8_t *k_cache, const float *k_scale,
+    const int8_t *v_cache, const float *v_scale, const int32_t *prefix_table,
+    const int32_t *prefix_len, const int32_t *block_tables,
+    const int32_t *seq_lens, float *out, int32_t num_seqs, int32_t num_heads,
+    int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+    int64_t num_blocks, int32_t prefix_blocks, int32_t max_blocks_per_seq,
+    float sm_scale, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -536,4 +536,55 @@ int pkv_prefill_attention(const void* q, const void* k, const void* v, int32_t d
   return pkv::launch_prefill(a, as_stream(stream));
 }
 
+size_t pkv_shared_prefix_attention_workspace_size(int32_t num_seqs, int32_t num_heads,
+                                                  int32_t num_kv_heads, int32_t head_dim,
+                                                  int32_t block_size, int64_t num_blocks,
+                                                  int32_t prefix_blocks,
+                                                  int32_t max_blocks_per_seq) {
+  if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || block_size <= 0 ||
+      prefix_blocks < 0 || max_blocks_per_seq < 0 || num_heads % num_kv_heads != 0)
+    return 0;
+  pkv::SharedPrefixArgs a;
+  a.own = decode_args(reinterpret_cast<const float*>(16), reinterpret_cast<const int8_t*>(16),
+                      nullptr, reinterpret_cast<const int8_t*>(16), nullptr, nullptr, nullptr,
+                      reinterpret_cast<float*>(16), num_seqs, num_heads, num_kv_heads, head_dim,
+                      block_size, num_blocks, max_blocks_per_seq, 1.0f);
+  a.prefix_table = nullptr;
+  a.prefix_len = nullptr;
+  a.prefix_width = prefix_blocks;
+  return pkv::shared_prefix_workspace_size(a);
+}
+
+int pkv_shared_prefix_attention(const float* q, const int8_t* k_cache, const float* k_scale,
+                                const int8_t* v_cache, const float* v_scale,
+                                const int32_t* prefix_table, const int32_t* prefix_len,
+                                const int32_t* block_tables, const int32_t* seq_lens, float* out,
+                                int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
+                                int32_t head_dim, int32_t block_size, int64_t num_blocks,
+                                int32_t prefix_blocks, int32_t max_blocks_per_seq, float sm_scale,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  pkv::SharedPrefixArgs a;
+  a.own = decode_args(q, k_cache, k_scale, v_cache, v_scale, block_tables, seq_lens, out, num_seqs,
+                      num_heads, num_kv_heads, head_dim, block_size, num_blocks,
+                      max_blocks_per_seq, sm_scale);
+  a.prefix_table = prefix_table;
+  a.prefix_len = prefix_len;
+  a.prefix_width = prefix_blocks;
+  const int rc = check_decode(a.own);
+  if (rc != PKV_OK) return rc;
+  if (prefix_blocks < 0) return fail(PKV_ERR_INVALID_ARGUMENT, "invalid prefix table");
+  if (head_dim > 128) return fail(PKV_ERR_INVALID_ARGUMENT, "supports head_dim % 32 == 0, <= 128");
+  if (num_seqs > 0 && prefix_blocks > 0 && (!prefix_table || !prefix_len))
+    return fail(PKV_ERR_INVALID_ARGUMENT, "null input or output pointer");
+  if ((int64_t)num_seqs * num_heads > 0x7fffffffLL - 256 ||
+      (int64_t)prefix_blocks * block_size > 0x7fffffffLL - 256)
+    return fail(PKV_ERR_UNSUPPORTED, "more than 2^31 rows or prefix tokens");
+  if (reinterpret_cast<uintptr_t>(q) % 16 != 0 || reinterpret_cast<uintptr_t>(out) % 16 != 0 ||
+      reinterpret_cast<uintptr_t>(k_cache) % 16 != 0 ||
+      reinterpret_cast<uintptr_t>(v_cache) % 16 != 0)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "q, out and the caches must be 16-byte aligned");
+  return pkv::launch_shared_prefix(a, workspace, workspace_bytes, as_stream(stream));
+}
+
 }  // extern "C"

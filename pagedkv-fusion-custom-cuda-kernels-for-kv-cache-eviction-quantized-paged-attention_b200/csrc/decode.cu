@@ -586,7 +586,7 @@ __global__ void __launch_bounds__(kFastThreads, 2)
       const int hg = v_jj * G + g0 + g;
       const int hq = (j0 + v_jj) * G + g0 + g;
       const float2 ml = s_ml[hg];
-      if (n_splits == 1) {
+      if (n_splits == 1 && out != nullptr) {
         const float inv = ml.y > 0.0f ? 1.0f / ml.y : 0.0f;
         reinterpret_cast<float4*>(out + ((int64_t)seq * num_heads + hq) * 128)[lane] =
             make_float4(acc[g][0] * inv, acc[g][1] * inv, acc[g][2] * inv, acc[g][3] * inv);
@@ -1603,7 +1603,7 @@ __global__ void __launch_bounds__(kGenThreads)
                          (int64_t)kvh * head_dim;
       acc = fmaf(s_p[t] * vs, (float)vr[d], acc);
     }
-    if (n_splits == 1) {
+    if (n_splits == 1 && out != nullptr) {
       out[((int64_t)seq * num_heads + h) * head_dim + d] = l > 0.0f ? acc / l : 0.0f;
     } else {
       const int64_t slot = ((int64_t)seq * max_splits + split) * num_heads + h;
@@ -2060,7 +2060,7 @@ __global__ void __launch_bounds__(256, TcCfg<G>::kMinBlocks)
     tmem_row_groups<G, NQ>(tmem + lane_base + C::kD2Col, [&](int g, float v) {
       const float acc = v * back;
       const int hq = j * G + g;
-      if (n_splits == 1) {
+      if (n_splits == 1 && out != nullptr) {
         out[((int64_t)seq * num_heads + hq) * 128 + e] = l[g] > 0.0f ? acc / l[g] : 0.0f;
       } else {
         const int64_t slot = ((int64_t)seq * max_splits + split) * num_heads + hq;
@@ -2512,7 +2512,7 @@ __global__ void __launch_bounds__(256, TcsCfg<G>::kMinBlocks)
       tmem_row_groups<G, NQ>(tmem + lane_base + C::kD2Col, [&](int g, float v) {
         const float acc = v * back;
         const int hq = un.j * G + g;
-        if (un.n_splits == 1) {
+        if (un.n_splits == 1 && out != nullptr) {
           out[((int64_t)un.seq * num_heads + hq) * 128 + e] = l[g] > 0.0f ? acc / l[g] : 0.0f;
         } else {
           const int64_t slot = ((int64_t)un.seq * max_splits + un.split) * num_heads + hq;
@@ -3328,7 +3328,9 @@ int largest_pow2_divisor_upto(int n, int cap) {
   return r;
 }
 
-Plan make_plan(const DecodeArgs& a) {
+// `partials`: a split plan (no stream kernel), whose kernel leaves every
+// split's (acc, m, l) when it is given no output.
+Plan make_plan(const DecodeArgs& a, bool partials = false) {
   Plan p;
   const int group = a.num_heads / a.num_kv_heads;
   const bool g_ok = group >= 1 && group <= 8 && (group & (group - 1)) == 0;
@@ -3368,7 +3370,7 @@ Plan make_plan(const DecodeArgs& a) {
     const int cs = group == 2 ? 8 : (group == 4 ? 16 : 24);
     if ((hkv == 1 || hkv == 2 || hkv == 4 || hkv == 8) && hkv * cs <= 128 &&
         a.num_seqs <= kStreamMaxSeqs && env_int("PKV_DECODE_TC_PAGES", 0) != 0 &&
-        env_int("PKV_DECODE_TC_SPLIT", 0) == 0) {
+        env_int("PKV_DECODE_TC_SPLIT", 0) == 0 && !partials) {
       // whole pages on the tensor cores, the stream kernel's scheduling (on
       // request: measured slower than the per-head kernel below, since one
       // CTA per SM keeps at most 8 pages of 16 KB in flight)
@@ -3398,7 +3400,8 @@ Plan make_plan(const DecodeArgs& a) {
     return p;
   }
   p.max_splits = std::max(1, (M + p.pages_per_split - 1) / p.pages_per_split);
-  if (p.fast && a.num_seqs <= kStreamMaxSeqs && env_int("PKV_DECODE_SPLIT", 0) == 0) {
+  if (p.fast && a.num_seqs <= kStreamMaxSeqs && env_int("PKV_DECODE_SPLIT", 0) == 0 &&
+      !partials) {
     p.stream = true;
     const int forced = env_int("PKV_DECODE_CTAS", 0);
     p.n_ctas = forced > 0 ? forced : 2 * sm_count();
@@ -3602,6 +3605,32 @@ cudaError_t launch_combine(const DecodeArgs& a, const Plan& p, const float* ws_a
   return cudaErrorInvalidValue;
 }
 
+// The split kernel of a plan without the stream kernel.
+int launch_split(const DecodeArgs& a, const Plan& p, float* ws_acc, float2* ws_ml,
+                 cudaStream_t stream) {
+  int rc = kOk;
+  if (p.tc) {
+    rc = launch_tc(a, p, ws_acc, ws_ml, stream);
+  } else if (p.fast) {
+    rc = a.block_size == 16 ? dispatch_hg<16>(a, p, ws_acc, ws_ml, stream)
+                            : dispatch_hg<32>(a, p, ws_acc, ws_ml, stream);
+  } else {
+    dim3 grid(a.num_seqs, p.max_splits, a.num_heads);
+    decode_generic_kernel<<<grid, kGenThreads, 0, stream>>>(
+        a.q, a.k_cache, a.k_scale, a.v_cache, a.v_scale, a.block_tables, a.seq_lens, a.out,
+        ws_acc, ws_ml, a.num_heads, a.num_kv_heads, a.head_dim, a.block_size, a.num_blocks,
+        a.max_blocks_per_seq, a.sm_scale * kLog2e, p.pages_per_split, p.max_splits,
+        device_error_word());
+  }
+  if (rc != kOk) return rc;
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) {
+    set_error(std::string("decode launch failed: ") + cudaGetErrorString(e));
+    return kCudaError;
+  }
+  return kOk;
+}
+
 }  // namespace
 
 size_t decode_workspace_size(const DecodeArgs& a) {
@@ -3654,33 +3683,29 @@ int launch_decode(const DecodeArgs& a, void* workspace, size_t workspace_bytes,
     ws_acc = reinterpret_cast<float*>(base);
     ws_ml = reinterpret_cast<float2*>(base + slots * a.head_dim * sizeof(float));
   }
-  int rc = kOk;
-  if (p.tc) {
-    rc = launch_tc(a, p, ws_acc, ws_ml, stream);
-  } else if (p.fast) {
-    rc = a.block_size == 16 ? dispatch_hg<16>(a, p, ws_acc, ws_ml, stream)
-                            : dispatch_hg<32>(a, p, ws_acc, ws_ml, stream);
-  } else {
-    dim3 grid(a.num_seqs, p.max_splits, a.num_heads);
-    decode_generic_kernel<<<grid, kGenThreads, 0, stream>>>(
-        a.q, a.k_cache, a.k_scale, a.v_cache, a.v_scale, a.block_tables, a.seq_lens, a.out,
-        ws_acc, ws_ml, a.num_heads, a.num_kv_heads, a.head_dim, a.block_size, a.num_blocks,
-        a.max_blocks_per_seq, a.sm_scale * kLog2e, p.pages_per_split, p.max_splits,
-        device_error_word());
-  }
+  const int rc = launch_split(a, p, ws_acc, ws_ml, stream);
   if (rc != kOk) return rc;
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) {
-    set_error(std::string("decode launch failed: ") + cudaGetErrorString(e));
-    return kCudaError;
-  }
   // Splits > 1 and empty sequences are finished by the combine.
-  e = launch_combine(a, p, ws_acc, ws_ml, stream);
+  const cudaError_t e = launch_combine(a, p, ws_acc, ws_ml, stream);
   if (e != cudaSuccess) {
     set_error(std::string("combine launch failed: ") + cudaGetErrorString(e));
     return kCudaError;
   }
   return kOk;
+}
+
+void decode_partials_plan(const DecodeArgs& a, int* max_splits, int* pages_per_split) {
+  const Plan p = make_plan(a, true);
+  *max_splits = p.max_splits;
+  *pages_per_split = p.pages_per_split;
+}
+
+int launch_decode_partials(const DecodeArgs& a, float* ws_acc, float2* ws_ml,
+                           cudaStream_t stream) {
+  if (a.num_seqs == 0) return kOk;
+  DecodeArgs b = a;
+  b.out = nullptr;
+  return launch_split(b, make_plan(a, true), ws_acc, ws_ml, stream);
 }
 
 }  // namespace pkv

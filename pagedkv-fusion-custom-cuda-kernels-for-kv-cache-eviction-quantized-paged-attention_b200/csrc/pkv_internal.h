@@ -156,4 +156,22 @@ int decode_kernel_launches(const DecodeArgs& a);
 int launch_decode(const DecodeArgs& a, void* workspace, size_t workspace_bytes,
                   cudaStream_t stream);
 
+// Decode as partials: the split kernel alone, every split's (acc, m in log2
+// units, l) at slot (seq * max_splits + split) * num_heads + head of ws_acc
+// [slots][head_dim] and ws_ml [slots]; a sequence has ceil(pages /
+// pages_per_split) splits, its other slots are not written.  `a.out` is unused.
+void decode_partials_plan(const DecodeArgs& a, int* max_splits, int* pages_per_split);
+int launch_decode_partials(const DecodeArgs& a, float* ws_acc, float2* ws_ml, cudaStream_t stream);
+
+// ---- prefix.cu ------------------------------------------------------------
+struct SharedPrefixArgs {
+  DecodeArgs own;  // queries, caches, each sequence's own pages, output
+  const int32_t* prefix_table;
+  const int32_t* prefix_len;
+  int prefix_width;
+};
+size_t shared_prefix_workspace_size(const SharedPrefixArgs& a);
+int launch_shared_prefix(const SharedPrefixArgs& a, void* workspace, size_t workspace_bytes,
+                         cudaStream_t stream);
+
 }  // namespace pkv

@@ -1,0 +1,696 @@
+// Decode attention for a batch that shares a prefix, over the INT8 paged
+// cache: the prefix's pages are read once for the whole batch instead of once
+// per sequence.
+//
+//   prefix_kernel   (KV head, 256 query rows, part of the prefix): partial
+//                   (acc, m, l) of every row over that part;
+//   the decode split kernels (decode.cu) on the sequences' own pages, asked
+//                   for partials;
+//   join_kernel     one warp per (sequence, query head): all partials of the
+//                   row, joined by their maxima.
+//
+// A query row is a (sequence, query head of the group) pair: with S sequences
+// and G heads per KV head, S G rows meet every K and V tile, so the products
+// are matrix products and run on tcgen05 kind::f16.  fp32 accuracy comes from
+// splitting the fp32 operands: INT8 codes are exact in fp16; a query row,
+// scaled by a power of two, is hi + lo in fp16 (22 bits), and so is p * v_scale.
+// Both halves accumulate into the same fp32 accumulator, so S and O are one
+// 128-column tile each.  (Three signed byte digits on kind::i8, as the decode
+// kernel for single sequences has them, would cost 3/4 of the tensor time but
+// three accumulators per product -- more tensor memory than there is -- and
+// about twice the instructions per score, which are what bounds this kernel.)
+//
+// Roles: two softmax warpgroups (one 128-row tile each, one thread per row),
+// four converting warps (global INT8 pages -> fp16 tiles in shared memory, and
+// the pages' scales), one MMA warp.  The two row tiles alternate on the tensor
+// cores as in prefill.cu.
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <string>
+
+#include "pkv_common.cuh"
+#include "pkv_internal.h"
+
+namespace pkv {
+namespace {
+
+constexpr int kRows = 128;
+constexpr int kKeys = 128;
+constexpr int kPrefixThreads = 13 * 32;
+constexpr int kConvWarp = 8, kMmaWarp = 12;
+constexpr float kLog2e = 1.4426950408889634f;
+// A row's maximum moves when a tile exceeds it by more than 2^kLazy, and p is
+// kept times 2^kPShift: at most 2^15 in fp16.  The low half has fp16's smallest
+// step, 2^-24, so p * v_scale is kept to 2^-25 - kPShift of the row's largest p
+// times the largest V scale.
+constexpr float kLazy = 2.0f;
+constexpr float kPShift = 13.0f;
+
+template <int DP>
+struct PrefixCfg {
+  static constexpr int kChunks = DP / 64;
+  static constexpr int kTileBytes = kKeys * DP * 2;
+  static constexpr int kStages = DP == 128 ? 3 : 6;
+  // Scales of a tile are reused by tile j + kSlots.  A tile's K stage is free
+  // again only after the softmax of tile j - 2 (3 stages) or j - 4 (6 stages).
+  static constexpr int kSlots = DP == 128 ? 2 : 4;
+  static constexpr int kOffQ = 0;  // [row tile][hi, lo]
+  static constexpr int kOffKV = 4 * kTileBytes;
+  static constexpr int kOffScale = kOffKV + kStages * kTileBytes;  // [slot][k, v][128]
+  static constexpr int kOffMask = kOffScale + kSlots * 2 * kKeys * 4;
+  static constexpr int kOffBar = kOffMask + kSlots * 16;
+  static constexpr int kBars = 2 * kStages + kSlots + 8 + 1;
+  static constexpr int kOffMisc = kOffBar + kBars * 8;
+  static constexpr int kSmemBytes = kOffMisc + 32;
+  static constexpr int kOCol = 256;
+  static_assert(kSmemBytes <= 227 * 1024, "shared memory");
+};
+
+struct PrefixParams {
+  const float* q;
+  const int8_t* k_cache;
+  const float* k_scale;
+  const int8_t* v_cache;
+  const float* v_scale;
+  const int32_t* table;       // [width]
+  const int32_t* prefix_len;  // [1]
+  float* acc;                 // [splits][num_seqs * heads][dim]
+  float2* ml;                 // [splits][num_seqs * heads]
+  int64_t num_blocks;
+  int num_seqs, heads, kv_heads, group, dim, bs, width, splits;
+  float qk_scale;  // sm_scale log2e
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Tokens of the prefix: the given length, at most what the table covers.
+__device__ __forceinline__ int prefix_tokens(const int32_t* len, int width, int bs) {
+  return min(max(*len, 0), width * bs);
+}
+
+// Four INT8 codes (little-endian) as two words of fp16 pairs, exact: byte + 128
+// in the low mantissa bits of 1024, minus 1152.
+__device__ __forceinline__ uint2 codes_to_half(uint32_t w) {
+  const uint32_t u = w ^ 0x80808080u;
+  const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+  const __half2 bias = __float2half2_rn(1152.0f);
+  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), bias);
+  const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+}
+
+template <int DP>
+__global__ void __launch_bounds__(kPrefixThreads, 1)
+    prefix_kernel(const PrefixParams p, int* err) {
+  using C = PrefixCfg<DP>;
+  extern __shared__ __align__(1024) uint8_t smem[];  // no static shared memory: 1024-aligned
+  float* s_scale = reinterpret_cast<float*>(smem + C::kOffScale);
+  uint32_t* s_mask = reinterpret_cast<uint32_t*>(smem + C::kOffMask);
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* kv_empty = kv_full + C::kStages;
+  uint64_t* sc_full = kv_empty + C::kStages;
+  uint64_t* q_full = sc_full + C::kSlots;  // per row tile, as the next three
+  uint64_t* s_full = q_full + 2;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_full = p_full + 2;
+  uint64_t* mma_done = o_full + 2;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
+  int* s_vmax = reinterpret_cast<int*>(smem + C::kOffMisc + 8);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int kvh = blockIdx.x % p.kv_heads, pair = blockIdx.x / p.kv_heads;
+  const int split = blockIdx.y;
+  const int rows = p.num_seqs * p.group;
+  const int len = prefix_tokens(p.prefix_len, p.width, p.bs);
+  if (blockIdx.x == 0 && split == 0 && tid == 0 && *p.prefix_len > len)
+    record_error(err, kDevSeqTooLong);
+  // this part's tokens: equal numbers of tiles
+  const int tiles = (len + kKeys - 1) / kKeys;
+  const int per_split = (tiles + p.splits - 1) / p.splits;
+  const int tile0 = min(split * per_split, tiles);
+  const int n = min(per_split, tiles - tile0);
+  const int two = pair * 256 + kRows < rows;  // the second row tile has rows
+
+  if (tid == 0) {
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(&kv_full[i], 128);
+      mbar_init(&kv_empty[i], 1);
+    }
+    for (int i = 0; i < C::kSlots; ++i) mbar_init(&sc_full[i], 128);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 128);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&o_full[i], 1);
+    }
+    mbar_init(mma_done, 1);
+    mbar_fence_init();
+    *s_vmax = 0;
+  }
+  if (warp == kMmaWarp) tmem_alloc(s_tmem, 512);
+  tmem_fence_before_sync();
+  __syncthreads();
+  tmem_fence_after_sync();
+  const uint32_t tmem = *s_tmem;
+  if (n > 0) {  // the largest V scale of this part: p * v_scale is kept relative to it
+    const int first = tile0 * kKeys / p.bs;
+    const int last = (min((tile0 + n) * kKeys, len) - 1) / p.bs;
+    float v = 0.0f;
+    for (int i = first + tid; i <= last; i += kPrefixThreads) {
+      const int phys = p.table[i];
+      if (phys >= 0 && (int64_t)phys < p.num_blocks)
+        v = fmaxf(v, fabsf(p.v_scale[(int64_t)phys * p.kv_heads + kvh]));
+    }
+    const unsigned m = __reduce_max_sync(0xffffffffu, __float_as_uint(v));
+    if (lane == 0) atomicMax(s_vmax, (int)m);
+  }
+  __syncthreads();
+  const float vmax = __int_as_float(*s_vmax);
+
+  if (warp >= kConvWarp && warp < kMmaWarp) {
+    // ---- pages to fp16 tiles -----------------------------------------------------
+    constexpr int kLanes = DP / 16;            // 16-byte pieces of a token row
+    constexpr int kStep = 128 / kLanes;        // token rows per pass
+    constexpr int kPass = kKeys / kStep;
+    const int ct = tid - kConvWarp * 32;
+    const int piece = ct % kLanes, row0 = ct / kLanes;
+    const int64_t row_bytes = (int64_t)p.kv_heads * p.dim;
+    const bool in_dim = piece * 16 < p.dim;
+    const float inv_vmax = vmax > 0.0f ? 1.0f / vmax : 0.0f;
+    bool ok = true;
+    uint4 raw[2][kPass];
+    auto fetch = [&](int j, int kind) {
+      const int8_t* base = (kind ? p.v_cache : p.k_cache) + (int64_t)kvh * p.dim + piece * 16;
+#pragma unroll
+      for (int i = 0; i < kPass; ++i) {
+        const int tok = (tile0 + j) * kKeys + row0 + i * kStep;
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (tok < len && in_dim) {
+          const int page = tok / p.bs;
+          const int phys = p.table[page];
+          if (phys >= 0 && (int64_t)phys < p.num_blocks)
+            w = __ldg(reinterpret_cast<const uint4*>(
+                base + ((int64_t)phys * p.bs + (tok - page * p.bs)) * row_bytes));
+        }
+        raw[kind][i] = w;
+      }
+    };
+    if (n > 0) fetch(0, 0);
+    for (int j = 0; j < n; ++j) {
+#pragma unroll
+      for (int kind = 0; kind < 2; ++kind) {
+        const int i = 2 * j + kind, st = i % C::kStages;
+        // the next tile's loads are in flight while this one is converted
+        if (kind == 0) fetch(j, 1);
+        else if (j + 1 < n) fetch(j + 1, 0);
+        if (ok && !mbar_wait_bounded(&kv_empty[st], ((uint32_t)(i / C::kStages) & 1u) ^ 1u, err)) {
+          record_error(err, kDevWaitTimeout);
+          ok = false;
+        }
+        if (kind == 0) {  // the tile's scales and which of its tokens count
+          const int slot = j % C::kSlots;
+          const int tok = (tile0 + j) * kKeys + ct;
+          float ks = 0.0f, vs = 0.0f;
+          bool good = tok < len;
+          if (good) {
+            const int phys = p.table[tok / p.bs];
+            good = phys >= 0 && (int64_t)phys < p.num_blocks;
+            if (good) {
+              ks = p.k_scale[(int64_t)phys * p.kv_heads + kvh] * p.qk_scale;
+              vs = p.v_scale[(int64_t)phys * p.kv_heads + kvh] * inv_vmax;
+            } else {
+              record_error(err, kDevBadBlockId);
+            }
+          }
+          s_scale[(slot * 2) * kKeys + ct] = ks;
+          s_scale[(slot * 2 + 1) * kKeys + ct] = vs;
+          const unsigned m = __ballot_sync(0xffffffffu, good);
+          if (lane == 0) s_mask[slot * 4 + (ct >> 5)] = m;
+          mbar_arrive(&sc_full[slot]);
+        }
+        uint8_t* tile = smem + C::kOffKV + st * C::kTileBytes + (piece / 4) * (kKeys * 128);
+#pragma unroll
+        for (int r = 0; r < kPass; ++r) {
+          const int row = row0 + r * kStep;
+          const uint4 w = raw[kind][r];
+          const uint2 a = codes_to_half(w.x), b = codes_to_half(w.y), c = codes_to_half(w.z),
+                      d = codes_to_half(w.w);
+          const int byte = (piece % 4) * 32;
+          *reinterpret_cast<uint4*>(tile + sw128_offset(row, byte)) = make_uint4(a.x, a.y, b.x, b.y);
+          *reinterpret_cast<uint4*>(tile + sw128_offset(row, byte + 16)) =
+              make_uint4(c.x, c.y, d.x, d.y);
+        }
+        fence_proxy_async_smem();  // an MMA operand
+        mbar_arrive(&kv_full[st]);
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    // ---- MMA issue --------------------------------------------------------------------
+    if (lane == 0 && n > 0) {
+      constexpr uint32_t kIdQK = umma_f16_idesc(0, 0, kRows, kKeys);
+      constexpr uint32_t kIdPV = umma_f16_idesc(0, 1, kRows, DP);
+      const uint32_t qa = smem_u32(smem + C::kOffQ), kv = smem_u32(smem + C::kOffKV);
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (ok && !mbar_wait_bounded(bar, parity, err)) {
+          record_error(err, kDevWaitTimeout);
+          ok = false;
+        }
+        tmem_fence_after_sync();
+      };
+      auto stage_of = [&](int i) { return kv + (uint32_t)(i % C::kStages) * C::kTileBytes; };
+      auto wait_tile = [&](int i) {
+        wait(&kv_full[i % C::kStages], (uint32_t)(i / C::kStages) & 1u);
+      };
+      auto release = [&](int i) {  // only if a later tile reuses the stage
+        if (i + C::kStages < 2 * n) umma_commit(&kv_empty[i % C::kStages]);
+      };
+      auto qk = [&](int x, int j) {
+        const uint32_t b = stage_of(2 * j);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t a = qa + (uint32_t)(2 * x + half) * C::kTileBytes;
+#pragma unroll
+          for (int kk = 0; kk < DP / 16; ++kk) {
+            const uint32_t off = (uint32_t)(kk / 4) * (kKeys * 128) + (uint32_t)(kk % 4) * 32;
+            umma_f16(tmem + x * 128, umma_sw128_desc(a + off, 16, 1024),
+                     umma_sw128_desc(b + off, 16, 1024), kIdQK, (half > 0 || kk > 0) ? 1u : 0u);
+          }
+        }
+        umma_commit(&s_full[x]);
+      };
+      // P of tokens 32 i .. 32 i + 31 is in columns 32 i: hi in 16, lo in 16
+      auto pv = [&](int x, int j) {
+        const uint32_t b = stage_of(2 * j + 1);
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 16; ++kk)
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+            umma_f16_ta(tmem + C::kOCol + x * 128,
+                        tmem + x * 128 + (kk / 2) * 32 + half * 16 + (kk % 2) * 8,
+                        umma_sw128_desc(b + kk * 2048, kKeys * 128, 1024), kIdPV,
+                        (j > 0 || kk > 0 || half > 0) ? 1u : 0u);
+        if (j == n - 1) umma_commit(&o_full[x]);
+      };
+      const int nx = two ? 2 : 1;
+      wait_tile(0);
+      for (int x = 0; x < nx; ++x) {
+        wait(&q_full[x], 0);
+        if (ok) qk(x, 0);
+      }
+      release(0);
+      for (int j = 0; j < n && ok; ++j) {
+        wait_tile(2 * j + 1);
+        for (int x = 0; x < nx; ++x) {
+          wait(&p_full[x], (uint32_t)j & 1u);
+          if (!ok) break;
+          pv(x, j);
+          if (x == nx - 1) release(2 * j + 1);
+          if (j + 1 < n) {
+            wait_tile(2 * j + 2);
+            if (!ok) break;
+            qk(x, j + 1);
+          }
+        }
+        if (j + 1 < n) release(2 * j + 2);
+      }
+      umma_commit(mma_done);
+      mbar_drain(mma_done, 0);  // every MMA is done before tensor memory is freed
+    }
+  } else if (warp < 8 && (warp < 4 || two)) {
+    // ---- query split, softmax, partials: thread = row --------------------------------------
+    const int x = warp >> 2, row = tid & 127;
+    const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+    const uint32_t s_addr = tmem + lanes + x * 128, o_addr = tmem + lanes + C::kOCol + x * 128;
+    const int r = pair * 256 + x * kRows + row;
+    const bool valid = r < rows;
+    const int seq = r / p.group;
+    const int64_t head_row = (int64_t)seq * p.heads + kvh * p.group + (r - seq * p.group);
+    float rf = 1.0f;  // power of two that the row was divided by
+    if (n > 0) {
+      const float4* src = reinterpret_cast<const float4*>(p.q + head_row * p.dim);
+      const int n4 = valid ? p.dim / 4 : 0;
+      float big = 0.0f;
+      for (int i = 0; i < n4; ++i) {
+        const float4 v = src[i];
+        big = fmaxf(fmaxf(big, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+      }
+      // largest magnitude to [2^10, 2^11): exact, and lo's steps stay far below hi's
+      float up = 1.0f;
+      if (big > 0.0f && big <= 3.402823466e38f) {
+        const int e = min(10 - ilogbf(big), 126);
+        up = exp2f((float)e);
+        rf = exp2f((float)-e);
+      }
+      uint8_t* hi_t = smem + C::kOffQ + (2 * x) * C::kTileBytes;
+      uint8_t* lo_t = hi_t + C::kTileBytes;
+#pragma unroll 1
+      for (int c = 0; c < DP / 8; ++c) {
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float4 v = 2 * c + i < n4 ? src[2 * c + i] : make_float4(0, 0, 0, 0);
+          f[4 * i] = v.x * up;
+          f[4 * i + 1] = v.y * up;
+          f[4 * i + 2] = v.z * up;
+          f[4 * i + 3] = v.w * up;
+        }
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+          const float2 b = __half22float2(h);
+          const __half2 l = __floats2half2_rn(f[2 * i] - b.x, f[2 * i + 1] - b.y);
+          hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+          lo[i] = *reinterpret_cast<const uint32_t*>(&l);
+        }
+        const uint32_t off = (c / 8) * (kRows * 128) + sw128_offset(row, (c % 8) * 16);
+        *reinterpret_cast<uint4*>(hi_t + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(lo_t + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+      fence_proxy_async_smem();  // an MMA operand
+      mbar_arrive(&q_full[x]);
+    }
+    float m = -INFINITY, l = 0.0f;  // m in units of S * k_scale * qk_scale
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      const int slot = j % C::kSlots;
+      if (ok && (!mbar_wait_bounded(&sc_full[slot], (uint32_t)(j / C::kSlots) & 1u, err) ||
+                 !mbar_wait_bounded(&s_full[x], (uint32_t)j & 1u, err))) {
+        record_error(err, kDevWaitTimeout);
+        ok = false;
+      }
+      __syncwarp();
+      tmem_fence_after_sync();
+      const float4* ks4 = reinterpret_cast<const float4*>(s_scale + slot * 2 * kKeys);
+      const float4* vs4 = ks4 + kKeys / 4;
+      uint32_t mask[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mask[i] = s_mask[slot * 4 + i];
+      float t = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t s[32];
+        tmem_load<32>(s_addr + c * 32, s);
+        tmem_wait_load();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float4 k = ks4[c * 8 + e];
+          const float y[4] = {__uint_as_float(s[4 * e]) * k.x, __uint_as_float(s[4 * e + 1]) * k.y,
+                              __uint_as_float(s[4 * e + 2]) * k.z,
+                              __uint_as_float(s[4 * e + 3]) * k.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (mask[c] >> (4 * e + i) & 1u) t = fmaxf(t, y[i]);
+        }
+      }
+      const bool move = valid && t > m && (m == -INFINITY || (t - m) * rf > kLazy);
+      if (__any_sync(0xffffffffu, move)) {
+        const float alpha = move ? ex2((m - t) * rf) : 1.0f;
+        if (move) m = t;
+        l *= alpha;
+        if (j > 0) {
+#pragma unroll
+          for (int c = 0; c < DP; c += 32) {
+            uint32_t o[32];
+            tmem_load<32>(o_addr + c, o);
+            tmem_wait_load();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_store<32>(o_addr + c, o);
+          }
+        }
+      }
+      const float ms = (m == -INFINITY ? 0.0f : m * rf) - kPShift;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t s[32];
+        tmem_load<32>(s_addr + c * 32, s);
+        tmem_wait_load();
+        uint32_t w[32];  // 16 columns of hi, 16 of lo
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float4 k = ks4[c * 8 + e], v = vs4[c * 8 + e];
+          const float kk[4] = {k.x, k.y, k.z, k.w}, vv[4] = {v.x, v.y, v.z, v.w};
+          float pr[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float y = fmaf(__uint_as_float(s[4 * e + i]) * kk[i], rf, -ms);
+            pr[i] = mask[c] >> (4 * e + i) & 1u ? ex2(y) : 0.0f;
+            sum[i] += pr[i];
+            pr[i] *= vv[i];
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const __half2 h = __floats2half2_rn(pr[2 * i], pr[2 * i + 1]);
+            const float2 b = __half22float2(h);
+            const __half2 lo = __floats2half2_rn(pr[2 * i] - b.x, pr[2 * i + 1] - b.y);
+            w[2 * e + i] = *reinterpret_cast<const uint32_t*>(&h);
+            w[16 + 2 * e + i] = *reinterpret_cast<const uint32_t*>(&lo);
+          }
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_store<32>(s_addr + c * 32, w);
+      }
+      tmem_wait_store();
+      tmem_fence_before_sync();
+      mbar_arrive(&p_full[x]);
+    }
+    if (n > 0) {
+      if (ok && !mbar_wait_bounded(&o_full[x], 0, err)) record_error(err, kDevWaitTimeout);
+      __syncwarp();
+      tmem_fence_after_sync();
+    }
+    const int64_t slot_row = (int64_t)split * p.num_seqs * p.heads + head_row;
+    if (valid) {
+      // nothing attended: (-inf, 0); every score NaN: a NaN that the join keeps
+      float2 ml = make_float2(m * rf - kPShift, l);
+      if (m == -INFINITY) ml = l == 0.0f ? make_float2(-INFINITY, 0.0f) : make_float2(-1e30f, l);
+      p.ml[slot_row] = ml;
+    }
+    if (n > 0) {
+#pragma unroll
+      for (int c = 0; c < DP; c += 32) {
+        uint32_t o[32];
+        tmem_load<32>(o_addr + c, o);
+        tmem_wait_load();
+        if (valid && c < p.dim) {
+          float4* dst = reinterpret_cast<float4*>(p.acc + slot_row * p.dim + c);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            dst[e] = make_float4(__uint_as_float(o[4 * e]) * vmax, __uint_as_float(o[4 * e + 1]) * vmax,
+                                 __uint_as_float(o[4 * e + 2]) * vmax,
+                                 __uint_as_float(o[4 * e + 3]) * vmax);
+        }
+      }
+    }
+  }
+  tmem_fence_before_sync();
+  __syncthreads();
+  if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
+}
+
+// One warp per (sequence, query head): the prefix's partials, then those of
+// the sequence's own pages, in that order (deterministic).  V = dim / 32.
+template <int V>
+__global__ void __launch_bounds__(128)
+    join_kernel(const int32_t* __restrict__ seq_lens, const float* __restrict__ pre_acc,
+                const float2* __restrict__ pre_ml, int pre_splits, const float* __restrict__ own_acc,
+                const float2* __restrict__ own_ml, float* __restrict__ out, int num_seqs, int heads,
+                int bs, int width, int pages_per_split, int own_splits) {
+  constexpr int D = 32 * V;
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int64_t rows = (int64_t)num_seqs * heads;
+  if (row >= rows) return;  // whole warps
+  const int seq = (int)(row / heads), head = (int)(row - (int64_t)seq * heads);
+  const int pages = covered_pages(seq_lens[seq], bs, width);
+  const int n_own = own_splits > 0 ? (pages + pages_per_split - 1) / pages_per_split : 0;
+  const int n = pre_splits + n_own;
+  const int64_t own0 = (int64_t)seq * own_splits * heads + head;
+  auto slot = [&](int i, const float*& acc) {
+    if (i < pre_splits) {
+      acc = pre_acc;
+      return (int64_t)i * rows + row;
+    }
+    acc = own_acc;
+    return own0 + (int64_t)(i - pre_splits) * heads;
+  };
+  auto load_ml = [&](int i) {
+    if (i >= n) return make_float2(-INFINITY, 0.0f);
+    const float* acc;
+    const int64_t s = slot(i, acc);
+    return __ldcg((i < pre_splits ? pre_ml : own_ml) + s);
+  };
+  float M = -INFINITY;
+  for (int b = 0; b < n; b += 32) M = fmaxf(M, load_ml(b + lane).x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  float den = 0.0f, sum[V];
+#pragma unroll
+  for (int c = 0; c < V; ++c) sum[c] = 0.0f;
+  for (int b = 0; b < n; b += 32) {
+    const float2 ml = load_ml(b + lane);
+    const float w = ml.x != -INFINITY ? exp2f(ml.x - M) : 0.0f;
+    if (ml.x != -INFINITY) den += w * ml.y;
+    const int nb = min(32, n - b);
+    for (int j0 = 0; j0 < nb; j0 += 8) {
+      float x[8][V];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float* acc;
+        const int64_t s = slot(b + min(j0 + j, nb - 1), acc);
+#pragma unroll
+        for (int c = 0; c < V; ++c) x[j][c] = __ldcg(acc + s * D + lane + 32 * c);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float wj = __shfl_sync(0xffffffffu, w, (j0 + j) & 31);
+        if (j0 + j < nb && wj != 0.0f) {  // empty parts were not written
+#pragma unroll
+          for (int c = 0; c < V; ++c) sum[c] += wj * x[j][c];
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
+  const float inv = den > 0.0f || den != den ? 1.0f / den : 0.0f;
+#pragma unroll
+  for (int c = 0; c < V; ++c)
+    out[row * D + lane + 32 * c] = den == 0.0f ? 0.0f : sum[c] * inv;
+}
+
+// Parts of the prefix: the CTAs run in waves of one per SM, a part of t tiles
+// costs about t + 2 tile times (query split, pipeline start, partial).
+int prefix_splits(const SharedPrefixArgs& a) {
+  const int64_t tiles =
+      std::max<int64_t>(1, ((int64_t)a.prefix_width * a.own.block_size + kKeys - 1) / kKeys);
+  const int64_t rows = (int64_t)a.own.num_seqs * (a.own.num_heads / a.own.num_kv_heads);
+  const int64_t ctas = (rows + 255) / 256 * a.own.num_kv_heads;
+  int best = 1;
+  int64_t best_cost = INT64_MAX;
+  for (int s = 1; s <= 148 && s <= tiles; ++s) {
+    const int64_t cost = (ctas * s + 147) / 148 * ((tiles + s - 1) / s + 2);
+    if (cost < best_cost) {
+      best_cost = cost;
+      best = s;
+    }
+  }
+  return best;
+}
+
+size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+struct PrefixWs {
+  size_t pre_acc, pre_ml, own_acc, own_ml, bytes;
+  int splits, own_splits, own_pages;
+};
+
+PrefixWs prefix_ws(const SharedPrefixArgs& a) {
+  PrefixWs w;
+  w.splits = a.prefix_width > 0 ? prefix_splits(a) : 0;
+  decode_partials_plan(a.own, &w.own_splits, &w.own_pages);
+  if (a.own.max_blocks_per_seq == 0) w.own_splits = 0;
+  const size_t rows = (size_t)a.own.num_seqs * a.own.num_heads;
+  const size_t pre = rows * w.splits, own = rows * w.own_splits;
+  w.pre_acc = 0;
+  w.pre_ml = up256(pre * a.own.head_dim * sizeof(float));
+  w.own_acc = w.pre_ml + up256(pre * sizeof(float2));
+  w.own_ml = w.own_acc + up256(own * a.own.head_dim * sizeof(float));
+  w.bytes = w.own_ml + up256(own * sizeof(float2)) + 256;
+  return w;
+}
+
+template <int DP>
+void launch_prefix_t(const PrefixParams& p, cudaStream_t stream) {
+  using C = PrefixCfg<DP>;
+  auto kern = prefix_kernel<DP>;
+  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+  const int64_t pairs = ((int64_t)p.num_seqs * p.group + 255) / 256;
+  const dim3 grid((unsigned)(pairs * p.kv_heads), (unsigned)p.splits);
+  kern<<<grid, kPrefixThreads, C::kSmemBytes, stream>>>(p, device_error_word());
+}
+
+}  // namespace
+
+size_t shared_prefix_workspace_size(const SharedPrefixArgs& a) { return prefix_ws(a).bytes; }
+
+int launch_shared_prefix(const SharedPrefixArgs& a, void* workspace, size_t workspace_bytes,
+                         cudaStream_t stream) {
+  const DecodeArgs& o = a.own;
+  if (o.num_seqs == 0) return kOk;
+  const PrefixWs w = prefix_ws(a);
+  if (workspace == nullptr || workspace_bytes < w.bytes) {
+    set_error("workspace too small for shared_prefix_attention: need " + std::to_string(w.bytes) +
+              " bytes");
+    return kWorkspace;
+  }
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 255) &
+                                             ~(uintptr_t)255);
+  float* pre_acc = reinterpret_cast<float*>(base + w.pre_acc);
+  float2* pre_ml = reinterpret_cast<float2*>(base + w.pre_ml);
+  float* own_acc = reinterpret_cast<float*>(base + w.own_acc);
+  float2* own_ml = reinterpret_cast<float2*>(base + w.own_ml);
+  if (w.splits > 0) {
+    PrefixParams p;
+    p.q = o.q;
+    p.k_cache = o.k_cache;
+    p.k_scale = o.k_scale;
+    p.v_cache = o.v_cache;
+    p.v_scale = o.v_scale;
+    p.table = a.prefix_table;
+    p.prefix_len = a.prefix_len;
+    p.acc = pre_acc;
+    p.ml = pre_ml;
+    p.num_blocks = o.num_blocks;
+    p.num_seqs = o.num_seqs;
+    p.heads = o.num_heads;
+    p.kv_heads = o.num_kv_heads;
+    p.group = o.num_heads / o.num_kv_heads;
+    p.dim = o.head_dim;
+    p.bs = o.block_size;
+    p.width = a.prefix_width;
+    p.splits = w.splits;
+    p.qk_scale = o.sm_scale * kLog2e;
+    if (o.head_dim <= 64) launch_prefix_t<64>(p, stream);
+    else launch_prefix_t<128>(p, stream);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) {
+      set_error(std::string("prefix launch failed: ") + cudaGetErrorString(e));
+      return kCudaError;
+    }
+  }
+  if (w.own_splits > 0) {
+    const int rc = launch_decode_partials(o, own_acc, own_ml, stream);
+    if (rc != kOk) return rc;
+  }
+  const int64_t rows = (int64_t)o.num_seqs * o.num_heads;
+  const unsigned grid = (unsigned)((rows + 3) / 4);
+#define PKV_JOIN(V)                                                                              \
+  case V:                                                                                        \
+    join_kernel<V><<<grid, 128, 0, stream>>>(o.seq_lens, pre_acc, pre_ml, w.splits, own_acc,     \
+                                             own_ml, o.out, o.num_seqs, o.num_heads,             \
+                                             o.block_size, o.max_blocks_per_seq, w.own_pages,    \
+                                             w.own_splits);                                      \
+    break;
+  switch (o.head_dim / 32) {
+    PKV_JOIN(1) PKV_JOIN(2) PKV_JOIN(3) PKV_JOIN(4)
+  }
+#undef PKV_JOIN
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) {
+    set_error(std::string("join launch failed: ") + cudaGetErrorString(e));
+    return kCudaError;
+  }
+  return kOk;
+}
+
+}  // namespace pkv

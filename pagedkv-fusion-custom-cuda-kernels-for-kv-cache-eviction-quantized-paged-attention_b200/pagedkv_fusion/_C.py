@@ -94,6 +94,11 @@ _prefill = _sig("pkv_prefill_attention",
                 [_P, _P, _P, _I32, _P, _P, _P, _P, _I32, _I64, _I64, _I32, _I32, _I32, _I64, _I64,
                  _I64, _I64, _I64, _I64, _F, _I32, _P])
 
+_prefix_ws = _sig("pkv_shared_prefix_attention_workspace_size",
+                  [_I32] * 5 + [_I64, _I32, _I32], _SZ)
+_prefix = _sig("pkv_shared_prefix_attention",
+               [_P] * 10 + [_I32] * 5 + [_I64, _I32, _I32, _F, _P, _SZ, _P])
+
 LIBRARY_PATH = str(_LIB_PATH)
 _DTYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
@@ -627,3 +632,48 @@ def prefill_attention(q, k, v, cu_seqlens, sm_scale, cu_seqlens_k=None, causal=T
                         qc.stride(1), kc.stride(0), kc.stride(1), vc.stride(0), vc.stride(1),
                         float(sm_scale), 1 if causal else 0, _stream(q)))
     return (out, lse) if return_lse else out
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous and 16-byte aligned: itself where it is, else a copy."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def shared_prefix_attention(q, k_cache_q, k_scale, v_cache_q, v_scale, prefix_table, prefix_len,
+                            block_tables, seq_lens, sm_scale):
+    """INT8 paged decode attention over [shared prefix | own tokens]."""
+    _check_inputs(q, k_cache_q, k_scale, v_cache_q, v_scale, prefix_table, prefix_len,
+                  block_tables, seq_lens)
+    _require(q.dtype == torch.float32, "q must be float32 (v1)")
+    _require(k_cache_q.dtype == torch.int8 and v_cache_q.dtype == torch.int8,
+             "k_cache_q and v_cache_q must be int8")
+    _require(k_scale.dtype == torch.float32 and v_scale.dtype == torch.float32,
+             "k_scale/v_scale must be float32")
+    _require(block_tables.dtype == torch.int32 and prefix_table.dtype == torch.int32,
+             "block_tables and prefix_table must be int32")
+    _require(q.dim() == 3 and k_cache_q.dim() == 4 and block_tables.dim() == 2
+             and prefix_table.dim() == 1,
+             "expected q [S, H, D], caches [NB, bs, Hkv, D], prefix_table [P], block_tables [S, M]")
+    S, H, D = q.shape
+    NB, bs, Hkv, Dk = k_cache_q.shape
+    _require(Dk == D and v_cache_q.shape == k_cache_q.shape, "cache head_dim must match q")
+    _require(tuple(k_scale.shape) == (NB, Hkv) and tuple(v_scale.shape) == (NB, Hkv),
+             "scales must be [num_blocks, num_kv_heads]")
+    _require(block_tables.shape[0] == S and seq_lens.numel() == S,
+             "block_tables/seq_lens must have num_seqs rows")
+    _require(prefix_len.numel() == 1 and prefix_len.dtype in (torch.int32, torch.int64),
+             "prefix_len must hold one integer")
+    _require(seq_lens.dtype in (torch.int32, torch.int64), "seq_lens must be int32 or int64")
+    qc, kc, vc = _aligned(q), _aligned(k_cache_q), _aligned(v_cache_q)
+    ks, vs, bt, pt = (t.contiguous() for t in (k_scale, v_scale, block_tables, prefix_table))
+    sl, pl = seq_lens.to(torch.int32).contiguous(), prefix_len.to(torch.int32)
+    out = torch.empty((S, H, D), dtype=torch.float32, device=q.device)
+    P, M = pt.shape[0], bt.shape[1]
+    with _on_device(q):
+        ws, wp = _workspace(_prefix_ws(S, H, Hkv, D, bs, NB, P, M), q.device)
+        _check(_prefix(qc.data_ptr(), kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(),
+                       pt.data_ptr(), pl.data_ptr(), bt.data_ptr(), sl.data_ptr(), out.data_ptr(),
+                       S, H, Hkv, D, bs, NB, P, M, float(sm_scale), wp,
+                       0 if ws is None else ws.numel(), _stream(q)))
+    return out

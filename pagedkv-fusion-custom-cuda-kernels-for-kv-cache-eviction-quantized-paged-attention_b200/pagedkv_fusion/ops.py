@@ -44,6 +44,7 @@ __all__ = [
     "qk_norm_rope",
     "append_kv",
     "prefill_attention",
+    "shared_prefix_attention",
 ]
 
 
@@ -415,3 +416,34 @@ def prefill_attention(q, k, v, cu_seqlens, sm_scale: float, cu_seqlens_k=None,
                               None if cu_seqlens_k is None else
                               st.to_device(cu_seqlens_k, torch.int32), causal, return_lse)
     return tuple(st.back(t) for t in got) if return_lse else st.back(got)
+
+
+# ---------------------------------------------------------------------------
+# Decode over a shared prefix
+# ---------------------------------------------------------------------------
+
+def shared_prefix_attention(q, k_cache_q, k_scale, v_cache_q, v_scale, prefix_table, prefix_len,
+                            block_tables, seq_lens, sm_scale: float):
+    """Decode-step attention over the INT8 paged cache for a batch whose
+    sequences share a prefix (a system prompt, a document): what
+    :func:`quant_paged_attention` gives for ``[prefix | own tokens]``, with
+    the prefix's pages read once for the whole batch.
+
+    ``q`` float32 ``[S, H, D]``, caches and scales as there.  ``prefix_table``
+    int32 ``[P]`` and ``prefix_len`` (one integer in a tensor, read on the
+    device, so a captured call follows it) give the prefix's pages;
+    ``block_tables`` ``[S, M]`` and ``seq_lens`` ``[S]`` those of each
+    sequence's own tokens, which start on a page of their own.  Any of the
+    lengths may be 0.  D a multiple of 32 up to 128, block size up to 64.
+    fp32 accuracy (about 1e-6 of the result).  No backward pass.
+    """
+    C = _lib()
+    args = (q, k_cache_q, k_scale, v_cache_q, v_scale, prefix_table, prefix_len, block_tables,
+            seq_lens)
+    if _all_cuda(*args):
+        return C.shared_prefix_attention(*args, sm_scale)
+    st = _Staging(*args)
+    types = (torch.float32, None, torch.float32, None, torch.float32, torch.int32, torch.int32,
+             torch.int32, torch.int32)
+    return st.back(C.shared_prefix_attention(*(st.to_device(a, t) for a, t in zip(args, types)),
+                                             sm_scale))
