@@ -47,6 +47,8 @@ constexpr int kLoadWarp = 8, kMmaWarp = 9, kCleanWarp = 10;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLazy = 8.0f;   // log2 growth of a row maximum that moves it
+// Of kPolyOf pairs of exponentials, kPolyTake go to the FMA units.
+constexpr int kPolyOf = 4, kPolyTake = 1;
 constexpr int kMaskedTiles = 4; // tiles with masked keys per CTA: 256 tokens span at most 3
 
 template <int DP>
@@ -156,6 +158,28 @@ __device__ __forceinline__ uint32_t nonfinite_mask(uint32_t w, __half) {
          ((w & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u);
 }
 
+// 2^x of two values on the FMA units (the special-function unit alone, 16 per
+// clock and SM, would take as long as the tensor cores): x = n + f, n the
+// nearest integer, 2^f by the degree-5 minimax polynomial on [-1/2, 1/2]
+// (relative error 2^-23.7, from a Remez exchange), n added to the exponent.
+// Below 2^-125 the result stays about there.  Not for NaN.
+__device__ __forceinline__ float2 exp2_poly2(uint64_t x) {
+  constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: the sum's low bits are n
+  float2 v = unpack_f32x2(x);
+  x = f32x2(fmaxf(v.x, -125.0f), fmaxf(v.y, -125.0f));
+  const uint64_t n = add_f32x2(x, f32x2(kRound, kRound));
+  const uint64_t f = sub_f32x2(x, sub_f32x2(n, f32x2(kRound, kRound)));
+  uint64_t y = f32x2(0.0013276472454890609f, 0.0013276472454890609f);
+  y = fma_f32x2(y, f, f32x2(0.009675540961325169f, 0.009675540961325169f));
+  y = fma_f32x2(y, f, f32x2(0.05550713092088699f, 0.05550713092088699f));
+  y = fma_f32x2(y, f, f32x2(0.24022120237350464f, 0.24022120237350464f));
+  y = fma_f32x2(y, f, f32x2(0.6931469440460205f, 0.6931469440460205f));
+  y = fma_f32x2(y, f, f32x2(1.0000001192092896f, 1.0000001192092896f));
+  const float2 r = unpack_f32x2(y), m = unpack_f32x2(n);
+  return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(m.x) << 23)),
+                     __int_as_float(__float_as_int(r.y) + (__float_as_int(m.y) << 23)));
+}
+
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -219,7 +243,6 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   __syncthreads();
   tmem_fence_after_sync();
   const uint32_t tmem = *s_tmem;
-
   if (s_work[0]) {
     const int q0 = s_work[1], lq = s_work[2], k0 = s_work[3], lk = s_work[4], t0 = s_work[5];
     const int shift = lk - lq;  // key of token i under the causal mask: i + shift
@@ -237,6 +260,9 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     const int first_masked =
         p.causal ? min(max(t0 + shift + 1, 0), lk) / kKeys : lk / kKeys;
 
+    if (warp >= 8) {
+    // 8 x 32 x 208 + 4 x 32 x 88 = 64,512 = 384 x 168, the registers at launch
+    registers_down<88>();
     if (warp == kLoadWarp) {
       // ---- loads: the Q tiles, then K and V tiles in turn ----------------------
       if (lane == 0 && n > 0) {
@@ -343,7 +369,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         umma_commit(mma_done);
         mbar_drain(mma_done, 0);  // every MMA is done before tensor memory is freed
       }
-    } else if (warp >= kCleanWarp) {
+    } else {
       // ---- V tiles with masked keys ----------------------------------------------
       const int t64 = tid - kCleanWarp * 32;
       bool ok = true;
@@ -381,7 +407,9 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         named_barrier(1, 64);
         if (t64 == 0) mbar_arrive(&kv_full[i % C::kStages]);
       }
-    } else if (warp < 8) {
+    }
+    } else {
+      registers_up<208>();
       // ---- softmax and epilogue: thread = row ---------------------------------------
       const int x = warp >> 2;
       const int row = tid & 127;
@@ -415,9 +443,13 @@ __global__ void __launch_bounds__(kPreThreads, 1)
 #pragma unroll
           for (int c = 0; c < kKeys; ++c) s[c] = c < seen ? s[c] : -INFINITY;
         }
-        float t = s[0];
+        float tm[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int c = 1; c < kKeys; ++c) t = fmaxf(t, s[c]);
+        for (int c = 4; c < kKeys - 4; c += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) tm[e] = max3_nan(tm[e], s[c + e], s[c + e + 4]);
+        const float t = max3_nan(max3_nan(tm[0], tm[1], max3_nan(tm[2], tm[3], s[kKeys - 4])),
+                                 s[kKeys - 3], max3_nan(s[kKeys - 2], s[kKeys - 1], tm[0]));
         // move the maximum where it grew by more than 2^kLazy (or from -inf);
         // each row by its own scores, so that its bits do not depend on others
         const bool move =
@@ -438,22 +470,36 @@ __global__ void __launch_bounds__(kPreThreads, 1)
             }
           }
         }
-        const float ms = m == -INFINITY ? 0.0f : m * p.scale_log2;
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        // a NaN score makes the whole row NaN
+        const float ms = t != t ? t : (m == -INFINITY ? 0.0f : m * p.scale_log2);
+        const uint64_t scale2 = f32x2(p.scale_log2, p.scale_log2), ms2 = f32x2(-ms, -ms);
+        uint64_t sum[2] = {0, 0};
+        auto exponentials = [&](auto poly) {
 #pragma unroll
-        for (int c = 0; c < kKeys; c += 32) {
-          uint32_t pk[16];
+          for (int c = 0; c < kKeys; c += 32) {
+            uint32_t pk[16];
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float a = exp2_approx(fmaf(s[c + e], p.scale_log2, -ms));
-            const float b = exp2_approx(fmaf(s[c + e + 1], p.scale_log2, -ms));
-            sum[e & 2] += a;
-            sum[(e & 2) + 1] += b;
-            pk[e / 2] = pack2(a, b, T());
+            for (int e = 0; e < 32; e += 2) {
+              const uint64_t y = fma_f32x2(f32x2(s[c + e], s[c + e + 1]), scale2, ms2);
+              float2 v;
+              if (decltype(poly)::value && (e / 2) % kPolyOf < kPolyTake) {
+                v = exp2_poly2(y);
+              } else {
+                v = unpack_f32x2(y);
+                v.x = exp2_approx(v.x);
+                v.y = exp2_approx(v.y);
+              }
+              sum[(e / 2) & 1] = add_f32x2(sum[(e / 2) & 1], f32x2(v.x, v.y));
+              pk[e / 2] = pack2(v.x, v.y, T());
+            }
+            tmem_store<16>(s_addr + c / 2, pk);
           }
-          tmem_store<16>(s_addr + c / 2, pk);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        };
+        // the polynomial has no zero for masked scores
+        if (j < first_masked) exponentials(std::true_type());
+        else exponentials(std::false_type());
+        const float2 l2 = unpack_f32x2(add_f32x2(sum[0], sum[1]));
+        l += l2.x + l2.y;
         tmem_wait_store();
         tmem_fence_before_sync();
         mbar_arrive(&p_full[x]);

@@ -274,13 +274,13 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       auto qk = [&](int x, int j) {
         const uint32_t b = stage_of(2 * j);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+        for (int half = 1; half >= 0; --half) {  // lo first: roundings of a small sum
           const uint32_t a = qa + (uint32_t)(2 * x + half) * C::kTileBytes;
 #pragma unroll
           for (int kk = 0; kk < DP / 16; ++kk) {
             const uint32_t off = (uint32_t)(kk / 4) * (kKeys * 128) + (uint32_t)(kk % 4) * 32;
             umma_f16(tmem + x * 128, umma_sw128_desc(a + off, 16, 1024),
-                     umma_sw128_desc(b + off, 16, 1024), kIdQK, (half > 0 || kk > 0) ? 1u : 0u);
+                     umma_sw128_desc(b + off, 16, 1024), kIdQK, (half < 1 || kk > 0) ? 1u : 0u);
           }
         }
         umma_commit(&s_full[x]);

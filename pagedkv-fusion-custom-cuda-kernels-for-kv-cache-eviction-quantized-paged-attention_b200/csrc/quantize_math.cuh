@@ -8,6 +8,8 @@
 
 #include <cstdint>
 
+#include "pkv_common.cuh"
+
 namespace pkv {
 
 template <typename T>
@@ -35,29 +37,6 @@ static __device__ __noinline__ uint32_t quantize_word_exact(float x0, float x1, 
          ((uint32_t)(quantize_one(x1, scale) & 255) << 8) |
          ((uint32_t)(quantize_one(x2, scale) & 255) << 16) |
          ((uint32_t)(quantize_one(x3, scale) & 255) << 24);
-}
-
-// Two fp32 lanes in one 64-bit register, for Blackwell's packed f32x2
-// arithmetic (each lane rounded exactly like the scalar instruction).
-__device__ __forceinline__ uint64_t f32x2(float lo, float hi) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
-  return d;
-}
-__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t sub_f32x2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
 }
 
 // Four codes packed little-endian.  Fast path, for a head whose absmax is
