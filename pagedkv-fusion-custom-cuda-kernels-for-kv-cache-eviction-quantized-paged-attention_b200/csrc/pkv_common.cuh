@@ -201,6 +201,16 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   }
 }
 
+// mbar_wait_bounded for hand-offs inside a CTA that take well under a
+// microsecond: a few plain tries first, since reading the timer takes about as
+// long as the wait.
+__device__ __forceinline__ bool mbar_wait_short(uint64_t* bar, uint32_t parity, const int* err) {
+#pragma unroll 1
+  for (int i = 0; i < 64; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait_bounded(bar, parity, err);
+}
+
 // Waits (at most limit_ns, ignoring the error word) for the phase of a
 // barrier that this thread's own copies complete: a producer calls it for
 // every load it issued before it exits, so that no copy can land in shared
@@ -343,6 +353,12 @@ __device__ __forceinline__ uint64_t umma_sw128_desc(uint32_t smem_addr, uint32_t
          ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) | (1ull << 46) | (2ull << 61);
 }
 
+// The same descriptor `bytes` further on (a multiple of 16; addresses stay
+// below 256 KB, so the 14 address bits do not overflow into the next field).
+__device__ __forceinline__ uint64_t umma_desc_at(uint64_t desc, uint32_t bytes) {
+  return desc + (uint64_t)(bytes >> 4);
+}
+
 // Instruction descriptor of tcgen05.mma .kind::i8 with an s32 accumulator:
 // A / B signed (1) or unsigned (0) 8-bit, K-major (0) or MN-major (1).
 __host__ __device__ constexpr uint32_t umma_i8_idesc(int a_signed, int b_signed, int a_mn,
@@ -370,23 +386,35 @@ __host__ __device__ constexpr uint32_t umma_f16_idesc(int bf16, int b_mn, int m,
 }
 
 // D[tmem] (+)= A * B^T for one K step of 16 values, A and B in shared memory.
-__device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b,
-                                         uint32_t idesc, uint32_t accumulate) {
+// Called by a whole converged warp, of which one lane, always the same, issues:
+// descriptors then stay in uniform registers (issued from a lane's own branch,
+// a 128 x 128 x 16 step took 70 to 94 clocks instead of its 64).
+__device__ __forceinline__ void umma_f16_warp(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b,
+                                              uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(tmem_d),
-      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0)
+      "{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
 // The same with A in tensor memory: lane = row, two values of K per column.
-__device__ __forceinline__ void umma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b,
-                                            uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void umma_f16_ta_warp(uint32_t tmem_d, uint32_t tmem_a,
+                                                 uint64_t desc_b, uint32_t idesc,
+                                                 uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(
-          tmem_d),
-      "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0)
+      "{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// umma_commit by the lane that the two functions above issue from.
+__device__ __forceinline__ void umma_commit_warp(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+          smem_u32(bar))
       : "memory");
 }
 

@@ -252,51 +252,54 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     }
   } else if (warp == kMmaWarp) {
     // ---- MMA issue --------------------------------------------------------------------
-    if (lane == 0 && n > 0) {
+    if (n > 0) {
       constexpr uint32_t kIdQK = umma_f16_idesc(0, 0, kRows, kKeys);
       constexpr uint32_t kIdPV = umma_f16_idesc(0, 1, kRows, DP);
-      const uint32_t qa = smem_u32(smem + C::kOffQ), kv = smem_u32(smem + C::kOffKV);
+      const uint32_t kv = smem_u32(smem + C::kOffKV);
+      const uint64_t q_desc = umma_sw128_desc(smem_u32(smem + C::kOffQ), 16, 1024);
+      const uint64_t k_desc = umma_sw128_desc(kv, 16, 1024);
+      const uint64_t v_desc = umma_sw128_desc(kv, kKeys * 128, 1024);
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (ok && !mbar_wait_bounded(bar, parity, err)) {
+        if (ok && !mbar_wait_short(bar, parity, err)) {
           record_error(err, kDevWaitTimeout);
           ok = false;
         }
         tmem_fence_after_sync();
       };
-      auto stage_of = [&](int i) { return kv + (uint32_t)(i % C::kStages) * C::kTileBytes; };
+      auto stage_of = [&](int i) { return (uint32_t)(i % C::kStages) * C::kTileBytes; };
       auto wait_tile = [&](int i) {
         wait(&kv_full[i % C::kStages], (uint32_t)(i / C::kStages) & 1u);
       };
       auto release = [&](int i) {  // only if a later tile reuses the stage
-        if (i + C::kStages < 2 * n) umma_commit(&kv_empty[i % C::kStages]);
+        if (i + C::kStages < 2 * n) umma_commit_warp(&kv_empty[i % C::kStages]);
       };
       auto qk = [&](int x, int j) {
-        const uint32_t b = stage_of(2 * j);
+        const uint64_t b = umma_desc_at(k_desc, stage_of(2 * j));
 #pragma unroll
         for (int half = 1; half >= 0; --half) {  // lo first: roundings of a small sum
-          const uint32_t a = qa + (uint32_t)(2 * x + half) * C::kTileBytes;
+          const uint64_t a = umma_desc_at(q_desc, (uint32_t)(2 * x + half) * C::kTileBytes);
 #pragma unroll
           for (int kk = 0; kk < DP / 16; ++kk) {
             const uint32_t off = (uint32_t)(kk / 4) * (kKeys * 128) + (uint32_t)(kk % 4) * 32;
-            umma_f16(tmem + x * 128, umma_sw128_desc(a + off, 16, 1024),
-                     umma_sw128_desc(b + off, 16, 1024), kIdQK, (half < 1 || kk > 0) ? 1u : 0u);
+            umma_f16_warp(tmem + x * 128, umma_desc_at(a, off), umma_desc_at(b, off), kIdQK,
+                          (half < 1 || kk > 0) ? 1u : 0u);
           }
         }
-        umma_commit(&s_full[x]);
+        umma_commit_warp(&s_full[x]);
       };
       // P of tokens 32 i .. 32 i + 31 is in columns 32 i: hi in 16, lo in 16
       auto pv = [&](int x, int j) {
-        const uint32_t b = stage_of(2 * j + 1);
+        const uint64_t b = umma_desc_at(v_desc, stage_of(2 * j + 1));
 #pragma unroll
         for (int kk = 0; kk < kKeys / 16; ++kk)
 #pragma unroll
           for (int half = 0; half < 2; ++half)
-            umma_f16_ta(tmem + C::kOCol + x * 128,
+            umma_f16_ta_warp(tmem + C::kOCol + x * 128,
                         tmem + x * 128 + (kk / 2) * 32 + half * 16 + (kk % 2) * 8,
-                        umma_sw128_desc(b + kk * 2048, kKeys * 128, 1024), kIdPV,
+                        umma_desc_at(b, kk * 2048), kIdPV,
                         (j > 0 || kk > 0 || half > 0) ? 1u : 0u);
-        if (j == n - 1) umma_commit(&o_full[x]);
+        if (j == n - 1) umma_commit_warp(&o_full[x]);
       };
       const int nx = two ? 2 : 1;
       wait_tile(0);
@@ -320,7 +323,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         }
         if (j + 1 < n) release(2 * j + 2);
       }
-      umma_commit(mma_done);
+      umma_commit_warp(mma_done);
       mbar_drain(mma_done, 0);  // every MMA is done before tensor memory is freed
     }
   } else if (warp < 8 && (warp < 4 || two)) {
@@ -382,7 +385,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     for (int j = 0; j < n; ++j) {
       const int slot = j % C::kSlots;
       if (ok && (!mbar_wait_bounded(&sc_full[slot], (uint32_t)(j / C::kSlots) & 1u, err) ||
-                 !mbar_wait_bounded(&s_full[x], (uint32_t)j & 1u, err))) {
+                 !mbar_wait_short(&s_full[x], (uint32_t)j & 1u, err))) {
         record_error(err, kDevWaitTimeout);
         ok = false;
       }
