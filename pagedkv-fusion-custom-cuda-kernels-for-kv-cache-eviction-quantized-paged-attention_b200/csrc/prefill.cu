@@ -19,8 +19,8 @@
 // then, which is safe because S(j) is complete only after P V (j - 1).
 //
 // Masked places hold no influence: masked scores become -inf by selection,
-// and in tiles that contain masked keys the V rows are cleaned first (two
-// warps, off the critical path): rows past the sequence become zero, and
+// and in tiles that contain masked keys the V rows are cleaned first (by
+// five warps, off the critical path): rows past the sequence become zero, and
 // where causal masking hides a key from some rows, its non-finite values are
 // taken out of the product and added, in the epilogue, to the rows that see
 // it.
@@ -42,13 +42,14 @@ namespace {
 
 constexpr int kRows = 128;      // rows of a row tile (MMA M)
 constexpr int kKeys = 128;      // keys of a tile (MMA N of Q K^T, K of P V)
-constexpr int kPreThreads = 384;  // softmax A, softmax B, load, MMA, 2 cleaning warps
-constexpr int kLoadWarp = 8, kMmaWarp = 9, kCleanWarp = 10;
+constexpr int kPreThreads = 512;  // softmax A and B (4 warps each), load, MMA A and B, cleaning (5)
+constexpr int kLoadWarp = 8, kMmaWarp = 9, kCleanWarp = 11;
+constexpr int kCleaners = kPreThreads - kCleanWarp * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLazy = 8.0f;   // log2 growth of a row maximum that moves it
-// Of kPolyOf pairs of exponentials, kPolyTake go to the FMA units.
-constexpr int kPolyOf = 4, kPolyTake = 1;
+constexpr int kPart = 64;        // keys of P that are handed over first
+constexpr int kEarly = 4;        // MMAs left of a step when the turn is passed on
 constexpr int kMaskedTiles = 4; // tiles with masked keys per CTA: 256 tokens span at most 3
 
 template <int DP>
@@ -59,7 +60,7 @@ struct PreCfg {
   static constexpr int kOffQ = 0;                       // two Q tiles
   static constexpr int kOffKV = 2 * kTileBytes;
   static constexpr int kOffBar = kOffKV + kStages * kTileBytes;
-  static constexpr int kBars = 2 * kStages + 8 + kMaskedTiles + 1;
+  static constexpr int kBars = 2 * kStages + 10 + kMaskedTiles + 3;
   static constexpr int kOffMisc = kOffBar + kBars * 8;
   static constexpr int kSmemBytes = kOffMisc + 64 + kMaskedTiles * 16 + 1024;
   static constexpr int kSCol = 0;                       // S / P of the two tiles
@@ -148,6 +149,17 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
 __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
 
+// Both 16-bit floats of a word times zero: +-0 if they are finite, else NaN.
+__device__ __forceinline__ uint32_t times_zero(uint32_t w, __nv_bfloat16) {
+  const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w),
+                                   __float2bfloat162_rn(0.0f));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t times_zero(uint32_t w, __half) {
+  const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&w), __float2half2_rn(0.0f));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
 // Whether either 16-bit float of a word is infinite or NaN (all exponent bits set).
 __device__ __forceinline__ uint32_t nonfinite_mask(uint32_t w, __nv_bfloat16) {
   return ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) |
@@ -156,28 +168,6 @@ __device__ __forceinline__ uint32_t nonfinite_mask(uint32_t w, __nv_bfloat16) {
 __device__ __forceinline__ uint32_t nonfinite_mask(uint32_t w, __half) {
   return ((w & 0x7c00u) == 0x7c00u ? 0xffffu : 0u) |
          ((w & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u);
-}
-
-// 2^x of two values on the FMA units (the special-function unit alone, 16 per
-// clock and SM, would take as long as the tensor cores): x = n + f, n the
-// nearest integer, 2^f by the degree-5 minimax polynomial on [-1/2, 1/2]
-// (relative error 2^-23.7, from a Remez exchange), n added to the exponent.
-// Below 2^-125 the result stays about there.  Not for NaN.
-__device__ __forceinline__ float2 exp2_poly2(uint64_t x) {
-  constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: the sum's low bits are n
-  float2 v = unpack_f32x2(x);
-  x = f32x2(fmaxf(v.x, -125.0f), fmaxf(v.y, -125.0f));
-  const uint64_t n = add_f32x2(x, f32x2(kRound, kRound));
-  const uint64_t f = sub_f32x2(x, sub_f32x2(n, f32x2(kRound, kRound)));
-  uint64_t y = f32x2(0.0013276472454890609f, 0.0013276472454890609f);
-  y = fma_f32x2(y, f, f32x2(0.009675540961325169f, 0.009675540961325169f));
-  y = fma_f32x2(y, f, f32x2(0.05550713092088699f, 0.05550713092088699f));
-  y = fma_f32x2(y, f, f32x2(0.24022120237350464f, 0.24022120237350464f));
-  y = fma_f32x2(y, f, f32x2(0.6931469440460205f, 0.6931469440460205f));
-  y = fma_f32x2(y, f, f32x2(1.0000001192092896f, 1.0000001192092896f));
-  const float2 r = unpack_f32x2(y), m = unpack_f32x2(n);
-  return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(m.x) << 23)),
-                     __int_as_float(__float_as_int(r.y) + (__float_as_int(m.y) << 23)));
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -200,10 +190,11 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   uint64_t* kv_empty = kv_full + C::kStages;
   uint64_t* q_full = kv_empty + C::kStages;  // per row tile, as the next three
   uint64_t* s_full = q_full + 2;
-  uint64_t* p_full = s_full + 2;
-  uint64_t* o_full = p_full + 2;
+  uint64_t* p_full = s_full + 2;  // [row tile][part of P]
+  uint64_t* o_full = p_full + 4;
   uint64_t* raw_full = o_full + 2;  // V tiles with masked keys, before they are cleaned
   uint64_t* mma_done = raw_full + kMaskedTiles;
+  uint64_t* turn = mma_done + 1;  // per row tile
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
   int* s_work = reinterpret_cast<int*>(smem + C::kOffMisc + 16);
   uint32_t* s_flags = reinterpret_cast<uint32_t*>(smem + C::kOffMisc + 64);  // [tile][4]
@@ -225,16 +216,19 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   if (tid == 32) {
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 1);
+      mbar_init(&kv_empty[i], 2);  // both MMA warps
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
+      mbar_init(&p_full[2 * i], 128);
+      mbar_init(&p_full[2 * i + 1], 128);
       mbar_init(&o_full[i], 1);
     }
     for (int i = 0; i < kMaskedTiles; ++i) mbar_init(&raw_full[i], 1);
-    mbar_init(mma_done, 1);
+    mbar_init(mma_done, 2);
+    mbar_init(&turn[0], 1);
+    mbar_init(&turn[1], 1);
     mbar_fence_init();
   }
   if (warp == kMmaWarp) tmem_alloc(s_tmem, 512);
@@ -261,8 +255,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         p.causal ? min(max(t0 + shift + 1, 0), lk) / kKeys : lk / kKeys;
 
     if (warp >= 8) {
-    // 8 x 32 x 208 + 4 x 32 x 88 = 64,512 = 384 x 168, the registers at launch
-    registers_down<88>();
+    // 256 x 200 + 256 x 56 = 65,536 = 512 x 128, the registers at launch
+    registers_down<56>();
     if (warp == kLoadWarp) {
       // ---- loads: the Q tiles, then K and V tiles in turn ----------------------
       if (lane == 0 && n > 0) {
@@ -302,72 +296,87 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         for (int x = 0; x < 2; ++x)
           if (n_tiles[x] > 0) mbar_drain(&q_full[x], 0);
       }
-    } else if (warp == kMmaWarp) {
-      // ---- MMA issue -------------------------------------------------------------
+    } else if (warp < kCleanWarp) {
+      // ---- MMA issue: a warp for each row tile, in strict turns -----------------------
+      // A wait that follows MMAs in a warp's queue returns only when they have
+      // been taken up, so with one warp for both tiles the tensor cores ran dry at
+      // every wait.  With two, one waits while the other's MMAs run; the turn is
+      // passed on before a step's last MMAs, to cover its own latency.  Without
+      // turns the tiles fall into step, and first their exponentials compete, then
+      // their products.
       if (n > 0) {
         constexpr uint32_t kIdQK = umma_f16_idesc(kBf16, 0, kRows, kKeys);
         constexpr uint32_t kIdPV = umma_f16_idesc(kBf16, 1, kRows, DP);
+        const int x = warp - kMmaWarp;
+        const int nt = n_tiles[x];
         const uint32_t kv = smem_u32(smem + C::kOffKV);
-        const uint64_t q_desc = umma_sw128_desc(smem_u32(smem + C::kOffQ), 16, 1024);
+        const uint64_t q_desc =
+            umma_sw128_desc(smem_u32(smem + C::kOffQ + x * C::kTileBytes), 16, 1024);
         const uint64_t k_desc = umma_sw128_desc(kv, 16, 1024);
         const uint64_t v_desc = umma_sw128_desc(kv, kKeys * 128, 1024);
+        const uint32_t s_col = tmem + C::kSCol + x * 128, o_col = tmem + C::kOCol + x * 128;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-          if (ok && !mbar_wait_short(bar, parity, err)) {
+          if (ok && !mbar_wait_spin(bar, parity, err)) {
             record_error(err, kDevWaitTimeout);
             ok = false;
           }
-          tmem_fence_after_sync();
         };
-        auto stage_of = [&](int i) { return (uint32_t)(i % C::kStages) * C::kTileBytes; };
         auto wait_load = [&](int i) {
           wait(&kv_full[i % C::kStages], (uint32_t)(i / C::kStages) & 1u);
         };
-        // a stage is released only if a later load reuses it
+        auto stage_of = [&](int i) { return (uint32_t)(i % C::kStages) * C::kTileBytes; };
+        // Both warps release a stage, each after it saw the load, and only if a
+        // later load reuses the stage.
         auto release = [&](int i) {
           if (i + C::kStages < 2 * n) umma_commit_warp(&kv_empty[i % C::kStages]);
         };
-        auto qk = [&](int x, int j) {
+        auto pass_turn = [&]() {
+          if (lane == 0) mbar_arrive(&turn[x ^ 1]);
+          __syncwarp();
+        };
+        auto qk = [&](int j, bool pass) {
           const uint64_t b = umma_desc_at(k_desc, stage_of(2 * j));
-          const uint64_t a = umma_desc_at(q_desc, (uint32_t)x * C::kTileBytes);
 #pragma unroll
           for (int kk = 0; kk < DP / 16; ++kk) {
             const uint32_t off = (uint32_t)(kk / 4) * (kKeys * 128) + (uint32_t)(kk % 4) * 32;
-            umma_f16_warp(tmem + C::kSCol + x * 128, umma_desc_at(a, off), umma_desc_at(b, off), kIdQK,
-                     kk > 0);
+            umma_f16_warp(s_col, umma_desc_at(q_desc, off), umma_desc_at(b, off), kIdQK, kk > 0);
+            if (kk == DP / 16 - kEarly && pass) pass_turn();
           }
           umma_commit_warp(&s_full[x]);
         };
-        auto pv = [&](int x, int j) {
-          const uint64_t b = umma_desc_at(v_desc, stage_of(2 * j + 1));
-#pragma unroll
-          for (int kk = 0; kk < kKeys / 16; ++kk)
-            umma_f16_ta_warp(tmem + C::kOCol + x * 128, tmem + C::kSCol + x * 128 + kk * 8,
-                        umma_desc_at(b, kk * 2048), kIdPV,
-                        (j > 0 || kk > 0) ? 1u : 0u);
-          if (j == n_tiles[x] - 1) umma_commit_warp(&o_full[x]);
-        };
         wait_load(0);
-        for (int x = 0; x < 2; ++x)
-          if (n_tiles[x] > 0) {
-            wait(&q_full[x], 0);
-            if (ok) qk(x, 0);
-          }
+        if (nt > 0) {
+          wait(&q_full[x], 0);
+          tmem_fence_after_sync();
+          if (ok) qk(0, false);
+        }
         release(0);
         for (int j = 0; j < n && ok; ++j) {
           wait_load(2 * j + 1);
-          for (int x = 0; x < 2; ++x) {
-            if (j >= n_tiles[x]) continue;
-            wait(&p_full[x], (uint32_t)j & 1u);
-            if (!ok) break;
-            pv(x, j);
-            if (x == 1 || n_tiles[1] <= j) release(2 * j + 1);
-            if (j + 1 < n_tiles[x]) {
-              wait_load(2 * j + 2);
-              if (!ok) break;
-              qk(x, j + 1);
+          if (j + 1 < n) wait_load(2 * j + 2);
+          if (x == 1 || j > 0) wait(&turn[x], (uint32_t)(x == 1 ? j : j - 1) & 1u);
+          if (j < nt) wait(&p_full[2 * x], (uint32_t)j & 1u);
+          tmem_fence_after_sync();
+          if (!ok) break;
+          if (j < nt) {
+            const uint64_t b = umma_desc_at(v_desc, stage_of(2 * j + 1));
+#pragma unroll
+            for (int kk = 0; kk < kKeys / 16; ++kk) {
+              if (kk == kPart / 16) {
+                wait(&p_full[2 * x + 1], (uint32_t)j & 1u);
+                tmem_fence_after_sync();
+              }
+              umma_f16_ta_warp(o_col, s_col + kk * 8, umma_desc_at(b, kk * 2048), kIdPV,
+                               (j > 0 || kk > 0) ? 1u : 0u);
             }
+            if (j == nt - 1) umma_commit_warp(&o_full[x]);
+            if (j + 1 < nt) qk(j + 1, true);  // over P (j): a warp's MMAs run in order
+            else pass_turn();
+          } else {
+            pass_turn();
           }
+          release(2 * j + 1);
           if (j + 1 < n) release(2 * j + 2);
         }
         umma_commit_warp(mma_done);
@@ -375,7 +384,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       }
     } else {
       // ---- V tiles with masked keys ----------------------------------------------
-      const int t64 = tid - kCleanWarp * 32;
+      const int ct = tid - kCleanWarp * 32;
       bool ok = true;
       for (int j = first_masked; j < n; ++j) {
         const int i = 2 * j + 1;
@@ -386,34 +395,39 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         if (ok) {
           uint8_t* tile = smem + C::kOffKV + (i % C::kStages) * C::kTileBytes;
           const int valid = min(lk - j * kKeys, kKeys);
-          for (int r = t64; r < C::kChunks * kKeys; r += 64) {  // a 128-byte row per thread
+          for (int r = ct; r < C::kChunks * kKeys; r += kCleaners) {  // a 128-byte row each
             const int key = r % kKeys;
             uint4* row = reinterpret_cast<uint4*>(tile + r * 128);
-            bool flagged = false;
-#pragma unroll 4
-            for (int u = 0; u < 8; ++u) {
-              if (key >= valid) {
-                row[u] = make_uint4(0, 0, 0, 0);
-                continue;
-              }
-              uint4 w = row[u];
-              const uint32_t a = nonfinite_mask(w.x, T()), b = nonfinite_mask(w.y, T()),
-                             c = nonfinite_mask(w.z, T()), d = nonfinite_mask(w.w, T());
-              if (a | b | c | d) {
-                row[u] = make_uint4(w.x & ~a, w.y & ~b, w.z & ~c, w.w & ~d);
-                flagged = true;
-              }
+            if (key >= valid) {
+#pragma unroll
+              for (int u = 0; u < 8; ++u) row[u] = make_uint4(0, 0, 0, 0);
+              continue;
             }
-            if (flagged) atomicOr(&s_flags[(j - first_masked) * 4 + key / 32], 1u << (key & 31));
+            uint4 w[8];
+            uint32_t any = 0u;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) w[u] = row[(u + r) & 7];  // lanes on different banks
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+              any |= times_zero(w[u].x, T()) | times_zero(w[u].y, T()) |
+                     times_zero(w[u].z, T()) | times_zero(w[u].w, T());
+            if ((any & 0x7fff7fffu) == 0u) continue;  // every value finite
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+              row[(u + r) & 7] = make_uint4(w[u].x & ~nonfinite_mask(w[u].x, T()),
+                                            w[u].y & ~nonfinite_mask(w[u].y, T()),
+                                            w[u].z & ~nonfinite_mask(w[u].z, T()),
+                                            w[u].w & ~nonfinite_mask(w[u].w, T()));
+            atomicOr(&s_flags[(j - first_masked) * 4 + key / 32], 1u << (key & 31));
           }
           fence_proxy_async_smem();  // an MMA operand
         }
-        named_barrier(1, 64);
-        if (t64 == 0) mbar_arrive(&kv_full[i % C::kStages]);
+        named_barrier(1, kCleaners);
+        if (ct == 0) mbar_arrive(&kv_full[i % C::kStages]);
       }
     }
     } else {
-      registers_up<208>();
+      registers_up<200>();
       // ---- softmax and epilogue: thread = row ---------------------------------------
       const int x = warp >> 2;
       const int row = tid & 127;
@@ -428,7 +442,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       const int nt = n_tiles[x];
       bool ok = true;
       for (int j = 0; j < nt; ++j) {
-        if (ok && !mbar_wait_short(&s_full[x], (uint32_t)j & 1u, err)) {
+        if (ok && !mbar_wait_spin(&s_full[x], (uint32_t)j & 1u, err)) {
           record_error(err, kDevWaitTimeout);
           ok = false;
         }
@@ -447,13 +461,18 @@ __global__ void __launch_bounds__(kPreThreads, 1)
 #pragma unroll
           for (int c = 0; c < kKeys; ++c) s[c] = c < seen ? s[c] : -INFINITY;
         }
-        float tm[4] = {s[0], s[1], s[2], s[3]};
+        float tm[8];
 #pragma unroll
-        for (int c = 4; c < kKeys - 4; c += 8)
+        for (int e = 0; e < 8; ++e) tm[e] = s[e];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) tm[e] = max3_nan(tm[e], s[c + e], s[c + e + 4]);
-        const float t = max3_nan(max3_nan(tm[0], tm[1], max3_nan(tm[2], tm[3], s[kKeys - 4])),
-                                 s[kKeys - 3], max3_nan(s[kKeys - 2], s[kKeys - 1], tm[0]));
+        for (int c = 8; c < kKeys - 8; c += 16)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) tm[e] = max3_nan(tm[e], s[c + e], s[c + e + 8]);
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) tm[e] = max3_nan(tm[e], tm[e + 1], s[kKeys - 8 + e]);
+        const float t = max3_nan(
+            max3_nan(tm[0], tm[2], s[kKeys - 7]), max3_nan(tm[4], tm[6], s[kKeys - 5]),
+            max3_nan(s[kKeys - 3], s[kKeys - 1], tm[0]));
         // move the maximum where it grew by more than 2^kLazy (or from -inf);
         // each row by its own scores, so that its bits do not depend on others
         const bool move =
@@ -478,35 +497,26 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         const float ms = t != t ? t : (m == -INFINITY ? 0.0f : m * p.scale_log2);
         const uint64_t scale2 = f32x2(p.scale_log2, p.scale_log2), ms2 = f32x2(-ms, -ms);
         uint64_t sum[2] = {0, 0};
-        auto exponentials = [&](auto poly) {
 #pragma unroll
-          for (int c = 0; c < kKeys; c += 32) {
-            uint32_t pk[16];
+        for (int c = 0; c < kKeys; c += 32) {
+          uint32_t pk[16];
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const uint64_t y = fma_f32x2(f32x2(s[c + e], s[c + e + 1]), scale2, ms2);
-              float2 v;
-              if (decltype(poly)::value && (e / 2) % kPolyOf < kPolyTake) {
-                v = exp2_poly2(y);
-              } else {
-                v = unpack_f32x2(y);
-                v.x = exp2_approx(v.x);
-                v.y = exp2_approx(v.y);
-              }
-              sum[(e / 2) & 1] = add_f32x2(sum[(e / 2) & 1], f32x2(v.x, v.y));
-              pk[e / 2] = pack2(v.x, v.y, T());
-            }
-            tmem_store<16>(s_addr + c / 2, pk);
+          for (int e = 0; e < 32; e += 2) {
+            float2 v = unpack_f32x2(fma_f32x2(f32x2(s[c + e], s[c + e + 1]), scale2, ms2));
+            v.x = exp2_approx(v.x);
+            v.y = exp2_approx(v.y);
+            sum[(e / 2) & 1] = add_f32x2(sum[(e / 2) & 1], f32x2(v.x, v.y));
+            pk[e / 2] = pack2(v.x, v.y, T());
           }
-        };
-        // the polynomial has no zero for masked scores
-        if (j < first_masked) exponentials(std::true_type());
-        else exponentials(std::false_type());
+          tmem_store<16>(s_addr + c / 2, pk);
+          if (c + 32 == kPart || c + 32 == kKeys) {  // P V can start (and end)
+            tmem_wait_store();
+            tmem_fence_before_sync();
+            mbar_arrive(&p_full[2 * x + (c + 32 == kKeys)]);
+          }
+        }
         const float2 l2 = unpack_f32x2(add_f32x2(sum[0], sum[1]));
         l += l2.x + l2.y;
-        tmem_wait_store();
-        tmem_fence_before_sync();
-        mbar_arrive(&p_full[x]);
       }
       if (nt > 0) {
         if (ok && !mbar_wait_bounded(&o_full[x], 0, err)) record_error(err, kDevWaitTimeout);

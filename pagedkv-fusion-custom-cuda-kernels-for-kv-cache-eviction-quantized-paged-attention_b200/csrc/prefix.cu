@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       const uint64_t v_desc = umma_sw128_desc(kv, kKeys * 128, 1024);
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (ok && !mbar_wait_short(bar, parity, err)) {
+        if (ok && !mbar_wait_spin(bar, parity, err)) {
           record_error(err, kDevWaitTimeout);
           ok = false;
         }
@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     for (int j = 0; j < n; ++j) {
       const int slot = j % C::kSlots;
       if (ok && (!mbar_wait_bounded(&sc_full[slot], (uint32_t)(j / C::kSlots) & 1u, err) ||
-                 !mbar_wait_short(&s_full[x], (uint32_t)j & 1u, err))) {
+                 !mbar_wait_spin(&s_full[x], (uint32_t)j & 1u, err))) {
         record_error(err, kDevWaitTimeout);
         ok = false;
       }
