@@ -39,6 +39,17 @@ int* device_error_word() {
   return ptrs[dev];
 }
 
+void allow_shared_memory(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return;
+  const uint64_t bit = 1ull << dev;
+  if (done.load(std::memory_order_acquire) & bit) return;
+  // on an error the launch fails and reports it
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) ==
+      cudaSuccess)
+    done.fetch_or(bit, std::memory_order_release);
+}
+
 }  // namespace pkv
 
 using pkv::set_error;

@@ -5,6 +5,7 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 #include <string>
@@ -14,6 +15,10 @@ namespace pkv {
 // Per-device error word (abi.cu).  Kernels record the first bad-input or
 // timeout event here instead of trapping.
 int* device_error_word();
+
+// Raises a kernel's dynamic shared memory limit, once per device: `done` is a
+// flag word of that kernel, one bit per device (abi.cu).
+void allow_shared_memory(const void* kernel, int bytes, std::atomic<uint64_t>& done);
 
 // Thread-local message for the last failing call (abi.cu).
 void set_error(const std::string& msg);

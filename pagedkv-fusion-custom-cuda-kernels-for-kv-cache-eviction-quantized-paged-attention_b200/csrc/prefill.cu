@@ -647,7 +647,8 @@ int launch_prefill_t(const PrefillArgs& a, cudaStream_t stream) {
     return kCudaError;
   }
   auto kern = prefill_kernel<T, DP>;
-  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+  static std::atomic<uint64_t> done{0};
+  allow_shared_memory(reinterpret_cast<const void*>(kern), C::kSmemBytes, done);
   // pairs of row tiles: at most this many over all sequences (and the rest)
   const int span = 2 * p.tile_tokens;
   const int64_t pairs = a.total_q / span + std::min<int64_t>(a.num_seqs + 1, a.total_q);

@@ -616,7 +616,8 @@ template <int DP>
 void launch_prefix_t(const PrefixParams& p, cudaStream_t stream) {
   using C = PrefixCfg<DP>;
   auto kern = prefix_kernel<DP>;
-  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+  static std::atomic<uint64_t> done{0};
+  allow_shared_memory(reinterpret_cast<const void*>(kern), C::kSmemBytes, done);
   const int64_t pairs = ((int64_t)p.num_seqs * p.group + 255) / 256;
   const dim3 grid((unsigned)(pairs * p.kv_heads), (unsigned)p.splits);
   kern<<<grid, kPrefixThreads, C::kSmemBytes, stream>>>(p, device_error_word());

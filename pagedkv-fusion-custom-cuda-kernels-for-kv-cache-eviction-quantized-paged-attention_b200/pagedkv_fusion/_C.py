@@ -82,22 +82,9 @@ _wtc_ws = _sig("pkv_write_to_cache_workspace_size", [_I64, _I32], _SZ)
 _wtc = _sig("pkv_write_to_cache",
             [_P, _P, _I32, _P, _P, _P, _I64, _I64, _I32, _I32, _I32, _P, _SZ, _P])
 
-_rope = _sig("pkv_qk_norm_rope",
-             [_P, _P, _I32, _P, _P, _P, _P, _P, _P, _I32, _F, _I64, _I32, _I32, _I32, _I32, _I64,
-              _I32, _I64, _I64, _I64, _I64, _P])
 _append_ws = _sig("pkv_append_kv_workspace_size", [_I64, _I64], _SZ)
-_append = _sig("pkv_append_kv",
-               [_P, _P, _I32, _P, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _I32, _I32, _I64, _I32,
-                _I64, _I64, _I64, _I64, _P, _SZ, _P])
-
-_prefill = _sig("pkv_prefill_attention",
-                [_P, _P, _P, _I32, _P, _P, _P, _P, _I32, _I64, _I64, _I32, _I32, _I32, _I64, _I64,
-                 _I64, _I64, _I64, _I64, _F, _I32, _P])
-
 _prefix_ws = _sig("pkv_shared_prefix_attention_workspace_size",
                   [_I32] * 5 + [_I64, _I32, _I32], _SZ)
-_prefix = _sig("pkv_shared_prefix_attention",
-               [_P] * 10 + [_I32] * 5 + [_I64, _I32, _I32, _F, _P, _SZ, _P])
 
 LIBRARY_PATH = str(_LIB_PATH)
 _DTYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -130,29 +117,39 @@ def _stream(t: torch.Tensor) -> int:
 _SAME_DEVICE = contextlib.nullcontext()
 
 
-def _on_device(t: torch.Tensor):
-    """Makes ``t``'s device the current one where it is not already."""
-    if t.device.index == torch.cuda.current_device():
-        return _SAME_DEVICE
-    return torch.cuda.device(t.device)
+def _on_device(index: int):
+    """Makes device ``index`` the current one where it is not already."""
+    return _SAME_DEVICE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
-def _check_inputs(*tensors):
-    """CUDA tensors of one device, none of which wants a gradient: the
-    operators that call this have no backward pass and must not drop one."""
-    first = tensors[0]
+def _check_inputs(*tensors) -> int:
+    """The device index of CUDA tensors of one device, none of which wants a
+    gradient: the operators that call this have no backward pass and must not
+    drop one.  Entries may be None."""
+    index = -1
     for t in tensors:
         if t is None:
             continue
-        _require(t.is_cuda, "all inputs must be CUDA tensors")
-        _require(t.device == first.device, "all inputs must be on one device")
-        _require(not (t.requires_grad and torch.is_grad_enabled()),
-                 "inputs that require grad: this operator has no backward pass")
+        if not t.is_cuda:
+            raise RuntimeError("all inputs must be CUDA tensors")
+        if index < 0:
+            index = t.get_device()
+        elif t.get_device() != index:
+            raise RuntimeError("all inputs must be on one device")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("inputs that require grad: this operator has no backward pass")
+    return index
 
 
 def _channels_last(t: torch.Tensor) -> torch.Tensor:
     """``t`` itself where its last dimension is contiguous, else a copy."""
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _as_contiguous(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    if t.dtype is not dtype:
+        t = t.to(dtype)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _workspace(nbytes: int, device) -> tuple[torch.Tensor | None, int]:
@@ -504,52 +501,71 @@ def write_to_cache(key, value, kv_cache_int8, scale_cache, slot_mapping, block_s
                 0 if ws is None else ws.numel(), _stream(kc)))
 
 
-def _check_rotary(rotary, positions, num_tokens: int, head_dim: int):
-    _require(rotary.dtype == torch.float32 and rotary.dim() == 2 and rotary.shape[1] % 2 == 0
-             and rotary.shape[1] <= head_dim,
-             "rotary must be a float32 [num_positions, rotary_dim] table, rotary_dim even and at "
-             "most head_dim")
-    _require(positions.dtype in (torch.int64, torch.int32) and positions.dim() == 1
-             and positions.shape[0] == num_tokens, "positions must be int64 or int32 [num_tokens]")
-    return rotary.contiguous(), positions.to(torch.int64).contiguous()
+_INTS = (torch.int64, torch.int32)
+_HALVES = (torch.float16, torch.bfloat16)
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
+
+def _check_rotary(rotary, positions, num_tokens: int, head_dim: int):
+    if not (rotary.dtype is _F32 and rotary.dim() == 2 and rotary.shape[1] % 2 == 0
+            and rotary.shape[1] <= head_dim):
+        raise RuntimeError("rotary must be a float32 [num_positions, rotary_dim] table, rotary_dim "
+                           "even and at most head_dim")
+    if not (positions.dtype in _INTS and positions.dim() == 1
+            and positions.shape[0] == num_tokens):
+        raise RuntimeError("positions must be int64 or int32 [num_tokens]")
+    return _as_contiguous(rotary, _F32), _as_contiguous(positions, torch.int64)
+
+
+# The checks of the operators below are plain attribute tests, and the calls
+# go through the METH_FASTCALL module: a decode step makes them for a few
+# microseconds of GPU work each.
 
 def qk_norm_rope(q, k, positions, rotary, q_weight=None, k_weight=None, eps=1e-6,
                  interleaved=False):
     """Per-head RMS norm (with weights) and rotary position of ``q``
     ``[T, H, D]`` and ``k`` ``[T, Hkv, D]`` (or None) in one launch."""
-    _check_inputs(q, k, positions, rotary, q_weight, k_weight)
-    _require(q.dim() == 3 and q.dtype in _DTYPE_CODE,
-             "q must be [num_tokens, num_heads, head_dim] float32, float16 or bfloat16")
+    dev = _check_inputs(q, k, positions, rotary, q_weight, k_weight)
+    dt = q.dtype
+    if q.dim() != 3 or dt not in _DTYPE_CODE:
+        raise RuntimeError("q must be [num_tokens, num_heads, head_dim] float32, float16 or "
+                           "bfloat16")
     T, H, D = q.shape
-    _require(0 < D <= 256, "head_dim must be 1 to 256")
+    if not 0 < D <= 256:
+        raise RuntimeError("head_dim must be 1 to 256")
     Hkv = 0
     if k is not None:
-        _require(k.dim() == 3 and k.dtype == q.dtype and k.shape[0] == T and k.shape[2] == D,
-                 "k must be [num_tokens, num_kv_heads, head_dim] of q's type")
+        if k.dim() != 3 or k.dtype is not dt or k.shape[0] != T or k.shape[2] != D:
+            raise RuntimeError("k must be [num_tokens, num_kv_heads, head_dim] of q's type")
         Hkv = k.shape[1]
     table, pos = _check_rotary(rotary, positions, T, D)
-    _require((q_weight is None) == (k_weight is None) or k is None,
-             "q_weight and k_weight go together")
+    if (q_weight is None) != (k_weight is None) and k is not None:
+        raise RuntimeError("q_weight and k_weight go together")
     weights = [w for w in (q_weight, k_weight) if w is not None]
-    for w in weights:
-        _require(w.dim() == 1 and w.shape[0] == D and w.dtype in (q.dtype, torch.float32)
-                 and w.dtype == weights[0].dtype,
-                 "weights must be [head_dim], both float32 or of q's type")
-    weights = [w.contiguous() for w in weights]
+    for i, w in enumerate(weights):
+        if not (w.dim() == 1 and w.shape[0] == D and (w.dtype is dt or w.dtype is _F32)
+                and w.dtype is weights[0].dtype):
+            raise RuntimeError("weights must be [head_dim], both float32 or of q's type")
+        weights[i] = w if w.is_contiguous() else w.contiguous()
     qc = _channels_last(q)
-    kc = None if k is None else _channels_last(k)
-    q_out = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
-    k_out = None if k is None else torch.empty((T, Hkv, D), dtype=q.dtype, device=q.device)
-    with _on_device(q):
-        _check(_rope(qc.data_ptr(), kc.data_ptr() if Hkv else None, _DTYPE_CODE[q.dtype],
-                     q_out.data_ptr(), k_out.data_ptr() if Hkv else None, pos.data_ptr(),
-                     table.data_ptr(), weights[0].data_ptr() if weights else None,
-                     weights[-1].data_ptr() if weights else None,
-                     1 if weights and weights[0].dtype == torch.float32 else 0, float(eps), T, H,
-                     Hkv, D, table.shape[1], table.shape[0], 1 if interleaved else 0,
-                     qc.stride(0), qc.stride(1), kc.stride(0) if Hkv else 0,
-                     kc.stride(1) if Hkv else 0, _stream(q)))
+    q_out = torch.empty((T, H, D), dtype=dt, device=q.device)
+    kp = kop = qwp = kwp = None
+    k_out, kt, kh = None, 0, 0
+    if k is not None:
+        k_out = torch.empty((T, Hkv, D), dtype=dt, device=q.device)
+        if Hkv:
+            kc = _channels_last(k)
+            kp, kop, kt, kh = kc.data_ptr(), k_out.data_ptr(), kc.stride(0), kc.stride(1)
+    if weights:
+        qwp, kwp = weights[0].data_ptr(), weights[-1].data_ptr()
+    with _on_device(dev):
+        rc = _fast.qk_norm_rope(
+            qc.data_ptr(), kp, _DTYPE_CODE[dt], q_out.data_ptr(), kop, pos.data_ptr(),
+            table.data_ptr(), qwp, kwp, 1 if weights and weights[0].dtype is _F32 else 0,
+            float(eps), T, H, Hkv, D, table.shape[1], table.shape[0], 1 if interleaved else 0,
+            qc.stride(0), qc.stride(1), kt, kh, _raw_stream(dev))
+    if rc:
+        _check(rc)
     return q_out, k_out
 
 
@@ -557,49 +573,60 @@ def append_kv(key, value, kv_cache_int8, scale_cache, slot_mapping, block_size: 
               positions=None, rotary=None, interleaved=False):
     """Rotate, quantize and append new tokens to the [2, NB, bs, Hkv, D]
     cache in place, keeping the pages' earlier tokens readable."""
-    _check_inputs(key, value, kv_cache_int8, scale_cache, slot_mapping, positions, rotary)
-    _require(key.dim() == 3 and key.dtype in _DTYPE_CODE and value.dtype == key.dtype
-             and value.shape == key.shape,
-             "key/value must be [num_tokens, Hkv, D] of one float32/float16/bfloat16 dtype")
-    _require(kv_cache_int8.dtype == torch.int8 and kv_cache_int8.dim() == 5
-             and kv_cache_int8.shape[0] == 2, "kv_cache_int8 must be int8 [2, NB, bs, Hkv, D]")
-    _require(kv_cache_int8.is_contiguous() and scale_cache.is_contiguous(),
-             "caches must be contiguous (they are written in place)")
+    dev = _check_inputs(key, value, kv_cache_int8, scale_cache, slot_mapping, positions, rotary)
+    dt = key.dtype
+    if key.dim() != 3 or dt not in _DTYPE_CODE or value.dtype is not dt or \
+            value.shape != key.shape:
+        raise RuntimeError("key/value must be [num_tokens, Hkv, D] of one float32/float16/bfloat16 "
+                           "dtype")
+    if kv_cache_int8.dtype is not torch.int8 or kv_cache_int8.dim() != 5 or \
+            kv_cache_int8.shape[0] != 2:
+        raise RuntimeError("kv_cache_int8 must be int8 [2, NB, bs, Hkv, D]")
+    if not (kv_cache_int8.is_contiguous() and scale_cache.is_contiguous()):
+        raise RuntimeError("caches must be contiguous (they are written in place)")
     _, NB, bs, Hkv, D = kv_cache_int8.shape
     T = key.shape[0]
-    _require(int(block_size) == bs, "block_size must match the cache")
-    _require(0 < bs <= 64, "supports block_size <= 64")
-    _require(0 < D <= 256, "head_dim must be 1 to 256")
-    _require(tuple(key.shape[1:]) == (Hkv, D), "key/value must be [num_tokens, Hkv, D]")
-    _require(scale_cache.dtype == torch.float32 and tuple(scale_cache.shape) == (2, NB, Hkv),
-             "scale_cache must be float32 [2, NB, Hkv]")
-    _require(slot_mapping.dtype in (torch.int64, torch.int32) and slot_mapping.dim() == 1
-             and slot_mapping.shape[0] == T, "slot_mapping must be int64 or int32 [num_tokens]")
-    _require((positions is None) == (rotary is None), "positions and rotary go together")
-    pos = table = None
+    if int(block_size) != bs:
+        raise RuntimeError("block_size must match the cache")
+    if not 0 < bs <= 64:
+        raise RuntimeError("supports block_size <= 64")
+    if not 0 < D <= 256:
+        raise RuntimeError("head_dim must be 1 to 256")
+    if key.shape[1] != Hkv or key.shape[2] != D:
+        raise RuntimeError("key/value must be [num_tokens, Hkv, D]")
+    if scale_cache.dtype is not _F32 or tuple(scale_cache.shape) != (2, NB, Hkv):
+        raise RuntimeError("scale_cache must be float32 [2, NB, Hkv]")
+    if not (slot_mapping.dtype in _INTS and slot_mapping.dim() == 1
+            and slot_mapping.shape[0] == T):
+        raise RuntimeError("slot_mapping must be int64 or int32 [num_tokens]")
+    if (positions is None) != (rotary is None):
+        raise RuntimeError("positions and rotary go together")
+    pp = tp = None
+    rot = rows = 0
     if rotary is not None:
         table, pos = _check_rotary(rotary, positions, T, D)
-        if table.shape[1] == 0:  # nothing to rotate
-            table = pos = None
+        rows, rot = table.shape
+        if rot:  # else nothing to rotate
+            pp, tp = pos.data_ptr(), table.data_ptr()
     kc, vc = _channels_last(key), _channels_last(value)
-    slots = slot_mapping.to(torch.int64).contiguous()
-    with _on_device(key):
-        ws, wp = _workspace(_append_ws(T, NB), key.device)
-        _check(_append(kc.data_ptr(), vc.data_ptr(), _DTYPE_CODE[key.dtype],
-                       kv_cache_int8.data_ptr(), scale_cache.data_ptr(), slots.data_ptr(),
-                       None if pos is None else pos.data_ptr(),
-                       None if table is None else table.data_ptr(), T, NB, bs, Hkv, D,
-                       0 if table is None else table.shape[1],
-                       0 if table is None else table.shape[0], 1 if interleaved else 0,
-                       kc.stride(0), kc.stride(1), vc.stride(0), vc.stride(1), wp,
-                       0 if ws is None else ws.numel(), _stream(key)))
+    slots = _as_contiguous(slot_mapping, torch.int64)
+    with _on_device(dev):
+        nbytes = _append_ws(T, NB)
+        ws, wp = _workspace(nbytes, key.device)
+        rc = _fast.append_kv(kc.data_ptr(), vc.data_ptr(), _DTYPE_CODE[dt],
+                             kv_cache_int8.data_ptr(), scale_cache.data_ptr(), slots.data_ptr(),
+                             pp, tp, T, NB, bs, Hkv, D, rot, rows, 1 if interleaved else 0,
+                             kc.stride(0), kc.stride(1), vc.stride(0), vc.stride(1), wp, nbytes,
+                             _raw_stream(dev))
+    if rc:
+        _check(rc)
 
 
 def _tma_rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` ``[tokens, heads, D]`` itself where tiles can be copied from it
     (contiguous channels, strides of 16 bytes, 16-byte aligned), else a copy."""
-    if t.numel() == 0 or (t.stride(2) == 1 and t.stride(0) > 0 and t.stride(1) > 0
-                          and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0
+    a, b, c = t.stride()
+    if t.numel() == 0 or (c == 1 and a > 0 and b > 0 and a % 8 == 0 and b % 8 == 0
                           and t.data_ptr() % 16 == 0):
         return t
     return t.clone(memory_format=torch.contiguous_format)
@@ -609,71 +636,83 @@ def prefill_attention(q, k, v, cu_seqlens, sm_scale, cu_seqlens_k=None, causal=T
                       return_lse=False):
     """Attention over packed prompts, ``[total_q, H, D]`` (and, with
     ``return_lse``, the float32 ``[total_q, H]`` log denominators)."""
-    _check_inputs(q, k, v, cu_seqlens, cu_seqlens_k)
-    _require(q.dim() == 3 and q.dtype in (torch.float16, torch.bfloat16),
-             "q must be [total_q, num_heads, head_dim] float16 or bfloat16")
+    dev = _check_inputs(q, k, v, cu_seqlens, cu_seqlens_k)
+    dt = q.dtype
+    if q.dim() != 3 or dt not in _HALVES:
+        raise RuntimeError("q must be [total_q, num_heads, head_dim] float16 or bfloat16")
     Tq, H, D = q.shape
-    _require(k.dim() == 3 and k.dtype == q.dtype and k.shape[2] == D and v.dtype == q.dtype
-             and v.shape == k.shape, "k and v must be [total_k, num_kv_heads, head_dim] of q's type")
-    Tk, Hkv, _ = k.shape
+    if k.dim() != 3 or k.dtype is not dt or k.shape[2] != D or v.dtype is not dt or \
+            v.shape != k.shape:
+        raise RuntimeError("k and v must be [total_k, num_kv_heads, head_dim] of q's type")
+    Tk, Hkv = k.shape[0], k.shape[1]
     cq = cu_seqlens
     ck = cu_seqlens if cu_seqlens_k is None else cu_seqlens_k
+    n = cq.shape[0] if cq.dim() == 1 else 0
     for c in (cq, ck):
-        _require(c.dtype == torch.int32 and c.dim() == 1 and c.shape[0] == cq.shape[0]
-                 and c.shape[0] > 0, "cu_seqlens must be int32 [num_seqs + 1]")
+        if c.dtype is not torch.int32 or c.dim() != 1 or c.shape[0] != n or n == 0:
+            raise RuntimeError("cu_seqlens must be int32 [num_seqs + 1]")
     cq, ck = cq.contiguous(), ck.contiguous()
     qc, kc, vc = _tma_rows(q), _tma_rows(k), _tma_rows(v)
-    out = torch.empty((Tq, H, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((Tq, H), dtype=torch.float32, device=q.device) if return_lse else None
-    with _on_device(q):
-        _check(_prefill(qc.data_ptr(), kc.data_ptr(), vc.data_ptr(), _DTYPE_CODE[q.dtype],
-                        out.data_ptr(), None if lse is None else lse.data_ptr(), cq.data_ptr(),
-                        ck.data_ptr(), cq.shape[0] - 1, Tq, Tk, H, Hkv, D, qc.stride(0),
-                        qc.stride(1), kc.stride(0), kc.stride(1), vc.stride(0), vc.stride(1),
-                        float(sm_scale), 1 if causal else 0, _stream(q)))
+    out = torch.empty((Tq, H, D), dtype=dt, device=q.device)
+    lse = torch.empty((Tq, H), dtype=_F32, device=q.device) if return_lse else None
+    with _on_device(dev):
+        rc = _fast.prefill_attention(
+            qc.data_ptr(), kc.data_ptr(), vc.data_ptr(), _DTYPE_CODE[dt], out.data_ptr(),
+            None if lse is None else lse.data_ptr(), cq.data_ptr(), ck.data_ptr(), n - 1, Tq, Tk,
+            H, Hkv, D, qc.stride(0), qc.stride(1), kc.stride(0), kc.stride(1), vc.stride(0),
+            vc.stride(1), float(sm_scale), 1 if causal else 0, _raw_stream(dev))
+    if rc:
+        _check(rc)
     return (out, lse) if return_lse else out
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     """``t`` contiguous and 16-byte aligned: itself where it is, else a copy."""
-    t = t.contiguous()
+    t = t if t.is_contiguous() else t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def shared_prefix_attention(q, k_cache_q, k_scale, v_cache_q, v_scale, prefix_table, prefix_len,
                             block_tables, seq_lens, sm_scale):
     """INT8 paged decode attention over [shared prefix | own tokens]."""
-    _check_inputs(q, k_cache_q, k_scale, v_cache_q, v_scale, prefix_table, prefix_len,
-                  block_tables, seq_lens)
-    _require(q.dtype == torch.float32, "q must be float32 (v1)")
-    _require(k_cache_q.dtype == torch.int8 and v_cache_q.dtype == torch.int8,
-             "k_cache_q and v_cache_q must be int8")
-    _require(k_scale.dtype == torch.float32 and v_scale.dtype == torch.float32,
-             "k_scale/v_scale must be float32")
-    _require(block_tables.dtype == torch.int32 and prefix_table.dtype == torch.int32,
-             "block_tables and prefix_table must be int32")
-    _require(q.dim() == 3 and k_cache_q.dim() == 4 and block_tables.dim() == 2
-             and prefix_table.dim() == 1,
-             "expected q [S, H, D], caches [NB, bs, Hkv, D], prefix_table [P], block_tables [S, M]")
+    dev = _check_inputs(q, k_cache_q, k_scale, v_cache_q, v_scale, prefix_table, prefix_len,
+                        block_tables, seq_lens)
+    if q.dtype is not _F32:
+        raise RuntimeError("q must be float32 (v1)")
+    if k_cache_q.dtype is not torch.int8 or v_cache_q.dtype is not torch.int8:
+        raise RuntimeError("k_cache_q and v_cache_q must be int8")
+    if k_scale.dtype is not _F32 or v_scale.dtype is not _F32:
+        raise RuntimeError("k_scale/v_scale must be float32")
+    if block_tables.dtype is not torch.int32 or prefix_table.dtype is not torch.int32:
+        raise RuntimeError("block_tables and prefix_table must be int32")
+    if q.dim() != 3 or k_cache_q.dim() != 4 or block_tables.dim() != 2 or prefix_table.dim() != 1:
+        raise RuntimeError("expected q [S, H, D], caches [NB, bs, Hkv, D], prefix_table [P], "
+                           "block_tables [S, M]")
     S, H, D = q.shape
     NB, bs, Hkv, Dk = k_cache_q.shape
-    _require(Dk == D and v_cache_q.shape == k_cache_q.shape, "cache head_dim must match q")
-    _require(tuple(k_scale.shape) == (NB, Hkv) and tuple(v_scale.shape) == (NB, Hkv),
-             "scales must be [num_blocks, num_kv_heads]")
-    _require(block_tables.shape[0] == S and seq_lens.numel() == S,
-             "block_tables/seq_lens must have num_seqs rows")
-    _require(prefix_len.numel() == 1 and prefix_len.dtype in (torch.int32, torch.int64),
-             "prefix_len must hold one integer")
-    _require(seq_lens.dtype in (torch.int32, torch.int64), "seq_lens must be int32 or int64")
+    if Dk != D or v_cache_q.shape != k_cache_q.shape:
+        raise RuntimeError("cache head_dim must match q")
+    if tuple(k_scale.shape) != (NB, Hkv) or tuple(v_scale.shape) != (NB, Hkv):
+        raise RuntimeError("scales must be [num_blocks, num_kv_heads]")
+    if block_tables.shape[0] != S or seq_lens.numel() != S:
+        raise RuntimeError("block_tables/seq_lens must have num_seqs rows")
+    if prefix_len.numel() != 1 or prefix_len.dtype not in _INTS:
+        raise RuntimeError("prefix_len must hold one integer")
+    if seq_lens.dtype not in _INTS:
+        raise RuntimeError("seq_lens must be int32 or int64")
     qc, kc, vc = _aligned(q), _aligned(k_cache_q), _aligned(v_cache_q)
-    ks, vs, bt, pt = (t.contiguous() for t in (k_scale, v_scale, block_tables, prefix_table))
-    sl, pl = seq_lens.to(torch.int32).contiguous(), prefix_len.to(torch.int32)
-    out = torch.empty((S, H, D), dtype=torch.float32, device=q.device)
+    ks, vs = _as_contiguous(k_scale, _F32), _as_contiguous(v_scale, _F32)
+    bt, pt = _as_contiguous(block_tables, torch.int32), _as_contiguous(prefix_table, torch.int32)
+    sl, pl = _as_contiguous(seq_lens, torch.int32), _as_contiguous(prefix_len, torch.int32)
+    out = torch.empty((S, H, D), dtype=_F32, device=q.device)
     P, M = pt.shape[0], bt.shape[1]
-    with _on_device(q):
-        ws, wp = _workspace(_prefix_ws(S, H, Hkv, D, bs, NB, P, M), q.device)
-        _check(_prefix(qc.data_ptr(), kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(),
-                       pt.data_ptr(), pl.data_ptr(), bt.data_ptr(), sl.data_ptr(), out.data_ptr(),
-                       S, H, Hkv, D, bs, NB, P, M, float(sm_scale), wp,
-                       0 if ws is None else ws.numel(), _stream(q)))
+    with _on_device(dev):
+        nbytes = _prefix_ws(S, H, Hkv, D, bs, NB, P, M)
+        ws, wp = _workspace(nbytes, q.device)
+        rc = _fast.shared_prefix_attention(
+            qc.data_ptr(), kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(),
+            pt.data_ptr(), pl.data_ptr(), bt.data_ptr(), sl.data_ptr(), out.data_ptr(), S, H, Hkv,
+            D, bs, NB, P, M, float(sm_scale), wp, nbytes, _raw_stream(dev))
+    if rc:
+        _check(rc)
     return out
