@@ -370,15 +370,16 @@ int launch_qk_t(const QkNormRopeArgs& p, cudaStream_t stream) {
 // append_kv
 // ---------------------------------------------------------------------------
 //
-// A work unit is (page touched by the call, K or V): the call's tokens in
-// that page set its scale together.  Up to kAppendScan tokens every CTA finds
-// its page's tokens by scanning the slots itself (one launch); above that, an
-// index kernel first chains the runs of consecutive tokens per page.
+// A work unit is a page touched by the call (its K or V half in small calls):
+// the call's tokens in that page set its scale together.  Up to kAppendScan
+// tokens every CTA finds its page's tokens by scanning the slots itself (one
+// launch); above that, an index kernel first chains the runs of consecutive
+// tokens per page.
 
 constexpr int kAppendThreads = 256;
 constexpr int kAppendWarps = kAppendThreads / 32;
 constexpr int kAppendMaxPage = 64;  // largest block_size
-constexpr int kAppendHold = 16;     // tokens of a head kept in registers
+constexpr int kAppendHold = 16;     // tokens of a head kept on chip
 
 template <typename T>
 struct AppendArgs {
@@ -415,20 +416,18 @@ __device__ __forceinline__ int64_t append_slot(const AppendArgs<T>& a, int64_t t
   return slot;
 }
 
-// Chunk c (VEC channels) of token t's head h, rotated when it is a key.
-template <typename T, int VEC, int NC>
-__device__ __forceinline__ void append_load(const AppendArgs<T>& a, bool is_key, int64_t t, int h,
-                                            int c, bool on, float (&y)[VEC]) {
-  const T* src = is_key ? a.key + t * a.k_tok + (int64_t)h * a.k_head
-                        : a.value + t * a.v_tok + (int64_t)h * a.v_head;
-  Chunk<T, VEC> x;
-  if (on) x = load_chunk<T, VEC>(src + c * VEC);
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) y[e] = on ? to_f32<T>(x.e[e]) : 0.0f;
-  if (!is_key || a.positions == nullptr) return;  // uniform for the CTA
+enum Rotation { kNoRotation = 0, kHalves = 1, kPairs = 2 };
+
+// Rotates chunk c (VEC channels, raw words x) of one head in place of y.  The
+// partner chunk of the half layout is another lane's when a head fits one
+// chunk per lane (NC = 1), else it is read from `src` again.  Every lane of
+// the warp calls.
+template <typename T, int VEC, int NC, int ROT>
+__device__ __forceinline__ void append_rotate(const AppendArgs<T>& a, const float* row,
+                                              const T* src, const Chunk<T, VEC>& x, int c, bool on,
+                                              float (&y)[VEC]) {
   const int half = a.rot / 2, d = c * VEC;
-  const float* row = a.table + a.positions[t] * a.rot;
-  if (a.interleaved && VEC > 1) {
+  if constexpr (ROT == kPairs && VEC > 1) {
 #pragma unroll
     for (int e = 0; e + 1 < VEC; e += 2) {
       if (on && d + e < a.rot) {
@@ -438,49 +437,51 @@ __device__ __forceinline__ void append_load(const AppendArgs<T>& a, bool is_key,
         y[e + 1] = rot_second(p, q, cc, ss);
       }
     }
-    return;
-  }
-  const bool first = a.interleaved ? (d & 1) == 0 : d < half;
-  Chunk<T, VEC> o;
-  if (VEC > 1 && NC == 1) {  // the partner chunk is another lane's
-    constexpr int W = VEC * sizeof(T) / 4 > 0 ? VEC * sizeof(T) / 4 : 1;
-    const int pc = first ? c + half / VEC : c - half / VEC;
-    const uint32_t* v32 = reinterpret_cast<const uint32_t*>(x.e);
-    uint32_t* o32 = reinterpret_cast<uint32_t*>(o.e);
-#pragma unroll
-    for (int u = 0; u < W; ++u) o32[u] = __shfl_sync(0xffffffffu, v32[u], pc & 31);
-  } else if (on && d < a.rot) {
-    const int pd = a.interleaved ? d ^ 1 : (first ? d + half : d - half);
-    o = load_chunk<T, VEC>(src + pd);
-  }
-  if (!on || d >= a.rot) return;
-  const int i = a.interleaved ? d / 2 : (first ? d : d - half);
-  alignas(16) float cc[VEC], ss[VEC];
-  if constexpr (VEC == 4) {
-    *reinterpret_cast<float4*>(cc) = *reinterpret_cast<const float4*>(row + i);
-    *reinterpret_cast<float4*>(ss) = *reinterpret_cast<const float4*>(row + half + i);
   } else {
-    cc[0] = row[i];
-    ss[0] = row[half + i];
-  }
+    const bool first = ROT == kPairs ? (d & 1) == 0 : d < half;
+    Chunk<T, VEC> o;
+    if constexpr (VEC > 1 && NC == 1) {
+      constexpr int W = VEC * sizeof(T) / 4;
+      const int pc = first ? c + half / VEC : c - half / VEC;
+      const uint32_t* v32 = reinterpret_cast<const uint32_t*>(x.e);
+      uint32_t* o32 = reinterpret_cast<uint32_t*>(o.e);
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    const float p = to_f32<T>(o.e[e]);
-    y[e] = first ? rot_first(y[e], p, cc[e], ss[e]) : rot_second(p, y[e], cc[e], ss[e]);
+      for (int u = 0; u < W; ++u) o32[u] = __shfl_sync(0xffffffffu, v32[u], pc & 31);
+    } else if (on && d < a.rot) {
+      o = load_chunk<T, VEC>(src + (ROT == kPairs ? d ^ 1 : (first ? d + half : d - half)));
+    }
+    if (on && d < a.rot) {
+      const int i = ROT == kPairs ? d / 2 : (first ? d : d - half);
+      alignas(16) float cc[VEC], ss[VEC];
+      if constexpr (VEC == 4) {
+        *reinterpret_cast<float4*>(cc) = *reinterpret_cast<const float4*>(row + i);
+        *reinterpret_cast<float4*>(ss) = *reinterpret_cast<const float4*>(row + half + i);
+      } else {
+        cc[0] = row[i];
+        ss[0] = row[half + i];
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float p = to_f32<T>(o.e[e]);
+        y[e] = first ? rot_first(y[e], p, cc[e], ss[e]) : rot_second(p, y[e], cc[e], ss[e]);
+      }
+    }
   }
 }
 
-// One page, K or V.  s_tok[offset] is the call's token for that offset or -1.
-// A warp owns a head: absmax of the new values, the page's scale, the earlier
-// codes moved to a larger scale, the new codes.  Up to kAppendHold tokens of
-// up to 128 channels stay in registers between the two steps (one read of the
-// inputs); more are read again (from L2).
-template <typename T, int VEC, int NC>
-__device__ void append_page(const AppendArgs<T>& a, int64_t page, bool is_key, const int* s_tok,
-                            int* s_list) {
-  __shared__ int s_meta[2];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (warp == 0) {  // compact list of (offset, token), ascending offsets
+// The call's tokens in one page, in ascending offsets.
+struct AppendList {
+  int off[kAppendMaxPage];
+  int tok[kAppendMaxPage];
+  int64_t pos[kAppendMaxPage];
+  int count, lowest;
+};
+
+// Compacts s_tok (a page's token per offset, or -1) into the list; whole CTA.
+template <typename T>
+__device__ void append_list(const AppendArgs<T>& a, const int* s_tok, AppendList& list) {
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
     int n = 0, lowest = a.bs;
     for (int b = 0; b < a.bs; b += 32) {
       const int off = b + lane;
@@ -488,106 +489,263 @@ __device__ void append_page(const AppendArgs<T>& a, int64_t page, bool is_key, c
       const unsigned m = __ballot_sync(0xffffffffu, t >= 0);
       if (t >= 0) {
         const int at = n + __popc(m & ((1u << lane) - 1u));
-        s_list[2 * at] = off;
-        s_list[2 * at + 1] = t;
+        list.off[at] = off;
+        list.tok[at] = t;
+        list.pos[at] = a.positions != nullptr ? a.positions[t] : 0;
       }
       if (m != 0 && lowest == a.bs) lowest = b + __ffs(m) - 1;
       n += __popc(m);
     }
     if (lane == 0) {
-      s_meta[0] = n;
-      s_meta[1] = lowest;
+      list.count = n;
+      list.lowest = lowest;
     }
   }
   __syncthreads();
-  const int n = s_meta[0], lowest = s_meta[1];
-  const int chunks = a.dim / VEC;
-  const int64_t tok_stride = (int64_t)a.kv_heads * a.dim;
-  int8_t* page_base = a.cache + (is_key ? 0 : a.blocks * a.bs * tok_stride) +
-                      page * a.bs * tok_stride;
-  float* scale_base = a.scales + (is_key ? 0 : a.blocks * a.kv_heads) + page * a.kv_heads;
-  constexpr bool kHold = NC == 1 && VEC == 4;
-  for (int h = warp; h < a.kv_heads; h += kAppendWarps) {
-    float held[kHold ? kAppendHold : 1][VEC];
-    uint32_t m = 0u;
-    auto fold = [&](const float (&y)[VEC]) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) m = max(m, __float_as_uint(y[e]) & 0x7fffffffu);
+}
+
+// The page's scale from the new values' absmax; the earlier codes, `row_bytes`
+// of them per offset below `lowest`, moved to it where it grew.
+__device__ __forceinline__ float append_scale(float amax, float* scale, float old, int lowest,
+                                              int8_t* head_base, int64_t tok_stride, int dim,
+                                              bool words) {
+  const int lane = threadIdx.x & 31;
+  const float step = amax > 0.0f ? __fdiv_rn(amax, 127.0f) : 0.0f;
+  const bool grow = step > old;
+  const float sc = lowest == 0 ? (step > 0.0f ? step : 1.0f) : (grow ? step : old);
+  __syncwarp();  // every lane has the old scale
+  if (lane == 0) *scale = sc;
+  if (lowest > 0 && grow) {
+    const float ratio = __fdiv_rn(old, sc);
+    auto move = [&](int8_t code) {
+      return (uint32_t)(__float2int_rn(__fmul_rn((float)code, ratio)) & 255);
     };
-    const bool hold = kHold && n <= kAppendHold;
-    if (hold) {
-#pragma unroll
-      for (int i = 0; i < (kHold ? kAppendHold : 1); ++i)
-        if (i < n) {
-          append_load<T, VEC, NC>(a, is_key, s_list[2 * i + 1], h, lane, lane < chunks, held[i]);
-          fold(held[i]);
-        }
-    } else {
-      for (int i = 0; i < n; ++i)
-#pragma unroll
-        for (int j = 0; j < NC; ++j) {
-          float y[VEC];
-          append_load<T, VEC, NC>(a, is_key, s_list[2 * i + 1], h, lane + 32 * j,
-                                  lane + 32 * j < chunks, y);
-          fold(y);
-        }
-    }
-    m = __reduce_max_sync(0xffffffffu, m);  // NaN bits exceed +inf: NaN wins
-    const float amax = __uint_as_float(m);
-    const float step = amax > 0.0f ? __fdiv_rn(amax, 127.0f) : 0.0f;
-    float old = 0.0f;
-    if (lowest > 0) old = scale_base[h];
-    const bool grow = step > old;
-    const float sc = lowest == 0 ? (step > 0.0f ? step : 1.0f) : (grow ? step : old);
-    __syncwarp();  // every lane has the old scale
-    if (lane == 0) scale_base[h] = sc;
-    if (lowest > 0 && grow) {
-      const float ratio = __fdiv_rn(old, sc);
-      for (int off = 0; off < lowest; ++off) {
-        int8_t* row = page_base + off * tok_stride + (int64_t)h * a.dim;
-#pragma unroll
-        for (int j = 0; j < NC; ++j) {
-          const int c = lane + 32 * j;
-          if (c < chunks) {
-            if constexpr (VEC == 4) {
-              const uint32_t w = *reinterpret_cast<const uint32_t*>(row + 4 * c);
-              uint32_t r = 0u;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float v = (float)(int8_t)(w >> (8 * e));
-                r |= (uint32_t)(__float2int_rn(__fmul_rn(v, ratio)) & 255) << (8 * e);
-              }
-              *reinterpret_cast<uint32_t*>(row + 4 * c) = r;
-            } else {
-              row[c] = (int8_t)__float2int_rn(__fmul_rn((float)row[c], ratio));
-            }
-          }
-        }
+    if (words) {
+      // lane = (offset, word): short rows keep the warp busy
+      const int per_row = dim / 4;
+#pragma unroll 4
+      for (int i = lane; i < lowest * per_row; i += 32) {
+        uint32_t* p = reinterpret_cast<uint32_t*>(head_base + (i / per_row) * tok_stride) + i % per_row;
+        const uint32_t w = *p;
+        *p = move((int8_t)w) | move((int8_t)(w >> 8)) << 8 | move((int8_t)(w >> 16)) << 16 |
+             move((int8_t)(w >> 24)) << 24;
       }
+    } else {
+      for (int off = 0; off < lowest; ++off)
+        for (int d = lane; d < dim; d += 32) {
+          int8_t* p = head_base + off * tok_stride + d;
+          *p = (int8_t)move(*p);
+        }
     }
-    const float rcp = __frcp_rn(sc);
-    const bool fast = isfinite(amax) && !isinf(rcp);
-    auto store = [&](int off, int c, const float (&y)[VEC]) {
-      int8_t* dst = page_base + off * tok_stride + (int64_t)h * a.dim + c * VEC;
+  }
+  return sc;
+}
+
+// One head of one page, K or V, by one warp, any shape: absmax of the new
+// values, the page's scale, the earlier codes moved, the new codes.  Inputs
+// are read twice.
+template <typename T, int VEC, int NC, int ROT>
+__device__ __noinline__ void append_head(const AppendArgs<T>& a, int64_t page, bool is_key,
+                                            int h, const AppendList& list) {
+  const int lane = threadIdx.x & 31;
+  const int n = list.count, lowest = list.lowest, chunks = a.dim / VEC;
+  const int64_t tok_stride = (int64_t)a.kv_heads * a.dim;
+  int8_t* head_base = a.cache + (is_key ? 0 : a.blocks * a.bs * tok_stride) +
+                      page * a.bs * tok_stride + (int64_t)h * a.dim;
+  float* scale = a.scales + (is_key ? 0 : a.blocks * a.kv_heads) + page * a.kv_heads + h;
+  const T* base = is_key ? a.key + (int64_t)h * a.k_head : a.value + (int64_t)h * a.v_head;
+  const int64_t step_tok = is_key ? a.k_tok : a.v_tok;
+  const float old = lowest > 0 ? *scale : 0.0f;
+
+  uint32_t m = 0u;
+  auto fold = [&](const float (&y)[VEC]) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) m = max(m, __float_as_uint(y[e]) & 0x7fffffffu);
+  };
+  auto load = [&](int i, int c, float (&y)[VEC]) {
+    const T* src = base + list.tok[i] * step_tok;
+    Chunk<T, VEC> x;
+    if (c < chunks) x = load_chunk<T, VEC>(src + c * VEC);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) y[e] = c < chunks ? to_f32<T>(x.e[e]) : 0.0f;
+    if constexpr (ROT != kNoRotation)
+      append_rotate<T, VEC, NC, ROT>(a, a.table + list.pos[i] * a.rot, src, x, c, c < chunks, y);
+  };
+  for (int i = 0; i < n; ++i)
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      float y[VEC];
+      load(i, lane + 32 * j, y);
+      fold(y);
+    }
+  m = __reduce_max_sync(0xffffffffu, m);  // NaN bits exceed +inf: NaN wins
+  const float amax = __uint_as_float(m);
+  const float sc = append_scale(amax, scale, old, lowest, head_base, tok_stride, a.dim, VEC == 4);
+  const float rcp = __frcp_rn(sc);
+  const bool fast = isfinite(amax) && !isinf(rcp);
+  for (int i = 0; i < n; ++i)
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const int c = lane + 32 * j;
+      float y[VEC];
+      load(i, c, y);
+      if (c >= chunks) continue;
+      int8_t* dst = head_base + list.off[i] * tok_stride + c * VEC;
       if constexpr (VEC == 4)
         *reinterpret_cast<uint32_t*>(dst) = quantize_word(y, sc, rcp, fast);
       else
         *dst = (int8_t)quantize_one(y[0], sc);
-    };
-    if (hold) {
+    }
+}
+
+// The same for up to kAppendHold tokens of up to 128 channels in 8-channel
+// pieces, half a warp per token (a warp's instruction serves two tokens).  All
+// rows of a head are copied to shared memory at once, so inputs are read once
+// and a warp has 4 KB in flight; the rotation is cheap enough to be done
+// again for the codes.  (Rows held in registers: one pair of tokens ahead left
+// each step waiting for HBM, all sixteen tokens spilled; 158 to 420 us for
+// 32,768 tokens of 8 heads against 108 us.)
+__device__ __forceinline__ void copy16_async(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+}
+
+// Starts the copies of one head's rows; copies_wait() before append_head8.
+template <typename T>
+__device__ __forceinline__ void append_fetch8(const AppendArgs<T>& a, bool is_key, int h,
+                                              const AppendList& list, T* raw) {
+  constexpr int kPer = 16 / sizeof(T);  // values of a 16-byte access
+  const int lane = threadIdx.x & 31, d = (lane & 15) * 8;
+  const T* base = (is_key ? a.key + (int64_t)h * a.k_head : a.value + (int64_t)h * a.v_head) + d;
+  const int64_t step_tok = is_key ? a.k_tok : a.v_tok;
+  if (d < a.dim)
+    for (int i = lane >> 4; i < list.count; i += 2)
 #pragma unroll
-      for (int i = 0; i < (kHold ? kAppendHold : 1); ++i)
-        if (i < n && lane < chunks) store(s_list[2 * i], lane, held[i]);
+      for (int u = 0; u < 8 / kPer; ++u)
+        copy16_async(raw + i * 128 + d + u * kPer, base + list.tok[i] * step_tok + u * kPer);
+}
+
+template <typename T, int ROT>
+__device__ __forceinline__ void append_head8(const AppendArgs<T>& a, int64_t page, bool is_key,
+                                             int h, const AppendList& list, const T* raw,
+                                             const float* table) {
+  constexpr int kPer = 16 / sizeof(T);
+  const int lane = threadIdx.x & 31, sub = lane >> 4, d = (lane & 15) * 8;
+  const int n = list.count, lowest = list.lowest;
+  const bool on = d < a.dim;
+  const int64_t tok_stride = (int64_t)a.kv_heads * a.dim;
+  int8_t* head_base = a.cache + (is_key ? 0 : a.blocks * a.bs * tok_stride) +
+                      page * a.bs * tok_stride + (int64_t)h * a.dim;
+  float* scale = a.scales + (is_key ? 0 : a.blocks * a.kv_heads) + page * a.kv_heads + h;
+  const float old = lowest > 0 ? *scale : 0.0f;
+
+  const int half = a.rot / 2;
+  const bool first = d < half;
+  const int col = ROT == kPairs ? d / 2 : (first ? d : d - half);  // of the table row
+  auto values = [&](int i, float (&y)[8]) {
+#pragma unroll
+    for (int u = 0; u < 8 / kPer; ++u) {
+      const Chunk<T, kPer> x = load_chunk<T, kPer>(raw + i * 128 + d + u * kPer);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) y[u * kPer + e] = to_f32<T>(x.e[e]);
+    }
+    if (ROT == kNoRotation || d >= a.rot) return;  // whole pieces: rot % 16 = 0, or pairs
+    const float* row = table + i * 128 + col;
+    if constexpr (ROT == kHalves) {
+      const T* other = raw + i * 128 + (first ? d + half : d - half);
+#pragma unroll
+      for (int u = 0; u < 8; u += 4) {
+        alignas(16) float cc[4], ss[4];
+        *reinterpret_cast<float4*>(cc) = *reinterpret_cast<const float4*>(row + u);
+        *reinterpret_cast<float4*>(ss) = *reinterpret_cast<const float4*>(row + half + u);
+        const Chunk<T, 4> o = load_chunk<T, 4>(other + u);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p = to_f32<T>(o.e[e]);
+          y[u + e] = first ? rot_first(y[u + e], p, cc[e], ss[e])
+                           : rot_second(p, y[u + e], cc[e], ss[e]);
+        }
+      }
     } else {
-      for (int i = 0; i < n; ++i)
 #pragma unroll
-        for (int j = 0; j < NC; ++j) {
-          const int c = lane + 32 * j;
-          float y[VEC];
-          append_load<T, VEC, NC>(a, is_key, s_list[2 * i + 1], h, c, c < chunks, y);
-          if (c < chunks) store(s_list[2 * i], c, y);
+      for (int e = 0; e < 8; e += 2)
+        if (d + e < a.rot) {
+          const float p = y[e], q = y[e + 1];
+          y[e] = rot_first(p, q, row[e / 2], row[half + e / 2]);
+          y[e + 1] = rot_second(p, q, row[e / 2], row[half + e / 2]);
         }
     }
+  };
+  uint32_t m = 0u;
+  if (on)
+#pragma unroll 2
+    for (int i = sub; i < n; i += 2) {
+      float y[8];
+      values(i, y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(y[e]) & 0x7fffffffu);
+    }
+  m = __reduce_max_sync(0xffffffffu, m);  // NaN bits exceed +inf: NaN wins
+  const float amax = __uint_as_float(m);
+  const float sc = append_scale(amax, scale, old, lowest, head_base, tok_stride, a.dim, true);
+  const float rcp = __frcp_rn(sc);
+  const bool fast = isfinite(amax) && !isinf(rcp);
+  if (on)
+#pragma unroll 2
+    for (int i = sub; i < n; i += 2) {
+      float y[8];
+      values(i, y);
+      const float lo[4] = {y[0], y[1], y[2], y[3]}, hi[4] = {y[4], y[5], y[6], y[7]};
+      *reinterpret_cast<uint2*>(head_base + list.off[i] * tok_stride + d) =
+          make_uint2(quantize_word(lo, sc, rcp, fast), quantize_word(hi, sc, rcp, fast));
+    }
+}
+
+// The heads of K, of V or of both by the CTA's warps.
+template <typename T, int VEC, int NC>
+__device__ __forceinline__ void append_heads(const AppendArgs<T>& a, int64_t page, bool key_part,
+                                             bool value_part, const AppendList& list) {
+  const int rows = (key_part ? a.kv_heads : 0) + (value_part ? a.kv_heads : 0);
+  const int warp = threadIdx.x >> 5;
+  const bool turns = a.positions != nullptr;
+  auto is_key = [&](int r) { return key_part && r < a.kv_heads; };
+  auto head = [&](int r) { return r < a.kv_heads ? r : r - a.kv_heads; };
+  if (VEC == 8 && list.count <= kAppendHold) {
+    extern __shared__ __align__(16) float s_rows[];  // table rows, then each warp's rows
+    T* raw = reinterpret_cast<T*>(s_rows + kAppendHold * 128) + warp * kAppendHold * 128;
+    if (key_part && turns)  // the tokens' table rows, once for all heads
+      for (int i = threadIdx.x; i < list.count * 32; i += kAppendThreads) {
+        const int tok = i / 32, at = (i % 32) * 4;
+        if (at < a.rot) copy16_async(s_rows + tok * 128 + at, a.table + list.pos[tok] * a.rot + at);
+      }
+    for (int r0 = 0; r0 < rows; r0 += kAppendWarps) {
+      const int r = r0 + warp;
+      if (r < rows) append_fetch8(a, is_key(r), head(r), list, raw);
+      copies_wait();
+      if (r0 == 0) __syncthreads();  // the table rows are every warp's copies
+      else __syncwarp();
+      if (r >= rows) continue;
+      if (!is_key(r) || !turns)
+        append_head8<T, kNoRotation>(a, page, is_key(r), head(r), list, raw, s_rows);
+      else if (a.interleaved)
+        append_head8<T, kPairs>(a, page, true, head(r), list, raw, s_rows);
+      else
+        append_head8<T, kHalves>(a, page, true, head(r), list, raw, s_rows);
+      __syncwarp();  // the rows are free for the warp's next head
+    }
+    return;
+  }
+  constexpr int kVec = VEC == 8 ? 4 : VEC;
+  for (int r = warp; r < rows; r += kAppendWarps) {
+    if (!is_key(r) || !turns)
+      append_head<T, kVec, NC, kNoRotation>(a, page, is_key(r), head(r), list);
+    else if (a.interleaved)
+      append_head<T, kVec, NC, kPairs>(a, page, true, head(r), list);
+    else
+      append_head<T, kVec, NC, kHalves>(a, page, true, head(r), list);
   }
 }
 
@@ -595,7 +753,8 @@ __device__ void append_page(const AppendArgs<T>& a, int64_t page, bool is_key, c
 // earlier token of the call is in that page.
 template <typename T, int VEC, int NC>
 __global__ void __launch_bounds__(kAppendThreads) append_scan_kernel(AppendArgs<T> a, int* err) {
-  __shared__ int s_tok[kAppendMaxPage], s_list[2 * kAppendMaxPage];
+  __shared__ int s_tok[kAppendMaxPage];
+  __shared__ AppendList s_list;
   __shared__ int s_taken;
   const int64_t t = blockIdx.x >> 1;
   const bool is_key = (blockIdx.x & 1) == 0;
@@ -613,15 +772,17 @@ __global__ void __launch_bounds__(kAppendThreads) append_scan_kernel(AppendArgs<
   }
   __syncthreads();
   if (s_taken) return;  // whole CTA
-  append_page<T, VEC, NC>(a, page, is_key, s_tok, s_list);
+  append_list(a, s_tok, s_list);
+  append_heads<T, VEC, NC>(a, page, is_key, !is_key, s_list);
 }
 
 // Index of larger calls.  A run head (a token whose predecessor is not in the
 // same page) pushes itself on its page's list: head[page] = last pushed + 1
-// (0: none), next[t] = the one before.  The first to push lists the page.
+// (0: none), next[t] = the one before.  The first to push lists the page and
+// itself.
 template <typename T>
 __global__ void __launch_bounds__(256)
-    append_index_kernel(AppendArgs<T> a, int* head, int* next, int* pages, int* count, int* err) {
+    append_index_kernel(AppendArgs<T> a, int* head, int* next, int2* pages, int* count, int* err) {
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (t >= a.tokens) return;
   const int64_t slot = append_slot(a, t, err);
@@ -633,23 +794,27 @@ __global__ void __launch_bounds__(256)
   }
   const int prev = atomicExch(&head[page], (int)t + 1);
   next[t] = prev;
-  if (prev == 0) pages[atomicAdd(count, 1)] = (int)page;
+  if (prev == 0) pages[atomicAdd(count, 1)] = make_int2((int)page, (int)t);
 }
 
 template <typename T, int VEC, int NC>
-__global__ void __launch_bounds__(kAppendThreads)
-    append_pages_kernel(AppendArgs<T> a, const int* head, const int* next, const int* pages,
+__global__ void __launch_bounds__(kAppendThreads, VEC == 8 ? 3 : 1)
+    append_pages_kernel(AppendArgs<T> a, const int* head, const int* next, const int2* pages,
                         const int* count, int* err) {
-  __shared__ int s_tok[kAppendMaxPage], s_list[2 * kAppendMaxPage];
-  const int units = 2 * *count;
+  __shared__ int s_tok[kAppendMaxPage];
+  __shared__ AppendList s_list;
+  const int units = *count;
   for (int u = blockIdx.x; u < units; u += gridDim.x) {
-    const int64_t page = pages[u >> 1];
+    const int2 entry = pages[u];
+    const int64_t page = entry.x;
     __syncthreads();  // the previous unit is done with s_tok and s_list
     for (int i = threadIdx.x; i < a.bs; i += kAppendThreads) s_tok[i] = -1;
     __syncthreads();
     if (threadIdx.x < 32) {
-      for (int link = head[page]; link != 0; link = next[link - 1]) {
-        for (int64_t t0 = link - 1; t0 < a.tokens; t0 += 32) {
+      // the run of the token that listed the page, then the runs pushed after it
+      int link = head[page];
+      for (int64_t start = entry.y;;) {
+        for (int64_t t0 = start; t0 < a.tokens; t0 += 32) {
           const int64_t t = t0 + threadIdx.x;
           const int64_t slot = t < a.tokens ? append_slot(a, t, err) : -1;
           const bool in = slot >= 0 && slot / a.bs == page;
@@ -659,10 +824,14 @@ __global__ void __launch_bounds__(kAppendThreads)
           if ((int)threadIdx.x < len) atomicMax(&s_tok[slot % a.bs], (int)t);
           if (len < 32) break;
         }
+        start = link - 1;
+        if (start == entry.y) break;
+        link = next[start];
       }
     }
     __syncthreads();
-    append_page<T, VEC, NC>(a, page, (u & 1) == 0, s_tok, s_list);
+    append_list(a, s_tok, s_list);
+    append_heads<T, VEC, NC>(a, page, true, true, s_list);
   }
 }
 
@@ -671,21 +840,27 @@ constexpr int64_t kAppendScan = 512;
 
 template <typename T, int VEC, int NC>
 void launch_append_n(const AppendArgs<T>& a, int* ws, cudaStream_t stream) {
+  constexpr int kStage = VEC == 8 ? kAppendHold * 128 * (4 + kAppendWarps * (int)sizeof(T)) : 0;
   int* err = device_error_word();
   if (a.tokens <= kAppendScan) {
-    append_scan_kernel<T, VEC, NC><<<(unsigned)(2 * a.tokens), kAppendThreads, 0, stream>>>(a, err);
+    static std::atomic<uint64_t> done{0};
+    allow_shared_memory(reinterpret_cast<const void*>(append_scan_kernel<T, VEC, NC>), kStage, done);
+    append_scan_kernel<T, VEC, NC>
+        <<<(unsigned)(2 * a.tokens), kAppendThreads, kStage, stream>>>(a, err);
     return;
   }
   int* head = ws;
   int* count = ws + a.blocks;
   int* next = count + 1;
-  int* pages = next + a.tokens;
+  int2* pages = reinterpret_cast<int2*>(next + a.tokens + ((a.blocks + 1 + a.tokens) & 1));  // ws is 8-byte aligned
   cudaMemsetAsync(head, 0, (size_t)(a.blocks + 1) * sizeof(int), stream);
   append_index_kernel<T><<<(unsigned)((a.tokens + 255) / 256), 256, 0, stream>>>(a, head, next,
                                                                                  pages, count, err);
-  const int64_t ctas = std::min<int64_t>(2 * a.tokens, 8LL * 148);
+  const int64_t ctas = std::min<int64_t>(a.tokens, 8LL * 148);
+  static std::atomic<uint64_t> done{0};
+  allow_shared_memory(reinterpret_cast<const void*>(append_pages_kernel<T, VEC, NC>), kStage, done);
   append_pages_kernel<T, VEC, NC>
-      <<<(unsigned)ctas, kAppendThreads, 0, stream>>>(a, head, next, pages, count, err);
+      <<<(unsigned)ctas, kAppendThreads, kStage, stream>>>(a, head, next, pages, count, err);
 }
 
 template <typename T>
@@ -711,13 +886,20 @@ int launch_append_t(const AppendKvArgs& p, int* ws, cudaStream_t stream) {
   a.rot = p.positions != nullptr ? p.rot : 0;
   a.interleaved = p.interleaved;
   auto aligned = [](const void* x, int n) { return reinterpret_cast<uintptr_t>(x) % n == 0; };
-  const bool vec = a.dim % 4 == 0 && a.k_tok % 4 == 0 && a.k_head % 4 == 0 && a.v_tok % 4 == 0 &&
-                   a.v_head % 4 == 0 && aligned(a.key, 4 * sizeof(T)) &&
-                   aligned(a.value, 4 * sizeof(T)) && aligned(a.cache, 4) &&
-                   (a.rot == 0 || a.interleaved || (a.rot % 8 == 0 && aligned(a.table, 16)));
-  if (vec && a.dim <= 128) launch_append_n<T, 4, 1>(a, ws, stream);
-  else if (vec) launch_append_n<T, 4, 2>(a, ws, stream);
-  else launch_append_n<T, 1, 8>(a, ws, stream);
+  auto rows_of = [&](int n, int bytes) {  // values and strides in pieces of n
+    return a.dim % n == 0 && a.k_tok % n == 0 && a.k_head % n == 0 && a.v_tok % n == 0 &&
+           a.v_head % n == 0 && aligned(a.key, bytes) && aligned(a.value, bytes);
+  };
+  // whole pieces are rotated, and table rows are read four values at a time
+  const bool halves = a.rot > 0 && !a.interleaved;
+  if (a.dim <= 128 && rows_of(8, 16) && aligned(a.cache, 8) &&
+      (a.rot == 0 || (a.rot % (halves ? 16 : 4) == 0 && aligned(a.table, 16))))
+    launch_append_n<T, 8, 1>(a, ws, stream);
+  else if (rows_of(4, 4 * (int)sizeof(T)) && aligned(a.cache, 4) &&
+           (!halves || (a.rot % 8 == 0 && aligned(a.table, 16))))
+    launch_append_n<T, 4, 2>(a, ws, stream);
+  else
+    launch_append_n<T, 1, 8>(a, ws, stream);
   return kOk;
 }
 
@@ -743,7 +925,8 @@ int launch_qk_norm_rope(const QkNormRopeArgs& a, cudaStream_t stream) {
 
 size_t append_kv_workspace_size(int64_t tokens, int64_t blocks) {
   if (tokens <= kAppendScan) return 0;
-  return (size_t)(blocks + 1 + 2 * tokens) * sizeof(int);
+  // list heads, page count, links, (page, first token) on an 8-byte boundary
+  return (size_t)(blocks + 1 + tokens + 1 + 2 * tokens) * sizeof(int) + 8;
 }
 
 int launch_append_kv(const AppendKvArgs& a, void* workspace, size_t workspace_bytes,
@@ -754,7 +937,7 @@ int launch_append_kv(const AppendKvArgs& a, void* workspace, size_t workspace_by
     set_error("workspace too small for append_kv");
     return kWorkspace;
   }
-  int* ws = static_cast<int*>(workspace);
+  int* ws = reinterpret_cast<int*>((reinterpret_cast<uintptr_t>(workspace) + 7) & ~(uintptr_t)7);
   switch (a.dtype) {
     case 0: launch_append_t<float>(a, ws, stream); break;
     case 1: launch_append_t<__half>(a, ws, stream); break;
