@@ -589,8 +589,9 @@ int pkv_shared_prefix_attention(const float* q, const int8_t* k_cache, const flo
   if (num_seqs > 0 && prefix_blocks > 0 && (!prefix_table || !prefix_len))
     return fail(PKV_ERR_INVALID_ARGUMENT, "null input or output pointer");
   if ((int64_t)num_seqs * num_heads > 0x7fffffffLL - 256 ||
-      (int64_t)prefix_blocks * block_size > 0x7fffffffLL - 256)
-    return fail(PKV_ERR_UNSUPPORTED, "more than 2^31 rows or prefix tokens");
+      (int64_t)prefix_blocks * block_size > 0x7fffffffLL - 256 ||
+      num_blocks > 0x7fffffffLL / block_size)
+    return fail(PKV_ERR_UNSUPPORTED, "more than 2^31 rows, prefix tokens or cache slots");
   if (reinterpret_cast<uintptr_t>(q) % 16 != 0 || reinterpret_cast<uintptr_t>(out) % 16 != 0 ||
       reinterpret_cast<uintptr_t>(k_cache) % 16 != 0 ||
       reinterpret_cast<uintptr_t>(v_cache) % 16 != 0)

@@ -22,8 +22,9 @@
 //
 // Roles: two softmax warpgroups (one 128-row tile each, one thread per row),
 // four converting warps (global INT8 pages -> fp16 tiles in shared memory, and
-// the pages' scales), one MMA warp.  The two row tiles alternate on the tensor
-// cores as in prefill.cu.
+// the pages' scales), one MMA warp per row tile; two warps idle, so that the
+// registers split evenly.  The row tiles take turns on the tensor cores as in
+// prefill.cu.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -38,8 +39,9 @@ namespace {
 
 constexpr int kRows = 128;
 constexpr int kKeys = 128;
-constexpr int kPrefixThreads = 13 * 32;
-constexpr int kConvWarp = 8, kMmaWarp = 12;
+constexpr int kPrefixThreads = 16 * 32;
+constexpr int kConvWarp = 8, kMmaWarp = 12, kIdleWarp = 14;
+constexpr int kEarly = 4;         // MMAs left of a step when the turn is passed on
 constexpr float kLog2e = 1.4426950408889634f;
 // A row's maximum moves when a tile exceeds it by more than 2^kLazy, and p is
 // kept times 2^kPShift: at most 2^15 in fp16.  The low half has fp16's smallest
@@ -61,7 +63,7 @@ struct PrefixCfg {
   static constexpr int kOffScale = kOffKV + kStages * kTileBytes;  // [slot][k, v][128]
   static constexpr int kOffMask = kOffScale + kSlots * 2 * kKeys * 4;
   static constexpr int kOffBar = kOffMask + kSlots * 16;
-  static constexpr int kBars = 2 * kStages + kSlots + 8 + 1;
+  static constexpr int kBars = 2 * kStages + kSlots + 8 + 3;
   static constexpr int kOffMisc = kOffBar + kBars * 8;
   static constexpr int kSmemBytes = kOffMisc + 32;
   static constexpr int kOCol = 256;
@@ -105,7 +107,9 @@ __device__ __forceinline__ uint2 codes_to_half(uint32_t w) {
   return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
 }
 
-template <int DP>
+// GROUPS: the pages hold a multiple of 16 tokens, so 16 columns of a tile share
+// their scales and one load serves them; else every token has its own.
+template <int DP, bool GROUPS>
 __global__ void __launch_bounds__(kPrefixThreads, 1)
     prefix_kernel(const PrefixParams p, int* err) {
   using C = PrefixCfg<DP>;
@@ -120,8 +124,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   uint64_t* p_full = s_full + 2;
   uint64_t* o_full = p_full + 2;
   uint64_t* mma_done = o_full + 2;
+  uint64_t* turn = mma_done + 1;  // per row tile
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
-  int* s_vmax = reinterpret_cast<int*>(smem + C::kOffMisc + 8);
+  float* s_vmax = reinterpret_cast<float*>(smem + C::kOffMisc + 16);  // of each converting warp
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kvh = blockIdx.x % p.kv_heads, pair = blockIdx.x / p.kv_heads;
@@ -140,7 +145,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   if (tid == 0) {
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(&kv_full[i], 128);
-      mbar_init(&kv_empty[i], 1);
+      mbar_init(&kv_empty[i], 2);  // both MMA warps
     }
     for (int i = 0; i < C::kSlots; ++i) mbar_init(&sc_full[i], 128);
     for (int i = 0; i < 2; ++i) {
@@ -149,31 +154,20 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       mbar_init(&p_full[i], 128);
       mbar_init(&o_full[i], 1);
     }
-    mbar_init(mma_done, 1);
+    mbar_init(mma_done, 2);
+    mbar_init(&turn[0], 1);
+    mbar_init(&turn[1], 1);
     mbar_fence_init();
-    *s_vmax = 0;
   }
   if (warp == kMmaWarp) tmem_alloc(s_tmem, 512);
   tmem_fence_before_sync();
   __syncthreads();
   tmem_fence_after_sync();
   const uint32_t tmem = *s_tmem;
-  if (n > 0) {  // the largest V scale of this part: p * v_scale is kept relative to it
-    const int first = tile0 * kKeys / p.bs;
-    const int last = (min((tile0 + n) * kKeys, len) - 1) / p.bs;
-    float v = 0.0f;
-    for (int i = first + tid; i <= last; i += kPrefixThreads) {
-      const int phys = p.table[i];
-      if (phys >= 0 && (int64_t)phys < p.num_blocks)
-        v = fmaxf(v, fabsf(p.v_scale[(int64_t)phys * p.kv_heads + kvh]));
-    }
-    const unsigned m = __reduce_max_sync(0xffffffffu, __float_as_uint(v));
-    if (lane == 0) atomicMax(s_vmax, (int)m);
-  }
-  __syncthreads();
-  const float vmax = __int_as_float(*s_vmax);
-
-  if (warp >= kConvWarp && warp < kMmaWarp) {
+  if (warp >= kConvWarp) {
+  // 256 x 152 + 256 x 104 = 65,536 = 512 x 128, the registers at launch
+  registers_down<104>();
+  if (warp < kMmaWarp) {
     // ---- pages to fp16 tiles -----------------------------------------------------
     constexpr int kLanes = DP / 16;            // 16-byte pieces of a token row
     constexpr int kStep = 128 / kLanes;        // token rows per pass
@@ -182,57 +176,93 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     const int piece = ct % kLanes, row0 = ct / kLanes;
     const int64_t row_bytes = (int64_t)p.kv_heads * p.dim;
     const bool in_dim = piece * 16 < p.dim;
-    const float inv_vmax = vmax > 0.0f ? 1.0f / vmax : 0.0f;
     bool ok = true;
     uint4 raw[2][kPass];
-    auto fetch = [&](int j, int kind) {
-      const int8_t* base = (kind ? p.v_cache : p.k_cache) + (int64_t)kvh * p.dim + piece * 16;
+    // Cache rows of this thread's tokens of a tile (-1: none), looked up while the
+    // previous tile is converted.
+    int at[kPass];
+    auto look_up = [&](int j) {
 #pragma unroll
       for (int i = 0; i < kPass; ++i) {
         const int tok = (tile0 + j) * kKeys + row0 + i * kStep;
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (tok < len && in_dim) {
+        at[i] = -1;
+        if (tok < len) {
           const int page = tok / p.bs;
           const int phys = p.table[page];
-          if (phys >= 0 && (int64_t)phys < p.num_blocks)
-            w = __ldg(reinterpret_cast<const uint4*>(
-                base + ((int64_t)phys * p.bs + (tok - page * p.bs)) * row_bytes));
+          if (phys >= 0 && (int64_t)phys < p.num_blocks) at[i] = phys * p.bs + (tok - page * p.bs);
         }
-        raw[kind][i] = w;
       }
     };
-    if (n > 0) fetch(0, 0);
+    auto fetch = [&](int kind) {
+      const int8_t* base = (kind ? p.v_cache : p.k_cache) + (int64_t)kvh * p.dim + piece * 16;
+#pragma unroll
+      for (int i = 0; i < kPass; ++i) {
+        raw[kind][i] = make_uint4(0, 0, 0, 0);
+        if (at[i] >= 0 && in_dim)
+          raw[kind][i] = __ldg(reinterpret_cast<const uint4*>(base + at[i] * row_bytes));
+      }
+    };
+    // scales of token ct of tile j: loaded with the tile's K rows
+    float ks = 0.0f, vs = 0.0f;
+    bool good = false;
+    auto fetch_scales = [&](int j) {
+      const int tok = (tile0 + j) * kKeys + ct;
+      ks = vs = 0.0f;
+      good = tok < len;
+      if (good) {
+        const int phys = p.table[tok / p.bs];
+        good = phys >= 0 && (int64_t)phys < p.num_blocks;
+        if (good) {
+          ks = p.k_scale[(int64_t)phys * p.kv_heads + kvh] * p.qk_scale;
+          vs = p.v_scale[(int64_t)phys * p.kv_heads + kvh];
+        } else {
+          record_error(err, kDevBadBlockId);
+        }
+      }
+    };
+    float inv_vmax = 0.0f;
+    if (n > 0) {
+      look_up(0);
+      fetch(0);
+      fetch_scales(0);
+      // the largest V scale of this part: p * v_scale is kept relative to it
+      const int first = tile0 * kKeys / p.bs;
+      const int last = (min((tile0 + n) * kKeys, len) - 1) / p.bs;
+      float v = 0.0f;
+      for (int i = first + ct; i <= last; i += 128) {
+        const int phys = p.table[i];
+        if (phys >= 0 && (int64_t)phys < p.num_blocks)
+          v = fmaxf(v, fabsf(p.v_scale[(int64_t)phys * p.kv_heads + kvh]));
+      }
+      v = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
+      if (lane == 0) s_vmax[warp - kConvWarp] = v;
+      named_barrier(1, 128);  // also seen by the softmax warps, through sc_full
+      const float vmax = fmaxf(fmaxf(s_vmax[0], s_vmax[1]), fmaxf(s_vmax[2], s_vmax[3]));
+      inv_vmax = vmax > 0.0f ? 1.0f / vmax : 0.0f;
+    }
     for (int j = 0; j < n; ++j) {
 #pragma unroll
       for (int kind = 0; kind < 2; ++kind) {
         const int i = 2 * j + kind, st = i % C::kStages;
         // the next tile's loads are in flight while this one is converted
-        if (kind == 0) fetch(j, 1);
-        else if (j + 1 < n) fetch(j + 1, 0);
+        if (kind == 0) {
+          fetch(1);
+          if (j + 1 < n) look_up(j + 1);
+        } else if (j + 1 < n) {
+          fetch(0);
+        }
         if (ok && !mbar_wait_bounded(&kv_empty[st], ((uint32_t)(i / C::kStages) & 1u) ^ 1u, err)) {
           record_error(err, kDevWaitTimeout);
           ok = false;
         }
         if (kind == 0) {  // the tile's scales and which of its tokens count
           const int slot = j % C::kSlots;
-          const int tok = (tile0 + j) * kKeys + ct;
-          float ks = 0.0f, vs = 0.0f;
-          bool good = tok < len;
-          if (good) {
-            const int phys = p.table[tok / p.bs];
-            good = phys >= 0 && (int64_t)phys < p.num_blocks;
-            if (good) {
-              ks = p.k_scale[(int64_t)phys * p.kv_heads + kvh] * p.qk_scale;
-              vs = p.v_scale[(int64_t)phys * p.kv_heads + kvh] * inv_vmax;
-            } else {
-              record_error(err, kDevBadBlockId);
-            }
-          }
           s_scale[(slot * 2) * kKeys + ct] = ks;
-          s_scale[(slot * 2 + 1) * kKeys + ct] = vs;
+          s_scale[(slot * 2 + 1) * kKeys + ct] = vs * inv_vmax;
           const unsigned m = __ballot_sync(0xffffffffu, good);
           if (lane == 0) s_mask[slot * 4 + (ct >> 5)] = m;
           mbar_arrive(&sc_full[slot]);
+          if (j + 1 < n) fetch_scales(j + 1);
         }
         uint8_t* tile = smem + C::kOffKV + st * C::kTileBytes + (piece / 4) * (kKeys * 128);
 #pragma unroll
@@ -250,83 +280,97 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         mbar_arrive(&kv_full[st]);
       }
     }
-  } else if (warp == kMmaWarp) {
-    // ---- MMA issue --------------------------------------------------------------------
+  } else if (warp < kIdleWarp) {
+    // ---- MMA issue: a warp for each row tile, in strict turns (see prefill.cu) ---------
     if (n > 0) {
       constexpr uint32_t kIdQK = umma_f16_idesc(0, 0, kRows, kKeys);
       constexpr uint32_t kIdPV = umma_f16_idesc(0, 1, kRows, DP);
+      const int x = warp - kMmaWarp;
+      const bool mine = x == 0 || two;
       const uint32_t kv = smem_u32(smem + C::kOffKV);
-      const uint64_t q_desc = umma_sw128_desc(smem_u32(smem + C::kOffQ), 16, 1024);
+      const uint64_t q_desc =
+          umma_sw128_desc(smem_u32(smem + C::kOffQ + 2 * x * C::kTileBytes), 16, 1024);
       const uint64_t k_desc = umma_sw128_desc(kv, 16, 1024);
       const uint64_t v_desc = umma_sw128_desc(kv, kKeys * 128, 1024);
+      const uint32_t s_col = tmem + x * 128, o_col = tmem + C::kOCol + x * 128;
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
         if (ok && !mbar_wait_spin(bar, parity, err)) {
           record_error(err, kDevWaitTimeout);
           ok = false;
         }
-        tmem_fence_after_sync();
       };
-      auto stage_of = [&](int i) { return (uint32_t)(i % C::kStages) * C::kTileBytes; };
       auto wait_tile = [&](int i) {
         wait(&kv_full[i % C::kStages], (uint32_t)(i / C::kStages) & 1u);
       };
-      auto release = [&](int i) {  // only if a later tile reuses the stage
+      auto stage_of = [&](int i) { return (uint32_t)(i % C::kStages) * C::kTileBytes; };
+      // Both warps release a stage, each after it saw the tile, and only if a
+      // later tile reuses the stage.
+      auto release = [&](int i) {
         if (i + C::kStages < 2 * n) umma_commit_warp(&kv_empty[i % C::kStages]);
       };
-      auto qk = [&](int x, int j) {
+      auto pass_turn = [&]() {
+        if (lane == 0) mbar_arrive(&turn[x ^ 1]);
+        __syncwarp();
+      };
+      auto qk = [&](int j, bool pass) {
         const uint64_t b = umma_desc_at(k_desc, stage_of(2 * j));
 #pragma unroll
         for (int half = 1; half >= 0; --half) {  // lo first: roundings of a small sum
-          const uint64_t a = umma_desc_at(q_desc, (uint32_t)(2 * x + half) * C::kTileBytes);
+          const uint64_t a = umma_desc_at(q_desc, (uint32_t)half * C::kTileBytes);
 #pragma unroll
           for (int kk = 0; kk < DP / 16; ++kk) {
             const uint32_t off = (uint32_t)(kk / 4) * (kKeys * 128) + (uint32_t)(kk % 4) * 32;
-            umma_f16_warp(tmem + x * 128, umma_desc_at(a, off), umma_desc_at(b, off), kIdQK,
+            umma_f16_warp(s_col, umma_desc_at(a, off), umma_desc_at(b, off), kIdQK,
                           (half < 1 || kk > 0) ? 1u : 0u);
+            if (half == 0 && kk == DP / 16 - kEarly && pass) pass_turn();
           }
         }
         umma_commit_warp(&s_full[x]);
       };
-      // P of tokens 32 i .. 32 i + 31 is in columns 32 i: hi in 16, lo in 16
-      auto pv = [&](int x, int j) {
-        const uint64_t b = umma_desc_at(v_desc, stage_of(2 * j + 1));
-#pragma unroll
-        for (int kk = 0; kk < kKeys / 16; ++kk)
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-            umma_f16_ta_warp(tmem + C::kOCol + x * 128,
-                        tmem + x * 128 + (kk / 2) * 32 + half * 16 + (kk % 2) * 8,
-                        umma_desc_at(b, kk * 2048), kIdPV,
-                        (j > 0 || kk > 0 || half > 0) ? 1u : 0u);
-        if (j == n - 1) umma_commit_warp(&o_full[x]);
-      };
-      const int nx = two ? 2 : 1;
       wait_tile(0);
-      for (int x = 0; x < nx; ++x) {
+      if (mine) {
         wait(&q_full[x], 0);
-        if (ok) qk(x, 0);
+        tmem_fence_after_sync();
+        if (ok) qk(0, false);
       }
       release(0);
       for (int j = 0; j < n && ok; ++j) {
         wait_tile(2 * j + 1);
-        for (int x = 0; x < nx; ++x) {
-          wait(&p_full[x], (uint32_t)j & 1u);
+        if (x == 1 || j > 0) wait(&turn[x], (uint32_t)(x == 1 ? j : j - 1) & 1u);
+        if (mine) wait(&p_full[x], (uint32_t)j & 1u);
+        tmem_fence_after_sync();
+        if (!ok) break;
+        if (mine) {
+          // P of tokens 32 i .. 32 i + 31 is in columns 32 i: hi in 16, lo in 16
+          const uint64_t b = umma_desc_at(v_desc, stage_of(2 * j + 1));
+#pragma unroll
+          for (int kk = 0; kk < kKeys / 16; ++kk)
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+              umma_f16_ta_warp(o_col, s_col + (kk / 2) * 32 + half * 16 + (kk % 2) * 8,
+                               umma_desc_at(b, kk * 2048), kIdPV,
+                               (j > 0 || kk > 0 || half > 0) ? 1u : 0u);
+          if (j == n - 1) umma_commit_warp(&o_full[x]);
+          // the next K tile is converted while these run (its stage was V (j - 1)'s)
+          if (j + 1 < n) wait_tile(2 * j + 2);
           if (!ok) break;
-          pv(x, j);
-          if (x == nx - 1) release(2 * j + 1);
-          if (j + 1 < n) {
-            wait_tile(2 * j + 2);
-            if (!ok) break;
-            qk(x, j + 1);
-          }
+          if (j + 1 < n) qk(j + 1, true);  // over P (j): a warp's MMAs run in order
+          else pass_turn();
+        } else {
+          if (j + 1 < n) wait_tile(2 * j + 2);
+          pass_turn();
         }
+        release(2 * j + 1);
         if (j + 1 < n) release(2 * j + 2);
       }
       umma_commit_warp(mma_done);
       mbar_drain(mma_done, 0);  // every MMA is done before tensor memory is freed
     }
-  } else if (warp < 8 && (warp < 4 || two)) {
+  }
+  } else {
+  registers_up<152>();
+  if (warp < 4 || two) {
     // ---- query split, softmax, partials: thread = row --------------------------------------
     const int x = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
@@ -337,45 +381,43 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     const int64_t head_row = (int64_t)seq * p.heads + kvh * p.group + (r - seq * p.group);
     float rf = 1.0f;  // power of two that the row was divided by
     if (n > 0) {
-      const float4* src = reinterpret_cast<const float4*>(p.q + head_row * p.dim);
-      const int n4 = valid ? p.dim / 4 : 0;
-      float big = 0.0f;
-      for (int i = 0; i < n4; ++i) {
-        const float4 v = src[i];
-        big = fmaxf(fmaxf(big, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
-      }
-      // largest magnitude to [2^10, 2^11): exact, and lo's steps stay far below hi's
-      float up = 1.0f;
-      if (big > 0.0f && big <= 3.402823466e38f) {
-        const int e = min(10 - ilogbf(big), 126);
-        up = exp2f((float)e);
-        rf = exp2f((float)-e);
-      }
+      // The warp takes its 32 rows one after the other, a lane per 4 channels.
+      // A row's largest magnitude is scaled to [2^10, 2^11): exact, and lo's steps
+      // stay far below hi's.
       uint8_t* hi_t = smem + C::kOffQ + (2 * x) * C::kTileBytes;
       uint8_t* lo_t = hi_t + C::kTileBytes;
-#pragma unroll 1
-      for (int c = 0; c < DP / 8; ++c) {
-        float f[8];
+      const int base = pair * 256 + warp * 32;
+#pragma unroll 4
+      for (int i = 0; i < 32; ++i) {
+        const int ri = base + i, si = ri / p.group;
+        float4 v = make_float4(0, 0, 0, 0);
+        if (ri < rows && lane * 4 < p.dim)
+          v = reinterpret_cast<const float4*>(
+              p.q + ((int64_t)si * p.heads + kvh * p.group + (ri - si * p.group)) * p.dim)[lane];
+        float big = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+        big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
+        // 2^e from the exponent bits: e = 10 - floor(log2 big), at most 126
+        int e = 137 - (int)(__float_as_uint(big) >> 23);
+        if (big == 0.0f || !(big <= 3.402823466e38f)) e = 0;
+        e = min(e, 126);
+        const float up = __int_as_float((e + 127) << 23);
+        if (lane == i) rf = __int_as_float((127 - e) << 23);
+        const float f[4] = {v.x * up, v.y * up, v.z * up, v.w * up};
+        uint32_t hi[2], lo[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float4 v = 2 * c + i < n4 ? src[2 * c + i] : make_float4(0, 0, 0, 0);
-          f[4 * i] = v.x * up;
-          f[4 * i + 1] = v.y * up;
-          f[4 * i + 2] = v.z * up;
-          f[4 * i + 3] = v.w * up;
-        }
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+        for (int u = 0; u < 2; ++u) {
+          const __half2 h = __floats2half2_rn(f[2 * u], f[2 * u + 1]);
           const float2 b = __half22float2(h);
-          const __half2 l = __floats2half2_rn(f[2 * i] - b.x, f[2 * i + 1] - b.y);
-          hi[i] = *reinterpret_cast<const uint32_t*>(&h);
-          lo[i] = *reinterpret_cast<const uint32_t*>(&l);
+          const __half2 r2 = __floats2half2_rn(f[2 * u] - b.x, f[2 * u + 1] - b.y);
+          hi[u] = *reinterpret_cast<const uint32_t*>(&h);
+          lo[u] = *reinterpret_cast<const uint32_t*>(&r2);
         }
-        const uint32_t off = (c / 8) * (kRows * 128) + sw128_offset(row, (c % 8) * 16);
-        *reinterpret_cast<uint4*>(hi_t + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(lo_t + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        if (lane * 4 < DP) {
+          const uint32_t off = (lane / 16) * (kRows * 128) +
+                               sw128_offset((warp & 3) * 32 + i, (lane % 16) * 8);
+          *reinterpret_cast<uint2*>(hi_t + off) = make_uint2(hi[0], hi[1]);
+          *reinterpret_cast<uint2*>(lo_t + off) = make_uint2(lo[0], lo[1]);
+        }
       }
       fence_proxy_async_smem();  // an MMA operand
       mbar_arrive(&q_full[x]);
@@ -391,28 +433,54 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       }
       __syncwarp();
       tmem_fence_after_sync();
-      const float4* ks4 = reinterpret_cast<const float4*>(s_scale + slot * 2 * kKeys);
-      const float4* vs4 = ks4 + kKeys / 4;
-      uint32_t mask[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) mask[i] = s_mask[slot * 4 + i];
-      float t = -INFINITY;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t s[32];
-        tmem_load<32>(s_addr + c * 32, s);
+      const float* ks = s_scale + slot * 2 * kKeys;
+      const float* vs = ks + kKeys;
+      const uint32_t* mask = s_mask + slot * 4;
+      const bool all = (mask[0] & mask[1] & mask[2] & mask[3]) == 0xffffffffu;
+      // Scores of chunk c (32 tokens) times their pages' K scales; tokens that do
+      // not count become -inf.  The next chunk's loads are issued before this one's
+      // arithmetic: each takes about 150 clocks.
+      uint32_t s[32];
+      tmem_load<32>(s_addr, s);
+      auto scores = [&](int c, uint64_t (&y)[16]) {
+        float k0 = 0.0f, k1 = 0.0f;
+        if constexpr (GROUPS) {
+          k0 = ks[c * 32];
+          k1 = ks[c * 32 + 16];
+        }
         tmem_wait_load();
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float4 k = ks4[c * 8 + e];
-          const float y[4] = {__uint_as_float(s[4 * e]) * k.x, __uint_as_float(s[4 * e + 1]) * k.y,
-                              __uint_as_float(s[4 * e + 2]) * k.z,
-                              __uint_as_float(s[4 * e + 3]) * k.w};
+        for (int e = 0; e < 16; ++e) {
+          const float g = e < 8 ? k0 : k1;
+          const uint64_t k =
+              GROUPS ? f32x2(g, g) : *reinterpret_cast<const uint64_t*>(ks + c * 32 + 2 * e);
+          y[e] = mul_f32x2(f32x2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), k);
+        }
+        tmem_load<32>(s_addr + ((c + 1) & 3) * 32, s);  // the last one: chunk 0 again
+        if (!all) {
+          const uint32_t bits = mask[c];
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (mask[c] >> (4 * e + i) & 1u) t = fmaxf(t, y[i]);
+          for (int e = 0; e < 16; ++e) {
+            const float2 a = unpack_f32x2(y[e]);
+            y[e] = f32x2(bits >> (2 * e) & 1u ? a.x : -INFINITY,
+                         bits >> (2 * e + 1) & 1u ? a.y : -INFINITY);
+          }
+        }
+      };
+      float tm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      // (rolled: unrolled, the two passes were 40 KB of code, and fetching it cost
+      // the first tile 16,000 clocks)
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint64_t y[16];
+        scores(c, y);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float2 a = unpack_f32x2(y[e]);
+          tm[e & 3] = max3_nan(tm[e & 3], a.x, a.y);
         }
       }
+      const float t = max3_nan(max3_nan(tm[0], tm[1], tm[2]), tm[3], tm[3]);
       const bool move = valid && t > m && (m == -INFINITY || (t - m) * rf > kLazy);
       if (__any_sync(0xffffffffu, move)) {
         const float alpha = move ? ex2((m - t) * rf) : 1.0f;
@@ -430,38 +498,44 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           }
         }
       }
-      const float ms = (m == -INFINITY ? 0.0f : m * rf) - kPShift;
-#pragma unroll
+      // a NaN score makes the whole row NaN
+      const float ms = t != t ? t : (m == -INFINITY ? 0.0f : m * rf) - kPShift;
+      const uint64_t rf2 = f32x2(rf, rf), ms2 = f32x2(-ms, -ms);
+      uint64_t sum[2] = {0, 0};
+#pragma unroll 1
       for (int c = 0; c < 4; ++c) {
-        uint32_t s[32];
-        tmem_load<32>(s_addr + c * 32, s);
-        tmem_wait_load();
-        uint32_t w[32];  // 16 columns of hi, 16 of lo
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float4 k = ks4[c * 8 + e], v = vs4[c * 8 + e];
-          const float kk[4] = {k.x, k.y, k.z, k.w}, vv[4] = {v.x, v.y, v.z, v.w};
-          float pr[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float y = fmaf(__uint_as_float(s[4 * e + i]) * kk[i], rf, -ms);
-            pr[i] = mask[c] >> (4 * e + i) & 1u ? ex2(y) : 0.0f;
-            sum[i] += pr[i];
-            pr[i] *= vv[i];
-          }
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const __half2 h = __floats2half2_rn(pr[2 * i], pr[2 * i + 1]);
-            const float2 b = __half22float2(h);
-            const __half2 lo = __floats2half2_rn(pr[2 * i] - b.x, pr[2 * i + 1] - b.y);
-            w[2 * e + i] = *reinterpret_cast<const uint32_t*>(&h);
-            w[16 + 2 * e + i] = *reinterpret_cast<const uint32_t*>(&lo);
-          }
+        uint64_t y[16];
+        float v0 = 0.0f, v1 = 0.0f;
+        if constexpr (GROUPS) {
+          v0 = vs[c * 32];
+          v1 = vs[c * 32 + 16];
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        scores(c, y);
+        uint32_t w[32];  // 16 columns of hi, 16 of lo
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float g = e < 8 ? v0 : v1;
+          const uint64_t v =
+              GROUPS ? f32x2(g, g) : *reinterpret_cast<const uint64_t*>(vs + c * 32 + 2 * e);
+          float2 z = unpack_f32x2(fma_f32x2(y[e], rf2, ms2));
+          z.x = ex2(z.x);
+          z.y = ex2(z.y);
+          const uint64_t pr = f32x2(z.x, z.y);
+          sum[e & 1] = add_f32x2(sum[e & 1], pr);
+          const uint64_t pv = mul_f32x2(pr, v);
+          const float2 f = unpack_f32x2(pv);
+          const __half2 hi = __floats2half2_rn(f.x, f.y);
+          const float2 b = __half22float2(hi);
+          const float2 r = unpack_f32x2(sub_f32x2(pv, f32x2(b.x, b.y)));
+          const __half2 lo = __floats2half2_rn(r.x, r.y);
+          w[e] = *reinterpret_cast<const uint32_t*>(&hi);
+          w[16 + e] = *reinterpret_cast<const uint32_t*>(&lo);
+        }
         tmem_store<32>(s_addr + c * 32, w);
       }
+      const float2 l2 = unpack_f32x2(add_f32x2(sum[0], sum[1]));
+      l += l2.x + l2.y;
+      tmem_wait_load();  // the load that ran ahead
       tmem_wait_store();
       tmem_fence_before_sync();
       mbar_arrive(&p_full[x]);
@@ -471,6 +545,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       __syncwarp();
       tmem_fence_after_sync();
     }
+    const float vmax = fmaxf(fmaxf(s_vmax[0], s_vmax[1]), fmaxf(s_vmax[2], s_vmax[3]));
     const int64_t slot_row = (int64_t)split * p.num_seqs * p.heads + head_row;
     if (valid) {
       // nothing attended: (-inf, 0); every score NaN: a NaN that the join keeps
@@ -494,6 +569,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         }
       }
     }
+  }
   }
   tmem_fence_before_sync();
   __syncthreads();
@@ -612,10 +688,10 @@ PrefixWs prefix_ws(const SharedPrefixArgs& a) {
   return w;
 }
 
-template <int DP>
+template <int DP, bool GROUPS>
 void launch_prefix_t(const PrefixParams& p, cudaStream_t stream) {
   using C = PrefixCfg<DP>;
-  auto kern = prefix_kernel<DP>;
+  auto kern = prefix_kernel<DP, GROUPS>;
   static std::atomic<uint64_t> done{0};
   allow_shared_memory(reinterpret_cast<const void*>(kern), C::kSmemBytes, done);
   const int64_t pairs = ((int64_t)p.num_seqs * p.group + 255) / 256;
@@ -664,8 +740,11 @@ int launch_shared_prefix(const SharedPrefixArgs& a, void* workspace, size_t work
     p.width = a.prefix_width;
     p.splits = w.splits;
     p.qk_scale = o.sm_scale * kLog2e;
-    if (o.head_dim <= 64) launch_prefix_t<64>(p, stream);
-    else launch_prefix_t<128>(p, stream);
+    const bool groups = o.block_size % 16 == 0;
+    if (o.head_dim <= 64)
+      groups ? launch_prefix_t<64, true>(p, stream) : launch_prefix_t<64, false>(p, stream);
+    else
+      groups ? launch_prefix_t<128, true>(p, stream) : launch_prefix_t<128, false>(p, stream);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) {
       set_error(std::string("prefix launch failed: ") + cudaGetErrorString(e));
