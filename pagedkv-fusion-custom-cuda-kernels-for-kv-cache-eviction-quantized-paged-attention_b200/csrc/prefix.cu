@@ -181,16 +181,26 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     // Cache rows of this thread's tokens of a tile (-1: none), looked up while the
     // previous tile is converted.
     int at[kPass];
+    int scale_phys = -1;  // page of the token whose scales this thread looks after
     auto look_up = [&](int j) {
+      int phys[kPass];
+      const int first = (tile0 + j) * kKeys;
+      const int last = len - 1;
+#pragma unroll
+      for (int i = 0; i < kPass; ++i)  // all loads first; past the end the last page again
+        phys[i] = p.table[min(first + row0 + i * kStep, last) / p.bs];
+      scale_phys = p.table[min(first + ct, last) / p.bs];
 #pragma unroll
       for (int i = 0; i < kPass; ++i) {
-        const int tok = (tile0 + j) * kKeys + row0 + i * kStep;
-        at[i] = -1;
-        if (tok < len) {
-          const int page = tok / p.bs;
-          const int phys = p.table[page];
-          if (phys >= 0 && (int64_t)phys < p.num_blocks) at[i] = phys * p.bs + (tok - page * p.bs);
-        }
+        const int tok = first + row0 + i * kStep;
+        const bool good = tok < len && phys[i] >= 0 && (int64_t)phys[i] < p.num_blocks;
+        at[i] = good ? phys[i] * p.bs + tok % p.bs : -1;
+      }
+      if (first + ct >= len) {
+        scale_phys = -1;
+      } else if (scale_phys < 0 || (int64_t)scale_phys >= p.num_blocks) {
+        scale_phys = -1;
+        record_error(err, kDevBadBlockId);
       }
     };
     auto fetch = [&](int kind) {
@@ -202,29 +212,19 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           raw[kind][i] = __ldg(reinterpret_cast<const uint4*>(base + at[i] * row_bytes));
       }
     };
-    // scales of token ct of tile j: loaded with the tile's K rows
+    // scales of the thread's token: loaded with the tile's K rows
     float ks = 0.0f, vs = 0.0f;
     bool good = false;
-    auto fetch_scales = [&](int j) {
-      const int tok = (tile0 + j) * kKeys + ct;
-      ks = vs = 0.0f;
-      good = tok < len;
-      if (good) {
-        const int phys = p.table[tok / p.bs];
-        good = phys >= 0 && (int64_t)phys < p.num_blocks;
-        if (good) {
-          ks = p.k_scale[(int64_t)phys * p.kv_heads + kvh] * p.qk_scale;
-          vs = p.v_scale[(int64_t)phys * p.kv_heads + kvh];
-        } else {
-          record_error(err, kDevBadBlockId);
-        }
-      }
+    auto fetch_scales = [&]() {
+      good = scale_phys >= 0;
+      ks = good ? p.k_scale[(int64_t)scale_phys * p.kv_heads + kvh] : 0.0f;
+      vs = good ? p.v_scale[(int64_t)scale_phys * p.kv_heads + kvh] : 0.0f;
     };
     float inv_vmax = 0.0f;
     if (n > 0) {
       look_up(0);
       fetch(0);
-      fetch_scales(0);
+      fetch_scales();
       // the largest V scale of this part: p * v_scale is kept relative to it
       const int first = tile0 * kKeys / p.bs;
       const int last = (min((tile0 + n) * kKeys, len) - 1) / p.bs;
@@ -250,6 +250,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           if (j + 1 < n) look_up(j + 1);
         } else if (j + 1 < n) {
           fetch(0);
+          fetch_scales();
         }
         if (ok && !mbar_wait_bounded(&kv_empty[st], ((uint32_t)(i / C::kStages) & 1u) ^ 1u, err)) {
           record_error(err, kDevWaitTimeout);
@@ -257,12 +258,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         }
         if (kind == 0) {  // the tile's scales and which of its tokens count
           const int slot = j % C::kSlots;
-          s_scale[(slot * 2) * kKeys + ct] = ks;
+          s_scale[(slot * 2) * kKeys + ct] = ks * p.qk_scale;
           s_scale[(slot * 2 + 1) * kKeys + ct] = vs * inv_vmax;
           const unsigned m = __ballot_sync(0xffffffffu, good);
           if (lane == 0) s_mask[slot * 4 + (ct >> 5)] = m;
           mbar_arrive(&sc_full[slot]);
-          if (j + 1 < n) fetch_scales(j + 1);
         }
         uint8_t* tile = smem + C::kOffKV + st * C::kTileBytes + (piece / 4) * (kKeys * 128);
 #pragma unroll
@@ -387,13 +387,21 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       uint8_t* hi_t = smem + C::kOffQ + (2 * x) * C::kTileBytes;
       uint8_t* lo_t = hi_t + C::kTileBytes;
       const int base = pair * 256 + warp * 32;
-#pragma unroll 4
-      for (int i = 0; i < 32; ++i) {
-        const int ri = base + i, si = ri / p.group;
-        float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll 1
+      for (int i0 = 0; i0 < 32; i0 += 8) {
+      float4 rowv[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {  // all loads first
+        const int ri = base + i0 + u, si = ri / p.group;
+        rowv[u] = make_float4(0, 0, 0, 0);
         if (ri < rows && lane * 4 < p.dim)
-          v = reinterpret_cast<const float4*>(
+          rowv[u] = reinterpret_cast<const float4*>(
               p.q + ((int64_t)si * p.heads + kvh * p.group + (ri - si * p.group)) * p.dim)[lane];
+      }
+#pragma unroll
+      for (int u8 = 0; u8 < 8; ++u8) {
+        const int i = i0 + u8;
+        const float4 v = rowv[u8];
         float big = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
         big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
         // 2^e from the exponent bits: e = 10 - floor(log2 big), at most 126
@@ -418,6 +426,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           *reinterpret_cast<uint2*>(hi_t + off) = make_uint2(hi[0], hi[1]);
           *reinterpret_cast<uint2*>(lo_t + off) = make_uint2(lo[0], lo[1]);
         }
+      }
       }
       fence_proxy_async_smem();  // an MMA operand
       mbar_arrive(&q_full[x]);
