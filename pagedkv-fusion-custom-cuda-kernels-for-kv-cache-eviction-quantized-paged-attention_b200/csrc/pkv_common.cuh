@@ -201,25 +201,13 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   }
 }
 
-__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(done)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return done != 0;
-}
-
 // mbar_wait_bounded for hand-offs inside a CTA that follow each other within a
-// microsecond: non-blocking tests first, since waking from a suspended try_wait
-// and reading the timer each take a good part of that.
-__device__ __forceinline__ bool mbar_wait_spin(uint64_t* bar, uint32_t parity, const int* err) {
+// microsecond: suspended tries first, since reading the timer takes a good part
+// of that.
+__device__ __forceinline__ bool mbar_wait_short(uint64_t* bar, uint32_t parity, const int* err) {
 #pragma unroll 1
-  for (int i = 0; i < 4096; ++i)
-    if (mbar_test_wait(bar, parity)) return true;
+  for (int i = 0; i < 64; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
   return mbar_wait_bounded(bar, parity, err);
 }
 

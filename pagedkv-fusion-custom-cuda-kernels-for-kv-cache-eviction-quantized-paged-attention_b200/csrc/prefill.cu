@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         const uint32_t s_col = tmem + C::kSCol + x * 128, o_col = tmem + C::kOCol + x * 128;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-          if (ok && !mbar_wait_spin(bar, parity, err)) {
+          if (ok && !mbar_wait_short(bar, parity, err)) {
             record_error(err, kDevWaitTimeout);
             ok = false;
           }
@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       const int nt = n_tiles[x];
       bool ok = true;
       for (int j = 0; j < nt; ++j) {
-        if (ok && !mbar_wait_spin(&s_full[x], (uint32_t)j & 1u, err)) {
+        if (ok && !mbar_wait_short(&s_full[x], (uint32_t)j & 1u, err)) {
           record_error(err, kDevWaitTimeout);
           ok = false;
         }

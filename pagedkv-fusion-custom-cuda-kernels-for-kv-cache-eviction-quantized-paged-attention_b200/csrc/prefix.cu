@@ -63,7 +63,7 @@ struct PrefixCfg {
   static constexpr int kOffScale = kOffKV + kStages * kTileBytes;  // [slot][k, v][128]
   static constexpr int kOffMask = kOffScale + kSlots * 2 * kKeys * 4;
   static constexpr int kOffBar = kOffMask + kSlots * 16;
-  static constexpr int kBars = 2 * kStages + kSlots + 8 + 3;
+  static constexpr int kBars = 2 * kStages + kSlots + 10 + 3;
   static constexpr int kOffMisc = kOffBar + kBars * 8;
   static constexpr int kSmemBytes = kOffMisc + 32;
   static constexpr int kOCol = 256;
@@ -121,8 +121,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   uint64_t* sc_full = kv_empty + C::kStages;
   uint64_t* q_full = sc_full + C::kSlots;  // per row tile, as the next three
   uint64_t* s_full = q_full + 2;
-  uint64_t* p_full = s_full + 2;
-  uint64_t* o_full = p_full + 2;
+  uint64_t* p_full = s_full + 2;  // [row tile][half of the tokens]
+  uint64_t* o_full = p_full + 4;
   uint64_t* mma_done = o_full + 2;
   uint64_t* turn = mma_done + 1;  // per row tile
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
@@ -151,7 +151,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 128);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
+      mbar_init(&p_full[2 * i], 128);
+      mbar_init(&p_full[2 * i + 1], 128);
       mbar_init(&o_full[i], 1);
     }
     mbar_init(mma_done, 2);
@@ -182,19 +183,26 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     // previous tile is converted.
     int at[kPass];
     int scale_phys = -1;  // page of the token whose scales this thread looks after
+    const float inv_bs = 1.0f / (float)p.bs;
     auto look_up = [&](int j) {
-      int phys[kPass];
       const int first = (tile0 + j) * kKeys;
-      const int last = len - 1;
+      const int page0 = first / p.bs, rem = first - page0 * p.bs;
+      const int last_page = (len - 1) / p.bs;
+      // page of token first + o, o < 128: (rem + o) / bs without a division (both
+      // are below 256, so the rounded product is off by far less than 0.5 / bs)
+      auto page_of = [&](int o) { return page0 + (int)(((float)(rem + o) + 0.5f) * inv_bs); };
+      int page[kPass], phys[kPass];
 #pragma unroll
-      for (int i = 0; i < kPass; ++i)  // all loads first; past the end the last page again
-        phys[i] = p.table[min(first + row0 + i * kStep, last) / p.bs];
-      scale_phys = p.table[min(first + ct, last) / p.bs];
+      for (int i = 0; i < kPass; ++i) {  // all loads first; past the end the last page again
+        page[i] = page_of(row0 + i * kStep);
+        phys[i] = p.table[min(page[i], last_page)];
+      }
+      scale_phys = p.table[min(page_of(ct), last_page)];
 #pragma unroll
       for (int i = 0; i < kPass; ++i) {
         const int tok = first + row0 + i * kStep;
         const bool good = tok < len && phys[i] >= 0 && (int64_t)phys[i] < p.num_blocks;
-        at[i] = good ? phys[i] * p.bs + tok % p.bs : -1;
+        at[i] = good ? phys[i] * p.bs + (tok - page[i] * p.bs) : -1;
       }
       if (first + ct >= len) {
         scale_phys = -1;
@@ -295,7 +303,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       const uint32_t s_col = tmem + x * 128, o_col = tmem + C::kOCol + x * 128;
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (ok && !mbar_wait_spin(bar, parity, err)) {
+        if (ok && !mbar_wait_short(bar, parity, err)) {
           record_error(err, kDevWaitTimeout);
           ok = false;
         }
@@ -338,19 +346,24 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       for (int j = 0; j < n && ok; ++j) {
         wait_tile(2 * j + 1);
         if (x == 1 || j > 0) wait(&turn[x], (uint32_t)(x == 1 ? j : j - 1) & 1u);
-        if (mine) wait(&p_full[x], (uint32_t)j & 1u);
+        if (mine) wait(&p_full[2 * x], (uint32_t)j & 1u);
         tmem_fence_after_sync();
         if (!ok) break;
         if (mine) {
           // P of tokens 32 i .. 32 i + 31 is in columns 32 i: hi in 16, lo in 16
           const uint64_t b = umma_desc_at(v_desc, stage_of(2 * j + 1));
 #pragma unroll
-          for (int kk = 0; kk < kKeys / 16; ++kk)
+          for (int kk = 0; kk < kKeys / 16; ++kk) {
+            if (kk == kKeys / 32) {
+              wait(&p_full[2 * x + 1], (uint32_t)j & 1u);
+              tmem_fence_after_sync();
+            }
 #pragma unroll
             for (int half = 0; half < 2; ++half)
               umma_f16_ta_warp(o_col, s_col + (kk / 2) * 32 + half * 16 + (kk % 2) * 8,
                                umma_desc_at(b, kk * 2048), kIdPV,
                                (j > 0 || kk > 0 || half > 0) ? 1u : 0u);
+          }
           if (j == n - 1) umma_commit_warp(&o_full[x]);
           // the next K tile is converted while these run (its stage was V (j - 1)'s)
           if (j + 1 < n) wait_tile(2 * j + 2);
@@ -387,16 +400,23 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       uint8_t* hi_t = smem + C::kOffQ + (2 * x) * C::kTileBytes;
       uint8_t* lo_t = hi_t + C::kTileBytes;
       const int base = pair * 256 + warp * 32;
+      int gi = base % p.group;
+      const float* row_ptr =
+          p.q + ((int64_t)(base / p.group) * p.heads + kvh * p.group + gi) * p.dim + lane * 4;
+      const int64_t wrap = (int64_t)(p.heads - p.group) * p.dim;  // to the next sequence's group
 #pragma unroll 1
       for (int i0 = 0; i0 < 32; i0 += 8) {
       float4 rowv[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) {  // all loads first
-        const int ri = base + i0 + u, si = ri / p.group;
         rowv[u] = make_float4(0, 0, 0, 0);
-        if (ri < rows && lane * 4 < p.dim)
-          rowv[u] = reinterpret_cast<const float4*>(
-              p.q + ((int64_t)si * p.heads + kvh * p.group + (ri - si * p.group)) * p.dim)[lane];
+        if (base + i0 + u < rows && lane * 4 < p.dim)
+          rowv[u] = *reinterpret_cast<const float4*>(row_ptr);
+        row_ptr += p.dim;
+        if (++gi == p.group) {
+          gi = 0;
+          row_ptr += wrap;
+        }
       }
 #pragma unroll
       for (int u8 = 0; u8 < 8; ++u8) {
@@ -436,7 +456,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     for (int j = 0; j < n; ++j) {
       const int slot = j % C::kSlots;
       if (ok && (!mbar_wait_bounded(&sc_full[slot], (uint32_t)(j / C::kSlots) & 1u, err) ||
-                 !mbar_wait_spin(&s_full[x], (uint32_t)j & 1u, err))) {
+                 !mbar_wait_short(&s_full[x], (uint32_t)j & 1u, err))) {
         record_error(err, kDevWaitTimeout);
         ok = false;
       }
@@ -451,12 +471,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       // arithmetic: each takes about 150 clocks.
       uint32_t s[32];
       tmem_load<32>(s_addr, s);
+      float k0 = ks[0], k1 = ks[16];  // GROUPS: of the chunk's two groups
       auto scores = [&](int c, uint64_t (&y)[16]) {
-        float k0 = 0.0f, k1 = 0.0f;
-        if constexpr (GROUPS) {
-          k0 = ks[c * 32];
-          k1 = ks[c * 32 + 16];
-        }
+        const int next = ((c + 1) & 3) * 32;
         tmem_wait_load();
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -465,7 +482,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
               GROUPS ? f32x2(g, g) : *reinterpret_cast<const uint64_t*>(ks + c * 32 + 2 * e);
           y[e] = mul_f32x2(f32x2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), k);
         }
-        tmem_load<32>(s_addr + ((c + 1) & 3) * 32, s);  // the last one: chunk 0 again
+        tmem_load<32>(s_addr + next, s);  // after the last one chunk 0 again
+        if constexpr (GROUPS) {
+          k0 = ks[next];
+          k1 = ks[next + 16];
+        }
         if (!all) {
           const uint32_t bits = mask[c];
 #pragma unroll
@@ -511,19 +532,20 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       const float ms = t != t ? t : (m == -INFINITY ? 0.0f : m * rf) - kPShift;
       const uint64_t rf2 = f32x2(rf, rf), ms2 = f32x2(-ms, -ms);
       uint64_t sum[2] = {0, 0};
+      float v0 = vs[0], v1 = vs[16];
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint64_t y[16];
-        float v0 = 0.0f, v1 = 0.0f;
+        const float u0 = v0, u1 = v1;
         if constexpr (GROUPS) {
-          v0 = vs[c * 32];
-          v1 = vs[c * 32 + 16];
+          v0 = vs[((c + 1) & 3) * 32];
+          v1 = vs[((c + 1) & 3) * 32 + 16];
         }
         scores(c, y);
         uint32_t w[32];  // 16 columns of hi, 16 of lo
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float g = e < 8 ? v0 : v1;
+          const float g = e < 8 ? u0 : u1;
           const uint64_t v =
               GROUPS ? f32x2(g, g) : *reinterpret_cast<const uint64_t*>(vs + c * 32 + 2 * e);
           float2 z = unpack_f32x2(fma_f32x2(y[e], rf2, ms2));
@@ -541,13 +563,18 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           w[16 + e] = *reinterpret_cast<const uint32_t*>(&lo);
         }
         tmem_store<32>(s_addr + c * 32, w);
+        if (c == 1) {  // half of P is there: its product can start
+          tmem_wait_store();
+          tmem_fence_before_sync();
+          mbar_arrive(&p_full[2 * x]);
+        }
       }
       const float2 l2 = unpack_f32x2(add_f32x2(sum[0], sum[1]));
       l += l2.x + l2.y;
       tmem_wait_load();  // the load that ran ahead
       tmem_wait_store();
       tmem_fence_before_sync();
-      mbar_arrive(&p_full[x]);
+      mbar_arrive(&p_full[2 * x + 1]);
     }
     if (n > 0) {
       if (ok && !mbar_wait_bounded(&o_full[x], 0, err)) record_error(err, kDevWaitTimeout);
