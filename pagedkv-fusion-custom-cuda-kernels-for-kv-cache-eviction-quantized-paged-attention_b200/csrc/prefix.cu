@@ -166,8 +166,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   tmem_fence_after_sync();
   const uint32_t tmem = *s_tmem;
   if (warp >= kConvWarp) {
-  // 256 x 152 + 256 x 104 = 65,536 = 512 x 128, the registers at launch
-  registers_down<104>();
+  // 256 x 136 + 256 x 120 = 65,536 = 512 x 128, the registers at launch
+  registers_down<120>();
   if (warp < kMmaWarp) {
     // ---- pages to fp16 tiles -----------------------------------------------------
     constexpr int kLanes = DP / 16;            // 16-byte pieces of a token row
@@ -179,30 +179,32 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     const bool in_dim = piece * 16 < p.dim;
     bool ok = true;
     uint4 raw[2][kPass];
-    // Cache rows of this thread's tokens of a tile (-1: none), looked up while the
-    // previous tile is converted.
-    int at[kPass];
-    int scale_phys = -1;  // page of the token whose scales this thread looks after
-    const float inv_bs = 1.0f / (float)p.bs;
+    // Pages of this thread's tokens of a tile and of the token whose scales it
+    // looks after; read while the previous tile is converted, used after that.
+    // The page of token first + o, o < 128, is page0 + (rem + o) / bs, the quotient
+    // exact as ((rem + o) * ceil(2^16 / bs)) >> 16 since rem + o < 256, bs <= 64.
+    int phys[kPass], scale_phys = -1, at[kPass];
+    int first = 0, page0 = 0, rem = 0;
+    const uint32_t inv_bs = (65536u + p.bs - 1) / p.bs;
+    const int last_page = n > 0 ? (len - 1) / p.bs : 0;
+    auto pages_past = [&](int o) { return (int)(((uint32_t)(rem + o) * inv_bs) >> 16); };
     auto look_up = [&](int j) {
-      const int first = (tile0 + j) * kKeys;
-      const int page0 = first / p.bs, rem = first - page0 * p.bs;
-      const int last_page = (len - 1) / p.bs;
-      // page of token first + o, o < 128: (rem + o) / bs without a division (both
-      // are below 256, so the rounded product is off by far less than 0.5 / bs)
-      auto page_of = [&](int o) { return page0 + (int)(((float)(rem + o) + 0.5f) * inv_bs); };
-      int page[kPass], phys[kPass];
+      first = (tile0 + j) * kKeys;
+      page0 = first / p.bs;
+      rem = first - page0 * p.bs;
 #pragma unroll
-      for (int i = 0; i < kPass; ++i) {  // all loads first; past the end the last page again
-        page[i] = page_of(row0 + i * kStep);
-        phys[i] = p.table[min(page[i], last_page)];
-      }
-      scale_phys = p.table[min(page_of(ct), last_page)];
+      for (int i = 0; i < kPass; ++i)  // past the end the last page again
+        phys[i] = p.table[min(page0 + pages_past(row0 + i * kStep), last_page)];
+      scale_phys = p.table[min(page0 + pages_past(ct), last_page)];
+    };
+    // cache rows from the pages (-1: no token, or a page outside the cache)
+    auto resolve = [&]() {
 #pragma unroll
       for (int i = 0; i < kPass; ++i) {
-        const int tok = first + row0 + i * kStep;
-        const bool good = tok < len && phys[i] >= 0 && (int64_t)phys[i] < p.num_blocks;
-        at[i] = good ? phys[i] * p.bs + (tok - page[i] * p.bs) : -1;
+        const int o = row0 + i * kStep;
+        const bool good =
+            first + o < len && phys[i] >= 0 && (int64_t)phys[i] < p.num_blocks;
+        at[i] = good ? phys[i] * p.bs + (rem + o - pages_past(o) * p.bs) : -1;
       }
       if (first + ct >= len) {
         scale_phys = -1;
@@ -231,6 +233,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     float inv_vmax = 0.0f;
     if (n > 0) {
       look_up(0);
+      resolve();
       fetch(0);
       fetch_scales();
       // the largest V scale of this part: p * v_scale is kept relative to it
@@ -257,6 +260,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           fetch(1);
           if (j + 1 < n) look_up(j + 1);
         } else if (j + 1 < n) {
+          resolve();
           fetch(0);
           fetch_scales();
         }
@@ -382,7 +386,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     }
   }
   } else {
-  registers_up<152>();
+  registers_up<136>();
   if (warp < 4 || two) {
     // ---- query split, softmax, partials: thread = row --------------------------------------
     const int x = warp >> 2, row = tid & 127;
