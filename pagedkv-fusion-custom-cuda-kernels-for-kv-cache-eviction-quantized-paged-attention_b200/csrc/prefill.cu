@@ -2,7 +2,8 @@
 // over the keys j of token i's sequence, causal from the sequences' ends
 // (j <= i + Lk - Lq), grouped heads, fp16 or bf16 with fp32 accumulators.
 //
-// One CTA owns two row tiles of 128 rows of one KV head.  A row is a (token,
+// An item of work is two row tiles of 128 rows of one KV head; one CTA per SM
+// takes items until none is left.  A row is a (token,
 // query head of the group) pair, so the G heads of a group share every K / V
 // tile that is loaded.  Keys come in tiles of 128 tokens; per row tile
 //   S = Q K^T    tcgen05 kind::f16, 128 x 128, K-major A and B from shared
@@ -45,8 +46,8 @@ constexpr int kKeys = 128;      // keys of a tile (MMA N of Q K^T, K of P V)
 constexpr int kPreThreads = 512;  // softmax A and B (4 warps each), load, MMA A and B, cleaning (5)
 constexpr int kLoadWarp = 8, kMmaWarp = 9, kCleanWarp = 11;
 constexpr int kCleaners = kPreThreads - kCleanWarp * 32;
+constexpr int kConsumerWarps = 8 + 2 + kCleaners / 32;  // of an item
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLazy = 8.0f;   // log2 growth of a row maximum that moves it
 constexpr int kPart = 64;        // keys of P that are handed over first
 constexpr int kEarly = 4;        // MMAs left of a step when the turn is passed on
@@ -56,15 +57,18 @@ template <int DP>
 struct PreCfg {
   static constexpr int kChunks = DP / 64;               // 128-byte column chunks
   static constexpr int kTileBytes = kKeys * DP * 2;     // a K, V or Q tile
-  static constexpr int kStages = DP == 128 ? 5 : 8;     // K / V ring
+  static constexpr int kStages = DP == 128 ? 4 : 8;     // K / V ring
+  static constexpr int kStageBytes = kRows * 128;       // output staging: 64 channels a tile
   static constexpr int kOffQ = 0;                       // two Q tiles
   static constexpr int kOffKV = 2 * kTileBytes;
-  static constexpr int kOffBar = kOffKV + kStages * kTileBytes;
-  static constexpr int kBars = 2 * kStages + 10 + kMaskedTiles + 3;
-  static constexpr int kOffMisc = kOffBar + kBars * 8;
-  static constexpr int kSmemBytes = kOffMisc + 64 + kMaskedTiles * 16 + 1024;
+  static constexpr int kOffOut = kOffKV + kStages * kTileBytes;
+  static constexpr int kOffBar = kOffOut + 2 * kStageBytes;
+  static constexpr int kBars = 2 * kStages + 2 + 2 + 2 + 4 + 2 + kMaskedTiles + 2 + 4 + 2;
+  static constexpr int kOffMisc = kOffBar + kBars * 8;  // 16-byte aligned
+  static constexpr int kSmemBytes = kOffMisc + 288 + 1024;
   static constexpr int kSCol = 0;                       // S / P of the two tiles
   static constexpr int kOCol = 256;
+  static_assert(kBars % 2 == 0 && kSmemBytes <= 227 * 1024, "shared memory");
 };
 
 struct PreParams {
@@ -85,24 +89,74 @@ struct PreWork {
   int t0;              // first token (in the sequence) of row tile 0
 };
 
+// An item of work: two row tiles of a sequence, one KV head, and the key tiles
+// that they see.
+struct PreItem {
+  PreWork at;
+  int kvh;
+  int n_tiles[2];    // key tiles of each row tile: up to the last key of its last token
+  int n;             // the larger; 0: nothing to load
+  int first_masked;  // tiles from here on hold keys that some row does not see
+  int kind;          // kNone: past the end of the work, kSome, kStop: the CTA is done
+};
+enum ItemKind { kNone = 0, kSome = 1, kStop = 2 };
+
+__device__ __forceinline__ void count_tiles(const PreParams& p, PreItem& w) {
+  const int shift = w.at.lk - w.at.lq;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int first = w.at.t0 + x * p.tile_tokens;
+    const int last = min(first + p.tile_tokens, w.at.lq) - 1;
+    const int keys =
+        first < w.at.lq ? (p.causal ? min(max(last + shift + 1, 0), w.at.lk) : w.at.lk) : 0;
+    w.n_tiles[x] = (keys + kKeys - 1) / kKeys;
+  }
+  w.n = max(w.n_tiles[0], w.n_tiles[1]);
+  w.first_masked = (p.causal ? min(max(w.at.t0 + shift + 1, 0), w.at.lk) : w.at.lk) / kKeys;
+}
+
+// Asks the hardware for a CTA of this grid that has not started yet (16 bytes
+// of answer, completed on bar), and reads the answer: its block index, or -1.
+__device__ __forceinline__ void request_block(void* answer, uint64_t* bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], "
+      "[%1];" ::"r"(smem_u32(answer)),
+      "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ int granted_block(const void* answer) {
+  uint32_t got, x;
+  asm volatile(
+      "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t.reg .b32 y, z, w;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, y, z, w}, r;\n\t}"
+      : "=r"(got), "=r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return got ? (int)x : -1;
+}
+
 // Sequence and token range of pair `pair` (of 2 * tile_tokens tokens).  Pairs
 // are numbered sequence by sequence, the last pair of a sequence first: under
 // a causal mask it is the longest, and long work should start early.  The rows
 // behind the last sequence form one more sequence without keys (zeros).
 // One warp; false when `pair` is past the end.
-__device__ bool find_work(const PreParams& p, int pair, PreWork& w, int* err) {
+__device__ __forceinline__ bool find_work(const PreParams& p, int pair, PreWork& w, int* err) {
   const int lane = threadIdx.x & 31;
   const int span = 2 * p.tile_tokens;
   int base = 0;
   for (int s0 = 0; s0 <= p.num_seqs; s0 += 32) {
     const int s = s0 + lane;
-    int q0 = 0, q1 = 0;
+    int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
     if (s < p.num_seqs) {
-      const int a = p.cu_q[s], b = p.cu_q[s + 1];
+      const int a = p.cu_q[s], b = p.cu_q[s + 1], ka = p.cu_k[s], kb = p.cu_k[s + 1];
       q0 = min(max(a, 0), p.total_q);
       q1 = min(max(b, q0), p.total_q);
-      const int ka = p.cu_k[s], kb = p.cu_k[s + 1];
-      if (pair == 0 && (a != q0 || b != q1 || ka < 0 || kb < ka || kb > p.total_k))
+      k0 = min(max(ka, 0), p.total_k);
+      k1 = min(max(kb, k0), p.total_k);
+      if (pair == 0 && (a != q0 || b != q1 || ka != k0 || kb != k1))
         record_error(err, kDevBadSeqlens);
     } else if (s == p.num_seqs) {
       q0 = min(max(p.cu_q[s], 0), p.total_q);
@@ -124,13 +178,8 @@ __device__ bool find_work(const PreParams& p, int pair, PreWork& w, int* err) {
       w.q0 = __shfl_sync(0xffffffffu, q0, src);
       w.lq = __shfl_sync(0xffffffffu, q1, src) - w.q0;
       w.t0 = (__shfl_sync(0xffffffffu, n, src) - 1 - local) * span;
-      const int seq = s0 + src;
-      w.k0 = 0;
-      w.lk = 0;
-      if (seq < p.num_seqs) {
-        w.k0 = min(max(p.cu_k[seq], 0), p.total_k);
-        w.lk = min(max(p.cu_k[seq + 1], w.k0), p.total_k) - w.k0;
-      }
+      w.k0 = __shfl_sync(0xffffffffu, k0, src);
+      w.lk = __shfl_sync(0xffffffffu, k1, src) - w.k0;
       return true;
     }
     base += total;
@@ -188,113 +237,171 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
   uint64_t* kv_empty = kv_full + C::kStages;
-  uint64_t* q_full = kv_empty + C::kStages;  // per row tile, as the next three
-  uint64_t* s_full = q_full + 2;
+  uint64_t* q_full = kv_empty + C::kStages;  // per row tile, as the next four
+  uint64_t* q_empty = q_full + 2;
+  uint64_t* s_full = q_empty + 2;
   uint64_t* p_full = s_full + 2;  // [row tile][part of P]
   uint64_t* o_full = p_full + 4;
   uint64_t* raw_full = o_full + 2;  // V tiles with masked keys, before they are cleaned
-  uint64_t* mma_done = raw_full + kMaskedTiles;
-  uint64_t* turn = mma_done + 1;  // per row tile
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
-  int* s_work = reinterpret_cast<int*>(smem + C::kOffMisc + 16);
-  uint32_t* s_flags = reinterpret_cast<uint32_t*>(smem + C::kOffMisc + 64);  // [tile][4]
+  uint64_t* turn = raw_full + kMaskedTiles;  // per row tile
+  uint64_t* item_full = turn + 2;            // two items in flight
+  uint64_t* item_empty = item_full + 2;
+  uint64_t* mma_done = item_empty + 2;
+  uint64_t* block_full = mma_done + 1;
+  uint8_t* answer = smem + C::kOffMisc;  // of request_block
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::kOffMisc + 16);
+  PreItem* s_item = reinterpret_cast<PreItem*>(smem + C::kOffMisc + 32);            // [2]
+  uint32_t* s_flags = reinterpret_cast<uint32_t*>(smem + C::kOffMisc + 32 + 96);    // [2][tile][4]
+  volatile int* s_fail = reinterpret_cast<int*>(smem + C::kOffMisc + 256);  // [group][item parity]
+  static_assert(sizeof(PreItem) <= 48 && kMaskedTiles == 4, "layout");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int kvh = blockIdx.x % p.kv_heads;
-  if (warp == 0) {
-    PreWork w = {0, 0, 0, 0, 0};
-    const bool any = find_work(p, blockIdx.x / p.kv_heads, w, err);
-    if (lane == 0) {
-      s_work[0] = any;
-      s_work[1] = w.q0;
-      s_work[2] = w.lq;
-      s_work[3] = w.k0;
-      s_work[4] = w.lk;
-      s_work[5] = w.t0;
-    }
-  }
-  if (tid == 32) {
+  if (tid == kLoadWarp * 32) {
+    prefetch_tensormap(&map_q);
+    prefetch_tensormap(&map_k);
+    prefetch_tensormap(&map_v);
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(&kv_full[i], 1);
       mbar_init(&kv_empty[i], 2);  // both MMA warps
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[2 * i], 128);
       mbar_init(&p_full[2 * i + 1], 128);
       mbar_init(&o_full[i], 1);
+      mbar_init(&turn[i], 1);
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], kConsumerWarps);
     }
     for (int i = 0; i < kMaskedTiles; ++i) mbar_init(&raw_full[i], 1);
     mbar_init(mma_done, 2);
-    mbar_init(&turn[0], 1);
-    mbar_init(&turn[1], 1);
+    mbar_init(block_full, 1);
     mbar_fence_init();
   }
+  if (tid < 6) s_fail[tid] = 0;
   if (warp == kMmaWarp) tmem_alloc(s_tmem, 512);
-  if (warp == kCleanWarp && lane < kMaskedTiles * 4) s_flags[lane] = 0u;
   tmem_fence_before_sync();
   __syncthreads();
   tmem_fence_after_sync();
   const uint32_t tmem = *s_tmem;
-  if (s_work[0]) {
-    const int q0 = s_work[1], lq = s_work[2], k0 = s_work[3], lk = s_work[4], t0 = s_work[5];
-    const int shift = lk - lq;  // key of token i under the causal mask: i + shift
-    // key tiles of each row tile: up to the last key that its last token sees
-    int n_tiles[2];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int first = t0 + x * p.tile_tokens;
-      const int last = min(first + p.tile_tokens, lq) - 1;
-      int keys = first < lq ? (p.causal ? min(max(last + shift + 1, 0), lk) : lk) : 0;
-      n_tiles[x] = (keys + kKeys - 1) / kKeys;
-    }
-    const int n = max(n_tiles[0], n_tiles[1]);
-    // tiles from here on hold keys that some row does not see
-    const int first_masked =
-        p.causal ? min(max(t0 + shift + 1, 0), lk) / kKeys : lk / kKeys;
 
-    if (warp >= 8) {
+  // ok: false in a thread whose wait gave up (bounded; then every wait of the grid
+  // gives up at once).  Such a thread goes through the rest of its item without
+  // waiting and without storing results, so that warps and named barriers stay
+  // whole, and its group leaves together at the next item.
+  bool ok = true;
+  auto wait = [&](uint64_t* bar, int phase) {
+    if (ok && !mbar_wait_short(bar, (uint32_t)phase & 1u, err)) {
+      record_error(err, kDevWaitTimeout);
+      ok = false;
+    }
+  };
+  // The K / V ring runs on over the items: load i of an item is ring use base + i.
+  int base = 0;
+  auto stage_of = [&](int i) { return (base + i) % C::kStages; };
+  // The next item, for a group of warps that share named barrier `bar`; false:
+  // leave, all of them.
+  auto next_item = [&](int k, int group, int bar, int threads) {
+    wait(&item_full[k & 1], k >> 1);
+    volatile int* fail = &s_fail[2 * group + (k & 1)];  // a fast thread may be an item ahead
+    if (!ok) *fail = 1;
+    named_barrier(bar, threads);
+    return !*fail && s_item[k & 1].kind != kStop;
+  };
+  auto item_done = [&](int k) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&item_empty[k & 1]);
+  };
+
+  if (warp >= 8) {
     // 256 x 200 + 256 x 56 = 65,536 = 512 x 128, the registers at launch
     registers_down<56>();
     if (warp == kLoadWarp) {
-      // ---- loads: the Q tiles, then K and V tiles in turn ----------------------
-      if (lane == 0 && n > 0) {
-        const uint64_t keep = l2_policy_evict_first();
-        for (int x = 0; x < 2; ++x) {
-          if (n_tiles[x] == 0) continue;
-          mbar_arrive_expect_tx(&q_full[x],
-                                (uint32_t)(C::kChunks * p.tile_tokens * p.group * 128));
-          for (int c = 0; c < C::kChunks; ++c)
-            tma_load_3d(smem + C::kOffQ + x * C::kTileBytes + c * kRows * 128, &map_q, &q_full[x],
-                        c * 64, kvh * p.group, q0 + t0 + x * p.tile_tokens, keep);
-        }
-        uint64_t hold;
-        asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(hold));
-        int i = 0;
-        bool ok = true;
-        for (int j = 0; j < n && ok; ++j) {
-          for (int kind = 0; kind < 2; ++kind, ++i) {
-            const int st = i % C::kStages;
-            if (!mbar_wait_bounded(&kv_empty[st], ((uint32_t)(i / C::kStages) & 1u) ^ 1u, err)) {
-              record_error(err, kDevWaitTimeout);
-              ok = false;
-              break;
-            }
+      // ---- items and loads ------------------------------------------------------------
+      // One CTA per SM takes one item after the other: its own block's, then those
+      // of blocks that have not started.  The next item's loads and its first
+      // product run during this one's epilogue.
+      const uint64_t once = l2_policy_evict_first(), hold = l2_policy_evict_last();
+      int q_loads[2] = {0, 0}, raw_loads = 0, k = 0;
+      int block = blockIdx.x;
+      auto publish = [&](const PreItem& w) {
+        if (k >= 2) wait(&item_empty[k & 1], (k >> 1) - 1);
+        if (lane < kMaskedTiles * 4) s_flags[(k & 1) * kMaskedTiles * 4 + lane] = 0u;
+        if (lane == 0) s_item[k & 1] = w;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&item_full[k & 1]);
+      };
+      auto ask = [&]() {
+        mbar_arrive_expect_tx(block_full, 16);
+        request_block(answer, block_full);
+      };
+      PreItem w = {};
+      for (; block >= 0 && ok; ++k) {
+        w.kvh = block % p.kv_heads;
+        w.kind = find_work(p, block / p.kv_heads, w.at, err) ? kSome : kNone;
+        if (w.kind == kNone) w.n = w.n_tiles[0] = w.n_tiles[1] = w.first_masked = 0;
+        else count_tiles(p, w);
+        publish(w);
+        if (lane == 0 && w.n > 0) {
+          auto load_kv = [&](int i) {
+            const int st = stage_of(i), j = i / 2, use = (base + i) / C::kStages;
+            if (use > 0) wait(&kv_empty[st], use - 1);
+            if (!ok) return;
             // a V tile with masked keys goes through the cleaning warps, which
             // complete kv_full in the load's place
-            uint64_t* bar =
-                kind == 1 && j >= first_masked ? &raw_full[j - first_masked] : &kv_full[st];
+            uint64_t* bar = (i & 1) && j >= w.first_masked
+                                ? &raw_full[raw_loads++ % kMaskedTiles] : &kv_full[st];
             mbar_arrive_expect_tx(bar, C::kTileBytes);
             for (int c = 0; c < C::kChunks; ++c)
               tma_load_3d(smem + C::kOffKV + st * C::kTileBytes + c * kKeys * 128,
-                          kind ? &map_v : &map_k, bar, c * 64, kvh, k0 + j * kKeys, hold);
+                          (i & 1) ? &map_v : &map_k, bar, c * 64, w.kvh, w.at.k0 + j * kKeys, hold);
+          };
+          int done = 0;
+          load_kv(done++);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (w.n_tiles[x] == 0) continue;
+            if (q_loads[x] > 0) wait(&q_empty[x], q_loads[x] - 1);
+            if (!ok) continue;
+            mbar_arrive_expect_tx(&q_full[x], (uint32_t)(C::kChunks * p.tile_tokens * p.group * 128));
+            for (int c = 0; c < C::kChunks; ++c)
+              tma_load_3d(smem + C::kOffQ + x * C::kTileBytes + c * kRows * 128, &map_q, &q_full[x],
+                          c * 64, w.kvh * p.group, w.at.q0 + w.at.t0 + x * p.tile_tokens, once);
+            ++q_loads[x];
           }
+          while (done < 2 * w.n && ok) {
+            // early enough to be answered by the end of the loads, late enough to
+            // leave the work to the CTA that is free first
+            if (done == max(2 * w.n - 2 * C::kStages, 1)) ask();
+            load_kv(done++);
+          }
+          base += done;
         }
-        drain_ring(kv_full, C::kStages, i);  // no copy outlives the CTA
-        for (int f = 0; 2 * (first_masked + f) + 1 < i; ++f) mbar_drain(&raw_full[f], 0);
+        if (lane == 0) {
+          if (w.n == 0) ask();
+          wait(block_full, k);
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        block = ok ? granted_block(answer) : -1;
+        fence_proxy_async_smem();  // the answer is read before the next one is written
+        __syncwarp();
+      }
+      w.kind = kStop;
+      if (ok) publish(w);
+      // no copy and no release outlives the CTA
+      if (lane == 0) {
+        drain_ring(kv_full, C::kStages, base);
+        drain_ring(kv_empty, C::kStages, base);
+        for (int f = max(raw_loads - kMaskedTiles, 0); f < raw_loads; ++f)
+          mbar_drain(&raw_full[f % kMaskedTiles], (uint32_t)(f / kMaskedTiles) & 1u);
+#pragma unroll
         for (int x = 0; x < 2; ++x)
-          if (n_tiles[x] > 0) mbar_drain(&q_full[x], 0);
+          if (q_loads[x] > 0) {
+            mbar_drain(&q_full[x], (uint32_t)(q_loads[x] - 1) & 1u);
+            mbar_drain(&q_empty[x], (uint32_t)(q_loads[x] - 1) & 1u);
+          }
       }
     } else if (warp < kCleanWarp) {
       // ---- MMA issue: a warp for each row tile, in strict turns -----------------------
@@ -304,74 +411,81 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       // passed on before a step's last MMAs, to cover its own latency.  Without
       // turns the tiles fall into step, and first their exponentials compete, then
       // their products.
-      if (n > 0) {
-        constexpr uint32_t kIdQK = umma_f16_idesc(kBf16, 0, kRows, kKeys);
-        constexpr uint32_t kIdPV = umma_f16_idesc(kBf16, 1, kRows, DP);
-        const int x = warp - kMmaWarp;
-        const int nt = n_tiles[x];
-        const uint32_t kv = smem_u32(smem + C::kOffKV);
-        const uint64_t q_desc =
-            umma_sw128_desc(smem_u32(smem + C::kOffQ + x * C::kTileBytes), 16, 1024);
-        const uint64_t k_desc = umma_sw128_desc(kv, 16, 1024);
-        const uint64_t v_desc = umma_sw128_desc(kv, kKeys * 128, 1024);
-        const uint32_t s_col = tmem + C::kSCol + x * 128, o_col = tmem + C::kOCol + x * 128;
-        bool ok = true;
-        auto wait = [&](uint64_t* bar, uint32_t parity) {
-          if (ok && !mbar_wait_short(bar, parity, err)) {
-            record_error(err, kDevWaitTimeout);
-            ok = false;
-          }
-        };
-        auto wait_load = [&](int i) {
-          wait(&kv_full[i % C::kStages], (uint32_t)(i / C::kStages) & 1u);
-        };
-        auto stage_of = [&](int i) { return (uint32_t)(i % C::kStages) * C::kTileBytes; };
-        // Both warps release a stage, each after it saw the load, and only if a
-        // later load reuses the stage.
-        auto release = [&](int i) {
-          if (i + C::kStages < 2 * n) umma_commit_warp(&kv_empty[i % C::kStages]);
-        };
-        auto pass_turn = [&]() {
-          if (lane == 0) mbar_arrive(&turn[x ^ 1]);
-          __syncwarp();
-        };
-        auto qk = [&](int j, bool pass) {
-          const uint64_t b = umma_desc_at(k_desc, stage_of(2 * j));
+      constexpr uint32_t kIdQK = umma_f16_idesc(kBf16, 0, kRows, kKeys);
+      constexpr uint32_t kIdPV = umma_f16_idesc(kBf16, 1, kRows, DP);
+      const int x = warp - kMmaWarp;
+      const uint32_t kv = smem_u32(smem + C::kOffKV);
+      const uint64_t q_desc =
+          umma_sw128_desc(smem_u32(smem + C::kOffQ + x * C::kTileBytes), 16, 1024);
+      const uint64_t k_desc = umma_sw128_desc(kv, 16, 1024);
+      const uint64_t v_desc = umma_sw128_desc(kv, kKeys * 128, 1024);
+      const uint32_t s_col = tmem + C::kSCol + x * 128, o_col = tmem + C::kOCol + x * 128;
+      // both warps release a stage, each after it saw the load
+      auto release = [&](int i) { umma_commit_warp(&kv_empty[stage_of(i)]); };
+      auto pass_turn = [&]() {
+        if (lane == 0) mbar_arrive(&turn[x ^ 1]);
+        __syncwarp();
+      };
+      auto qk = [&](int j, bool last, bool pass) {
+        const uint64_t b = umma_desc_at(k_desc, (uint32_t)stage_of(2 * j) * C::kTileBytes);
 #pragma unroll
-          for (int kk = 0; kk < DP / 16; ++kk) {
-            const uint32_t off = (uint32_t)(kk / 4) * (kKeys * 128) + (uint32_t)(kk % 4) * 32;
-            umma_f16_warp(s_col, umma_desc_at(q_desc, off), umma_desc_at(b, off), kIdQK, kk > 0);
-            if (kk == DP / 16 - kEarly && pass) pass_turn();
-          }
-          umma_commit_warp(&s_full[x]);
-        };
-        wait_load(0);
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const uint32_t off = (uint32_t)(kk / 4) * (kKeys * 128) + (uint32_t)(kk % 4) * 32;
+          umma_f16_warp(s_col, umma_desc_at(q_desc, off), umma_desc_at(b, off), kIdQK, kk > 0);
+          if (kk == DP / 16 - kEarly && pass) pass_turn();
+        }
+        umma_commit_warp(&s_full[x]);
+        if (last) umma_commit_warp(&q_empty[x]);
+      };
+      int q_uses = 0, p_uses = 0, steps = 0;
+      // a warp's lanes give up together
+      auto wait_warp = [&](uint64_t* bar, int phase) {
+        wait(bar, phase);
+        ok = __all_sync(0xffffffffu, ok);
+      };
+      auto wait_load_warp = [&](int i) {
+        wait_warp(&kv_full[stage_of(i)], (base + i) / C::kStages);
+      };
+      for (int k = 0;; ++k) {
+        wait_warp(&item_full[k & 1], k >> 1);
+        if (!ok) break;
+        const PreItem* item = &s_item[k & 1];
+        const int nt = x ? item->n_tiles[1] : item->n_tiles[0], n = item->n;
+        const bool stop = item->kind == kStop;
+        item_done(k);
+        if (stop) break;
+        if (n == 0) continue;
+        wait_load_warp(0);
         if (nt > 0) {
-          wait(&q_full[x], 0);
+          wait_warp(&q_full[x], q_uses++);
           tmem_fence_after_sync();
-          if (ok) qk(0, false);
+          if (ok) qk(0, nt == 1, false);  // S is free: the last P V ran before
         }
         release(0);
-        for (int j = 0; j < n && ok; ++j) {
-          wait_load(2 * j + 1);
-          if (j + 1 < n) wait_load(2 * j + 2);
-          if (x == 1 || j > 0) wait(&turn[x], (uint32_t)(x == 1 ? j : j - 1) & 1u);
-          if (j < nt) wait(&p_full[2 * x], (uint32_t)j & 1u);
+        for (int j = 0; j < n && ok; ++j, ++steps) {
+          wait_load_warp(2 * j + 1);
+          if (j + 1 < n) wait_load_warp(2 * j + 2);
+          if (x == 1 || steps > 0) wait_warp(&turn[x], x == 1 ? steps : steps - 1);
+          // (P of a new item also says that its rows' last results are read from O)
+          if (j < nt) wait_warp(&p_full[2 * x], p_uses);
           tmem_fence_after_sync();
           if (!ok) break;
           if (j < nt) {
-            const uint64_t b = umma_desc_at(v_desc, stage_of(2 * j + 1));
+            const uint64_t b = umma_desc_at(v_desc, (uint32_t)stage_of(2 * j + 1) * C::kTileBytes);
 #pragma unroll
             for (int kk = 0; kk < kKeys / 16; ++kk) {
               if (kk == kPart / 16) {
-                wait(&p_full[2 * x + 1], (uint32_t)j & 1u);
+                wait_warp(&p_full[2 * x + 1], p_uses);
                 tmem_fence_after_sync();
+                if (!ok) break;
               }
               umma_f16_ta_warp(o_col, s_col + kk * 8, umma_desc_at(b, kk * 2048), kIdPV,
                                (j > 0 || kk > 0) ? 1u : 0u);
             }
+            if (!ok) break;
+            ++p_uses;
             if (j == nt - 1) umma_commit_warp(&o_full[x]);
-            if (j + 1 < nt) qk(j + 1, true);  // over P (j): a warp's MMAs run in order
+            if (j + 1 < nt) qk(j + 1, j + 2 == nt, true);  // over P (j): a warp's MMAs run in order
             else pass_turn();
           } else {
             pass_turn();
@@ -379,73 +493,90 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           release(2 * j + 1);
           if (j + 1 < n) release(2 * j + 2);
         }
-        umma_commit_warp(mma_done);
-        mbar_drain(mma_done, 0);  // every MMA is done before tensor memory is freed
+        base += 2 * n;
       }
+      umma_commit_warp(mma_done);
+      mbar_drain(mma_done, 0);  // every MMA is done before tensor memory is freed
     } else {
       // ---- V tiles with masked keys ----------------------------------------------
       const int ct = tid - kCleanWarp * 32;
-      bool ok = true;
-      for (int j = first_masked; j < n; ++j) {
-        const int i = 2 * j + 1;
-        if (ok && !mbar_wait_bounded(&raw_full[j - first_masked], 0, err)) {
-          record_error(err, kDevWaitTimeout);
-          ok = false;
-        }
-        if (ok) {
-          uint8_t* tile = smem + C::kOffKV + (i % C::kStages) * C::kTileBytes;
-          const int valid = min(lk - j * kKeys, kKeys);
-          for (int r = ct; r < C::kChunks * kKeys; r += kCleaners) {  // a 128-byte row each
-            const int key = r % kKeys;
-            uint4* row = reinterpret_cast<uint4*>(tile + r * 128);
-            if (key >= valid) {
+      int cleaned = 0;
+      for (int k = 0; next_item(k, 2, 1, kCleaners); ++k) {
+        const PreItem& w = s_item[k & 1];
+        const int n = w.n, first_masked = w.first_masked, lk = w.at.lk;
+        uint32_t* flags = s_flags + (k & 1) * kMaskedTiles * 4;
+        for (int j = first_masked; j < n; ++j, ++cleaned) {
+          wait(&raw_full[cleaned % kMaskedTiles], cleaned / kMaskedTiles);
+          if (ok) {
+            uint8_t* tile = smem + C::kOffKV + stage_of(2 * j + 1) * C::kTileBytes;
+            const int valid = min(lk - j * kKeys, kKeys);
+            for (int r = ct; r < C::kChunks * kKeys; r += kCleaners) {  // a 128-byte row each
+              const int key = r % kKeys;
+              uint4* row = reinterpret_cast<uint4*>(tile + r * 128);
+              if (key >= valid) {
 #pragma unroll
-              for (int u = 0; u < 8; ++u) row[u] = make_uint4(0, 0, 0, 0);
-              continue;
+                for (int u = 0; u < 8; ++u) row[u] = make_uint4(0, 0, 0, 0);
+                continue;
+              }
+              uint32_t any = 0u;
+#pragma unroll
+              for (int u = 0; u < 8; ++u) {
+                const uint4 v = row[(u + r) & 7];  // lanes on different banks
+                any |= times_zero(v.x, T()) | times_zero(v.y, T()) | times_zero(v.z, T()) |
+                       times_zero(v.w, T());
+              }
+              if ((any & 0x7fff7fffu) == 0u) continue;  // every value finite
+              for (int u = 0; u < 8; ++u) {
+                uint4 v = row[u];
+                v.x &= ~nonfinite_mask(v.x, T());
+                v.y &= ~nonfinite_mask(v.y, T());
+                v.z &= ~nonfinite_mask(v.z, T());
+                v.w &= ~nonfinite_mask(v.w, T());
+                row[u] = v;
+              }
+              atomicOr(&flags[(j - first_masked) * 4 + key / 32], 1u << (key & 31));
             }
-            uint4 w[8];
-            uint32_t any = 0u;
-#pragma unroll
-            for (int u = 0; u < 8; ++u) w[u] = row[(u + r) & 7];  // lanes on different banks
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-              any |= times_zero(w[u].x, T()) | times_zero(w[u].y, T()) |
-                     times_zero(w[u].z, T()) | times_zero(w[u].w, T());
-            if ((any & 0x7fff7fffu) == 0u) continue;  // every value finite
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-              row[(u + r) & 7] = make_uint4(w[u].x & ~nonfinite_mask(w[u].x, T()),
-                                            w[u].y & ~nonfinite_mask(w[u].y, T()),
-                                            w[u].z & ~nonfinite_mask(w[u].z, T()),
-                                            w[u].w & ~nonfinite_mask(w[u].w, T()));
-            atomicOr(&s_flags[(j - first_masked) * 4 + key / 32], 1u << (key & 31));
+            fence_proxy_async_smem();  // an MMA operand
           }
-          fence_proxy_async_smem();  // an MMA operand
+          named_barrier(1, kCleaners);
+          if (ct == 0) mbar_arrive(&kv_full[stage_of(2 * j + 1)]);
         }
-        named_barrier(1, kCleaners);
-        if (ct == 0) mbar_arrive(&kv_full[i % C::kStages]);
+        base += 2 * n;
+        item_done(k);
       }
     }
-    } else {
-      registers_up<200>();
-      // ---- softmax and epilogue: thread = row ---------------------------------------
-      const int x = warp >> 2;
-      const int row = tid & 127;
-      const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-      const uint32_t s_addr = tmem + lanes + C::kSCol + x * 128;
-      const uint32_t o_addr = tmem + lanes + C::kOCol + x * 128;
-      const int tok = t0 + x * p.tile_tokens + row / p.group;  // in the sequence
-      const bool valid = row < p.tile_tokens * p.group && tok < lq;
-      // keys below `limit` are seen
-      const int limit = valid ? (p.causal ? min(tok + shift + 1, lk) : lk) : 0;
+  } else {
+    registers_up<200>();
+    // ---- softmax and epilogue: thread = row ---------------------------------------
+    const int x = warp >> 2;
+    const int row = tid & 127;
+    const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+    const uint32_t s_addr = tmem + lanes + C::kSCol + x * 128;
+    const uint32_t o_addr = tmem + lanes + C::kOCol + x * 128;
+    const int row_tok = row / p.group;
+    const uint32_t inv_group = (65536u + p.group - 1) / p.group;  // exact below 128 * 128
+    int s_uses = 0, o_uses = 0;
+    for (int k = 0; next_item(k, x, 2 + x, 128); ++k) {
+      // Its fields are read where they are needed: the loop below has no register
+      // to spare.
+      const PreItem& w = s_item[k & 1];
+      if (w.kind == kNone) {
+        item_done(k);
+        continue;
+      }
+      const int nt = x ? w.n_tiles[1] : w.n_tiles[0];
+      // keys below `limit` are seen; columns of tiles from `first_masked` on are tested
+      const int first_masked = w.first_masked;
+      int limit = 0;
+      bool valid;
+      {
+        const int tok = w.at.t0 + x * p.tile_tokens + row_tok, lq = w.at.lq, lk = w.at.lk;
+        valid = row_tok < p.tile_tokens && tok < lq;
+        if (valid) limit = p.causal ? min(tok + lk - lq + 1, lk) : lk;
+      }
       float m = -INFINITY, l = 0.0f;
-      const int nt = n_tiles[x];
-      bool ok = true;
       for (int j = 0; j < nt; ++j) {
-        if (ok && !mbar_wait_short(&s_full[x], (uint32_t)j & 1u, err)) {
-          record_error(err, kDevWaitTimeout);
-          ok = false;
-        }
+        wait(&s_full[x], s_uses++);
         __syncwarp();
         tmem_fence_after_sync();
         float s[kKeys];
@@ -481,15 +612,15 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           const float alpha = move ? exp2_approx((m - t) * p.scale_log2) : 1.0f;
           if (move) m = t;
           l *= alpha;
-          if (j > 0) {
-#pragma unroll
-            for (int c = 0; c < DP; c += 32) {
-              uint32_t o[32];
-              tmem_load<32>(o_addr + c, o);
+          if (j > 0) {  // seldom: small pieces, since the scores are in registers
+#pragma unroll 1
+            for (int c = 0; c < DP; c += 16) {
+              uint32_t o[16];
+              tmem_load<16>(o_addr + c, o);
               tmem_wait_load();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-              tmem_store<32>(o_addr + c, o);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_store<16>(o_addr + c, o);
             }
           }
         }
@@ -519,51 +650,76 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         l += l2.x + l2.y;
       }
       if (nt > 0) {
-        if (ok && !mbar_wait_bounded(&o_full[x], 0, err)) record_error(err, kDevWaitTimeout);
+        wait(&o_full[x], o_uses++);
         __syncwarp();
         tmem_fence_after_sync();
       }
       const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-      uint32_t flags = 0u;
-      for (int f = 0; f < kMaskedTiles * 4; ++f) flags |= s_flags[f];
-      const int64_t out_row = ((int64_t)(q0 + tok) * p.heads + kvh * p.group + row % p.group);
-      T* out = static_cast<T*>(p.out) + out_row * p.dim;
+      const uint32_t* flags = s_flags + (k & 1) * kMaskedTiles * 4;
+      uint32_t flagged = 0u;
+      if (first_masked < w.n)
+        for (int f = 0; f < kMaskedTiles * 4; ++f) flagged |= flags[f];
+      // The rows leave in whole lines, 64 channels at a time, through a buffer
+      // whose 16-byte pieces are swizzled against bank conflicts.
+      uint8_t* stage = smem + C::kOffOut + x * C::kStageBytes;
+      uint8_t* mine = stage + row * 128;
+      const int tok0 = w.at.t0 + x * p.tile_tokens;
+      const int rows = min(p.tile_tokens, max(w.at.lq - tok0, 0)) * p.group;
+#pragma unroll 1
+      for (int c0 = 0; c0 < DP; c0 += 64) {
+        named_barrier(2 + x, 128);  // the buffer is free
+#pragma unroll 1
+        for (int c = c0; c < c0 + 64; c += 32) {
+          uint32_t o[32];
+          if (nt > 0) {
+            tmem_load<32>(o_addr + c, o);
+            tmem_wait_load();
+          }
+          const bool none = nt == 0 || l == 0.0f;
 #pragma unroll
-      for (int c = 0; c < DP; c += 32) {
-        uint32_t o[32];
-        if (nt > 0) {
-          tmem_load<32>(o_addr + c, o);
-          tmem_wait_load();
-        } else {
+          for (int e = 0; e < 32; e += 8) {
+            uint32_t r[4];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0u;
+            for (int u = 0; u < 4; ++u)
+              r[u] = none ? 0u : pack2(__uint_as_float(o[e + 2 * u]) * inv,
+                                       __uint_as_float(o[e + 2 * u + 1]) * inv, T());
+            *reinterpret_cast<uint4*>(mine + ((((c & 32) + e) / 8) ^ (row & 7)) * 16) =
+                make_uint4(r[0], r[1], r[2], r[3]);
+          }
         }
-        if (!valid) continue;
-        float f[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) f[e] = l == 0.0f ? 0.0f : __uint_as_float(o[e]) * inv;
-        if (flags != 0u) {  // non-finite values of keys that this row sees
-          for (int k = 0; k < kMaskedTiles * kKeys; ++k) {
-            const int key = first_masked * kKeys + k;
-            if (!(s_flags[k / 32] >> (k & 31) & 1u) || key >= limit) continue;
-            const T* vr = static_cast<const T*>(p.v) + (int64_t)(k0 + key) * p.v_tok +
-                          (int64_t)kvh * p.v_head + c;
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const float v = c + e < p.dim ? widen(vr[e]) : 0.0f;
-              if (!isfinite(v)) f[e] += v;
+        if (flagged != 0u && valid) {  // non-finite values of keys that this row sees
+#pragma unroll 1
+          for (int i = 0; i < kMaskedTiles * kKeys; ++i) {
+            const int key = first_masked * kKeys + i;
+            if (!(flags[i / 32] >> (i & 31) & 1u) || key >= limit) continue;
+            const T* vr = static_cast<const T*>(p.v) + (int64_t)(w.at.k0 + key) * p.v_tok +
+                          (int64_t)w.kvh * p.v_head;
+#pragma unroll 1
+            for (int d = c0; d < min(c0 + 64, p.dim); ++d) {
+              const float v = widen(vr[d]);
+              if (isfinite(v)) continue;
+              T* at = reinterpret_cast<T*>(mine + (((d & 63) / 8) ^ (row & 7)) * 16) + (d & 7);
+              const uint32_t sum = pack2(widen(*at) + v, 0.0f, T());
+              *reinterpret_cast<uint16_t*>(at) = (uint16_t)sum;
             }
           }
         }
-#pragma unroll
-        for (int e = 0; e < 32; e += 8)
-          if (c + e < p.dim)
-            *reinterpret_cast<uint4*>(out + c + e) =
-                make_uint4(pack2(f[e], f[e + 1], T()), pack2(f[e + 2], f[e + 3], T()),
-                           pack2(f[e + 4], f[e + 5], T()), pack2(f[e + 6], f[e + 7], T()));
+        named_barrier(2 + x, 128);
+        const int piece = row & 7;
+        if (ok && c0 + piece * 8 < p.dim)
+          for (int r = row >> 3; r < rows; r += 16) {
+            const int rt = (int)(((uint32_t)r * inv_group) >> 16);
+            const int64_t to = (int64_t)(w.at.q0 + tok0 + rt) * p.heads + w.kvh * p.group +
+                               (r - rt * p.group);
+            *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + to * p.dim + c0 + piece * 8) =
+                *reinterpret_cast<const uint4*>(stage + r * 128 + (piece ^ (r & 7)) * 16);
+          }
       }
-      if (valid && p.lse != nullptr)
-        p.lse[out_row] = l == 0.0f ? -INFINITY : fmaf(m, p.scale, logf(l));
+      if (ok && valid && p.lse != nullptr)
+        p.lse[(int64_t)(w.at.q0 + tok0 + row_tok) * p.heads + w.kvh * p.group + row -
+              row_tok * p.group] =
+            l == 0.0f ? -INFINITY : fmaf(m, p.scale, logf(l));
+      item_done(k);
     }
   }
   tmem_fence_before_sync();

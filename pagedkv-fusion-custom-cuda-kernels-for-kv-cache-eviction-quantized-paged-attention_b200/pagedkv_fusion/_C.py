@@ -96,6 +96,7 @@ _DTYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 # library again and retries once, so the environment is not read per call.
 _FUSED_WS_CACHE: dict = {}
 _SELECT_WS_CACHE: dict = {}
+_PREFIX_WS_CACHE: dict = {}
 _ERR_WORKSPACE = 3
 
 
@@ -706,13 +707,22 @@ def shared_prefix_attention(q, k_cache_q, k_scale, v_cache_q, v_scale, prefix_ta
     sl, pl = _as_contiguous(seq_lens, torch.int32), _as_contiguous(prefix_len, torch.int32)
     out = torch.empty((S, H, D), dtype=_F32, device=q.device)
     P, M = pt.shape[0], bt.shape[1]
+    key = (S, H, Hkv, D, bs, NB, P, M)
+    nbytes = _PREFIX_WS_CACHE.get(key)
+    if nbytes is None:
+        if len(_PREFIX_WS_CACHE) >= 1024:  # a serving loop meets ever new table widths
+            _PREFIX_WS_CACHE.clear()
+        nbytes = _PREFIX_WS_CACHE[key] = _prefix_ws(*key)
     with _on_device(dev):
-        nbytes = _prefix_ws(S, H, Hkv, D, bs, NB, P, M)
-        ws, wp = _workspace(nbytes, q.device)
-        rc = _fast.shared_prefix_attention(
-            qc.data_ptr(), kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(),
-            pt.data_ptr(), pl.data_ptr(), bt.data_ptr(), sl.data_ptr(), out.data_ptr(), S, H, Hkv,
-            D, bs, NB, P, M, float(sm_scale), wp, nbytes, _raw_stream(dev))
+        for attempt in (0, 1):
+            ws, wp = _workspace(nbytes, q.device)
+            rc = _fast.shared_prefix_attention(
+                qc.data_ptr(), kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(),
+                pt.data_ptr(), pl.data_ptr(), bt.data_ptr(), sl.data_ptr(), out.data_ptr(), S, H,
+                Hkv, D, bs, NB, P, M, float(sm_scale), wp, nbytes, _raw_stream(dev))
+            if rc != _ERR_WORKSPACE or attempt:
+                break
+            nbytes = _PREFIX_WS_CACHE[key] = _prefix_ws(*key)  # the plan's switches changed
     if rc:
         _check(rc)
     return out
