@@ -14,7 +14,6 @@ this module fails with ``ImportError`` when that library has not been built.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes as ct
 from pathlib import Path
 
@@ -115,12 +114,23 @@ def _stream(t: torch.Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
-_SAME_DEVICE = contextlib.nullcontext()
+_current_device = torch._C._cuda_getDevice
 
 
-def _on_device(index: int):
-    """Makes device ``index`` the current one where it is not already."""
-    return _SAME_DEVICE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+def _call(fn, index: int, *args) -> None:
+    """``fn(*args)`` with device ``index`` current; raises on a nonzero status."""
+    if index == _current_device():
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args)
+    if rc:
+        _check(rc)
+
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor shaped like ``t``."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _check_inputs(*tensors) -> int:
@@ -542,31 +552,36 @@ def qk_norm_rope(q, k, positions, rotary, q_weight=None, k_weight=None, eps=1e-6
     table, pos = _check_rotary(rotary, positions, T, D)
     if (q_weight is None) != (k_weight is None) and k is not None:
         raise RuntimeError("q_weight and k_weight go together")
-    weights = [w for w in (q_weight, k_weight) if w is not None]
-    for i, w in enumerate(weights):
-        if not (w.dim() == 1 and w.shape[0] == D and (w.dtype is dt or w.dtype is _F32)
-                and w.dtype is weights[0].dtype):
-            raise RuntimeError("weights must be [head_dim], both float32 or of q's type")
-        weights[i] = w if w.is_contiguous() else w.contiguous()
+    qwp = kwp = None
+    w32 = 0
+    if q_weight is not None or k_weight is not None:
+        qw = q_weight if q_weight is not None else k_weight
+        kw = k_weight if k_weight is not None else q_weight
+        wdt = qw.dtype
+        for w in (qw, kw):
+            if w.dim() != 1 or w.shape[0] != D or w.dtype is not wdt or \
+                    not (wdt is dt or wdt is _F32):
+                raise RuntimeError("weights must be [head_dim], both float32 or of q's type")
+        if not qw.is_contiguous():
+            qw = qw.contiguous()
+        if not kw.is_contiguous():
+            kw = kw.contiguous()
+        qwp, kwp, w32 = qw.data_ptr(), kw.data_ptr(), 1 if wdt is _F32 else 0
     qc = _channels_last(q)
-    q_out = torch.empty((T, H, D), dtype=dt, device=q.device)
-    kp = kop = qwp = kwp = None
-    k_out, kt, kh = None, 0, 0
+    q_out = _like(q)
+    kp = kop = k_out = None
+    kt = kh = 0
     if k is not None:
-        k_out = torch.empty((T, Hkv, D), dtype=dt, device=q.device)
+        k_out = _like(k)
         if Hkv:
             kc = _channels_last(k)
-            kp, kop, kt, kh = kc.data_ptr(), k_out.data_ptr(), kc.stride(0), kc.stride(1)
-    if weights:
-        qwp, kwp = weights[0].data_ptr(), weights[-1].data_ptr()
-    with _on_device(dev):
-        rc = _fast.qk_norm_rope(
-            qc.data_ptr(), kp, _DTYPE_CODE[dt], q_out.data_ptr(), kop, pos.data_ptr(),
-            table.data_ptr(), qwp, kwp, 1 if weights and weights[0].dtype is _F32 else 0,
-            float(eps), T, H, Hkv, D, table.shape[1], table.shape[0], 1 if interleaved else 0,
-            qc.stride(0), qc.stride(1), kt, kh, _raw_stream(dev))
-    if rc:
-        _check(rc)
+            kt, kh, _ = kc.stride()
+            kp, kop = kc.data_ptr(), k_out.data_ptr()
+    qt, qh, _ = qc.stride()
+    rows, rot = table.shape
+    _call(_fast.qk_norm_rope, dev, qc.data_ptr(), kp, _DTYPE_CODE[dt], q_out.data_ptr(), kop,
+          pos.data_ptr(), table.data_ptr(), qwp, kwp, w32, float(eps), T, H, Hkv, D, rot, rows,
+          1 if interleaved else 0, qt, qh, kt, kh, _raw_stream(dev))
     return q_out, k_out
 
 
@@ -611,16 +626,13 @@ def append_kv(key, value, kv_cache_int8, scale_cache, slot_mapping, block_size: 
             pp, tp = pos.data_ptr(), table.data_ptr()
     kc, vc = _channels_last(key), _channels_last(value)
     slots = _as_contiguous(slot_mapping, torch.int64)
-    with _on_device(dev):
-        nbytes = _append_ws(T, NB)
-        ws, wp = _workspace(nbytes, key.device)
-        rc = _fast.append_kv(kc.data_ptr(), vc.data_ptr(), _DTYPE_CODE[dt],
-                             kv_cache_int8.data_ptr(), scale_cache.data_ptr(), slots.data_ptr(),
-                             pp, tp, T, NB, bs, Hkv, D, rot, rows, 1 if interleaved else 0,
-                             kc.stride(0), kc.stride(1), vc.stride(0), vc.stride(1), wp, nbytes,
-                             _raw_stream(dev))
-    if rc:
-        _check(rc)
+    nbytes = _append_ws(T, NB)
+    ws, wp = _workspace(nbytes, key.device)
+    kt, kh, _ = kc.stride()
+    vt, vh, _ = vc.stride()
+    _call(_fast.append_kv, dev, kc.data_ptr(), vc.data_ptr(), _DTYPE_CODE[dt],
+          kv_cache_int8.data_ptr(), scale_cache.data_ptr(), slots.data_ptr(), pp, tp, T, NB, bs,
+          Hkv, D, rot, rows, 1 if interleaved else 0, kt, kh, vt, vh, wp, nbytes, _raw_stream(dev))
 
 
 def _tma_rows(t: torch.Tensor) -> torch.Tensor:
@@ -654,16 +666,12 @@ def prefill_attention(q, k, v, cu_seqlens, sm_scale, cu_seqlens_k=None, causal=T
             raise RuntimeError("cu_seqlens must be int32 [num_seqs + 1]")
     cq, ck = cq.contiguous(), ck.contiguous()
     qc, kc, vc = _tma_rows(q), _tma_rows(k), _tma_rows(v)
-    out = torch.empty((Tq, H, D), dtype=dt, device=q.device)
+    out = _like(q)
     lse = torch.empty((Tq, H), dtype=_F32, device=q.device) if return_lse else None
-    with _on_device(dev):
-        rc = _fast.prefill_attention(
-            qc.data_ptr(), kc.data_ptr(), vc.data_ptr(), _DTYPE_CODE[dt], out.data_ptr(),
-            None if lse is None else lse.data_ptr(), cq.data_ptr(), ck.data_ptr(), n - 1, Tq, Tk,
-            H, Hkv, D, qc.stride(0), qc.stride(1), kc.stride(0), kc.stride(1), vc.stride(0),
-            vc.stride(1), float(sm_scale), 1 if causal else 0, _raw_stream(dev))
-    if rc:
-        _check(rc)
+    _call(_fast.prefill_attention, dev, qc.data_ptr(), kc.data_ptr(), vc.data_ptr(),
+          _DTYPE_CODE[dt], out.data_ptr(), None if lse is None else lse.data_ptr(), cq.data_ptr(),
+          ck.data_ptr(), n - 1, Tq, Tk, H, Hkv, D, *qc.stride()[:2], *kc.stride()[:2],
+          *vc.stride()[:2], float(sm_scale), 1 if causal else 0, _raw_stream(dev))
     return (out, lse) if return_lse else out
 
 
@@ -705,7 +713,7 @@ def shared_prefix_attention(q, k_cache_q, k_scale, v_cache_q, v_scale, prefix_ta
     ks, vs = _as_contiguous(k_scale, _F32), _as_contiguous(v_scale, _F32)
     bt, pt = _as_contiguous(block_tables, torch.int32), _as_contiguous(prefix_table, torch.int32)
     sl, pl = _as_contiguous(seq_lens, torch.int32), _as_contiguous(prefix_len, torch.int32)
-    out = torch.empty((S, H, D), dtype=_F32, device=q.device)
+    out = _like(q)
     P, M = pt.shape[0], bt.shape[1]
     key = (S, H, Hkv, D, bs, NB, P, M)
     nbytes = _PREFIX_WS_CACHE.get(key)
@@ -713,16 +721,18 @@ def shared_prefix_attention(q, k_cache_q, k_scale, v_cache_q, v_scale, prefix_ta
         if len(_PREFIX_WS_CACHE) >= 1024:  # a serving loop meets ever new table widths
             _PREFIX_WS_CACHE.clear()
         nbytes = _PREFIX_WS_CACHE[key] = _prefix_ws(*key)
-    with _on_device(dev):
-        for attempt in (0, 1):
-            ws, wp = _workspace(nbytes, q.device)
-            rc = _fast.shared_prefix_attention(
-                qc.data_ptr(), kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(),
-                pt.data_ptr(), pl.data_ptr(), bt.data_ptr(), sl.data_ptr(), out.data_ptr(), S, H,
-                Hkv, D, bs, NB, P, M, float(sm_scale), wp, nbytes, _raw_stream(dev))
-            if rc != _ERR_WORKSPACE or attempt:
-                break
-            nbytes = _PREFIX_WS_CACHE[key] = _prefix_ws(*key)  # the plan's switches changed
-    if rc:
-        _check(rc)
+    args = (qc.data_ptr(), kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(),
+            pt.data_ptr(), pl.data_ptr(), bt.data_ptr(), sl.data_ptr(), out.data_ptr(), S, H, Hkv,
+            D, bs, NB, P, M, float(sm_scale))
+
+    def launch(wp, nbytes, stream):  # the planner's switches may have changed: ask again once
+        rc = _fast.shared_prefix_attention(*args, wp, nbytes, stream)
+        if rc != _ERR_WORKSPACE:
+            return rc
+        need = _PREFIX_WS_CACHE[key] = _prefix_ws(*key)
+        again, ap = _workspace(need, q.device)
+        return _fast.shared_prefix_attention(*args, ap, need, stream)
+
+    ws, wp = _workspace(nbytes, q.device)
+    _call(launch, dev, wp, nbytes, _raw_stream(dev))
     return out
