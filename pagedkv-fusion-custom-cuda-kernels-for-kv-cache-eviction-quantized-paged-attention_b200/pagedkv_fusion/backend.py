@@ -21,8 +21,14 @@ What differs is underneath:
 * ``capture_decode`` returns an :class:`~pagedkv_fusion.ops.DecodePlan`
   for a CUDA-graph decode loop at a fixed batch shape.
 
-Like the reference, prefill steps go to the fallback backend; ``supports``
-tells a caller which decode shapes the kernels take.
+Like the reference, ``forward`` sends prefill steps to the fallback backend;
+``supports`` tells a caller which decode shapes the kernels take.  Beyond the
+reference's surface, for a caller that has its own model code:
+
+* ``prefill_forward`` is the prompt's attention over packed sequences;
+* ``append_to_cache`` rotates the keys on the way and keeps a started page's
+  earlier tokens readable (``write_to_cache`` replaces the page's scale);
+* ``shared_prefix_forward`` decodes a batch whose sequences share a prefix.
 """
 
 from __future__ import annotations
@@ -120,6 +126,59 @@ class PagedKVFusionBackend:
         plan's ``run()``."""
         return ops.DecodePlan(query, kv_cache_int8[0], scale_cache[0], kv_cache_int8[1],
                               scale_cache[1], metadata.block_tables, metadata.seq_lens, scale)
+
+    def prefill_forward(
+        self,
+        query: torch.Tensor,          # [total_q, num_heads, head_dim]
+        key: torch.Tensor,            # [total_k, num_kv_heads, head_dim]
+        value: torch.Tensor,
+        cu_seqlens: torch.Tensor,     # [num_seqs + 1] int32
+        scale: float,
+        cu_seqlens_k: torch.Tensor | None = None,
+    ) -> torch.Tensor:
+        """Causal attention of packed prompts (float16 / bfloat16): see
+        :func:`~pagedkv_fusion.ops.prefill_attention`."""
+        return ops.prefill_attention(query, key, value, cu_seqlens, scale,
+                                     cu_seqlens_k=cu_seqlens_k)
+
+    def append_to_cache(
+        self,
+        key: torch.Tensor,            # [num_tokens, num_kv_heads, head_dim]
+        value: torch.Tensor,
+        kv_cache_int8: torch.Tensor,  # [2, num_blocks, block_size, nkv, hd]
+        scale_cache: torch.Tensor,    # [2, num_blocks, num_kv_heads]
+        slot_mapping: torch.Tensor,   # [num_tokens] -> block * block_size + offset
+        block_size: int,
+        positions: torch.Tensor | None = None,
+        rotary: torch.Tensor | None = None,
+        interleaved: bool = False,
+    ) -> None:
+        """Rotates (with ``positions`` and ``rotary``), quantizes and appends
+        new tokens in place: see :func:`~pagedkv_fusion.ops.append_kv`."""
+        ops.append_kv(key, value, kv_cache_int8, scale_cache, slot_mapping, block_size,
+                      positions=positions, rotary=rotary, interleaved=interleaved)
+
+    def shared_prefix_forward(
+        self,
+        query: torch.Tensor,          # [num_seqs, num_heads, head_dim] float32
+        kv_cache_int8: torch.Tensor,  # [2, num_blocks, block_size, nkv, hd]
+        scale_cache: torch.Tensor,    # [2, num_blocks, num_kv_heads]
+        metadata: PagedKVFusionMetadata,
+        prefix_table: torch.Tensor,   # [prefix_blocks] int32, pages of the common prefix
+        prefix_len: torch.Tensor,     # one integer
+        scale: float,
+    ) -> torch.Tensor:
+        """``decode_forward`` for sequences behind a common prefix:
+        ``metadata`` describes their own tokens.  See
+        :func:`~pagedkv_fusion.ops.shared_prefix_attention`."""
+        return ops.shared_prefix_attention(
+            query,
+            kv_cache_int8[0], scale_cache[0],
+            kv_cache_int8[1], scale_cache[1],
+            prefix_table, prefix_len,
+            metadata.block_tables, metadata.seq_lens,
+            scale,
+        )
 
     def forward(self, *args, is_prefill: bool, **kwargs):
         """Prefill (and a build without the native library) goes to the
