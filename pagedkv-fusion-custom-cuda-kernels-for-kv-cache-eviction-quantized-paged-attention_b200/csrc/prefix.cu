@@ -70,6 +70,17 @@ struct PrefixCfg {
   static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 };
 
+// The tensor cores cut off the bits that an fp32 sum cannot hold, so a long sum
+// shrinks by about 2e-8 per product added (16 a tile; 4.1e-6 after 15 tiles).
+// Every few tiles O is therefore added to a sum of its own, rounded to nearest,
+// and started anew.  Where tensor memory has columns left (head_dim up to 64, or
+// one row tile) the sum is there and takes O every 2 tiles: 13,130 tokens, 8 rows a
+// head, head_dim 64 are then off by 9.3e-7 of the result (1.4e-6 at every 4) for 1%
+// of the time.  Else it is in global memory and takes O every 8: 32,768 tokens, 256
+// rows a head are off by 2.6e-6 in 79 us; 4.8e-6 in 74 us without sums, 1.6e-6 in
+// 85 us at every 4.
+constexpr int kFlushNear = 2, kFlushFar = 8;
+
 struct PrefixParams {
   const float* q;
   const int8_t* k_cache;
@@ -80,6 +91,7 @@ struct PrefixParams {
   const int32_t* prefix_len;  // [1]
   float* acc;                 // [splits][num_seqs * heads][dim]
   float2* ml;                 // [splits][num_seqs * heads]
+  float4* sums;               // per CTA and row tile: [DP / 4][128 rows], O of earlier tiles
   int64_t num_blocks;
   int num_seqs, heads, kv_heads, group, dim, bs, width, splits;
   float qk_scale;  // sm_scale log2e
@@ -140,7 +152,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   const int per_split = (tiles + p.splits - 1) / p.splits;
   const int tile0 = min(split * per_split, tiles);
   const int n = min(per_split, tiles - tile0);
-  const int two = pair * 256 + kRows < rows;  // the second row tile has rows
+  const bool two = pair * 256 + kRows < rows;  // the second row tile has rows
+  const bool near = DP == 64 || !two;          // see kFlushNear
+  const int flush = near ? kFlushNear : kFlushFar;
 
   if (tid == 0) {
     for (int i = 0; i < C::kStages; ++i) {
@@ -366,7 +380,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
             for (int half = 0; half < 2; ++half)
               umma_f16_ta_warp(o_col, s_col + (kk / 2) * 32 + half * 16 + (kk % 2) * 8,
                                umma_desc_at(b, kk * 2048), kIdPV,
-                               (j > 0 || kk > 0 || half > 0) ? 1u : 0u);
+                               (j % flush > 0 || kk > 0 || half > 0) ? 1u : 0u);
           }
           if (j == n - 1) umma_commit_warp(&o_full[x]);
           // the next K tile is converted while these run (its stage was V (j - 1)'s)
@@ -455,6 +469,12 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       fence_proxy_async_smem();  // an MMA operand
       mbar_arrive(&q_full[x]);
     }
+    // Warps without rows only keep the hand-offs going.
+    const bool busy = r - lane < rows;
+    const bool flushes = n > flush;
+    const uint32_t o2_addr = DP == 64 ? o_addr + 64 : tmem + lanes + C::kOCol + 128;
+    float4* sums = p.sums + (((int64_t)split * gridDim.x + blockIdx.x) * 2 + x) * (DP / 4) * kRows + row;
+    float since = 1.0f;  // by what O's unit has changed since `sums` was written
     float m = -INFINITY, l = 0.0f;  // m in units of S * k_scale * qk_scale
     bool ok = true;
     for (int j = 0; j < n; ++j) {
@@ -466,6 +486,42 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       }
       __syncwarp();
       tmem_fence_after_sync();
+      if (!busy) {
+        mbar_arrive(&p_full[2 * x]);
+        mbar_arrive(&p_full[2 * x + 1]);
+        continue;
+      }
+      if (j > 0 && j % flush == 0) {
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 16) {
+          alignas(16) uint32_t o[16], was[16];
+          tmem_load<16>(o_addr + c, o);
+          if (j == flush) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) was[e] = 0u;
+          } else if (near) {
+            tmem_load<16>(o2_addr + c, was);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<float4*>(&was[4 * e]) = sums[(c / 4 + e) * kRows];
+          }
+          tmem_wait_load();
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            o[e] = __float_as_uint(
+                fmaf(__uint_as_float(was[e]), since, __uint_as_float(o[e])));
+          if (near) {
+            tmem_store<16>(o2_addr + c, o);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              sums[(c / 4 + e) * kRows] = *reinterpret_cast<const float4*>(&o[4 * e]);
+          }
+        }
+        tmem_wait_store();
+        since = 1.0f;
+      }
       const float* ks = s_scale + slot * 2 * kKeys;
       const float* vs = ks + kKeys;
       const uint32_t* mask = s_mask + slot * 4;
@@ -520,15 +576,16 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         const float alpha = move ? ex2((m - t) * rf) : 1.0f;
         if (move) m = t;
         l *= alpha;
-        if (j > 0) {
-#pragma unroll
-          for (int c = 0; c < DP; c += 32) {
-            uint32_t o[32];
-            tmem_load<32>(o_addr + c, o);
+        since *= alpha;
+        if (j % flush != 0) {
+#pragma unroll 1
+          for (int c = 0; c < DP; c += 16) {
+            uint32_t o[16];
+            tmem_load<16>(o_addr + c, o);
             tmem_wait_load();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_store<32>(o_addr + c, o);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_store<16>(o_addr + c, o);
           }
         }
       }
@@ -594,20 +651,47 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       p.ml[slot_row] = ml;
     }
     if (n > 0) {
+      // The rows leave through the tile's query buffers (every product with them is
+      // done) in whole lines; 16-byte pieces are swizzled against bank conflicts.
+      uint8_t* stage = smem + C::kOffQ + 2 * x * C::kTileBytes;
+      if (busy) {
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 16) {
+          uint32_t o[16];
+          alignas(16) uint32_t was[16];
+          tmem_load<16>(o_addr + c, o);
+          if (!flushes) {
 #pragma unroll
-      for (int c = 0; c < DP; c += 32) {
-        uint32_t o[32];
-        tmem_load<32>(o_addr + c, o);
-        tmem_wait_load();
-        if (valid && c < p.dim) {
-          float4* dst = reinterpret_cast<float4*>(p.acc + slot_row * p.dim + c);
+            for (int e = 0; e < 16; ++e) was[e] = 0u;
+          } else if (near) {
+            tmem_load<16>(o2_addr + c, was);
+          } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            dst[e] = make_float4(__uint_as_float(o[4 * e]) * vmax, __uint_as_float(o[4 * e + 1]) * vmax,
-                                 __uint_as_float(o[4 * e + 2]) * vmax,
-                                 __uint_as_float(o[4 * e + 3]) * vmax);
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<float4*>(&was[4 * e]) = sums[(c / 4 + e) * kRows];
+          }
+          tmem_wait_load();
+          auto total = [&](int e) {
+            return fmaf(__uint_as_float(was[e]), since, __uint_as_float(o[e])) * vmax;
+          };
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<float4*>(stage + row * DP * 4 + (((c / 4 + e) ^ (row & 7)) * 16)) =
+                make_float4(total(4 * e), total(4 * e + 1), total(4 * e + 2), total(4 * e + 3));
         }
       }
+      __syncwarp();  // a warp writes out its own rows
+      constexpr int kPieces = DP / 4;
+      const int piece = lane % kPieces;
+      if (piece * 4 < p.dim)
+        for (int i = lane / kPieces; i < 32; i += 32 / kPieces) {
+          const int ri = r - lane + i, si = ri / p.group, rr = (warp & 3) * 32 + i;
+          if (ri >= rows) break;
+          const int64_t to = (int64_t)split * p.num_seqs * p.heads + (int64_t)si * p.heads +
+                             kvh * p.group + (ri - si * p.group);
+          *reinterpret_cast<float4*>(p.acc + to * p.dim + piece * 4) =
+              *reinterpret_cast<const float4*>(stage + rr * DP * 4 + ((piece ^ (rr & 7)) * 16));
+        }
     }
   }
   }
@@ -709,7 +793,7 @@ int prefix_splits(const SharedPrefixArgs& a) {
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 struct PrefixWs {
-  size_t pre_acc, pre_ml, own_acc, own_ml, bytes;
+  size_t pre_acc, pre_ml, own_acc, own_ml, sums, bytes;
   int splits, own_splits, own_pages;
 };
 
@@ -724,7 +808,14 @@ PrefixWs prefix_ws(const SharedPrefixArgs& a) {
   w.pre_ml = up256(pre * a.own.head_dim * sizeof(float));
   w.own_acc = w.pre_ml + up256(pre * sizeof(float2));
   w.own_ml = w.own_acc + up256(own * a.own.head_dim * sizeof(float));
-  w.bytes = w.own_ml + up256(own * sizeof(float2)) + 256;
+  w.sums = w.own_ml + up256(own * sizeof(float2));
+  const size_t ctas =
+      ((size_t)a.own.num_seqs * (a.own.num_heads / a.own.num_kv_heads) + 255) / 256 *
+      a.own.num_kv_heads * w.splits;
+  const size_t tiles = (size_t)a.prefix_width * a.own.block_size / kKeys + 1;
+  const bool far = a.own.head_dim > 64 && w.splits > 0 &&
+                   (tiles + w.splits - 1) / w.splits > (size_t)kFlushFar;
+  w.bytes = w.sums + (far ? ctas * 2 * kRows * 128 * sizeof(float) : 0) + 256;
   return w;
 }
 
@@ -770,6 +861,7 @@ int launch_shared_prefix(const SharedPrefixArgs& a, void* workspace, size_t work
     p.prefix_len = a.prefix_len;
     p.acc = pre_acc;
     p.ml = pre_ml;
+    p.sums = reinterpret_cast<float4*>(base + w.sums);
     p.num_blocks = o.num_blocks;
     p.num_seqs = o.num_seqs;
     p.heads = o.num_heads;
