@@ -609,11 +609,15 @@ __device__ __forceinline__ void copy16_async(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src)
                : "memory");
 }
+__device__ __forceinline__ void copies_group() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>  // all but the last N groups
 __device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Starts the copies of one head's rows; copies_wait() before append_head8.
+// Starts the copies of one head's rows.
 template <typename T>
 __device__ __forceinline__ void append_fetch8(const AppendArgs<T>& a, bool is_key, int h,
                                               const AppendList& list, T* raw) {
@@ -642,54 +646,50 @@ __device__ __forceinline__ void append_head8(const AppendArgs<T>& a, int64_t pag
   float* scale = a.scales + (is_key ? 0 : a.blocks * a.kv_heads) + page * a.kv_heads + h;
   const float old = lowest > 0 ? *scale : 0.0f;
 
+  // The lane's channels: two groups of 4, with the half layout a group and its
+  // partners, so that a rotation needs no other lane.
   const int half = a.rot / 2;
-  const bool first = d < half;
-  const int col = ROT == kPairs ? d / 2 : (first ? d : d - half);  // of the table row
+  const bool turned = ROT != kNoRotation && d < a.rot;  // whole pieces: rot % 8 = 0
+  const int d0 = ROT == kHalves && turned ? d / 2 : d;
+  const int d1 = ROT == kHalves && turned ? half + d / 2 : d + 4;
   auto values = [&](int i, float (&y)[8]) {
+    const Chunk<T, 4> x0 = load_chunk<T, 4>(raw + i * 128 + d0);
+    const Chunk<T, 4> x1 = load_chunk<T, 4>(raw + i * 128 + d1);
 #pragma unroll
-    for (int u = 0; u < 8 / kPer; ++u) {
-      const Chunk<T, kPer> x = load_chunk<T, kPer>(raw + i * 128 + d + u * kPer);
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) y[u * kPer + e] = to_f32<T>(x.e[e]);
+    for (int e = 0; e < 4; ++e) {
+      y[e] = to_f32<T>(x0.e[e]);
+      y[4 + e] = to_f32<T>(x1.e[e]);
     }
-    if (ROT == kNoRotation || d >= a.rot) return;  // whole pieces: rot % 16 = 0, or pairs
-    const float* row = table + i * 128 + col;
-    if constexpr (ROT == kHalves) {
-      const T* other = raw + i * 128 + (first ? d + half : d - half);
+    if (ROT == kNoRotation || !turned) return;
+    const float4 c = *reinterpret_cast<const float4*>(table + i * 128 + d / 2);
+    const float4 s = *reinterpret_cast<const float4*>(table + i * 128 + half + d / 2);
+    constexpr int kStep = ROT == kPairs ? 2 : 1;  // between the pairs' first values
+    constexpr int kOther = ROT == kPairs ? 1 : 4;
 #pragma unroll
-      for (int u = 0; u < 8; u += 4) {
-        alignas(16) float cc[4], ss[4];
-        *reinterpret_cast<float4*>(cc) = *reinterpret_cast<const float4*>(row + u);
-        *reinterpret_cast<float4*>(ss) = *reinterpret_cast<const float4*>(row + half + u);
-        const Chunk<T, 4> o = load_chunk<T, 4>(other + u);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p = to_f32<T>(o.e[e]);
-          y[u + e] = first ? rot_first(y[u + e], p, cc[e], ss[e])
-                           : rot_second(p, y[u + e], cc[e], ss[e]);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; e += 2)
-        if (d + e < a.rot) {
-          const float p = y[e], q = y[e + 1];
-          y[e] = rot_first(p, q, row[e / 2], row[half + e / 2]);
-          y[e + 1] = rot_second(p, q, row[e / 2], row[half + e / 2]);
-        }
+    for (int e = 0; e < 4; e += 2) {
+      float* f = &y[e * kStep];
+      const uint64_t cc = e == 0 ? f32x2(c.x, c.y) : f32x2(c.z, c.w);
+      const uint64_t ss = e == 0 ? f32x2(s.x, s.y) : f32x2(s.z, s.w);
+      const uint64_t u = f32x2(f[0], f[kStep]), v = f32x2(f[kOther], f[kOther + kStep]);
+      // Packed products, scalar sums: of packed products and a packed sum the
+      // assembler makes one fma, with one rounding less.
+      const float2 uc = unpack_f32x2(mul_f32x2(u, cc)), us = unpack_f32x2(mul_f32x2(u, ss));
+      const float2 vc = unpack_f32x2(mul_f32x2(v, cc)), vs = unpack_f32x2(mul_f32x2(v, ss));
+      f[0] = __fsub_rn(uc.x, vs.x), f[kStep] = __fsub_rn(uc.y, vs.y);
+      f[kOther] = __fadd_rn(vc.x, us.x), f[kOther + kStep] = __fadd_rn(vc.y, us.y);
     }
   };
-  uint32_t m = 0u;
+  float big = 0.0f;
   if (on)
 #pragma unroll 2
     for (int i = sub; i < n; i += 2) {
       float y[8];
       values(i, y);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(y[e]) & 0x7fffffffu);
+      for (int e = 0; e < 8; e += 2) big = max3_nan(big, fabsf(y[e]), fabsf(y[e + 1]));
     }
-  m = __reduce_max_sync(0xffffffffu, m);  // NaN bits exceed +inf: NaN wins
-  const float amax = __uint_as_float(m);
+  // NaN bits exceed +inf: NaN wins
+  const float amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
   const float sc = append_scale(amax, scale, old, lowest, head_base, tok_stride, a.dim, true);
   const float rcp = __frcp_rn(sc);
   const bool fast = isfinite(amax) && !isinf(rcp);
@@ -699,13 +699,20 @@ __device__ __forceinline__ void append_head8(const AppendArgs<T>& a, int64_t pag
       float y[8];
       values(i, y);
       const float lo[4] = {y[0], y[1], y[2], y[3]}, hi[4] = {y[4], y[5], y[6], y[7]};
-      *reinterpret_cast<uint2*>(head_base + list.off[i] * tok_stride + d) =
-          make_uint2(quantize_word(lo, sc, rcp, fast), quantize_word(hi, sc, rcp, fast));
+      int8_t* dst = head_base + list.off[i] * tok_stride;
+      const uint32_t w0 = quantize_word(lo, sc, rcp, fast), w1 = quantize_word(hi, sc, rcp, fast);
+      if constexpr (ROT == kHalves) {
+        *reinterpret_cast<uint32_t*>(dst + d0) = w0;
+        *reinterpret_cast<uint32_t*>(dst + d1) = w1;
+      } else {
+        *reinterpret_cast<uint2*>(dst + d) = make_uint2(w0, w1);
+      }
     }
 }
 
-// The heads of K, of V or of both by the CTA's warps.
-template <typename T, int VEC, int NC>
+// The heads of K, of V or of both by the CTA's warps.  With BUFS = 2 a warp's next
+// head is on its way while it works on one.
+template <typename T, int VEC, int NC, int BUFS>
 __device__ __forceinline__ void append_heads(const AppendArgs<T>& a, int64_t page, bool key_part,
                                              bool value_part, const AppendList& list) {
   const int rows = (key_part ? a.kv_heads : 0) + (value_part ? a.kv_heads : 0);
@@ -715,26 +722,40 @@ __device__ __forceinline__ void append_heads(const AppendArgs<T>& a, int64_t pag
   auto head = [&](int r) { return r < a.kv_heads ? r : r - a.kv_heads; };
   if (VEC == 8 && list.count <= kAppendHold) {
     extern __shared__ __align__(16) float s_rows[];  // table rows, then each warp's rows
-    T* raw = reinterpret_cast<T*>(s_rows + kAppendHold * 128) + warp * kAppendHold * 128;
+    T* raw = reinterpret_cast<T*>(s_rows + kAppendHold * 128) + warp * BUFS * kAppendHold * 128;
     if (key_part && turns)  // the tokens' table rows, once for all heads
       for (int i = threadIdx.x; i < list.count * 32; i += kAppendThreads) {
         const int tok = i / 32, at = (i % 32) * 4;
         if (at < a.rot) copy16_async(s_rows + tok * 128 + at, a.table + list.pos[tok] * a.rot + at);
       }
-    for (int r0 = 0; r0 < rows; r0 += kAppendWarps) {
-      const int r = r0 + warp;
-      if (r < rows) append_fetch8(a, is_key(r), head(r), list, raw);
-      copies_wait();
+    if (warp < rows) append_fetch8(a, is_key(warp), head(warp), list, raw);
+    copies_group();
+    for (int r0 = 0, buf = 0; r0 < rows; r0 += kAppendWarps) {
+      const int r = r0 + warp, next = r + kAppendWarps;
+      if (BUFS == 2) {
+        if (next < rows) append_fetch8(a, is_key(next), head(next), list, raw + (buf ^ 1) * kAppendHold * 128);
+        copies_group();
+        copies_wait<1>();
+      } else {
+        copies_wait<0>();
+      }
       if (r0 == 0) __syncthreads();  // the table rows are every warp's copies
       else __syncwarp();
       if (r >= rows) continue;
+      const T* rows_of = raw + buf * kAppendHold * 128;
       if (!is_key(r) || !turns)
-        append_head8<T, kNoRotation>(a, page, is_key(r), head(r), list, raw, s_rows);
+        append_head8<T, kNoRotation>(a, page, is_key(r), head(r), list, rows_of, s_rows);
       else if (a.interleaved)
-        append_head8<T, kPairs>(a, page, true, head(r), list, raw, s_rows);
+        append_head8<T, kPairs>(a, page, true, head(r), list, rows_of, s_rows);
       else
-        append_head8<T, kHalves>(a, page, true, head(r), list, raw, s_rows);
-      __syncwarp();  // the rows are free for the warp's next head
+        append_head8<T, kHalves>(a, page, true, head(r), list, rows_of, s_rows);
+      __syncwarp();  // the rows are free for another head
+      if (BUFS == 2) {
+        buf ^= 1;
+      } else if (next < rows) {
+        append_fetch8(a, is_key(next), head(next), list, raw);
+        copies_group();
+      }
     }
     return;
   }
@@ -773,7 +794,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_scan_kernel(AppendArgs<
   __syncthreads();
   if (s_taken) return;  // whole CTA
   append_list(a, s_tok, s_list);
-  append_heads<T, VEC, NC>(a, page, is_key, !is_key, s_list);
+  append_heads<T, VEC, NC, 1>(a, page, is_key, !is_key, s_list);
 }
 
 // Index of larger calls.  A run head (a token whose predecessor is not in the
@@ -797,6 +818,10 @@ __global__ void __launch_bounds__(256)
   if (prev == 0) pages[atomicAdd(count, 1)] = make_int2((int)page, (int)t);
 }
 
+// Three CTAs of an SM have 200 KB of rows on chip either way.
+template <typename T>
+constexpr int kAppendBufs = sizeof(T) == 2 ? 2 : 1;
+
 template <typename T, int VEC, int NC>
 __global__ void __launch_bounds__(kAppendThreads, VEC == 8 ? 3 : 1)
     append_pages_kernel(AppendArgs<T> a, const int* head, const int* next, const int2* pages,
@@ -817,11 +842,12 @@ __global__ void __launch_bounds__(kAppendThreads, VEC == 8 ? 3 : 1)
         for (int64_t t0 = start; t0 < a.tokens; t0 += 32) {
           const int64_t t = t0 + threadIdx.x;
           const int64_t slot = t < a.tokens ? append_slot(a, t, err) : -1;
-          const bool in = slot >= 0 && slot / a.bs == page;
+          const int64_t at = slot - page * a.bs;
+          const bool in = slot >= 0 && at >= 0 && at < a.bs;
           // the run ends at the first token of another page
           const unsigned out = __ballot_sync(0xffffffffu, !in);
           const int len = out == 0 ? 32 : __ffs(out) - 1;
-          if ((int)threadIdx.x < len) atomicMax(&s_tok[slot % a.bs], (int)t);
+          if ((int)threadIdx.x < len) atomicMax(&s_tok[at], (int)t);
           if (len < 32) break;
         }
         start = link - 1;
@@ -831,7 +857,7 @@ __global__ void __launch_bounds__(kAppendThreads, VEC == 8 ? 3 : 1)
     }
     __syncthreads();
     append_list(a, s_tok, s_list);
-    append_heads<T, VEC, NC>(a, page, true, true, s_list);
+    append_heads<T, VEC, NC, kAppendBufs<T>>(a, page, true, true, s_list);
   }
 }
 
@@ -840,13 +866,15 @@ constexpr int64_t kAppendScan = 512;
 
 template <typename T, int VEC, int NC>
 void launch_append_n(const AppendArgs<T>& a, int* ws, cudaStream_t stream) {
-  constexpr int kStage = VEC == 8 ? kAppendHold * 128 * (4 + kAppendWarps * (int)sizeof(T)) : 0;
+  auto stage = [](int bufs) {
+    return VEC == 8 ? kAppendHold * 128 * (4 + kAppendWarps * bufs * (int)sizeof(T)) : 0;
+  };
   int* err = device_error_word();
   if (a.tokens <= kAppendScan) {
     static std::atomic<uint64_t> done{0};
-    allow_shared_memory(reinterpret_cast<const void*>(append_scan_kernel<T, VEC, NC>), kStage, done);
+    allow_shared_memory(reinterpret_cast<const void*>(append_scan_kernel<T, VEC, NC>), stage(1), done);
     append_scan_kernel<T, VEC, NC>
-        <<<(unsigned)(2 * a.tokens), kAppendThreads, kStage, stream>>>(a, err);
+        <<<(unsigned)(2 * a.tokens), kAppendThreads, stage(1), stream>>>(a, err);
     return;
   }
   int* head = ws;
@@ -858,9 +886,9 @@ void launch_append_n(const AppendArgs<T>& a, int* ws, cudaStream_t stream) {
                                                                                  pages, count, err);
   const int64_t ctas = std::min<int64_t>(a.tokens, 8LL * 148);
   static std::atomic<uint64_t> done{0};
-  allow_shared_memory(reinterpret_cast<const void*>(append_pages_kernel<T, VEC, NC>), kStage, done);
+  allow_shared_memory(reinterpret_cast<const void*>(append_pages_kernel<T, VEC, NC>), stage(kAppendBufs<T>), done);
   append_pages_kernel<T, VEC, NC>
-      <<<(unsigned)ctas, kAppendThreads, kStage, stream>>>(a, head, next, pages, count, err);
+      <<<(unsigned)ctas, kAppendThreads, stage(kAppendBufs<T>), stream>>>(a, head, next, pages, count, err);
 }
 
 template <typename T>
@@ -893,7 +921,7 @@ int launch_append_t(const AppendKvArgs& p, int* ws, cudaStream_t stream) {
   // whole pieces are rotated, and table rows are read four values at a time
   const bool halves = a.rot > 0 && !a.interleaved;
   if (a.dim <= 128 && rows_of(8, 16) && aligned(a.cache, 8) &&
-      (a.rot == 0 || (a.rot % (halves ? 16 : 4) == 0 && aligned(a.table, 16))))
+      (a.rot % 8 == 0 && (a.rot == 0 || aligned(a.table, 16))))
     launch_append_n<T, 8, 1>(a, ws, stream);
   else if (rows_of(4, 4 * (int)sizeof(T)) && aligned(a.cache, 4) &&
            (!halves || (a.rot % 8 == 0 && aligned(a.table, 16))))
