@@ -14,6 +14,7 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "pkv_common.cuh"
 #include "pkv_internal.h"
@@ -602,9 +603,14 @@ __device__ __noinline__ void append_head(const AppendArgs<T>& a, int64_t page, b
 // pieces, half a warp per token (a warp's instruction serves two tokens).  All
 // rows of a head are copied to shared memory at once, so inputs are read once
 // and a warp has 4 KB in flight; the rotation is cheap enough to be done
-// again for the codes.  (Rows held in registers: one pair of tokens ahead left
-// each step waiting for HBM, all sixteen tokens spilled; 158 to 420 us for
-// 32,768 tokens of 8 heads against 108 us.)
+// again for the codes.  32,768 bf16 tokens of 8 heads in pages of 16: 79 us
+// (201 MB, 31 us at the copy rate), issue slots 61% busy -- bound by the
+// instructions for a value and the latencies of a page's steps (its tokens' list,
+// its rows, the maximum, the codes), which 24 warps an SM do not hide.  Slower were:
+// rows held in registers (one pair of tokens ahead left each step waiting for
+// HBM, all sixteen tokens spilled; 158 to 420 us); half a warp per token with all
+// heads, maxima exchanged by the CTA (135 us); the next page's list and rows read
+// ahead (95 us).
 __device__ __forceinline__ void copy16_async(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src)
                : "memory");
@@ -641,6 +647,7 @@ __device__ __forceinline__ void append_head8(const AppendArgs<T>& a, int64_t pag
   const int n = list.count, lowest = list.lowest;
   const bool on = d < a.dim;
   const int64_t tok_stride = (int64_t)a.kv_heads * a.dim;
+  const int stride32 = (int)tok_stride;
   int8_t* head_base = a.cache + (is_key ? 0 : a.blocks * a.bs * tok_stride) +
                       page * a.bs * tok_stride + (int64_t)h * a.dim;
   float* scale = a.scales + (is_key ? 0 : a.blocks * a.kv_heads) + page * a.kv_heads + h;
@@ -681,7 +688,7 @@ __device__ __forceinline__ void append_head8(const AppendArgs<T>& a, int64_t pag
   };
   float big = 0.0f;
   if (on)
-#pragma unroll 2
+#pragma unroll 4
     for (int i = sub; i < n; i += 2) {
       float y[8];
       values(i, y);
@@ -694,12 +701,12 @@ __device__ __forceinline__ void append_head8(const AppendArgs<T>& a, int64_t pag
   const float rcp = __frcp_rn(sc);
   const bool fast = isfinite(amax) && !isinf(rcp);
   if (on)
-#pragma unroll 2
+#pragma unroll 4
     for (int i = sub; i < n; i += 2) {
       float y[8];
       values(i, y);
       const float lo[4] = {y[0], y[1], y[2], y[3]}, hi[4] = {y[4], y[5], y[6], y[7]};
-      int8_t* dst = head_base + list.off[i] * tok_stride;
+      int8_t* dst = head_base + (int64_t)list.off[i] * stride32;
       const uint32_t w0 = quantize_word(lo, sc, rcp, fast), w1 = quantize_word(hi, sc, rcp, fast);
       if constexpr (ROT == kHalves) {
         *reinterpret_cast<uint32_t*>(dst + d0) = w0;
@@ -712,7 +719,7 @@ __device__ __forceinline__ void append_head8(const AppendArgs<T>& a, int64_t pag
 
 // The heads of K, of V or of both by the CTA's warps.  With BUFS = 2 a warp's next
 // head is on its way while it works on one.
-template <typename T, int VEC, int NC, int BUFS>
+template <typename T, int VEC, int NC, int HOLD, int BUFS>
 __device__ __forceinline__ void append_heads(const AppendArgs<T>& a, int64_t page, bool key_part,
                                              bool value_part, const AppendList& list) {
   const int rows = (key_part ? a.kv_heads : 0) + (value_part ? a.kv_heads : 0);
@@ -720,9 +727,9 @@ __device__ __forceinline__ void append_heads(const AppendArgs<T>& a, int64_t pag
   const bool turns = a.positions != nullptr;
   auto is_key = [&](int r) { return key_part && r < a.kv_heads; };
   auto head = [&](int r) { return r < a.kv_heads ? r : r - a.kv_heads; };
-  if (VEC == 8 && list.count <= kAppendHold) {
+  if (VEC == 8 && list.count <= HOLD) {
     extern __shared__ __align__(16) float s_rows[];  // table rows, then each warp's rows
-    T* raw = reinterpret_cast<T*>(s_rows + kAppendHold * 128) + warp * BUFS * kAppendHold * 128;
+    T* raw = reinterpret_cast<T*>(s_rows + HOLD * 128) + warp * BUFS * HOLD * 128;
     if (key_part && turns)  // the tokens' table rows, once for all heads
       for (int i = threadIdx.x; i < list.count * 32; i += kAppendThreads) {
         const int tok = i / 32, at = (i % 32) * 4;
@@ -733,7 +740,7 @@ __device__ __forceinline__ void append_heads(const AppendArgs<T>& a, int64_t pag
     for (int r0 = 0, buf = 0; r0 < rows; r0 += kAppendWarps) {
       const int r = r0 + warp, next = r + kAppendWarps;
       if (BUFS == 2) {
-        if (next < rows) append_fetch8(a, is_key(next), head(next), list, raw + (buf ^ 1) * kAppendHold * 128);
+        if (next < rows) append_fetch8(a, is_key(next), head(next), list, raw + (buf ^ 1) * HOLD * 128);
         copies_group();
         copies_wait<1>();
       } else {
@@ -742,7 +749,7 @@ __device__ __forceinline__ void append_heads(const AppendArgs<T>& a, int64_t pag
       if (r0 == 0) __syncthreads();  // the table rows are every warp's copies
       else __syncwarp();
       if (r >= rows) continue;
-      const T* rows_of = raw + buf * kAppendHold * 128;
+      const T* rows_of = raw + buf * HOLD * 128;
       if (!is_key(r) || !turns)
         append_head8<T, kNoRotation>(a, page, is_key(r), head(r), list, rows_of, s_rows);
       else if (a.interleaved)
@@ -794,7 +801,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_scan_kernel(AppendArgs<
   __syncthreads();
   if (s_taken) return;  // whole CTA
   append_list(a, s_tok, s_list);
-  append_heads<T, VEC, NC, 1>(a, page, is_key, !is_key, s_list);
+  append_heads<T, VEC, NC, kAppendHold, 1>(a, page, is_key, !is_key, s_list);
 }
 
 // Index of larger calls.  A run head (a token whose predecessor is not in the
@@ -818,12 +825,13 @@ __global__ void __launch_bounds__(256)
   if (prev == 0) pages[atomicAdd(count, 1)] = make_int2((int)page, (int)t);
 }
 
-// Three CTAs of an SM have 200 KB of rows on chip either way.
-template <typename T>
-constexpr int kAppendBufs = sizeof(T) == 2 ? 2 : 1;
+// Rows on chip: two heads of 16 tokens a warp, or one of 32 (block_size up to 32),
+// in 16 bits.
+template <typename T, int HOLD>
+constexpr int kAppendBufs = sizeof(T) == 2 && HOLD == 16 ? 2 : 1;
 
-template <typename T, int VEC, int NC>
-__global__ void __launch_bounds__(kAppendThreads, VEC == 8 ? 3 : 1)
+template <typename T, int VEC, int NC, int HOLD>
+__global__ void __launch_bounds__(kAppendThreads, VEC == 8 ? (HOLD == 16 ? 3 : 2) : 1)
     append_pages_kernel(AppendArgs<T> a, const int* head, const int* next, const int2* pages,
                         const int* count, int* err) {
   __shared__ int s_tok[kAppendMaxPage];
@@ -857,7 +865,7 @@ __global__ void __launch_bounds__(kAppendThreads, VEC == 8 ? 3 : 1)
     }
     __syncthreads();
     append_list(a, s_tok, s_list);
-    append_heads<T, VEC, NC, kAppendBufs<T>>(a, page, true, true, s_list);
+    append_heads<T, VEC, NC, HOLD, kAppendBufs<T, HOLD>>(a, page, true, true, s_list);
   }
 }
 
@@ -866,15 +874,13 @@ constexpr int64_t kAppendScan = 512;
 
 template <typename T, int VEC, int NC>
 void launch_append_n(const AppendArgs<T>& a, int* ws, cudaStream_t stream) {
-  auto stage = [](int bufs) {
-    return VEC == 8 ? kAppendHold * 128 * (4 + kAppendWarps * bufs * (int)sizeof(T)) : 0;
-  };
+  constexpr int kStage = VEC == 8 ? kAppendHold * 128 * (4 + kAppendWarps * (int)sizeof(T)) : 0;
   int* err = device_error_word();
   if (a.tokens <= kAppendScan) {
     static std::atomic<uint64_t> done{0};
-    allow_shared_memory(reinterpret_cast<const void*>(append_scan_kernel<T, VEC, NC>), stage(1), done);
+    allow_shared_memory(reinterpret_cast<const void*>(append_scan_kernel<T, VEC, NC>), kStage, done);
     append_scan_kernel<T, VEC, NC>
-        <<<(unsigned)(2 * a.tokens), kAppendThreads, stage(1), stream>>>(a, err);
+        <<<(unsigned)(2 * a.tokens), kAppendThreads, kStage, stream>>>(a, err);
     return;
   }
   int* head = ws;
@@ -885,10 +891,20 @@ void launch_append_n(const AppendArgs<T>& a, int* ws, cudaStream_t stream) {
   append_index_kernel<T><<<(unsigned)((a.tokens + 255) / 256), 256, 0, stream>>>(a, head, next,
                                                                                  pages, count, err);
   const int64_t ctas = std::min<int64_t>(a.tokens, 8LL * 148);
-  static std::atomic<uint64_t> done{0};
-  allow_shared_memory(reinterpret_cast<const void*>(append_pages_kernel<T, VEC, NC>), stage(kAppendBufs<T>), done);
-  append_pages_kernel<T, VEC, NC>
-      <<<(unsigned)ctas, kAppendThreads, stage(kAppendBufs<T>), stream>>>(a, head, next, pages, count, err);
+  auto pages_of = [&](auto hold) {
+    constexpr int kHold = decltype(hold)::value;
+    constexpr int kStage = VEC == 8 ? kHold * 128 * (4 + kAppendWarps * kAppendBufs<T, kHold> * (int)sizeof(T)) : 0;
+    auto kernel = append_pages_kernel<T, VEC, NC, kHold>;
+    static std::atomic<uint64_t> done{0};
+    allow_shared_memory(reinterpret_cast<const void*>(kernel), kStage, done);
+    kernel<<<(unsigned)ctas, kAppendThreads, kStage, stream>>>(a, head, next, pages, count, err);
+  };
+  // 16,384 bf16 tokens of 8 heads in pages of 32 take 62 us a call so, 162 us with
+  // their rows read twice (append_head).
+  if constexpr (VEC == 8 && sizeof(T) == 2) {
+    if (a.bs > kAppendHold) return pages_of(std::integral_constant<int, 32>{});
+  }
+  pages_of(std::integral_constant<int, kAppendHold>{});
 }
 
 template <typename T>

@@ -259,6 +259,21 @@ def test_append_kv(cuda, dtype, counts, fills, kv_heads, dim, bs, rot, interleav
     check_append(cuda, key, value, cache, scales, slots, bs, pos, table, interleaved)
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("counts,fills,kv_heads,dim,bs,rot,interleaved", [
+    ([700, 33], [0, 7], 5, 128, 32, 128, False),  # pages of more than 16 tokens
+    ([600], [3], 6, 96, 32, 40, True),
+    ([600, 70], [1, 0], 6, 64, 16, 24, False),    # rotary widths of 8 modulo 16
+    ([560], [0], 12, 128, 16, 72, False),         # 24 heads for 8 warps
+    ([14, 2], [2, 0], 9, 128, 16, 40, False),
+    ([600], [0], 3, 128, 16, 12, True),           # half a piece rotated
+])
+def test_append_kv_whole_pages(cuda, dtype, counts, fills, kv_heads, dim, bs, rot, interleaved):
+    key, value, cache, scales, slots, pos, table = append_problem(
+        len(counts) + rot, counts, fills, kv_heads, dim, bs, DTYPES[dtype], rot)
+    check_append(cuda, key, value, cache, scales, slots, bs, pos, table, interleaved)
+
+
 @pytest.mark.parametrize("n", [50, 1400])
 def test_append_kv_any_order_equal_slots_and_padding(cuda, n):
     """Tokens in shuffled order, slots that come twice, padding and slots
