@@ -22,22 +22,29 @@
 //
 // Roles: two softmax warpgroups (one 128-row tile each, one thread per row),
 // four converting warps (global INT8 pages -> fp16 tiles in shared memory, and
-// the pages' scales), one MMA warp per row tile; two warps idle, so that the
+// the pages' scales; the codes come by cp.async into the half of their stage that
+// is converted last), one MMA warp per row tile; two warps idle, so that the
 // registers split evenly.  The row tiles take turns on the tensor cores as in
-// prefill.cu.
+// prefill.cu.  Where a KV head has at most 128 rows (SHARED), both warpgroups work
+// on the one row tile, and the free tensor memory holds the next tile's scores.
 //
 // What bounds it: 32,768 tokens for 64 sequences of 32 query heads (8 KV heads,
 // head_dim 128) are 69 GFLOP with both halves (41 us at the cuBLAS rate) and 67 MB
-// (10 us); the kernel takes 80 us, its tensor pipe 45% and its issue slots 49% busy:
-// per score two roundings, two scale products and an exponential, and for 144 CTAs
-// of 14 or 15 tiles the first query split and load, and the partials' stores, are
-// not hidden by anything.  With one row tile (at most 128 rows a KV head) a step is
-// a chain that nothing overlaps: a tile for 20 rows takes 4.6 us, for 256 rows 5.6 us.
+// (10 us); the kernel takes 80 us, its tensor pipe 45% and its issue slots 49% busy.
+// A row tile's step is about 2,400 clocks of products (S reads both operands from
+// shared memory) and 4,900 of softmax, of which the other row tile hides half; 144
+// CTAs of 14 or 15 tiles also pay for the query split, the first loads and the
+// partials' stores.  With one row tile a step was a chain that nothing overlapped:
+// 16,384 tokens, 20 rows of each of 40 KV heads took 159 us with one warpgroup,
+// 140 us with two, and take 122 us with two buffers of scores.
+// (Loads into registers cost the converting warps 2,000 clocks for 8 loads a
+// thread: with 200 KB of shared memory in use the L1 cache holds few misses.)
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "pkv_common.cuh"
 #include "pkv_internal.h"
@@ -58,16 +65,18 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 2.0f;
 constexpr float kPShift = 13.0f;
 
-template <int DP>
+template <int DP, bool SHARED>
 struct PrefixCfg {
   static constexpr int kChunks = DP / 64;
   static constexpr int kTileBytes = kKeys * DP * 2;
-  static constexpr int kStages = DP == 128 ? 3 : 6;
-  // Scales of a tile are reused by tile j + kSlots.  A tile's K stage is free
-  // again only after the softmax of tile j - 2 (3 stages) or j - 4 (6 stages).
+  static constexpr int kStages = DP == 128 ? (SHARED ? 4 : 3) : 6;
+  // Scales of a tile are reused by tile j + kSlots.  They are written after the
+  // copies of tile j were started, which waits for stages that P V (j - 2) frees (3
+  // or 4 stages), or a product behind P V (j - 4) (6 stages).
   static constexpr int kSlots = DP == 128 ? 2 : 4;
   static constexpr int kOffQ = 0;  // [row tile][hi, lo]
-  static constexpr int kOffKV = 4 * kTileBytes;
+  static constexpr int kOffXch = 2 * kTileBytes;  // SHARED: values exchanged within a row
+  static constexpr int kOffKV = SHARED ? kOffXch + 4096 : 4 * kTileBytes;
   static constexpr int kOffScale = kOffKV + kStages * kTileBytes;  // [slot][k, v][128]
   static constexpr int kOffMask = kOffScale + kSlots * 2 * kKeys * 4;
   static constexpr int kOffBar = kOffMask + kSlots * 16;
@@ -111,6 +120,24 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// 16 bytes of global memory to shared memory, or zeros.
+__device__ __forceinline__ void copy16_if(bool on, uint32_t dst, const int8_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(on ? 16u : 0u)
+               : "memory");
+}
+// A float of read-only memory, or zero.  (In assembly: of a load behind a branch the
+// compiler takes the products in the branch too, and so waits for it there.)
+__device__ __forceinline__ float load_if(bool on, const float* p) {
+  float v;
+  asm volatile(
+      "{\n\t.reg .pred on;\n\tsetp.ne.u32 on, %2, 0;\n\tmov.f32 %0, 0f00000000;\n\t"
+      "@on ld.global.nc.f32 %0, [%1];\n\t}"
+      : "=&f"(v)
+      : "l"(p), "r"((uint32_t)on));
+  return v;
+}
+
 // Tokens of the prefix: the given length, at most what the table covers.
 __device__ __forceinline__ int prefix_tokens(const int32_t* len, int width, int bs) {
   return min(max(*len, 0), width * bs);
@@ -129,10 +156,13 @@ __device__ __forceinline__ uint2 codes_to_half(uint32_t w) {
 
 // GROUPS: the pages hold a multiple of 16 tokens, so 16 columns of a tile share
 // their scales and one load serves them; else every token has its own.
-template <int DP, bool GROUPS>
+// SHARED: one row tile (at most 128 rows a KV head).  Both softmax groups then work
+// on it, each on 64 of a tile's tokens and half of O's columns: a thread and the one
+// 128 further have a row, and exchange its maximum by shared memory.
+template <int DP, bool GROUPS, bool SHARED>
 __global__ void __launch_bounds__(kPrefixThreads, 1)
     prefix_kernel(const PrefixParams p, int* err) {
-  using C = PrefixCfg<DP>;
+  using C = PrefixCfg<DP, SHARED>;
   extern __shared__ __align__(1024) uint8_t smem[];  // no static shared memory: 1024-aligned
   float* s_scale = reinterpret_cast<float*>(smem + C::kOffScale);
   uint32_t* s_mask = reinterpret_cast<uint32_t*>(smem + C::kOffMask);
@@ -143,6 +173,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   uint64_t* s_full = q_full + 2;
   uint64_t* p_full = s_full + 2;  // [row tile][half of the tokens]
   uint64_t* o_full = p_full + 4;
+  uint64_t* pv_done = o_full + 1;  // SHARED: every tile's P V
   uint64_t* mma_done = o_full + 2;
   uint64_t* turn = mma_done + 1;  // per row tile
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
@@ -160,18 +191,18 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   const int per_split = (tiles + p.splits - 1) / p.splits;
   const int tile0 = min(split * per_split, tiles);
   const int n = min(per_split, tiles - tile0);
-  const bool two = pair * 256 + kRows < rows;  // the second row tile has rows
+  const bool two = !SHARED && pair * 256 + kRows < rows;  // the second row tile has rows
   const bool near = DP == 64 || !two;          // see kFlushNear
   const int flush = near ? kFlushNear : kFlushFar;
 
   if (tid == 0) {
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(&kv_full[i], 128);
-      mbar_init(&kv_empty[i], 2);  // both MMA warps
+      mbar_init(&kv_empty[i], two ? 2 : 1);  // the MMA warps at work
     }
     for (int i = 0; i < C::kSlots; ++i) mbar_init(&sc_full[i], 128);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 128);
+      mbar_init(&q_full[i], SHARED ? 256 : 128);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[2 * i], 128);
       mbar_init(&p_full[2 * i + 1], 128);
@@ -197,67 +228,98 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     constexpr int kPass = kKeys / kStep;
     const int ct = tid - kConvWarp * 32;
     const int piece = ct % kLanes, row0 = ct / kLanes;
-    const int64_t row_bytes = (int64_t)p.kv_heads * p.dim;
+    const uint32_t row_bytes = (uint32_t)(p.kv_heads * p.dim);
     const bool in_dim = piece * 16 < p.dim;
+    constexpr int kFar = C::kStages / 3;  // tiles that are on their way
+    // With three stages the next K waits for V (j - 1)'s, and V (j) is not to wait
+    // for that: both copies are started after both conversions.  With four, each
+    // after its own.
+    constexpr bool kBetween = C::kStages == 4;
     bool ok = true;
-    uint4 raw[2][kPass];
-    // Pages of this thread's tokens of a tile and of the token whose scales it
-    // looks after; read while the previous tile is converted, used after that.
-    // The page of token first + o, o < 128, is page0 + (rem + o) / bs, the quotient
-    // exact as ((rem + o) * ceil(2^16 / bs)) >> 16 since rem + o < 256, bs <= 64.
-    int phys[kPass], scale_phys = -1, at[kPass];
-    int first = 0, page0 = 0, rem = 0;
-    const uint32_t inv_bs = (65536u + p.bs - 1) / p.bs;
+    // Cache rows of a tile's tokens, found a tile ahead by the warp's lanes (with
+    // GROUPS lane l & 7 finds those of 16 tokens, else a lane finds 4) and handed
+    // to the threads that read them by shuffle.
+    constexpr int kFinds = GROUPS ? 1 : 4;
+    constexpr uint32_t kNoRow = 0xffffffffu;  // no token, or a page outside the cache
+    uint32_t at[kFinds];
+    int entry[kFinds], rem[kFinds];  // of the next tile
     const int last_page = n > 0 ? (len - 1) / p.bs : 0;
-    auto pages_past = [&](int o) { return (int)(((uint32_t)(rem + o) * inv_bs) >> 16); };
+    auto token = [&](int j, int u) {
+      return (tile0 + j) * kKeys + (GROUPS ? (lane & 7) * 16 : u * 32 + lane);
+    };
     auto look_up = [&](int j) {
-      first = (tile0 + j) * kKeys;
-      page0 = first / p.bs;
-      rem = first - page0 * p.bs;
 #pragma unroll
-      for (int i = 0; i < kPass; ++i)  // past the end the last page again
-        phys[i] = p.table[min(page0 + pages_past(row0 + i * kStep), last_page)];
-      scale_phys = p.table[min(page0 + pages_past(ct), last_page)];
-    };
-    // cache rows from the pages (-1: no token, or a page outside the cache)
-    auto resolve = [&]() {
-#pragma unroll
-      for (int i = 0; i < kPass; ++i) {
-        const int o = row0 + i * kStep;
-        const bool good =
-            first + o < len && phys[i] >= 0 && (int64_t)phys[i] < p.num_blocks;
-        at[i] = good ? phys[i] * p.bs + (rem + o - pages_past(o) * p.bs) : -1;
-      }
-      if (first + ct >= len) {
-        scale_phys = -1;
-      } else if (scale_phys < 0 || (int64_t)scale_phys >= p.num_blocks) {
-        scale_phys = -1;
-        record_error(err, kDevBadBlockId);
+      for (int u = 0; u < kFinds; ++u) {
+        const int page = token(j, u) / p.bs;
+        rem[u] = token(j, u) - page * p.bs;
+        entry[u] = p.table[min(page, last_page)];  // past the end the last page again
       }
     };
-    auto fetch = [&](int kind) {
-      const int8_t* base = (kind ? p.v_cache : p.k_cache) + (int64_t)kvh * p.dim + piece * 16;
+    // scales of the thread's token, of the tile at hand and those on their way
+    float ks[kFar] = {}, vs[kFar] = {};
+    bool good[kFar] = {};
+    auto resolve = [&](int j) {
+      int phys;  // of the thread's own token
+      if constexpr (GROUPS) {
+        phys = __shfl_sync(0xffffffffu, entry[0], ct / 16);
+      } else {
+        phys = entry[0];
 #pragma unroll
-      for (int i = 0; i < kPass; ++i) {
-        raw[kind][i] = make_uint4(0, 0, 0, 0);
-        if (at[i] >= 0 && in_dim)
-          raw[kind][i] = __ldg(reinterpret_cast<const uint4*>(base + at[i] * row_bytes));
+        for (int u = 1; u < kFinds; ++u)
+          if (ct / 32 == u) phys = entry[u];
+      }
+      const bool counts = (tile0 + j) * kKeys + ct < len;
+      const bool ok_page = counts && phys >= 0 && (int64_t)phys < p.num_blocks;
+      if (counts && !ok_page) record_error(err, kDevBadBlockId);
+      good[kFar - 1] = ok_page;
+      ks[kFar - 1] = load_if(ok_page, p.k_scale + (int64_t)phys * p.kv_heads + kvh);
+      vs[kFar - 1] = load_if(ok_page, p.v_scale + (int64_t)phys * p.kv_heads + kvh);
+#pragma unroll
+      for (int u = 0; u < kFinds; ++u) {
+        const bool in = token(j, u) < len && entry[u] >= 0 && (int64_t)entry[u] < p.num_blocks;
+        at[u] = in ? (uint32_t)entry[u] * p.bs + rem[u] : kNoRow;
       }
     };
-    // scales of the thread's token: loaded with the tile's K rows
-    float ks = 0.0f, vs = 0.0f;
-    bool good = false;
-    auto fetch_scales = [&]() {
-      good = scale_phys >= 0;
-      ks = good ? p.k_scale[(int64_t)scale_phys * p.kv_heads + kvh] : 0.0f;
-      vs = good ? p.v_scale[(int64_t)scale_phys * p.kv_heads + kvh] : 0.0f;
+    // Item i is tile i / 2, K or V.  Its codes are copied into the second half of its
+    // stage, kFar tiles ahead; each thread converts what it copied.
+    auto stage_of = [&](int i) { return smem + C::kOffKV + (i % C::kStages) * C::kTileBytes; };
+    auto issue = [&](int j, int kind) {
+      if (kFar == 2 && kind == 0)
+        ks[0] = ks[kFar - 1], vs[0] = vs[kFar - 1], good[0] = good[kFar - 1];
+      if (j < n) {
+        if (kind == 0) {
+          resolve(j);
+          if (j + 1 < n) look_up(j + 1);
+        }
+        const int i = 2 * j + kind, st = i % C::kStages;
+        if (ok && !mbar_wait_bounded(&kv_empty[st], ((uint32_t)(i / C::kStages) & 1u) ^ 1u, err)) {
+          record_error(err, kDevWaitTimeout);
+          ok = false;
+        }
+        const int8_t* base = (kind ? p.v_cache : p.k_cache) + (int64_t)kvh * p.dim + piece * 16;
+        const uint32_t dst = smem_u32(stage_of(i)) + C::kTileBytes / 2 + ct * 16;
+#pragma unroll
+        for (int r = 0; r < kPass; ++r) {
+          const int o = r * kStep;
+          const uint32_t row =
+              GROUPS ? __shfl_sync(0xffffffffu, at[0], o / 16 + row0 / 16)
+                     : __shfl_sync(0xffffffffu, at[GROUPS ? 0 : o / 32], o % 32 + row0);
+          const bool on = row != kNoRow && in_dim;
+          // (rows past the length on its last page are read: any codes will do)
+          const uint64_t from = (uint64_t)(on ? row + (GROUPS ? row0 % 16 : 0) : 0) * row_bytes;
+          copy16_if(on, dst + r * 2048, base + from);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
     };
     float inv_vmax = 0.0f;
     if (n > 0) {
       look_up(0);
-      resolve();
-      fetch(0);
-      fetch_scales();
+#pragma unroll
+      for (int j = 0; j < kFar; ++j) {
+        issue(j, 0);
+        issue(j, 1);
+      }
       // the largest V scale of this part: p * v_scale is kept relative to it
       const int first = tile0 * kKeys / p.bs;
       const int last = (min((tile0 + n) * kKeys, len) - 1) / p.bs;
@@ -276,42 +338,43 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     for (int j = 0; j < n; ++j) {
 #pragma unroll
       for (int kind = 0; kind < 2; ++kind) {
-        const int i = 2 * j + kind, st = i % C::kStages;
-        // the next tile's loads are in flight while this one is converted
-        if (kind == 0) {
-          fetch(1);
-          if (j + 1 < n) look_up(j + 1);
-        } else if (j + 1 < n) {
-          resolve();
-          fetch(0);
-          fetch_scales();
-        }
-        if (ok && !mbar_wait_bounded(&kv_empty[st], ((uint32_t)(i / C::kStages) & 1u) ^ 1u, err)) {
-          record_error(err, kDevWaitTimeout);
-          ok = false;
-        }
+        const int i = 2 * j + kind;
         if (kind == 0) {  // the tile's scales and which of its tokens count
           const int slot = j % C::kSlots;
-          s_scale[(slot * 2) * kKeys + ct] = ks * p.qk_scale;
-          s_scale[(slot * 2 + 1) * kKeys + ct] = vs * inv_vmax;
-          const unsigned m = __ballot_sync(0xffffffffu, good);
+          s_scale[(slot * 2) * kKeys + ct] = ks[0] * p.qk_scale;
+          s_scale[(slot * 2 + 1) * kKeys + ct] = vs[0] * inv_vmax;
+          const unsigned m = __ballot_sync(0xffffffffu, good[0]);
           if (lane == 0) s_mask[slot * 4 + (ct >> 5)] = m;
           mbar_arrive(&sc_full[slot]);
         }
-        uint8_t* tile = smem + C::kOffKV + st * C::kTileBytes + (piece / 4) * (kKeys * 128);
+        if (kind == 0 || kBetween)
+          asm volatile("cp.async.wait_group %0;" ::"n"(2 * kFar - 1) : "memory");
+        else
+          asm volatile("cp.async.wait_group %0;" ::"n"(2 * kFar - 2) : "memory");
+        uint4 raw[kPass];
 #pragma unroll
-        for (int r = 0; r < kPass; ++r) {
-          const int row = row0 + r * kStep;
-          const uint4 w = raw[kind][r];
+        for (int r = 0; r < kPass; ++r)
+          raw[r] = *reinterpret_cast<const uint4*>(stage_of(i) + C::kTileBytes / 2 + (r * 128 + ct) * 16);
+        named_barrier(1, 128);  // every code is read
+        uint8_t* tile = stage_of(i) + (piece / 4) * (kKeys * 128);
+        const uint32_t off = sw128_offset(row0, (piece % 4) * 32);
+        const uint32_t off16 = sw128_offset(row0, (piece % 4) * 32 + 16);
+#pragma unroll
+        for (int r = 0; r < kPass; ++r) {  // (kStep % 8 = 0: one swizzle for all)
+          const uint4 w = raw[r];
           const uint2 a = codes_to_half(w.x), b = codes_to_half(w.y), c = codes_to_half(w.z),
                       d = codes_to_half(w.w);
-          const int byte = (piece % 4) * 32;
-          *reinterpret_cast<uint4*>(tile + sw128_offset(row, byte)) = make_uint4(a.x, a.y, b.x, b.y);
-          *reinterpret_cast<uint4*>(tile + sw128_offset(row, byte + 16)) =
+          *reinterpret_cast<uint4*>(tile + off + r * kStep * 128) = make_uint4(a.x, a.y, b.x, b.y);
+          *reinterpret_cast<uint4*>(tile + off16 + r * kStep * 128) =
               make_uint4(c.x, c.y, d.x, d.y);
         }
         fence_proxy_async_smem();  // an MMA operand
-        mbar_arrive(&kv_full[st]);
+        mbar_arrive(&kv_full[i % C::kStages]);
+        if (kBetween) issue(j + 1, kind);
+      }
+      if (!kBetween) {
+        issue(j + kFar, 0);
+        issue(j + kFar, 1);
       }
     }
   } else if (warp < kIdleWarp) {
@@ -338,8 +401,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         wait(&kv_full[i % C::kStages], (uint32_t)(i / C::kStages) & 1u);
       };
       auto stage_of = [&](int i) { return (uint32_t)(i % C::kStages) * C::kTileBytes; };
-      // Both warps release a stage, each after it saw the tile, and only if a
-      // later tile reuses the stage.
+      // The warps at work release a stage, each after it saw the tile, and only if
+      // a later tile reuses the stage.
       auto release = [&](int i) {
         if (i + C::kStages < 2 * n) umma_commit_warp(&kv_empty[i % C::kStages]);
       };
@@ -347,6 +410,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         if (lane == 0) mbar_arrive(&turn[x ^ 1]);
         __syncwarp();
       };
+      auto s_of = [&](int j) { return s_col + (SHARED ? (uint32_t)(j & 1) * 128 : 0u); };
       auto qk = [&](int j, bool pass) {
         const uint64_t b = umma_desc_at(k_desc, stage_of(2 * j));
 #pragma unroll
@@ -355,27 +419,32 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
 #pragma unroll
           for (int kk = 0; kk < DP / 16; ++kk) {
             const uint32_t off = (uint32_t)(kk / 4) * (kKeys * 128) + (uint32_t)(kk % 4) * 32;
-            umma_f16_warp(s_col, umma_desc_at(a, off), umma_desc_at(b, off), kIdQK,
+            umma_f16_warp(s_of(j), umma_desc_at(a, off), umma_desc_at(b, off), kIdQK,
                           (half < 1 || kk > 0) ? 1u : 0u);
             if (half == 0 && kk == DP / 16 - kEarly && pass) pass_turn();
           }
         }
-        umma_commit_warp(&s_full[x]);
+        umma_commit_warp(&s_full[SHARED ? j & 1 : x]);
       };
-      wait_tile(0);
       if (mine) {
+        wait_tile(0);
         wait(&q_full[x], 0);
         tmem_fence_after_sync();
         if (ok) qk(0, false);
-      }
-      release(0);
-      for (int j = 0; j < n && ok; ++j) {
-        wait_tile(2 * j + 1);
-        if (x == 1 || j > 0) wait(&turn[x], (uint32_t)(x == 1 ? j : j - 1) & 1u);
-        if (mine) wait(&p_full[2 * x], (uint32_t)j & 1u);
-        tmem_fence_after_sync();
-        if (!ok) break;
-        if (mine) {
+        release(0);
+        for (int j = 0; j < n && ok; ++j) {
+          if (SHARED && j + 1 < n) {  // into the other S, whose P (j - 1) is used up
+            wait_tile(2 * j + 2);
+            if (!ok) break;
+            tmem_fence_after_sync();
+            qk(j + 1, false);
+            release(2 * j + 2);
+          }
+          wait_tile(2 * j + 1);
+          if (two && (x == 1 || j > 0)) wait(&turn[x], (uint32_t)(x == 1 ? j : j - 1) & 1u);
+          wait(&p_full[2 * x], (uint32_t)j & 1u);
+          tmem_fence_after_sync();
+          if (!ok) break;
           // P of tokens 32 i .. 32 i + 31 is in columns 32 i: hi in 16, lo in 16
           const uint64_t b = umma_desc_at(v_desc, stage_of(2 * j + 1));
 #pragma unroll
@@ -386,22 +455,23 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
             }
 #pragma unroll
             for (int half = 0; half < 2; ++half)
-              umma_f16_ta_warp(o_col, s_col + (kk / 2) * 32 + half * 16 + (kk % 2) * 8,
+              umma_f16_ta_warp(o_col, s_of(j) + (kk / 2) * 32 + half * 16 + (kk % 2) * 8,
                                umma_desc_at(b, kk * 2048), kIdPV,
                                (j % flush > 0 || kk > 0 || half > 0) ? 1u : 0u);
           }
           if (j == n - 1) umma_commit_warp(&o_full[x]);
-          // the next K tile is converted while these run (its stage was V (j - 1)'s)
+          release(2 * j + 1);
+          if constexpr (SHARED) {
+            umma_commit_warp(pv_done);
+            continue;
+          }
+          // the next K tile is converted while these run
           if (j + 1 < n) wait_tile(2 * j + 2);
           if (!ok) break;
           if (j + 1 < n) qk(j + 1, true);  // over P (j): a warp's MMAs run in order
           else pass_turn();
-        } else {
-          if (j + 1 < n) wait_tile(2 * j + 2);
-          pass_turn();
+          if (j + 1 < n) release(2 * j + 2);
         }
-        release(2 * j + 1);
-        if (j + 1 < n) release(2 * j + 2);
       }
       umma_commit_warp(mma_done);
       mbar_drain(mma_done, 0);  // every MMA is done before tensor memory is freed
@@ -409,11 +479,15 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   }
   } else {
   registers_up<136>();
-  if (warp < 4 || two) {
+  if (SHARED || warp < 4 || two) {
     // ---- query split, softmax, partials: thread = row --------------------------------------
-    const int x = warp >> 2, row = tid & 127;
+    const int x = SHARED ? 0 : warp >> 2, row = tid & 127;
+    const int half = SHARED ? warp >> 2 : 0;
+    // exchanged between the two threads of a row: [tile parity][half][row], then [row]
+    float* xch = reinterpret_cast<float*>(smem + C::kOffXch);
+    auto meet = [&]() { named_barrier(2 + (warp & 3), 64); };
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-    const uint32_t s_addr = tmem + lanes + x * 128, o_addr = tmem + lanes + C::kOCol + x * 128;
+    const uint32_t s_addr0 = tmem + lanes + x * 128, o_addr = tmem + lanes + C::kOCol + x * 128;
     const int r = pair * 256 + x * kRows + row;
     const bool valid = r < rows;
     const int seq = r / p.group;
@@ -425,13 +499,15 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       // stay far below hi's.
       uint8_t* hi_t = smem + C::kOffQ + (2 * x) * C::kTileBytes;
       uint8_t* lo_t = hi_t + C::kTileBytes;
-      const int base = pair * 256 + warp * 32;
-      int gi = base % p.group;
+      const int base = pair * 256 + (SHARED ? warp & 3 : warp) * 32;
+      const int i_end = SHARED ? 16 + half * 16 : 32;
+      const int from = base + half * 16;
+      int gi = from % p.group;
       const float* row_ptr =
-          p.q + ((int64_t)(base / p.group) * p.heads + kvh * p.group + gi) * p.dim + lane * 4;
+          p.q + ((int64_t)(from / p.group) * p.heads + kvh * p.group + gi) * p.dim + lane * 4;
       const int64_t wrap = (int64_t)(p.heads - p.group) * p.dim;  // to the next sequence's group
 #pragma unroll 1
-      for (int i0 = 0; i0 < 32; i0 += 8) {
+      for (int i0 = half * 16; i0 < i_end; i0 += 8) {
       float4 rowv[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) {  // all loads first
@@ -476,32 +552,51 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       }
       fence_proxy_async_smem();  // an MMA operand
       mbar_arrive(&q_full[x]);
+      if constexpr (SHARED) {
+        if (lane / 16 == half) xch[2 * 2 * kRows + row] = rf;
+        meet();
+        rf = xch[2 * 2 * kRows + row];
+      }
     }
     // Warps without rows only keep the hand-offs going.
     const bool busy = r - lane < rows;
     const bool flushes = n > flush;
     const uint32_t o2_addr = DP == 64 ? o_addr + 64 : tmem + lanes + C::kOCol + 128;
     float4* sums = p.sums + (((int64_t)split * gridDim.x + blockIdx.x) * 2 + x) * (DP / 4) * kRows + row;
+    const int col0 = half * (DP / 2), col1 = SHARED ? col0 + DP / 2 : DP;  // of O
+    const int part0 = half * 2, part1 = SHARED ? part0 + 2 : 4;  // chunks of a tile
     float since = 1.0f;  // by what O's unit has changed since `sums` was written
     float m = -INFINITY, l = 0.0f;  // m in units of S * k_scale * qk_scale
     bool ok = true;
     for (int j = 0; j < n; ++j) {
       const int slot = j % C::kSlots;
       if (ok && (!mbar_wait_bounded(&sc_full[slot], (uint32_t)(j / C::kSlots) & 1u, err) ||
-                 !mbar_wait_short(&s_full[x], (uint32_t)j & 1u, err))) {
+                 !mbar_wait_short(&s_full[SHARED ? j & 1 : x],
+                                  (uint32_t)(SHARED ? j >> 1 : j) & 1u, err))) {
         record_error(err, kDevWaitTimeout);
         ok = false;
       }
       __syncwarp();
       tmem_fence_after_sync();
+      // S (j) does not tell that P (j - 1) was taken, nor that O has P V (j - 1).
+      auto wait_pv = [&]() {
+        if (j > 0 && ok && !mbar_wait_short(pv_done, (uint32_t)(j - 1) & 1u, err)) {
+          record_error(err, kDevWaitTimeout);
+          ok = false;
+        }
+        __syncwarp();
+        tmem_fence_after_sync();
+      };
       if (!busy) {
-        mbar_arrive(&p_full[2 * x]);
-        mbar_arrive(&p_full[2 * x + 1]);
+        if constexpr (SHARED) wait_pv();  // else an arrival could count for tile j - 1
+        if (!SHARED || half == 0) mbar_arrive(&p_full[2 * x]);
+        if (!SHARED || half == 1) mbar_arrive(&p_full[2 * x + 1]);
         continue;
       }
-      if (j > 0 && j % flush == 0) {
+      const uint32_t s_addr = s_addr0 + (SHARED ? (uint32_t)(j & 1) * 128 : 0u);
+      auto flush_o = [&]() {
 #pragma unroll 1
-        for (int c = 0; c < DP; c += 16) {
+        for (int c = col0; c < col1; c += 16) {
           alignas(16) uint32_t o[16], was[16];
           tmem_load<16>(o_addr + c, o);
           if (j == flush) {
@@ -529,7 +624,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         }
         tmem_wait_store();
         since = 1.0f;
-      }
+      };
+      if (!SHARED && j > 0 && j % flush == 0) flush_o();
       const float* ks = s_scale + slot * 2 * kKeys;
       const float* vs = ks + kKeys;
       const uint32_t* mask = s_mask + slot * 4;
@@ -538,10 +634,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       // not count become -inf.  The next chunk's loads are issued before this one's
       // arithmetic: each takes about 150 clocks.
       uint32_t s[32];
-      tmem_load<32>(s_addr, s);
-      float k0 = ks[0], k1 = ks[16];  // GROUPS: of the chunk's two groups
+      tmem_load<32>(s_addr + part0 * 32, s);
+      float k0 = ks[part0 * 32], k1 = ks[part0 * 32 + 16];  // GROUPS: of the chunk's two groups
       auto scores = [&](int c, uint64_t (&y)[16]) {
-        const int next = ((c + 1) & 3) * 32;
+        const int next = (c + 1 < part1 ? c + 1 : part0) * 32;
         tmem_wait_load();
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -550,7 +646,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
               GROUPS ? f32x2(g, g) : *reinterpret_cast<const uint64_t*>(ks + c * 32 + 2 * e);
           y[e] = mul_f32x2(f32x2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), k);
         }
-        tmem_load<32>(s_addr + next, s);  // after the last one chunk 0 again
+        tmem_load<32>(s_addr + next, s);  // after the last one the first again
         if constexpr (GROUPS) {
           k0 = ks[next];
           k1 = ks[next + 16];
@@ -569,7 +665,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       // (rolled: unrolled, the two passes were 40 KB of code, and fetching it cost
       // the first tile 16,000 clocks)
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
+      for (int c = part0; c < part1; ++c) {
         uint64_t y[16];
         scores(c, y);
 #pragma unroll
@@ -578,14 +674,29 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           tm[e & 3] = max3_nan(tm[e & 3], a.x, a.y);
         }
       }
-      const float t = max3_nan(max3_nan(tm[0], tm[1], tm[2]), tm[3], tm[3]);
+      float t = max3_nan(max3_nan(tm[0], tm[1], tm[2]), tm[3], tm[3]);
+      if constexpr (SHARED) {
+        float* of = xch + (j & 1) * 2 * kRows + row;
+        of[half * kRows] = t;
+        meet();
+        const float u = of[(half ^ 1) * kRows];
+        t = max3_nan(t, u, u);
+        wait_pv();
+        if (j > 0 && j % flush == 0) {
+          flush_o();
+          tmem_fence_before_sync();
+          meet();  // P of the first half lets the product start
+          tmem_fence_after_sync();
+        }
+      }
       const bool move = valid && t > m && (m == -INFINITY || (t - m) * rf > kLazy);
       if (__any_sync(0xffffffffu, move)) {
         const float alpha = move ? ex2((m - t) * rf) : 1.0f;
         if (move) m = t;
         l *= alpha;
         since *= alpha;
-        if (j % flush != 0) {
+        // (all columns by the first group: its P lets the product start)
+        if (j % flush != 0 && half == 0) {
 #pragma unroll 1
           for (int c = 0; c < DP; c += 16) {
             uint32_t o[16];
@@ -601,9 +712,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       const float ms = t != t ? t : (m == -INFINITY ? 0.0f : m * rf) - kPShift;
       const uint64_t rf2 = f32x2(rf, rf), ms2 = f32x2(-ms, -ms);
       uint64_t sum[2] = {0, 0};
-      float v0 = vs[0], v1 = vs[16];
+      float v0 = vs[part0 * 32], v1 = vs[part0 * 32 + 16];
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
+      for (int c = part0; c < part1; ++c) {
         uint64_t y[16];
         const float u0 = v0, u1 = v1;
         if constexpr (GROUPS) {
@@ -632,7 +743,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           w[16 + e] = *reinterpret_cast<const uint32_t*>(&lo);
         }
         tmem_store<32>(s_addr + c * 32, w);
-        if (c == 1) {  // half of P is there: its product can start
+        if (!SHARED && c == 1) {  // half of P is there: its product can start
           tmem_wait_store();
           tmem_fence_before_sync();
           mbar_arrive(&p_full[2 * x]);
@@ -643,7 +754,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       tmem_wait_load();  // the load that ran ahead
       tmem_wait_store();
       tmem_fence_before_sync();
-      mbar_arrive(&p_full[2 * x + 1]);
+      mbar_arrive(&p_full[2 * x + (SHARED ? half : 1)]);
     }
     if (n > 0) {
       if (ok && !mbar_wait_bounded(&o_full[x], 0, err)) record_error(err, kDevWaitTimeout);
@@ -652,7 +763,15 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     }
     const float vmax = fmaxf(fmaxf(s_vmax[0], s_vmax[1]), fmaxf(s_vmax[2], s_vmax[3]));
     const int64_t slot_row = (int64_t)split * p.num_seqs * p.heads + head_row;
-    if (valid) {
+    if constexpr (SHARED) {  // the row's sum: the first tokens' half, then the others'
+      if (n > 0 && busy) {
+        float* of = xch + (n & 1) * 2 * kRows + row;
+        of[half * kRows] = l;
+        meet();
+        l = of[0] + of[kRows];
+      }
+    }
+    if (valid && half == 0) {
       // nothing attended: (-inf, 0); every score NaN: a NaN that the join keeps
       float2 ml = make_float2(m * rf - kPShift, l);
       if (m == -INFINITY) ml = l == 0.0f ? make_float2(-INFINITY, 0.0f) : make_float2(-1e30f, l);
@@ -664,7 +783,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       uint8_t* stage = smem + C::kOffQ + 2 * x * C::kTileBytes;
       if (busy) {
 #pragma unroll 1
-        for (int c = 0; c < DP; c += 16) {
+        for (int c = col0; c < col1; c += 16) {
           uint32_t o[16];
           alignas(16) uint32_t was[16];
           tmem_load<16>(o_addr + c, o);
@@ -688,11 +807,13 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
                 make_float4(total(4 * e), total(4 * e + 1), total(4 * e + 2), total(4 * e + 3));
         }
       }
-      __syncwarp();  // a warp writes out its own rows
+      if constexpr (SHARED) meet();
+      __syncwarp();  // a warp writes out its own rows, or half of them
       constexpr int kPieces = DP / 4;
       const int piece = lane % kPieces;
       if (piece * 4 < p.dim)
-        for (int i = lane / kPieces; i < 32; i += 32 / kPieces) {
+        for (int i = half * 16 + lane / kPieces; i < (SHARED ? 16 + half * 16 : 32);
+             i += 32 / kPieces) {
           const int ri = r - lane + i, si = ri / p.group, rr = (warp & 3) * 32 + i;
           if (ri >= rows) break;
           const int64_t to = (int64_t)split * p.num_seqs * p.heads + (int64_t)si * p.heads +
@@ -826,10 +947,10 @@ PrefixWs prefix_ws(const SharedPrefixArgs& a) {
   return w;
 }
 
-template <int DP, bool GROUPS>
+template <int DP, bool GROUPS, bool SHARED>
 void launch_prefix_t(const PrefixParams& p, cudaStream_t stream) {
-  using C = PrefixCfg<DP>;
-  auto kern = prefix_kernel<DP, GROUPS>;
+  using C = PrefixCfg<DP, SHARED>;
+  auto kern = prefix_kernel<DP, GROUPS, SHARED>;
   static std::atomic<uint64_t> done{0};
   allow_shared_memory(reinterpret_cast<const void*>(kern), C::kSmemBytes, done);
   const int64_t pairs = ((int64_t)p.num_seqs * p.group + 255) / 256;
@@ -880,10 +1001,18 @@ int launch_shared_prefix(const SharedPrefixArgs& a, void* workspace, size_t work
     p.splits = w.splits;
     p.qk_scale = o.sm_scale * kLog2e;
     const bool groups = o.block_size % 16 == 0;
-    if (o.head_dim <= 64)
-      groups ? launch_prefix_t<64, true>(p, stream) : launch_prefix_t<64, false>(p, stream);
-    else
-      groups ? launch_prefix_t<128, true>(p, stream) : launch_prefix_t<128, false>(p, stream);
+    const bool shared = o.num_seqs * (o.num_heads / o.num_kv_heads) <= kRows;
+    auto with = [&](auto dp, auto g, auto s) {
+      launch_prefix_t<decltype(dp)::value, decltype(g)::value, decltype(s)::value>(p, stream);
+    };
+    auto with_dim = [&](auto g, auto s) {
+      o.head_dim <= 64 ? with(std::integral_constant<int, 64>{}, g, s)
+                       : with(std::integral_constant<int, 128>{}, g, s);
+    };
+    auto with_groups = [&](auto s) {
+      groups ? with_dim(std::true_type{}, s) : with_dim(std::false_type{}, s);
+    };
+    shared ? with_groups(std::true_type{}) : with_groups(std::false_type{});
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) {
       set_error(std::string("prefix launch failed: ") + cudaGetErrorString(e));

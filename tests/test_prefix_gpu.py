@@ -123,6 +123,19 @@ def test_matches_reference(cuda, prefix, lens, heads, kv_heads, dim, bs):
     check(problem(prefix + dim, prefix, lens, heads, kv_heads, dim, bs))
 
 
+@pytest.mark.parametrize("prefix,lens,heads,dim,bs", [
+    (6000, [9, 1], 40, 128, 16),       # 2 rows of a KV head: most warps have none
+    (6000, [9, 1, 0], 40, 64, 16),
+    (4990, [3] * 40, 40, 128, 16),     # 40 rows: a warp and a part of one
+    (4990, [3] * 70, 40, 96, 24),
+    (4500, [1] * 130, 40, 128, 16),    # a row and a half tile: sums beside O in memory
+    (4500, [1] * 130, 40, 64, 32),
+])
+def test_parts_of_many_tiles(cuda, prefix, lens, heads, dim, bs):
+    """Many KV heads leave each CTA 12 to 16 tiles of the prefix."""
+    check(problem(prefix + dim, prefix, lens, heads, heads, dim, bs))
+
+
 @pytest.mark.parametrize("prefix,heads,kv_heads,bs", [(1024, 8, 8, 16), (320, 32, 8, 16),
                                                       (96, 8, 2, 32)])
 def test_agrees_with_decode_over_joined_tables(cuda, prefix, heads, kv_heads, bs):
