@@ -1603,7 +1603,7 @@ __global__ void __launch_bounds__(kGenThreads)
                          (int64_t)kvh * head_dim;
       acc = fmaf(s_p[t] * vs, (float)vr[d], acc);
     }
-    if (n_splits == 1 && out != nullptr) {
+    if (n_splits == 1) {
       out[((int64_t)seq * num_heads + h) * head_dim + d] = l > 0.0f ? acc / l : 0.0f;
     } else {
       const int64_t slot = ((int64_t)seq * max_splits + split) * num_heads + h;
@@ -3694,10 +3694,12 @@ int launch_decode(const DecodeArgs& a, void* workspace, size_t workspace_bytes,
   return kOk;
 }
 
-void decode_partials_plan(const DecodeArgs& a, int* max_splits, int* pages_per_split) {
+bool decode_partials_plan(const DecodeArgs& a, int* max_splits, int* pages_per_split) {
   const Plan p = make_plan(a, true);
+  if (!p.fast) return false;
   *max_splits = p.max_splits;
   *pages_per_split = p.pages_per_split;
+  return true;
 }
 
 int launch_decode_partials(const DecodeArgs& a, float* ws_acc, float2* ws_ml,

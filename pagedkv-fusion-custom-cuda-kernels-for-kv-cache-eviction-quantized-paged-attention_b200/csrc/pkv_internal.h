@@ -165,7 +165,9 @@ int launch_decode(const DecodeArgs& a, void* workspace, size_t workspace_bytes,
 // units, l) at slot (seq * max_splits + split) * num_heads + head of ws_acc
 // [slots][head_dim] and ws_ml [slots]; a sequence has ceil(pages /
 // pages_per_split) splits, its other slots are not written.  `a.out` is unused.
-void decode_partials_plan(const DecodeArgs& a, int* max_splits, int* pages_per_split);
+// The plan is false for shapes that only the generic kernel takes; those are not
+// launched so.
+bool decode_partials_plan(const DecodeArgs& a, int* max_splits, int* pages_per_split);
 int launch_decode_partials(const DecodeArgs& a, float* ws_acc, float2* ws_ml, cudaStream_t stream);
 
 // ---- prefix.cu ------------------------------------------------------------

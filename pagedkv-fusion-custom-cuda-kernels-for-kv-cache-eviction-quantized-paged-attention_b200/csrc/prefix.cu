@@ -36,7 +36,7 @@
 // CTAs of 14 or 15 tiles also pay for the query split, the first loads and the
 // partials' stores.  With one row tile a step was a chain that nothing overlapped:
 // 16,384 tokens, 20 rows of each of 40 KV heads took 159 us with one warpgroup,
-// 140 us with two, and take 122 us with two buffers of scores.
+// 144 us with two, and take 122 us with two buffers of scores.
 // (Loads into registers cost the converting warps 2,000 clocks for 8 loads a
 // thread: with 200 KB of shared memory in use the L1 cache holds few misses.)
 #include <cuda_fp16.h>
@@ -829,6 +829,223 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
 }
 
+// ---------------------------------------------------------------------------
+// Own tokens of the shapes that the decode split kernels do not take (head_dim 32,
+// 64 and 96, groups of other than 1, 2, 4 or 8 heads, other page sizes).
+// ---------------------------------------------------------------------------
+//
+// A CTA of 128 threads has up to 8 query heads of one KV head and a part of one
+// sequence's pages, 64 tokens at a time: LP lanes a token, 16 codes of K and of V a
+// lane, all loaded at once; products in fp32 on the CUDA cores (a few heads do not
+// fill a tensor-core tile).  Partials as the decode split kernels leave them, for
+// the join.  A call with 32 sequences of 20 to 520 tokens behind 4,000, 32 / 8 heads,
+// head_dim 96, takes 44 us so, 294 us with the decode kernel for any shape (a CTA per
+// query head, a warp per token, a thread per channel).
+constexpr int kOwnTokens = 64, kOwnHeads = 8;
+
+struct OwnParams {
+  const float* q;
+  const int8_t* k_cache;
+  const float* k_scale;
+  const int8_t* v_cache;
+  const float* v_scale;
+  const int32_t* tables;
+  const int32_t* lens;
+  float* acc;
+  float2* ml;
+  int64_t num_blocks;
+  int heads, kv_heads, group, dim, bs, width, pages_per_split, splits;
+  float qk_scale;
+};
+
+// Four INT8 codes as floats, exact: byte + 128 in the mantissa of 2^23.
+__device__ __forceinline__ void codes_to_float(uint32_t w, float* f) {
+  const uint32_t u = w ^ 0x80808080u;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    f[e] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + e)) - 8388736.0f;
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int b = 16; b > 0; b /= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, b));
+  return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int b = 16; b > 0; b /= 2) v += __shfl_xor_sync(0xffffffffu, v, b);
+  return v;
+}
+
+template <int LP>
+__global__ void __launch_bounds__(128) own_kernel(const OwnParams p, int* err) {
+  constexpr int kAtOnce = 128 / LP, kPer = kOwnTokens / kAtOnce, D = LP * 16;
+  constexpr int kRed = 16 * LP / 32;  // channels a lane has after the reduction
+  constexpr uint32_t kNoRow = 0xffffffffu;
+  __shared__ __align__(16) float s_q[kOwnHeads][D];
+  __shared__ __align__(16) float s_red[4][kOwnHeads][D];
+  __shared__ float s_p[kOwnHeads][kOwnTokens];
+  __shared__ float s_ks[kOwnTokens], s_vs[kOwnTokens];
+  __shared__ uint32_t s_row[kOwnTokens];
+  __shared__ float s_m[kOwnHeads], s_l[kOwnHeads], s_alpha[kOwnHeads];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int seq = blockIdx.x / p.splits, split = blockIdx.x % p.splits;
+  const int chunks = (p.group + kOwnHeads - 1) / kOwnHeads;
+  const int kvh = blockIdx.y / chunks, g0 = (blockIdx.y % chunks) * kOwnHeads;
+  const int ng = min(kOwnHeads, p.group - g0);
+  const int want = max(p.lens[seq], 0);
+  const int len = (int)min((int64_t)want, (int64_t)p.width * p.bs);
+  if (len != want && split == 0 && blockIdx.y == 0 && tid == 0) record_error(err, kDevSeqTooLong);
+  const int64_t t0 = (int64_t)split * p.pages_per_split * p.bs;
+  const int64_t t1 = min((int64_t)len, t0 + p.pages_per_split * p.bs);
+  if (t0 >= t1) return;
+  const int head0 = kvh * p.group + g0;
+  for (int i = tid; i < ng * D; i += 128) {
+    const int g = i / D, d = i % D;
+    s_q[g][d] = d < p.dim ? p.q[((int64_t)seq * p.heads + head0 + g) * p.dim + d] : 0.0f;
+  }
+  if (tid < kOwnHeads) s_m[tid] = -INFINITY, s_l[tid] = 0.0f;
+  const int piece = tid % LP, tok0 = tid / LP;
+  const uint32_t row_bytes = (uint32_t)(p.kv_heads * p.dim);
+  const int64_t base = (int64_t)kvh * p.dim + piece * 16;
+  float acc[kOwnHeads];
+#pragma unroll
+  for (int g = 0; g < kOwnHeads; ++g) acc[g] = 0.0f;
+
+  for (int64_t t = t0; t < t1; t += kOwnTokens) {
+    __syncthreads();  // the last tokens' values are used up
+    if (tid < kOwnTokens) {
+      const int64_t at = t + tid;
+      int phys = -1, page = 0;
+      if (at < t1) {
+        page = (int)at / p.bs;  // (lengths are 32-bit)
+        phys = p.tables[(int64_t)seq * p.width + page];
+        if (phys < 0 || (int64_t)phys >= p.num_blocks) {
+          phys = -1;
+          record_error(err, kDevBadBlockId);
+        }
+      }
+      s_row[tid] = phys < 0 ? kNoRow : (uint32_t)phys * p.bs + ((uint32_t)at - (uint32_t)page * p.bs);
+      s_ks[tid] = phys < 0 ? 0.0f : p.k_scale[(int64_t)phys * p.kv_heads + kvh] * p.qk_scale;
+      s_vs[tid] = phys < 0 ? 0.0f : p.v_scale[(int64_t)phys * p.kv_heads + kvh];
+    }
+    __syncthreads();
+    uint4 k[kPer], v[kPer];
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      const uint32_t row = s_row[tok0 + u * kAtOnce];
+      k[u] = v[u] = make_uint4(0, 0, 0, 0);
+      if (row != kNoRow && piece * 16 < p.dim) {
+        const int64_t at = base + (int64_t)((uint64_t)row * row_bytes);
+        k[u] = __ldg(reinterpret_cast<const uint4*>(p.k_cache + at));
+        v[u] = __ldg(reinterpret_cast<const uint4*>(p.v_cache + at));
+      }
+    }
+    {
+      float f[kPer][16];
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) {
+        codes_to_float(k[u].x, &f[u][0]);
+        codes_to_float(k[u].y, &f[u][4]);
+        codes_to_float(k[u].z, &f[u][8]);
+        codes_to_float(k[u].w, &f[u][12]);
+      }
+#pragma unroll 1
+      for (int g = 0; g < ng; ++g) {
+        float dot[kPer];
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) dot[u] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const float4 q = *reinterpret_cast<const float4*>(&s_q[g][piece * 16 + e]);
+#pragma unroll
+          for (int u = 0; u < kPer; ++u)
+            dot[u] = fmaf(q.w, f[u][e + 3],
+                          fmaf(q.z, f[u][e + 2], fmaf(q.y, f[u][e + 1], fmaf(q.x, f[u][e], dot[u]))));
+        }
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) {
+#pragma unroll
+          for (int b = 1; b < LP; b *= 2) dot[u] += __shfl_xor_sync(0xffffffffu, dot[u], b);
+          const int i = tok0 + u * kAtOnce;
+          if (piece == 0) s_p[g][i] = s_row[i] != kNoRow ? dot[u] * s_ks[i] : -INFINITY;
+        }
+      }
+    }
+    __syncthreads();
+    for (int g = warp; g < ng; g += 4) {
+      const float a = s_p[g][lane], b = s_p[g][lane + 32];
+      const float m_old = s_m[g], m = fmaxf(m_old, warp_max(fmaxf(a, b)));
+      // (a token that does not count weighs 0; a NaN score makes the sum NaN)
+      const float pa = a == -INFINITY ? 0.0f : exp2f(a - m), pb = b == -INFINITY ? 0.0f : exp2f(b - m);
+      const float l = warp_sum(pa + pb);
+      s_p[g][lane] = pa * s_vs[lane];
+      s_p[g][lane + 32] = pb * s_vs[lane + 32];
+      if (lane == 0) {
+        const float alpha = m_old == -INFINITY ? 0.0f : exp2f(m_old - m);
+        s_alpha[g] = alpha;
+        s_l[g] = s_l[g] * alpha + l;
+        s_m[g] = m;
+      }
+    }
+    __syncthreads();
+    {
+      float f[kPer][16];
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) {
+        codes_to_float(v[u].x, &f[u][0]);
+        codes_to_float(v[u].y, &f[u][4]);
+        codes_to_float(v[u].z, &f[u][8]);
+        codes_to_float(v[u].w, &f[u][12]);
+      }
+#pragma unroll 1
+      for (int g = 0; g < ng; ++g) {
+        float part[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) part[e] = 0.0f;
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) {
+          const float w = s_p[g][tok0 + u * kAtOnce];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) part[e] = fmaf(w, f[u][e], part[e]);
+        }
+        // the sum over the warp's tokens, a part of the channels to each lane
+        int n = 16, first = 0;
+#pragma unroll
+        for (int b = 16; b >= LP; b /= 2) {
+          n /= 2;
+          const bool up = lane & b;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e < n) {
+              const float give = up ? part[e] : part[n + e], keep = up ? part[n + e] : part[e];
+              part[e] = keep + __shfl_xor_sync(0xffffffffu, give, b);
+            }
+          if (up) first += n;
+        }
+#pragma unroll
+        for (int e = 0; e < kRed; ++e) s_red[warp][g][piece * 16 + first + e] = part[e];
+      }
+    }
+    __syncthreads();
+    if (tid < D)
+#pragma unroll
+      for (int g = 0; g < kOwnHeads; ++g)
+        if (g < ng)
+          acc[g] = acc[g] * s_alpha[g] +
+                   ((s_red[0][g][tid] + s_red[1][g][tid]) + (s_red[2][g][tid] + s_red[3][g][tid]));
+  }
+  const int64_t slot = ((int64_t)seq * p.splits + split) * p.heads + head0;
+#pragma unroll
+  for (int g = 0; g < kOwnHeads; ++g)
+    if (g < ng && tid < p.dim) p.acc[(slot + g) * p.dim + tid] = acc[g];
+  // nothing attended: (-inf, 0); every score NaN: a NaN that the join keeps
+  if (tid < ng) {
+    const float m = s_m[tid], l = s_l[tid];
+    p.ml[slot + tid] = make_float2(m == -INFINITY && l != 0.0f ? -1e30f : m, l);
+  }
+}
+
 // One warp per (sequence, query head): the prefix's partials, then those of
 // the sequence's own pages, in that order (deterministic).  V = dim / 32.
 template <int V>
@@ -924,12 +1141,22 @@ size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 struct PrefixWs {
   size_t pre_acc, pre_ml, own_acc, own_ml, sums, bytes;
   int splits, own_splits, own_pages;
+  bool own_decode;  // own tokens by the decode split kernels
 };
 
 PrefixWs prefix_ws(const SharedPrefixArgs& a) {
   PrefixWs w;
   w.splits = a.prefix_width > 0 ? prefix_splits(a) : 0;
-  decode_partials_plan(a.own, &w.own_splits, &w.own_pages);
+  w.own_decode = decode_partials_plan(a.own, &w.own_splits, &w.own_pages);
+  if (!w.own_decode) {
+    // Parts of 64 tokens, or longer where the tables are wide (their width says
+    // little about the lengths): at most 8 to 64 parts a sequence.
+    const int64_t units = (int64_t)a.own.num_seqs * a.own.num_kv_heads;
+    const int most = (int)std::min<int64_t>(64, std::max<int64_t>(8, 4736 / std::max<int64_t>(units, 1)));
+    w.own_pages = std::max({1, kOwnTokens / a.own.block_size,
+                            (a.own.max_blocks_per_seq + most - 1) / most});
+    w.own_splits = (a.own.max_blocks_per_seq + w.own_pages - 1) / w.own_pages;
+  }
   if (a.own.max_blocks_per_seq == 0) w.own_splits = 0;
   const size_t rows = (size_t)a.own.num_seqs * a.own.num_heads;
   const size_t pre = rows * w.splits, own = rows * w.own_splits;
@@ -956,6 +1183,50 @@ void launch_prefix_t(const PrefixParams& p, cudaStream_t stream) {
   const int64_t pairs = ((int64_t)p.num_seqs * p.group + 255) / 256;
   const dim3 grid((unsigned)(pairs * p.kv_heads), (unsigned)p.splits);
   kern<<<grid, kPrefixThreads, C::kSmemBytes, stream>>>(p, device_error_word());
+}
+
+int launch_own(const DecodeArgs& o, const PrefixWs& w, float* acc, float2* ml,
+               cudaStream_t stream) {
+  OwnParams p;
+  p.q = o.q;
+  p.k_cache = o.k_cache;
+  p.k_scale = o.k_scale;
+  p.v_cache = o.v_cache;
+  p.v_scale = o.v_scale;
+  p.tables = o.block_tables;
+  p.lens = o.seq_lens;
+  p.acc = acc;
+  p.ml = ml;
+  p.num_blocks = o.num_blocks;
+  p.heads = o.num_heads;
+  p.kv_heads = o.num_kv_heads;
+  p.group = o.num_heads / o.num_kv_heads;
+  p.dim = o.head_dim;
+  p.bs = o.block_size;
+  p.width = o.max_blocks_per_seq;
+  p.pages_per_split = w.own_pages;
+  p.splits = w.own_splits;
+  p.qk_scale = o.sm_scale * kLog2e;
+  const int64_t x = (int64_t)o.num_seqs * w.own_splits;
+  const int64_t y = (int64_t)o.num_kv_heads * ((p.group + kOwnHeads - 1) / kOwnHeads);
+  if (x > 0x7fffffffLL || y > 65535) {
+    set_error("more than 2^31 parts or 65,535 groups of heads");
+    return kUnsupported;
+  }
+  const dim3 grid((unsigned)x, (unsigned)y);
+  int* err = device_error_word();
+  if (o.head_dim == 32)
+    own_kernel<2><<<grid, 128, 0, stream>>>(p, err);
+  else if (o.head_dim == 64)
+    own_kernel<4><<<grid, 128, 0, stream>>>(p, err);
+  else
+    own_kernel<8><<<grid, 128, 0, stream>>>(p, err);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) {
+    set_error(std::string("own tokens launch failed: ") + cudaGetErrorString(e));
+    return kCudaError;
+  }
+  return kOk;
 }
 
 }  // namespace
@@ -1020,7 +1291,8 @@ int launch_shared_prefix(const SharedPrefixArgs& a, void* workspace, size_t work
     }
   }
   if (w.own_splits > 0) {
-    const int rc = launch_decode_partials(o, own_acc, own_ml, stream);
+    const int rc = w.own_decode ? launch_decode_partials(o, own_acc, own_ml, stream)
+                                : launch_own(o, w, own_acc, own_ml, stream);
     if (rc != kOk) return rc;
   }
   const int64_t rows = (int64_t)o.num_seqs * o.num_heads;

@@ -136,6 +136,43 @@ def test_parts_of_many_tiles(cuda, prefix, lens, heads, dim, bs):
     check(problem(prefix + dim, prefix, lens, heads, heads, dim, bs))
 
 
+@pytest.mark.parametrize("prefix,lens,heads,kv_heads,dim,bs,wide", [
+    (40, [3000, 64, 65, 0, 1, 63], 12, 4, 96, 16, 2000),  # parts of more than 64 tokens
+    (0, [1000, 5, 128], 22, 2, 128, 16, 0),               # 11 heads: a group in two parts
+    (16, [700, 300], 5, 5, 32, 8, 3000),
+    (50, [200, 49, 48], 16, 2, 64, 24, 5),                # 48 tokens of 2 pages at a time
+    (50, [200, 64], 3, 3, 64, 64, 0),
+])
+def test_own_tokens_of_any_shape(cuda, prefix, lens, heads, kv_heads, dim, bs, wide):
+    from pagedkv_fusion import _C, ops
+    p = problem(prefix + dim, prefix, lens, heads, kv_heads, dim, bs, wide=wide)
+    want = check(p)
+    for bad in (float("nan"), float("inf")):
+        q = p["q"].clone()
+        q[1, heads - 1] = bad
+        out = ops.shared_prefix_attention(**dict(p, q=q))
+        assert bool((~out[1, heads - 1].isfinite()).all())
+        out[1, heads - 1] = want[1, heads - 1]
+        assert torch.equal(out, want)
+    # tokens on a page outside the cache do not count, nor those past the table
+    tables = p["block_tables"].clone()
+    tables[0, 1] = p["k_cache_q"].shape[0]
+    out = ops.shared_prefix_attention(**dict(p, block_tables=tables))
+    assert _C.read_device_error() == 1
+    kept = dict(p, block_tables=p["block_tables"].clone(), seq_lens=p["seq_lens"].clone())
+    kept["block_tables"][0, 1:-1] = p["block_tables"][0, 2:]
+    kept["seq_lens"][0] -= bs
+    again, tol = reference(kept)
+    assert bool(((out[0].double() - again[0]).abs() <= tol[0]).all())
+    lens = p["seq_lens"].clone()
+    lens[0] = p["block_tables"].shape[1] * bs + 1
+    full = dict(p, block_tables=p["block_tables"].clamp(min=0))
+    out = ops.shared_prefix_attention(**dict(full, seq_lens=lens))
+    assert _C.read_device_error() == 4
+    lens[0] -= 1
+    assert torch.equal(out, ops.shared_prefix_attention(**dict(full, seq_lens=lens)))
+
+
 @pytest.mark.parametrize("prefix,heads,kv_heads,bs", [(1024, 8, 8, 16), (320, 32, 8, 16),
                                                       (96, 8, 2, 32)])
 def test_agrees_with_decode_over_joined_tables(cuda, prefix, heads, kv_heads, bs):
