@@ -601,8 +601,8 @@ __device__ __noinline__ void append_head(const AppendArgs<T>& a, int64_t page, b
     }
 }
 
-// The same for up to kAppendHold tokens of up to 128 channels in 8-channel
-// pieces, half a warp per token (a warp's instruction serves two tokens).  All
+// The same for pages whose rows fit on chip, in 8-channel pieces: half a warp per
+// token (a warp's instruction serves two), or a warp above 128 channels.  All
 // rows of a head are copied to shared memory at once, so inputs are read once
 // and a warp has 4 KB in flight; the rotation is cheap enough to be done
 // again for the codes.  32,768 bf16 tokens of 8 heads in pages of 16: 79 us
@@ -626,26 +626,27 @@ __device__ __forceinline__ void copies_wait() {
 }
 
 // Starts the copies of one head's rows.
-template <typename T>
+template <typename T, int ROW>
 __device__ __forceinline__ void append_fetch8(const AppendArgs<T>& a, bool is_key, int h,
                                               const AppendList& list, T* raw) {
   constexpr int kPer = 16 / sizeof(T);  // values of a 16-byte access
-  const int lane = threadIdx.x & 31, d = (lane & 15) * 8;
+  constexpr int kLanes = ROW / 8;  // of a token
+  const int lane = threadIdx.x & 31, d = lane % kLanes * 8;
   const T* base = (is_key ? a.key + (int64_t)h * a.k_head : a.value + (int64_t)h * a.v_head) + d;
   const int64_t step_tok = is_key ? a.k_tok : a.v_tok;
   if (d < a.dim)
-    for (int i = lane >> 4; i < list.count; i += 2)
+    for (int i = lane / kLanes; i < list.count; i += 32 / kLanes)
 #pragma unroll
       for (int u = 0; u < 8 / kPer; ++u)
-        copy16_async(raw + i * 128 + d + u * kPer, base + list.tok[i] * step_tok + u * kPer);
+        copy16_async(raw + i * ROW + d + u * kPer, base + list.tok[i] * step_tok + u * kPer);
 }
 
-template <typename T, int ROT>
+template <typename T, int ROT, int ROW>
 __device__ __forceinline__ void append_head8(const AppendArgs<T>& a, int64_t page, bool is_key,
                                              int h, const AppendList& list, const T* raw,
                                              const float* table) {
-  constexpr int kPer = 16 / sizeof(T);
-  const int lane = threadIdx.x & 31, sub = lane >> 4, d = (lane & 15) * 8;
+  constexpr int kLanes = ROW / 8;  // of a token
+  const int lane = threadIdx.x & 31, sub = lane / kLanes, d = lane % kLanes * 8;
   const int n = list.count, lowest = list.lowest;
   const bool on = d < a.dim;
   const int64_t tok_stride = (int64_t)a.kv_heads * a.dim;
@@ -662,16 +663,16 @@ __device__ __forceinline__ void append_head8(const AppendArgs<T>& a, int64_t pag
   const int d0 = ROT == kHalves && turned ? d / 2 : d;
   const int d1 = ROT == kHalves && turned ? half + d / 2 : d + 4;
   auto values = [&](int i, float (&y)[8]) {
-    const Chunk<T, 4> x0 = load_chunk<T, 4>(raw + i * 128 + d0);
-    const Chunk<T, 4> x1 = load_chunk<T, 4>(raw + i * 128 + d1);
+    const Chunk<T, 4> x0 = load_chunk<T, 4>(raw + i * ROW + d0);
+    const Chunk<T, 4> x1 = load_chunk<T, 4>(raw + i * ROW + d1);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       y[e] = to_f32<T>(x0.e[e]);
       y[4 + e] = to_f32<T>(x1.e[e]);
     }
     if (ROT == kNoRotation || !turned) return;
-    const float4 c = *reinterpret_cast<const float4*>(table + i * 128 + d / 2);
-    const float4 s = *reinterpret_cast<const float4*>(table + i * 128 + half + d / 2);
+    const float4 c = *reinterpret_cast<const float4*>(table + i * ROW + d / 2);
+    const float4 s = *reinterpret_cast<const float4*>(table + i * ROW + half + d / 2);
     constexpr int kStep = ROT == kPairs ? 2 : 1;  // between the pairs' first values
     constexpr int kOther = ROT == kPairs ? 1 : 4;
 #pragma unroll
@@ -691,7 +692,7 @@ __device__ __forceinline__ void append_head8(const AppendArgs<T>& a, int64_t pag
   float big = 0.0f;
   if (on)
 #pragma unroll 4
-    for (int i = sub; i < n; i += 2) {
+    for (int i = sub; i < n; i += 32 / kLanes) {
       float y[8];
       values(i, y);
 #pragma unroll
@@ -704,7 +705,7 @@ __device__ __forceinline__ void append_head8(const AppendArgs<T>& a, int64_t pag
   const bool fast = isfinite(amax) && !isinf(rcp);
   if (on)
 #pragma unroll 4
-    for (int i = sub; i < n; i += 2) {
+    for (int i = sub; i < n; i += 32 / kLanes) {
       float y[8];
       values(i, y);
       const float lo[4] = {y[0], y[1], y[2], y[3]}, hi[4] = {y[4], y[5], y[6], y[7]};
@@ -730,19 +731,20 @@ __device__ __forceinline__ void append_heads(const AppendArgs<T>& a, int64_t pag
   auto is_key = [&](int r) { return key_part && r < a.kv_heads; };
   auto head = [&](int r) { return r < a.kv_heads ? r : r - a.kv_heads; };
   if (VEC == 8 && list.count <= HOLD) {
+    constexpr int ROW = NC * 128;
     extern __shared__ __align__(16) float s_rows[];  // table rows, then each warp's rows
-    T* raw = reinterpret_cast<T*>(s_rows + HOLD * 128) + warp * BUFS * HOLD * 128;
+    T* raw = reinterpret_cast<T*>(s_rows + HOLD * ROW) + warp * BUFS * HOLD * ROW;
     if (key_part && turns)  // the tokens' table rows, once for all heads
-      for (int i = threadIdx.x; i < list.count * 32; i += kAppendThreads) {
-        const int tok = i / 32, at = (i % 32) * 4;
-        if (at < a.rot) copy16_async(s_rows + tok * 128 + at, a.table + list.pos[tok] * a.rot + at);
+      for (int i = threadIdx.x; i < list.count * (ROW / 4); i += kAppendThreads) {
+        const int tok = i / (ROW / 4), at = i % (ROW / 4) * 4;
+        if (at < a.rot) copy16_async(s_rows + tok * ROW + at, a.table + list.pos[tok] * a.rot + at);
       }
-    if (warp < rows) append_fetch8(a, is_key(warp), head(warp), list, raw);
+    if (warp < rows) append_fetch8<T, ROW>(a, is_key(warp), head(warp), list, raw);
     copies_group();
     for (int r0 = 0, buf = 0; r0 < rows; r0 += kAppendWarps) {
       const int r = r0 + warp, next = r + kAppendWarps;
       if (BUFS == 2) {
-        if (next < rows) append_fetch8(a, is_key(next), head(next), list, raw + (buf ^ 1) * HOLD * 128);
+        if (next < rows) append_fetch8<T, ROW>(a, is_key(next), head(next), list, raw + (buf ^ 1) * HOLD * ROW);
         copies_group();
         copies_wait<1>();
       } else {
@@ -751,18 +753,18 @@ __device__ __forceinline__ void append_heads(const AppendArgs<T>& a, int64_t pag
       if (r0 == 0) __syncthreads();  // the table rows are every warp's copies
       else __syncwarp();
       if (r >= rows) continue;
-      const T* rows_of = raw + buf * HOLD * 128;
+      const T* rows_of = raw + buf * HOLD * ROW;
       if (!is_key(r) || !turns)
-        append_head8<T, kNoRotation>(a, page, is_key(r), head(r), list, rows_of, s_rows);
+        append_head8<T, kNoRotation, ROW>(a, page, is_key(r), head(r), list, rows_of, s_rows);
       else if (a.interleaved)
-        append_head8<T, kPairs>(a, page, true, head(r), list, rows_of, s_rows);
+        append_head8<T, kPairs, ROW>(a, page, true, head(r), list, rows_of, s_rows);
       else
-        append_head8<T, kHalves>(a, page, true, head(r), list, rows_of, s_rows);
+        append_head8<T, kHalves, ROW>(a, page, true, head(r), list, rows_of, s_rows);
       __syncwarp();  // the rows are free for another head
       if (BUFS == 2) {
         buf ^= 1;
       } else if (next < rows) {
-        append_fetch8(a, is_key(next), head(next), list, raw);
+        append_fetch8<T, ROW>(a, is_key(next), head(next), list, raw);
         copies_group();
       }
     }
@@ -827,13 +829,18 @@ __global__ void __launch_bounds__(256)
   if (prev == 0) pages[atomicAdd(count, 1)] = make_int2((int)page, (int)t);
 }
 
-// Rows on chip: two heads of 16 tokens a warp, or one of 32 (block_size up to 32),
-// in 16 bits.
-template <typename T, int HOLD>
-constexpr int kAppendBufs = sizeof(T) == 2 && HOLD == 16 ? 2 : 1;
+// Rows on chip, HOLD tokens of NC x 128 channels: two heads a warp where three CTAs
+// of an SM can have them, else one.
+template <typename T, int NC, int HOLD>
+constexpr int kAppendBufs = HOLD * NC * (int)sizeof(T) <= 32 ? 2 : 1;
+template <typename T, int NC, int HOLD>
+constexpr int kAppendStage =
+    HOLD * NC * 128 * (4 + kAppendWarps * kAppendBufs<T, NC, HOLD> * (int)sizeof(T));
+constexpr int append_ctas(int bytes) { return bytes <= 75 * 1024 ? 3 : bytes <= 112 * 1024 ? 2 : 1; }
 
 template <typename T, int VEC, int NC, int HOLD>
-__global__ void __launch_bounds__(kAppendThreads, VEC == 8 ? (HOLD == 16 ? 3 : 2) : 1)
+__global__ void __launch_bounds__(kAppendThreads,
+                                  VEC == 8 ? append_ctas(kAppendStage<T, NC, HOLD>) : 1)
     append_pages_kernel(AppendArgs<T> a, const int* head, const int* next, const int2* pages,
                         const int* count, int* err) {
   __shared__ int s_tok[kAppendMaxPage];
@@ -867,7 +874,7 @@ __global__ void __launch_bounds__(kAppendThreads, VEC == 8 ? (HOLD == 16 ? 3 : 2
     }
     __syncthreads();
     append_list(a, s_tok, s_list);
-    append_heads<T, VEC, NC, HOLD, kAppendBufs<T, HOLD>>(a, page, true, true, s_list);
+    append_heads<T, VEC, NC, HOLD, kAppendBufs<T, NC, HOLD>>(a, page, true, true, s_list);
   }
 }
 
@@ -876,14 +883,18 @@ constexpr int64_t kAppendScan = 512;
 
 template <typename T, int VEC, int NC>
 void launch_append_n(const AppendArgs<T>& a, int* ws, cudaStream_t stream) {
-  constexpr int kStage = VEC == 8 ? kAppendHold * 128 * (4 + kAppendWarps * (int)sizeof(T)) : 0;
   int* err = device_error_word();
   if (a.tokens <= kAppendScan) {
-    static std::atomic<uint64_t> done{0};
-    allow_shared_memory(reinterpret_cast<const void*>(append_scan_kernel<T, VEC, NC>), kStage, done);
-    append_scan_kernel<T, VEC, NC>
-        <<<(unsigned)(2 * a.tokens), kAppendThreads, kStage, stream>>>(a, err);
-    return;
+    if constexpr (VEC == 8 && NC == 2) {
+      return launch_append_n<T, 4, 2>(a, ws, stream);  // few tokens a page, more CTAs an SM
+    } else {
+      constexpr int kStage = VEC == 8 ? kAppendHold * 128 * (4 + kAppendWarps * (int)sizeof(T)) : 0;
+      auto kernel = append_scan_kernel<T, VEC, NC>;
+      static std::atomic<uint64_t> done{0};
+      allow_shared_memory(reinterpret_cast<const void*>(kernel), kStage, done);
+      kernel<<<(unsigned)(2 * a.tokens), kAppendThreads, kStage, stream>>>(a, err);
+      return;
+    }
   }
   int* head = ws;
   int* count = ws + a.blocks;
@@ -895,15 +906,20 @@ void launch_append_n(const AppendArgs<T>& a, int* ws, cudaStream_t stream) {
   const int64_t ctas = std::min<int64_t>(a.tokens, 8LL * 148);
   auto pages_of = [&](auto hold) {
     constexpr int kHold = decltype(hold)::value;
-    constexpr int kStage = VEC == 8 ? kHold * 128 * (4 + kAppendWarps * kAppendBufs<T, kHold> * (int)sizeof(T)) : 0;
+    constexpr int kStage = VEC == 8 ? kAppendStage<T, NC, kHold> : 0;
+    static_assert(kStage <= 227 * 1024 - 4096, "shared memory");
     auto kernel = append_pages_kernel<T, VEC, NC, kHold>;
     static std::atomic<uint64_t> done{0};
     allow_shared_memory(reinterpret_cast<const void*>(kernel), kStage, done);
     kernel<<<(unsigned)ctas, kAppendThreads, kStage, stream>>>(a, head, next, pages, count, err);
   };
-  // 16,384 bf16 tokens of 8 heads in pages of 32 take 62 us a call so, 162 us with
-  // their rows read twice (append_head).
-  if constexpr (VEC == 8 && sizeof(T) == 2) {
+  // Larger pages are kept whole as far as shared memory goes.  16,384 tokens of 8
+  // heads, us a call, against rows read twice (append_head): bf16 in pages of 32 61
+  // and 162, of 64 82 and 175; fp32 in pages of 32 84 and 168.
+  if constexpr (VEC == 8 && sizeof(T) * NC <= 2) {
+    if (a.bs > 32) return pages_of(std::integral_constant<int, 64>{});
+  }
+  if constexpr (VEC == 8 && sizeof(T) * NC <= 4) {
     if (a.bs > kAppendHold) return pages_of(std::integral_constant<int, 32>{});
   }
   pages_of(std::integral_constant<int, kAppendHold>{});
@@ -938,9 +954,9 @@ int launch_append_t(const AppendKvArgs& p, int* ws, cudaStream_t stream) {
   };
   // whole pieces are rotated, and table rows are read four values at a time
   const bool halves = a.rot > 0 && !a.interleaved;
-  if (a.dim <= 128 && rows_of(8, 16) && aligned(a.cache, 8) &&
-      (a.rot % 8 == 0 && (a.rot == 0 || aligned(a.table, 16))))
-    launch_append_n<T, 8, 1>(a, ws, stream);
+  if (rows_of(8, 16) && aligned(a.cache, 8) && a.rot % 8 == 0 &&
+      (a.rot == 0 || aligned(a.table, 16)))
+    a.dim <= 128 ? launch_append_n<T, 8, 1>(a, ws, stream) : launch_append_n<T, 8, 2>(a, ws, stream);
   else if (rows_of(4, 4 * (int)sizeof(T)) && aligned(a.cache, 4) &&
            (!halves || (a.rot % 8 == 0 && aligned(a.table, 16))))
     launch_append_n<T, 4, 2>(a, ws, stream);

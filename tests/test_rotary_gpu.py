@@ -267,6 +267,11 @@ def test_append_kv(cuda, dtype, counts, fills, kv_heads, dim, bs, rot, interleav
     ([560], [0], 12, 128, 16, 72, False),         # 24 heads for 8 warps
     ([14, 2], [2, 0], 9, 128, 16, 40, False),
     ([600], [0], 3, 128, 16, 12, True),           # half a piece rotated
+    ([700, 33], [0, 7], 3, 256, 16, 256, False),  # a token for a whole warp
+    ([600], [3], 2, 192, 16, 96, True),
+    ([600], [0], 2, 256, 32, 64, False),
+    ([700, 65], [5, 0], 3, 128, 64, 128, False),  # pages of 64 tokens
+    ([640], [0], 2, 256, 64, 8, True),
 ])
 def test_append_kv_whole_pages(cuda, dtype, counts, fills, kv_heads, dim, bs, rot, interleaved):
     key, value, cache, scales, slots, pos, table = append_problem(
