@@ -3341,6 +3341,11 @@ Plan make_plan(const DecodeArgs& a, bool partials = false) {
   p.fast = a.head_dim == 128 && (a.block_size == 16 || a.block_size == 32) && g_ok && aligned &&
            (int64_t)a.num_blocks * a.block_size < (int64_t)1 << 31 && env_int("PKV_DECODE_GENERIC", 0) == 0;
   const int M = a.max_blocks_per_seq;
+  // CTAs to split for.  Partials are always joined, by a kernel that also has the
+  // prefix's, so half as many pay: behind a prefix of 1,000 tokens 96 sequences of 5
+  // to 300 tokens with 16 KV heads take 45.6 us, 51.3 at 888; 4 of 20 to 6,000 with 8
+  // 36 us and 40 (one of 8,000 and 15 of 100, 8 query heads: 45.8 us and 44.1).
+  const int64_t target = env_int("PKV_DECODE_TARGET_CTAS", partials ? 444 : 888);
   if (p.fast) {
     p.g = group;
     const int cap = std::min(128 / a.block_size, 16 / group);
@@ -3352,7 +3357,6 @@ Plan make_plan(const DecodeArgs& a, bool partials = false) {
     const int max_pages = (p.hg * p.g <= 8 ? 512 : 256) / a.block_size;
     const int groups = a.num_kv_heads / p.hg;
     int pps = max_pages;
-    const int64_t target = env_int("PKV_DECODE_TARGET_CTAS", 888);
     while (pps > pps_stage && (int64_t)a.num_seqs * groups * ((M + pps - 1) / pps) < target)
       pps /= 2;
     const int forced = env_int("PKV_DECODE_SPLIT_PAGES", 0);
@@ -3388,8 +3392,7 @@ Plan make_plan(const DecodeArgs& a, bool partials = false) {
     // one CTA per (sequence, KV head, split of 8..32 pages)
     p.tc = true;
     int pps = group <= 4 ? TcCfg<4>::kMaxPages : TcCfg<8>::kMaxPages;
-    while (pps > 8 && (int64_t)a.num_seqs * a.num_kv_heads * ((M + pps - 1) / pps) <
-                          env_int("PKV_DECODE_TARGET_CTAS", 888))
+    while (pps > 8 && (int64_t)a.num_seqs * a.num_kv_heads * ((M + pps - 1) / pps) < target)
       pps /= 2;
     const int forced = env_int("PKV_DECODE_SPLIT_PAGES", 0);
     if (forced > 0)
