@@ -2,8 +2,9 @@
 // over the keys j of token i's sequence, causal from the sequences' ends
 // (j <= i + Lk - Lq), grouped heads, fp16 or bf16 with fp32 accumulators.
 //
-// An item of work is two row tiles of 128 rows of one KV head; one CTA per SM
-// takes items until none is left.  A row is a (token,
+// An item of work is two row tiles of 128 rows of one KV head (one row tile in calls
+// that would leave half of the SMs without); one CTA per SM takes items until none
+// is left.  A row is a (token,
 // query head of the group) pair, so the G heads of a group share every K / V
 // tile that is loaded.  Keys come in tiles of 128 tokens; per row tile
 //   S = Q K^T    tcgen05 kind::f16, 128 x 128, K-major A and B from shared
@@ -94,6 +95,7 @@ struct PreParams {
   int64_t v_tok, v_head;
   int num_seqs, total_q, total_k;
   int heads, kv_heads, group, dim, tile_tokens;
+  int item_tiles;  // row tiles of an item: 2, or 1 in calls of few items
   float scale_log2, scale;
   int causal;
 };
@@ -122,7 +124,7 @@ __device__ __forceinline__ void count_tiles(const PreParams& p, PreItem& w) {
     const int first = w.at.t0 + x * p.tile_tokens;
     const int last = min(first + p.tile_tokens, w.at.lq) - 1;
     const int keys =
-        first < w.at.lq ? (p.causal ? min(max(last + shift + 1, 0), w.at.lk) : w.at.lk) : 0;
+        first < w.at.lq && x < p.item_tiles ? (p.causal ? min(max(last + shift + 1, 0), w.at.lk) : w.at.lk) : 0;
     w.n_tiles[x] = (keys + kKeys - 1) / kKeys;
   }
   w.n = max(w.n_tiles[0], w.n_tiles[1]);
@@ -152,14 +154,14 @@ __device__ __forceinline__ int granted_block(const void* answer) {
   return got ? (int)x : -1;
 }
 
-// Sequence and token range of pair `pair` (of 2 * tile_tokens tokens).  Pairs
+// Sequence and token range of pair `pair` (of item_tiles * tile_tokens tokens).  Pairs
 // are numbered sequence by sequence, the last pair of a sequence first: under
 // a causal mask it is the longest, and long work should start early.  The rows
 // behind the last sequence form one more sequence without keys (zeros).
 // One warp; false when `pair` is past the end.
 __device__ __forceinline__ bool find_work(const PreParams& p, int pair, PreWork& w, int* err) {
   const int lane = threadIdx.x & 31;
-  const int span = 2 * p.tile_tokens;
+  const int span = p.item_tiles * p.tile_tokens;
   int base = 0;
   for (int s0 = 0; s0 <= p.num_seqs; s0 += 32) {
     const int s = s0 + lane;
@@ -585,7 +587,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       bool valid;
       {
         const int tok = w.at.t0 + x * p.tile_tokens + row_tok, lq = w.at.lq, lk = w.at.lk;
-        valid = row_tok < p.tile_tokens && tok < lq;
+        valid = row_tok < p.tile_tokens && tok < lq && x < p.item_tiles;
         if (valid) limit = p.causal ? min(tok + lk - lq + 1, lk) : lk;
       }
       float m = -INFINITY, l = 0.0f;
@@ -678,7 +680,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       uint8_t* stage = smem + C::kOffOut + x * C::kStageBytes;
       uint8_t* mine = stage + row * 128;
       const int tok0 = w.at.t0 + x * p.tile_tokens;
-      const int rows = min(p.tile_tokens, max(w.at.lq - tok0, 0)) * p.group;
+      const int rows =
+          x < p.item_tiles ? min(p.tile_tokens, max(w.at.lq - tok0, 0)) * p.group : 0;
 #pragma unroll 1
       for (int c0 = 0; c0 < DP; c0 += 64) {
         named_barrier(2 + x, 128);  // the buffer is free
@@ -819,10 +822,16 @@ int launch_prefill_t(const PrefillArgs& a, cudaStream_t stream) {
   auto kern = prefill_kernel<T, DP>;
   static std::atomic<uint64_t> done{0};
   allow_shared_memory(reinterpret_cast<const void*>(kern), C::kSmemBytes, done);
-  // pairs of row tiles: at most this many over all sequences (and the rest)
-  const int span = 2 * p.tile_tokens;
-  const int64_t pairs = a.total_q / span + std::min<int64_t>(a.num_seqs + 1, a.total_q);
-  kern<<<(unsigned)(pairs * a.kv_heads), kPreThreads, C::kSmemBytes, stream>>>(
+  // at most so many items over all sequences (and the rest)
+  auto items = [&](int tiles) {
+    return (a.total_q / (tiles * p.tile_tokens) + std::min<int64_t>(a.num_seqs + 1, a.total_q)) *
+           a.kv_heads;
+  };
+  // While half of the 148 SMs have no item, an item is one row tile: 1,500 tokens of
+  // 8 heads take 30.5 us a call, 34.5 in pairs; 100 tokens behind 4,900 keys, 32 / 8
+  // heads, 77.5 us and 84.6.
+  p.item_tiles = items(2) <= 148 / 2 ? 1 : 2;
+  kern<<<(unsigned)items(p.item_tiles), kPreThreads, C::kSmemBytes, stream>>>(
       mq, mk, mv, p, device_error_word());
   return kOk;
 }
