@@ -114,6 +114,7 @@ struct PreItem {
   int n;             // the larger; 0: nothing to load
   int first_masked;  // tiles from here on hold keys that some row does not see
   int kind;          // kNone: past the end of the work, kSome, kStop: the CTA is done
+  int check;         // the grid's first item: its CTA checks the sequences' ends
 };
 enum ItemKind { kNone = 0, kSome = 1, kStop = 2 };
 
@@ -159,7 +160,7 @@ __device__ __forceinline__ int granted_block(const void* answer) {
 // a causal mask it is the longest, and long work should start early.  The rows
 // behind the last sequence form one more sequence without keys (zeros).
 // One warp; false when `pair` is past the end.
-__device__ __forceinline__ bool find_work(const PreParams& p, int pair, PreWork& w, int* err) {
+__device__ __forceinline__ bool find_work(const PreParams& p, int pair, PreWork& w) {
   const int lane = threadIdx.x & 31;
   const int span = p.item_tiles * p.tile_tokens;
   int base = 0;
@@ -172,8 +173,6 @@ __device__ __forceinline__ bool find_work(const PreParams& p, int pair, PreWork&
       q1 = min(max(b, q0), p.total_q);
       k0 = min(max(ka, 0), p.total_k);
       k1 = min(max(kb, k0), p.total_k);
-      if (pair == 0 && (a != q0 || b != q1 || ka != k0 || kb != k1))
-        record_error(err, kDevBadSeqlens);
     } else if (s == p.num_seqs) {
       q0 = min(max(p.cu_q[s], 0), p.total_q);
       q1 = p.total_q;
@@ -201,6 +200,18 @@ __device__ __forceinline__ bool find_work(const PreParams& p, int pair, PreWork&
     base += total;
   }
   return false;
+}
+
+// Reports cu_seqlens that do not ascend within the tensors, every entry, by `n`
+// threads.  (Apart from find_work, which stops at the pair that it looks for.)
+__device__ __forceinline__ void check_seqlens(const PreParams& p, int thread, int n, int* err) {
+  bool bad = false;
+  for (int s = thread; s <= p.num_seqs; s += n) {
+    const int q = p.cu_q[s], k = p.cu_k[s];
+    bad |= q < (s > 0 ? p.cu_q[s - 1] : 0) || q > p.total_q;
+    bad |= k < (s > 0 ? p.cu_k[s - 1] : 0) || k > p.total_k;
+  }
+  if (bad) record_error(err, kDevBadSeqlens);
 }
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
@@ -356,7 +367,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       PreItem w = {};
       for (; block >= 0 && ok; ++k) {
         w.kvh = block % p.kv_heads;
-        w.kind = find_work(p, block / p.kv_heads, w.at, err) ? kSome : kNone;
+        w.kind = find_work(p, block / p.kv_heads, w.at) ? kSome : kNone;
+        w.check = block == 0;
         if (w.kind == kNone) w.n = w.n_tiles[0] = w.n_tiles[1] = w.first_masked = 0;
         else count_tiles(p, w);
         publish(w);
@@ -558,6 +570,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           if (ct == 0) mbar_arrive(&kv_full[stage_of(2 * j + 1)]);
         }
         base += 2 * n;
+        if (w.check) check_seqlens(p, ct, kCleaners, err);
         item_done(k);
       }
     }
