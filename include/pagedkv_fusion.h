@@ -362,7 +362,8 @@ int pkv_append_kv(const void *key, const void *value, int32_t dtype,
  * are in elements, multiples of 8, pointers 16-byte aligned, channels
  * contiguous, out contiguous.  head_dim a multiple of 8 up to 128, at most
  * 128 query heads per KV head, sm_scale > 0.  cu_seqlens that do not ascend
- * within the tensors record PKV_DEVERR_BAD_SEQLENS and are clamped.
+ * within the tensors record PKV_DEVERR_BAD_SEQLENS and are cut to the tensors
+ * and to the largest entry before them.
  */
 int pkv_prefill_attention(const void *q, const void *k, const void *v,
                           int32_t dtype, void *out, float *lse,

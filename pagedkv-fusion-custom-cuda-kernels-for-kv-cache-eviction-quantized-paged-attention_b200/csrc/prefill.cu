@@ -163,20 +163,38 @@ __device__ __forceinline__ int granted_block(const void* answer) {
 __device__ __forceinline__ bool find_work(const PreParams& p, int pair, PreWork& w) {
   const int lane = threadIdx.x & 31;
   const int span = p.item_tiles * p.tile_tokens;
-  int base = 0;
+  int base = 0, q_end = 0, k_end = 0;  // the largest ends so far
   for (int s0 = 0; s0 <= p.num_seqs; s0 += 32) {
     const int s = s0 + lane;
     int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
-    if (s < p.num_seqs) {
-      const int a = p.cu_q[s], b = p.cu_q[s + 1], ka = p.cu_k[s], kb = p.cu_k[s + 1];
-      q0 = min(max(a, 0), p.total_q);
-      q1 = min(max(b, q0), p.total_q);
-      k0 = min(max(ka, 0), p.total_k);
-      k1 = min(max(kb, k0), p.total_k);
-    } else if (s == p.num_seqs) {
+    if (s <= p.num_seqs) {
+      const bool rest = s == p.num_seqs;
       q0 = min(max(p.cu_q[s], 0), p.total_q);
-      q1 = p.total_q;
+      k0 = min(max(p.cu_k[s], 0), p.total_k);
+      q1 = rest ? p.total_q : min(max(p.cu_q[s + 1], 0), p.total_q);
+      k1 = rest ? k0 : min(max(p.cu_k[s + 1], 0), p.total_k);
     }
+    // An entry below an earlier one counts as the largest before it: sequences then
+    // share no row, and all of them together have no more items than the grid.
+    const bool falls = q1 < q0 || k1 < k0 || (lane == 0 && (q0 < q_end || k0 < k_end));
+    if (__any_sync(0xffffffffu, falls)) {
+      int qm = max(max(q0, q1), q_end), km = max(max(k0, k1), k_end);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int a = __shfl_up_sync(0xffffffffu, qm, o), b = __shfl_up_sync(0xffffffffu, km, o);
+        if (lane >= o) {
+          qm = max(qm, a);
+          km = max(km, b);
+        }
+      }
+      const int a = __shfl_up_sync(0xffffffffu, qm, 1), b = __shfl_up_sync(0xffffffffu, km, 1);
+      q0 = lane > 0 ? a : max(q0, q_end);
+      k0 = lane > 0 ? b : max(k0, k_end);
+      q1 = s <= p.num_seqs ? qm : q0;
+      k1 = s < p.num_seqs ? km : k0;
+    }
+    q_end = __shfl_sync(0xffffffffu, q1, 31);
+    k_end = __shfl_sync(0xffffffffu, k1, 31);
     const int n = (q1 - q0 + span - 1) / span;
     int incl = n;
 #pragma unroll

@@ -1,9 +1,12 @@
 """prefill_attention's cu_seqlens: lists of more than 32 sequences that do not
-ascend within the tensors are reported wherever the mistake is.
+ascend within the tensors are reported wherever the mistake is, and give what
+the list gives whose entries are cut to the tensors and to the largest before
+them: every row is written, by one sequence.
 """
 
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
@@ -46,3 +49,50 @@ def test_empty_sequences_and_thousands_are_no_mistake(cuda):
     assert cuda.read_device_error() == 0
     ops.prefill_attention(q, k, v, entries([-1]), 0.1)
     assert cuda.read_device_error() == 6
+
+
+def ragged(rng, n, top):
+    """A list of n + 1 entries that rises, falls and leaves [0, top]."""
+    up = np.sort(rng.integers(0, top + 1, n + 1))
+    for at in rng.integers(0, n + 1, max(2, n // 8)):
+        up[at] = rng.integers(-20, top + 100)
+    return up.tolist()
+
+
+def cut(values, top):
+    return np.maximum.accumulate(np.clip(values, 0, top)).tolist()
+
+
+def filled_with_nan(t):
+    """Freed memory of t's size that holds NaN, which the next output gets."""
+    t = torch.full_like(t, float("nan"))
+    torch.cuda.synchronize()
+    del t
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("q_list,k_list", [
+    ([0, 300] * 20 + [300], None),     # the same rows again and again: more items than the grid
+    ([0, 300, 0, 0, 150, 100, 300], None),
+    ([0, 100, 50, 400], [0, 100, 200, 350]),
+    ([0, 100, 200, 350], [0, 200, 100, 400]),
+    ([0, 900, 120], None),
+    ("ragged", "ragged"),
+    ("ragged", None),
+])
+def test_falling_entries_share_no_rows(cuda, dtype, q_list, k_list):
+    from pagedkv_fusion import ops
+    rng = np.random.default_rng(3)
+    q, k, v = problem(7, [400], [400], 8, 2, 64, dtype)
+    for n in ((5, 40, 130) if q_list == "ragged" else (0,)):
+        cq = ragged(rng, n, 400) if n else q_list
+        ck = ragged(rng, n, 400) if k_list == "ragged" else (k_list or cq)
+        good = [entries(cut(c, 400)) for c in (cq, ck)]
+        want, lse = ops.prefill_attention(q, k, v, good[0], 0.1, cu_seqlens_k=good[1], return_lse=True)
+        assert cuda.read_device_error() == 0
+        filled_with_nan(q)
+        out, got = ops.prefill_attention(q, k, v, entries(cq), 0.1, cu_seqlens_k=entries(ck),
+                                         return_lse=True)
+        assert cuda.read_device_error() == 6
+        first = good[0][0]  # (rows in front of the first sequence are not its)
+        assert torch.equal(out[first:], want[first:]) and torch.equal(got[first:], lse[first:])
