@@ -355,8 +355,8 @@ int pkv_append_kv(const void *key, const void *value, int32_t dtype,
  * cu_seqlens_k[s + 1] of k and v (int32 [num_seqs + 1]).  Under `causal`,
  * token i of a sequence of Lq tokens and Lk keys sees keys j <= i + Lk - Lq
  * (a chunk of a longer prompt is a sequence with more keys than tokens).
- * Rows that see no key, and rows of q behind the last sequence, become zero,
- * with lse -inf; lse (nullable, float32 [total_q, num_heads]) is the natural
+ * Rows that see no key, and rows of q behind the last sequence or in front of
+ * the first, become zero, with lse -inf; lse (nullable, float32 [total_q, num_heads]) is the natural
  * logarithm of the softmax denominator.  Values of keys that a row does not
  * see, NaN and infinities included, do not reach it.  Token and head strides
  * are in elements, multiples of 8, pointers 16-byte aligned, channels

@@ -508,7 +508,8 @@ int pkv_prefill_attention(const void* q, const void* k, const void* v, int32_t d
   if (!(sm_scale > 0.0f) || sm_scale > 3.0e38f)
     return fail(PKV_ERR_INVALID_ARGUMENT, "sm_scale must be positive and finite");
   if (total_q > 0x7fffffffLL - 256 || total_k > 0x7fffffffLL - 256 ||
-      (total_q + num_seqs + 1) * (int64_t)num_kv_heads > 0x7fffffffLL)
+      num_seqs > 0x7fffffff - 256 ||
+      (total_q + num_seqs + 2) * (int64_t)num_kv_heads > 0x7fffffffLL)
     return fail(PKV_ERR_UNSUPPORTED, "too many rows for one call");
   if (total_q == 0) return PKV_OK;
   if (!q || !out || !cu_seqlens_q || !cu_seqlens_k || (total_k > 0 && (!k || !v)))

@@ -158,13 +158,14 @@ __device__ __forceinline__ int granted_block(const void* answer) {
 // Sequence and token range of pair `pair` (of item_tiles * tile_tokens tokens).  Pairs
 // are numbered sequence by sequence, the last pair of a sequence first: under
 // a causal mask it is the longest, and long work should start early.  The rows
-// behind the last sequence form one more sequence without keys (zeros).
+// behind the last sequence and those in front of the first form two more
+// sequences without keys (zeros).
 // One warp; false when `pair` is past the end.
 __device__ __forceinline__ bool find_work(const PreParams& p, int pair, PreWork& w) {
   const int lane = threadIdx.x & 31;
   const int span = p.item_tiles * p.tile_tokens;
   int base = 0, q_end = 0, k_end = 0;  // the largest ends so far
-  for (int s0 = 0; s0 <= p.num_seqs; s0 += 32) {
+  for (int s0 = 0; s0 <= p.num_seqs + 1; s0 += 32) {
     const int s = s0 + lane;
     int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
     if (s <= p.num_seqs) {
@@ -192,6 +193,10 @@ __device__ __forceinline__ bool find_work(const PreParams& p, int pair, PreWork&
       k0 = lane > 0 ? b : max(k0, k_end);
       q1 = s <= p.num_seqs ? qm : q0;
       k1 = s < p.num_seqs ? km : k0;
+    }
+    if (s == p.num_seqs + 1) {  // in front of the first
+      q0 = k0 = k1 = 0;
+      q1 = min(max(p.cu_q[0], 0), p.total_q);
     }
     q_end = __shfl_sync(0xffffffffu, q1, 31);
     k_end = __shfl_sync(0xffffffffu, k1, 31);
@@ -853,16 +858,16 @@ int launch_prefill_t(const PrefillArgs& a, cudaStream_t stream) {
   auto kern = prefill_kernel<T, DP>;
   static std::atomic<uint64_t> done{0};
   allow_shared_memory(reinterpret_cast<const void*>(kern), C::kSmemBytes, done);
-  // at most so many items over all sequences (and the rest)
-  auto items = [&](int tiles) {
-    return (a.total_q / (tiles * p.tile_tokens) + std::min<int64_t>(a.num_seqs + 1, a.total_q)) *
-           a.kv_heads;
+  // at most so many items over so many sequences
+  auto items = [&](int tiles, int64_t seqs) {
+    return (a.total_q / (tiles * p.tile_tokens) + std::min(seqs, a.total_q)) * a.kv_heads;
   };
   // While half of the 148 SMs have no item, an item is one row tile: 1,500 tokens of
   // 8 heads take 30.5 us a call, 34.5 in pairs; 100 tokens behind 4,900 keys, 32 / 8
   // heads, 77.5 us and 84.6.
-  p.item_tiles = items(2) <= 148 / 2 ? 1 : 2;
-  kern<<<(unsigned)items(p.item_tiles), kPreThreads, C::kSmemBytes, stream>>>(
+  p.item_tiles = items(2, (int64_t)a.num_seqs + 1) <= 148 / 2 ? 1 : 2;
+  // (with the rows behind and in front of all sequences)
+  kern<<<(unsigned)items(p.item_tiles, (int64_t)a.num_seqs + 2), kPreThreads, C::kSmemBytes, stream>>>(
       mq, mk, mv, p, device_error_word());
   return kOk;
 }

@@ -402,8 +402,8 @@ def prefill_attention(q, k, v, cu_seqlens, sm_scale: float, cu_seqlens_k=None,
 
     Returns ``[total_q, H, D]`` in the inputs' type, and with ``return_lse``
     also the float32 ``[total_q, H]`` logarithms of the softmax denominators.
-    Rows that see no key, and rows behind the last sequence, are zero (lse
-    -inf).  What a row does not see does not reach it, whatever its value.
+    Rows that see no key, and rows behind the last sequence or in front of the
+    first, are zero (lse -inf).  What a row does not see does not reach it, whatever its value.
     No backward pass.
     """
     C = _lib()

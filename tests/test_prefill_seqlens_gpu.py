@@ -1,7 +1,8 @@
 """prefill_attention's cu_seqlens: lists of more than 32 sequences that do not
 ascend within the tensors are reported wherever the mistake is, and give what
 the list gives whose entries are cut to the tensors and to the largest before
-them: every row is written, by one sequence.
+them: every row is written, by one sequence.  Rows in front of the first
+sequence are zero, as those behind the last are.
 """
 
 from __future__ import annotations
@@ -96,3 +97,24 @@ def test_falling_entries_share_no_rows(cuda, dtype, q_list, k_list):
         assert cuda.read_device_error() == 6
         first = good[0][0]  # (rows in front of the first sequence are not its)
         assert torch.equal(out[first:], want[first:]) and torch.equal(got[first:], lse[first:])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("rows,cu", [
+    (100, [10, 60]), (100, [10, 60, 100]), (100, [100]), (100, [37]), (100, [100, 100, 100]),
+    (5000, [4990, 4995]), (700, [1] + [1 + 22 * i for i in range(1, 31)]),
+    (700, [300] + [300 + 10 * i for i in range(1, 41)]), (300, [500, 600]),
+])
+def test_rows_in_front_of_the_first_sequence(cuda, dtype, rows, cu):
+    import math
+    from pagedkv_fusion import ops
+    q, k, v = problem(rows, [rows], [rows], 8, 2, 64, dtype)
+    filled_with_nan(q)
+    out, lse = ops.prefill_attention(q, k, v, entries(cu), 0.1, return_lse=True)
+    a, b = min(cu[0], rows), min(cu[-1], rows)
+    assert cuda.read_device_error() == (6 if cu[-1] > rows else 0)
+    for rest in (slice(0, a), slice(b, None)):
+        assert bool((out[rest] == 0).all()) and bool((lse[rest] == -math.inf).all())
+    if b > a:
+        want, wlse = ops.prefill_attention(q[a:b], k[a:b], v[a:b], entries(cu) - a, 0.1, return_lse=True)
+        assert torch.equal(out[a:b], want) and torch.equal(lse[a:b], wlse)
