@@ -556,6 +556,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         const PreItem& w = s_item[k & 1];
         const int n = w.n, first_masked = w.first_masked, lk = w.at.lk;
         uint32_t* flags = s_flags + (k & 1) * kMaskedTiles * 4;
+        if (w.check) check_seqlens(p, ct, kCleaners, err);  // beside the first loads
         for (int j = first_masked; j < n; ++j, ++cleaned) {
           wait(&raw_full[cleaned % kMaskedTiles], cleaned / kMaskedTiles);
           if (ok) {
@@ -593,7 +594,6 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           if (ct == 0) mbar_arrive(&kv_full[stage_of(2 * j + 1)]);
         }
         base += 2 * n;
-        if (w.check) check_seqlens(p, ct, kCleaners, err);
         item_done(k);
       }
     }
