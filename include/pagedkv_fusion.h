@@ -383,11 +383,11 @@ int pkv_prefill_attention(const void *q, const void *k, const void *v,
  * prefix_table (int32 [prefix_blocks], pages shared by every sequence, the
  * last one possibly partial) and the sequence's own seq_lens[s] tokens through
  * block_tables[s].  The prefix's pages are read once for the batch.  A
- * sequence without any token yields zeros.  A prefix_len beyond the table
- * records PKV_DEVERR_SEQ_TOO_LONG and is cut to it; tokens on a page outside
- * the cache record PKV_DEVERR_BAD_BLOCK_ID and are not attended.  Envelope:
- * head_dim % 32 == 0 and <= 128, block_size <= 64, num_heads % num_kv_heads
- * == 0; q, out and the caches 16-byte aligned.  prefix_blocks and
+ * sequence without any token yields zeros.  A prefix_len or a sequence's length
+ * beyond its table records PKV_DEVERR_SEQ_TOO_LONG and is cut to it; tokens on
+ * a page outside the cache record PKV_DEVERR_BAD_BLOCK_ID and are not attended.
+ * Envelope: head_dim % 32 == 0 and <= 128, block_size <= 64, num_heads %
+ * num_kv_heads == 0; q, out and the caches 16-byte aligned.  prefix_blocks and
  * max_blocks_per_seq may be 0.  The workspace holds the partial results and
  * needs no initialisation.
  */

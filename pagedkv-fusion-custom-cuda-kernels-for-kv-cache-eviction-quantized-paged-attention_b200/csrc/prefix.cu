@@ -1048,18 +1048,25 @@ __global__ void __launch_bounds__(128) own_kernel(const OwnParams p, int* err) {
 
 // One warp per (sequence, query head): the prefix's partials, then those of
 // the sequence's own pages, in that order (deterministic).  V = dim / 32.
+// Tables without any page have no kernel that reports lengths beyond them, so
+// this one does.
 template <int V>
 __global__ void __launch_bounds__(128)
     join_kernel(const int32_t* __restrict__ seq_lens, const float* __restrict__ pre_acc,
                 const float2* __restrict__ pre_ml, int pre_splits, const float* __restrict__ own_acc,
                 const float2* __restrict__ own_ml, float* __restrict__ out, int num_seqs, int heads,
-                int bs, int width, int pages_per_split, int own_splits) {
+                int bs, int width, int pages_per_split, int own_splits,
+                const int32_t* __restrict__ prefix_len, int* err) {
   constexpr int D = 32 * V;
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int64_t rows = (int64_t)num_seqs * heads;
   if (row >= rows) return;  // whole warps
   const int seq = (int)(row / heads), head = (int)(row - (int64_t)seq * heads);
+  if (lane == 0 && head == 0 &&
+      ((own_splits == 0 && seq_lens[seq] > 0) ||
+       (seq == 0 && pre_splits == 0 && prefix_len != nullptr && *prefix_len > 0)))
+    record_error(err, kDevSeqTooLong);
   const int pages = covered_pages(seq_lens[seq], bs, width);
   const int n_own = own_splits > 0 ? (pages + pages_per_split - 1) / pages_per_split : 0;
   const int n = pre_splits + n_own;
@@ -1302,7 +1309,7 @@ int launch_shared_prefix(const SharedPrefixArgs& a, void* workspace, size_t work
     join_kernel<V><<<grid, 128, 0, stream>>>(o.seq_lens, pre_acc, pre_ml, w.splits, own_acc,     \
                                              own_ml, o.out, o.num_seqs, o.num_heads,             \
                                              o.block_size, o.max_blocks_per_seq, w.own_pages,    \
-                                             w.own_splits);                                      \
+                                             w.own_splits, a.prefix_len, device_error_word());   \
     break;
   switch (o.head_dim / 32) {
     PKV_JOIN(1) PKV_JOIN(2) PKV_JOIN(3) PKV_JOIN(4)
