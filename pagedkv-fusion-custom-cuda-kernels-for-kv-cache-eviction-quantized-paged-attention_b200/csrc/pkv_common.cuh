@@ -33,9 +33,10 @@ enum DeviceError : int {
 
 // Pages a decode split may read for a sequence: ceil(L / bs), clamped to the
 // block-table width (a longer seq_len is recorded as kDevSeqTooLong and only
-// the covered tokens are attended).  Negative lengths count as 0.
+// the covered tokens are attended).  Negative lengths count as 0.  (L + bs - 1
+// would overflow for the largest lengths.)
 __device__ __forceinline__ int covered_pages(int L, int bs, int max_blocks_per_seq) {
-  const int want = L > 0 ? (L + bs - 1) / bs : 0;
+  const int want = L > 0 ? (L - 1) / bs + 1 : 0;
   return want < max_blocks_per_seq ? want : max_blocks_per_seq;
 }
 

@@ -45,3 +45,28 @@ def test_lengths_beyond_tables_without_pages(cuda, heads, kv_heads, dim, bs):
     assert bool((call(**none) == 0).all()) and cuda.read_device_error() == 4
     assert bool((call(**none, seq_lens=zero, prefix_len=torch.zeros_like(p["prefix_len"])) == 0).all())
     assert cuda.read_device_error() == 0
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,bs", [(8, 8, 128, 16), (32, 8, 128, 16), (8, 2, 128, 32),
+                                                   (6, 2, 96, 16), (14, 2, 64, 64)])
+def test_the_largest_lengths_are_cut_to_the_table(cuda, heads, kv_heads, dim, bs):
+    """Lengths whose number of pages, rounded up, does not fit in 32 bits."""
+    from pagedkv_fusion import ops
+    p = problem(2, 100, [9, 40, 200], heads, kv_heads, dim, bs)
+    p["block_tables"].clamp_(min=0)
+    covered = p["block_tables"].shape[1] * bs
+    decode = {k: p[k] for k in p if not k.startswith("prefix")}
+    for i in range(3):
+        full, huge = p["seq_lens"].clone(), p["seq_lens"].clone()
+        full[i] = covered
+        for n in (2 ** 31 - 1, 2 ** 31 - bs, covered + 1):
+            huge[i] = n
+            for call, args in ((ops.shared_prefix_attention, p), (ops.quant_paged_attention, decode)):
+                want = call(**dict(args, seq_lens=full))
+                assert cuda.read_device_error() == 0
+                assert torch.equal(call(**dict(args, seq_lens=huge)), want), (call.__name__, i, n)
+                assert cuda.read_device_error() == 4
+    want = ops.shared_prefix_attention(**dict(p, prefix_len=p["prefix_len"] * 0 + len(p["prefix_table"]) * bs))
+    assert torch.equal(ops.shared_prefix_attention(**dict(p, prefix_len=p["prefix_len"] * 0 + 2 ** 31 - 1)),
+                       want)
+    assert cuda.read_device_error() == 4
