@@ -87,16 +87,16 @@ struct PrefixCfg {
   static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 };
 
-// The tensor cores cut off the bits that an fp32 sum cannot hold, so a long sum
-// shrinks by about 2e-8 per product added (16 a tile; 4.1e-6 after 15 tiles).
-// Every few tiles O is therefore added to a sum of its own, rounded to nearest,
-// and started anew.  Where tensor memory has columns left (head_dim up to 64, or
-// one row tile) the sum is there and takes O every 2 tiles: 13,130 tokens, 8 rows a
-// head, head_dim 64 are then off by 9.3e-7 of the result (1.4e-6 at every 4) for 1%
-// of the time.  Else it is in global memory and takes O every 8: 32,768 tokens, 256
-// rows a head are off by 2.6e-6 in 79 us; 4.8e-6 in 74 us without sums, 1.6e-6 in
-// 85 us at every 4.
-constexpr int kFlushNear = 2, kFlushFar = 8;
+// The tensor cores cut off the bits that an fp32 sum cannot hold, so a sum of one
+// sign shrinks by 8e-7 in a tile (16 products; 6.4e-6 in 8 tiles), one of mixed
+// signs by about a third of that.  Every few tiles O is therefore added to a sum of
+// its own, rounded to nearest, and started anew.  Where tensor memory has columns
+// left (head_dim up to 64, or one row tile) the sum is there and takes O every 2
+// tiles: V of one sign is then off by 1.6e-6 of the result in the mean.  Else it is in
+// global memory and takes O every 5: V of one sign is off by 4.1e-6, of mixed
+// signs by 1.9e-6, and 32,768 tokens for 64 sequences, 32 / 8 heads take 115 us a call.
+// Every 8 were 6.3e-6, 2.6e-6 and 112 us, every 4 3.2e-6, 1.6e-6 and 118 us.
+constexpr int kFlushNear = 2, kFlushFar = 5;
 
 struct PrefixParams {
   const float* q;
