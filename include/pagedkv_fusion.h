@@ -377,6 +377,30 @@ int pkv_prefill_attention(const void *q, const void *k, const void *v,
                           float sm_scale, int32_t causal, void *stream);
 
 /*
+ * The same with a workspace, which needs no initialisation.  The tensor cores
+ * cut the bits of a product that the fp32 sum cannot hold: a sum over n keys
+ * whose terms have one sign comes out too small by up to 6.6e-9 n of itself.
+ * Sums are therefore rounded to nearest every 16,384 keys, which ends the loss
+ * at 1.1e-4: with head_dim up to 64 in the call above too, above that where the
+ * call has a workspace.  Its size is 0 for calls that need none (head_dim up to
+ * 64, or no more than 16,384 keys in all).  workspace may be NULL.
+ */
+size_t pkv_prefill_attention_workspace_size(int64_t total_q, int64_t total_k,
+                                            int32_t head_dim);
+int pkv_prefill_attention_ws(const void *q, const void *k, const void *v,
+                             int32_t dtype, void *out, float *lse,
+                             const int32_t *cu_seqlens_q,
+                             const int32_t *cu_seqlens_k, int32_t num_seqs,
+                             int64_t total_q, int64_t total_k,
+                             int32_t num_heads, int32_t num_kv_heads,
+                             int32_t head_dim, int64_t q_token_stride,
+                             int64_t q_head_stride, int64_t k_token_stride,
+                             int64_t k_head_stride, int64_t v_token_stride,
+                             int64_t v_head_stride, float sm_scale,
+                             int32_t causal, void *workspace,
+                             size_t workspace_bytes, void *stream);
+
+/*
  * Decode-step attention for a batch that shares a prefix: as
  * pkv_quant_paged_attention over the tokens [prefix | own tokens] of each
  * sequence, where the prefix_len[0] tokens of the prefix are reached through

@@ -3,6 +3,7 @@
 // messages (csrc/eviction_score.cu:105-110, csrc/quant_paged_attention.cu:
 // 181-197), then dispatch to the kernel launchers.
 #include <cuda_runtime.h>
+#include <algorithm>
 
 #include <cstdint>
 #include <mutex>
@@ -487,13 +488,23 @@ int pkv_append_kv(const void* key, const void* value, int32_t dtype, int8_t* kv_
   return pkv::launch_append_kv(a, workspace, workspace_bytes, as_stream(stream));
 }
 
-int pkv_prefill_attention(const void* q, const void* k, const void* v, int32_t dtype, void* out,
-                          float* lse, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
-                          int32_t num_seqs, int64_t total_q, int64_t total_k, int32_t num_heads,
-                          int32_t num_kv_heads, int32_t head_dim, int64_t q_token_stride,
-                          int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,
-                          int64_t v_token_stride, int64_t v_head_stride, float sm_scale,
-                          int32_t causal, void* stream) {
+size_t pkv_prefill_attention_workspace_size(int64_t total_q, int64_t total_k, int32_t head_dim) {
+  pkv::PrefillArgs a;
+  a.total_q = std::max<int64_t>(total_q, 0);
+  a.total_k = total_k;
+  a.dim = head_dim;
+  return pkv::prefill_workspace_size(a);
+}
+
+int pkv_prefill_attention_ws(const void* q, const void* k, const void* v, int32_t dtype, void* out,
+                             float* lse, const int32_t* cu_seqlens_q,
+                             const int32_t* cu_seqlens_k, int32_t num_seqs, int64_t total_q,
+                             int64_t total_k, int32_t num_heads, int32_t num_kv_heads,
+                             int32_t head_dim, int64_t q_token_stride, int64_t q_head_stride,
+                             int64_t k_token_stride, int64_t k_head_stride,
+                             int64_t v_token_stride, int64_t v_head_stride, float sm_scale,
+                             int32_t causal, void* workspace, size_t workspace_bytes,
+                             void* stream) {
   clear_error();
   if (num_seqs < 0 || total_q < 0 || total_k < 0 || num_heads <= 0 || num_kv_heads <= 0)
     return fail(PKV_ERR_INVALID_ARGUMENT, "invalid prefill shape");
@@ -545,7 +556,21 @@ int pkv_prefill_attention(const void* q, const void* k, const void* v, int32_t d
   a.v_head_stride = v_head_stride;
   a.sm_scale = sm_scale;
   a.causal = causal != 0;
-  return pkv::launch_prefill(a, as_stream(stream));
+  return pkv::launch_prefill(a, workspace, workspace_bytes, as_stream(stream));
+}
+
+int pkv_prefill_attention(const void* q, const void* k, const void* v, int32_t dtype, void* out,
+                          float* lse, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                          int32_t num_seqs, int64_t total_q, int64_t total_k, int32_t num_heads,
+                          int32_t num_kv_heads, int32_t head_dim, int64_t q_token_stride,
+                          int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,
+                          int64_t v_token_stride, int64_t v_head_stride, float sm_scale,
+                          int32_t causal, void* stream) {
+  return pkv_prefill_attention_ws(q, k, v, dtype, out, lse, cu_seqlens_q, cu_seqlens_k, num_seqs,
+                                  total_q, total_k, num_heads, num_kv_heads, head_dim,
+                                  q_token_stride, q_head_stride, k_token_stride, k_head_stride,
+                                  v_token_stride, v_head_stride, sm_scale, causal, nullptr, 0,
+                                  stream);
 }
 
 size_t pkv_shared_prefix_attention_workspace_size(int32_t num_seqs, int32_t num_heads,

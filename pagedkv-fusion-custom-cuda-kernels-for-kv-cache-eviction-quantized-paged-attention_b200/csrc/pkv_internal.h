@@ -104,7 +104,10 @@ struct PrefillArgs {
   float sm_scale;
   bool causal;
 };
-int launch_prefill(const PrefillArgs& a, cudaStream_t stream);
+// The workspace is nullable: without it O is summed over all keys at once.
+size_t prefill_workspace_size(const PrefillArgs& a);
+int launch_prefill(const PrefillArgs& a, void* workspace, size_t workspace_bytes,
+                   cudaStream_t stream);
 
 // ---- eviction.cu ----------------------------------------------------------
 int launch_eviction_scores(const float* recency, const float* frequency, const float* attn,

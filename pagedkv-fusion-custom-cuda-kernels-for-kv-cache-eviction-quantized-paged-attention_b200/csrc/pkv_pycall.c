@@ -148,22 +148,23 @@ static PyObject* py_append_kv(PyObject* self, PyObject* const* a, Py_ssize_t n) 
                                        (size_t)wsb, stream));
 }
 
-/* The arguments of pkv_prefill_attention. */
+/* The arguments of pkv_prefill_attention_ws. */
 static PyObject* py_prefill_attention(PyObject* self, PyObject* const* a, Py_ssize_t n) {
-  void *q, *k, *v, *out, *lse, *cq, *ck, *stream;
+  void *q, *k, *v, *out, *lse, *cq, *ck, *ws, *stream;
   int32_t dtype, seqs, heads, kv, dim, causal;
-  int64_t tq, tk, qt, qh, kt, kh, vt, vh;
+  int64_t tq, tk, qt, qh, kt, kh, vt, vh, wsb;
   float scale;
   (void)self;
-  if (!nargs_ok(n, 23, "prefill_attention")) return NULL;
+  if (!nargs_ok(n, 25, "prefill_attention")) return NULL;
   if (PTR(0, q) || PTR(1, k) || PTR(2, v) || I32(3, dtype) || PTR(4, out) || PTR(5, lse) ||
       PTR(6, cq) || PTR(7, ck) || I32(8, seqs) || I64(9, tq) || I64(10, tk) || I32(11, heads) ||
       I32(12, kv) || I32(13, dim) || I64(14, qt) || I64(15, qh) || I64(16, kt) || I64(17, kh) ||
-      I64(18, vt) || I64(19, vh) || F32(20, scale) || I32(21, causal) || PTR(22, stream))
+      I64(18, vt) || I64(19, vh) || F32(20, scale) || I32(21, causal) || PTR(22, ws) ||
+      I64(23, wsb) || PTR(24, stream))
     return NULL;
-  return PyLong_FromLong(pkv_prefill_attention(q, k, v, dtype, out, lse, cq, ck, seqs, tq, tk,
-                                               heads, kv, dim, qt, qh, kt, kh, vt, vh, scale,
-                                               causal, stream));
+  return PyLong_FromLong(pkv_prefill_attention_ws(q, k, v, dtype, out, lse, cq, ck, seqs, tq, tk,
+                                                  heads, kv, dim, qt, qh, kt, kh, vt, vh, scale,
+                                                  causal, ws, (size_t)wsb, stream));
 }
 
 /* The arguments of pkv_shared_prefix_attention. */
@@ -196,7 +197,7 @@ static PyMethodDef kMethods[] = {
     {"append_kv", (PyCFunction)(void (*)(void))py_append_kv, METH_FASTCALL,
      "pkv_append_kv; returns the status code"},
     {"prefill_attention", (PyCFunction)(void (*)(void))py_prefill_attention, METH_FASTCALL,
-     "pkv_prefill_attention; returns the status code"},
+     "pkv_prefill_attention_ws; returns the status code"},
     {"shared_prefix_attention", (PyCFunction)(void (*)(void))py_shared_prefix_attention,
      METH_FASTCALL, "pkv_shared_prefix_attention; returns the status code"},
     {NULL, NULL, 0, NULL}};

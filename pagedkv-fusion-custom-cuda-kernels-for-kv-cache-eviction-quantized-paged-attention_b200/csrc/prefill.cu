@@ -67,6 +67,15 @@ constexpr float kLazy = 8.0f;   // log2 growth of a row maximum that moves it
 constexpr int kPart = 64;        // keys of P that are handed over first
 constexpr int kEarly = 4;        // MMAs left of a step when the turn is passed on
 constexpr int kMaskedTiles = 4; // tiles with masked keys per CTA: 256 tokens span at most 3
+// The tensor cores cut off the bits that an fp32 sum cannot hold: O loses up to
+// 8.4e-7 of a sum of one sign in a tile (measured: 8.2e-7; fp16, 131,072 keys: 8.4e-4,
+// twice the step of a 16-bit output).  Every so many tiles O is therefore added to a
+// sum of its own, rounded to nearest, and started anew.  With head_dim up to 64 the
+// sum has columns of tensor memory; above that it is in the call's workspace.  Calls
+// without so many keys have a kernel without that (LONG = false), since the softmax
+// loop has no register to spare: 16 packed prompts take 92 us, 94.5 with it.  600
+// tokens behind 16,400 keys, 32 / 8 heads, take 265 us, 257 summed at once.
+constexpr int kStretch = 128;
 
 template <int DP>
 struct PreCfg {
@@ -98,6 +107,10 @@ struct PreParams {
   int item_tiles;  // row tiles of an item: 2, or 1 in calls of few items
   float scale_log2, scale;
   int causal;
+  // LONG: per slot and row tile [DP / 4][128 rows], O of earlier stretches (DP = 128)
+  float4* sums;
+  int* ticket;  // zero: the next CTA's slot of sums
+  int slots;
 };
 
 struct PreWork {
@@ -275,7 +288,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool LONG>
 __global__ void __launch_bounds__(kPreThreads, 1)
     prefill_kernel(const __grid_constant__ CUtensorMap map_q,
                    const __grid_constant__ CUtensorMap map_k,
@@ -303,6 +316,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   PreItem* s_item = reinterpret_cast<PreItem*>(smem + C::kOffMisc + 32);            // [2]
   uint32_t* s_flags = reinterpret_cast<uint32_t*>(smem + C::kOffMisc + 32 + 96);    // [2][tile][4]
   volatile int* s_fail = reinterpret_cast<int*>(smem + C::kOffMisc + 256);  // [group][item parity]
+  // O is taken before tile j > 0 where j & s_take[0] = 0; s_take[1]: the CTA's slot
+  volatile int* s_take = reinterpret_cast<int*>(smem + C::kOffMisc + 280);
   static_assert(sizeof(PreItem) <= 48 && kMaskedTiles == 4, "layout");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -329,6 +344,12 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     mbar_init(mma_done, 2);
     mbar_init(block_full, 1);
     mbar_fence_init();
+    if constexpr (LONG) {
+      const int slot = DP > 64 ? atomicAdd(p.ticket, 1) : 0;
+      // (there are as many slots as SMs, and a CTA an SM)
+      s_take[0] = slot < p.slots ? kStretch - 1 : 0x7fffffff;
+      s_take[1] = slot;
+    }
   }
   if (tid < 6) s_fail[tid] = 0;
   if (warp == kMmaWarp) tmem_alloc(s_tmem, 512);
@@ -489,6 +510,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         if (last) umma_commit_warp(&q_empty[x]);
       };
       int q_uses = 0, p_uses = 0, steps = 0;
+      const int take = LONG ? s_take[0] : 0x7fffffff;
       // a warp's lanes give up together
       auto wait_warp = [&](uint64_t* bar, int phase) {
         wait(bar, phase);
@@ -531,7 +553,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
                 if (!ok) break;
               }
               umma_f16_ta_warp(o_col, s_col + kk * 8, umma_desc_at(b, kk * 2048), kIdPV,
-                               (j > 0 || kk > 0) ? 1u : 0u);
+                               ((j & take) != 0 || kk > 0) ? 1u : 0u);
             }
             if (!ok) break;
             ++p_uses;
@@ -606,6 +628,11 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     const uint32_t s_addr = tmem + lanes + C::kSCol + x * 128;
     const uint32_t o_addr = tmem + lanes + C::kOCol + x * 128;
     const int row_tok = row / p.group;
+    const int take = LONG ? s_take[0] : 0x7fffffff;
+    const uint32_t o2_addr = o_addr + 64;  // of head_dim up to 64
+    auto sums = [&]() {  // the row's, 4 channels every 128
+      return p.sums + ((int64_t)s_take[1] * 2 + x) * (DP / 4) * kRows + row;
+    };
     const uint32_t inv_group = (65536u + p.group - 1) / p.group;  // exact below 128 * 128
     int s_uses = 0, o_uses = 0;
     for (int k = 0; next_item(k, x, 2 + x, 128); ++k) {
@@ -631,6 +658,36 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         wait(&s_full[x], s_uses++);
         __syncwarp();
         tmem_fence_after_sync();
+        if (LONG && j > 0 && (j & take) == 0) {  // O has the products of all tiles before j
+          float4* sum = sums();
+#pragma unroll 1
+          for (int c = 0; c < DP; c += 16) {
+            alignas(16) uint32_t o[16], was[16];
+            tmem_load<16>(o_addr + c, o);
+            if (j == take + 1) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) was[e] = 0u;
+            } else if (DP == 64) {
+              tmem_load<16>(o2_addr + c, was);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                *reinterpret_cast<float4*>(&was[4 * e]) = sum[(c / 4 + e) * kRows];
+            }
+            tmem_wait_load();
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              o[e] = __float_as_uint(__uint_as_float(was[e]) + __uint_as_float(o[e]));
+            if (DP == 64) {
+              tmem_store<16>(o2_addr + c, o);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                sum[(c / 4 + e) * kRows] = *reinterpret_cast<const float4*>(&o[4 * e]);
+            }
+          }
+          tmem_wait_store();
+        }
         float s[kKeys];
         {
           uint32_t(&u)[kKeys] = reinterpret_cast<uint32_t(&)[kKeys]>(s);
@@ -665,14 +722,24 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           if (move) m = t;
           l *= alpha;
           if (j > 0) {  // seldom: small pieces, since the scores are in registers
+            const bool taken = LONG && j > take;  // there is a sum
+            float4* sum = sums();
 #pragma unroll 1
-            for (int c = 0; c < DP; c += 16) {
+            for (int c = 0; c < (DP == 64 && taken ? 2 * DP : DP); c += 16) {
               uint32_t o[16];
-              tmem_load<16>(o_addr + c, o);
+              tmem_load<16>(o_addr + c, o);  // (a sum's columns follow O's)
               tmem_wait_load();
 #pragma unroll
               for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
               tmem_store<16>(o_addr + c, o);
+            }
+            if (DP > 64 && taken) {
+#pragma unroll 1
+              for (int c = 0; c < DP / 4; ++c) {
+                float4 v = sum[c * kRows];
+                v.x *= alpha, v.y *= alpha, v.z *= alpha, v.w *= alpha;
+                sum[c * kRows] = v;
+              }
             }
           }
         }
@@ -727,6 +794,20 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           if (nt > 0) {
             tmem_load<32>(o_addr + c, o);
             tmem_wait_load();
+          }
+          if (LONG && nt - 1 > take) {  // and what was taken before
+            alignas(16) uint32_t was[32];
+            if (DP == 64) {
+              tmem_load<32>(o2_addr + c, was);
+              tmem_wait_load();
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                *reinterpret_cast<float4*>(&was[4 * e]) = sums()[(c / 4 + e) * kRows];
+            }
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              o[e] = __float_as_uint(__uint_as_float(was[e]) + __uint_as_float(o[e]));
           }
           const bool none = nt == 0 || l == 0.0f;
 #pragma unroll
@@ -818,8 +899,10 @@ bool make_map(CUtensorMap* map, const void* base, int bf16, int dim, int heads, 
   return r == CUDA_SUCCESS;
 }
 
-template <typename T, int DP>
-int launch_prefill_t(const PrefillArgs& a, cudaStream_t stream) {
+constexpr int kSumSlots = 148;  // one CTA an SM
+
+template <typename T, int DP, bool LONG>
+int launch_prefill_t(const PrefillArgs& a, void* workspace, cudaStream_t stream) {
   using C = PreCfg<DP>;
   const int bf16 = a.dtype == 2;
   PreParams p;
@@ -841,6 +924,16 @@ int launch_prefill_t(const PrefillArgs& a, cudaStream_t stream) {
   p.scale = a.sm_scale;
   p.scale_log2 = a.sm_scale * kLog2e;
   p.causal = a.causal ? 1 : 0;
+  p.sums = nullptr;
+  p.ticket = nullptr;
+  p.slots = kSumSlots;
+  if (LONG && DP > 64) {
+    uint8_t* ws = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 255) &
+                                             ~(uintptr_t)255);
+    p.ticket = reinterpret_cast<int*>(ws);
+    p.sums = reinterpret_cast<float4*>(ws + 256);
+    cudaMemsetAsync(p.ticket, 0, sizeof(int), stream);
+  }
   CUtensorMap mq, mk, mv;
   // without keys the key maps are never used, but a map needs memory
   const bool none = a.total_k == 0;
@@ -855,7 +948,7 @@ int launch_prefill_t(const PrefillArgs& a, cudaStream_t stream) {
     set_error("cuTensorMapEncodeTiled failed for q, k or v");
     return kCudaError;
   }
-  auto kern = prefill_kernel<T, DP>;
+  auto kern = prefill_kernel<T, DP, LONG>;
   static std::atomic<uint64_t> done{0};
   allow_shared_memory(reinterpret_cast<const void*>(kern), C::kSmemBytes, done);
   // at most so many items over so many sequences
@@ -874,15 +967,32 @@ int launch_prefill_t(const PrefillArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
-int launch_prefill(const PrefillArgs& a, cudaStream_t stream) {
+size_t prefill_workspace_size(const PrefillArgs& a) {
+  if (a.total_q == 0 || a.dim <= 64 || a.total_k <= (int64_t)kStretch * kKeys) return 0;
+  return 256 + 256 + (size_t)kSumSlots * 2 * kRows * 128 * sizeof(float);
+}
+
+int launch_prefill(const PrefillArgs& a, void* workspace, size_t workspace_bytes,
+                   cudaStream_t stream) {
   if (a.total_q == 0) return kOk;
-  int rc;
-  if (a.dtype == 1)
-    rc = a.dim <= 64 ? launch_prefill_t<__half, 64>(a, stream)
-                     : launch_prefill_t<__half, 128>(a, stream);
-  else
-    rc = a.dim <= 64 ? launch_prefill_t<__nv_bfloat16, 64>(a, stream)
-                     : launch_prefill_t<__nv_bfloat16, 128>(a, stream);
+  if (workspace != nullptr && workspace_bytes < prefill_workspace_size(a)) {
+    set_error("workspace too small for prefill_attention: need " +
+              std::to_string(prefill_workspace_size(a)) + " bytes");
+    return kWorkspace;
+  }
+  auto with = [&](auto t, auto dp) {
+    using T = decltype(t);
+    constexpr int DP = decltype(dp)::value;
+    const bool more = a.total_k > (int64_t)kStretch * kKeys;  // than one stretch
+    return more && (DP == 64 || workspace != nullptr)
+               ? launch_prefill_t<T, DP, true>(a, workspace, stream)
+               : launch_prefill_t<T, DP, false>(a, workspace, stream);
+  };
+  auto with_dim = [&](auto t) {
+    return a.dim <= 64 ? with(t, std::integral_constant<int, 64>{})
+                       : with(t, std::integral_constant<int, 128>{});
+  };
+  const int rc = a.dtype == 1 ? with_dim(__half()) : with_dim(__nv_bfloat16());
   if (rc != kOk) return rc;
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) {

@@ -81,6 +81,7 @@ _wtc_ws = _sig("pkv_write_to_cache_workspace_size", [_I64, _I32], _SZ)
 _wtc = _sig("pkv_write_to_cache",
             [_P, _P, _I32, _P, _P, _P, _I64, _I64, _I32, _I32, _I32, _P, _SZ, _P])
 
+_prefill_ws = _sig("pkv_prefill_attention_workspace_size", [_I64, _I64, _I32], _SZ)
 _append_ws = _sig("pkv_append_kv_workspace_size", [_I64, _I64], _SZ)
 _prefix_ws = _sig("pkv_shared_prefix_attention_workspace_size",
                   [_I32] * 5 + [_I64, _I32, _I32], _SZ)
@@ -668,10 +669,12 @@ def prefill_attention(q, k, v, cu_seqlens, sm_scale, cu_seqlens_k=None, causal=T
     qc, kc, vc = _tma_rows(q), _tma_rows(k), _tma_rows(v)
     out = _like(q)
     lse = torch.empty((Tq, H), dtype=_F32, device=q.device) if return_lse else None
+    nbytes = _prefill_ws(Tq, Tk, D) if Tk > 8192 else 0  # (none for so few keys)
+    ws, wp = _workspace(nbytes, q.device)
     _call(_fast.prefill_attention, dev, qc.data_ptr(), kc.data_ptr(), vc.data_ptr(),
           _DTYPE_CODE[dt], out.data_ptr(), None if lse is None else lse.data_ptr(), cq.data_ptr(),
           ck.data_ptr(), n - 1, Tq, Tk, H, Hkv, D, *qc.stride()[:2], *kc.stride()[:2],
-          *vc.stride()[:2], float(sm_scale), 1 if causal else 0, _raw_stream(dev))
+          *vc.stride()[:2], float(sm_scale), 1 if causal else 0, wp, nbytes, _raw_stream(dev))
     return (out, lse) if return_lse else out
 
 

@@ -403,8 +403,10 @@ def prefill_attention(q, k, v, cu_seqlens, sm_scale: float, cu_seqlens_k=None,
     Returns ``[total_q, H, D]`` in the inputs' type, and with ``return_lse``
     also the float32 ``[total_q, H]`` logarithms of the softmax denominators.
     Rows that see no key, and rows behind the last sequence or in front of the
-    first, are zero (lse -inf).  What a row does not see does not reach it, whatever its value.
-    No backward pass.
+    first, are zero (lse -inf).  What a row does not see does not reach it,
+    whatever its value.  The probabilities are rounded to the inputs' type for
+    their product with ``v``; its sums are fp32, and however long the keys a sum
+    of one sign is kept to 1.1e-4.  No backward pass.
     """
     C = _lib()
     given = [t for t in (q, k, v, cu_seqlens, cu_seqlens_k) if t is not None]
