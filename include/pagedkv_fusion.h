@@ -362,8 +362,9 @@ int pkv_append_kv(const void *key, const void *value, int32_t dtype,
  * are in elements, multiples of 8, pointers 16-byte aligned, channels
  * contiguous, out contiguous.  head_dim a multiple of 8 up to 128, at most
  * 128 query heads per KV head, sm_scale > 0.  cu_seqlens that do not ascend
- * within the tensors record PKV_DEVERR_BAD_SEQLENS and are cut to the tensors
- * and to the largest entry before them.
+ * within the tensors record PKV_DEVERR_BAD_SEQLENS and are cut to the tensors,
+ * those of q also to the largest entry before them; a sequence whose keys end
+ * before they begin has none.
  */
 int pkv_prefill_attention(const void *q, const void *k, const void *v,
                           int32_t dtype, void *out, float *lse,

@@ -177,42 +177,33 @@ __device__ __forceinline__ int granted_block(const void* answer) {
 __device__ __forceinline__ bool find_work(const PreParams& p, int pair, PreWork& w) {
   const int lane = threadIdx.x & 31;
   const int span = p.item_tiles * p.tile_tokens;
-  int base = 0, q_end = 0, k_end = 0;  // the largest ends so far
-  for (int s0 = 0; s0 <= p.num_seqs + 1; s0 += 32) {
+  int base = 0;
+  int q_end = 0;  // the largest end up to the last 32 that fell
+  const int front = p.num_seqs + 1;
+  for (int s0 = 0; s0 <= front; s0 += 32) {
     const int s = s0 + lane;
-    int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
-    if (s <= p.num_seqs) {
-      const bool rest = s == p.num_seqs;
-      q0 = min(max(p.cu_q[s], 0), p.total_q);
-      k0 = min(max(p.cu_k[s], 0), p.total_k);
-      q1 = rest ? p.total_q : min(max(p.cu_q[s + 1], 0), p.total_q);
-      k1 = rest ? k0 : min(max(p.cu_k[s + 1], 0), p.total_k);
+    int q0 = 0, q1 = 0;
+    if (s <= front) {
+      q0 = s < front ? min(max(p.cu_q[s], 0), p.total_q) : 0;
+      q1 = s == p.num_seqs ? p.total_q : min(max(p.cu_q[s < front ? s + 1 : 0], 0), p.total_q);
     }
     // An entry below an earlier one counts as the largest before it: sequences then
     // share no row, and all of them together have no more items than the grid.
-    const bool falls = q1 < q0 || k1 < k0 || (lane == 0 && (q0 < q_end || k0 < k_end));
+    const bool falls = q1 < q0 || (lane == 0 && s < front && q0 < q_end);
     if (__any_sync(0xffffffffu, falls)) {
-      int qm = max(max(q0, q1), q_end), km = max(max(k0, k1), k_end);
+      int most = max(max(q0, q1), q_end);
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int a = __shfl_up_sync(0xffffffffu, qm, o), b = __shfl_up_sync(0xffffffffu, km, o);
-        if (lane >= o) {
-          qm = max(qm, a);
-          km = max(km, b);
-        }
+        const int x = __shfl_up_sync(0xffffffffu, most, o);
+        if (lane >= o) most = max(most, x);
       }
-      const int a = __shfl_up_sync(0xffffffffu, qm, 1), b = __shfl_up_sync(0xffffffffu, km, 1);
-      q0 = lane > 0 ? a : max(q0, q_end);
-      k0 = lane > 0 ? b : max(k0, k_end);
-      q1 = s <= p.num_seqs ? qm : q0;
-      k1 = s < p.num_seqs ? km : k0;
+      const int before = __shfl_up_sync(0xffffffffu, most, 1);
+      if (s < front) {
+        q0 = lane > 0 ? before : max(q0, q_end);
+        q1 = most;
+      }
+      q_end = __shfl_sync(0xffffffffu, q1, 31);
     }
-    if (s == p.num_seqs + 1) {  // in front of the first
-      q0 = k0 = k1 = 0;
-      q1 = min(max(p.cu_q[0], 0), p.total_q);
-    }
-    q_end = __shfl_sync(0xffffffffu, q1, 31);
-    k_end = __shfl_sync(0xffffffffu, k1, 31);
     const int n = (q1 - q0 + span - 1) / span;
     int incl = n;
 #pragma unroll
@@ -229,8 +220,11 @@ __device__ __forceinline__ bool find_work(const PreParams& p, int pair, PreWork&
       w.q0 = __shfl_sync(0xffffffffu, q0, src);
       w.lq = __shfl_sync(0xffffffffu, q1, src) - w.q0;
       w.t0 = (__shfl_sync(0xffffffffu, n, src) - 1 - local) * span;
-      w.k0 = __shfl_sync(0xffffffffu, k0, src);
-      w.lk = __shfl_sync(0xffffffffu, k1, src) - w.k0;
+      w.k0 = w.lk = 0;
+      if (s0 + src < p.num_seqs) {  // (keys may be shared: they are only read)
+        w.k0 = min(max(p.cu_k[s0 + src], 0), p.total_k);
+        w.lk = min(max(p.cu_k[s0 + src + 1], w.k0), p.total_k) - w.k0;
+      }
       return true;
     }
     base += total;

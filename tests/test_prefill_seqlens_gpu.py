@@ -1,7 +1,7 @@
 """prefill_attention's cu_seqlens: lists of more than 32 sequences that do not
-ascend within the tensors are reported wherever the mistake is, and give what
-the list gives whose entries are cut to the tensors and to the largest before
-them: every row is written, by one sequence.  Rows in front of the first
+ascend within the tensors are reported wherever the mistake is.  Entries are cut
+to the tensors, those of the rows also to the largest before them: every row is
+written, by one sequence.  Rows in front of the first
 sequence are zero, as those behind the last are.
 """
 
@@ -60,8 +60,13 @@ def ragged(rng, n, top):
     return up.tolist()
 
 
-def cut(values, top):
-    return np.maximum.accumulate(np.clip(values, 0, top)).tolist()
+def cut(q_list, k_list, top):
+    """The same sequences as good lists: the keys of each laid out anew, as the
+    places of its rows in the key tensor."""
+    q_cut = np.maximum.accumulate(np.clip(q_list, 0, top)).tolist()
+    ends = np.clip(k_list, 0, top).tolist()
+    keys = [np.arange(a, max(a, b)) for a, b in zip(ends, ends[1:])]
+    return q_cut, [0] + np.cumsum([len(x) for x in keys]).tolist(), np.concatenate(keys).astype(int)
 
 
 def filled_with_nan(t):
@@ -78,6 +83,8 @@ def filled_with_nan(t):
     ([0, 100, 50, 400], [0, 100, 200, 350]),
     ([0, 100, 200, 350], [0, 200, 100, 400]),
     ([0, 900, 120], None),
+    ([0, 100, -2 ** 31, 2 ** 31 - 1, 400], None),
+    ([0, 100, 400], [5, -2 ** 31, 2 ** 31 - 1]),
     ("ragged", "ragged"),
     ("ragged", None),
 ])
@@ -88,14 +95,15 @@ def test_falling_entries_share_no_rows(cuda, dtype, q_list, k_list):
     for n in ((5, 40, 130) if q_list == "ragged" else (0,)):
         cq = ragged(rng, n, 400) if n else q_list
         ck = ragged(rng, n, 400) if k_list == "ragged" else (k_list or cq)
-        good = [entries(cut(c, 400)) for c in (cq, ck)]
-        want, lse = ops.prefill_attention(q, k, v, good[0], 0.1, cu_seqlens_k=good[1], return_lse=True)
+        q_cut, k_cut, at = cut(cq, ck, 400)
+        want, lse = ops.prefill_attention(q, k[at], v[at], entries(q_cut), 0.1,
+                                          cu_seqlens_k=entries(k_cut), return_lse=True)
         assert cuda.read_device_error() == 0
         filled_with_nan(q)
         out, got = ops.prefill_attention(q, k, v, entries(cq), 0.1, cu_seqlens_k=entries(ck),
                                          return_lse=True)
         assert cuda.read_device_error() == 6
-        first = good[0][0]  # (rows in front of the first sequence are not its)
+        first = q_cut[0]  # (rows in front of the first sequence are not its)
         assert torch.equal(out[first:], want[first:]) and torch.equal(got[first:], lse[first:])
 
 
