@@ -4,9 +4,9 @@
 //
 // An item of work is two row tiles of 128 rows of one KV head (one row tile in calls
 // that would leave half of the SMs without); one CTA per SM takes items until none
-// is left.  A row is a (token,
-// query head of the group) pair, so the G heads of a group share every K / V
-// tile that is loaded.  Keys come in tiles of 128 tokens; per row tile
+// is left.  A row is a (token, query head of the group) pair, so the G heads of a
+// group share every K / V tile that is loaded.  Keys come in tiles of 128 tokens;
+// per row tile
 //   S = Q K^T    tcgen05 kind::f16, 128 x 128, K-major A and B from shared
 //                memory, S in 128 columns of tensor memory;
 //   P = exp2(scale log2e (S - m)), one thread per row, written back over S as
@@ -14,6 +14,12 @@
 //   O += P V     A = P from tensor memory, B = the V tile read MN-major.
 // The two row tiles alternate: while the softmax warps of one turn S into P,
 // the tensor cores work for the other.
+//
+// P has 16 bits because the second product has: B is V as it was given, and A is of
+// B's type.  The denominator sums the unrounded values.  Outputs of mixed signs are
+// then off by 3.0e-4 (fp16) or 2.3e-3 (bf16) of their root mean square, where rounding
+// the output alone leaves 2.1e-4 and 1.7e-3; P as two 16-bit numbers would be
+// half as many products again and 64 more columns of stores a row.
 //
 // The running maximum m is moved only when a tile's maximum exceeds it by
 // more than 2^8 (the exponentials then stay below 2^8, exact enough in fp32
@@ -28,12 +34,17 @@
 // it.
 //
 // What bounds it: 8,192 tokens, 32 query heads of 8 KV heads, causal, head_dim
-// 128 are 550 GFLOP (323 us at the cuBLAS rate) and took 470 us at best
-// (1.17 PFLOP/s), 515 to 550 us in a long run, where the card's power limit
-// lowers the clock to about 1.67 GHz.  The tensor pipe is half busy; a row tile's
-// step is a chain -- product, softmax, second half of the softmax beside the first
-// half of P V, P V -- and two row tiles (tensor memory holds no third) fill each
-// other's gaps only in part.  16 packed prompts of 17 to 900 tokens: 93 us.
+// 128 are 550 GFLOP (323 us at the cuBLAS rate) and took 466 us at best
+// (1.18 PFLOP/s), 515 to 550 us in a long run, where the card's power limit
+// lowers the clock to about 1.67 GHz; without the mask 984 us for 1,100 GFLOP.  The
+// tensor pipe is half busy; a row tile's step is a chain -- product, softmax,
+// second half of the softmax beside the first half of P V, P V -- and two row
+// tiles (at head_dim 128 tensor memory holds no third) fill each other's gaps only
+// in part.  16 packed prompts of 17 to 900 tokens: 92 us, of which 22 steps an SM
+// are about 47 us, and the rest its seven items' own starts and ends.  64 or 128
+// channels are multiplied: 8,192 tokens of head_dim 64 take 423 us (floor 162), of 32
+// as much (81), of 80 and 96 458 us (202 and 242).  2,000 prompts of 1 to 8 tokens
+// take 1.8 ms: 16,000 items, each found by a search among the sequences.
 // Measured on the way, at 8,192 tokens: one thread issuing from its own branch
 // 647 us, a converged warp with one elected lane 577 us, a warp per row tile in
 // strict turns 505 us (the two unordered: slower than one; P handed over in

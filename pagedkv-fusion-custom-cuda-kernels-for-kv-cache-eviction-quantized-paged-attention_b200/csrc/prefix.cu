@@ -30,7 +30,7 @@
 //
 // What bounds it: 32,768 tokens for 64 sequences of 32 query heads (8 KV heads,
 // head_dim 128) are 69 GFLOP with both halves (41 us at the cuBLAS rate) and 67 MB
-// (10 us); the kernel takes 80 us, its tensor pipe 45% and its issue slots 49% busy.
+// (10 us); the kernel takes 83 us, its tensor pipe 43% and its issue slots 46% busy.
 // A row tile's step is about 2,400 clocks of products (S reads both operands from
 // shared memory) and 4,900 of softmax, of which the other row tile hides half; 144
 // CTAs of 14 or 15 tiles also pay for the query split, the first loads and the

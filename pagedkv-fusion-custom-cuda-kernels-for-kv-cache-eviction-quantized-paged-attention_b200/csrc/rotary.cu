@@ -89,10 +89,12 @@ struct QkArgs {
 // 16-byte access each.  The partners of the half layout are R/2 channels
 // away, in another lane: their raw words come by shuffle, so a row is read
 // once.  The table entries of a lane are the same for all its rows.
-// What bounds it: HBM (a row is read and written once); RPG = 4 keeps four
-// independent loads in flight and reads the table a quarter as often.  16,384
-// tokens of 40 + 40 heads in fp16, head_dim 128: 115 us for 675 MB (5.9 TB/s, 0.90
-// of the copy rate).
+// What bounds it: without norms HBM (a row is read and written once); RPG = 4
+// keeps four independent loads in flight and reads the table a quarter as often.
+// 16,384 tokens of 40 + 40 heads in fp16, head_dim 128: 115 us for 675 MB (5.9 TB/s,
+// 0.90 of the copy rate).  With norms and weights the instructions for a value: 32 +
+// 8 heads in bf16 116 us for 344 MB (floor 53 us; issue slots 73% busy, DRAM 31%).
+// A decode step of 64 tokens, 32 + 8 heads with norms: 3.0 us.
 template <typename T, int VEC, int LPR, int NC, int RPG, bool NORM, bool INTER>
 __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkArgs<T> a, int* err) {
   const int rows = a.heads + a.kv_heads;
@@ -238,7 +240,9 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkArgs<T> a, int* err
 }
 
 // Any head_dim, rotary width, alignment and stride: one warp per row, one
-// value per access, the partner value read from memory again.
+// value per access, the partner value read from memory again.  Bound by its
+// accesses: 16,384 tokens of 40 + 40 heads in fp16, 24 of 96 channels rotated, take
+// 362 us for 503 MB (floor 77 us), 20 of 80 with norms 482 us for 419 MB (64 us).
 template <typename T, bool NORM>
 __global__ void __launch_bounds__(256)
     qk_norm_rope_scalar_kernel(QkArgs<T> a, bool interleaved, int* err) {
@@ -886,7 +890,12 @@ __global__ void __launch_bounds__(kAppendThreads,
   }
 }
 
-// Largest call that scans its slots in every CTA.
+// Largest call that scans its slots in every CTA, a launch instead of three.  us on the
+// device, scan and index (bf16, 128 channels, pages of 16), prompts: 8 heads, 256
+// tokens 12.0 and 19.5, 512 15.2 and 20.8, 1,024 21.2 and 22.7, 2,048 34.8 and 23.6;
+// 40 heads, 256 22.0 and 24.0, 512 37.1 and 27.9.  Single tokens of as many
+// sequences: 8 heads, 256 11.1 and 12.9, 512 17.1 and 18.8, 768 24.4 and 21.6; 40 heads,
+// 128 17.4 and 19.3, 256 31.4 and 29.8, 512 63.5 and 45.2.
 constexpr int64_t kAppendScan = 512;
 
 template <typename T, int VEC, int NC>
