@@ -104,6 +104,26 @@ def test_long_ranges(cuda, n, m, heads, kv_heads, dim, growth):
     assert torch.equal(out, again)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+def test_denominators_and_no_mask(cuda, dim, causal):
+    """lse of long rows: the scores' error and the sums' as for short ones."""
+    from pagedkv_fusion import ops
+    n, m = 150, 20001
+    q, k, v = problem(dim, n, m, 4, 2, dim, "bf16")
+    scale = dim ** -0.5
+    out, lse = ops.prefill_attention(q, k, v, cumulative([n]), scale, cu_seqlens_k=cumulative([m]),
+                                     causal=causal, return_lse=True)
+    assert cuda.read_device_error() == 0
+    hidden = torch.arange(m, device="cuda") > (torch.arange(n, device="cuda") + (m - n if causal else m))[:, None]
+    for h in range(4):
+        s = (q[:, h].double() @ k[:, h // 2].double().T * scale).masked_fill_(hidden, -math.inf)
+        want = torch.softmax(s, 1) @ v[:, h // 2].double()
+        assert bool(((out[:, h].double() - want).abs() <= want * (2 ** -8 + 2 * CUT + 2 ** -8)).all())
+        ref = torch.logsumexp(s, 1)
+        assert bool(((lse[:, h].double() - ref).abs() <= 2e-4 + 2.0 ** -20 * ref.abs()).all())
+
+
 def test_sequences_of_a_batch_and_nonfinite_values(cuda):
     """Long and short sequences packed give what each gives alone; a NaN stays in
     its rows."""
