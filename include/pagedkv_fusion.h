@@ -429,6 +429,91 @@ int pkv_shared_prefix_attention(
     int64_t num_blocks, int32_t prefix_blocks, int32_t max_blocks_per_seq,
     float sm_scale, void *workspace, size_t workspace_bytes, void *stream);
 
+/*
+ * Attention of new tokens over the INT8 paged cache that they were appended to
+ * (one token, a few, or a chunk of a prompt of each sequence): out[i, h, :] =
+ * softmax(sm_scale * q[i, h] . K^T) V over the keys j <= i + L - Lq of token i's
+ * sequence, where sequence s is rows cu_seqlens[s] .. cu_seqlens[s + 1] (Lq) of
+ * q and out [total_q, num_heads, head_dim] (PKV_DTYPE_*) and its seq_lens[s] (L)
+ * cached tokens, the new ones last, are reached through block_tables[s]; caches,
+ * scales and GQA as in pkv_quant_paged_attention.  Rows that see no key, and rows
+ * behind the last sequence or in front of the first, become zero, with lse -inf;
+ * lse (nullable, float32 [total_q, num_heads]) is the natural logarithm of the
+ * softmax denominator.  Lengths beyond the table record PKV_DEVERR_SEQ_TOO_LONG
+ * and are cut to it; tokens on a page outside the cache record
+ * PKV_DEVERR_BAD_BLOCK_ID and are not attended; cu_seqlens that do not ascend
+ * within the tensor record PKV_DEVERR_BAD_SEQLENS and are cut as in
+ * pkv_prefill_attention.  head_dim a multiple of 32 up to 256, block_size <= 64;
+ * q's strides, in elements, of multiples of 16 bytes, channels contiguous, q, out
+ * and the caches 16-byte aligned, out contiguous.  The workspace needs no
+ * initialisation.
+ */
+size_t pkv_chunk_attention_workspace_size(int64_t total_q, int32_t num_seqs,
+                                          int32_t num_heads,
+                                          int32_t num_kv_heads, int32_t head_dim,
+                                          int32_t block_size,
+                                          int32_t max_blocks_per_seq);
+int pkv_chunk_attention(const void *q, int32_t dtype, const int8_t *k_cache,
+                        const float *k_scale, const int8_t *v_cache,
+                        const float *v_scale, const int32_t *block_tables,
+                        const int32_t *seq_lens, const int32_t *cu_seqlens,
+                        void *out, float *lse, int64_t total_q, int32_t num_seqs,
+                        int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                        int32_t block_size, int64_t num_blocks,
+                        int32_t max_blocks_per_seq, int64_t q_token_stride,
+                        int64_t q_head_stride, float sm_scale, void *workspace,
+                        size_t workspace_bytes, void *stream);
+
+/*
+ * Adds to weights (float32 [num_blocks, block_size], one per cached token) what the
+ * call's tokens attend to it: the sum over tokens i and the mean over heads h of
+ * exp(sm_scale * q[i, h] . k_j - lse[i, h]), tokens, keys and masks as in
+ * pkv_chunk_attention.  lse (float32 [total_q, num_heads], contiguous) is what that
+ * call returned, or NULL: then it is computed first.  A row whose lse is -inf adds
+ * nothing; NaN reaches the weights of the keys that its row sees.  Pages may be in
+ * several tables; the result does not depend on the order of execution (sums meet as
+ * integers, in steps of 2^-38).  total_q * num_heads <= 2^25.
+ */
+size_t pkv_accumulate_attention_workspace_size(
+    int64_t total_q, int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
+    int32_t head_dim, int32_t block_size, int64_t num_blocks,
+    int32_t max_blocks_per_seq, int32_t has_lse);
+int pkv_accumulate_attention(float *weights, const void *q, int32_t dtype,
+                             const int8_t *k_cache, const float *k_scale,
+                             const int32_t *block_tables, const int32_t *seq_lens,
+                             const int32_t *cu_seqlens, const float *lse,
+                             int64_t total_q, int32_t num_seqs, int32_t num_heads,
+                             int32_t num_kv_heads, int32_t head_dim,
+                             int32_t block_size, int64_t num_blocks,
+                             int32_t max_blocks_per_seq, int64_t q_token_stride,
+                             int64_t q_head_stride, float sm_scale,
+                             void *workspace, size_t workspace_bytes,
+                             void *stream);
+
+/*
+ * Evicts single tokens.  Of a sequence of L > keep tokens stay the first `sinks`, the
+ * last `recent` and the heaviest of the others by `weights` (of equal ones the
+ * earlier; NaN is heaviest), `keep` in all.  They move, in order, to the front of the
+ * sequence's pages, in place, in kv_cache int8 [2, num_blocks, block_size,
+ * num_kv_heads, head_dim], scale_cache fp32 [2, num_blocks, num_kv_heads] and weights
+ * fp32 [num_blocks, block_size].  A page's new scale is the largest old scale of the
+ * tokens it now holds, per KV head, K and V apart; codes become rint(code * (old /
+ * new)) where old < new.  The slots that the sequence no longer uses keep their codes
+ * and get weight 0.  lens_out int32 [num_seqs] receives the new lengths, kept int32
+ * [num_seqs, keep] the old places of the tokens that stay, ascending, then -1.
+ * Sequences of at most `keep` tokens stay as they are, and so do those with a page
+ * outside the cache (PKV_DEVERR_BAD_BLOCK_ID; their row of kept is -1).  The pages of a
+ * sequence that is cut must not be in another sequence's table.  keep >= 1,
+ * sinks + recent <= keep, block_size <= 64, head_dim <= 256.
+ */
+int pkv_evict_tokens(int8_t *kv_cache, float *scale_cache, float *weights,
+                     const int32_t *block_tables, const int32_t *seq_lens,
+                     int32_t *lens_out, int32_t *kept, int32_t num_seqs,
+                     int64_t num_blocks, int32_t block_size,
+                     int32_t num_kv_heads, int32_t head_dim,
+                     int32_t max_blocks_per_seq, int32_t keep, int32_t sinks,
+                     int32_t recent, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -625,4 +625,186 @@ int pkv_shared_prefix_attention(const float* q, const int8_t* k_cache, const flo
   return pkv::launch_shared_prefix(a, workspace, workspace_bytes, as_stream(stream));
 }
 
+static pkv::ChunkArgs chunk_args(const void* q, int32_t dtype, const int8_t* k_cache,
+                                 const float* k_scale, const int8_t* v_cache, const float* v_scale,
+                                 const int32_t* tables, const int32_t* lens, const int32_t* cu,
+                                 void* out, float* lse, int64_t total_q, int32_t seqs,
+                                 int32_t heads, int32_t kv_heads, int32_t dim, int32_t block_size,
+                                 int64_t num_blocks, int32_t width, int64_t q_tok, int64_t q_head,
+                                 float sm_scale) {
+  pkv::ChunkArgs a;
+  a.q = q;
+  a.dtype = dtype;
+  a.k_cache = k_cache;
+  a.k_scale = k_scale;
+  a.v_cache = v_cache;
+  a.v_scale = v_scale;
+  a.tables = tables;
+  a.lens = lens;
+  a.cu = cu;
+  a.out = out;
+  a.lse = lse;
+  a.total_q = total_q;
+  a.num_blocks = num_blocks;
+  a.q_token_stride = q_tok;
+  a.q_head_stride = q_head;
+  a.seqs = seqs;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.dim = dim;
+  a.block_size = block_size;
+  a.width = width;
+  a.sm_scale = sm_scale;
+  return a;
+}
+
+// What the two calls over new tokens and their pages have in common: sizes, and what
+// they point to.
+static int check_chunk_sizes(const pkv::ChunkArgs& a) {
+  if (a.total_q < 0 || a.seqs < 0 || a.heads <= 0 || a.kv_heads <= 0 || a.num_blocks < 0 ||
+      a.width < 0)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "invalid query or cache shape");
+  if (a.dtype < 0 || a.dtype > 2)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "q must be float32, float16 or bfloat16");
+  if (a.heads % a.kv_heads != 0)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "num_heads must be a multiple of num_kv_heads");
+  if (a.dim <= 0 || a.dim % 32 != 0 || a.dim > 256)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "supports head_dim % 32 == 0, <= 256");
+  if (a.block_size <= 0 || a.block_size > 64)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "supports block_size <= 64");
+  const int64_t most = 0x7fffffffLL - 1024;
+  if (a.total_q * a.heads > most || a.total_q > most / a.heads ||
+      (int64_t)a.width * a.block_size > most || a.num_blocks > most / a.block_size)
+    return fail(PKV_ERR_UNSUPPORTED, "more than 2^31 rows, tokens of a table or cache slots");
+  return PKV_OK;
+}
+
+static int check_chunk(const pkv::ChunkArgs& a) {
+  const int rc = check_chunk_sizes(a);
+  if (rc != PKV_OK) return rc;
+  const int64_t per_16 = a.dtype == PKV_DTYPE_F32 ? 4 : 8;
+  if (a.total_q > 0 && (a.q_token_stride % per_16 != 0 || a.q_head_stride % per_16 != 0))
+    return fail(PKV_ERR_INVALID_ARGUMENT, "q's strides must be multiples of 16 bytes");
+  if (reinterpret_cast<uintptr_t>(a.q) % 16 != 0 || reinterpret_cast<uintptr_t>(a.out) % 16 != 0 ||
+      reinterpret_cast<uintptr_t>(a.k_cache) % 16 != 0 ||
+      reinterpret_cast<uintptr_t>(a.v_cache) % 16 != 0)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "q, out and the caches must be 16-byte aligned");
+  if (a.total_q > 0 && (!a.q || !a.cu || (a.seqs > 0 && (!a.lens || (a.width > 0 && !a.tables)))))
+    return fail(PKV_ERR_INVALID_ARGUMENT, "null input or output pointer");
+  if (a.total_q > 0 && a.num_blocks > 0 && (!a.k_cache || !a.k_scale))
+    return fail(PKV_ERR_INVALID_ARGUMENT, "null input or output pointer");
+  return PKV_OK;
+}
+
+size_t pkv_chunk_attention_workspace_size(int64_t total_q, int32_t num_seqs, int32_t num_heads,
+                                          int32_t num_kv_heads, int32_t head_dim,
+                                          int32_t block_size, int32_t max_blocks_per_seq) {
+  const pkv::ChunkArgs a = chunk_args(
+      nullptr, 0, nullptr, nullptr, reinterpret_cast<const int8_t*>(16), nullptr, nullptr, nullptr,
+      nullptr, nullptr, nullptr, total_q, num_seqs, num_heads, num_kv_heads, head_dim, block_size, 0,
+      max_blocks_per_seq, 0, 0, 1.0f);
+  if (check_chunk_sizes(a) != PKV_OK) return 0;
+  return pkv::chunk_workspace_size(a);
+}
+
+int pkv_chunk_attention(const void* q, int32_t dtype, const int8_t* k_cache, const float* k_scale,
+                        const int8_t* v_cache, const float* v_scale, const int32_t* block_tables,
+                        const int32_t* seq_lens, const int32_t* cu_seqlens, void* out, float* lse,
+                        int64_t total_q, int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
+                        int32_t head_dim, int32_t block_size, int64_t num_blocks,
+                        int32_t max_blocks_per_seq, int64_t q_token_stride, int64_t q_head_stride,
+                        float sm_scale, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  pkv::ChunkArgs a =
+      chunk_args(q, dtype, k_cache, k_scale, v_cache, v_scale, block_tables, seq_lens, cu_seqlens,
+                 out, lse, total_q, num_seqs, num_heads, num_kv_heads, head_dim, block_size,
+                 num_blocks, max_blocks_per_seq, q_token_stride, q_head_stride, sm_scale);
+  const int rc = check_chunk(a);
+  if (rc != PKV_OK) return rc;
+  if (total_q > 0 && (!out || (num_blocks > 0 && (!v_cache || !v_scale))))
+    return fail(PKV_ERR_INVALID_ARGUMENT, "null input or output pointer");
+  // (an empty cache may have no address; without one the call would be for lse alone)
+  if (a.v_cache == nullptr) a.v_cache = reinterpret_cast<const int8_t*>(16);
+  return pkv::launch_chunk(a, workspace, workspace_bytes, as_stream(stream));
+}
+
+size_t pkv_accumulate_attention_workspace_size(int64_t total_q, int32_t num_seqs,
+                                               int32_t num_heads, int32_t num_kv_heads,
+                                               int32_t head_dim, int32_t block_size,
+                                               int64_t num_blocks, int32_t max_blocks_per_seq,
+                                               int32_t has_lse) {
+  const pkv::ChunkArgs a = chunk_args(
+      nullptr, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr,
+      has_lse ? reinterpret_cast<float*>(16) : nullptr, total_q, num_seqs, num_heads, num_kv_heads,
+      head_dim, block_size, 0, max_blocks_per_seq, 0, 0, 1.0f);
+  if (num_blocks < 0 || check_chunk_sizes(a) != PKV_OK) return 0;
+  pkv::ChunkArgs b = a;
+  b.num_blocks = num_blocks;
+  return pkv::accumulate_workspace_size(b);
+}
+
+int pkv_accumulate_attention(float* weights, const void* q, int32_t dtype, const int8_t* k_cache,
+                             const float* k_scale, const int32_t* block_tables,
+                             const int32_t* seq_lens, const int32_t* cu_seqlens, const float* lse,
+                             int64_t total_q, int32_t num_seqs, int32_t num_heads,
+                             int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                             int64_t num_blocks, int32_t max_blocks_per_seq, int64_t q_token_stride,
+                             int64_t q_head_stride, float sm_scale, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+  clear_error();
+  const pkv::ChunkArgs a =
+      chunk_args(q, dtype, k_cache, k_scale, nullptr, nullptr, block_tables, seq_lens, cu_seqlens,
+                 nullptr, const_cast<float*>(lse), total_q, num_seqs, num_heads, num_kv_heads,
+                 head_dim, block_size, num_blocks, max_blocks_per_seq, q_token_stride,
+                 q_head_stride, sm_scale);
+  const int rc = check_chunk(a);
+  if (rc != PKV_OK) return rc;
+  if (total_q > 0 && num_blocks > 0 && !weights)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "null input or output pointer");
+  if (total_q * num_heads > 1 << 25)
+    return fail(PKV_ERR_UNSUPPORTED, "more than 2^25 rows of queries");
+  return pkv::launch_accumulate(a, weights, workspace, workspace_bytes, as_stream(stream));
+}
+
+int pkv_evict_tokens(int8_t* kv_cache, float* scale_cache, float* weights,
+                     const int32_t* block_tables, const int32_t* seq_lens, int32_t* lens_out,
+                     int32_t* kept, int32_t num_seqs, int64_t num_blocks, int32_t block_size,
+                     int32_t num_kv_heads, int32_t head_dim, int32_t max_blocks_per_seq,
+                     int32_t keep, int32_t sinks, int32_t recent, void* stream) {
+  clear_error();
+  if (num_seqs < 0 || num_blocks < 0 || num_kv_heads <= 0 || max_blocks_per_seq < 0)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "invalid cache or table shape");
+  if (head_dim <= 0 || head_dim > 256)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "head_dim must be 1 to 256");
+  if (block_size <= 0 || block_size > 64)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "supports block_size <= 64");
+  if (keep < 1 || sinks < 0 || recent < 0 || (int64_t)sinks + recent > keep)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "keep must be positive and hold sinks and recent");
+  const int64_t most = 0x7fffffffLL - 65536;
+  if ((int64_t)max_blocks_per_seq * block_size > most || num_blocks > most / block_size ||
+      keep > most || (int64_t)num_seqs * (2 * (int64_t)num_kv_heads + 1) > most / 8)
+    return fail(PKV_ERR_UNSUPPORTED, "more than 2^31 tokens of a table, cache slots or CTAs");
+  if (num_seqs > 0 && (!seq_lens || !lens_out || !kept || (max_blocks_per_seq > 0 && !block_tables) ||
+                       (num_blocks > 0 && (!kv_cache || !scale_cache || !weights))))
+    return fail(PKV_ERR_INVALID_ARGUMENT, "null input or output pointer");
+  pkv::EvictArgs a;
+  a.cache = kv_cache;
+  a.scales = scale_cache;
+  a.weights = weights;
+  a.tables = block_tables;
+  a.lens = seq_lens;
+  a.lens_out = lens_out;
+  a.kept = kept;
+  a.num_blocks = num_blocks;
+  a.seqs = num_seqs;
+  a.block_size = block_size;
+  a.kv_heads = num_kv_heads;
+  a.dim = head_dim;
+  a.width = max_blocks_per_seq;
+  a.keep = keep;
+  a.sinks = sinks;
+  a.recent = recent;
+  return pkv::launch_evict(a, as_stream(stream));
+}
+
 }  // extern "C"

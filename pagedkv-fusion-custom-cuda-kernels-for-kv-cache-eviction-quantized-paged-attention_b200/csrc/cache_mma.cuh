@@ -1,0 +1,221 @@
+// Pieces of the kernels in which a warp multiplies INT8 pages by mma.sync: the codes go
+// from shared memory to fp16 fragments in registers, where they are exact, and rows of
+// queries are fp16 with a power of two apart (two numbers, 22 bits, for fp32 queries).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "pkv_common.cuh"
+
+namespace pkv {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Asynchronous copies of 16 or 4 bytes of global memory to shared memory, or zeros.
+__device__ __forceinline__ void copy16_if(bool on, uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(on ? 16u : 0u)
+               : "memory");
+}
+__device__ __forceinline__ void copy4_if(bool on, uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src),
+               "r"(on ? 4u : 0u)
+               : "memory");
+}
+__device__ __forceinline__ void copies_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Four INT8 codes (little-endian) as two words of fp16 pairs, exact: byte + 128
+// in the low mantissa bits of 1024, minus 1152.
+__device__ __forceinline__ uint2 codes_to_half(uint32_t w) {
+  const uint32_t u = w ^ 0x80808080u;
+  const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+  const __half2 bias = __float2half2_rn(1152.0f);
+  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), bias);
+  const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+}
+
+__device__ __forceinline__ uint32_t word_of(__half2 h) {
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// d += a b, 16 x 8 x 16, fp16 with fp32 sums.
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint4 a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ float widen(float v) { return v; }
+__device__ __forceinline__ float widen(__half v) { return __half2float(v); }
+__device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// Four consecutive values, 8- (16-bit types) or 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p) {
+  if constexpr (sizeof(T) == 4) {
+    return *reinterpret_cast<const float4*>(p);
+  } else {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    const T* v = reinterpret_cast<const T*>(&w);
+    return make_float4(widen(v[0]), widen(v[1]), widen(v[2]), widen(v[3]));
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float4 v) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = v;
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+    *reinterpret_cast<uint2*>(p) = make_uint2(word_of(a), word_of(b));
+  } else {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a),
+                                              *reinterpret_cast<const uint32_t*>(&b));
+  }
+}
+
+// The power of two that takes a row of largest magnitude `big` to [2^10, 2^11), as
+// its exponent; 0 for rows that are zero or not finite.
+__device__ __forceinline__ int row_exponent(float big) {
+  int e = 137 - (int)(__float_as_uint(big) >> 23);
+  if (big == 0.0f || !(big <= 3.402823466e38f)) e = 0;
+  return min(e, 126);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
+
+// 16 rows of queries in shared memory in the order in which lanes read mma operands:
+// [half][DP / 16][lane] of 16 bytes.  Called by `warps` warps, each for some rows; lane
+// = 4 channels.  A k step of 16 stands for channels p * 64 + t * 16 + w * 4 + 0..3 of
+// lane t (of 4), step p * 4 + w, as the codes are read: 16 bytes a lane.
+// row(r) is the row's first channel or null; factor[r] becomes what its products have
+// to be multiplied by.
+template <typename T, int DP, int HALVES, typename Row>
+__device__ __forceinline__ void stage_queries(uint4* frag, float* factor, int dim, int warp,
+                                              int warps, Row row) {
+  const int lane = threadIdx.x & 31;
+  for (int r = warp; r < 16; r += warps) {
+    const T* from = row(r);
+    constexpr int kParts = (DP + 127) / 128;
+    float4 v[kParts];
+    float big = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) {
+      const int c = i * 128 + lane * 4;
+      v[i] = from != nullptr && c < dim ? load4(from + c) : make_float4(0, 0, 0, 0);
+      big = fmaxf(big, fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w))));
+    }
+    float up = 1.0f, down = 1.0f;
+    if constexpr (!std::is_same<T, __half>::value) {
+      big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
+      const int e = row_exponent(big);
+      up = power_of_two(e);
+      down = power_of_two(-e);
+    }
+    if (lane == 0) factor[r] = down;
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) {
+      const int c = i * 128 + lane * 4;
+      if (c >= DP) continue;
+      const float f[4] = {v[i].x * up, v[i].y * up, v[i].z * up, v[i].w * up};
+      const __half2 h0 = __floats2half2_rn(f[0], f[1]), h1 = __floats2half2_rn(f[2], f[3]);
+      uint32_t* to = reinterpret_cast<uint32_t*>(
+                         &frag[(c / 64 * 4 + c % 16 / 4) * 32 + (r & 7) * 4 + c % 64 / 16]) +
+                     (r >> 3);
+      to[0] = word_of(h0);
+      to[2] = word_of(h1);
+      if constexpr (HALVES == 2) {
+        const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
+        to += DP / 16 * 32 * 4;
+        to[0] = word_of(__floats2half2_rn(f[0] - b0.x, f[1] - b0.y));
+        to[2] = word_of(__floats2half2_rn(f[2] - b1.x, f[3] - b1.y));
+      }
+    }
+  }
+}
+
+// 16-byte piece of a key's row of DP codes in shared memory, so that the lanes that
+// read 8 keys' pieces at once (K: pieces t, keys g; V: pieces g, keys 2 t) meet no bank
+// twice.
+template <int DP>
+__device__ __forceinline__ int piece_at(int key, int piece) {
+  if constexpr (DP >= 128)
+    return (piece & ~7) | ((piece & 7) ^ ((key & 6) ^ ((key & 1) << 2)));
+  else
+    return piece ^ ((key >> 1) & 3);
+}
+
+// ---------------------------------------------------------------------------
+// The plan of a call over packed new tokens and their sequences' pages
+// ---------------------------------------------------------------------------
+
+struct PlanSeq {
+  int q0, lq;   // the sequence's rows in the packed queries
+  int len;      // its cached tokens, the new ones among them
+  int splits;   // parts of its keys
+  int first;    // first item
+  int slot;     // first partial result (sequences of more than one part)
+  int unit;     // first counter of the same
+  int pad;
+};
+
+struct PlanHead {
+  int items;         // in all
+  int split_keys;    // keys of a part
+  int q_begin, q_end;  // rows of all sequences
+  int pad[4];
+};
+
+struct PlanArgs {
+  const int32_t* cu;
+  const int32_t* lens;
+  int seqs, total_q;
+  int group, kv_heads, block_size, width;
+  int rows;           // rows of an item
+  int target;         // items to aim at where sequences are split; 0: parts of `least` keys
+  int least;          // keys of the smallest part, a multiple of `round`
+  int round;
+  PlanHead* head;
+  PlanSeq* seq;       // [seqs]
+  int* counters;      // [counts], zeroed
+  int counts;
+};
+
+// Splits sequences into parts so that about `target` items have equal work.  Sequences
+// of more than one part have fewer than 2 target items.
+int launch_plan(const PlanArgs& a, int* err, cudaStream_t stream);
+
+// The sequence of an item; one warp, a search of 32 at a time.
+__device__ __forceinline__ int plan_find(const PlanSeq* seq, int seqs, int item) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = seqs;  // the last sequence of [lo, lo + n) whose first item is <= item
+  while (n > 1) {
+    const int step = (n + 31) / 32;
+    const int at = lo + lane * step;
+    const bool below = lane * step < n && seq[at].first <= item;
+    const int last = 31 - __clz(__ballot_sync(0xffffffffu, below));
+    lo += last * step;
+    n = min(step, n - last * step);
+  }
+  return lo;
+}
+
+}  // namespace pkv

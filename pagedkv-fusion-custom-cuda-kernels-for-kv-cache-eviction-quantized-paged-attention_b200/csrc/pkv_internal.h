@@ -184,4 +184,47 @@ size_t shared_prefix_workspace_size(const SharedPrefixArgs& a);
 int launch_shared_prefix(const SharedPrefixArgs& a, void* workspace, size_t workspace_bytes,
                          cudaStream_t stream);
 
+// ---- chunk.cu --------------------------------------------------------------
+struct ChunkArgs {
+  const void* q;
+  int dtype;  // 0 fp32, 1 fp16, 2 bf16: of q and out
+  const int8_t* k_cache;
+  const float* k_scale;
+  const int8_t* v_cache;  // null: only lse is computed
+  const float* v_scale;
+  const int32_t* tables;  // [seqs, width]
+  const int32_t* lens;    // [seqs]
+  const int32_t* cu;      // [seqs + 1]
+  void* out;
+  float* lse;  // nullable
+  int64_t total_q, num_blocks;
+  int64_t q_token_stride, q_head_stride;  // elements, of 16 bytes
+  int seqs, heads, kv_heads, dim, block_size, width;
+  float sm_scale;
+};
+size_t chunk_workspace_size(const ChunkArgs& a);
+int launch_chunk(const ChunkArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t stream);
+
+// ---- weights.cu ------------------------------------------------------------
+// q, the K cache and the tables of `a`, and a.lse as input (nullable: computed first);
+// a.v_cache, a.v_scale and a.out are unused.  weights [num_blocks, block_size] is added to.
+size_t accumulate_workspace_size(const ChunkArgs& a);
+int launch_accumulate(const ChunkArgs& a, float* weights, void* workspace, size_t workspace_bytes,
+                      cudaStream_t stream);
+
+// ---- evict.cu ----------------------------------------------------------------
+struct EvictArgs {
+  int8_t* cache;   // [2, num_blocks, block_size, kv_heads, dim]
+  float* scales;   // [2, num_blocks, kv_heads]
+  float* weights;  // [num_blocks, block_size]
+  const int32_t* tables;
+  const int32_t* lens;
+  int32_t* lens_out;
+  int32_t* kept;   // [seqs, keep]
+  int64_t num_blocks;
+  int seqs, block_size, kv_heads, dim, width;
+  int keep, sinks, recent;
+};
+int launch_evict(const EvictArgs& a, cudaStream_t stream);
+
 }  // namespace pkv

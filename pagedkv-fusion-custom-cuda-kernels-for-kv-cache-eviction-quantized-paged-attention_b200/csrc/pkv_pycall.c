@@ -1,5 +1,5 @@
 /* Direct CPython calls into the C ABI for the eviction latency path and the
- * prompt and shared-prefix operators.
+ * prompt, shared-prefix and growing-cache operators.
  *
  * The eviction decision (score 16K blocks, select the k lowest) takes
  * ~13 us on the GPU, so the host cost of reaching the launch matters: a
@@ -185,6 +185,59 @@ static PyObject* py_shared_prefix_attention(PyObject* self, PyObject* const* a, 
                                                      ws, (size_t)wsb, stream));
 }
 
+/* The arguments of pkv_chunk_attention. */
+static PyObject* py_chunk_attention(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  void *q, *kc, *ks, *vc, *vs, *bt, *sl, *cu, *out, *lse, *ws, *stream;
+  int32_t dtype, seqs, heads, kv, dim, bs, width;
+  int64_t tq, blocks, qt, qh, wsb;
+  float scale;
+  (void)self;
+  if (!nargs_ok(n, 25, "chunk_attention")) return NULL;
+  if (PTR(0, q) || I32(1, dtype) || PTR(2, kc) || PTR(3, ks) || PTR(4, vc) || PTR(5, vs) ||
+      PTR(6, bt) || PTR(7, sl) || PTR(8, cu) || PTR(9, out) || PTR(10, lse) || I64(11, tq) ||
+      I32(12, seqs) || I32(13, heads) || I32(14, kv) || I32(15, dim) || I32(16, bs) ||
+      I64(17, blocks) || I32(18, width) || I64(19, qt) || I64(20, qh) || F32(21, scale) ||
+      PTR(22, ws) || I64(23, wsb) || PTR(24, stream))
+    return NULL;
+  return PyLong_FromLong(pkv_chunk_attention(q, dtype, kc, ks, vc, vs, bt, sl, cu, out, lse, tq,
+                                             seqs, heads, kv, dim, bs, blocks, width, qt, qh,
+                                             scale, ws, (size_t)wsb, stream));
+}
+
+/* The arguments of pkv_accumulate_attention. */
+static PyObject* py_accumulate_attention(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  void *w, *q, *kc, *ks, *bt, *sl, *cu, *lse, *ws, *stream;
+  int32_t dtype, seqs, heads, kv, dim, bs, width;
+  int64_t tq, blocks, qt, qh, wsb;
+  float scale;
+  (void)self;
+  if (!nargs_ok(n, 23, "accumulate_attention")) return NULL;
+  if (PTR(0, w) || PTR(1, q) || I32(2, dtype) || PTR(3, kc) || PTR(4, ks) || PTR(5, bt) ||
+      PTR(6, sl) || PTR(7, cu) || PTR(8, lse) || I64(9, tq) || I32(10, seqs) || I32(11, heads) ||
+      I32(12, kv) || I32(13, dim) || I32(14, bs) || I64(15, blocks) || I32(16, width) ||
+      I64(17, qt) || I64(18, qh) || F32(19, scale) || PTR(20, ws) || I64(21, wsb) ||
+      PTR(22, stream))
+    return NULL;
+  return PyLong_FromLong(pkv_accumulate_attention(w, q, dtype, kc, ks, bt, sl, cu, lse, tq, seqs,
+                                                  heads, kv, dim, bs, blocks, width, qt, qh, scale,
+                                                  ws, (size_t)wsb, stream));
+}
+
+/* The arguments of pkv_evict_tokens. */
+static PyObject* py_evict_tokens(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  void *cache, *scales, *w, *bt, *sl, *lens, *kept, *stream;
+  int32_t seqs, bs, kv, dim, width, keep, sinks, recent;
+  int64_t blocks;
+  (void)self;
+  if (!nargs_ok(n, 17, "evict_tokens")) return NULL;
+  if (PTR(0, cache) || PTR(1, scales) || PTR(2, w) || PTR(3, bt) || PTR(4, sl) || PTR(5, lens) ||
+      PTR(6, kept) || I32(7, seqs) || I64(8, blocks) || I32(9, bs) || I32(10, kv) || I32(11, dim) ||
+      I32(12, width) || I32(13, keep) || I32(14, sinks) || I32(15, recent) || PTR(16, stream))
+    return NULL;
+  return PyLong_FromLong(pkv_evict_tokens(cache, scales, w, bt, sl, lens, kept, seqs, blocks, bs,
+                                          kv, dim, width, keep, sinks, recent, stream));
+}
+
 static PyMethodDef kMethods[] = {
     {"eviction_scores", (PyCFunction)(void (*)(void))py_eviction_scores, METH_FASTCALL,
      "pkv_eviction_scores; returns the status code"},
@@ -200,6 +253,12 @@ static PyMethodDef kMethods[] = {
      "pkv_prefill_attention_ws; returns the status code"},
     {"shared_prefix_attention", (PyCFunction)(void (*)(void))py_shared_prefix_attention,
      METH_FASTCALL, "pkv_shared_prefix_attention; returns the status code"},
+    {"chunk_attention", (PyCFunction)(void (*)(void))py_chunk_attention, METH_FASTCALL,
+     "pkv_chunk_attention; returns the status code"},
+    {"accumulate_attention", (PyCFunction)(void (*)(void))py_accumulate_attention, METH_FASTCALL,
+     "pkv_accumulate_attention; returns the status code"},
+    {"evict_tokens", (PyCFunction)(void (*)(void))py_evict_tokens, METH_FASTCALL,
+     "pkv_evict_tokens; returns the status code"},
     {NULL, NULL, 0, NULL}};
 
 static struct PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_pkv_pycall",

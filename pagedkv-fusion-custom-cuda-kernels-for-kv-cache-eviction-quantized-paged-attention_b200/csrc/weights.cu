@@ -1,0 +1,333 @@
+// Attention weights gathered per cached token: what the eviction statistics are made of.
+//
+//   weights[page(j), offset(j)] += 1/H sum over the call's tokens i and heads h of
+//                                  exp(scale q[i, h] . k_j - lse[i, h]),  j <= i + L - Lq
+//
+// with lse as the attention gave it, or taken first by the attention's own kernel
+// without its second product.
+//
+//   gather_kernel   an item is (sequence, KV head, 256 keys, at most 1,024 query rows).
+//                   A warp keeps 32 keys as fragments in registers and lets the rows
+//                   pass, 16 at a time, from shared memory; each lane sums its keys'
+//                   columns over the rows.
+//   spread_kernel   adds the sums to the weights.
+//
+// Sums of several items, and of sequences that share pages, meet as integers of 2^-38
+// in a workspace, so that the order of their arrival changes nothing.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <string>
+#include <type_traits>
+
+#include "cache_mma.cuh"
+#include "pkv_internal.h"
+
+namespace pkv {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr int kWarpKeys = 32;
+constexpr int kKeys = kWarps * kWarpKeys;  // of an item
+constexpr int kItemRows = 1024;            // fp32 sums of 64 values a lane, then exact
+constexpr float kUnit = 274877906944.0f;   // 2^38: 2^25 of weight before bit 63
+constexpr unsigned long long kNotFinite = 1ull << 63;
+
+struct GatherParams {
+  const void* q;
+  const int8_t* k_cache;
+  const float* k_scale;
+  const int32_t* tables;
+  const float* lse;
+  const PlanHead* head;
+  const PlanSeq* seq;
+  unsigned long long* sums;  // [num_blocks, block_size], zero for pages in the tables
+  int64_t q_tok, q_head;
+  int64_t num_blocks;
+  int seqs, heads, kv_heads, group, dim, bs, width;
+  float qk_scale;
+};
+
+template <typename T, int DP, int HALVES>
+__global__ void __launch_bounds__(kThreads, DP > 128 ? 1 : 2) gather_kernel(const GatherParams p, int* err) {
+  constexpr int kSteps = DP / 16;
+  constexpr int kTiles = kWarpKeys / 8;
+  __shared__ uint4 s_q[HALVES * kSteps * 32];
+  __shared__ float s_factor[16], s_lse[16];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int items = p.head->items;
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    const int s = plan_find(p.seq, p.seqs, item);
+    const PlanSeq seq = p.seq[s];
+    const int local = item - seq.first;
+    const int kvh = local % p.kv_heads;
+    const int64_t all_rows = seq.lq * (int64_t)p.group;
+    const int chunks = (int)((all_rows + kItemRows - 1) / kItemRows);
+    const int chunk = local / p.kv_heads % chunks, part = local / p.kv_heads / chunks;
+    const int k0 = part * kKeys + warp * kWarpKeys;  // of this warp
+    const int shift = seq.len - seq.lq;
+    const int32_t* table = p.tables + (int64_t)s * p.width;
+    // rows of this item that see the item's first key
+    const int64_t r_end = min(all_rows, (chunk + 1) * (int64_t)kItemRows);
+    const int64_t r_first = max((int64_t)(part * kKeys - shift), (int64_t)0) * p.group;
+    const int64_t r_begin = max(chunk * (int64_t)kItemRows, r_first / 16 * 16);
+
+    // this warp's keys: lane = key, then fragments
+    const int key = k0 + lane, page = key / p.bs;
+    const bool counts = key < seq.len;
+    const int phys = counts ? table[page] : -1;
+    const bool good = counts && phys >= 0 && (int64_t)phys < p.num_blocks;
+    if (counts && !good) record_error(err, kDevBadBlockId);
+    const uint32_t at = good ? (uint32_t)phys * p.bs + (key - page * p.bs) : 0xffffffffu;
+    const float ks = good ? p.k_scale[(int64_t)phys * p.kv_heads + kvh] : 0.0f;
+    const unsigned mask = __ballot_sync(0xffffffffu, good);
+    uint2 b[kTiles][kSteps];
+    float scale[kTiles][2];
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+      const uint32_t row = __shfl_sync(0xffffffffu, at, n * 8 + g);
+      uint4 w[DP / 64];
+#pragma unroll
+      for (int c = 0; c < DP / 64; ++c) {
+        const int piece = c * 4 + t;
+        w[c] = make_uint4(0, 0, 0, 0);
+        if (row != 0xffffffffu && piece * 16 < p.dim)
+          w[c] = __ldg(reinterpret_cast<const uint4*>(
+              p.k_cache + ((int64_t)row * p.kv_heads + kvh) * p.dim + piece * 16));
+      }
+#pragma unroll
+      for (int c = 0; c < DP / 64; ++c) {
+        b[n][c * 4] = codes_to_half(w[c].x);
+        b[n][c * 4 + 1] = codes_to_half(w[c].y);
+        b[n][c * 4 + 2] = codes_to_half(w[c].z);
+        b[n][c * 4 + 3] = codes_to_half(w[c].w);
+      }
+      scale[n][0] = __shfl_sync(0xffffffffu, ks, n * 8 + 2 * t);
+      scale[n][1] = __shfl_sync(0xffffffffu, ks, n * 8 + 2 * t + 1);
+    }
+    float sum[kTiles][2] = {};
+    for (int64_t r0 = r_begin; r0 < r_end; r0 += 16) {
+      const int rows = (int)min((int64_t)16, r_end - r0);
+      __syncthreads();  // the last rows are used
+      stage_queries<T, DP, HALVES>(s_q, s_factor, p.dim, warp, kWarps, [&](int r) -> const T* {
+        if (r >= rows) return nullptr;
+        const int tok = (int)((r0 + r) / p.group);
+        return static_cast<const T*>(p.q) + (seq.q0 + tok) * p.q_tok +
+               (kvh * p.group + (int)(r0 + r - (int64_t)tok * p.group)) * p.q_head;
+      });
+      if (tid < 16) {
+        float v = -INFINITY;
+        if (tid < rows) {
+          const int tok = (int)((r0 + tid) / p.group);
+          v = p.lse[(int64_t)(seq.q0 + tok) * p.heads + kvh * p.group + (r0 + tid - (int64_t)tok * p.group)];
+        }
+        s_lse[tid] = v;
+      }
+      __syncthreads();
+      float d[kTiles][4] = {};
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+        for (int h = HALVES - 1; h >= 0; --h) {
+          const uint4 a = s_q[(h * kSteps + k) * 32 + lane];
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n) mma_f16(d[n], a, b[n][k].x, b[n][k].y);
+        }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int row = g + 8 * r;
+        const float f = s_factor[row] * p.qk_scale;
+        const float lse = s_lse[row];
+        // a row without keys (lse -inf) adds nothing
+        const bool none = row >= rows || lse == -INFINITY;
+        const int limit = none ? 0 : (int)((r0 + row) / p.group) + 1 + shift;
+        const float base = none ? 0.0f : lse * kLog2e;
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int at_key = n * 8 + 2 * t + e;
+            const float x = ex2(fmaf(d[n][2 * r + e], scale[n][e] * f, -base));
+            sum[n][e] += (mask >> at_key & 1u) && k0 + at_key < limit ? x : 0.0f;
+          }
+      }
+    }
+    // the lanes of a column, then one adds
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], x);
+        const int from = n * 8 + 2 * t + e;
+        const uint32_t slot = __shfl_sync(0xffffffffu, at, from);
+        if (g == 0 && slot != 0xffffffffu && r_begin < r_end) {
+          const float v = sum[n][e];
+          if (v < 33554432.0f) {
+            const unsigned long long u = __float2ull_rn(v * kUnit);
+            if (u != 0) atomicAdd(p.sums + slot, u);
+          } else {
+            atomicOr(p.sums + slot, kNotFinite);  // NaN, or lse of other tokens
+          }
+        }
+      }
+  }
+}
+
+// The workspace of the tables' pages becomes zero, or is added to the weights.  A page
+// may be in several tables: whoever comes first takes its sum and leaves a zero.
+template <bool ADD>
+__global__ void __launch_bounds__(256) spread_kernel(const int32_t* tables, const int32_t* lens,
+                                                     unsigned long long* sums, float* weights,
+                                                     int64_t num_blocks, int bs, int width,
+                                                     int64_t slots, float inv_heads) {
+  const int64_t per_seq = (int64_t)width * bs;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < slots; i += gridDim.x * 256ll) {
+    const int64_t s = i / per_seq;
+    const int at = (int)(i - s * per_seq);
+    if (at >= lens[s]) continue;
+    const int page = at / bs, phys = tables[s * width + page];
+    if (phys < 0 || (int64_t)phys >= num_blocks) continue;
+    const int64_t slot = (int64_t)phys * bs + (at - page * bs);
+    if constexpr (ADD) {
+      const unsigned long long u = atomicExch(sums + slot, 0ull);
+      if (u != 0)
+        weights[slot] += u & kNotFinite ? __int_as_float(0x7fffffff)
+                                        : (float)((double)u * (1.0 / (double)kUnit)) * inv_heads;
+    } else {
+      sums[slot] = 0ull;
+    }
+  }
+}
+
+struct Layout {
+  size_t head, seq, lse, sums, inner, total;
+};
+
+Layout layout(const ChunkArgs& a) {
+  Layout l;
+  size_t at = 0;
+  const auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  l.head = take(sizeof(PlanHead));
+  l.seq = take(sizeof(PlanSeq) * (size_t)a.seqs);
+  l.sums = take((size_t)a.num_blocks * a.block_size * 8);
+  l.lse = take(a.lse == nullptr ? (size_t)a.total_q * a.heads * 4 : 0);
+  l.inner = at;
+  if (a.lse == nullptr) {
+    ChunkArgs b = a;
+    b.v_cache = nullptr;
+    at += chunk_workspace_size(b);
+  }
+  l.total = at + 256;
+  return l;
+}
+
+template <typename T, int DP>
+void launch_gather(const ChunkArgs& a, const float* lse, uint8_t* ws, const Layout& lay, int* err,
+                   cudaStream_t stream) {
+  constexpr int HALVES = sizeof(T) == 4 ? 2 : 1;
+  GatherParams p;
+  p.q = a.q;
+  p.k_cache = a.k_cache;
+  p.k_scale = a.k_scale;
+  p.tables = a.tables;
+  p.lse = lse;
+  p.head = reinterpret_cast<PlanHead*>(ws + lay.head);
+  p.seq = reinterpret_cast<PlanSeq*>(ws + lay.seq);
+  p.sums = reinterpret_cast<unsigned long long*>(ws + lay.sums);
+  p.q_tok = a.q_token_stride;
+  p.q_head = a.q_head_stride;
+  p.num_blocks = a.num_blocks;
+  p.seqs = a.seqs;
+  p.heads = a.heads;
+  p.kv_heads = a.kv_heads;
+  p.group = a.heads / a.kv_heads;
+  p.dim = a.dim;
+  p.bs = a.block_size;
+  p.width = a.width;
+  p.qk_scale = a.sm_scale * kLog2e;
+  const int64_t parts = ((int64_t)a.width * a.block_size + kKeys - 1) / kKeys;
+  const int64_t chunks = a.total_q * p.group / kItemRows + std::min<int64_t>(a.seqs, a.total_q);
+  const int64_t most = 148 * (DP > 128 ? 1 : 2);
+  const int64_t grid = std::min(most, std::min(most, parts) * chunks * a.kv_heads);
+  gather_kernel<T, DP, HALVES><<<(unsigned)grid, kThreads, 0, stream>>>(p, err);
+}
+
+}  // namespace
+
+size_t accumulate_workspace_size(const ChunkArgs& a) {
+  if (a.total_q == 0 || a.seqs == 0 || a.width == 0) return 0;
+  return layout(a).total;
+}
+
+int launch_accumulate(const ChunkArgs& a, float* weights, void* workspace, size_t workspace_bytes,
+                      cudaStream_t stream) {
+  if (a.total_q == 0 || a.seqs == 0 || a.width == 0) return kOk;
+  const Layout lay = layout(a);
+  if (workspace == nullptr || workspace_bytes < lay.total) {
+    set_error("workspace too small for accumulate_attention: need " + std::to_string(lay.total) +
+              " bytes");
+    return kWorkspace;
+  }
+  uint8_t* ws = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 255) &
+                                           ~(uintptr_t)255);
+  int* err = device_error_word();
+  const float* lse = a.lse;
+  if (lse == nullptr) {
+    ChunkArgs b = a;
+    b.v_cache = nullptr;
+    b.lse = reinterpret_cast<float*>(ws + lay.lse);
+    lse = b.lse;
+    const int rc = launch_chunk(b, ws + lay.inner, chunk_workspace_size(b), stream);
+    if (rc != kOk) return rc;
+  }
+  PlanArgs plan;
+  plan.cu = a.cu;
+  plan.lens = a.lens;
+  plan.seqs = a.seqs;
+  plan.total_q = (int)a.total_q;
+  plan.group = a.heads / a.kv_heads;
+  plan.kv_heads = a.kv_heads;
+  plan.block_size = a.block_size;
+  plan.width = a.width;
+  plan.rows = kItemRows;
+  plan.target = 0;  // parts of the smallest size
+  plan.least = kKeys;
+  plan.round = kKeys;
+  plan.head = reinterpret_cast<PlanHead*>(ws + lay.head);
+  plan.seq = reinterpret_cast<PlanSeq*>(ws + lay.seq);
+  plan.counters = nullptr;
+  plan.counts = 0;
+  const int rc = launch_plan(plan, err, stream);
+  if (rc != kOk) return rc;
+  auto* sums = reinterpret_cast<unsigned long long*>(ws + lay.sums);
+  const int64_t slots = (int64_t)a.seqs * a.width * a.block_size;
+  const unsigned grid = (unsigned)std::min<int64_t>((slots + 255) / 256, 148 * 8);
+  spread_kernel<false><<<grid, 256, 0, stream>>>(a.tables, a.lens, sums, weights, a.num_blocks,
+                                                 a.block_size, a.width, slots, 0.0f);
+  const auto with_dim = [&](auto t) {
+    using T = decltype(t);
+    if (a.dim <= 64) launch_gather<T, 64>(a, lse, ws, lay, err, stream);
+    else if (a.dim <= 128) launch_gather<T, 128>(a, lse, ws, lay, err, stream);
+    else launch_gather<T, 256>(a, lse, ws, lay, err, stream);
+  };
+  if (a.dtype == 0) with_dim(0.0f);
+  else if (a.dtype == 1) with_dim(__half());
+  else with_dim(__nv_bfloat16());
+  spread_kernel<true><<<grid, 256, 0, stream>>>(a.tables, a.lens, sums, weights, a.num_blocks,
+                                                a.block_size, a.width, slots, 1.0f / a.heads);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) {
+    set_error(std::string("accumulate launch failed: ") + cudaGetErrorString(e));
+    return kCudaError;
+  }
+  return kOk;
+}
+
+}  // namespace pkv

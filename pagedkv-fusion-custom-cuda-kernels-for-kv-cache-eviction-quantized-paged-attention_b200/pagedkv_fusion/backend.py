@@ -28,7 +28,11 @@ reference's surface, for a caller that has its own model code:
 * ``prefill_forward`` is the prompt's attention over packed sequences;
 * ``append_to_cache`` rotates the keys on the way and keeps a started page's
   earlier tokens readable (``write_to_cache`` replaces the page's scale);
-* ``shared_prefix_forward`` decodes a batch whose sequences share a prefix.
+* ``shared_prefix_forward`` decodes a batch whose sequences share a prefix;
+* ``chunk_forward`` attends any number of new tokens of each sequence over the
+  INT8 cache (chunked prompts, drafted tokens, 16-bit decode);
+* ``accumulate_weights`` gathers their attention weights per cached token, and
+  ``evict_tokens`` cuts sequences to their heaviest tokens.
 """
 
 from __future__ import annotations
@@ -179,6 +183,61 @@ class PagedKVFusionBackend:
             metadata.block_tables, metadata.seq_lens,
             scale,
         )
+
+    def chunk_forward(
+        self,
+        query: torch.Tensor,          # [total_q, num_heads, head_dim]
+        kv_cache_int8: torch.Tensor,  # [2, num_blocks, block_size, nkv, hd]
+        scale_cache: torch.Tensor,    # [2, num_blocks, num_kv_heads]
+        metadata: PagedKVFusionMetadata,
+        cu_seqlens: torch.Tensor,     # [num_seqs + 1] int32
+        scale: float,
+        return_lse: bool = False,
+    ):
+        """Attention of new tokens that are in the cache already:
+        ``metadata.seq_lens`` counts them.  See
+        :func:`~pagedkv_fusion.ops.chunk_attention`."""
+        return ops.chunk_attention(
+            query,
+            kv_cache_int8[0], scale_cache[0],
+            kv_cache_int8[1], scale_cache[1],
+            metadata.block_tables, metadata.seq_lens, cu_seqlens,
+            scale, return_lse=return_lse,
+        )
+
+    def accumulate_weights(
+        self,
+        weights: torch.Tensor,        # [num_blocks, block_size] float32, added to
+        query: torch.Tensor,          # [total_q, num_heads, head_dim]
+        kv_cache_int8: torch.Tensor,  # [2, num_blocks, block_size, nkv, hd]
+        scale_cache: torch.Tensor,    # [2, num_blocks, num_kv_heads]
+        metadata: PagedKVFusionMetadata,
+        cu_seqlens: torch.Tensor,     # [num_seqs + 1] int32
+        scale: float,
+        lse: torch.Tensor | None = None,
+    ) -> None:
+        """Adds the new tokens' attention weights to their cached tokens': see
+        :func:`~pagedkv_fusion.ops.accumulate_attention`."""
+        ops.accumulate_attention(weights, query, kv_cache_int8[0], scale_cache[0],
+                                 metadata.block_tables, metadata.seq_lens, cu_seqlens, scale,
+                                 lse=lse)
+
+    def evict_tokens(
+        self,
+        kv_cache_int8: torch.Tensor,  # [2, num_blocks, block_size, nkv, hd]
+        scale_cache: torch.Tensor,    # [2, num_blocks, num_kv_heads]
+        weights: torch.Tensor,        # [num_blocks, block_size] float32
+        metadata: PagedKVFusionMetadata,
+        keep: int,
+        sinks: int = 0,
+        recent: int = 0,
+    ) -> PagedKVFusionMetadata:
+        """Cuts the sequences to ``keep`` tokens in place and returns the
+        metadata with their new lengths: see
+        :func:`~pagedkv_fusion.ops.evict_tokens`."""
+        lens, _ = ops.evict_tokens(kv_cache_int8, scale_cache, weights, metadata.block_tables,
+                                   metadata.seq_lens, keep, sinks=sinks, recent=recent)
+        return dataclasses.replace(metadata, seq_lens=lens)
 
     def forward(self, *args, is_prefill: bool, **kwargs):
         """Prefill (and a build without the native library) goes to the

@@ -45,6 +45,9 @@ __all__ = [
     "append_kv",
     "prefill_attention",
     "shared_prefix_attention",
+    "chunk_attention",
+    "accumulate_attention",
+    "evict_tokens",
 ]
 
 
@@ -450,3 +453,83 @@ def shared_prefix_attention(q, k_cache_q, k_scale, v_cache_q, v_scale, prefix_ta
              torch.int32, torch.int32)
     return st.back(C.shared_prefix_attention(*(st.to_device(a, t) for a, t in zip(args, types)),
                                              sm_scale))
+
+
+# ---------------------------------------------------------------------------
+# A growing cache: new tokens' attention, their weights, eviction of tokens
+# ---------------------------------------------------------------------------
+
+def chunk_attention(q, k_cache_q, k_scale, v_cache_q, v_scale, block_tables, seq_lens, cu_seqlens,
+                    sm_scale: float, return_lse: bool = False):
+    """Attention of new tokens over the INT8 paged cache that holds them: one
+    token of a sequence, a few drafted ones, or the next chunk of a prompt, and
+    any mixture of these in one call.
+
+    ``q`` ``[total_q, H, D]`` (float32, float16 or bfloat16; strided views with
+    contiguous channels are read in place) holds the sequences' new tokens one
+    behind the other, sequence s in rows ``cu_seqlens[s] .. cu_seqlens[s + 1]``
+    (int32 ``[S + 1]``).  ``seq_lens`` ``[S]`` counts a sequence's tokens in the
+    cache, the new ones among them (:func:`append_kv` comes first): token i of Lq
+    sees the cached tokens ``j <= i + L - Lq``.  Caches, scales and tables as in
+    :func:`quant_paged_attention`.  D a multiple of 32 up to 256, block size up to
+    64, any group of query heads.
+
+    Returns ``[total_q, H, D]`` in ``q``'s type, and with ``return_lse`` also the
+    float32 ``[total_q, H]`` natural logarithms of the softmax denominators.  Rows
+    that see no token, and rows behind the last sequence or in front of the first,
+    are zero (lse -inf).  fp32 queries keep fp32 accuracy; for 16-bit ones the
+    probabilities have fp16's 11 bits in their product with the values.  No
+    backward pass.
+    """
+    C = _lib()
+    args = (q, k_cache_q, k_scale, v_cache_q, v_scale, block_tables, seq_lens, cu_seqlens)
+    if _all_cuda(*args):
+        return C.chunk_attention(*args, sm_scale, return_lse)
+    st = _Staging(*args)
+    types = (None, None, torch.float32, None, torch.float32, torch.int32, torch.int32, torch.int32)
+    got = C.chunk_attention(*(st.to_device(a, t) for a, t in zip(args, types)), sm_scale,
+                            return_lse)
+    return tuple(st.back(t) for t in got) if return_lse else st.back(got)
+
+
+def accumulate_attention(weights, q, k_cache_q, k_scale, block_tables, seq_lens, cu_seqlens,
+                         sm_scale: float, lse=None) -> None:
+    """Adds to ``weights`` (float32 ``[NB, bs]``, one per cached token, in place)
+    what the new tokens ``q`` attend to it: the sum over the tokens and the mean
+    over the query heads of their softmax probabilities, so that every token
+    spreads a weight of 1.
+
+    Arguments as in :func:`chunk_attention`; ``lse`` are the log denominators that
+    it returned for the same tokens, computed first where they are not given.  The
+    result feeds :func:`eviction_scores` as ``attn_weights`` (whole blocks) and
+    :func:`evict_tokens` (single tokens); to let old weight fade, scale
+    ``weights`` between calls.  A page in several tables gathers from all of them.
+    The result does not depend on the order of execution.  A page that is given to
+    a new sequence needs its weights zeroed.  ``weights`` must be a contiguous CUDA
+    tensor, as all the others.  No backward pass.
+    """
+    _lib().accumulate_attention(weights, q, k_cache_q, k_scale, block_tables, seq_lens, cu_seqlens,
+                                sm_scale, lse)
+
+
+def evict_tokens(kv_cache_int8, scale_cache, weights, block_tables, seq_lens, keep: int,
+                 sinks: int = 0, recent: int = 0):
+    """Evicts single tokens from the paged INT8 cache by the weights that they
+    gathered (:func:`accumulate_attention`), in place.
+
+    A sequence of more than ``keep`` tokens keeps its first ``sinks``, its last
+    ``recent`` and the heaviest of the others (of equal weights the earlier one,
+    NaN heaviest), ``keep`` in all; they move, in order, to the front of its pages
+    in ``kv_cache_int8`` ``[2, NB, bs, Hkv, D]``, ``scale_cache`` ``[2, NB, Hkv]``
+    and ``weights`` ``[NB, bs]``.  A page takes the largest scale of the tokens it
+    then holds, and codes of smaller scales are rounded to it.  Slots no longer
+    used get weight 0.  Shorter sequences stay as they are.  Rotated keys keep the
+    positions that they were rotated by.
+
+    Returns ``(lens, kept)``: the new lengths, int32 ``[S]``, and the old places of
+    the tokens that stayed, int32 ``[S, keep]``, ascending, then -1.  The pages
+    behind the new lengths are free.  A sequence that is cut must not share pages
+    with another one.  CUDA tensors only.
+    """
+    return _lib().evict_tokens(kv_cache_int8, scale_cache, weights, block_tables, seq_lens, keep,
+                               sinks, recent)
