@@ -80,7 +80,7 @@ __device__ __forceinline__ float4 load4(const T* p) {
   }
 }
 template <typename T>
-__device__ __forceinline__ void store4(T* p, float4 v) {
+__device__ __forceinline__ void store4(T* p, float4 v) {  // (aligned as above)
   if constexpr (sizeof(T) == 4) {
     *reinterpret_cast<float4*>(p) = v;
   } else if constexpr (std::is_same<T, __half>::value) {
@@ -102,17 +102,34 @@ __device__ __forceinline__ int row_exponent(float big) {
 }
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
 
-// 16 rows of queries in shared memory in the order in which lanes read mma operands:
-// [half][DP / 16][lane] of 16 bytes.  Called by `warps` warps, each for some rows; lane
-// = 4 channels.  A k step of 16 stands for channels p * 64 + t * 16 + w * 4 + 0..3 of
-// lane t (of 4), step p * 4 + w, as the codes are read: 16 bytes a lane.
-// row(r) is the row's first channel or null; factor[r] becomes what its products have
-// to be multiplied by.
+// Codes as they stand in a word, plus 128, as fp16 pairs of 2^-24 times that: a byte in the
+// low bits of fp16 is a subnormal number, which the tensor cores multiply exactly.
+// (3 instructions a word instead of 5; the sum of 128 q is taken off beforehand.)
+__device__ __forceinline__ uint2 codes_plus_128(uint32_t w) {
+  const uint32_t u = w ^ 0x80808080u;
+  return make_uint2(__byte_perm(u, 0, 0x4140), __byte_perm(u, 0, 0x4342));
+}
+
+// Two 8 x 8 matrices' worth of 16-bit values turned around: lane (g, t) has row g, columns
+// 2 t and 2 t + 1 of the transposed one.
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
+}
+
+// `count` rows of queries (a multiple of 8) in shared memory in the order in which lanes
+// read mma operands: [8 rows][half][DP / 16][lane] of 8 bytes.  Called by `warps` warps,
+// each for some rows; lane = 4 channels.  A k step of 16 stands for channels
+// p * 64 + t * 16 + w * 4 + 0..3 of lane t (of 4), step p * 4 + w, as the codes are read:
+// 16 bytes a lane.  row(r) is the row's first channel or null; factor[r] becomes what its
+// products have to be multiplied by, start[r] what their sums start from where codes come
+// as codes_plus_128.
 template <typename T, int DP, int HALVES, typename Row>
-__device__ __forceinline__ void stage_queries(uint4* frag, float* factor, int dim, int warp,
-                                              int warps, Row row) {
+__device__ __forceinline__ void stage_queries(uint2* frag, float* factor, float* start, int dim,
+                                              int count, int warp, int warps, Row row) {
   const int lane = threadIdx.x & 31;
-  for (int r = warp; r < 16; r += warps) {
+  for (int r = warp; r < count; r += warps) {
     const T* from = row(r);
     constexpr int kParts = (DP + 127) / 128;
     float4 v[kParts];
@@ -130,25 +147,87 @@ __device__ __forceinline__ void stage_queries(uint4* frag, float* factor, int di
       up = power_of_two(e);
       down = power_of_two(-e);
     }
-    if (lane == 0) factor[r] = down;
+    float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < kParts; ++i) {
       const int c = i * 128 + lane * 4;
       if (c >= DP) continue;
       const float f[4] = {v[i].x * up, v[i].y * up, v[i].z * up, v[i].w * up};
       const __half2 h0 = __floats2half2_rn(f[0], f[1]), h1 = __floats2half2_rn(f[2], f[3]);
-      uint32_t* to = reinterpret_cast<uint32_t*>(
-                         &frag[(c / 64 * 4 + c % 16 / 4) * 32 + (r & 7) * 4 + c % 64 / 16]) +
-                     (r >> 3);
-      to[0] = word_of(h0);
-      to[2] = word_of(h1);
+      uint2* to = &frag[(r >> 3) * (HALVES * DP / 16 * 32) + (c / 64 * 4 + c % 16 / 4) * 32 +
+                        (r & 7) * 4 + c % 64 / 16];
+      *to = make_uint2(word_of(h0), word_of(h1));
+      const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
+      sum += (b0.x + b0.y) + (b1.x + b1.y);
       if constexpr (HALVES == 2) {
-        const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
-        to += DP / 16 * 32 * 4;
-        to[0] = word_of(__floats2half2_rn(f[0] - b0.x, f[1] - b0.y));
-        to[2] = word_of(__floats2half2_rn(f[2] - b1.x, f[3] - b1.y));
+        const __half2 l0 = __floats2half2_rn(f[0] - b0.x, f[1] - b0.y);
+        const __half2 l1 = __floats2half2_rn(f[2] - b1.x, f[3] - b1.y);
+        to[DP / 16 * 32] = make_uint2(word_of(l0), word_of(l1));
+        const float2 c0 = __half22float2(l0), c1 = __half22float2(l1);
+        sum += (c0.x + c0.y) + (c1.x + c1.y);
       }
     }
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    if (lane == 0) {
+      factor[r] = down;
+      start[r] = sum * -7.62939453125e-6f;  // 128 / 2^24
+    }
+  }
+}
+
+// One row of queries in the four lanes t of a lane group g, as operands of 8 columns:
+// channels p * 64 + t * 16 + w * 4 + 0..3 for step p * 4 + w.  `from` is row g's first
+// channel or null.  factor and start, as above, are those of rows 2 t and 2 t + 1.
+template <typename T, int DP, int HALVES>
+__device__ __forceinline__ void load_queries(const T* from, int dim, uint2 (&frag)[HALVES][DP / 16],
+                                             float (&factor)[2], float (&start)[2]) {
+  const int lane = threadIdx.x & 31, t = lane & 3;
+  float4 v[DP / 16];
+  float big = 0.0f;
+#pragma unroll
+  for (int p = 0; p < DP / 64; ++p) {
+    const int c = p * 64 + t * 16;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      float4& x = v[p * 4 + w];
+      x = from != nullptr && c < dim ? load4(from + c + w * 4) : make_float4(0, 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < DP / 16; ++k)
+    big = fmaxf(big, fmaxf(fmaxf(fabsf(v[k].x), fabsf(v[k].y)), fmaxf(fabsf(v[k].z), fabsf(v[k].w))));
+  float up = 1.0f, down = 1.0f;
+  if constexpr (!std::is_same<T, __half>::value) {
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    const int e = row_exponent(big);
+    up = power_of_two(e);
+    down = power_of_two(-e);
+  }
+  float sum = 0.0f;
+#pragma unroll
+  for (int k = 0; k < DP / 16; ++k) {
+    const float f[4] = {v[k].x * up, v[k].y * up, v[k].z * up, v[k].w * up};
+    const __half2 h0 = __floats2half2_rn(f[0], f[1]), h1 = __floats2half2_rn(f[2], f[3]);
+    frag[0][k] = make_uint2(word_of(h0), word_of(h1));
+    const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
+    sum += (b0.x + b0.y) + (b1.x + b1.y);
+    if constexpr (HALVES == 2) {
+      const __half2 l0 = __floats2half2_rn(f[0] - b0.x, f[1] - b0.y);
+      const __half2 l1 = __floats2half2_rn(f[2] - b1.x, f[3] - b1.y);
+      frag[HALVES - 1][k] = make_uint2(word_of(l0), word_of(l1));
+      const float2 c0 = __half22float2(l0), c1 = __half22float2(l1);
+      sum += (c0.x + c0.y) + (c1.x + c1.y);
+    }
+  }
+  sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+  sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+  sum *= -7.62939453125e-6f;  // 128 / 2^24
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    factor[e] = __shfl_sync(0xffffffffu, down, 8 * t + 4 * e);
+    start[e] = __shfl_sync(0xffffffffu, sum, 8 * t + 4 * e);
   }
 }
 
@@ -167,21 +246,23 @@ __device__ __forceinline__ int piece_at(int key, int piece) {
 // The plan of a call over packed new tokens and their sequences' pages
 // ---------------------------------------------------------------------------
 
+constexpr float kCodeUnit = 16777216.0f;  // 2^24: what codes_plus_128 divides by
+
+// A sequence's work: its query rows of a KV head in blocks of `rows`, a unit each, times
+// its keys in steps of `step`, one at least, behind `over` places that stand for what a
+// unit costs however short.  Units follow each other sequence by sequence, and in a
+// sequence block by block, the KV heads of a block next to one another.  Sequences of
+// less than `from` or more than `to` rows of a KV head are left to another kernel.
 struct PlanSeq {
-  int q0, lq;   // the sequence's rows in the packed queries
-  int len;      // its cached tokens, the new ones among them
-  int splits;   // parts of its keys
-  int first;    // first item
-  int slot;     // first partial result (sequences of more than one part)
-  int unit;     // first counter of the same
-  int pad;
+  int64_t first;  // places in front of the sequence's
+  int q0, lq;     // its rows in the packed queries
+  int len;        // its cached tokens, the new ones among them
+  int steps;      // of a unit
 };
 
 struct PlanHead {
-  int items;         // in all
-  int split_keys;    // keys of a part
+  int64_t places;      // in all
   int q_begin, q_end;  // rows of all sequences
-  int pad[4];
 };
 
 struct PlanArgs {
@@ -189,31 +270,26 @@ struct PlanArgs {
   const int32_t* lens;
   int seqs, total_q;
   int group, kv_heads, block_size, width;
-  int rows;           // rows of an item
-  int target;         // items to aim at where sequences are split; 0: parts of `least` keys
-  int least;          // keys of the smallest part, a multiple of `round`
-  int round;
+  int rows, step, over;
+  int64_t from, to;
   PlanHead* head;
-  PlanSeq* seq;       // [seqs]
-  int* counters;      // [counts], zeroed
+  PlanSeq* seq;   // [seqs]
+  int* counters;  // [counts], zeroed
   int counts;
 };
 
-// Splits sequences into parts so that about `target` items have equal work.  Sequences
-// of more than one part have fewer than 2 target items.
 int launch_plan(const PlanArgs& a, int* err, cudaStream_t stream);
 
-// The sequence of an item; one warp, a search of 32 at a time.
-__device__ __forceinline__ int plan_find(const PlanSeq* seq, int seqs, int item) {
+// The sequence of a place; one warp, a search of 32 at a time.
+__device__ __forceinline__ int plan_find(const PlanSeq* seq, int seqs, int64_t place) {
   const int lane = threadIdx.x & 31;
-  int lo = 0, n = seqs;  // the last sequence of [lo, lo + n) whose first item is <= item
+  int lo = 0, n = seqs;  // the last sequence of [lo, lo + n) whose first place is <= this
   while (n > 1) {
-    const int step = (n + 31) / 32;
-    const int at = lo + lane * step;
-    const bool below = lane * step < n && seq[at].first <= item;
+    const int stride = (n + 31) / 32;
+    const bool below = lane * stride < n && seq[lo + lane * stride].first <= place;
     const int last = 31 - __clz(__ballot_sync(0xffffffffu, below));
-    lo += last * step;
-    n = min(step, n - last * step);
+    lo += last * stride;
+    n = min(stride, n - last * stride);
   }
   return lo;
 }

@@ -7,9 +7,11 @@
 // in fp16; the products run on the tensor cores with fp32 sums, the K scales on the
 // scores and the V scales on the probabilities.
 //
-//   plan_kernel   one CTA: the sequences' rows and lengths, checked; how many parts
-//                 each one's keys are split into; the items' numbers;
-//   rows_kernel   an item is (sequence, 16 query rows of a KV head, part of the keys).
+//   plan_kernel   one CTA: the sequences' rows and lengths, checked, and where in all of
+//                 the work each sequence's begins;
+//   rows_kernel   a unit is 8 query rows of a KV head and its sequence's keys; each
+//                 warp takes an equal share of the units' steps of 16 keys;
+//   join_kernel   units that more than 8 warps share.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -22,139 +24,151 @@
 namespace pkv {
 namespace {
 
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 256;
+constexpr int kPlanWarps = kPlanThreads / 32;
 
-// Inclusive sum (or maximum) over the CTA; `carry` of the warps by shared memory.
-template <typename V, typename Op>
-__device__ __forceinline__ V scan_cta(V v, V* shared, Op op) {
+// Inclusive scans over the CTA's threads; `all` is the result over all of them.
+__device__ __forceinline__ int scan_max(int v, int* shared, int* all) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const V x = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v = op(v, x);
+    const int x = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v = max(v, x);
   }
-  __syncthreads();
   if (lane == 31) shared[warp] = v;
   __syncthreads();
-  if (warp > 0) {
-    V before = shared[0];
-    for (int w = 1; w < warp; ++w) before = op(before, shared[w]);
-    v = op(v, before);
+  int front = 0, most = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanWarps; ++w) {
+    if (w < warp) front = max(front, shared[w]);
+    most = max(most, shared[w]);
   }
+  *all = most;
+  return max(v, front);
+}
+__device__ __forceinline__ int64_t scan_sum(int64_t v, int64_t* shared, int64_t* all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t x = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += x;
+  }
+  if (lane == 31) shared[warp] = v;
+  __syncthreads();
+  int64_t sum = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanWarps; ++w) {
+    if (w == warp) v += sum;
+    sum += shared[w];
+  }
+  *all = sum;
   return v;
 }
 
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs p, int* err) {
-  __shared__ int64_t s_scan[kPlanThreads / 32];
-  __shared__ int64_t s_carry[4];
+  __shared__ int s_max[kPlanWarps];
+  __shared__ int64_t s_sum[kPlanWarps];
+  __shared__ int s_end[kPlanThreads];
   const int tid = threadIdx.x;
   for (int i = tid; i < p.counts; i += kPlanThreads) p.counters[i] = 0;
-  const auto most = [](int64_t a, int64_t b) { return a > b ? a : b; };
-  const auto sum = [](int64_t a, int64_t b) { return a + b; };
-  // rows and lengths; an entry of cu below an earlier one counts as the largest
-  // before it
-  int64_t end = min(max(p.cu[0], 0), p.total_q), work = 0;
-  const int q_begin = (int)end;
-  bool bad = tid == 0 && (p.cu[0] < 0 || p.cu[0] > p.total_q), longer = false;
+  const int64_t room = (int64_t)p.width * p.block_size;
+  // an entry of cu below an earlier one counts as the largest before it
+  const int first = p.cu[0];
+  int end = min(max(first, 0), p.total_q);
+  const int q_begin = end;
+  bool bad = first < 0 || first > p.total_q, longer = false;
+  int64_t base = 0;
   for (int s0 = 0; s0 < p.seqs; s0 += kPlanThreads) {
     const int s = s0 + tid;
-    int64_t q1 = 0;
-    int len = 0;
+    int q1 = 0, len = 0;
     if (s < p.seqs) {
-      const int c = p.cu[s + 1];
+      const int c = p.cu[s + 1], given = p.lens[s];
       q1 = min(max(c, 0), p.total_q);
       bad |= c < p.cu[s] || c > p.total_q;
-      const int64_t room = (int64_t)p.width * p.block_size;
-      len = max(p.lens[s], 0);
-      longer |= len > room;
-      len = (int)min((int64_t)len, room);
+      longer |= given > room;
+      len = (int)min((int64_t)max(given, 0), room);
     }
-    const int64_t incl = most(scan_cta(q1, s_scan, most), end);
+    int most;
+    const int incl = max(scan_max(q1, s_max, &most), end);
+    s_end[tid] = incl;
     __syncthreads();
-    if (tid < kPlanThreads && (tid & 31) == 31) s_scan[tid >> 5] = incl;
-    int64_t before = __shfl_up_sync(0xffffffffu, incl, 1);
-    __syncthreads();
-    if ((tid & 31) == 0) before = tid > 0 ? s_scan[(tid >> 5) - 1] : end;
+    const int before = tid > 0 ? s_end[tid - 1] : end;
+    const int lq = incl - before;
+    const int steps = max((len + p.step - 1) / p.step, 1);
+    const int64_t rows = lq * (int64_t)p.group;
+    const bool ours = s < p.seqs && rows >= p.from && rows <= p.to;
+    const int64_t mine =
+        ours ? (rows + p.rows - 1) / p.rows * p.kv_heads * (steps + p.over) : 0;
+    int64_t all;
+    const int64_t at = scan_sum(mine, s_sum, &all);
     if (s < p.seqs) {
       PlanSeq q;
-      q.q0 = (int)before;
-      q.lq = (int)(incl - before);
+      q.first = base + at - mine;
+      q.q0 = before;
+      q.lq = lq;
       q.len = len;
+      q.steps = steps;
       p.seq[s] = q;
-      work += (int64_t)((q.lq * (int64_t)p.group + p.rows - 1) / p.rows) * p.kv_heads * len;
     }
-    end = s_scan[kPlanThreads / 32 - 1];
+    base += all;
+    end = max(end, most);
+    __syncthreads();
   }
   if (bad) record_error(err, kDevBadSeqlens);
   if (longer) record_error(err, kDevSeqTooLong);
-  const int64_t mine = scan_cta(work, s_scan, sum);
-  if (tid == kPlanThreads - 1) s_carry[0] = mine;
-  __syncthreads();
-  int64_t part = p.target > 0 ? (s_carry[0] + p.target - 1) / p.target : 0;
-  part = (most(part, p.least) + p.round - 1) / p.round * p.round;
-  const int split = (int)(part < (1 << 30) ? part : 1 << 30);
-  int64_t items = 0, slots = 0, units = 0;
-  for (int s0 = 0; s0 < p.seqs; s0 += kPlanThreads) {
-    const int s = s0 + tid;
-    int n = 0, u = 0, parts = 1;
-    if (s < p.seqs) {
-      const PlanSeq q = p.seq[s];
-      u = (int)((q.lq * (int64_t)p.group + p.rows - 1) / p.rows) * p.kv_heads;
-      if (q.len > split) parts = (q.len - 1) / split + 1;
-      n = u * parts;
-    }
-    const int64_t a = scan_cta((int64_t)n, s_scan, sum);
-    const int64_t b = scan_cta((int64_t)(parts > 1 ? n : 0), s_scan, sum);
-    const int64_t c = scan_cta((int64_t)(parts > 1 ? u : 0), s_scan, sum);
-    if (s < p.seqs) {
-      PlanSeq* q = &p.seq[s];
-      q->splits = parts;
-      q->first = (int)(items + a - n);
-      q->slot = (int)(slots + b - (parts > 1 ? n : 0));
-      q->unit = (int)(units + c - (parts > 1 ? u : 0));
-    }
-    __syncthreads();
-    if (tid == kPlanThreads - 1) s_carry[1] = a, s_carry[2] = b, s_carry[3] = c;
-    __syncthreads();
-    items += s_carry[1], slots += s_carry[2], units += s_carry[3];
-  }
   if (tid == 0) {
-    p.head->items = (int)items;
-    p.head->split_keys = split;
-    p.head->q_begin = q_begin;
-    p.head->q_end = (int)end;
+    PlanHead h;
+    h.places = base;
+    h.q_begin = q_begin;
+    h.q_end = end;
+    *p.head = h;
   }
 }
 
 // ---------------------------------------------------------------------------
-// 16 rows of a KV head over a part of the keys, by mma.sync
+// 8 rows of a KV head over a part of the keys, by mma.sync
 // ---------------------------------------------------------------------------
+//
+// Keys are the products' M and rows their N: one decoded token's 4 or 8 heads fill an
+// n8 tile, where they would leave most of an m16 tile empty, and a lane's accumulators
+// for 128 channels of V are 32 instead of 64.  S comes with a lane's keys in rows of
+// the fragment; movmatrix turns the probabilities for the second product.
+//
+// Warps work alone, each with a ring of stages of 16 keys that cp.async fills two steps
+// ahead: each has the same share of all units' steps, so that they end together, and
+// while one of them waits for the first pages of its next unit the others go on.  (CTAs
+// of 8 warps on one unit met at its start and end and took 94 us for 64 sequences of
+// 2,050 tokens, 75 us with equal shares.)
 
-constexpr int kStep = 16;      // keys of a warp's step
-constexpr int kRowWarps = 8;
-constexpr int kRowThreads = kRowWarps * 32;
-constexpr int kRows = 16;
+constexpr int kStep = 16;      // keys of a step
+constexpr int kRows = 8;
+constexpr int kRowWarps = 8;   // of a CTA
+constexpr int kStages = 3;
+constexpr int kOver = 6;       // steps that a unit's start and end cost
+constexpr int kLeast = 16;     // places of a warp's share
+constexpr int kJoinHere = 8;   // parts that the last of them joins; more are left to join_kernel
 // A row's maximum moves when a step exceeds it by more than 2^kLazy, and p is kept times
 // 2^kPShift, at most 2^15 in fp16, times its key's V scale over a power of two above the
 // warp's largest: fp16's smallest step, 2^-24, is then 2^-37 of the row's largest p.
 constexpr float kLazy = 2.0f;
 constexpr float kPShift = 13.0f;
 
-template <int DP, int HALVES, bool PV>
+template <int DP, int HALVES, bool PV, bool WHOLE>
 struct RowsCfg {
-  static constexpr int kStages = 3;
   static constexpr int kCodeBytes = (PV ? 2 : 1) * kStep * DP;  // K, then V
-  static constexpr int kStageBytes = kCodeBytes + 2 * kStep * 4 + 16;  // scales, which keys count
-  static constexpr int kRingBytes = kStages * kStageBytes;             // of a warp
-  static constexpr int kPitch = DP + 4;  // floats of a row of results
-  static constexpr int kOffQ = kRowWarps * kRingBytes;
-  static constexpr int kOffMl = kOffQ + HALVES * DP / 16 * 512;
-  static constexpr int kOffMisc = kOffMl + kRowWarps * kRows * 8;
-  static constexpr int kSmemBytes = kOffMisc + kRows * 4 + 16;
-  static constexpr int kSlotO = PV ? kRows * DP * 4 : 0;
-  static constexpr int kSlotBytes = kSlotO + kRows * 8;
-  static_assert(!PV || kRows * kPitch * 4 <= kRingBytes, "results of a warp take its ring's place");
-  static_assert(kSmemBytes <= 227 * 1024, "shared memory");
+  // and the K and V scales: of the step, or of each key with the mask of those that count
+  static constexpr int kStageBytes = kCodeBytes + (WHOLE ? 16 : 2 * kStep * 4 + 16);
+  static constexpr int kRingBytes = kStages * kStageBytes;  // of a warp
+  static constexpr int kSmemBytes = kRowWarps * kRingBytes;
+  static constexpr int kCtas = PV && DP > 128 ? 1 : 2;  // per SM
+  static_assert(kCtas * (kSmemBytes + 1024) <= 228 * 1024, "shared memory");
+};
+
+// A part of a unit: rows of O, then (m, l) of each.
+template <int DP, bool PV>
+struct Slot {
+  static constexpr int kMl = PV ? kRows * DP * 4 : 0;
+  static constexpr int kBytes = kMl + kRows * 8;
 };
 
 struct RowsParams {
@@ -166,395 +180,593 @@ struct RowsParams {
   const int32_t* tables;
   void* out;
   float* lse;  // nullable
+  float* logits;  // nullable, without PV: [total_q * heads][logit_pitch], in powers of two
+  int64_t logit_pitch;
   const PlanHead* head;
   const PlanSeq* seq;
-  int* counters;
-  uint8_t* slots;
+  int* counters;   // per warp: of the unit that begins in it and goes on behind it
+  uint8_t* slots;  // per warp two: of the unit that it begins with, and that it ends with
   int64_t q_tok, q_head;  // strides, elements
   int64_t num_blocks;
   int seqs, total_q, heads, kv_heads, group, dim, bs, width;
-  float qk_scale;  // sm_scale log2e
+  int warps;       // of the grid
+  float qk_scale;  // sm_scale log2e 2^24
 };
 
-// Without PV only the denominators are taken (p.lse).
-template <typename T, int DP, int HALVES, bool PV>
-__global__ void __launch_bounds__(kRowThreads, PV && DP > 128 ? 1 : 2)
+// A unit as the warps that share it see it.
+struct RowsUnit {
+  PlanSeq seq;
+  int s, unit;      // sequence, and which of its units
+  int64_t at;       // its first place
+  int kvh, block;
+  int rows;
+  int warp0, parts; // the warps that have steps of it
+
+  __device__ __forceinline__ void find(const RowsParams& p, int64_t place, int64_t share) {
+    for (;;) {  // (sequences that are not this kernel's have no places)
+      seq = p.seq[s];
+      const int64_t all = (seq.lq * (int64_t)p.group + kRows - 1) / kRows * p.kv_heads;
+      unit = (int)min((place - seq.first) / (seq.steps + kOver), all);
+      const int64_t next = s + 1 < p.seqs ? p.seq[s + 1].first : p.head->places;
+      if (place < next) break;
+      ++s;
+    }
+    at = seq.first + (int64_t)unit * (seq.steps + kOver);
+    kvh = unit % p.kv_heads;
+    block = unit / p.kv_heads;
+    rows = (int)min((int64_t)kRows, seq.lq * (int64_t)p.group - (int64_t)block * kRows);
+    warp0 = (int)((at + kOver) / share);
+    parts = (int)((at + kOver + seq.steps - 1) / share) - warp0 + 1;
+  }
+  // the keys that row r sees: those below its token's place, counted from the end
+  __device__ __forceinline__ int limit(const RowsParams& p, int r) const {
+    return r < rows ? (int)((block * (int64_t)kRows + r) / p.group) + 1 + seq.len - seq.lq : 0;
+  }
+  // row r as (token, head) of the packed tensors
+  __device__ __forceinline__ int64_t token(const RowsParams& p, int r, int* head) const {
+    const int64_t i = block * (int64_t)kRows + r;
+    const int tok = (int)(i / p.group);
+    *head = kvh * p.group + (int)(i - (int64_t)tok * p.group);
+    return seq.q0 + tok;
+  }
+  template <int BYTES>
+  __device__ __forceinline__ uint8_t* slot(const RowsParams& p, int part) const {
+    return p.slots + (int64_t)(2 * (warp0 + part) + (part == 0 ? 1 : 0)) * BYTES;
+  }
+};
+
+__device__ __forceinline__ int64_t rows_share(const RowsParams& p) {
+  return max((p.head->places + p.warps - 1) / p.warps, (int64_t)kLeast);
+}
+
+__device__ __forceinline__ float row_scale(float l) { return l > 0.0f || l != l ? 1.0f / l : 0.0f; }
+__device__ __forceinline__ float row_lse(float m, float l) {
+  return l == 0.0f ? -INFINITY : (m + log2f(l)) * (1.0f / kLog2e);
+}
+
+// Without PV only the denominators are taken (p.lse).  WHOLE: pages of a multiple of 16
+// tokens, so that a step's keys share their scales and are one run of memory.
+template <typename T, int DP, int HALVES, bool PV, bool WHOLE>
+__global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, HALVES, PV, WHOLE>::kCtas)
     rows_kernel(const RowsParams p, int* err) {
-  using C = RowsCfg<DP, HALVES, PV>;
+  using C = RowsCfg<DP, HALVES, PV, WHOLE>;
+  using S = Slot<DP, PV>;
   constexpr int kPieces = DP / 16;              // 16-byte pieces of a key's codes
   constexpr int kPasses = kPieces * kStep / 32; // copies a lane makes of K or V
-  constexpr int kQuads = PV ? DP / 4 : 1;       // of a row's results
-  constexpr int kTiles = PV ? DP / 8 : 0;       // accumulators of 8 channels
+  constexpr int kAhead = 32 / kPieces;          // keys between them
+  constexpr int kTiles = PV ? DP / 16 : 1;      // accumulators of 16 channels
+  constexpr int kSteps = DP / 16;
+  constexpr int kV = kStep * DP;                // V of a stage
+  constexpr int kRun = DP >= 128 ? 16 : 8;      // consecutive channels of a lane's results
+  constexpr int kRuns = (DP + 127) / 128;
   extern __shared__ __align__(128) uint8_t smem[];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int g = lane >> 2, t = lane & 3;
-  uint8_t* ring = smem + warp * C::kRingBytes;
-  uint4* s_q = reinterpret_cast<uint4*>(smem + C::kOffQ);
-  float2* s_ml = reinterpret_cast<float2*>(smem + C::kOffMl);  // [warp][row]
-  float* s_factor = reinterpret_cast<float*>(smem + C::kOffMisc);
-  int* s_last = reinterpret_cast<int*>(smem + C::kOffMisc + kRows * 4);
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int warp = blockIdx.x * kRowWarps + (threadIdx.x >> 5);  // of the grid
+  uint8_t* ring = smem + (threadIdx.x >> 5) * C::kRingBytes;
 
   // rows in front of the first and behind the last sequence become zero
-  const int64_t front = (int64_t)p.head->q_begin * p.heads;
-  const int64_t behind = (int64_t)p.head->q_end * p.heads;
+  const PlanHead head = *p.head;
+  const int64_t front = (int64_t)head.q_begin * p.heads;
+  const int64_t behind = (int64_t)head.q_end * p.heads;
   const int64_t outside = front + (int64_t)p.total_q * p.heads - behind;
-  for (int64_t i = blockIdx.x * kRowWarps + warp; i < outside; i += gridDim.x * kRowWarps) {
+  for (int64_t i = warp; i < outside; i += p.warps) {
     const int64_t r = i < front ? i : behind + i - front;
     for (int c = lane * 4; PV && c < p.dim; c += 128)
       store4(static_cast<T*>(p.out) + r * p.dim + c, make_float4(0, 0, 0, 0));
     if (lane == 0 && p.lse != nullptr) p.lse[r] = -INFINITY;
   }
 
-  const int items = p.head->items, split_keys = p.head->split_keys;
-  for (int item = blockIdx.x; item < items; item += gridDim.x) {
-    const int s = plan_find(p.seq, p.seqs, item);
-    const PlanSeq seq = p.seq[s];
-    // KV heads next to one another share pages; then row blocks, then parts
-    const int local = item - seq.first;
-    const int kvh = local % p.kv_heads;
-    const int blocks = (int)((seq.lq * (int64_t)p.group + kRows - 1) / kRows);
-    const int unit = local % (p.kv_heads * blocks);
-    const int block = unit / p.kv_heads, part = local / (p.kv_heads * blocks);
-    const int rows = (int)min((int64_t)kRows, seq.lq * (int64_t)p.group - (int64_t)block * kRows);
-    // keys that row r sees: those below its token's place, counted from the end
-    const auto limit_of = [&](int r) {
-      return r < rows ? (int)((block * (int64_t)kRows + r) / p.group) + 1 + seq.len - seq.lq : 0;
-    };
-    const int k0 = part * split_keys;
-    const int k1 = min(min(seq.len, k0 + split_keys), limit_of(rows - 1));
-    const int steps = k1 > k0 ? (k1 - k0 + kStep - 1) / kStep : 0;
-    const int32_t* table = p.tables + (int64_t)s * p.width;
+  // what a lane copies and reads of a stage
+  const int64_t token_bytes = (int64_t)p.kv_heads * p.dim;
+  const int piece = lane % kPieces, key_in = lane / kPieces;
+  const bool on = piece * 16 < p.dim;
+  const uint32_t copy_at = key_in * DP + piece_at<DP>(key_in, piece) * 16;
+  const uint32_t k_at = g * DP + piece_at<DP>(g, t) * 16;
+  const uint32_t v_at = DP >= 128 ? 2 * t * DP + piece_at<DP>(2 * t, g) * 16
+                                  : 2 * t * DP + piece_at<DP>(2 * t, g >> 1) * 16 + (g & 1) * 8;
+  constexpr uint32_t kOdd = DP >= 128 ? 64 : 0;  // of an odd key, in piece_at
 
-    // Step i of this warp is keys k0 + (i kRowWarps + warp) kStep and on.  Lanes 0-15 find
-    // its keys' rows, a step ahead; entry and rem are those of the next step to copy.
-    const int mine = steps > warp ? (steps - warp - 1) / kRowWarps + 1 : 0;
-    const auto key_of = [&](int i) { return k0 + (i * kRowWarps + warp) * kStep; };
-    int entry = -1, rem = 0;
-    const auto look_up = [&](int i) {
-      const int key = key_of(i) + (lane & 15);
-      const int page = key / p.bs;
-      rem = key - page * p.bs;
-      entry = key < k1 ? table[page] : -1;
-    };
-    const auto issue = [&](int i) {
-      if (i < mine) {
-        uint8_t* stage = ring + (i % C::kStages) * C::kStageBytes;
-        const bool counts = key_of(i) + (lane & 15) < k1;
-        const bool good = counts && entry >= 0 && (int64_t)entry < p.num_blocks;
-        if (counts && !good) record_error(err, kDevBadBlockId);
-        const uint32_t at = good ? (uint32_t)entry * p.bs + rem : 0xffffffffu;
-        const float* scale = lane < 16 ? p.k_scale : p.v_scale;
-        if (PV || lane < 16) copy4_if(good, smem_u32(stage + C::kCodeBytes + lane * 4),
-                 scale + (good ? (int64_t)entry * p.kv_heads + kvh : 0));
-        const unsigned mask = __ballot_sync(0xffffffffu, good);
-        if (lane == 0) *reinterpret_cast<uint32_t*>(stage + C::kCodeBytes + 128) = mask & 0xffffu;
+  const int64_t share = rows_share(p);
+  int64_t now = warp * share;
+  const int64_t stop = min(now + share, head.places);
+  RowsUnit u;
+  if (now < stop) u.s = plan_find(p.seq, p.seqs, now);
+  for (; now < stop; now = u.at + u.seq.steps + kOver) {
+    u.find(p, now, share);
+    const int first_step = (int)max(now - u.at - kOver, (int64_t)0);
+    const int end_step = (int)min((int64_t)u.seq.steps, stop - u.at - kOver);
+    if (end_step <= first_step) continue;  // none of its steps
+    const int kvh = u.kvh, rows = u.rows;
+    const int k0 = first_step * kStep;
+    const int k1 = min(min(u.seq.len, end_step * kStep), u.limit(p, rows - 1));
+    const int32_t* table = p.tables + (int64_t)u.s * p.width;
+
+    // Keys' pages are looked up a step ahead: entry and rem are those of the next step
+    // to copy, of its first key (WHOLE) or of key lane % 16.
+    const int step_pages = kStep / p.bs, step_rem = kStep - step_pages * p.bs;
+    int key = k0 + (WHOLE ? 0 : lane & 15);
+    int page = key / p.bs, rem = key - page * p.bs;
+    int entry = key < k1 ? table[page] : -1;
+    int next_left = k1 - k0;  // keys from the next step to copy on
+    int copied = 0;           // its stage
+    uint32_t gone = 0;        // WHOLE: stages whose page is outside the cache
+    const int64_t col = kvh * p.dim + (on ? piece * 16 : 0);
+    const int8_t* k_col = p.k_cache + col;
+    const int8_t* v_col = PV ? p.v_cache + col : nullptr;
+    const auto issue = [&]() {
+      if (next_left > 0) {
+        uint8_t* stage = ring + copied * C::kStageBytes;
+        const uint32_t to = smem_u32(stage);
+        if constexpr (WHOLE) {
+          const bool good = entry >= 0 && (int64_t)entry < p.num_blocks;
+          gone = good ? gone & ~(1u << copied) : gone | 1u << copied;
+          if (!good) record_error(err, kDevBadBlockId);
+          if (good) {
+            if (lane < (PV ? 2 : 1))
+              copy4_if(true, to + C::kCodeBytes + lane * 4,
+                       (lane == 0 ? p.k_scale : p.v_scale) + (int64_t)entry * p.kv_heads + kvh);
+            const int64_t from = ((int64_t)entry * p.bs + rem + key_in) * token_bytes;
+            const int8_t* kp = k_col + from;
+            const int8_t* vp = v_col + from;
 #pragma unroll
-        for (int c = 0; c < kPasses; ++c) {
-          const int key = (c * 32 + lane) / kPieces, piece = lane % kPieces;
-          const uint32_t row = __shfl_sync(0xffffffffu, at, key);
-          const bool on = row != 0xffffffffu && piece * 16 < p.dim;
-          const int64_t from =
-              on ? ((int64_t)row * p.kv_heads + kvh) * p.dim + piece * 16 : 0;
-          const uint32_t to = smem_u32(stage + key * DP + piece_at<DP>(key, piece) * 16);
-          copy16_if(on, to, p.k_cache + from);
-          if constexpr (PV) copy16_if(on, to + kStep * DP, p.v_cache + from);
+            for (int c = 0; c < kPasses; ++c) {
+              // (the swizzle of key c kAhead + key_in from that of key_in)
+              const uint32_t at =
+                  (copy_at ^ (DP == 128 ? (c & 1) * 64 : DP == 256 ? (c & 3) * 32 : 0)) + c * kAhead * DP;
+              copy16_if(true, to + at, kp);
+              if constexpr (PV) copy16_if(true, to + at + kV, vp);
+              kp += kAhead * token_bytes;
+              if constexpr (PV) vp += kAhead * token_bytes;
+            }
+          }
+        } else {
+          const bool counts = (lane & 15) < next_left;
+          const bool good = counts && entry >= 0 && (int64_t)entry < p.num_blocks;
+          if (counts && !good) record_error(err, kDevBadBlockId);
+          if (PV || lane < 16)
+            copy4_if(good, to + C::kCodeBytes + lane * 4,
+                     (lane < 16 ? p.k_scale : p.v_scale) +
+                         (good ? (int64_t)entry * p.kv_heads + kvh : 0));
+          const unsigned mask = __ballot_sync(0xffffffffu, good) & 0xffffu;
+          if (lane == 0) *reinterpret_cast<uint32_t*>(stage + C::kCodeBytes + 128) = mask;
+          const uint32_t at = good ? (uint32_t)entry * p.bs + rem : 0xffffffffu;
+#pragma unroll 1
+          for (int c = 0; c < kPasses; ++c) {
+            const int k = c * kAhead + key_in;
+            const uint32_t row = __shfl_sync(0xffffffffu, at, k);
+            const bool there = row != 0xffffffffu && on;
+            const int64_t from = there ? row * token_bytes : 0;
+            const uint32_t dst = to + k * DP + piece_at<DP>(k, piece) * 16;
+            copy16_if(there, dst, k_col + from);
+            if constexpr (PV) copy16_if(there, dst + kV, v_col + from);
+          }
         }
-        if (i + 1 < mine) look_up(i + 1);
+        copied = copied + 1 == kStages ? 0 : copied + 1;
+        next_left -= kStep;
+        key += kStep;
+        page += step_pages;
+        rem += step_rem;
+        if (rem >= p.bs) {
+          rem -= p.bs;
+          ++page;
+        }
+        entry = key < k1 ? table[page] : -1;
       }
       copies_commit();
     };
-    if (mine > 0) look_up(0);
 #pragma unroll
-    for (int i = 0; i < C::kStages - 1; ++i) issue(i);
+    for (int i = 0; i < kStages - 1; ++i) issue();
 
-    stage_queries<T, DP, HALVES>(s_q, s_factor, p.dim, warp, kRowWarps, [&](int r) -> const T* {
-      if (r >= rows) return nullptr;
-      const int64_t i = block * (int64_t)kRows + r;
-      const int tok = (int)(i / p.group);
-      return static_cast<const T*>(p.q) + (seq.q0 + tok) * p.q_tok +
-             (kvh * p.group + (int)(i - (int64_t)tok * p.group)) * p.q_head;
-    });
-    __syncthreads();
-    const float f0 = s_factor[g] * p.qk_scale, f1 = s_factor[g + 8] * p.qk_scale;
-    const int limit0 = limit_of(g), limit1 = limit_of(g + 8);
-    const int clear = limit_of(0);  // every row sees the keys below
+    // a lane's rows are 2 t and 2 t + 1
+    uint2 qr[HALVES][kSteps];
+    float f[2], start[2];
+    {
+      int h;
+      const int64_t tok = u.token(p, g, &h);
+      load_queries<T, DP, HALVES>(
+          g < rows ? static_cast<const T*>(p.q) + tok * p.q_tok + h * p.q_head : nullptr, p.dim, qr,
+          f, start);
+      f[0] *= p.qk_scale;
+      f[1] *= p.qk_scale;
+    }
+    const int limit0 = u.limit(p, 2 * t), limit1 = u.limit(p, 2 * t + 1);
+    const int clear = min(u.limit(p, 0), k1);  // every row sees the keys below
+    float* logit[2] = {nullptr, nullptr};
+    if constexpr (!PV) {
+      if (p.logits != nullptr)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          int h;
+          const int64_t tok = u.token(p, 2 * t + r, &h);
+          if (2 * t + r < rows) logit[r] = p.logits + (tok * p.heads + h) * p.logit_pitch + g;
+        }
+    }
 
-    float o[PV ? kTiles : 1][4];
+    // p is 2^(score - base); base moves where a score is above most
+    float o[kTiles][4];
 #pragma unroll
     for (int i = 0; i < kTiles; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
-    int unit_e = -127;  // O is in units of 2^unit_e (of V scales) / 2^kPShift
+    float base[2] = {0.0f, 0.0f}, most[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    // O is in units of `unit_v`, a power of two above the V scales so far, so that p
+    // times scale stays in fp16
+    float unit_v = 0.0f, inv_v = 0.0f;
 
-    for (int i = 0; i < mine; ++i) {
-      copies_wait<C::kStages - 2>();
+    int used = 0;  // the stage
+    for (int key_now = k0; key_now < k1; key_now += kStep) {
+      copies_wait<kStages - 2>();
       __syncwarp();
-      issue(i + C::kStages - 1);
-      const uint8_t* stage = ring + (i % C::kStages) * C::kStageBytes;
+      issue();
+      const uint8_t* stage = ring + used * C::kStageBytes;
       const float* scales = reinterpret_cast<const float*>(stage + C::kCodeBytes);
-      const uint32_t mask = *reinterpret_cast<const uint32_t*>(stage + C::kCodeBytes + 128);
-      // scores: rows g, g + 8; keys 8 n + 2 t, 8 n + 2 t + 1
-      float sc[2][HALVES][4] = {};
+      const bool lost = WHOLE && (gone >> used & 1u);
+      used = used + 1 == kStages ? 0 : used + 1;
+      if (lost) continue;
+      // scores: keys g and g + 8, rows as above: (g, first), (g, second), (g + 8, ...);
+      // two sums, since a product waits 25 clocks for the one before it
+      float sc[4] = {start[0], start[1], start[0], start[1]}, sd[4] = {};
 #pragma unroll
       for (int pc = 0; pc < DP / 64; ++pc) {
-        uint4 w[2];
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-          w[n] = *reinterpret_cast<const uint4*>(stage + (n * 8 + g) * DP +
-                                                 piece_at<DP>(n * 8 + g, pc * 4 + t) * 16);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint2 b[2];
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-            b[n] = codes_to_half(e == 0 ? w[n].x : e == 1 ? w[n].y : e == 2 ? w[n].z : w[n].w);
-#pragma unroll
-          for (int h = 0; h < HALVES; ++h) {
-            const uint4 a = s_q[(h * (DP / 16) + pc * 4 + e) * 32 + lane];
-#pragma unroll
-            for (int n = 0; n < 2; ++n) mma_f16(sc[n][h], a, b[n].x, b[n].y);
-          }
-        }
-      }
-      float y[2][4];
-      float vs[2][2];
-      const int key0 = key_of(i) + 2 * t;
-      const bool all = mask == 0xffffu && key_of(i) + kStep <= clear;
-      uint32_t vmax = 0u;
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const float2 ks = *reinterpret_cast<const float2*>(scales + n * 8 + 2 * t);
-        float2 v = make_float2(0.0f, 0.0f);
-        if constexpr (PV) v = *reinterpret_cast<const float2*>(scales + kStep + n * 8 + 2 * t);
-        vs[n][0] = v.x;
-        vs[n][1] = v.y;
+        // (piece pc * 4 + t: bit 2 turned by odd pc)
+        const uint32_t at = (k_at ^ ((pc & 1) * 64)) + pc / 2 * 128;
+        const uint4 w0 = *reinterpret_cast<const uint4*>(stage + at);
+        const uint4 w1 = *reinterpret_cast<const uint4*>(stage + at + 8 * DP);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float x = sc[n][0][e];
-          if constexpr (HALVES == 2) x += sc[n][1][e];
-          y[n][e] = x * ((e & 1) ? ks.y : ks.x) * (e < 2 ? f0 : f1);
+          const uint2 x = codes_plus_128(e == 0 ? w0.x : e == 1 ? w0.y : e == 2 ? w0.z : w0.w);
+          const uint2 y = codes_plus_128(e == 0 ? w1.x : e == 1 ? w1.y : e == 2 ? w1.z : w1.w);
+          const uint4 a = make_uint4(x.x, y.x, x.y, y.y);
+          if constexpr (HALVES == 2) mma_f16(sd, a, qr[HALVES - 1][pc * 4 + e].x, qr[HALVES - 1][pc * 4 + e].y);
+          if (HALVES == 1 && (e & 1)) mma_f16(sd, a, qr[0][pc * 4 + e].x, qr[0][pc * 4 + e].y);
+          else mma_f16(sc, a, qr[0][pc * 4 + e].x, qr[0][pc * 4 + e].y);
         }
-        const uint32_t a = __float_as_uint(fabsf(v.x)), b = __float_as_uint(fabsf(v.y));
-        vmax = max(vmax, max(a < 0x7f800000u ? a : 0u, b < 0x7f800000u ? b : 0u));
       }
-      const auto seen = [&](int n, int e) {
-        const int key = n * 8 + (e & 1);  // + 2 t
-        return (mask >> (key + 2 * t) & 1u) && key0 + key < (e < 2 ? limit0 : limit1);
+      float ks[2], vs[2] = {0.0f, 0.0f};
+      uint32_t mask = 0xffffu;
+      if constexpr (WHOLE) {
+        const float2 x = *reinterpret_cast<const float2*>(scales);
+        ks[0] = ks[1] = x.x;
+        if constexpr (PV) vs[0] = vs[1] = x.y;
+      } else {
+        ks[0] = scales[g], ks[1] = scales[g + 8];
+        if constexpr (PV) vs[0] = scales[kStep + g], vs[1] = scales[kStep + g + 8];
+        mask = *reinterpret_cast<const uint32_t*>(stage + C::kCodeBytes + 128);
+      }
+      const bool all = (WHOLE || mask == 0xffffu) && key_now + kStep <= clear;
+      const auto seen = [&](int e) {  // e as in sc
+        const int k = g + (e >> 1) * 8;
+        return (WHOLE ? key_now + k < k1 : mask >> k & 1u) &&
+               key_now + k < ((e & 1) ? limit1 : limit0);
       };
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sc[e] = (sc[e] + sd[e]) * (ks[e >> 1] * f[e & 1]);
       if (!all) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (!seen(n, e)) y[n][e] = -INFINITY;
+        for (int e = 0; e < 4; ++e)
+          if (!seen(e)) sc[e] = -INFINITY;
       }
-      if constexpr (PV) vmax = __reduce_max_sync(0xffffffffu, vmax);
-      float t0 = fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[1][0], y[1][1]));
-      float t1 = fmaxf(fmaxf(y[0][2], y[0][3]), fmaxf(y[1][2], y[1][3]));
-#pragma unroll
-      for (int x = 1; x <= 2; x <<= 1) {
-        t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, x));
-        t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, x));
+      bool move = fmaxf(sc[0], sc[2]) > most[0] || fmaxf(sc[1], sc[3]) > most[1];
+      if constexpr (PV) {
+        const float v0 = fabsf(vs[0]), v1 = fabsf(vs[1]);
+        move |= v0 > unit_v && v0 <= 3.0e38f;
+        if constexpr (!WHOLE) move |= v1 > unit_v && v1 <= 3.0e38f;
       }
-      // power of two above the V scales, so that p times scale stays in fp16
-      const int e_now = (int)(vmax >> 23) - 126;
-      const bool grow = vmax != 0u && e_now > unit_e;
-      const bool move0 = t0 > m0 + kLazy || (m0 == -INFINITY && t0 > m0);
-      const bool move1 = t1 > m1 + kLazy || (m1 == -INFINITY && t1 > m1);
-      if (__any_sync(0xffffffffu, move0 || move1) || grow) {
-        const float a0 = move0 ? ex2(m0 - t0) : 1.0f, a1 = move1 ? ex2(m1 - t1) : 1.0f;
-        if (move0) m0 = t0;
-        if (move1) m1 = t1;
-        l0 *= a0;
-        l1 *= a1;
+      if (__any_sync(0xffffffffu, move)) {
         float down = 1.0f;
-        if (grow) {
-          down = unit_e - e_now < -126 ? 0.0f : power_of_two(unit_e - e_now);
-          unit_e = e_now;
+        if constexpr (PV) {
+          const auto finite = [](float v) {
+            v = fabsf(v);
+            return v <= 3.0e38f ? __float_as_uint(v) : 0u;
+          };
+          const uint32_t big = __reduce_max_sync(0xffffffffu, max(finite(vs[0]), finite(vs[1])));
+          if (__uint_as_float(big) > unit_v) {
+            const float unit_now = power_of_two(min(max((int)(big >> 23) - 126, -126), 126));
+            inv_v = 1.0f / unit_now;
+            down = unit_v * inv_v;
+            unit_v = unit_now;
+          }
         }
-#pragma unroll
-        for (int n = 0; n < kTiles; ++n) {
-          o[n][0] *= a0 * down;
-          o[n][1] *= a0 * down;
-          o[n][2] *= a1 * down;
-          o[n][3] *= a1 * down;
-        }
-      }
-      const float base0 = m0 == -INFINITY ? 0.0f : m0 - kPShift;
-      const float base1 = m1 == -INFINITY ? 0.0f : m1 - kPShift;
-      const float inv_unit = power_of_two(-max(unit_e, -126));
-      uint32_t hi[2][2], lo[2][2] = {};  // [n][rows g, g + 8]
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
+        float a[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float x0 = ex2(y[n][2 * r] - (r ? base1 : base0));
-          const float x1 = ex2(y[n][2 * r + 1] - (r ? base1 : base0));
-          (r ? l1 : l0) += x0 + x1;
-          if constexpr (!PV) continue;
-          float z0 = x0 * (vs[n][0] * inv_unit), z1 = x1 * (vs[n][1] * inv_unit);
-          if (!all) {
-            if (!seen(n, 2 * r)) z0 = 0.0f;
-            if (!seen(n, 2 * r + 1)) z1 = 0.0f;
+          float top = fmaxf(sc[r], sc[r + 2]);
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+          a[r] = 1.0f;
+          if (top > most[r]) {
+            const float to = top - kPShift;
+            a[r] = most[r] == -INFINITY ? 0.0f : ex2(base[r] - to);
+            base[r] = to;
+            most[r] = top + kLazy;
+          }
+          l[r] *= a[r];
+          a[r] *= down;
+        }
+        if constexpr (PV) {
+#pragma unroll
+          for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[c][e] *= a[e & 1];
+        }
+      }
+      if constexpr (!PV) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          if (logit[r] != nullptr) {
+            if (key_now + g < k1) logit[r][key_now] = sc[r];
+            if (key_now + g + 8 < k1) logit[r][key_now + 8] = sc[r + 2];
+          }
+      }
+      uint32_t hi[2], lo[2];  // keys g, g + 8
+      const float v0 = vs[0] * inv_v, v1 = vs[1] * inv_v;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float x0 = ex2(sc[2 * k] - base[0]), x1 = ex2(sc[2 * k + 1] - base[1]);
+        l[0] += x0;
+        l[1] += x1;
+        if constexpr (PV) {
+          float z0 = x0 * (k ? v1 : v0), z1 = x1 * (k ? v1 : v0);
+          if (!all) {  // (a V scale that is not finite does not reach rows in front)
+            if (!seen(2 * k)) z0 = 0.0f;
+            if (!seen(2 * k + 1)) z1 = 0.0f;
           }
           const __half2 h = __floats2half2_rn(z0, z1);
-          hi[n][r] = word_of(h);
+          hi[k] = transpose_8x8(word_of(h));
           if constexpr (HALVES == 2) {
             const float2 b = __half22float2(h);
-            lo[n][r] = word_of(__floats2half2_rn(z0 - b.x, z1 - b.y));
+            lo[k] = transpose_8x8(word_of(__floats2half2_rn(z0 - b.x, z1 - b.y)));
           }
         }
-      if constexpr (!PV) continue;
-      const uint4 pa = make_uint4(hi[0][0], hi[0][1], hi[1][0], hi[1][1]);
-      const uint4 pb = HALVES == 2 ? make_uint4(lo[0][0], lo[0][1], lo[1][0], lo[1][1]) : pa;
-      // O: channel c * 128 + g * 16 + 4 w + e of V is column g of accumulator
-      // c * 16 + 4 w + e (of 64 channels: g * 8 + 4 w + e)
-      const uint8_t* vt = stage + kStep * DP;
-      constexpr int kWords = DP >= 128 ? 4 : 2;
+      }
+      if constexpr (PV) {
+        // O: channels c * 128 + g * 16 + 4 w + e (of 64: g * 8 + 4 w + e) of lane (g, .)
+        // are rows g (even e) and g + 8 (odd e) of accumulator c * 8 + 2 w + e / 2
+        const uint8_t* vt = stage + kV;
+        constexpr int kWords = DP >= 128 ? 4 : 2;
 #pragma unroll
-      for (int c = 0; c < (DP + 127) / 128; ++c) {
-        uint32_t w[4][kWords];  // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+        for (int c = 0; c < kRuns; ++c) {
+          uint32_t w[4][kWords];  // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int key = 2 * t + (k & 1) + (k >> 1) * 8;
-          if constexpr (DP >= 128) {
-            const uint4 x = *reinterpret_cast<const uint4*>(vt + key * DP +
-                                                            piece_at<DP>(key, c * 8 + g) * 16);
-            w[k][0] = x.x, w[k][1] = x.y, w[k][2 % kWords] = x.z, w[k][3 % kWords] = x.w;
-          } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(
-                vt + key * DP + piece_at<DP>(key, g >> 1) * 16 + (g & 1) * 8);
-            w[k][0] = x.x, w[k][1] = x.y;
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t at = ((k & 1) ? (v_at ^ kOdd) + DP : v_at) + (k >> 1) * 8 * DP + c * 128;
+            if constexpr (DP >= 128) {
+              const uint4 x = *reinterpret_cast<const uint4*>(vt + at);
+              w[k][0] = x.x, w[k][1] = x.y, w[k][2 % kWords] = x.z, w[k][3 % kWords] = x.w;
+            } else {
+              const uint2 x = *reinterpret_cast<const uint2*>(vt + at);
+              w[k][0] = x.x, w[k][1] = x.y;
+            }
           }
-        }
 #pragma unroll
-        for (int x = 0; x < kWords; ++x) {
-          const uint2 b01 = codes_to_half(__byte_perm(w[0][x], w[1][x], 0x5140));
-          const uint2 b23 = codes_to_half(__byte_perm(w[0][x], w[1][x], 0x7362));
-          const uint2 c01 = codes_to_half(__byte_perm(w[2][x], w[3][x], 0x5140));
-          const uint2 c23 = codes_to_half(__byte_perm(w[2][x], w[3][x], 0x7362));
-          const int at = c * 16 + x * 4;
-          mma_f16(o[at], pa, b01.x, c01.x);
-          mma_f16(o[at + 1], pa, b01.y, c01.y);
-          mma_f16(o[at + 2], pa, b23.x, c23.x);
-          mma_f16(o[at + 3], pa, b23.y, c23.y);
-          if constexpr (HALVES == 2) {
-            mma_f16(o[at], pb, b01.x, c01.x);
-            mma_f16(o[at + 1], pb, b01.y, c01.y);
-            mma_f16(o[at + 2], pb, b23.x, c23.x);
-            mma_f16(o[at + 3], pb, b23.y, c23.y);
+          for (int x = 0; x < kWords; ++x) {
+            const uint2 b01 = codes_to_half(__byte_perm(w[0][x], w[1][x], 0x5140));
+            const uint2 b23 = codes_to_half(__byte_perm(w[0][x], w[1][x], 0x7362));
+            const uint2 c01 = codes_to_half(__byte_perm(w[2][x], w[3][x], 0x5140));
+            const uint2 c23 = codes_to_half(__byte_perm(w[2][x], w[3][x], 0x7362));
+            const uint4 a0 = make_uint4(b01.x, b01.y, c01.x, c01.y);
+            const uint4 a1 = make_uint4(b23.x, b23.y, c23.x, c23.y);
+            if constexpr (HALVES == 2) {
+              mma_f16(o[c * 8 + 2 * x], a0, lo[0], lo[1]);
+              mma_f16(o[c * 8 + 2 * x + 1], a1, lo[0], lo[1]);
+            }
+            mma_f16(o[c * 8 + 2 * x], a0, hi[0], hi[1]);
+            mma_f16(o[c * 8 + 2 * x + 1], a1, hi[0], hi[1]);
           }
         }
       }
     }
     copies_wait<0>();
     __syncwarp();
-    // The warps' results meet in shared memory, each in its own ring.
 #pragma unroll
-    for (int x = 1; x <= 2; x <<= 1) {
-      l0 += __shfl_xor_sync(0xffffffffu, l0, x);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, x);
-    }
-    if (t == 0) {
-      s_ml[warp * kRows + g] = make_float2(m0, l0);
-      s_ml[warp * kRows + g + 8] = make_float2(m1, l1);
-    }
-    if (PV && mine > 0) {
-      const float up = power_of_two(max(unit_e, -126));
-      float* mine_o = reinterpret_cast<float*>(ring);
-      constexpr int kRun = DP >= 128 ? 16 : 8;  // consecutive channels of a column
+    for (int r = 0; r < 2; ++r)
 #pragma unroll
-      for (int c = 0; c < (DP + 127) / 128; ++c)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float* to = mine_o + (g + (e >> 1) * 8) * C::kPitch + c * 128 + (2 * t + (e & 1)) * kRun;
-#pragma unroll
-          for (int x = 0; x < kRun; x += 4)
-            *reinterpret_cast<float4*>(to + x) =
-                make_float4(o[c * 16 + x][e] * up, o[c * 16 + x + 1][e] * up,
-                            o[c * 16 + x + 2][e] * up, o[c * 16 + x + 3][e] * up);
-        }
-    }
-    __syncthreads();
-    const bool whole = seq.splits == 1;
-    uint8_t* slot = p.slots + (int64_t)(seq.slot + local) * C::kSlotBytes;
-    // O, m, l of row r over the parts given by get(i) -> (m, l), at(i) -> O
-    const auto store_row = [&](int r, int c, float4 acc, float m, float l) {
-      const int64_t i = block * (int64_t)kRows + r;
-      const int tok = (int)(i / p.group);
-      const int64_t to = (int64_t)(seq.q0 + tok) * p.heads + kvh * p.group + (i - (int64_t)tok * p.group);
-      const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-      if (PV && c < p.dim)
-        store4(static_cast<T*>(p.out) + to * p.dim + c,
-               l == 0.0f ? make_float4(0, 0, 0, 0)
-                         : make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
-      if (c == 0 && p.lse != nullptr)
-        p.lse[to] = l == 0.0f ? -INFINITY : (m - kPShift + log2f(l)) * (1.0f / kLog2e);
+      for (int x = 4; x < 32; x <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], x);
+    // channels c * 128 + g * kRun + 4 x on of row 2 t + r
+    const auto result = [&](int r, int c, int x, float by) {
+      const int at = c * 8 + 2 * x;
+      return make_float4(o[at][r] * by, o[at][r + 2] * by, o[at + 1][r] * by, o[at + 1][r + 2] * by);
     };
-    const int live = min(kRowWarps, steps);
-    for (int x = tid; x < rows * kQuads; x += kRowThreads) {
-      const int r = x / kQuads, c = x % kQuads * 4;
-      float m = -INFINITY, l = 0.0f;
-      for (int w = 0; w < live; ++w) m = fmaxf(m, s_ml[w * kRows + r].x);
-      float4 acc = make_float4(0, 0, 0, 0);
-      for (int w = 0; w < live; ++w) {
-        const float2 ml = s_ml[w * kRows + r];
-        // (a warp without a score above -inf has l = 0 and O = 0, or a NaN)
-        const float f = ml.x == -INFINITY ? 1.0f : ex2(ml.x - m);
-        l += ml.y * f;
+    if (u.parts == 1) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        if (2 * t + r >= rows) continue;
+        int h;
+        const int64_t tok = u.token(p, 2 * t + r, &h);
         if constexpr (PV) {
-          const float4 v = *reinterpret_cast<const float4*>(
-              reinterpret_cast<const float*>(smem + w * C::kRingBytes) + r * C::kPitch + c);
-          acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+          T* to = static_cast<T*>(p.out) + (tok * p.heads + h) * p.dim;
+          const float by = row_scale(l[r]) * unit_v;
+#pragma unroll
+          for (int c = 0; c < kRuns; ++c)
+#pragma unroll
+            for (int x = 0; x < kRun / 4; ++x)
+              if (c * 128 + g * kRun + 4 * x < p.dim)
+                store4(to + c * 128 + g * kRun + 4 * x,
+                       l[r] == 0.0f ? make_float4(0, 0, 0, 0) : result(r, c, x, by));
+        }
+        if (g == 0 && p.lse != nullptr) p.lse[tok * p.heads + h] = row_lse(base[r], l[r]);
+      }
+      continue;
+    }
+    uint8_t* slot = u.slot<S::kBytes>(p, warp - u.warp0);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      if (2 * t + r >= rows) continue;
+      if constexpr (PV) {
+        float* to = reinterpret_cast<float*>(slot) + (2 * t + r) * DP;
+#pragma unroll
+        for (int c = 0; c < kRuns; ++c)
+#pragma unroll
+          for (int x = 0; x < kRun / 4; ++x)
+            *reinterpret_cast<float4*>(to + c * 128 + g * kRun + 4 * x) = result(r, c, x, unit_v);
+      }
+      if (g == 0) {
+        // nothing attended: (-inf, 0); every score NaN: l is
+        const float m = most[r] == -INFINITY && l[r] == l[r] ? -INFINITY : base[r];
+        reinterpret_cast<float2*>(slot + S::kMl)[2 * t + r] = make_float2(m, l[r]);
+      }
+    }
+    if (u.parts > kJoinHere) continue;
+    __syncwarp();
+    int last = 0;
+    if (lane == 0) last = atomic_add_acq_rel_gpu(&p.counters[u.warp0], 1) == u.parts - 1;
+    if (!__shfl_sync(0xffffffffu, last, 0)) continue;
+    // the last part to end joins all of them, in order: lane r the rows' factors,
+    // then a row at a time
+    float by[kJoinHere] = {}, m = -INFINITY, sum = 0.0f;
+    {
+      float2 ml[kJoinHere];
+#pragma unroll
+      for (int i = 0; i < kJoinHere; ++i) {
+        ml[i] = make_float2(-INFINITY, 0.0f);
+        if (i < u.parts && lane < rows)
+          ml[i] = __ldcg(reinterpret_cast<const float2*>(u.slot<S::kBytes>(p, i) + S::kMl) + lane);
+        m = fmaxf(m, ml[i].x);
+      }
+#pragma unroll
+      for (int i = 0; i < kJoinHere; ++i) {
+        by[i] = ml[i].x == -INFINITY ? 0.0f : ex2(ml[i].x - m);
+        sum += ml[i].y * by[i];
+      }
+    }
+    for (int r = 0; r < rows; ++r) {
+      int h;
+      const int64_t tok = u.token(p, r, &h);
+      const float mr = __shfl_sync(0xffffffffu, m, r), lr = __shfl_sync(0xffffffffu, sum, r);
+      if constexpr (PV) {
+#pragma unroll
+        for (int c = 0; c < (DP + 127) / 128; ++c) {
+          const int at = c * 128 + lane * 4;
+          float4 v[kJoinHere], acc = make_float4(0, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < kJoinHere; ++i) {
+            v[i] = make_float4(0, 0, 0, 0);
+            if (i < u.parts && at < DP)
+              v[i] = __ldcg(reinterpret_cast<const float4*>(
+                  reinterpret_cast<const float*>(u.slot<S::kBytes>(p, i)) + r * DP + at));
+          }
+#pragma unroll
+          for (int i = 0; i < kJoinHere; ++i) {
+            const float k = __shfl_sync(0xffffffffu, by[i], r);
+            if (k == 0.0f) continue;
+            acc.x += v[i].x * k, acc.y += v[i].y * k, acc.z += v[i].z * k, acc.w += v[i].w * k;
+          }
+          const float inv = row_scale(lr);
+          if (at < p.dim)
+            store4(static_cast<T*>(p.out) + (tok * p.heads + h) * p.dim + at,
+                   lr == 0.0f ? make_float4(0, 0, 0, 0)
+                              : make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
         }
       }
-      if (whole) {
-        store_row(r, c, acc, m, l);
-      } else {
-        if constexpr (PV) *reinterpret_cast<float4*>(slot + (r * DP + c) * 4) = acc;
-        if (c == 0) *reinterpret_cast<float2*>(slot + C::kSlotO + r * 8) = make_float2(m, l);
-      }
+      if (lane == 0 && p.lse != nullptr) p.lse[tok * p.heads + h] = row_lse(mr, lr);
     }
-    __syncthreads();  // the slot is written; the ring and s_q are free
-    if (whole) continue;
-    const int units = p.kv_heads * blocks;
-    if (tid == 0)
-      *s_last = atomic_add_acq_rel_gpu(&p.counters[seq.unit + unit], 1) == seq.splits - 1;
-    __syncthreads();
-    if (!*s_last) continue;
-    // the last part to end joins all of them, in order
-    const uint8_t* first = p.slots + (int64_t)(seq.slot + unit) * C::kSlotBytes;
-    const int64_t pitch = (int64_t)units * C::kSlotBytes;
-    for (int x = tid; x < rows * kQuads; x += kRowThreads) {
-      const int r = x / kQuads, c = x % kQuads * 4;
-      float m = -INFINITY, l = 0.0f;
-      float4 acc = make_float4(0, 0, 0, 0);
-      for (int i = 0; i < seq.splits; ++i) {
-        const float2 ml =
-            __ldcg(reinterpret_cast<const float2*>(first + i * pitch + C::kSlotO + r * 8));
-        if (ml.x == -INFINITY && ml.y == 0.0f) continue;
-        float4 v = make_float4(0, 0, 0, 0);
-        if constexpr (PV)
-          v = __ldcg(reinterpret_cast<const float4*>(first + i * pitch + (r * DP + c) * 4));
-        const float big = fmaxf(m, ml.x);
-        const float f = m == -INFINITY ? 1.0f : ex2(m - big);
-        const float k = ml.x == -INFINITY ? 1.0f : ex2(ml.x - big);
-        m = big;
-        l = l * f + ml.y * k;
-        acc.x = acc.x * f + v.x * k, acc.y = acc.y * f + v.y * k;
-        acc.z = acc.z * f + v.z * k, acc.w = acc.w * f + v.w * k;
-      }
-      store_row(r, c, acc, m, l);
-    }
-    __syncthreads();
   }
 }
 
-// Items to aim at where sequences are split: a few for every place on the card, so
-// that unequal ones even out.
-constexpr int kTarget = 148 * 2 * 3;
-constexpr int kLeast = 256;
+// Units of many parts (few long sequences): a CTA for each eight warps, in which no more
+// than one begins, a row for every four of its own, each of which takes a quarter of the
+// parts.
+template <typename T, int DP, bool PV>
+__global__ void __launch_bounds__(1024, 1) join_kernel(const RowsParams p) {
+  using S = Slot<DP, PV>;
+  constexpr int kWide = (DP + 127) / 128;
+  __shared__ float4 s_o[32][kWide * 32];
+  __shared__ float2 s_ml[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int r = warp & 7, quarter = warp >> 3;
+  const int64_t share = rows_share(p);
+  // the unit at the end of the eight shares, if it begins in them
+  static_assert(kJoinHere >= kRowWarps, "one unit of more parts in so many warps");
+  const int64_t place = (int64_t)(blockIdx.x + 1) * kRowWarps * share - 1;
+  if (place >= p.head->places) return;
+  RowsUnit u;
+  u.s = plan_find(p.seq, p.seqs, place);
+  u.find(p, place, share);
+  if (u.warp0 / kRowWarps != (int)blockIdx.x || u.parts <= kJoinHere) return;
+  const int each = (u.parts + 3) / 4, i0 = quarter * each, i1 = min(i0 + each, u.parts);
+  float m = -INFINITY, l = 0.0f;
+  float4 acc[kWide];
+#pragma unroll
+  for (int c = 0; c < kWide; ++c) acc[c] = make_float4(0, 0, 0, 0);
+  const auto add = [&](float2 ml, const float4 (&v)[kWide]) {
+    if (ml.x == -INFINITY) return;
+    const float big = fmaxf(m, ml.x), f = m == -INFINITY ? 0.0f : ex2(m - big), k = ex2(ml.x - big);
+    m = big;
+    l = l * f + ml.y * k;
+#pragma unroll
+    for (int c = 0; c < kWide; ++c) {
+      acc[c].x = acc[c].x * f + v[c].x * k, acc[c].y = acc[c].y * f + v[c].y * k;
+      acc[c].z = acc[c].z * f + v[c].z * k, acc[c].w = acc[c].w * f + v[c].w * k;
+    }
+  };
+  constexpr int kBatch = DP > 128 ? 2 : 4;
+  if (r < u.rows)
+    for (int i = i0; i < i1; i += kBatch) {
+      float2 ml[kBatch];
+      float4 v[kBatch][kWide];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const bool there = i + b < i1;
+        const uint8_t* from = u.slot<S::kBytes>(p, there ? i + b : i);
+        ml[b] = there ? __ldcg(reinterpret_cast<const float2*>(from + S::kMl) + r)
+                      : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+        for (int c = 0; c < kWide; ++c) {
+          v[b][c] = make_float4(0, 0, 0, 0);
+          if (PV && c * 128 + lane * 4 < DP)
+            v[b][c] = __ldcg(reinterpret_cast<const float4*>(
+                reinterpret_cast<const float*>(from) + r * DP + c * 128 + lane * 4));
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) add(ml[b], v[b]);
+    }
+#pragma unroll
+  for (int c = 0; c < kWide; ++c) s_o[warp][c * 32 + lane] = acc[c];
+  if (lane == 0) s_ml[warp] = make_float2(m, l);
+  __syncthreads();
+  if (quarter > 0 || r >= u.rows) return;
+  for (int w = warp + 8; w < 32; w += 8) {
+    float4 v[kWide];
+#pragma unroll
+    for (int c = 0; c < kWide; ++c) v[c] = s_o[w][c * 32 + lane];
+    add(s_ml[w], v);
+  }
+  int h;
+  const int64_t tok = u.token(p, r, &h);
+  const float inv = row_scale(l);
+  if constexpr (PV) {
+#pragma unroll
+    for (int c = 0; c < kWide; ++c)
+      if (c * 128 + lane * 4 < p.dim)
+        store4(static_cast<T*>(p.out) + (tok * p.heads + h) * p.dim + c * 128 + lane * 4,
+               l == 0.0f ? make_float4(0, 0, 0, 0)
+                         : make_float4(acc[c].x * inv, acc[c].y * inv, acc[c].z * inv, acc[c].w * inv));
+  }
+  if (lane == 0 && p.lse != nullptr) p.lse[tok * p.heads + h] = row_lse(m, l);
+}
+
+constexpr int kMostWarps = 148 * 2 * kRowWarps;
 
 struct ChunkLayout {
   size_t head, seq, counters, slots, total;
@@ -571,19 +783,16 @@ ChunkLayout chunk_layout(const ChunkArgs& a) {
   };
   l.head = take(sizeof(PlanHead));
   l.seq = take(sizeof(PlanSeq) * (size_t)a.seqs);
-  l.counters = take(sizeof(int) * 2 * kTarget);
-  // without a table wider than the smallest part nothing is split
-  const bool splits = (int64_t)a.width * a.block_size > kLeast;
-  const size_t slot = (a.v_cache != nullptr ? kRows * dp * 4 : 0) + kRows * 8;
-  l.slots = take(splits ? (size_t)2 * kTarget * slot : 0);
+  l.counters = take(sizeof(int) * kMostWarps);
+  l.slots = take((size_t)2 * kMostWarps * ((a.v_cache != nullptr ? kRows * dp * 4 : 0) + kRows * 8));
   l.total = at + 256;
   return l;
 }
 
-template <typename T, int DP, bool PV>
+template <typename T, int DP, bool PV, bool WHOLE>
 int launch_rows(const ChunkArgs& a, uint8_t* ws, cudaStream_t stream) {
   constexpr int HALVES = sizeof(T) == 4 ? 2 : 1;
-  using C = RowsCfg<DP, HALVES, PV>;
+  using C = RowsCfg<DP, HALVES, PV, WHOLE>;
   const ChunkLayout lay = chunk_layout(a);
   RowsParams p;
   p.q = a.q;
@@ -594,6 +803,8 @@ int launch_rows(const ChunkArgs& a, uint8_t* ws, cudaStream_t stream) {
   p.tables = a.tables;
   p.out = a.out;
   p.lse = a.lse;
+  p.logits = a.logits;
+  p.logit_pitch = (int64_t)a.width * a.block_size;
   p.head = reinterpret_cast<PlanHead*>(ws + lay.head);
   p.seq = reinterpret_cast<PlanSeq*>(ws + lay.seq);
   p.counters = reinterpret_cast<int*>(ws + lay.counters);
@@ -609,7 +820,7 @@ int launch_rows(const ChunkArgs& a, uint8_t* ws, cudaStream_t stream) {
   p.dim = a.dim;
   p.bs = a.block_size;
   p.width = a.width;
-  p.qk_scale = a.sm_scale * kLog2e;
+  p.qk_scale = a.sm_scale * kLog2e * kCodeUnit;
   PlanArgs plan;
   plan.cu = a.cu;
   plan.lens = a.lens;
@@ -620,23 +831,31 @@ int launch_rows(const ChunkArgs& a, uint8_t* ws, cudaStream_t stream) {
   plan.block_size = a.block_size;
   plan.width = a.width;
   plan.rows = kRows;
-  plan.target = kTarget;
-  plan.least = kLeast;
-  plan.round = kStep;
+  plan.step = kStep;
+  plan.over = kOver;
+  plan.from = 0;
+  plan.to = INT64_MAX;
   plan.head = reinterpret_cast<PlanHead*>(ws + lay.head);
   plan.seq = reinterpret_cast<PlanSeq*>(ws + lay.seq);
   plan.counters = p.counters;
-  plan.counts = 2 * kTarget;
+  plan.counts = kMostWarps;
   int* err = device_error_word();
   const int rc = launch_plan(plan, err, stream);
   if (rc != kOk) return rc;
-  auto kern = rows_kernel<T, DP, HALVES, PV>;
+  auto kern = rows_kernel<T, DP, HALVES, PV, WHOLE>;
   static std::atomic<uint64_t> done{0};
   allow_shared_memory(reinterpret_cast<const void*>(kern), C::kSmemBytes, done);
+  // no more warps than have their least share of the longest that the batch can be
   const int64_t units = (a.total_q * p.group / kRows + std::min<int64_t>(a.seqs, a.total_q) + 1) * a.kv_heads;
-  const int64_t parts = (int64_t)a.width * a.block_size / kLeast + 1;
-  const int64_t most = 148 * (PV && DP > 128 ? 1 : 2);
-  kern<<<(unsigned)std::min(most, units * std::min<int64_t>(parts, most)), kRowThreads, C::kSmemBytes, stream>>>(p, err);
+  const int64_t steps = ((int64_t)a.width * a.block_size + kStep - 1) / kStep + 1 + kOver;
+  const int64_t most = 148 * C::kCtas;
+  const int64_t each = (int64_t)kRowWarps * kLeast;
+  const int64_t ctas = std::min(most, units >= most * each ? most : (units * steps + each - 1) / each);
+  p.warps = (int)ctas * kRowWarps;
+  kern<<<(unsigned)ctas, kRowWarps * 32, C::kSmemBytes, stream>>>(p, err);
+  // a unit of so many parts needs so many steps
+  if ((steps - kOver) > (int64_t)kLeast * (kJoinHere - 1))
+    join_kernel<T, DP, PV><<<(unsigned)ctas, 1024, 0, stream>>>(p);
   return kOk;
 }
 
@@ -664,14 +883,18 @@ int launch_chunk(const ChunkArgs& a, void* workspace, size_t workspace_bytes, cu
                                            ~(uintptr_t)255);
   const auto with_dim = [&](auto t) {
     using T = decltype(t);
-    const auto with = [&](auto dp) {
+    const auto with = [&](auto dp, auto pv) {
       constexpr int DP = decltype(dp)::value;
-      return a.v_cache != nullptr ? launch_rows<T, DP, true>(a, ws, stream)
-                                  : launch_rows<T, DP, false>(a, ws, stream);
+      constexpr bool PV = decltype(pv)::value;
+      return a.block_size % kStep == 0 ? launch_rows<T, DP, PV, true>(a, ws, stream)
+                                       : launch_rows<T, DP, PV, false>(a, ws, stream);
     };
-    return a.dim <= 64    ? with(std::integral_constant<int, 64>{})
-           : a.dim <= 128 ? with(std::integral_constant<int, 128>{})
-                          : with(std::integral_constant<int, 256>{});
+    const auto with_pv = [&](auto dp) {
+      return a.v_cache != nullptr ? with(dp, std::true_type{}) : with(dp, std::false_type{});
+    };
+    return a.dim <= 64    ? with_pv(std::integral_constant<int, 64>{})
+           : a.dim <= 128 ? with_pv(std::integral_constant<int, 128>{})
+                          : with_pv(std::integral_constant<int, 256>{});
   };
   const int rc = a.dtype == 0 ? with_dim(0.0f) : a.dtype == 1 ? with_dim(__half()) : with_dim(__nv_bfloat16());
   if (rc != kOk) return rc;

@@ -197,6 +197,7 @@ struct ChunkArgs {
   const int32_t* cu;      // [seqs + 1]
   void* out;
   float* lse;  // nullable
+  float* logits = nullptr;  // with lse alone: also the scores, [total_q * heads][width * block_size]
   int64_t total_q, num_blocks;
   int64_t q_token_stride, q_head_stride;  // elements, of 16 bytes
   int seqs, heads, kv_heads, dim, block_size, width;

@@ -52,27 +52,27 @@ struct GatherParams {
 template <typename T, int DP, int HALVES>
 __global__ void __launch_bounds__(kThreads, DP > 128 ? 1 : 2) gather_kernel(const GatherParams p, int* err) {
   constexpr int kSteps = DP / 16;
-  constexpr int kTiles = kWarpKeys / 8;
-  __shared__ uint4 s_q[HALVES * kSteps * 32];
-  __shared__ float s_factor[16], s_lse[16];
+  constexpr int kTiles = kWarpKeys / 16;
+  constexpr int kPass = 16;  // rows at a time
+  __shared__ uint2 s_q[kPass / 8 * HALVES * kSteps * 32];
+  __shared__ float s_factor[kPass], s_start[kPass], s_lse[kPass];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int items = p.head->items;
-  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+  const int64_t items = p.head->places;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const int s = plan_find(p.seq, p.seqs, item);
     const PlanSeq seq = p.seq[s];
-    const int local = item - seq.first;
-    const int kvh = local % p.kv_heads;
+    const int unit = (int)((item - seq.first) / seq.steps);
+    const int part = (int)(item - seq.first) - unit * seq.steps;
+    const int kvh = unit % p.kv_heads, chunk = unit / p.kv_heads;
     const int64_t all_rows = seq.lq * (int64_t)p.group;
-    const int chunks = (int)((all_rows + kItemRows - 1) / kItemRows);
-    const int chunk = local / p.kv_heads % chunks, part = local / p.kv_heads / chunks;
     const int k0 = part * kKeys + warp * kWarpKeys;  // of this warp
     const int shift = seq.len - seq.lq;
     const int32_t* table = p.tables + (int64_t)s * p.width;
     // rows of this item that see the item's first key
     const int64_t r_end = min(all_rows, (chunk + 1) * (int64_t)kItemRows);
     const int64_t r_first = max((int64_t)(part * kKeys - shift), (int64_t)0) * p.group;
-    const int64_t r_begin = max(chunk * (int64_t)kItemRows, r_first / 16 * 16);
+    const int64_t r_begin = max(chunk * (int64_t)kItemRows, r_first / kPass * kPass);
 
     // this warp's keys: lane = key, then fragments
     const int key = k0 + lane, page = key / p.bs;
@@ -81,43 +81,47 @@ __global__ void __launch_bounds__(kThreads, DP > 128 ? 1 : 2) gather_kernel(cons
     const bool good = counts && phys >= 0 && (int64_t)phys < p.num_blocks;
     if (counts && !good) record_error(err, kDevBadBlockId);
     const uint32_t at = good ? (uint32_t)phys * p.bs + (key - page * p.bs) : 0xffffffffu;
-    const float ks = good ? p.k_scale[(int64_t)phys * p.kv_heads + kvh] : 0.0f;
+    const float ks = good ? p.k_scale[(int64_t)phys * p.kv_heads + kvh] * p.qk_scale : 0.0f;
     const unsigned mask = __ballot_sync(0xffffffffu, good);
-    uint2 b[kTiles][kSteps];
+    uint4 a[kTiles][kSteps];
     float scale[kTiles][2];
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
-      const uint32_t row = __shfl_sync(0xffffffffu, at, n * 8 + g);
-      uint4 w[DP / 64];
+      uint4 w[2][DP / 64];
 #pragma unroll
-      for (int c = 0; c < DP / 64; ++c) {
-        const int piece = c * 4 + t;
-        w[c] = make_uint4(0, 0, 0, 0);
-        if (row != 0xffffffffu && piece * 16 < p.dim)
-          w[c] = __ldg(reinterpret_cast<const uint4*>(
-              p.k_cache + ((int64_t)row * p.kv_heads + kvh) * p.dim + piece * 16));
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t row = __shfl_sync(0xffffffffu, at, n * 16 + r * 8 + g);
+        scale[n][r] = __shfl_sync(0xffffffffu, ks, n * 16 + r * 8 + g);
+#pragma unroll
+        for (int c = 0; c < DP / 64; ++c) {
+          const int piece = c * 4 + t;
+          w[r][c] = make_uint4(0, 0, 0, 0);
+          if (row != 0xffffffffu && piece * 16 < p.dim)
+            w[r][c] = __ldg(reinterpret_cast<const uint4*>(
+                p.k_cache + ((int64_t)row * p.kv_heads + kvh) * p.dim + piece * 16));
+        }
       }
 #pragma unroll
-      for (int c = 0; c < DP / 64; ++c) {
-        b[n][c * 4] = codes_to_half(w[c].x);
-        b[n][c * 4 + 1] = codes_to_half(w[c].y);
-        b[n][c * 4 + 2] = codes_to_half(w[c].z);
-        b[n][c * 4 + 3] = codes_to_half(w[c].w);
-      }
-      scale[n][0] = __shfl_sync(0xffffffffu, ks, n * 8 + 2 * t);
-      scale[n][1] = __shfl_sync(0xffffffffu, ks, n * 8 + 2 * t + 1);
+      for (int c = 0; c < DP / 64; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const auto word = [&](const uint4& v) { return e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w; };
+          const uint2 x = codes_plus_128(word(w[0][c])), y = codes_plus_128(word(w[1][c]));
+          a[n][c * 4 + e] = make_uint4(x.x, y.x, x.y, y.y);
+        }
     }
-    float sum[kTiles][2] = {};
-    for (int64_t r0 = r_begin; r0 < r_end; r0 += 16) {
-      const int rows = (int)min((int64_t)16, r_end - r0);
+    float sum[kTiles][2] = {};  // keys g and g + 8
+    for (int64_t r0 = r_begin; r0 < r_end; r0 += kPass) {
+      const int rows = (int)min((int64_t)kPass, r_end - r0);
       __syncthreads();  // the last rows are used
-      stage_queries<T, DP, HALVES>(s_q, s_factor, p.dim, warp, kWarps, [&](int r) -> const T* {
-        if (r >= rows) return nullptr;
-        const int tok = (int)((r0 + r) / p.group);
-        return static_cast<const T*>(p.q) + (seq.q0 + tok) * p.q_tok +
-               (kvh * p.group + (int)(r0 + r - (int64_t)tok * p.group)) * p.q_head;
-      });
-      if (tid < 16) {
+      stage_queries<T, DP, HALVES>(
+          s_q, s_factor, s_start, p.dim, kPass, warp, kWarps, [&](int r) -> const T* {
+            if (r >= rows) return nullptr;
+            const int tok = (int)((r0 + r) / p.group);
+            return static_cast<const T*>(p.q) + (seq.q0 + tok) * p.q_tok +
+                   (kvh * p.group + (int)(r0 + r - (int64_t)tok * p.group)) * p.q_head;
+          });
+      if (tid < kPass) {
         float v = -INFINITY;
         if (tid < rows) {
           const int tok = (int)((r0 + tid) / p.group);
@@ -126,45 +130,51 @@ __global__ void __launch_bounds__(kThreads, DP > 128 ? 1 : 2) gather_kernel(cons
         s_lse[tid] = v;
       }
       __syncthreads();
-      float d[kTiles][4] = {};
 #pragma unroll
-      for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-        for (int h = HALVES - 1; h >= 0; --h) {
-          const uint4 a = s_q[(h * kSteps + k) * 32 + lane];
-#pragma unroll
-          for (int n = 0; n < kTiles; ++n) mma_f16(d[n], a, b[n][k].x, b[n][k].y);
-        }
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = g + 8 * r;
-        const float f = s_factor[row] * p.qk_scale;
-        const float lse = s_lse[row];
-        // a row without keys (lse -inf) adds nothing
-        const bool none = row >= rows || lse == -INFINITY;
-        const int limit = none ? 0 : (int)((r0 + row) / p.group) + 1 + shift;
-        const float base = none ? 0.0f : lse * kLog2e;
+      for (int u = 0; u < kPass / 8; ++u) {
+        if (u * 8 >= rows) break;
+        float d[kTiles][4];
 #pragma unroll
         for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int at_key = n * 8 + 2 * t + e;
-            const float x = ex2(fmaf(d[n][2 * r + e], scale[n][e] * f, -base));
-            sum[n][e] += (mask >> at_key & 1u) && k0 + at_key < limit ? x : 0.0f;
+          for (int e = 0; e < 4; ++e) d[n][e] = s_start[u * 8 + 2 * t + (e & 1)];
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+          for (int h = HALVES - 1; h >= 0; --h) {
+            const uint2 b = s_q[((u * HALVES + h) * kSteps + k) * 32 + lane];
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n) mma_f16(d[n], a[n][k], b.x, b.y);
           }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = u * 8 + 2 * t + e;
+          const float lse = s_lse[row], f = s_factor[row];
+          // a row without keys (lse -inf) adds nothing
+          const bool none = row >= rows || lse == -INFINITY;
+          const int limit = none ? 0 : (int)((r0 + row) / p.group) + 1 + shift;
+          const float base = none ? 0.0f : lse * kLog2e;
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const int at_key = n * 16 + r * 8 + g;
+              const float x = ex2(fmaf(d[n][2 * r + e], scale[n][r] * f, -base));
+              sum[n][r] += (mask >> at_key & 1u) && k0 + at_key < limit ? x : 0.0f;
+            }
+        }
       }
     }
-    // the lanes of a column, then one adds
+    // the lanes of a key, then one adds
 #pragma unroll
     for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-#pragma unroll
-        for (int x = 4; x < 32; x <<= 1) sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], x);
-        const int from = n * 8 + 2 * t + e;
-        const uint32_t slot = __shfl_sync(0xffffffffu, at, from);
-        if (g == 0 && slot != 0xffffffffu && r_begin < r_end) {
-          const float v = sum[n][e];
+      for (int r = 0; r < 2; ++r) {
+        sum[n][r] += __shfl_xor_sync(0xffffffffu, sum[n][r], 1);
+        sum[n][r] += __shfl_xor_sync(0xffffffffu, sum[n][r], 2);
+        const uint32_t slot = __shfl_sync(0xffffffffu, at, n * 16 + r * 8 + g);
+        if (t == 0 && slot != 0xffffffffu && r_begin < r_end) {
+          const float v = sum[n][r];
           if (v < 33554432.0f) {
             const unsigned long long u = __float2ull_rn(v * kUnit);
             if (u != 0) atomicAdd(p.sums + slot, u);
@@ -251,7 +261,7 @@ void launch_gather(const ChunkArgs& a, const float* lse, uint8_t* ws, const Layo
   p.dim = a.dim;
   p.bs = a.block_size;
   p.width = a.width;
-  p.qk_scale = a.sm_scale * kLog2e;
+  p.qk_scale = a.sm_scale * kLog2e * kCodeUnit;
   const int64_t parts = ((int64_t)a.width * a.block_size + kKeys - 1) / kKeys;
   const int64_t chunks = a.total_q * p.group / kItemRows + std::min<int64_t>(a.seqs, a.total_q);
   const int64_t most = 148 * (DP > 128 ? 1 : 2);
@@ -297,9 +307,10 @@ int launch_accumulate(const ChunkArgs& a, float* weights, void* workspace, size_
   plan.block_size = a.block_size;
   plan.width = a.width;
   plan.rows = kItemRows;
-  plan.target = 0;  // parts of the smallest size
-  plan.least = kKeys;
-  plan.round = kKeys;
+  plan.step = kKeys;
+  plan.over = 0;
+  plan.from = 0;
+  plan.to = INT64_MAX;
   plan.head = reinterpret_cast<PlanHead*>(ws + lay.head);
   plan.seq = reinterpret_cast<PlanSeq*>(ws + lay.seq);
   plan.counters = nullptr;
