@@ -12,9 +12,11 @@
 //   rows_kernel   a unit is 8 query rows of a KV head and its sequence's keys; each
 //                 warp takes an equal share of the units' steps of 16 keys;
 //   join_kernel   units that more than 8 warps share.
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <mutex>
 #include <string>
 #include <type_traits>
 
@@ -134,8 +136,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs p, in
 // for 128 channels of V are 32 instead of 64.  S comes with a lane's keys in rows of
 // the fragment; movmatrix turns the probabilities for the second product.
 //
-// Warps work alone, each with a ring of stages of 16 keys that cp.async fills two steps
-// ahead: each has the same share of all units' steps, so that they end together, and
+// Warps work alone, each with a ring of stages of 16 keys that is filled two steps ahead
+// (by TMA, two boxes a step; by cp.async where steps are not within a page): each has the same share of all units' steps, so that they end together, and
 // while one of them waits for the first pages of its next unit the others go on.  (CTAs
 // of 8 warps on one unit met at its start and end and took 94 us for 64 sequences of
 // 2,050 tokens, 75 us with equal shares.)
@@ -143,7 +145,6 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs p, in
 constexpr int kStep = 16;      // keys of a step
 constexpr int kRows = 8;
 constexpr int kRowWarps = 8;   // of a CTA
-constexpr int kStages = 3;
 constexpr int kOver = 6;       // steps that a unit's start and end cost
 constexpr int kLeast = 16;     // places of a warp's share
 constexpr int kJoinHere = 8;   // parts that the last of them joins; more are left to join_kernel
@@ -153,16 +154,28 @@ constexpr int kJoinHere = 8;   // parts that the last of them joins; more are le
 constexpr float kLazy = 2.0f;
 constexpr float kPShift = 13.0f;
 
-template <int DP, int HALVES, bool PV, bool WHOLE>
+template <int DP, bool PV, bool WHOLE>
 struct RowsCfg {
-  static constexpr int kCodeBytes = (PV ? 2 : 1) * kStep * DP;  // K, then V
-  // and the K and V scales: of the step, or of each key with the mask of those that count
-  static constexpr int kStageBytes = kCodeBytes + (WHOLE ? 16 : 2 * kStep * 4 + 16);
-  static constexpr int kRingBytes = kStages * kStageBytes;  // of a warp
-  static constexpr int kSmemBytes = kRowWarps * kRingBytes;
+  static constexpr int kStages = PV || DP > 128 ? 3 : 5;
+  static constexpr int kCodeBytes = (PV ? 2 : 1) * kStep * DP;  // of a stage: K, then V
+  // behind all stages' codes: the K and V scales, of the step, or of each key with the
+  // mask of those that count
+  static constexpr int kScaleBytes = WHOLE ? 8 : 2 * kStep * 4 + 16;
+  static constexpr int kRingBytes = kStages * kCodeBytes;  // of a warp
+  static constexpr int kOffScale = kRowWarps * kRingBytes;
+  static constexpr int kOffBar = kOffScale + kRowWarps * kStages * kScaleBytes;
+  static constexpr int kSmemBytes = kOffBar + (WHOLE ? kRowWarps * kStages * 8 : 0);
   static constexpr int kCtas = PV && DP > 128 ? 1 : 2;  // per SM
   static_assert(kCtas * (kSmemBytes + 1024) <= 228 * 1024, "shared memory");
 };
+
+// The key in row g (of 8) of a step's fragments.  With rows of 128 bytes it is such that
+// the lanes that read K at once (two g, pieces t or t + 4) and V at once (pieces g, keys of
+// four even or four odd rows) meet no bank twice under the copies' 128-byte swizzle.
+template <int DP, bool WHOLE>
+__device__ __forceinline__ int key_of_row(int g) {
+  return DP == 128 && WHOLE ? (0x37621540 >> (4 * g)) & 7 : g;
+}
 
 // A part of a unit: rows of O, then (m, l) of each.
 template <int DP, bool PV>
@@ -245,11 +258,13 @@ __device__ __forceinline__ float row_lse(float m, float l) {
 }
 
 // Without PV only the denominators are taken (p.lse).  WHOLE: pages of a multiple of 16
-// tokens, so that a step's keys share their scales and are one run of memory.
+// tokens, so that a step's keys share their scales and are one box of the caches' maps.
 template <typename T, int DP, int HALVES, bool PV, bool WHOLE>
-__global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, HALVES, PV, WHOLE>::kCtas)
-    rows_kernel(const RowsParams p, int* err) {
-  using C = RowsCfg<DP, HALVES, PV, WHOLE>;
+__global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, PV, WHOLE>::kCtas)
+    rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                const RowsParams p, int* err) {
+  using C = RowsCfg<DP, PV, WHOLE>;
+  constexpr int kStages = C::kStages;
   using S = Slot<DP, PV>;
   constexpr int kPieces = DP / 16;              // 16-byte pieces of a key's codes
   constexpr int kPasses = kPieces * kStep / 32; // copies a lane makes of K or V
@@ -259,10 +274,25 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, HALVES, PV, WHOLE>
   constexpr int kV = kStep * DP;                // V of a stage
   constexpr int kRun = DP >= 128 ? 16 : 8;      // consecutive channels of a lane's results
   constexpr int kRuns = (DP + 127) / 128;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int warp = blockIdx.x * kRowWarps + (threadIdx.x >> 5);  // of the grid
-  uint8_t* ring = smem + (threadIdx.x >> 5) * C::kRingBytes;
+  const int in_cta = threadIdx.x >> 5;
+  const int warp = blockIdx.x * kRowWarps + in_cta;  // of the grid
+  uint8_t* ring = smem + in_cta * C::kRingBytes;
+  uint8_t* ring_scale = smem + C::kOffScale + in_cta * kStages * C::kScaleBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBar) + in_cta * kStages;
+  uint32_t phases = 0;  // of the stages' barriers: the next wait's
+  uint64_t hold = 0;
+  if constexpr (WHOLE) {
+    if (lane == 0) {
+      prefetch_tensormap(&map_k);
+      if (PV) prefetch_tensormap(&map_v);
+      for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1);
+      mbar_fence_init();
+    }
+    __syncwarp();
+    hold = l2_policy_evict_first();
+  }
 
   // rows in front of the first and behind the last sequence become zero
   const PlanHead head = *p.head;
@@ -280,11 +310,19 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, HALVES, PV, WHOLE>
   const int64_t token_bytes = (int64_t)p.kv_heads * p.dim;
   const int piece = lane % kPieces, key_in = lane / kPieces;
   const bool on = piece * 16 < p.dim;
-  const uint32_t copy_at = key_in * DP + piece_at<DP>(key_in, piece) * 16;
-  const uint32_t k_at = g * DP + piece_at<DP>(g, t) * 16;
-  const uint32_t v_at = DP >= 128 ? 2 * t * DP + piece_at<DP>(2 * t, g) * 16
-                                  : 2 * t * DP + piece_at<DP>(2 * t, g >> 1) * 16 + (g & 1) * 8;
-  constexpr uint32_t kOdd = DP >= 128 ? 64 : 0;  // of an odd key, in piece_at
+  // key, and its place in a stage, of a lane's rows g and g + 8, and of columns 2 t and
+  // 2 t + 1 (and + 8) of the transposed probabilities
+  const int kg = key_of_row<DP, WHOLE>(g);
+  const int kv0 = key_of_row<DP, WHOLE>(2 * t), kv1 = key_of_row<DP, WHOLE>(2 * t + 1);
+  const auto swizzle = [&](int k, int pc) {
+    return DP == 128 && WHOLE ? pc ^ (k & 7) : piece_at<DP>(k, pc);
+  };
+  const uint32_t k_at = kg * DP + swizzle(kg, t) * 16;
+  const auto v_place = [&](int k) {
+    return (uint32_t)(DP >= 128 ? k * DP + swizzle(k, g) * 16
+                                : k * DP + swizzle(k, g >> 1) * 16 + (g & 1) * 8);
+  };
+  const uint32_t v_at[2] = {v_place(kv0), v_place(kv1)};
 
   const int64_t share = rows_share(p);
   int64_t now = warp * share;
@@ -315,40 +353,35 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, HALVES, PV, WHOLE>
     const int8_t* v_col = PV ? p.v_cache + col : nullptr;
     const auto issue = [&]() {
       if (next_left > 0) {
-        uint8_t* stage = ring + copied * C::kStageBytes;
-        const uint32_t to = smem_u32(stage);
+        uint8_t* stage = ring + copied * C::kCodeBytes;
+        uint8_t* scale = ring_scale + copied * C::kScaleBytes;
         if constexpr (WHOLE) {
           const bool good = entry >= 0 && (int64_t)entry < p.num_blocks;
           gone = good ? gone & ~(1u << copied) : gone | 1u << copied;
-          if (!good) record_error(err, kDevBadBlockId);
           if (good) {
             if (lane < (PV ? 2 : 1))
-              copy4_if(true, to + C::kCodeBytes + lane * 4,
+              copy4_if(true, smem_u32(scale) + lane * 4,
                        (lane == 0 ? p.k_scale : p.v_scale) + (int64_t)entry * p.kv_heads + kvh);
-            const int64_t from = ((int64_t)entry * p.bs + rem + key_in) * token_bytes;
-            const int8_t* kp = k_col + from;
-            const int8_t* vp = v_col + from;
-#pragma unroll
-            for (int c = 0; c < kPasses; ++c) {
-              // (the swizzle of key c kAhead + key_in from that of key_in)
-              const uint32_t at =
-                  (copy_at ^ (DP == 128 ? (c & 1) * 64 : DP == 256 ? (c & 3) * 32 : 0)) + c * kAhead * DP;
-              copy16_if(true, to + at, kp);
-              if constexpr (PV) copy16_if(true, to + at + kV, vp);
-              kp += kAhead * token_bytes;
-              if constexpr (PV) vp += kAhead * token_bytes;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&full[copied], C::kCodeBytes);
+              const int token = entry * p.bs + rem;
+              tma_load_3d(stage, &map_k, &full[copied], 0, kvh, token, hold);
+              if (PV) tma_load_3d(stage + kV, &map_v, &full[copied], 0, kvh, token, hold);
             }
+          } else {
+            record_error(err, kDevBadBlockId);
           }
         } else {
           const bool counts = (lane & 15) < next_left;
           const bool good = counts && entry >= 0 && (int64_t)entry < p.num_blocks;
           if (counts && !good) record_error(err, kDevBadBlockId);
+          const uint32_t to = smem_u32(stage);
           if (PV || lane < 16)
-            copy4_if(good, to + C::kCodeBytes + lane * 4,
+            copy4_if(good, smem_u32(scale) + lane * 4,
                      (lane < 16 ? p.k_scale : p.v_scale) +
                          (good ? (int64_t)entry * p.kv_heads + kvh : 0));
           const unsigned mask = __ballot_sync(0xffffffffu, good) & 0xffffu;
-          if (lane == 0) *reinterpret_cast<uint32_t*>(stage + C::kCodeBytes + 128) = mask;
+          if (lane == 0) *reinterpret_cast<uint32_t*>(scale + 128) = mask;
           const uint32_t at = good ? (uint32_t)entry * p.bs + rem : 0xffffffffu;
 #pragma unroll 1
           for (int c = 0; c < kPasses; ++c) {
@@ -398,7 +431,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, HALVES, PV, WHOLE>
         for (int r = 0; r < 2; ++r) {
           int h;
           const int64_t tok = u.token(p, 2 * t + r, &h);
-          if (2 * t + r < rows) logit[r] = p.logits + (tok * p.heads + h) * p.logit_pitch + g;
+          if (2 * t + r < rows) logit[r] = p.logits + (tok * p.heads + h) * p.logit_pitch + kg;
         }
     }
 
@@ -418,12 +451,20 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, HALVES, PV, WHOLE>
       copies_wait<kStages - 2>();
       __syncwarp();
       issue();
-      const uint8_t* stage = ring + used * C::kStageBytes;
-      const float* scales = reinterpret_cast<const float*>(stage + C::kCodeBytes);
-      const bool lost = WHOLE && (gone >> used & 1u);
+      const uint8_t* stage = ring + used * C::kCodeBytes;
+      const float* scales = reinterpret_cast<const float*>(ring_scale + used * C::kScaleBytes);
+      const int here = used;
       used = used + 1 == kStages ? 0 : used + 1;
-      if (lost) continue;
-      // scores: keys g and g + 8, rows as above: (g, first), (g, second), (g + 8, ...);
+      if constexpr (WHOLE) {
+        if (gone >> here & 1u) continue;
+        if (!mbar_wait_short(&full[here], phases >> here & 1u, err)) {
+          record_error(err, kDevWaitTimeout);
+          mbar_drain(&full[here], phases >> here & 1u);  // no copy outlives the CTA
+        }
+        phases ^= 1u << here;
+        __syncwarp();
+      }
+      // scores: keys of rows g and g + 8, query rows as above: (g, first), (g, second), (g + 8, ...);
       // two sums, since a product waits 25 clocks for the one before it
       float sc[4] = {start[0], start[1], start[0], start[1]}, sd[4] = {};
 #pragma unroll
@@ -431,7 +472,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, HALVES, PV, WHOLE>
         // (piece pc * 4 + t: bit 2 turned by odd pc)
         const uint32_t at = (k_at ^ ((pc & 1) * 64)) + pc / 2 * 128;
         const uint4 w0 = *reinterpret_cast<const uint4*>(stage + at);
-        const uint4 w1 = *reinterpret_cast<const uint4*>(stage + at + 8 * DP);
+        const uint4 w1 = *reinterpret_cast<const uint4*>(stage + at + 8 * DP);  // (the same swizzle)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint2 x = codes_plus_128(e == 0 ? w0.x : e == 1 ? w0.y : e == 2 ? w0.z : w0.w);
@@ -449,13 +490,13 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, HALVES, PV, WHOLE>
         ks[0] = ks[1] = x.x;
         if constexpr (PV) vs[0] = vs[1] = x.y;
       } else {
-        ks[0] = scales[g], ks[1] = scales[g + 8];
-        if constexpr (PV) vs[0] = scales[kStep + g], vs[1] = scales[kStep + g + 8];
-        mask = *reinterpret_cast<const uint32_t*>(stage + C::kCodeBytes + 128);
+        ks[0] = scales[kg], ks[1] = scales[kg + 8];
+        if constexpr (PV) vs[0] = scales[kStep + kg], vs[1] = scales[kStep + kg + 8];
+        mask = reinterpret_cast<const uint32_t*>(scales)[2 * kStep];
       }
       const bool all = (WHOLE || mask == 0xffffu) && key_now + kStep <= clear;
       const auto seen = [&](int e) {  // e as in sc
-        const int k = g + (e >> 1) * 8;
+        const int k = kg + (e >> 1) * 8;
         return (WHOLE ? key_now + k < k1 : mask >> k & 1u) &&
                key_now + k < ((e & 1) ? limit1 : limit0);
       };
@@ -514,8 +555,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, HALVES, PV, WHOLE>
 #pragma unroll
         for (int r = 0; r < 2; ++r)
           if (logit[r] != nullptr) {
-            if (key_now + g < k1) logit[r][key_now] = sc[r];
-            if (key_now + g + 8 < k1) logit[r][key_now + 8] = sc[r + 2];
+            if (key_now + kg < k1) logit[r][key_now] = sc[r];
+            if (key_now + kg + 8 < k1) logit[r][key_now + 8] = sc[r + 2];
           }
       }
       uint32_t hi[2], lo[2];  // keys g, g + 8
@@ -546,10 +587,10 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, HALVES, PV, WHOLE>
         constexpr int kWords = DP >= 128 ? 4 : 2;
 #pragma unroll
         for (int c = 0; c < kRuns; ++c) {
-          uint32_t w[4][kWords];  // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+          uint32_t w[4][kWords];  // keys kv0, kv1, kv0 + 8, kv1 + 8
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint32_t at = ((k & 1) ? (v_at ^ kOdd) + DP : v_at) + (k >> 1) * 8 * DP + c * 128;
+            const uint32_t at = v_at[k & 1] + (k >> 1) * 8 * DP + c * 128;
             if constexpr (DP >= 128) {
               const uint4 x = *reinterpret_cast<const uint4*>(vt + at);
               w[k][0] = x.x, w[k][1] = x.y, w[k][2 % kWords] = x.z, w[k][3 % kWords] = x.w;
@@ -766,6 +807,43 @@ __global__ void __launch_bounds__(1024, 1) join_kernel(const RowsParams p) {
   if (lane == 0 && p.lse != nullptr) p.lse[tok * p.heads + h] = row_lse(m, l);
 }
 
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(p);
+  });
+  return fn;
+}
+
+// A cache as (channel, head, token of all pages); boxes of `channels` codes of one head
+// and `tokens` tokens, swizzled within rows of 64 or 128 bytes.  Channels past head_dim
+// load as zero.
+bool cache_map(CUtensorMap* map, const int8_t* cache, const ChunkArgs& a, int channels, int tokens) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return false;
+  if (a.num_blocks == 0) return true;  // (never used)
+  cuuint64_t dims[3] = {(cuuint64_t)a.dim, (cuuint64_t)a.kv_heads,
+                        (cuuint64_t)a.num_blocks * a.block_size};
+  cuuint64_t strides[2] = {(cuuint64_t)a.dim, (cuuint64_t)a.dim * a.kv_heads};
+  cuuint32_t box[3] = {(cuuint32_t)channels, 1, (cuuint32_t)tokens};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<int8_t*>(cache), dims, strides, box,
+            estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            channels == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 constexpr int kMostWarps = 148 * 2 * kRowWarps;
 
 struct ChunkLayout {
@@ -792,7 +870,7 @@ ChunkLayout chunk_layout(const ChunkArgs& a) {
 template <typename T, int DP, bool PV, bool WHOLE>
 int launch_rows(const ChunkArgs& a, uint8_t* ws, cudaStream_t stream) {
   constexpr int HALVES = sizeof(T) == 4 ? 2 : 1;
-  using C = RowsCfg<DP, HALVES, PV, WHOLE>;
+  using C = RowsCfg<DP, PV, WHOLE>;
   const ChunkLayout lay = chunk_layout(a);
   RowsParams p;
   p.q = a.q;
@@ -852,7 +930,13 @@ int launch_rows(const ChunkArgs& a, uint8_t* ws, cudaStream_t stream) {
   const int64_t each = (int64_t)kRowWarps * kLeast;
   const int64_t ctas = std::min(most, units >= most * each ? most : (units * steps + each - 1) / each);
   p.warps = (int)ctas * kRowWarps;
-  kern<<<(unsigned)ctas, kRowWarps * 32, C::kSmemBytes, stream>>>(p, err);
+  CUtensorMap map_k = {}, map_v = {};
+  if (WHOLE && (!cache_map(&map_k, a.k_cache, a, DP, kStep) ||
+                (PV && !cache_map(&map_v, a.v_cache, a, DP, kStep)))) {
+    set_error("cuTensorMapEncodeTiled failed for the caches");
+    return kCudaError;
+  }
+  kern<<<(unsigned)ctas, kRowWarps * 32, C::kSmemBytes, stream>>>(map_k, map_v, p, err);
   // a unit of so many parts needs so many steps
   if ((steps - kOver) > (int64_t)kLeast * (kJoinHere - 1))
     join_kernel<T, DP, PV><<<(unsigned)ctas, 1024, 0, stream>>>(p);
@@ -886,8 +970,9 @@ int launch_chunk(const ChunkArgs& a, void* workspace, size_t workspace_bytes, cu
     const auto with = [&](auto dp, auto pv) {
       constexpr int DP = decltype(dp)::value;
       constexpr bool PV = decltype(pv)::value;
-      return a.block_size % kStep == 0 ? launch_rows<T, DP, PV, true>(a, ws, stream)
-                                       : launch_rows<T, DP, PV, false>(a, ws, stream);
+      if constexpr (DP <= 128)
+        if (a.block_size % kStep == 0) return launch_rows<T, DP, PV, true>(a, ws, stream);
+      return launch_rows<T, DP, PV, false>(a, ws, stream);
     };
     const auto with_pv = [&](auto dp) {
       return a.v_cache != nullptr ? with(dp, std::true_type{}) : with(dp, std::false_type{});
