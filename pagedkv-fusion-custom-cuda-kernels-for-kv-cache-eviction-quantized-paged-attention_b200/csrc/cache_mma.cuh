@@ -278,7 +278,8 @@ struct PlanArgs {
   int counts;
 };
 
-int launch_plan(const PlanArgs& a, int* err, cudaStream_t stream);
+// One or two plans of a call, the second for another kernel.
+int launch_plan(const PlanArgs& a, const PlanArgs* second, int* err, cudaStream_t stream);
 
 // The sequence of a place; one warp, a search of 32 at a time.
 __device__ __forceinline__ int plan_find(const PlanSeq* seq, int seqs, int64_t place) {

@@ -12,6 +12,7 @@
 //   rows_kernel   a unit is 8 query rows of a KV head and its sequence's keys; each
 //                 warp takes an equal share of the units' steps of 16 keys;
 //   join_kernel   units that more than 8 warps share.
+// Sequences of more rows than 8 go to chunk_tc.cu.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -21,6 +22,7 @@
 #include <type_traits>
 
 #include "cache_mma.cuh"
+#include "chunk.h"
 #include "pkv_internal.h"
 
 namespace pkv {
@@ -67,7 +69,8 @@ __device__ __forceinline__ int64_t scan_sum(int64_t v, int64_t* shared, int64_t*
   return v;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs p, int* err) {
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs first_plan, const PlanArgs second_plan, int* err) {
+  const PlanArgs p = blockIdx.x == 0 ? first_plan : second_plan;
   __shared__ int s_max[kPlanWarps];
   __shared__ int64_t s_sum[kPlanWarps];
   __shared__ int s_end[kPlanThreads];
@@ -846,8 +849,22 @@ bool cache_map(CUtensorMap* map, const int8_t* cache, const ChunkArgs& a, int ch
 
 constexpr int kMostWarps = 148 * 2 * kRowWarps;
 
+// Which kernels a call's sequences go to: those of up to 8 rows of a KV head to the warps
+// of rows_kernel, the others to chunk_tc.cu, where it takes the shapes.  The lengths are on
+// the device, so a call launches both unless its sizes tell: at most one token a sequence
+// (decode), or more heads a group than a row tile, or one sequence of many tokens.
+struct Division {
+  bool rows, tc;
+};
+Division division_of(const ChunkArgs& a) {
+  const int group = a.heads / a.kv_heads;
+  if (!chunk_tc_takes(a) || (a.total_q <= a.seqs && group <= kRows)) return {true, false};
+  if (group > kRows || (a.seqs <= 1 && a.total_q * group > kRows)) return {false, true};
+  return {true, true};
+}
+
 struct ChunkLayout {
-  size_t head, seq, counters, slots, total;
+  size_t head, seq, counters, slots, head2, seq2, tc, total;
 };
 
 ChunkLayout chunk_layout(const ChunkArgs& a) {
@@ -859,10 +876,14 @@ ChunkLayout chunk_layout(const ChunkArgs& a) {
     at += (bytes + 255) / 256 * 256;
     return here;
   };
+  const Division d = division_of(a);
   l.head = take(sizeof(PlanHead));
   l.seq = take(sizeof(PlanSeq) * (size_t)a.seqs);
-  l.counters = take(sizeof(int) * kMostWarps);
-  l.slots = take((size_t)2 * kMostWarps * ((a.v_cache != nullptr ? kRows * dp * 4 : 0) + kRows * 8));
+  l.counters = take(d.rows ? sizeof(int) * kMostWarps : 0);
+  l.slots = take(d.rows ? (size_t)2 * kMostWarps * ((a.v_cache != nullptr ? kRows * dp * 4 : 0) + kRows * 8) : 0);
+  l.head2 = take(d.tc ? sizeof(PlanHead) : 0);
+  l.seq2 = take(d.tc ? sizeof(PlanSeq) * (size_t)a.seqs : 0);
+  l.tc = take(d.tc ? chunk_tc_workspace_size(a) : 0);
   l.total = at + 256;
   return l;
 }
@@ -899,27 +920,6 @@ int launch_rows(const ChunkArgs& a, uint8_t* ws, cudaStream_t stream) {
   p.bs = a.block_size;
   p.width = a.width;
   p.qk_scale = a.sm_scale * kLog2e * kCodeUnit;
-  PlanArgs plan;
-  plan.cu = a.cu;
-  plan.lens = a.lens;
-  plan.seqs = a.seqs;
-  plan.total_q = (int)a.total_q;
-  plan.group = p.group;
-  plan.kv_heads = a.kv_heads;
-  plan.block_size = a.block_size;
-  plan.width = a.width;
-  plan.rows = kRows;
-  plan.step = kStep;
-  plan.over = kOver;
-  plan.from = 0;
-  plan.to = INT64_MAX;
-  plan.head = reinterpret_cast<PlanHead*>(ws + lay.head);
-  plan.seq = reinterpret_cast<PlanSeq*>(ws + lay.seq);
-  plan.counters = p.counters;
-  plan.counts = kMostWarps;
-  int* err = device_error_word();
-  const int rc = launch_plan(plan, err, stream);
-  if (rc != kOk) return rc;
   auto kern = rows_kernel<T, DP, HALVES, PV, WHOLE>;
   static std::atomic<uint64_t> done{0};
   allow_shared_memory(reinterpret_cast<const void*>(kern), C::kSmemBytes, done);
@@ -936,7 +936,8 @@ int launch_rows(const ChunkArgs& a, uint8_t* ws, cudaStream_t stream) {
     set_error("cuTensorMapEncodeTiled failed for the caches");
     return kCudaError;
   }
-  kern<<<(unsigned)ctas, kRowWarps * 32, C::kSmemBytes, stream>>>(map_k, map_v, p, err);
+  kern<<<(unsigned)ctas, kRowWarps * 32, C::kSmemBytes, stream>>>(map_k, map_v, p,
+                                                                  device_error_word());
   // a unit of so many parts needs so many steps
   if ((steps - kOver) > (int64_t)kLeast * (kJoinHere - 1))
     join_kernel<T, DP, PV><<<(unsigned)ctas, 1024, 0, stream>>>(p);
@@ -945,8 +946,9 @@ int launch_rows(const ChunkArgs& a, uint8_t* ws, cudaStream_t stream) {
 
 }  // namespace
 
-int launch_plan(const PlanArgs& a, int* err, cudaStream_t stream) {
-  plan_kernel<<<1, kPlanThreads, 0, stream>>>(a, err);
+int launch_plan(const PlanArgs& a, const PlanArgs* second, int* err, cudaStream_t stream) {
+  plan_kernel<<<second != nullptr ? 2 : 1, kPlanThreads, 0, stream>>>(a, second != nullptr ? *second : a,
+                                                                      err);
   return kOk;
 }
 
@@ -965,6 +967,35 @@ int launch_chunk(const ChunkArgs& a, void* workspace, size_t workspace_bytes, cu
   }
   uint8_t* ws = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 255) &
                                            ~(uintptr_t)255);
+  const ChunkLayout lay = chunk_layout(a);
+  const Division d = division_of(a);
+  PlanArgs plan;
+  plan.cu = a.cu;
+  plan.lens = a.lens;
+  plan.seqs = a.seqs;
+  plan.total_q = (int)a.total_q;
+  plan.group = a.heads / a.kv_heads;
+  plan.kv_heads = a.kv_heads;
+  plan.block_size = a.block_size;
+  plan.width = a.width;
+  plan.rows = kRows;
+  plan.step = kStep;
+  plan.over = kOver;
+  plan.from = 0;
+  plan.to = d.tc ? kRows : INT64_MAX;
+  plan.head = reinterpret_cast<PlanHead*>(ws + lay.head);
+  plan.seq = reinterpret_cast<PlanSeq*>(ws + lay.seq);
+  plan.counters = reinterpret_cast<int*>(ws + lay.counters);
+  plan.counts = kMostWarps;
+  PlanArgs plan2 = chunk_tc_plan(plan);
+  plan2.from = d.rows ? kRows + 1 : 0;
+  plan2.to = INT64_MAX;
+  plan2.head = reinterpret_cast<PlanHead*>(ws + lay.head2);
+  plan2.seq = reinterpret_cast<PlanSeq*>(ws + lay.seq2);
+  launch_plan(d.rows ? plan : plan2, d.rows && d.tc ? &plan2 : nullptr, device_error_word(), stream);
+  int rc = kOk;
+  if (d.tc) rc = launch_chunk_tc(a, plan2.head, plan2.seq, ws + lay.tc, !d.rows, stream);
+  if (rc != kOk) return rc;
   const auto with_dim = [&](auto t) {
     using T = decltype(t);
     const auto with = [&](auto dp, auto pv) {
@@ -981,7 +1012,8 @@ int launch_chunk(const ChunkArgs& a, void* workspace, size_t workspace_bytes, cu
            : a.dim <= 128 ? with_pv(std::integral_constant<int, 128>{})
                           : with_pv(std::integral_constant<int, 256>{});
   };
-  const int rc = a.dtype == 0 ? with_dim(0.0f) : a.dtype == 1 ? with_dim(__half()) : with_dim(__nv_bfloat16());
+  if (d.rows)
+    rc = a.dtype == 0 ? with_dim(0.0f) : a.dtype == 1 ? with_dim(__half()) : with_dim(__nv_bfloat16());
   if (rc != kOk) return rc;
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) {

@@ -1,0 +1,1014 @@
+// Attention of new tokens over the INT8 paged cache (see chunk.cu) where a KV head has
+// more rows than one mma.sync tile: chunks of prompts, drafted tokens of wide groups.
+//
+// A unit is 256 query rows (token, head of the group) of one KV head over the keys that
+// its last row sees, in tiles of 128 keys; one CTA per SM takes an equal share of all
+// units' tiles.  A unit that is cut leaves partial results, joined by a kernel behind.
+// Per row tile of 128 rows
+//   S = Q K^T    tcgen05 kind::f16, K's codes as exact fp16, Q as fp16 times a power of
+//                two per row (two numbers, hi and lo, for fp32 queries);
+//   P = exp2(...) times the key's V scale, fp16 (again two for fp32), written over S;
+//   O += P V     V's codes as fp16 read MN-major.
+// The row tiles take turns on the tensor cores as in prefill.cu, whose P in 16 bits this
+// kernel's 16-bit form shares; a unit of at most 128 rows has its even key tiles taken by
+// the one and its odd ones by the other, joined at its end.
+//
+// Roles: two softmax warpgroups (thread = row), four converting warps (pages by
+// cp.async into the half of a stage that is converted last), an issuing warp per row
+// tile; two warps idle so that the registers split evenly.  Every role finds the CTA's
+// segments by itself; rings and barriers run on over them.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <string>
+#include <type_traits>
+
+#include "cache_mma.cuh"
+#include "chunk.h"
+#include "pkv_internal.h"
+
+namespace pkv {
+namespace {
+
+constexpr int kTileRows = 128;
+constexpr int kUnitRows = 256;
+constexpr int kKeys = 128;
+constexpr int kThreads = 512;
+constexpr int kConvWarp = 8, kMmaWarp = 12, kIdleWarp = 14;
+constexpr int kEarly = 4;      // MMAs left of a step when the turn is passed on
+constexpr int kOver = 3;       // tiles that a unit's start and end cost
+constexpr int kLeast = 6;      // places of a CTA's share
+// A row's maximum moves when a tile exceeds it by more than 2^kLazy, and p is kept times
+// 2^kPShift: at most 2^15 in fp16.
+constexpr float kLazy = 2.0f;
+constexpr float kPShift = 13.0f;
+
+template <int DP, int HALVES>
+struct TcCfg {
+  static constexpr int kTileBytes = kKeys * DP * 2;
+  static constexpr int kStages = DP == 128 ? (HALVES == 1 ? 4 : 3) : 6;
+  // Scales of a tile are reused by tile j + kSlots.  They are written after the copies of
+  // tile j were started, which waits for stages that P V (j - 2) frees (3 or 4 stages), or
+  // P V (j - 3) (6 stages).
+  static constexpr int kSlots = DP == 128 ? 2 : 4;
+  // The tensor cores cut off the bits that an fp32 sum cannot hold (8e-7 of a tile's sum
+  // of one sign): every so many tiles O is added to a sum of its own, rounded to nearest,
+  // and started anew.  16-bit results take it every 16,384 keys as prefill.cu's.
+  static constexpr int kFlush = HALVES == 2 ? 5 : 128;
+  static constexpr int kOffQ = 0;  // [row tile][hi, lo]; results leave through them
+  static constexpr int kOffKV = 2 * HALVES * kTileBytes;
+  static constexpr int kOffScale = kOffKV + kStages * kTileBytes;  // [slot][k, v][128]
+  static constexpr int kOffMask = kOffScale + kSlots * 2 * kKeys * 4;
+  static constexpr int kOffMax = kOffMask + kSlots * 16;  // [slot][converting warp]
+  // (base, l) of the rows of a row tile: behind the results in its query tile, or apart
+  static constexpr int kOffMl = DP == 128 ? kOffQ + 16384 : kOffMax + kSlots * 16;
+  static constexpr int kMlPitch = DP == 128 ? HALVES * kTileBytes : kTileRows * 8;
+  static constexpr int kOffBar = kOffMax + kSlots * 16 + (DP == 128 ? 0 : 2 * kTileRows * 8);
+  static constexpr int kBars = 2 * kStages + kSlots + 2 + 2 + 4 + 2 + 2 + 1;
+  static constexpr int kOffMisc = kOffBar + kBars * 8;
+  static constexpr int kSmemBytes = kOffMisc + 16;
+  static constexpr int kOCol = 256;
+  // 512 registers x 128: softmax and the others
+  static constexpr int kSoftRegs = 184, kOtherRegs = 72;
+  static_assert(kSmemBytes <= 227 * 1024, "shared memory");
+  static_assert(256 * (kSoftRegs + kOtherRegs) <= 65536, "registers");
+};
+
+struct TcParams {
+  const void* q;
+  const int8_t* k_cache;
+  const float* k_scale;
+  const int8_t* v_cache;
+  const float* v_scale;
+  const int32_t* tables;
+  void* out;
+  float* lse;  // nullable
+  const PlanHead* head;
+  const PlanSeq* seq;
+  uint8_t* slots;  // per CTA two: of the unit that it begins with, and that it ends with
+  float4* sums;    // per CTA and row tile: [DP / 4][128 rows], O of earlier tiles
+  int64_t q_tok, q_head;
+  int64_t num_blocks;
+  int seqs, total_q, heads, kv_heads, group, dim, bs, width;
+  int ctas;
+  int zero_rows;   // this kernel is the one that zeroes rows outside all sequences
+  float qk_scale;  // sm_scale log2e
+};
+
+template <int DP>
+struct TcSlot {
+  static constexpr int kMl = kUnitRows * DP * 4;
+  static constexpr int kBytes = kMl + kUnitRows * 8;
+};
+
+__device__ __forceinline__ int64_t tc_share(const TcParams& p) {
+  return max((p.head->places + p.ctas - 1) / p.ctas, (int64_t)kLeast);
+}
+
+// A unit, and the part of it that a CTA has.
+struct TcUnit {
+  PlanSeq seq;
+  int s, kvh, block, rows;
+  int64_t at;          // first place
+  int cta0, parts;
+  int tile0, n;        // the CTA's tiles of it
+  int tiles[2];        // of each row tile, from tile0 on
+  bool dual;           // the row tiles share the rows, and the tiles in turns
+
+  __device__ __forceinline__ void find(const TcParams& p, int64_t place, int64_t share) {
+    int unit;
+    for (;;) {  // (sequences that are not this kernel's have no places)
+      seq = p.seq[s];
+      unit = (int)((place - seq.first) / (seq.steps + kOver));
+      const int64_t next = s + 1 < p.seqs ? p.seq[s + 1].first : p.head->places;
+      if (place < next) break;
+      ++s;
+    }
+    at = seq.first + (int64_t)unit * (seq.steps + kOver);
+    kvh = unit % p.kv_heads;
+    block = unit / p.kv_heads;
+    rows = (int)min((int64_t)kUnitRows, seq.lq * (int64_t)p.group - (int64_t)block * kUnitRows);
+    cta0 = (int)((at + kOver) / share);
+    parts = (int)((at + kOver + seq.steps - 1) / share) - cta0 + 1;
+    dual = rows <= kTileRows && seq.steps > 1;
+  }
+  __device__ __forceinline__ void cut(const TcParams& p, int64_t now, int64_t stop) {
+    tile0 = (int)max(now - at - kOver, (int64_t)0);
+    const int end = (int)max(min((int64_t)seq.steps, stop - at - kOver), (int64_t)tile0);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int last = min((x + 1) * kTileRows, rows) - 1;
+      const int keys = last >= x * kTileRows || dual ? max(limit(p, min(last, rows - 1)), 0) : 0;
+      tiles[x] = max(min((keys + kKeys - 1) / kKeys, end) - tile0, 0);
+    }
+    n = max(tiles[0], tiles[1]);
+  }
+  __device__ __forceinline__ bool empty(int64_t stop) const { return stop <= at + kOver; }
+  // the keys that row r sees
+  __device__ __forceinline__ int limit(const TcParams& p, int r) const {
+    return r < rows ? min((int)((block * (int64_t)kUnitRows + r) / p.group) + 1 + seq.len - seq.lq,
+                          seq.len)
+                    : 0;
+  }
+  __device__ __forceinline__ int64_t token(const TcParams& p, int r, int* head) const {
+    const int64_t i = block * (int64_t)kUnitRows + r;
+    const int tok = (int)(i / p.group);
+    *head = kvh * p.group + (int)(i - (int64_t)tok * p.group);
+    return seq.q0 + tok;
+  }
+  template <int BYTES>
+  __device__ __forceinline__ uint8_t* slot(const TcParams& p, int part) const {
+    return p.slots + (int64_t)(2 * (cta0 + part) + (part == 0 ? 1 : 0)) * BYTES;
+  }
+};
+
+__device__ __forceinline__ float load_if(bool on, const float* p) {
+  float v;
+  asm volatile(
+      "{\n\t.reg .pred on;\n\tsetp.ne.u32 on, %2, 0;\n\tmov.f32 %0, 0f00000000;\n\t"
+      "@on ld.global.nc.f32 %0, [%1];\n\t}"
+      : "=&f"(v)
+      : "l"(p), "r"((uint32_t)on));
+  return v;
+}
+
+template <typename T, int DP, int HALVES>
+__global__ void __launch_bounds__(kThreads, 1) chunk_tc_kernel(const TcParams p, int* err) {
+  using C = TcCfg<DP, HALVES>;
+  using S = TcSlot<DP>;
+  constexpr int kStages = C::kStages, kSlots = C::kSlots;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  float* s_scale = reinterpret_cast<float*>(smem + C::kOffScale);
+  uint32_t* s_mask = reinterpret_cast<uint32_t*>(smem + C::kOffMask);
+  float* s_max = reinterpret_cast<float*>(smem + C::kOffMax);
+  const auto s_ml = [&](int x) { return reinterpret_cast<float2*>(smem + C::kOffMl + x * C::kMlPitch); };
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* kv_empty = kv_full + kStages;
+  uint64_t* sc_full = kv_empty + kStages;
+  uint64_t* q_full = sc_full + kSlots;  // per row tile, as the next three
+  uint64_t* s_full = q_full + 2;
+  uint64_t* p_full = s_full + 2;  // [row tile][half of the tokens]
+  uint64_t* o_full = p_full + 4;
+  uint64_t* turn = o_full + 2;
+  uint64_t* mma_done = turn + 2;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const PlanHead head = *p.head;
+  const int64_t share = tc_share(p);
+  const int64_t begin = blockIdx.x * share, stop = min(begin + share, head.places);
+  // rows in front of the first and behind the last sequence become zero
+  if (p.zero_rows) {
+    const int64_t front = (int64_t)head.q_begin * p.heads;
+    const int64_t behind = (int64_t)head.q_end * p.heads;
+    const int64_t outside = front + (int64_t)p.total_q * p.heads - behind;
+    for (int64_t i = blockIdx.x * (kThreads / 32) + warp; i < outside; i += gridDim.x * (kThreads / 32)) {
+      const int64_t r = i < front ? i : behind + i - front;
+      for (int c = lane * 4; c < p.dim; c += 128)
+        store4(static_cast<T*>(p.out) + r * p.dim + c, make_float4(0, 0, 0, 0));
+      if (lane == 0 && p.lse != nullptr) p.lse[r] = -INFINITY;
+    }
+  }
+  if (begin >= stop) return;
+
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&kv_full[i], 128);
+      mbar_init(&kv_empty[i], 2);
+    }
+    for (int i = 0; i < kSlots; ++i) mbar_init(&sc_full[i], 128);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 128);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[2 * i], 128);
+      mbar_init(&p_full[2 * i + 1], 128);
+      mbar_init(&o_full[i], 1);
+      mbar_init(&turn[i], 1);
+    }
+    mbar_init(mma_done, 2);
+    mbar_fence_init();
+  }
+  if (warp == kMmaWarp) tmem_alloc(s_tmem, 512);
+  tmem_fence_before_sync();
+  __syncthreads();
+  tmem_fence_after_sync();
+  const uint32_t tmem = *s_tmem;
+  // ok: false in a thread whose wait gave up (bounded; then every wait of the grid gives
+  // up at once).  It goes on without waiting and without storing results.
+  bool ok = true;
+  const auto wait = [&](uint64_t* bar, int phase) {
+    if (ok && !mbar_wait_short(bar, (uint32_t)phase & 1u, err)) {
+      record_error(err, kDevWaitTimeout);
+      ok = false;
+    }
+  };
+  int tiles_before = 0;  // of the CTA's earlier segments
+
+  if (warp >= kConvWarp) {
+    registers_down<C::kOtherRegs>();
+    if (warp < kMmaWarp) {
+      // ---- pages to fp16 tiles ---------------------------------------------------------
+      constexpr int kLanes = DP / 16;      // 16-byte pieces of a token row
+      constexpr int kStep = 128 / kLanes;  // token rows per pass
+      constexpr int kPass = kKeys / kStep;
+      // With three stages the next K waits for V (j - 1)'s, and V (j) is not to wait for
+      // that: both copies are started after both conversions.  Else each after its own.
+      constexpr bool kBetween = kStages > 3;
+      const int ct = tid - kConvWarp * 32;
+      const int piece = ct % kLanes, row0 = ct / kLanes;
+      const uint32_t row_bytes = (uint32_t)(p.kv_heads * p.dim);
+      const bool in_dim = piece * 16 < p.dim;
+      constexpr uint32_t kNoRow = 0xffffffffu;  // no token, or a page outside the cache
+      const auto stage_of = [&](int i) { return smem + C::kOffKV + (i % kStages) * C::kTileBytes; };
+      TcUnit u;
+      u.s = plan_find(p.seq, p.seqs, begin);
+      for (int64_t now = begin; now < stop; now = u.at + u.seq.steps + kOver) {
+        u.find(p, now, share);
+        if (u.empty(stop)) continue;
+        u.cut(p, now, stop);
+        const int n = u.n, len = u.seq.len;
+        const int32_t* table = p.tables + (int64_t)u.s * p.width;
+        const int last_page = (len - 1) / p.bs;
+        // A tile's 8 groups of 16 tokens are on one page each, found a tile ahead by the
+        // lanes (lane & 7 = group) and handed on by shuffle.
+        uint32_t at = kNoRow;
+        int entry = 0, rem = 0;
+        float ks = 0.0f, vs = 0.0f;
+        bool good = false;
+        const auto look_up = [&](int j) {
+          const int token = (u.tile0 + j) * kKeys + (lane & 7) * 16;
+          const int page = token / p.bs;
+          rem = token - page * p.bs;
+          entry = table[min(page, last_page)];  // past the end the last page again
+        };
+        const auto issue = [&](int j, int kind) {
+          if (j < n) {
+            if (kind == 0) {
+              const int phys = __shfl_sync(0xffffffffu, entry, ct / 16);
+              const bool counts = (u.tile0 + j) * kKeys + ct < len;
+              good = counts && phys >= 0 && (int64_t)phys < p.num_blocks;
+              if (counts && !good) record_error(err, kDevBadBlockId);
+              ks = load_if(good, p.k_scale + (int64_t)phys * p.kv_heads + u.kvh);
+              vs = load_if(good, p.v_scale + (int64_t)phys * p.kv_heads + u.kvh);
+              const bool in = (u.tile0 + j) * kKeys + (lane & 7) * 16 < len && entry >= 0 &&
+                              (int64_t)entry < p.num_blocks;
+              at = in ? (uint32_t)entry * p.bs + rem : kNoRow;
+              if (j + 1 < n) look_up(j + 1);
+            }
+            const int i = 2 * (tiles_before + j) + kind;
+            wait(&kv_empty[i % kStages], i / kStages + 1);
+            const int8_t* base = (kind ? p.v_cache : p.k_cache) + (int64_t)u.kvh * p.dim + piece * 16;
+            const uint32_t dst = smem_u32(stage_of(i)) + C::kTileBytes / 2 + ct * 16;
+#pragma unroll
+            for (int r = 0; r < kPass; ++r) {
+              const uint32_t row = __shfl_sync(0xffffffffu, at, r * kStep / 16 + row0 / 16);
+              const bool on = row != kNoRow && in_dim;
+              // (rows past the length on its last page are read: any codes will do)
+              const uint64_t from =
+                  (uint64_t)(on ? row + (r * kStep + row0) % 16 : 0) * row_bytes;
+              copy16_if(on, dst + r * 2048, base + (on ? from : 0));
+            }
+          }
+          copies_commit();
+        };
+        if (n > 0) look_up(0);
+        issue(0, 0);
+        issue(0, 1);
+        for (int j = 0; j < n; ++j) {
+#pragma unroll
+          for (int kind = 0; kind < 2; ++kind) {
+            const int i = 2 * (tiles_before + j) + kind;
+            if (kind == 0) {  // the tile's scales and which of its tokens count
+              const int slot = (tiles_before + j) % kSlots;
+              s_scale[(slot * 2) * kKeys + ct] = ks * p.qk_scale;
+              s_scale[(slot * 2 + 1) * kKeys + ct] = vs;
+              const unsigned m = __ballot_sync(0xffffffffu, good);
+              const float a = fabsf(vs);
+              const uint32_t big = __reduce_max_sync(0xffffffffu, a <= 3.0e38f ? __float_as_uint(a) : 0u);
+              if (lane == 0) {
+                s_mask[slot * 4 + (ct >> 5)] = m;
+                s_max[slot * 4 + (ct >> 5)] = __uint_as_float(big);
+              }
+              mbar_arrive(&sc_full[slot]);
+            }
+            if (kind == 0 || kBetween) copies_wait<1>();
+            else copies_wait<0>();
+            uint4 raw[kPass];
+#pragma unroll
+            for (int r = 0; r < kPass; ++r)
+              raw[r] = *reinterpret_cast<const uint4*>(stage_of(i) + C::kTileBytes / 2 + (r * 128 + ct) * 16);
+            named_barrier(1, 128);  // every code is read
+            uint8_t* tile = stage_of(i) + (piece / 4) * (kKeys * 128);
+            const uint32_t off = sw128_offset(row0, (piece % 4) * 32);
+            const uint32_t off16 = sw128_offset(row0, (piece % 4) * 32 + 16);
+#pragma unroll
+            for (int r = 0; r < kPass; ++r) {  // (kStep % 8 = 0: one swizzle for all)
+              const uint4 w = raw[r];
+              const uint2 a = codes_to_half(w.x), b = codes_to_half(w.y), c = codes_to_half(w.z),
+                          d = codes_to_half(w.w);
+              *reinterpret_cast<uint4*>(tile + off + r * kStep * 128) = make_uint4(a.x, a.y, b.x, b.y);
+              *reinterpret_cast<uint4*>(tile + off16 + r * kStep * 128) =
+                  make_uint4(c.x, c.y, d.x, d.y);
+            }
+            fence_proxy_async_smem();  // an MMA operand
+            mbar_arrive(&kv_full[i % kStages]);
+            if (kBetween) issue(j + 1, kind);
+          }
+          if (!kBetween) {
+            issue(j + 1, 0);
+            issue(j + 1, 1);
+          }
+        }
+        tiles_before += n;
+      }
+      copies_wait<0>();
+      if (ct == 0) drain_ring(kv_empty, kStages, 2 * tiles_before);  // no release outlives the CTA
+    } else if (warp < kIdleWarp) {
+      // ---- MMA issue: a warp for each row tile, in strict turns (see prefill.cu) ---------
+      constexpr uint32_t kIdQK = umma_f16_idesc(0, 0, kTileRows, kKeys);
+      constexpr uint32_t kIdPV = umma_f16_idesc(0, 1, kTileRows, DP);
+      const int x = warp - kMmaWarp;
+      const uint32_t kv = smem_u32(smem + C::kOffKV);
+      const uint64_t q_desc =
+          umma_sw128_desc(smem_u32(smem + C::kOffQ + x * HALVES * C::kTileBytes), 16, 1024);
+      const uint64_t k_desc = umma_sw128_desc(kv, 16, 1024);
+      const uint64_t v_desc = umma_sw128_desc(kv, kKeys * 128, 1024);
+      const uint32_t s_col = tmem + x * 128, o_col = tmem + C::kOCol + x * 128;
+      // a warp's lanes give up together
+      const auto wait_warp = [&](uint64_t* bar, int phase) {
+        wait(bar, phase);
+        ok = __all_sync(0xffffffffu, ok);
+      };
+      const auto item = [&](int i) { return 2 * tiles_before + i; };
+      const auto wait_load = [&](int i) { wait_warp(&kv_full[item(i) % kStages], item(i) / kStages); };
+      const auto stage_at = [&](int i) { return (uint32_t)(item(i) % kStages) * C::kTileBytes; };
+      // both warps release a stage, each after it saw the load
+      const auto release = [&](int i) { umma_commit_warp(&kv_empty[item(i) % kStages]); };
+      const auto pass_over = [&](int i) {
+        if (lane == 0) mbar_arrive(&kv_empty[item(i) % kStages]);
+        __syncwarp();
+      };
+      const auto pass_turn = [&]() {
+        if (lane == 0) mbar_arrive(&turn[x ^ 1]);
+        __syncwarp();
+      };
+      const auto qk = [&](int j, bool pass) {
+        const uint64_t b = umma_desc_at(k_desc, stage_at(2 * j));
+#pragma unroll
+        for (int half = HALVES - 1; half >= 0; --half) {  // lo first: roundings of a small sum
+          const uint64_t a = umma_desc_at(q_desc, (uint32_t)half * C::kTileBytes);
+#pragma unroll
+          for (int kk = 0; kk < DP / 16; ++kk) {
+            const uint32_t off = (uint32_t)(kk / 4) * (kKeys * 128) + (uint32_t)(kk % 4) * 32;
+            umma_f16_warp(s_col, umma_desc_at(a, off), umma_desc_at(b, off), kIdQK,
+                          (half < HALVES - 1 || kk > 0) ? 1u : 0u);
+            if (half == 0 && kk == DP / 16 - kEarly && pass) pass_turn();
+          }
+        }
+        umma_commit_warp(&s_full[x]);
+      };
+      int q_uses = 0, p_uses = 0, steps = 0;
+      // c: how many tiles this row tile has had
+      const auto pv = [&](int j, int c) {
+        const uint64_t b = umma_desc_at(v_desc, stage_at(2 * j + 1));
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 16; ++kk) {
+          if (kk == kKeys / 32) {
+            wait_warp(&p_full[2 * x + 1], p_uses);
+            tmem_fence_after_sync();
+            if (!ok) return;
+          }
+          // P of tokens 32 i .. 32 i + 31 is in columns 32 i: hi in 16, lo in 16; or
+          // (16 bits) of token t in columns t / 2
+#pragma unroll
+          for (int half = 0; half < HALVES; ++half) {
+            const uint32_t a =
+                HALVES == 2 ? s_col + (kk / 2) * 32 + half * 16 + (kk % 2) * 8 : s_col + kk * 8;
+            umma_f16_ta_warp(o_col, a, umma_desc_at(b, kk * 2048), kIdPV,
+                             (c % C::kFlush > 0 || kk > 0 || half > 0) ? 1u : 0u);
+          }
+        }
+        ++p_uses;
+      };
+      TcUnit u;
+      u.s = plan_find(p.seq, p.seqs, begin);
+      for (int64_t now = begin; now < stop && ok; now = u.at + u.seq.steps + kOver) {
+        u.find(p, now, share);
+        if (u.empty(stop)) continue;
+        u.cut(p, now, stop);
+        const int n = u.n, nt = x ? u.tiles[1] : u.tiles[0];
+        if (n == 0) continue;
+        if (u.dual) {
+          // this warp's tiles are x, x + 2, ...
+          if (x < n) wait_warp(&q_full[x], q_uses++);
+          for (int j = 0; j < n && ok; ++j) {
+            wait_load(2 * j);
+            if (!ok) break;
+            if ((j & 1) != x) {
+              pass_over(2 * j);
+              wait_load(2 * j + 1);
+              pass_over(2 * j + 1);
+              continue;
+            }
+            tmem_fence_after_sync();
+            qk(j, false);
+            release(2 * j);
+            wait_load(2 * j + 1);
+            wait_warp(&p_full[2 * x], p_uses);
+            tmem_fence_after_sync();
+            if (!ok) break;
+            pv(j, j / 2);
+            if (!ok) break;
+            if (j + 2 >= n) umma_commit_warp(&o_full[x]);
+            release(2 * j + 1);
+          }
+        } else {
+          wait_load(0);
+          if (nt > 0) {
+            wait_warp(&q_full[x], q_uses++);
+            tmem_fence_after_sync();
+            if (ok) qk(0, false);
+          }
+          release(0);
+          for (int j = 0; j < n && ok; ++j, ++steps) {
+            wait_load(2 * j + 1);
+            if (j + 1 < n) wait_load(2 * j + 2);
+            if (x == 1 || steps > 0) wait_warp(&turn[x], x == 1 ? steps : steps - 1);
+            if (j < nt) wait_warp(&p_full[2 * x], p_uses);
+            tmem_fence_after_sync();
+            if (!ok) break;
+            if (j < nt) {
+              pv(j, j);
+              if (!ok) break;
+              if (j == nt - 1) umma_commit_warp(&o_full[x]);
+              if (j + 1 < nt) qk(j + 1, true);  // over P (j): a warp's MMAs run in order
+              else pass_turn();
+            } else {
+              pass_turn();
+            }
+            release(2 * j + 1);
+            if (j + 1 < n) release(2 * j + 2);
+          }
+        }
+        tiles_before += n;
+      }
+      umma_commit_warp(mma_done);
+      mbar_drain(mma_done, 0);  // every MMA is done before tensor memory is freed
+    }
+  } else {
+    registers_up<C::kSoftRegs>();
+    // ---- query split, softmax, results: thread = row --------------------------------------
+    const int x = warp >> 2, row = tid & 127;
+    const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+    const uint32_t s_addr = tmem + lanes + x * 128, o_addr = tmem + lanes + C::kOCol + x * 128;
+    const uint32_t o2_addr = o_addr + 64;  // DP = 64: O of earlier tiles
+    float4* sums = p.sums + ((int64_t)blockIdx.x * 2 + x) * (DP / 4) * kTileRows + row;
+    uint8_t* q_tile = smem + C::kOffQ + x * HALVES * C::kTileBytes;
+    const auto meet = [&]() { named_barrier(2 + x, 128); };
+    int s_uses = 0, o_uses = 0;
+    TcUnit u;
+    u.s = plan_find(p.seq, p.seqs, begin);
+    for (int64_t now = begin; now < stop; now = u.at + u.seq.steps + kOver) {
+      u.find(p, now, share);
+      if (u.empty(stop)) continue;
+      u.cut(p, now, stop);
+      const bool dual = u.dual;
+      const int first = dual ? x : 0, by = dual ? 2 : 1;
+      const int nt = dual ? u.n : (x ? u.tiles[1] : u.tiles[0]);  // its tiles: first, first + by, ... < nt
+      const int r0 = dual ? 0 : x * kTileRows;
+      const int r = r0 + row;
+      const bool valid = r < u.rows;
+      const int limit = u.limit(p, r);
+      const bool busy = r - lane < u.rows;  // warps without rows only keep the hand-offs going
+      // tiles from here on hold keys that some row of the warp does not see
+      const int first_masked = max(u.limit(p, r - lane), 0) / kKeys - u.tile0;
+      float rf = 1.0f;  // power of two that the row was divided by
+      if (first < nt) {
+        // The warp takes its 32 rows one after the other, a lane per 4 channels.  A row's
+        // largest magnitude is scaled to [2^10, 2^11): exact, and lo's steps stay far
+        // below hi's.  (fp16 queries are as they are.)
+        const int base = r - lane;
+#pragma unroll 1
+        for (int i0 = 0; i0 < 32; i0 += 8) {
+          float4 rowv[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {  // all loads first
+            rowv[e] = make_float4(0, 0, 0, 0);
+            if (base + i0 + e < u.rows && lane * 4 < p.dim) {
+              int h;
+              const int64_t tok = u.token(p, base + i0 + e, &h);
+              rowv[e] = load4(static_cast<const T*>(p.q) + tok * p.q_tok + h * p.q_head + lane * 4);
+            }
+          }
+#pragma unroll
+          for (int e8 = 0; e8 < 8; ++e8) {
+            const int i = i0 + e8;
+            const float4 v = rowv[e8];
+            float up = 1.0f;
+            if constexpr (!std::is_same<T, __half>::value) {
+              float big = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+              big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
+              const int e = row_exponent(big);
+              up = power_of_two(e);
+              if (lane == i) rf = power_of_two(-e);
+            }
+            const float f[4] = {v.x * up, v.y * up, v.z * up, v.w * up};
+            uint32_t hi[2], lo[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const __half2 h = __floats2half2_rn(f[2 * e], f[2 * e + 1]);
+              hi[e] = word_of(h);
+              if constexpr (HALVES == 2) {
+                const float2 b = __half22float2(h);
+                lo[e] = word_of(__floats2half2_rn(f[2 * e] - b.x, f[2 * e + 1] - b.y));
+              }
+            }
+            if (lane * 4 < DP) {
+              const uint32_t off = (lane / 16) * (kTileRows * 128) +
+                                   sw128_offset((warp & 3) * 32 + i, (lane % 16) * 8);
+              *reinterpret_cast<uint2*>(q_tile + off) = make_uint2(hi[0], hi[1]);
+              if constexpr (HALVES == 2)
+                *reinterpret_cast<uint2*>(q_tile + C::kTileBytes + off) = make_uint2(lo[0], lo[1]);
+            }
+          }
+        }
+        fence_proxy_async_smem();  // an MMA operand
+        mbar_arrive(&q_full[x]);
+      }
+      float since = 1.0f;  // by what O's unit has changed since the sum was written
+      float m = -INFINITY, l = 0.0f;  // m in units of S * k_scale * qk_scale
+      float unit_v = 0.0f, inv_v = 0.0f;  // a power of two above the V scales so far: O's unit
+      int c_tile = 0;  // tiles so far
+      for (int j = first; j < nt; j += by, ++c_tile) {
+        const int jj = tiles_before + j, slot = jj % kSlots;
+        wait(&sc_full[slot], jj / kSlots);
+        wait(&s_full[x], s_uses++);
+        __syncwarp();
+        tmem_fence_after_sync();
+        if (!busy) {
+          mbar_arrive(&p_full[2 * x]);
+          mbar_arrive(&p_full[2 * x + 1]);
+          continue;
+        }
+        if (c_tile > 0 && c_tile % C::kFlush == 0) {  // O has the products of all earlier tiles
+#pragma unroll 1
+          for (int c = 0; c < DP; c += 16) {
+            alignas(16) uint32_t o[16], was[16];
+            tmem_load<16>(o_addr + c, o);
+            if (c_tile == C::kFlush) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) was[e] = 0u;
+            } else if (DP == 64) {
+              tmem_load<16>(o2_addr + c, was);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                *reinterpret_cast<float4*>(&was[4 * e]) = sums[(c / 4 + e) * kTileRows];
+            }
+            tmem_wait_load();
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              o[e] = __float_as_uint(fmaf(__uint_as_float(was[e]), since, __uint_as_float(o[e])));
+            if (DP == 64) {
+              tmem_store<16>(o2_addr + c, o);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                sums[(c / 4 + e) * kTileRows] = *reinterpret_cast<const float4*>(&o[4 * e]);
+            }
+          }
+          tmem_wait_store();
+          since = 1.0f;
+        }
+        const float* ks = s_scale + slot * 2 * kKeys;
+        const float* vs = ks + kKeys;
+        const uint4 mask = *reinterpret_cast<const uint4*>(s_mask + slot * 4);
+        const float4 vm = *reinterpret_cast<const float4*>(s_max + slot * 4);
+        const bool masked =
+            (mask.x & mask.y & mask.z & mask.w) != 0xffffffffu || j >= first_masked;
+        float s[kKeys];
+        {
+          uint32_t(&w)[kKeys] = reinterpret_cast<uint32_t(&)[kKeys]>(s);
+#pragma unroll
+          for (int c = 0; c < kKeys; c += 32)
+            tmem_load<32>(s_addr + c, reinterpret_cast<uint32_t(&)[32]>(w[c]));
+          tmem_wait_load();
+        }
+#pragma unroll
+        for (int c = 0; c < kKeys; c += 16) {  // 16 tokens share their scale
+          const float k = ks[c];
+          const uint64_t k2 = f32x2(k, k);
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            const float2 y = unpack_f32x2(mul_f32x2(f32x2(s[c + e], s[c + e + 1]), k2));
+            s[c + e] = y.x;
+            s[c + e + 1] = y.y;
+          }
+        }
+        const int seen = limit - (u.tile0 + j) * kKeys;  // columns below this are seen
+        if (masked) {
+#pragma unroll
+          for (int c = 0; c < kKeys; ++c) {
+            const uint32_t w = c < 32 ? mask.x : c < 64 ? mask.y : c < 96 ? mask.z : mask.w;
+            s[c] = c < seen && (w >> (c & 31) & 1u) ? s[c] : -INFINITY;
+          }
+        }
+        float tm[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) tm[e] = s[e];
+#pragma unroll
+        for (int c = 8; c < kKeys - 8; c += 16)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) tm[e] = max3_nan(tm[e], s[c + e], s[c + e + 8]);
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) tm[e] = max3_nan(tm[e], tm[e + 1], s[kKeys - 8 + e]);
+        const float t = max3_nan(
+            max3_nan(tm[0], tm[2], s[kKeys - 7]), max3_nan(tm[4], tm[6], s[kKeys - 5]),
+            max3_nan(s[kKeys - 3], s[kKeys - 1], tm[0]));
+        const bool move = valid && t > m && (m == -INFINITY || (t - m) * rf > kLazy);
+        const float big = fmaxf(fmaxf(vm.x, vm.y), fmaxf(vm.z, vm.w));
+        if (__any_sync(0xffffffffu, move || big > unit_v)) {
+          float alpha = move ? (m == -INFINITY ? 0.0f : ex2((m - t) * rf)) : 1.0f;
+          if (move) m = t;
+          l *= alpha;
+          if (big > unit_v) {  // (the same in all threads)
+            const int e = min(max((int)(__float_as_uint(big) >> 23) - 126, -126), 126);
+            const float unit_now = power_of_two(e);
+            inv_v = power_of_two(-e);
+            alpha *= unit_v * inv_v;
+            unit_v = unit_now;
+          }
+          since *= alpha;
+          if (c_tile % C::kFlush != 0) {
+#pragma unroll 1
+            for (int c = 0; c < DP; c += 16) {
+              uint32_t o[16];
+              tmem_load<16>(o_addr + c, o);
+              tmem_wait_load();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_store<16>(o_addr + c, o);
+            }
+          }
+        }
+        // a NaN score makes the whole row NaN
+        const float ms = t != t ? t : (m == -INFINITY ? 0.0f : m * rf) - kPShift;
+        const uint64_t rf2 = f32x2(rf, rf), ms2 = f32x2(-ms, -ms);
+        uint64_t sum[2] = {0, 0};
+#pragma unroll
+        for (int c = 0; c < kKeys; c += 32) {
+          uint32_t hi[16], lo[HALVES == 2 ? 16 : 1];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float g = vs[c + (e & 16)] * inv_v;
+            float2 z = unpack_f32x2(fma_f32x2(f32x2(s[c + e], s[c + e + 1]), rf2, ms2));
+            z.x = ex2(z.x);
+            z.y = ex2(z.y);
+            const uint64_t pr = f32x2(z.x, z.y);
+            sum[(e / 2) & 1] = add_f32x2(sum[(e / 2) & 1], pr);
+            const uint64_t pv = mul_f32x2(pr, f32x2(g, g));
+            float2 f = unpack_f32x2(pv);
+            if (masked) {  // (a V scale that is not finite does not reach rows in front)
+              if (s[c + e] == -INFINITY) f.x = 0.0f;
+              if (s[c + e + 1] == -INFINITY) f.y = 0.0f;
+            }
+            const __half2 h = __floats2half2_rn(f.x, f.y);
+            hi[e / 2] = word_of(h);
+            if constexpr (HALVES == 2) {
+              const float2 b = __half22float2(h);
+              lo[e / 2] = word_of(__floats2half2_rn(f.x - b.x, f.y - b.y));
+            }
+          }
+          if constexpr (HALVES == 2) {
+            tmem_store<16>(s_addr + c, hi);
+            tmem_store<16>(s_addr + c + 16, lo);
+          } else {
+            tmem_store<16>(s_addr + c / 2, hi);
+          }
+          if (c == 32 || c == 96) {  // half of P is there: its product can start
+            tmem_wait_store();
+            tmem_fence_before_sync();
+            mbar_arrive(&p_full[2 * x + (c == 96)]);
+          }
+        }
+        const float2 l2 = unpack_f32x2(add_f32x2(sum[0], sum[1]));
+        l += l2.x + l2.y;
+      }
+      tiles_before += u.n;
+      const bool had = first < nt;
+      if (had) {
+        wait(&o_full[x], o_uses++);
+        __syncwarp();
+        tmem_fence_after_sync();
+      }
+      // ---- results ------------------------------------------------------------------
+      const bool flushed = c_tile > C::kFlush;
+      // 32 channels of the row's O, times by
+      const auto take = [&](int c, float by, float (&f)[32]) {
+        if (!had) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) f[e] = 0.0f;
+          return;
+        }
+        uint32_t o[32];
+        tmem_load<32>(o_addr + c, o);
+        tmem_wait_load();
+        if (flushed) {
+          alignas(16) uint32_t was[32];
+          if (DP == 64) {
+            tmem_load<32>(o2_addr + c, was);
+            tmem_wait_load();
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<float4*>(&was[4 * e]) = sums[(c / 4 + e) * kTileRows];
+          }
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            o[e] = __float_as_uint(fmaf(__uint_as_float(was[e]), since, __uint_as_float(o[e])));
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) f[e] = __uint_as_float(o[e]) * by;
+      };
+      // base such that O and l are sums of 2^(score - base)
+      float base = m == -INFINITY && l == l ? -INFINITY : (m == -INFINITY ? 0.0f : m * rf) - kPShift;
+      float mine = unit_v;  // what this thread's O is multiplied by
+      uint8_t* stage = smem + C::kOffQ + x * HALVES * C::kTileBytes;  // rows of 128 bytes, swizzled
+      uint8_t* other = smem + C::kOffQ + HALVES * C::kTileBytes;
+      if (dual) {  // the row's two halves meet in the first warpgroup
+        s_ml(x)[row] = make_float2(base, l);
+        named_barrier(4, 256);
+        const float2 a = s_ml(0)[row], b = s_ml(1)[row];
+        const float top = fmaxf(a.x, b.x);
+        const float fa = a.x == -INFINITY ? 0.0f : ex2(a.x - top);
+        const float fb = b.x == -INFINITY ? 0.0f : ex2(b.x - top);
+        mine *= x ? fb : fa;
+        if ((x ? b.x : a.x) == -INFINITY) mine = 0.0f;
+        base = top;
+        l = (a.x == -INFINITY ? 0.0f : a.y * fa) + (b.x == -INFINITY ? 0.0f : b.y * fb);
+      }
+      const bool whole = u.parts == 1;
+      const bool stores = !dual || x == 0;
+      const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+      uint8_t* slot = u.slot<S::kBytes>(p, (int)blockIdx.x - u.cta0);
+      const int rows = min(kTileRows, u.rows - r0);
+      // 32 channels at a time through shared memory, so that they leave in whole lines
+#pragma unroll 1
+      for (int c = 0; c < DP; c += 32) {
+        float f[32];
+        take(c, mine, f);
+        if (dual) {
+          if (x == 1) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<float4*>(other + row * 128 + ((e ^ (row & 7)) * 16)) =
+                  make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
+          }
+          named_barrier(4, 256);
+          if (x == 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float4 v = *reinterpret_cast<const float4*>(other + row * 128 + ((e ^ (row & 7)) * 16));
+              f[4 * e] += v.x, f[4 * e + 1] += v.y, f[4 * e + 2] += v.z, f[4 * e + 3] += v.w;
+            }
+          }
+          named_barrier(4, 256);
+        }
+        if (!stores) continue;
+        const bool none = whole && l == 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float k = whole ? inv : 1.0f;
+          *reinterpret_cast<float4*>(stage + row * 128 + ((e ^ (row & 7)) * 16)) =
+              none ? make_float4(0, 0, 0, 0)
+                   : make_float4(f[4 * e] * k, f[4 * e + 1] * k, f[4 * e + 2] * k, f[4 * e + 3] * k);
+        }
+        meet();
+        const int piece = row & 7, at = c + piece * 4;
+        if (ok && at < p.dim)
+          for (int i = row >> 3; i < rows; i += 16) {
+            const float4 v = *reinterpret_cast<const float4*>(stage + i * 128 + ((piece ^ (i & 7)) * 16));
+            if (whole) {
+              int h;
+              const int64_t tok = u.token(p, r0 + i, &h);
+              store4(static_cast<T*>(p.out) + (tok * p.heads + h) * p.dim + at, v);
+            } else {
+              *reinterpret_cast<float4*>(reinterpret_cast<float*>(slot) + (r0 + i) * DP + at) = v;
+            }
+          }
+        meet();  // the buffer is free
+      }
+      if (ok && valid && stores) {
+        if (whole) {
+          if (p.lse != nullptr) {
+            int h;
+            const int64_t tok = u.token(p, r, &h);
+            p.lse[tok * p.heads + h] =
+                l == 0.0f ? -INFINITY : (base + log2f(l)) * (1.0f / kLog2e);
+          }
+        } else {
+          reinterpret_cast<float2*>(slot + S::kMl)[r] = make_float2(base, l);
+        }
+      }
+    }
+  }
+  tmem_fence_before_sync();
+  __syncthreads();
+  if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
+}
+
+// Units that were cut: a warp per row, all parts in order.
+constexpr int kJoinRows = 32;  // of a CTA
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) join_tc_kernel(const TcParams p) {
+  using S = TcSlot<DP>;
+  constexpr int kBatch = 4;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t share = tc_share(p);
+  // the unit at the end of the CTA's share, if it begins there
+  const int64_t place = (int64_t)(blockIdx.x + 1) * share - 1;
+  if (place >= p.head->places) return;
+  TcUnit u;
+  u.s = plan_find(p.seq, p.seqs, place);
+  u.find(p, place, share);
+  if (u.cta0 != (int)blockIdx.x || u.parts == 1) return;
+  for (int r = blockIdx.y * kJoinRows + warp; r < min(u.rows, (int)(blockIdx.y + 1) * kJoinRows); r += 8) {
+    float m = -INFINITY, l = 0.0f;
+    float4 acc = make_float4(0, 0, 0, 0);
+    const bool in = lane * 4 < p.dim;
+    for (int i = 0; i < u.parts; i += kBatch) {
+      float2 ml[kBatch];
+      float4 v[kBatch];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const bool there = i + b < u.parts;
+        const uint8_t* from = u.slot<S::kBytes>(p, there ? i + b : i);
+        ml[b] = there ? __ldcg(reinterpret_cast<const float2*>(from + S::kMl) + r)
+                      : make_float2(-INFINITY, 0.0f);
+        v[b] = in ? __ldcg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(from) + r * DP + lane * 4))
+                  : make_float4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        if (ml[b].x == -INFINITY) continue;
+        const float big = fmaxf(m, ml[b].x);
+        const float f = m == -INFINITY ? 0.0f : ex2(m - big), k = ex2(ml[b].x - big);
+        m = big;
+        l = l * f + ml[b].y * k;
+        acc.x = acc.x * f + v[b].x * k, acc.y = acc.y * f + v[b].y * k;
+        acc.z = acc.z * f + v[b].z * k, acc.w = acc.w * f + v[b].w * k;
+      }
+    }
+    int h;
+    const int64_t tok = u.token(p, r, &h);
+    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    if (in)
+      store4(static_cast<T*>(p.out) + (tok * p.heads + h) * p.dim + lane * 4,
+             l == 0.0f ? make_float4(0, 0, 0, 0)
+                       : make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+    if (lane == 0 && p.lse != nullptr)
+      p.lse[tok * p.heads + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * (1.0f / kLog2e);
+  }
+}
+
+struct TcLayout {
+  size_t slots, sums, total;
+};
+
+TcLayout tc_layout(const ChunkArgs& a) {
+  const int dp = a.dim <= 64 ? 64 : 128;
+  const int64_t tiles = ((int64_t)a.width * a.block_size + kKeys - 1) / kKeys;
+  const int flush = a.dtype == 0 ? TcCfg<128, 2>::kFlush : TcCfg<128, 1>::kFlush;
+  TcLayout l;
+  size_t at = 0;
+  const auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  l.slots = take((size_t)2 * kChunkTcCtas * (dp == 64 ? TcSlot<64>::kBytes : TcSlot<128>::kBytes));
+  l.sums = take(dp == 128 && tiles > flush ? (size_t)kChunkTcCtas * 2 * kTileRows * dp * 4 : 0);
+  l.total = at;
+  return l;
+}
+
+template <typename T, int DP>
+int launch_tc(const ChunkArgs& a, PlanHead* head, PlanSeq* seq, uint8_t* ws, bool zero_rows,
+              cudaStream_t stream) {
+  constexpr int HALVES = sizeof(T) == 4 ? 2 : 1;
+  using C = TcCfg<DP, HALVES>;
+  const TcLayout lay = tc_layout(a);
+  TcParams p;
+  p.q = a.q;
+  p.k_cache = a.k_cache;
+  p.k_scale = a.k_scale;
+  p.v_cache = a.v_cache;
+  p.v_scale = a.v_scale;
+  p.tables = a.tables;
+  p.out = a.out;
+  p.lse = a.lse;
+  p.head = head;
+  p.seq = seq;
+  p.slots = ws + lay.slots;
+  p.sums = reinterpret_cast<float4*>(ws + lay.sums);
+  p.q_tok = a.q_token_stride;
+  p.q_head = a.q_head_stride;
+  p.num_blocks = a.num_blocks;
+  p.seqs = a.seqs;
+  p.total_q = (int)a.total_q;
+  p.heads = a.heads;
+  p.kv_heads = a.kv_heads;
+  p.group = a.heads / a.kv_heads;
+  p.dim = a.dim;
+  p.bs = a.block_size;
+  p.width = a.width;
+  p.qk_scale = a.sm_scale * kLog2e;
+  p.zero_rows = zero_rows ? 1 : 0;
+  // no more CTAs than have their least share of the longest that the batch can be
+  const int64_t units =
+      (a.total_q * p.group / kUnitRows + std::min<int64_t>(a.seqs, a.total_q) + 1) * a.kv_heads;
+  const int64_t steps = ((int64_t)a.width * a.block_size + kKeys - 1) / kKeys + 1 + kOver;
+  const int64_t ctas = std::min<int64_t>(
+      kChunkTcCtas, units >= (int64_t)kChunkTcCtas * kLeast ? kChunkTcCtas : (units * steps + kLeast - 1) / kLeast);
+  p.ctas = (int)ctas;
+  auto kern = chunk_tc_kernel<T, DP, HALVES>;
+  static std::atomic<uint64_t> done{0};
+  allow_shared_memory(reinterpret_cast<const void*>(kern), C::kSmemBytes, done);
+  kern<<<(unsigned)ctas, kThreads, C::kSmemBytes, stream>>>(p, device_error_word());
+  if (ctas > 1)
+    join_tc_kernel<T, DP><<<dim3((unsigned)ctas, kUnitRows / kJoinRows), 256, 0, stream>>>(p);
+  return kOk;
+}
+
+}  // namespace
+
+bool chunk_tc_takes(const ChunkArgs& a) {
+  return a.v_cache != nullptr && a.dim <= 128 && a.block_size % 16 == 0;
+}
+
+PlanArgs chunk_tc_plan(const PlanArgs& base) {
+  PlanArgs p = base;
+  p.rows = kUnitRows;
+  p.step = kKeys;
+  p.over = kOver;
+  p.counters = nullptr;
+  p.counts = 0;
+  return p;
+}
+
+size_t chunk_tc_workspace_size(const ChunkArgs& a) { return tc_layout(a).total; }
+
+int launch_chunk_tc(const ChunkArgs& a, PlanHead* head, PlanSeq* seq, uint8_t* ws, bool zero_rows,
+                    cudaStream_t stream) {
+  const auto with_dim = [&](auto t) {
+    using T = decltype(t);
+    return a.dim <= 64 ? launch_tc<T, 64>(a, head, seq, ws, zero_rows, stream)
+                       : launch_tc<T, 128>(a, head, seq, ws, zero_rows, stream);
+  };
+  return a.dtype == 0   ? with_dim(0.0f)
+         : a.dtype == 1 ? with_dim(__half())
+                        : with_dim(__nv_bfloat16());
+}
+
+}  // namespace pkv

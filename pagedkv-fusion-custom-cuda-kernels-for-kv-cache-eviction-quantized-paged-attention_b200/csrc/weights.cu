@@ -315,7 +315,7 @@ int launch_accumulate(const ChunkArgs& a, float* weights, void* workspace, size_
   plan.seq = reinterpret_cast<PlanSeq*>(ws + lay.seq);
   plan.counters = nullptr;
   plan.counts = 0;
-  const int rc = launch_plan(plan, err, stream);
+  const int rc = launch_plan(plan, nullptr, err, stream);
   if (rc != kOk) return rc;
   auto* sums = reinterpret_cast<unsigned long long*>(ws + lay.sums);
   const int64_t slots = (int64_t)a.seqs * a.width * a.block_size;
