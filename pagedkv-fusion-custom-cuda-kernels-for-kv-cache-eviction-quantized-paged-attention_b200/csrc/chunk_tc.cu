@@ -47,20 +47,17 @@ constexpr float kPShift = 13.0f;
 template <int DP, int HALVES>
 struct TcCfg {
   static constexpr int kTileBytes = kKeys * DP * 2;
-  static constexpr int kStages = DP == 128 ? (HALVES == 1 ? 4 : 3) : 6;
-  // Scales of a tile are reused by tile j + kSlots.  They are written after the copies of
-  // tile j were started, which waits for stages that P V (j - 2) frees (3 or 4 stages), or
-  // P V (j - 3) (6 stages).
-  static constexpr int kSlots = DP == 128 ? 2 : 4;
+  static constexpr int kStages = DP == 128 ? (HALVES == 1 ? 5 : 3) : 6;
+  static constexpr int kSlots = 4;  // scales of so many tiles: at most three are in flight
   // The tensor cores cut off the bits that an fp32 sum cannot hold (8e-7 of a tile's sum
   // of one sign): every so many tiles O is added to a sum of its own, rounded to nearest,
   // and started anew.  16-bit results take it every 16,384 keys as prefill.cu's.
   static constexpr int kFlush = HALVES == 2 ? 5 : 128;
   static constexpr int kOffQ = 0;  // [row tile][hi, lo]; results leave through them
   static constexpr int kOffKV = 2 * HALVES * kTileBytes;
-  static constexpr int kOffScale = kOffKV + kStages * kTileBytes;  // [slot][k, v][128]
-  static constexpr int kOffMask = kOffScale + kSlots * 2 * kKeys * 4;
-  static constexpr int kOffMax = kOffMask + kSlots * 16;  // [slot][converting warp]
+  static constexpr int kOffScale = kOffKV + kStages * kTileBytes;  // [slot][k, v][8 groups]
+  static constexpr int kOffMask = kOffScale + kSlots * 64;  // [slot][converting warp] bytes
+  static constexpr int kOffMax = kOffMask + kSlots * 4;     // [slot][converting warp]
   // (base, l) of the rows of a row tile: behind the results in its query tile, or apart
   static constexpr int kOffMl = DP == 128 ? kOffQ + 16384 : kOffMax + kSlots * 16;
   static constexpr int kMlPitch = DP == 128 ? HALVES * kTileBytes : kTileRows * 8;
@@ -147,14 +144,14 @@ struct TcUnit {
   __device__ __forceinline__ bool empty(int64_t stop) const { return stop <= at + kOver; }
   // the keys that row r sees
   __device__ __forceinline__ int limit(const TcParams& p, int r) const {
-    return r < rows ? min((int)((block * (int64_t)kUnitRows + r) / p.group) + 1 + seq.len - seq.lq,
+    return r < rows ? min((int)((uint32_t)(block * kUnitRows + r) / (uint32_t)p.group) + 1 + seq.len - seq.lq,
                           seq.len)
                     : 0;
   }
   __device__ __forceinline__ int64_t token(const TcParams& p, int r, int* head) const {
-    const int64_t i = block * (int64_t)kUnitRows + r;
-    const int tok = (int)(i / p.group);
-    *head = kvh * p.group + (int)(i - (int64_t)tok * p.group);
+    const uint32_t i = block * kUnitRows + r;  // (a call has less than 2^31 rows)
+    const uint32_t tok = i / (uint32_t)p.group;
+    *head = kvh * p.group + (int)(i - tok * (uint32_t)p.group);
     return seq.q0 + tok;
   }
   template <int BYTES>
@@ -180,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc_kernel(const TcParams p,
   constexpr int kStages = C::kStages, kSlots = C::kSlots;
   extern __shared__ __align__(1024) uint8_t smem[];
   float* s_scale = reinterpret_cast<float*>(smem + C::kOffScale);
-  uint32_t* s_mask = reinterpret_cast<uint32_t*>(smem + C::kOffMask);
+  uint8_t* s_mask = smem + C::kOffMask;
   float* s_max = reinterpret_cast<float*>(smem + C::kOffMax);
   const auto s_ml = [&](int x) { return reinterpret_cast<float2*>(smem + C::kOffMl + x * C::kMlPitch); };
   uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
@@ -286,11 +283,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc_kernel(const TcParams p,
           if (j < n) {
             if (kind == 0) {
               const int phys = __shfl_sync(0xffffffffu, entry, ct / 16);
-              const bool counts = (u.tile0 + j) * kKeys + ct < len;
-              good = counts && phys >= 0 && (int64_t)phys < p.num_blocks;
-              if (counts && !good) record_error(err, kDevBadBlockId);
-              ks = load_if(good, p.k_scale + (int64_t)phys * p.kv_heads + u.kvh);
-              vs = load_if(good, p.v_scale + (int64_t)phys * p.kv_heads + u.kvh);
+              const bool counts = (u.tile0 + j) * kKeys + (ct & ~15) < len;
+              const bool page = phys >= 0 && (int64_t)phys < p.num_blocks;
+              good = page || !counts;  // (the rows' limits hide what is behind the length)
+              if (!good) record_error(err, kDevBadBlockId);
+              ks = load_if(page && counts, p.k_scale + (int64_t)phys * p.kv_heads + u.kvh);
+              vs = load_if(page && counts, p.v_scale + (int64_t)phys * p.kv_heads + u.kvh);
               const bool in = (u.tile0 + j) * kKeys + (lane & 7) * 16 < len && entry >= 0 &&
                               (int64_t)entry < p.num_blocks;
               at = in ? (uint32_t)entry * p.bs + rem : kNoRow;
@@ -321,13 +319,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc_kernel(const TcParams p,
             const int i = 2 * (tiles_before + j) + kind;
             if (kind == 0) {  // the tile's scales and which of its tokens count
               const int slot = (tiles_before + j) % kSlots;
-              s_scale[(slot * 2) * kKeys + ct] = ks * p.qk_scale;
-              s_scale[(slot * 2 + 1) * kKeys + ct] = vs;
+              if (ct % 16 == 0) {
+                s_scale[slot * 16 + ct / 16] = ks * p.qk_scale;
+                s_scale[slot * 16 + 8 + ct / 16] = vs;
+              }
               const unsigned m = __ballot_sync(0xffffffffu, good);
+              // the largest V scale of the warp's groups; infinity where one is not finite
               const float a = fabsf(vs);
-              const uint32_t big = __reduce_max_sync(0xffffffffu, a <= 3.0e38f ? __float_as_uint(a) : 0u);
+              const uint32_t big =
+                  __reduce_max_sync(0xffffffffu, a <= 3.0e38f ? __float_as_uint(a) : 0x7f800000u);
               if (lane == 0) {
-                s_mask[slot * 4 + (ct >> 5)] = m;
+                s_mask[slot * 4 + (ct >> 5)] = (uint8_t)((m & 1u) | (m >> 16 & 1u) << 1);
                 s_max[slot * 4 + (ct >> 5)] = __uint_as_float(big);
               }
               mbar_arrive(&sc_full[slot]);
@@ -579,6 +581,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc_kernel(const TcParams p,
       float since = 1.0f;  // by what O's unit has changed since the sum was written
       float m = -INFINITY, l = 0.0f;  // m in units of S * k_scale * qk_scale
       float unit_v = 0.0f, inv_v = 0.0f;  // a power of two above the V scales so far: O's unit
+      bool spoilt = false;  // the row sees a V scale that is not finite
       int c_tile = 0;  // tiles so far
       for (int j = first; j < nt; j += by, ++c_tile) {
         const int jj = tiles_before + j, slot = jj % kSlots;
@@ -621,12 +624,28 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc_kernel(const TcParams p,
           tmem_wait_store();
           since = 1.0f;
         }
-        const float* ks = s_scale + slot * 2 * kKeys;
-        const float* vs = ks + kKeys;
-        const uint4 mask = *reinterpret_cast<const uint4*>(s_mask + slot * 4);
+        const float* ks = s_scale + slot * 16;
+        const float* vs = ks + 8;
+        const uint32_t groups = *reinterpret_cast<const uint32_t*>(s_mask + slot * 4);
         const float4 vm = *reinterpret_cast<const float4*>(s_max + slot * 4);
-        const bool masked =
-            (mask.x & mask.y & mask.z & mask.w) != 0xffffffffu || j >= first_masked;
+        const bool scaled = groups != 0x03030303u || j >= first_masked;
+        if (scaled) {
+          // scores times their K scales, the masked ones -inf by selection, in place
+          // (seldom: a rolled loop)
+          const int seen = limit - (u.tile0 + j) * kKeys;  // columns below this are seen
+#pragma unroll 1
+          for (int c = 0; c < kKeys; c += 16) {
+            uint32_t w[16];
+            tmem_load<16>(s_addr + c, w);
+            tmem_wait_load();
+            const int here = groups >> (c / 32 * 8 + c / 16 % 2) & 1u ? seen - c : 0;
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              w[e] = e < here ? __float_as_uint(__uint_as_float(w[e]) * ks[c / 16]) : 0xff800000u;
+            tmem_store<16>(s_addr + c, w);
+          }
+          tmem_wait_store();
+        }
         float s[kKeys];
         {
           uint32_t(&w)[kKeys] = reinterpret_cast<uint32_t(&)[kKeys]>(s);
@@ -637,21 +656,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc_kernel(const TcParams p,
         }
 #pragma unroll
         for (int c = 0; c < kKeys; c += 16) {  // 16 tokens share their scale
-          const float k = ks[c];
+          const float k = scaled ? 1.0f : ks[c / 16];
           const uint64_t k2 = f32x2(k, k);
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
             const float2 y = unpack_f32x2(mul_f32x2(f32x2(s[c + e], s[c + e + 1]), k2));
             s[c + e] = y.x;
             s[c + e + 1] = y.y;
-          }
-        }
-        const int seen = limit - (u.tile0 + j) * kKeys;  // columns below this are seen
-        if (masked) {
-#pragma unroll
-          for (int c = 0; c < kKeys; ++c) {
-            const uint32_t w = c < 32 ? mask.x : c < 64 ? mask.y : c < 96 ? mask.z : mask.w;
-            s[c] = c < seen && (w >> (c & 31) & 1u) ? s[c] : -INFINITY;
           }
         }
         float tm[8];
@@ -667,7 +678,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc_kernel(const TcParams p,
             max3_nan(tm[0], tm[2], s[kKeys - 7]), max3_nan(tm[4], tm[6], s[kKeys - 5]),
             max3_nan(s[kKeys - 3], s[kKeys - 1], tm[0]));
         const bool move = valid && t > m && (m == -INFINITY || (t - m) * rf > kLazy);
-        const float big = fmaxf(fmaxf(vm.x, vm.y), fmaxf(vm.z, vm.w));
+        float big = fmaxf(fmaxf(vm.x, vm.y), fmaxf(vm.z, vm.w));
+        if (big > 3.0e38f) {
+          // A V scale that is not finite makes the rows that see it NaN, and only those: it
+          // counts as 0 in the products.
+          big = 0.0f;
+          for (int c = 0; c < kKeys / 16; ++c) {
+            const float v = fabsf(vs[c]);
+            if (v <= 3.0e38f) big = fmaxf(big, v);
+            else if ((u.tile0 + j) * kKeys + c * 16 < limit) spoilt = true;
+          }
+        }
         if (__any_sync(0xffffffffu, move || big > unit_v)) {
           float alpha = move ? (m == -INFINITY ? 0.0f : ex2((m - t) * rf)) : 1.0f;
           if (move) m = t;
@@ -699,20 +720,19 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc_kernel(const TcParams p,
 #pragma unroll
         for (int c = 0; c < kKeys; c += 32) {
           uint32_t hi[16], lo[HALVES == 2 ? 16 : 1];
+          float g0 = vs[c / 16] * inv_v, g1 = vs[c / 16 + 1] * inv_v;
+          if (!(fabsf(g0) <= 1.0f)) g0 = 0.0f;
+          if (!(fabsf(g1) <= 1.0f)) g1 = 0.0f;
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            const float g = vs[c + (e & 16)] * inv_v;
+            const float g = (e & 16) ? g1 : g0;
             float2 z = unpack_f32x2(fma_f32x2(f32x2(s[c + e], s[c + e + 1]), rf2, ms2));
             z.x = ex2(z.x);
             z.y = ex2(z.y);
             const uint64_t pr = f32x2(z.x, z.y);
             sum[(e / 2) & 1] = add_f32x2(sum[(e / 2) & 1], pr);
             const uint64_t pv = mul_f32x2(pr, f32x2(g, g));
-            float2 f = unpack_f32x2(pv);
-            if (masked) {  // (a V scale that is not finite does not reach rows in front)
-              if (s[c + e] == -INFINITY) f.x = 0.0f;
-              if (s[c + e + 1] == -INFINITY) f.y = 0.0f;
-            }
+            const float2 f = unpack_f32x2(pv);
             const __half2 h = __floats2half2_rn(f.x, f.y);
             hi[e / 2] = word_of(h);
             if constexpr (HALVES == 2) {
@@ -773,7 +793,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc_kernel(const TcParams p,
       };
       // base such that O and l are sums of 2^(score - base)
       float base = m == -INFINITY && l == l ? -INFINITY : (m == -INFINITY ? 0.0f : m * rf) - kPShift;
-      float mine = unit_v;  // what this thread's O is multiplied by
+      float mine = spoilt ? __int_as_float(0x7fffffff) : unit_v;  // what this thread's O is multiplied by
       uint8_t* stage = smem + C::kOffQ + x * HALVES * C::kTileBytes;  // rows of 128 bytes, swizzled
       uint8_t* other = smem + C::kOffQ + HALVES * C::kTileBytes;
       if (dual) {  // the row's two halves meet in the first warpgroup
@@ -784,7 +804,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc_kernel(const TcParams p,
         const float fa = a.x == -INFINITY ? 0.0f : ex2(a.x - top);
         const float fb = b.x == -INFINITY ? 0.0f : ex2(b.x - top);
         mine *= x ? fb : fa;
-        if ((x ? b.x : a.x) == -INFINITY) mine = 0.0f;
+        if ((x ? b.x : a.x) == -INFINITY && !spoilt) mine = 0.0f;
         base = top;
         l = (a.x == -INFINITY ? 0.0f : a.y * fa) + (b.x == -INFINITY ? 0.0f : b.y * fb);
       }
