@@ -829,10 +829,10 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// A cache as (channel, head, token of all pages); boxes of `channels` codes of one head
-// and `tokens` tokens, swizzled within rows of 64 or 128 bytes.  Channels past head_dim
-// load as zero.
-bool cache_map(CUtensorMap* map, const int8_t* cache, const ChunkArgs& a, int channels, int tokens) {
+}  // namespace
+
+bool cache_map(CUtensorMap* map, const int8_t* cache, const ChunkArgs& a, int channels, int tokens,
+               bool swizzle) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return false;
   if (a.num_blocks == 0) return true;  // (never used)
@@ -843,9 +843,13 @@ bool cache_map(CUtensorMap* map, const int8_t* cache, const ChunkArgs& a, int ch
   cuuint32_t estr[3] = {1, 1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<int8_t*>(cache), dims, strides, box,
             estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            channels == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+            !swizzle         ? CU_TENSOR_MAP_SWIZZLE_NONE
+            : channels == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                             : CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+
+namespace {
 
 constexpr int kMostWarps = 148 * 2 * kRowWarps;
 
@@ -931,8 +935,8 @@ int launch_rows(const ChunkArgs& a, uint8_t* ws, cudaStream_t stream) {
   const int64_t ctas = std::min(most, units >= most * each ? most : (units * steps + each - 1) / each);
   p.warps = (int)ctas * kRowWarps;
   CUtensorMap map_k = {}, map_v = {};
-  if (WHOLE && (!cache_map(&map_k, a.k_cache, a, DP, kStep) ||
-                (PV && !cache_map(&map_v, a.v_cache, a, DP, kStep)))) {
+  if (WHOLE && (!cache_map(&map_k, a.k_cache, a, DP, kStep, true) ||
+                (PV && !cache_map(&map_v, a.v_cache, a, DP, kStep, true)))) {
     set_error("cuTensorMapEncodeTiled failed for the caches");
     return kCudaError;
   }

@@ -1,10 +1,18 @@
 // What chunk.cu and chunk_tc.cu know of each other.
 #pragma once
 
+#include <cuda.h>
+
 #include "cache_mma.cuh"
 #include "pkv_internal.h"
 
 namespace pkv {
+
+// A cache as (channel, head, token of all pages); boxes of `channels` codes of one head
+// and `tokens` tokens, plain or swizzled within rows of 64 or 128 bytes.  Channels past
+// head_dim load as zero.
+bool cache_map(CUtensorMap* map, const int8_t* cache, const ChunkArgs& a, int channels, int tokens,
+               bool swizzle);
 
 constexpr int kChunkTcCtas = 148;  // one per SM
 

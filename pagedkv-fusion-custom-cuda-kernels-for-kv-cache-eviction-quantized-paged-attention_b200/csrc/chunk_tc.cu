@@ -13,10 +13,10 @@
 // kernel's 16-bit form shares; a unit of at most 128 rows has its even key tiles taken by
 // the one and its odd ones by the other, joined at its end.
 //
-// Roles: two softmax warpgroups (thread = row), four converting warps (pages by
-// cp.async into the half of a stage that is converted last), an issuing warp per row
-// tile; two warps idle so that the registers split evenly.  Every role finds the CTA's
-// segments by itself; rings and barriers run on over them.
+// Roles: two softmax warpgroups (thread = row), a loading warp (16 tokens of a page a
+// box, by TMA into the half of a stage that is converted last, and the scales), four
+// converting warps, an issuing warp per row tile; one warp idles.  Every role finds the
+// CTA's segments by itself; rings and barriers run on over them.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -35,7 +35,7 @@ constexpr int kTileRows = 128;
 constexpr int kUnitRows = 256;
 constexpr int kKeys = 128;
 constexpr int kThreads = 512;
-constexpr int kConvWarp = 8, kMmaWarp = 12, kIdleWarp = 14;
+constexpr int kConvWarp = 8, kMmaWarp = 12, kLoadWarp = 14;
 constexpr int kEarly = 4;      // MMAs left of a step when the turn is passed on
 constexpr int kOver = 3;       // tiles that a unit's start and end cost
 constexpr int kLeast = 6;      // places of a CTA's share
@@ -56,13 +56,13 @@ struct TcCfg {
   static constexpr int kOffQ = 0;  // [row tile][hi, lo]; results leave through them
   static constexpr int kOffKV = 2 * HALVES * kTileBytes;
   static constexpr int kOffScale = kOffKV + kStages * kTileBytes;  // [slot][k, v][8 groups]
-  static constexpr int kOffMask = kOffScale + kSlots * 64;  // [slot][converting warp] bytes
-  static constexpr int kOffMax = kOffMask + kSlots * 4;     // [slot][converting warp]
+  static constexpr int kOffMask = kOffScale + kSlots * 64;  // [slot]: bits of the groups that count
+  static constexpr int kOffMax = kOffMask + kSlots * 4;     // [slot]: the largest V scale
   // (base, l) of the rows of a row tile: behind the results in its query tile, or apart
-  static constexpr int kOffMl = DP == 128 ? kOffQ + 16384 : kOffMax + kSlots * 16;
+  static constexpr int kOffMl = DP == 128 ? kOffQ + 16384 : kOffMax + kSlots * 4;
   static constexpr int kMlPitch = DP == 128 ? HALVES * kTileBytes : kTileRows * 8;
-  static constexpr int kOffBar = kOffMax + kSlots * 16 + (DP == 128 ? 0 : 2 * kTileRows * 8);
-  static constexpr int kBars = 2 * kStages + kSlots + 2 + 2 + 4 + 2 + 2 + 1;
+  static constexpr int kOffBar = kOffMax + kSlots * 4 + (DP == 128 ? 0 : 2 * kTileRows * 8);
+  static constexpr int kBars = 3 * kStages + kSlots + 2 + 2 + 4 + 2 + 2 + 1;
   static constexpr int kOffMisc = kOffBar + kBars * 8;
   static constexpr int kSmemBytes = kOffMisc + 16;
   static constexpr int kOCol = 256;
@@ -171,18 +171,21 @@ __device__ __forceinline__ float load_if(bool on, const float* p) {
 }
 
 template <typename T, int DP, int HALVES>
-__global__ void __launch_bounds__(kThreads, 1) chunk_tc_kernel(const TcParams p, int* err) {
+__global__ void __launch_bounds__(kThreads, 1)
+    chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                    const TcParams p, int* err) {
   using C = TcCfg<DP, HALVES>;
   using S = TcSlot<DP>;
   constexpr int kStages = C::kStages, kSlots = C::kSlots;
   extern __shared__ __align__(1024) uint8_t smem[];
   float* s_scale = reinterpret_cast<float*>(smem + C::kOffScale);
-  uint8_t* s_mask = smem + C::kOffMask;
+  uint32_t* s_mask = reinterpret_cast<uint32_t*>(smem + C::kOffMask);
   float* s_max = reinterpret_cast<float*>(smem + C::kOffMax);
   const auto s_ml = [&](int x) { return reinterpret_cast<float2*>(smem + C::kOffMl + x * C::kMlPitch); };
   uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
   uint64_t* kv_empty = kv_full + kStages;
-  uint64_t* sc_full = kv_empty + kStages;
+  uint64_t* raw_full = kv_empty + kStages;  // codes that are not converted yet
+  uint64_t* sc_full = raw_full + kStages;
   uint64_t* q_full = sc_full + kSlots;  // per row tile, as the next three
   uint64_t* s_full = q_full + 2;
   uint64_t* p_full = s_full + 2;  // [row tile][half of the tokens]
@@ -213,8 +216,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc_kernel(const TcParams p,
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&kv_full[i], 128);
       mbar_init(&kv_empty[i], 2);
+      mbar_init(&raw_full[i], 1);
     }
-    for (int i = 0; i < kSlots; ++i) mbar_init(&sc_full[i], 128);
+    for (int i = 0; i < kSlots; ++i) mbar_init(&sc_full[i], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 128);
       mbar_init(&s_full[i], 1);
@@ -241,132 +245,126 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc_kernel(const TcParams p,
     }
   };
   int tiles_before = 0;  // of the CTA's earlier segments
+  int loaded = 0;        // tiles, by the loading warp
 
   if (warp >= kConvWarp) {
     registers_down<C::kOtherRegs>();
     if (warp < kMmaWarp) {
-      // ---- pages to fp16 tiles ---------------------------------------------------------
+      // ---- codes to fp16 tiles ---------------------------------------------------------
       constexpr int kLanes = DP / 16;      // 16-byte pieces of a token row
       constexpr int kStep = 128 / kLanes;  // token rows per pass
       constexpr int kPass = kKeys / kStep;
-      // With three stages the next K waits for V (j - 1)'s, and V (j) is not to wait for
-      // that: both copies are started after both conversions.  Else each after its own.
-      constexpr bool kBetween = kStages > 3;
       const int ct = tid - kConvWarp * 32;
       const int piece = ct % kLanes, row0 = ct / kLanes;
-      const uint32_t row_bytes = (uint32_t)(p.kv_heads * p.dim);
-      const bool in_dim = piece * 16 < p.dim;
-      constexpr uint32_t kNoRow = 0xffffffffu;  // no token, or a page outside the cache
-      const auto stage_of = [&](int i) { return smem + C::kOffKV + (i % kStages) * C::kTileBytes; };
+      const uint32_t off = (piece / 4) * (kKeys * 128) + sw128_offset(row0, (piece % 4) * 32);
+      const uint32_t off16 = (piece / 4) * (kKeys * 128) + sw128_offset(row0, (piece % 4) * 32 + 16);
       TcUnit u;
       u.s = plan_find(p.seq, p.seqs, begin);
+      int st = 0, use = 0;
       for (int64_t now = begin; now < stop; now = u.at + u.seq.steps + kOver) {
+        u.find(p, now, share);
+        if (u.empty(stop)) continue;
+        u.cut(p, now, stop);
+#pragma unroll 1
+        for (int i = 0; i < 2 * u.n; ++i) {  // K and V in turns
+          uint8_t* tile = smem + C::kOffKV + st * C::kTileBytes;
+          wait(&raw_full[st], use);
+          uint4 raw[kPass];
+#pragma unroll
+          for (int r = 0; r < kPass; ++r)
+            raw[r] = *reinterpret_cast<const uint4*>(tile + C::kTileBytes / 2 + (r * 128 + ct) * 16);
+          named_barrier(1, 128);  // every code is read
+#pragma unroll
+          for (int r = 0; r < kPass; ++r) {  // (kStep % 8 = 0: one swizzle for all)
+            const uint4 w = raw[r];
+            const uint2 a = codes_to_half(w.x), b = codes_to_half(w.y), c = codes_to_half(w.z),
+                        d = codes_to_half(w.w);
+            *reinterpret_cast<uint4*>(tile + off + r * kStep * 128) = make_uint4(a.x, a.y, b.x, b.y);
+            *reinterpret_cast<uint4*>(tile + off16 + r * kStep * 128) = make_uint4(c.x, c.y, d.x, d.y);
+          }
+          fence_proxy_async_smem();  // an MMA operand
+          mbar_arrive(&kv_full[st]);
+          if (++st == kStages) st = 0, ++use;
+        }
+      }
+    } else if (warp == kLoadWarp) {
+      // ---- pages and scales ---------------------------------------------------------------
+      // Lane l has the tile's group l & 7 of 16 tokens, which is on one page: its entry is
+      // loaded two tiles ahead, its scales (K: lanes 0-7, V: 8-15) one.
+      const uint64_t hold = l2_policy_evict_last();
+      const float* scales = lane < 8 ? p.k_scale : p.v_scale;
+      if (lane == 0) {
+        prefetch_tensormap(&map_k);
+        prefetch_tensormap(&map_v);
+      }
+      TcUnit u;
+      u.s = plan_find(p.seq, p.seqs, begin);
+      for (int64_t now = begin; now < stop && ok; now = u.at + u.seq.steps + kOver) {
         u.find(p, now, share);
         if (u.empty(stop)) continue;
         u.cut(p, now, stop);
         const int n = u.n, len = u.seq.len;
         const int32_t* table = p.tables + (int64_t)u.s * p.width;
-        const int last_page = (len - 1) / p.bs;
-        // A tile's 8 groups of 16 tokens are on one page each, found a tile ahead by the
-        // lanes (lane & 7 = group) and handed on by shuffle.
-        uint32_t at = kNoRow;
-        int entry = 0, rem = 0;
-        float ks = 0.0f, vs = 0.0f;
-        bool good = false;
-        const auto look_up = [&](int j) {
-          const int token = (u.tile0 + j) * kKeys + (lane & 7) * 16;
-          const int page = token / p.bs;
-          rem = token - page * p.bs;
-          entry = table[min(page, last_page)];  // past the end the last page again
+        const auto token_of = [&](int j) { return (u.tile0 + j) * kKeys + (lane & 7) * 16; };
+        const auto entry_of = [&](int j) {
+          return j < n && token_of(j) < len ? table[token_of(j) / p.bs] : -1;
         };
-        const auto issue = [&](int j, int kind) {
-          if (j < n) {
-            if (kind == 0) {
-              const int phys = __shfl_sync(0xffffffffu, entry, ct / 16);
-              const bool counts = (u.tile0 + j) * kKeys + (ct & ~15) < len;
-              const bool page = phys >= 0 && (int64_t)phys < p.num_blocks;
-              good = page || !counts;  // (the rows' limits hide what is behind the length)
-              if (!good) record_error(err, kDevBadBlockId);
-              ks = load_if(page && counts, p.k_scale + (int64_t)phys * p.kv_heads + u.kvh);
-              vs = load_if(page && counts, p.v_scale + (int64_t)phys * p.kv_heads + u.kvh);
-              const bool in = (u.tile0 + j) * kKeys + (lane & 7) * 16 < len && entry >= 0 &&
-                              (int64_t)entry < p.num_blocks;
-              at = in ? (uint32_t)entry * p.bs + rem : kNoRow;
-              if (j + 1 < n) look_up(j + 1);
-            }
-            const int i = 2 * (tiles_before + j) + kind;
-            wait(&kv_empty[i % kStages], i / kStages + 1);
-            const int8_t* base = (kind ? p.v_cache : p.k_cache) + (int64_t)u.kvh * p.dim + piece * 16;
-            const uint32_t dst = smem_u32(stage_of(i)) + C::kTileBytes / 2 + ct * 16;
-#pragma unroll
-            for (int r = 0; r < kPass; ++r) {
-              const uint32_t row = __shfl_sync(0xffffffffu, at, r * kStep / 16 + row0 / 16);
-              const bool on = row != kNoRow && in_dim;
-              // (rows past the length on its last page are read: any codes will do)
-              const uint64_t from =
-                  (uint64_t)(on ? row + (r * kStep + row0) % 16 : 0) * row_bytes;
-              copy16_if(on, dst + r * 2048, base + (on ? from : 0));
-            }
-          }
-          copies_commit();
+        const auto good = [&](int entry) { return entry >= 0 && (int64_t)entry < p.num_blocks; };
+        const auto scale_of = [&](int entry) {
+          return load_if(lane < 16 && good(entry), scales + (int64_t)entry * p.kv_heads + u.kvh);
         };
-        if (n > 0) look_up(0);
-        issue(0, 0);
-        issue(0, 1);
+        int entry = entry_of(0), entry1 = entry_of(1);
+        float scale = scale_of(entry);
         for (int j = 0; j < n; ++j) {
+          const int entry2 = entry_of(j + 2);
+          const float scale1 = scale_of(entry1);
+          const int token = token_of(j), jj = tiles_before + j, slot = jj % kSlots;
+          const bool there = lane < 8 && good(entry);
+          const unsigned boxes = __ballot_sync(0xffffffffu, there);
+          if (token < len && !good(entry)) record_error(err, kDevBadBlockId);
+          const int at = entry * p.bs + token % p.bs;
 #pragma unroll
           for (int kind = 0; kind < 2; ++kind) {
-            const int i = 2 * (tiles_before + j) + kind;
-            if (kind == 0) {  // the tile's scales and which of its tokens count
-              const int slot = (tiles_before + j) % kSlots;
-              if (ct % 16 == 0) {
-                s_scale[slot * 16 + ct / 16] = ks * p.qk_scale;
-                s_scale[slot * 16 + 8 + ct / 16] = vs;
-              }
-              const unsigned m = __ballot_sync(0xffffffffu, good);
-              // the largest V scale of the warp's groups; infinity where one is not finite
-              const float a = fabsf(vs);
-              const uint32_t big =
-                  __reduce_max_sync(0xffffffffu, a <= 3.0e38f ? __float_as_uint(a) : 0x7f800000u);
+            const int i = 2 * jj + kind, st = i % kStages;
+            wait(&kv_empty[st], i / kStages + 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            if (kind == 0) {
+              // (what the slot held is used: three tiles at most are in flight)
+              if (lane < 16) s_scale[slot * 16 + lane] = lane < 8 ? scale * p.qk_scale : scale;
+              // groups behind the length are hidden by the rows' limits
+              const unsigned count = boxes | __ballot_sync(0xffffffffu, token >= len);
+              // the largest V scale; infinity where one is not finite
+              const float a = fabsf(scale);
+              const uint32_t big = __reduce_max_sync(
+                  0xffffffffu, lane < 8 || lane >= 16 ? 0u : a <= 3.0e38f ? __float_as_uint(a) : 0x7f800000u);
               if (lane == 0) {
-                s_mask[slot * 4 + (ct >> 5)] = (uint8_t)((m & 1u) | (m >> 16 & 1u) << 1);
-                s_max[slot * 4 + (ct >> 5)] = __uint_as_float(big);
+                s_mask[slot] = count & 0xffu;
+                s_max[slot] = __uint_as_float(big);
               }
-              mbar_arrive(&sc_full[slot]);
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&sc_full[slot]);
             }
-            if (kind == 0 || kBetween) copies_wait<1>();
-            else copies_wait<0>();
-            uint4 raw[kPass];
-#pragma unroll
-            for (int r = 0; r < kPass; ++r)
-              raw[r] = *reinterpret_cast<const uint4*>(stage_of(i) + C::kTileBytes / 2 + (r * 128 + ct) * 16);
-            named_barrier(1, 128);  // every code is read
-            uint8_t* tile = stage_of(i) + (piece / 4) * (kKeys * 128);
-            const uint32_t off = sw128_offset(row0, (piece % 4) * 32);
-            const uint32_t off16 = sw128_offset(row0, (piece % 4) * 32 + 16);
-#pragma unroll
-            for (int r = 0; r < kPass; ++r) {  // (kStep % 8 = 0: one swizzle for all)
-              const uint4 w = raw[r];
-              const uint2 a = codes_to_half(w.x), b = codes_to_half(w.y), c = codes_to_half(w.z),
-                          d = codes_to_half(w.w);
-              *reinterpret_cast<uint4*>(tile + off + r * kStep * 128) = make_uint4(a.x, a.y, b.x, b.y);
-              *reinterpret_cast<uint4*>(tile + off16 + r * kStep * 128) =
-                  make_uint4(c.x, c.y, d.x, d.y);
-            }
-            fence_proxy_async_smem();  // an MMA operand
-            mbar_arrive(&kv_full[i % kStages]);
-            if (kBetween) issue(j + 1, kind);
+            if (lane == 0) mbar_arrive_expect_tx(&raw_full[st], __popc(boxes) * 16 * DP);
+            __syncwarp();
+            if (there)
+              tma_load_3d(smem + C::kOffKV + st * C::kTileBytes + C::kTileBytes / 2 + (lane & 7) * 16 * DP,
+                          kind ? &map_v : &map_k, &raw_full[st], 0, u.kvh, at, hold);
           }
-          if (!kBetween) {
-            issue(j + 1, 0);
-            issue(j + 1, 1);
-          }
+          if (!ok) break;
+          entry = entry1;
+          entry1 = entry2;
+          scale = scale1;
+          loaded = jj + 1;
         }
         tiles_before += n;
       }
-      copies_wait<0>();
-      if (ct == 0) drain_ring(kv_empty, kStages, 2 * tiles_before);  // no release outlives the CTA
-    } else if (warp < kIdleWarp) {
+      // no copy and no release outlives the CTA
+      if (lane == 0) {
+        drain_ring(raw_full, kStages, 2 * loaded);
+        drain_ring(kv_empty, kStages, 2 * loaded);
+      }
+    } else if (warp < kLoadWarp) {
       // ---- MMA issue: a warp for each row tile, in strict turns (see prefill.cu) ---------
       constexpr uint32_t kIdQK = umma_f16_idesc(0, 0, kTileRows, kKeys);
       constexpr uint32_t kIdPV = umma_f16_idesc(0, 1, kTileRows, DP);
@@ -626,9 +624,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc_kernel(const TcParams p,
         }
         const float* ks = s_scale + slot * 16;
         const float* vs = ks + 8;
-        const uint32_t groups = *reinterpret_cast<const uint32_t*>(s_mask + slot * 4);
-        const float4 vm = *reinterpret_cast<const float4*>(s_max + slot * 4);
-        const bool scaled = groups != 0x03030303u || j >= first_masked;
+        const uint32_t groups = s_mask[slot];
+        const bool scaled = groups != 0xffu || j >= first_masked;
         if (scaled) {
           // scores times their K scales, the masked ones -inf by selection, in place
           // (seldom: a rolled loop)
@@ -638,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc_kernel(const TcParams p,
             uint32_t w[16];
             tmem_load<16>(s_addr + c, w);
             tmem_wait_load();
-            const int here = groups >> (c / 32 * 8 + c / 16 % 2) & 1u ? seen - c : 0;
+            const int here = groups >> (c / 16) & 1u ? seen - c : 0;
 #pragma unroll
             for (int e = 0; e < 16; ++e)
               w[e] = e < here ? __float_as_uint(__uint_as_float(w[e]) * ks[c / 16]) : 0xff800000u;
@@ -678,7 +675,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc_kernel(const TcParams p,
             max3_nan(tm[0], tm[2], s[kKeys - 7]), max3_nan(tm[4], tm[6], s[kKeys - 5]),
             max3_nan(s[kKeys - 3], s[kKeys - 1], tm[0]));
         const bool move = valid && t > m && (m == -INFINITY || (t - m) * rf > kLazy);
-        float big = fmaxf(fmaxf(vm.x, vm.y), fmaxf(vm.z, vm.w));
+        float big = s_max[slot];
         if (big > 3.0e38f) {
           // A V scale that is not finite makes the rows that see it NaN, and only those: it
           // counts as 0 in the products.
@@ -995,7 +992,12 @@ int launch_tc(const ChunkArgs& a, PlanHead* head, PlanSeq* seq, uint8_t* ws, boo
   auto kern = chunk_tc_kernel<T, DP, HALVES>;
   static std::atomic<uint64_t> done{0};
   allow_shared_memory(reinterpret_cast<const void*>(kern), C::kSmemBytes, done);
-  kern<<<(unsigned)ctas, kThreads, C::kSmemBytes, stream>>>(p, device_error_word());
+  CUtensorMap map_k = {}, map_v = {};
+  if (!cache_map(&map_k, a.k_cache, a, DP, 16, false) || !cache_map(&map_v, a.v_cache, a, DP, 16, false)) {
+    set_error("cuTensorMapEncodeTiled failed for the caches");
+    return kCudaError;
+  }
+  kern<<<(unsigned)ctas, kThreads, C::kSmemBytes, stream>>>(map_k, map_v, p, device_error_word());
   if (ctas > 1)
     join_tc_kernel<T, DP><<<dim3((unsigned)ctas, kUnitRows / kJoinRows), 256, 0, stream>>>(p);
   return kOk;
