@@ -39,10 +39,11 @@ constexpr int kConvWarp = 8, kMmaWarp = 12, kLoadWarp = 14;
 constexpr int kEarly = 4;      // MMAs left of a step when the turn is passed on
 constexpr int kOver = 3;       // tiles that a unit's start and end cost
 constexpr int kLeast = 6;      // places of a CTA's share
-// A row's maximum moves when a tile exceeds it by more than 2^kLazy, and p is kept times
-// 2^kPShift: at most 2^15 in fp16.
-constexpr float kLazy = 2.0f;
-constexpr float kPShift = 13.0f;
+// p is kept times 2^kPShift.  A row's maximum moves in front of the next tile when a tile
+// exceeded it by more than 2^kLazy, at once when it would exceed it by more than 2^kRoom:
+// p is at most 2^15 in fp16, whose smallest step, 2^-24, is 2^-30 of the row's largest.
+constexpr float kLazy = 4.0f, kRoom = 9.0f;
+constexpr float kPShift = 6.0f;
 
 template <int DP, int HALVES>
 struct TcCfg {
@@ -56,7 +57,8 @@ struct TcCfg {
   static constexpr int kOffQ = 0;  // [row tile][hi, lo]; results leave through them
   static constexpr int kOffKV = 2 * HALVES * kTileBytes;
   static constexpr int kOffScale = kOffKV + kStages * kTileBytes;  // [slot][k, v][8 groups]
-  static constexpr int kOffMask = kOffScale + kSlots * 64;  // [slot]: bits of the groups that count
+  static constexpr int kOffMask = kOffScale + kSlots * 64;  // [slot]: bits of the groups that count, K scales
+                                                            // that are negative or not finite
   static constexpr int kOffMax = kOffMask + kSlots * 4;     // [slot]: the largest V scale
   // (base, l) of the rows of a row tile: behind the results in its query tile, or apart
   static constexpr int kOffMl = DP == 128 ? kOffQ + 16384 : kOffMax + kSlots * 4;
@@ -67,7 +69,7 @@ struct TcCfg {
   static constexpr int kSmemBytes = kOffMisc + 16;
   static constexpr int kOCol = 256;
   // 512 registers x 128: softmax and the others
-  static constexpr int kSoftRegs = 184, kOtherRegs = 72;
+  static constexpr int kSoftRegs = 192, kOtherRegs = 64;
   static_assert(kSmemBytes <= 227 * 1024, "shared memory");
   static_assert(256 * (kSoftRegs + kOtherRegs) <= 65536, "registers");
 };
@@ -251,13 +253,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     registers_down<C::kOtherRegs>();
     if (warp < kMmaWarp) {
       // ---- codes to fp16 tiles ---------------------------------------------------------
-      constexpr int kLanes = DP / 16;      // 16-byte pieces of a token row
+      // 8 codes a lane and pass: 8 lanes' stores are then 8 pieces of one row (16 codes a
+      // lane met every bank twice)
+      constexpr int kLanes = DP / 8;
       constexpr int kStep = 128 / kLanes;  // token rows per pass
       constexpr int kPass = kKeys / kStep;
       const int ct = tid - kConvWarp * 32;
       const int piece = ct % kLanes, row0 = ct / kLanes;
-      const uint32_t off = (piece / 4) * (kKeys * 128) + sw128_offset(row0, (piece % 4) * 32);
-      const uint32_t off16 = (piece / 4) * (kKeys * 128) + sw128_offset(row0, (piece % 4) * 32 + 16);
       TcUnit u;
       u.s = plan_find(p.seq, p.seqs, begin);
       int st = 0, use = 0;
@@ -269,18 +271,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 2 * u.n; ++i) {  // K and V in turns
           uint8_t* tile = smem + C::kOffKV + st * C::kTileBytes;
           wait(&raw_full[st], use);
-          uint4 raw[kPass];
+          uint2 raw[kPass];
 #pragma unroll
           for (int r = 0; r < kPass; ++r)
-            raw[r] = *reinterpret_cast<const uint4*>(tile + C::kTileBytes / 2 + (r * 128 + ct) * 16);
+            raw[r] = *reinterpret_cast<const uint2*>(tile + C::kTileBytes / 2 + (r * 128 + ct) * 8);
           named_barrier(1, 128);  // every code is read
 #pragma unroll
-          for (int r = 0; r < kPass; ++r) {  // (kStep % 8 = 0: one swizzle for all)
-            const uint4 w = raw[r];
-            const uint2 a = codes_to_half(w.x), b = codes_to_half(w.y), c = codes_to_half(w.z),
-                        d = codes_to_half(w.w);
-            *reinterpret_cast<uint4*>(tile + off + r * kStep * 128) = make_uint4(a.x, a.y, b.x, b.y);
-            *reinterpret_cast<uint4*>(tile + off16 + r * kStep * 128) = make_uint4(c.x, c.y, d.x, d.y);
+          for (int r = 0; r < kPass; ++r) {
+            const uint2 a = codes_to_half(raw[r].x), b = codes_to_half(raw[r].y);
+            // (8 rows further the swizzle is the same)
+            const uint32_t off = sw128_offset(row0 + r * kStep % 8, (piece % 8) * 16) + r * kStep / 8 * 1024;
+            *reinterpret_cast<uint4*>(tile + (piece / 8) * (kKeys * 128) + off) =
+                make_uint4(a.x, a.y, b.x, b.y);
           }
           fence_proxy_async_smem();  // an MMA operand
           mbar_arrive(&kv_full[st]);
@@ -334,12 +336,13 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (lane < 16) s_scale[slot * 16 + lane] = lane < 8 ? scale * p.qk_scale : scale;
               // groups behind the length are hidden by the rows' limits
               const unsigned count = boxes | __ballot_sync(0xffffffffu, token >= len);
+              const bool odd = __any_sync(0xffffffffu, lane < 8 && !(scale >= 0.0f && scale <= 3.0e38f));
               // the largest V scale; infinity where one is not finite
               const float a = fabsf(scale);
               const uint32_t big = __reduce_max_sync(
                   0xffffffffu, lane < 8 || lane >= 16 ? 0u : a <= 3.0e38f ? __float_as_uint(a) : 0x7f800000u);
               if (lane == 0) {
-                s_mask[slot] = count & 0xffu;
+                s_mask[slot] = (count & 0xffu) | (odd ? 0x100u : 0u);
                 s_max[slot] = __uint_as_float(big);
               }
               __syncwarp();
@@ -578,12 +581,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       float since = 1.0f;  // by what O's unit has changed since the sum was written
       float m = -INFINITY, l = 0.0f;  // m in units of S * k_scale * qk_scale
+      float next = -INFINITY;         // what m becomes in front of the next tile
       float unit_v = 0.0f, inv_v = 0.0f;  // a power of two above the V scales so far: O's unit
       bool spoilt = false;  // the row sees a V scale that is not finite
       int c_tile = 0;  // tiles so far
       for (int j = first; j < nt; j += by, ++c_tile) {
         const int jj = tiles_before + j, slot = jj % kSlots;
         wait(&sc_full[slot], jj / kSlots);
+        const float* ks = s_scale + slot * 16;
+        const float* vs = ks + 8;
+        const uint32_t groups = s_mask[slot];
+        float big = s_max[slot];
+        const bool scaled = groups != 0xffu || j >= first_masked;
         wait(&s_full[x], s_uses++);
         __syncwarp();
         tmem_fence_after_sync();
@@ -622,10 +631,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_wait_store();
           since = 1.0f;
         }
-        const float* ks = s_scale + slot * 16;
-        const float* vs = ks + 8;
-        const uint32_t groups = s_mask[slot];
-        const bool scaled = groups != 0xffu || j >= first_masked;
         if (scaled) {
           // scores times their K scales, the masked ones -inf by selection, in place
           // (seldom: a rolled loop)
@@ -651,31 +656,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_load<32>(s_addr + c, reinterpret_cast<uint32_t(&)[32]>(w[c]));
           tmem_wait_load();
         }
-#pragma unroll
-        for (int c = 0; c < kKeys; c += 16) {  // 16 tokens share their scale
-          const float k = scaled ? 1.0f : ks[c / 16];
-          const uint64_t k2 = f32x2(k, k);
-#pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            const float2 y = unpack_f32x2(mul_f32x2(f32x2(s[c + e], s[c + e + 1]), k2));
-            s[c + e] = y.x;
-            s[c + e + 1] = y.y;
-          }
-        }
-        float tm[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) tm[e] = s[e];
-#pragma unroll
-        for (int c = 8; c < kKeys - 8; c += 16)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) tm[e] = max3_nan(tm[e], s[c + e], s[c + e + 8]);
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) tm[e] = max3_nan(tm[e], tm[e + 1], s[kKeys - 8 + e]);
-        const float t = max3_nan(
-            max3_nan(tm[0], tm[2], s[kKeys - 7]), max3_nan(tm[4], tm[6], s[kKeys - 5]),
-            max3_nan(s[kKeys - 3], s[kKeys - 1], tm[0]));
-        const bool move = valid && t > m && (m == -INFINITY || (t - m) * rf > kLazy);
-        float big = s_max[slot];
         if (big > 3.0e38f) {
           // A V scale that is not finite makes the rows that see it NaN, and only those: it
           // counts as 0 in the products.
@@ -686,44 +666,25 @@ __global__ void __launch_bounds__(kThreads, 1)
             else if ((u.tile0 + j) * kKeys + c * 16 < limit) spoilt = true;
           }
         }
-        if (__any_sync(0xffffffffu, move || big > unit_v)) {
-          float alpha = move ? (m == -INFINITY ? 0.0f : ex2((m - t) * rf)) : 1.0f;
-          if (move) m = t;
-          l *= alpha;
-          if (big > unit_v) {  // (the same in all threads)
-            const int e = min(max((int)(__float_as_uint(big) >> 23) - 126, -126), 126);
-            const float unit_now = power_of_two(e);
-            inv_v = power_of_two(-e);
-            alpha *= unit_v * inv_v;
-            unit_v = unit_now;
-          }
-          since *= alpha;
-          if (c_tile % C::kFlush != 0) {
-#pragma unroll 1
-            for (int c = 0; c < DP; c += 16) {
-              uint32_t o[16];
-              tmem_load<16>(o_addr + c, o);
-              tmem_wait_load();
-#pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-              tmem_store<16>(o_addr + c, o);
-            }
-          }
-        }
-        // a NaN score makes the whole row NaN
-        const float ms = t != t ? t : (m == -INFINITY ? 0.0f : m * rf) - kPShift;
-        const uint64_t rf2 = f32x2(rf, rf), ms2 = f32x2(-ms, -ms);
-        uint64_t sum[2] = {0, 0};
-#pragma unroll
-        for (int c = 0; c < kKeys; c += 32) {
+        // P is taken with the maximum as it was: the tile's own is looked for beside the
+        // first half's exponentials, and moves it in front of the next tile, or, where P
+        // would leave fp16 (the first tile, seldom another), at once.
+        bool move = valid && next > m;
+        float t = next;
+        uint64_t sum[2];
+        float ms;
+        const auto part = [&](int c) {  // P of tokens c .. c + 31
           uint32_t hi[16], lo[HALVES == 2 ? 16 : 1];
           float g0 = vs[c / 16] * inv_v, g1 = vs[c / 16 + 1] * inv_v;
+          const float k0 = scaled ? rf : ks[c / 16] * rf, k1 = scaled ? rf : ks[c / 16 + 1] * rf;
+          const uint64_t ms2 = f32x2(-ms, -ms);
           if (!(fabsf(g0) <= 1.0f)) g0 = 0.0f;
           if (!(fabsf(g1) <= 1.0f)) g1 = 0.0f;
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
             const float g = (e & 16) ? g1 : g0;
-            float2 z = unpack_f32x2(fma_f32x2(f32x2(s[c + e], s[c + e + 1]), rf2, ms2));
+            const float k = (e & 16) ? k1 : k0;
+            float2 z = unpack_f32x2(fma_f32x2(f32x2(s[c + e], s[c + e + 1]), f32x2(k, k), ms2));
             z.x = ex2(z.x);
             z.y = ex2(z.y);
             const uint64_t pr = f32x2(z.x, z.y);
@@ -743,12 +704,63 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else {
             tmem_store<16>(s_addr + c / 2, hi);
           }
-          if (c == 32 || c == 96) {  // half of P is there: its product can start
-            tmem_wait_store();
-            tmem_fence_before_sync();
-            mbar_arrive(&p_full[2 * x + (c == 96)]);
+        };
+        for (;;) {
+          if (__any_sync(0xffffffffu, move || big > unit_v)) {
+            float alpha = move ? (m == -INFINITY ? 0.0f : ex2((m - t) * rf)) : 1.0f;
+            if (move) m = t;
+            l *= alpha;
+            if (big > unit_v) {  // (the same in all threads)
+              const int e = min(max((int)(__float_as_uint(big) >> 23) - 126, -126), 126);
+              inv_v = power_of_two(-e);
+              alpha *= unit_v * inv_v;
+              unit_v = power_of_two(e);
+            }
+            since *= alpha;
+            if (c_tile % C::kFlush != 0) {
+#pragma unroll 1
+              for (int c = 0; c < DP; c += 16) {
+                uint32_t o[16];
+                tmem_load<16>(o_addr + c, o);
+                tmem_wait_load();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                tmem_store<16>(o_addr + c, o);
+              }
+            }
           }
+          ms = (m == -INFINITY ? 0.0f : m * rf) - kPShift;
+          sum[0] = sum[1] = 0;
+          part(0);
+          part(32);
+          // The largest of each 16 tokens, which share their scale, then times it.  (K scales
+          // that would change the order are among the scores already.)
+          t = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < kKeys; c += 16) {
+            float tm[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) tm[e] = max3_nan(s[c + e], s[c + e + 4], s[c + e + 8]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) tm[e] = max3_nan(tm[e], tm[e + 2], s[c + 12 + e]);
+            tm[0] = max3_nan(tm[0], tm[1], s[c + 14]);
+            const float k = scaled ? 1.0f : ks[c / 16];
+            t = max3_nan(t, max3_nan(tm[0], s[c + 15], s[c + 15]) * k, t);
+          }
+          // (NaN moves nothing, and makes the row NaN)
+          move = valid && t > m && (m == -INFINITY || (t - m) * rf > kRoom);
+          if (!__any_sync(0xffffffffu, move)) break;
+          big = 0.0f;
         }
+        next = (t - m) * rf > kLazy ? t : m;
+        tmem_wait_store();
+        tmem_fence_before_sync();
+        mbar_arrive(&p_full[2 * x]);  // half of P is there: its product can start
+        part(64);
+        part(96);
+        tmem_wait_store();
+        tmem_fence_before_sync();
+        mbar_arrive(&p_full[2 * x + 1]);
         const float2 l2 = unpack_f32x2(add_f32x2(sum[0], sum[1]));
         l += l2.x + l2.y;
       }
