@@ -528,26 +528,34 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int first_masked = max(u.limit(p, r - lane), 0) / kKeys - u.tile0;
       float rf = 1.0f;  // power of two that the row was divided by
       if (first < nt) {
-        // The warp takes its 32 rows one after the other, a lane per 4 channels.  A row's
-        // largest magnitude is scaled to [2^10, 2^11): exact, and lo's steps stay far
-        // below hi's.  (fp16 queries are as they are.)
-        const int base = r - lane;
+        // The warp takes its 32 rows one after the other, a lane per 4 channels; eight loads
+        // first, each row's address from the lane of the row.  A row's largest magnitude is
+        // scaled to [2^10, 2^11): exact, and lo's steps stay far below hi's.  (fp16 queries
+        // are as they are.)
+        constexpr int kBatch = 8;  // (a rolled loop: the code of more is fetched for longer)
+        const T* mine = nullptr;
+        if (valid) {
+          int h;
+          const int64_t tok = u.token(p, r, &h);
+          mine = static_cast<const T*>(p.q) + tok * p.q_tok + h * p.q_head;
+        }
+        const int count = min(u.rows - (r - lane), 32);  // of the warp's rows (or none)
+        const bool in = lane * 4 < p.dim;
 #pragma unroll 1
-        for (int i0 = 0; i0 < 32; i0 += 8) {
-          float4 rowv[8];
+        for (int i0 = 0; i0 < 32; i0 += kBatch) {
+          using Raw = std::conditional_t<sizeof(T) == 4, uint4, uint2>;
+          Raw raw[kBatch];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {  // all loads first
-            rowv[e] = make_float4(0, 0, 0, 0);
-            if (base + i0 + e < u.rows && lane * 4 < p.dim) {
-              int h;
-              const int64_t tok = u.token(p, base + i0 + e, &h);
-              rowv[e] = load4(static_cast<const T*>(p.q) + tok * p.q_tok + h * p.q_head + lane * 4);
-            }
+          for (int e = 0; e < kBatch; ++e) {
+            const T* from = reinterpret_cast<const T*>(
+                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), i0 + e));
+            raw[e] = Raw{};
+            if (i0 + e < count && in) raw[e] = *reinterpret_cast<const Raw*>(from + lane * 4);
           }
 #pragma unroll
-          for (int e8 = 0; e8 < 8; ++e8) {
+          for (int e8 = 0; e8 < kBatch; ++e8) {
             const int i = i0 + e8;
-            const float4 v = rowv[e8];
+            const float4 v = load4(reinterpret_cast<const T*>(&raw[e8]));
             float up = 1.0f;
             if constexpr (!std::is_same<T, __half>::value) {
               float big = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
