@@ -734,7 +734,7 @@ size_t pkv_accumulate_attention_workspace_size(int64_t total_q, int32_t num_seqs
                                                int64_t num_blocks, int32_t max_blocks_per_seq,
                                                int32_t has_lse) {
   const pkv::ChunkArgs a = chunk_args(
-      nullptr, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr,
+      nullptr, 0, reinterpret_cast<const int8_t*>(16), nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr,
       has_lse ? reinterpret_cast<float*>(16) : nullptr, total_q, num_seqs, num_heads, num_kv_heads,
       head_dim, block_size, 0, max_blocks_per_seq, 0, 0, 1.0f);
   if (num_blocks < 0 || check_chunk_sizes(a) != PKV_OK) return 0;

@@ -11,6 +11,7 @@
 #include <type_traits>
 
 #include "pkv_common.cuh"
+#include "pkv_internal.h"
 
 namespace pkv {
 
@@ -251,8 +252,10 @@ constexpr float kCodeUnit = 16777216.0f;  // 2^24: what codes_plus_128 divides b
 // A sequence's work: its query rows of a KV head in blocks of `rows`, a unit each, times
 // its keys in steps of `step`, one at least, behind `over` places that stand for what a
 // unit costs however short.  Units follow each other sequence by sequence, and in a
-// sequence block by block, the KV heads of a block next to one another.  Sequences of
-// less than `from` or more than `to` rows of a KV head are left to another kernel.
+// sequence block by block, the KV heads of a block next to one another.  A plan has all
+// sequences, or those of few rows of a KV head (at most few_rows, or so short that blocks
+// of 8 rows have no more than few_steps steps of 16 keys), or the others.
+enum PlanWhich { kPlanAll = 0, kPlanFew = 1, kPlanMany = 2 };
 struct PlanSeq {
   int64_t first;  // places in front of the sequence's
   int q0, lq;     // its rows in the packed queries
@@ -271,7 +274,7 @@ struct PlanArgs {
   int seqs, total_q;
   int group, kv_heads, block_size, width;
   int rows, step, over;
-  int64_t from, to;
+  int which, few_rows, few_steps;
   PlanHead* head;
   PlanSeq* seq;   // [seqs]
   int* counters;  // [counts], zeroed
@@ -279,7 +282,8 @@ struct PlanArgs {
 };
 
 // One or two plans of a call, the second for another kernel.
-int launch_plan(const PlanArgs& a, const PlanArgs* second, int* err, cudaStream_t stream);
+int launch_plan(const PlanArgs& a, const PlanArgs* second, const ZeroArgs& zero, int* err,
+                cudaStream_t stream);
 
 // The sequence of a place; one warp, a search of 32 at a time.
 __device__ __forceinline__ int plan_find(const PlanSeq* seq, int seqs, int64_t place) {

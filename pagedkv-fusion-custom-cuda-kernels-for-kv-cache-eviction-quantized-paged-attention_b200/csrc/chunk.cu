@@ -69,7 +69,22 @@ __device__ __forceinline__ int64_t scan_sum(int64_t v, int64_t* shared, int64_t*
   return v;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs first_plan, const PlanArgs second_plan, int* err) {
+__global__ void __launch_bounds__(kPlanThreads)
+    plan_kernel(const PlanArgs first_plan, const PlanArgs second_plan, int plans, const ZeroArgs z,
+                int* err) {
+  if ((int)blockIdx.x >= plans) {
+    const int64_t per_seq = (int64_t)z.width * z.block_size, slots = per_seq * z.seqs;
+    const int64_t step = (int64_t)(gridDim.x - plans) * kPlanThreads;
+    for (int64_t i = (int64_t)(blockIdx.x - plans) * kPlanThreads + threadIdx.x; i < slots; i += step) {
+      const int64_t s = i / per_seq;
+      const int at = (int)(i - s * per_seq), page = at / z.block_size;
+      if (at >= z.lens[s]) continue;
+      const int phys = z.tables[s * z.width + page];
+      if (phys >= 0 && (int64_t)phys < z.num_blocks)
+        z.sums[(int64_t)phys * z.block_size + at - page * z.block_size] = 0;
+    }
+    return;
+  }
   const PlanArgs p = blockIdx.x == 0 ? first_plan : second_plan;
   __shared__ int s_max[kPlanWarps];
   __shared__ int64_t s_sum[kPlanWarps];
@@ -101,7 +116,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs first
     const int lq = incl - before;
     const int steps = max((len + p.step - 1) / p.step, 1);
     const int64_t rows = lq * (int64_t)p.group;
-    const bool ours = s < p.seqs && rows >= p.from && rows <= p.to;
+    const bool few = rows <= p.few_rows ||
+                     (rows + 7) / 8 * p.kv_heads * (int64_t)((len + 15) / 16) <= p.few_steps;
+    const bool ours = s < p.seqs && (p.which == kPlanAll || few == (p.which == kPlanFew));
     const int64_t mine =
         ours ? (rows + p.rows - 1) / p.rows * p.kv_heads * (steps + p.over) : 0;
     int64_t all;
@@ -853,18 +870,24 @@ namespace {
 
 constexpr int kMostWarps = 148 * 2 * kRowWarps;
 
-// Which kernels a call's sequences go to: those of up to 8 rows of a KV head to the warps
-// of rows_kernel, the others to chunk_tc.cu, where it takes the shapes.  The lengths are on
-// the device, so a call launches both unless its sizes tell: at most one token a sequence
-// (decode), or more heads a group than a row tile, or one sequence of many tokens.
+// Which kernels a call's sequences go to: those of few rows to the warps of rows_kernel,
+// the others to chunk_tc.cu, where it takes the shapes.  (24 sequences of 1 to 8 tokens in
+// groups of 4: 63 us by the warps; split at 8 rows 76 us and 33 us, since a unit there
+// costs 10 to 15 us to start and end.)  The lengths are on the device, so a call launches
+// both unless its sizes tell.
+constexpr int kFewRows = 32, kFewSteps = 4096;
 struct Division {
   bool rows, tc;
 };
 Division division_of(const ChunkArgs& a) {
   const int group = a.heads / a.kv_heads;
-  if (!chunk_tc_takes(a) || (a.total_q <= a.seqs && group <= kRows)) return {true, false};
-  if (group > kRows || (a.seqs <= 1 && a.total_q * group > kRows)) return {false, true};
-  return {true, true};
+  const int64_t most_rows = a.total_q * group;
+  const int64_t units = (most_rows / kRows + std::min<int64_t>(a.seqs, a.total_q)) * a.kv_heads;
+  const int64_t steps = (int64_t)a.width * a.block_size / kStep + 1;
+  if (a.v_cache == nullptr || !chunk_tc_takes(a) || most_rows <= kFewRows ||
+      (a.total_q <= a.seqs && group <= kFewRows) || units <= kFewSteps / steps)
+    return {true, false};
+  return {group <= kFewRows, true};
 }
 
 struct ChunkLayout {
@@ -950,10 +973,20 @@ int launch_rows(const ChunkArgs& a, uint8_t* ws, cudaStream_t stream) {
 
 }  // namespace
 
-int launch_plan(const PlanArgs& a, const PlanArgs* second, int* err, cudaStream_t stream) {
-  plan_kernel<<<second != nullptr ? 2 : 1, kPlanThreads, 0, stream>>>(a, second != nullptr ? *second : a,
-                                                                      err);
+int launch_plan(const PlanArgs& a, const PlanArgs* second, const ZeroArgs& zero, int* err,
+                cudaStream_t stream) {
+  const int plans = second != nullptr ? 2 : 1;
+  const int64_t slots = zero.sums != nullptr ? (int64_t)zero.seqs * zero.width * zero.block_size : 0;
+  const int64_t zeros = std::min<int64_t>((slots + 4 * kPlanThreads - 1) / (4 * kPlanThreads), 148 * 4);
+  plan_kernel<<<(unsigned)(plans + zeros), kPlanThreads, 0, stream>>>(
+      a, second != nullptr ? *second : a, plans, zero, err);
   return kOk;
+}
+
+const PlanSeq* chunk_plan(const ChunkArgs& a, void* workspace) {
+  uint8_t* ws = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 255) &
+                                           ~(uintptr_t)255);
+  return reinterpret_cast<const PlanSeq*>(ws + chunk_layout(a).seq);
 }
 
 // (without a V cache only the denominators are taken)
@@ -985,18 +1018,19 @@ int launch_chunk(const ChunkArgs& a, void* workspace, size_t workspace_bytes, cu
   plan.rows = kRows;
   plan.step = kStep;
   plan.over = kOver;
-  plan.from = 0;
-  plan.to = d.tc ? kRows : INT64_MAX;
+  plan.which = d.tc ? kPlanFew : kPlanAll;
+  plan.few_rows = kFewRows;
+  plan.few_steps = d.rows ? kFewSteps : 0;
   plan.head = reinterpret_cast<PlanHead*>(ws + lay.head);
   plan.seq = reinterpret_cast<PlanSeq*>(ws + lay.seq);
   plan.counters = reinterpret_cast<int*>(ws + lay.counters);
   plan.counts = kMostWarps;
   PlanArgs plan2 = chunk_tc_plan(plan);
-  plan2.from = d.rows ? kRows + 1 : 0;
-  plan2.to = INT64_MAX;
+  plan2.which = d.rows ? kPlanMany : kPlanAll;
   plan2.head = reinterpret_cast<PlanHead*>(ws + lay.head2);
   plan2.seq = reinterpret_cast<PlanSeq*>(ws + lay.seq2);
-  launch_plan(d.rows ? plan : plan2, d.rows && d.tc ? &plan2 : nullptr, device_error_word(), stream);
+  launch_plan(d.rows ? plan : plan2, d.rows && d.tc ? &plan2 : nullptr, a.zero, device_error_word(),
+              stream);
   int rc = kOk;
   if (d.tc) rc = launch_chunk_tc(a, plan2.head, plan2.seq, ws + lay.tc, !d.rows, stream);
   if (rc != kOk) return rc;

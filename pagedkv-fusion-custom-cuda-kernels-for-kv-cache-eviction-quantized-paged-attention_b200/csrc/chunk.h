@@ -14,12 +14,98 @@ namespace pkv {
 bool cache_map(CUtensorMap* map, const int8_t* cache, const ChunkArgs& a, int channels, int tokens,
                bool swizzle);
 
+// Where launch_chunk left the sequences' rows and lengths (of calls without a V cache).
+const PlanSeq* chunk_plan(const ChunkArgs& a, void* workspace);
+
+constexpr int kTileUnitRows = 256;
+constexpr int kTileKeys = 128;
+constexpr int kTileOver = 3;   // tiles that a unit's start and end cost
+constexpr int kTileLeast = 6;  // places of a CTA's share
+
+// Work of kernels whose units are 256 query rows of a KV head, in tiles of 128 keys:
+// each of `ctas` CTAs has the same share of the plan's places.
+struct TileWork {
+  const PlanHead* head;
+  const PlanSeq* seq;
+  int seqs, group, kv_heads, ctas;
+};
+
+__device__ __forceinline__ int64_t tile_share(const TileWork& p) {
+  return max((p.head->places + p.ctas - 1) / p.ctas, (int64_t)kTileLeast);
+}
+
+// A unit, and the part of it that a CTA has.
+struct TileUnit {
+  PlanSeq seq;
+  int s, kvh, block, rows;
+  int64_t at;          // first place
+  int cta0, parts;
+  int tile0, n;        // the CTA's tiles of it
+  int tiles[2];        // of each row tile, from tile0 on
+  bool dual;           // the row tiles share the rows, and the tiles in turns
+
+  __device__ __forceinline__ void find(const TileWork& p, int64_t place, int64_t share) {
+    int unit;
+    for (;;) {  // (sequences that are not this kernel's have no places)
+      seq = p.seq[s];
+      unit = (int)((place - seq.first) / (seq.steps + kTileOver));
+      const int64_t next = s + 1 < p.seqs ? p.seq[s + 1].first : p.head->places;
+      if (place < next) break;
+      ++s;
+    }
+    at = seq.first + (int64_t)unit * (seq.steps + kTileOver);
+    kvh = unit % p.kv_heads;
+    block = unit / p.kv_heads;
+    rows = (int)min((int64_t)kTileUnitRows, seq.lq * (int64_t)p.group - (int64_t)block * kTileUnitRows);
+    cta0 = (int)((at + kTileOver) / share);
+    parts = (int)((at + kTileOver + seq.steps - 1) / share) - cta0 + 1;
+    dual = rows <= (kTileUnitRows / 2) && seq.steps > 1;
+  }
+  __device__ __forceinline__ void cut(const TileWork& p, int64_t now, int64_t stop) {
+    tile0 = (int)max(now - at - kTileOver, (int64_t)0);
+    const int end = (int)max(min((int64_t)seq.steps, stop - at - kTileOver), (int64_t)tile0);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int last = min((x + 1) * (kTileUnitRows / 2), rows) - 1;
+      const int keys = last >= x * (kTileUnitRows / 2) || dual ? max(limit(p, min(last, rows - 1)), 0) : 0;
+      tiles[x] = max(min((keys + kTileKeys - 1) / kTileKeys, end) - tile0, 0);
+    }
+    n = max(tiles[0], tiles[1]);
+  }
+  __device__ __forceinline__ bool empty(int64_t stop) const { return stop <= at + kTileOver; }
+  // the keys that row r sees
+  __device__ __forceinline__ int limit(const TileWork& p, int r) const {
+    return r < rows ? min((int)((uint32_t)(block * kTileUnitRows + r) / (uint32_t)p.group) + 1 + seq.len - seq.lq,
+                          seq.len)
+                    : 0;
+  }
+  __device__ __forceinline__ int64_t token(const TileWork& p, int r, int* head) const {
+    const uint32_t i = block * kTileUnitRows + r;  // (a call has less than 2^31 rows)
+    const uint32_t tok = i / (uint32_t)p.group;
+    *head = kvh * p.group + (int)(i - tok * (uint32_t)p.group);
+    return seq.q0 + tok;
+  }
+};
+
+__device__ __forceinline__ float load_if(bool on, const float* p) {
+  float v;
+  asm volatile(
+      "{\n\t.reg .pred on;\n\tsetp.ne.u32 on, %2, 0;\n\tmov.f32 %0, 0f00000000;\n\t"
+      "@on ld.global.nc.f32 %0, [%1];\n\t}"
+      : "=&f"(v)
+      : "l"(p), "r"((uint32_t)on));
+  return v;
+}
+
 constexpr int kChunkTcCtas = 148;  // one per SM
 
 // Whether the tensor-memory kernel takes this call's shapes.
 bool chunk_tc_takes(const ChunkArgs& a);
 // Its plan, from one with the call's sizes.
 PlanArgs chunk_tc_plan(const PlanArgs& base);
+// CTAs of a launch: no more than have their least share of the longest that the batch can
+// be.
+int chunk_tc_ctas(const ChunkArgs& a);
 size_t chunk_tc_workspace_size(const ChunkArgs& a);
 // The units of a plan in head and seq; with zero_rows also rows outside all sequences.
 int launch_chunk_tc(const ChunkArgs& a, PlanHead* head, PlanSeq* seq, uint8_t* ws, bool zero_rows,

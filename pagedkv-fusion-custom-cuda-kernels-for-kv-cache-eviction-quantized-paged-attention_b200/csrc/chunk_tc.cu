@@ -32,13 +32,13 @@ namespace pkv {
 namespace {
 
 constexpr int kTileRows = 128;
-constexpr int kUnitRows = 256;
-constexpr int kKeys = 128;
+constexpr int kUnitRows = kTileUnitRows;
+constexpr int kKeys = kTileKeys;
 constexpr int kThreads = 512;
 constexpr int kConvWarp = 8, kMmaWarp = 12, kLoadWarp = 14;
 constexpr int kEarly = 4;      // MMAs left of a step when the turn is passed on
-constexpr int kOver = 3;       // tiles that a unit's start and end cost
-constexpr int kLeast = 6;      // places of a CTA's share
+constexpr int kOver = kTileOver;
+constexpr int kLeast = kTileLeast;
 // p is kept times 2^kPShift.  A row's maximum moves in front of the next tile when a tile
 // exceeded it by more than 2^kLazy, at once when it would exceed it by more than 2^kRoom:
 // p is at most 2^15 in fp16, whose smallest step, 2^-24, is 2^-30 of the row's largest.
@@ -74,7 +74,7 @@ struct TcCfg {
   static_assert(256 * (kSoftRegs + kOtherRegs) <= 65536, "registers");
 };
 
-struct TcParams {
+struct TcParams : TileWork {
   const void* q;
   const int8_t* k_cache;
   const float* k_scale;
@@ -83,14 +83,11 @@ struct TcParams {
   const int32_t* tables;
   void* out;
   float* lse;  // nullable
-  const PlanHead* head;
-  const PlanSeq* seq;
   uint8_t* slots;  // per CTA two: of the unit that it begins with, and that it ends with
   float4* sums;    // per CTA and row tile: [DP / 4][128 rows], O of earlier tiles
   int64_t q_tok, q_head;
   int64_t num_blocks;
-  int seqs, total_q, heads, kv_heads, group, dim, bs, width;
-  int ctas;
+  int total_q, heads, dim, bs, width;
   int zero_rows;   // this kernel is the one that zeroes rows outside all sequences
   float qk_scale;  // sm_scale log2e
 };
@@ -101,75 +98,9 @@ struct TcSlot {
   static constexpr int kBytes = kMl + kUnitRows * 8;
 };
 
-__device__ __forceinline__ int64_t tc_share(const TcParams& p) {
-  return max((p.head->places + p.ctas - 1) / p.ctas, (int64_t)kLeast);
-}
-
-// A unit, and the part of it that a CTA has.
-struct TcUnit {
-  PlanSeq seq;
-  int s, kvh, block, rows;
-  int64_t at;          // first place
-  int cta0, parts;
-  int tile0, n;        // the CTA's tiles of it
-  int tiles[2];        // of each row tile, from tile0 on
-  bool dual;           // the row tiles share the rows, and the tiles in turns
-
-  __device__ __forceinline__ void find(const TcParams& p, int64_t place, int64_t share) {
-    int unit;
-    for (;;) {  // (sequences that are not this kernel's have no places)
-      seq = p.seq[s];
-      unit = (int)((place - seq.first) / (seq.steps + kOver));
-      const int64_t next = s + 1 < p.seqs ? p.seq[s + 1].first : p.head->places;
-      if (place < next) break;
-      ++s;
-    }
-    at = seq.first + (int64_t)unit * (seq.steps + kOver);
-    kvh = unit % p.kv_heads;
-    block = unit / p.kv_heads;
-    rows = (int)min((int64_t)kUnitRows, seq.lq * (int64_t)p.group - (int64_t)block * kUnitRows);
-    cta0 = (int)((at + kOver) / share);
-    parts = (int)((at + kOver + seq.steps - 1) / share) - cta0 + 1;
-    dual = rows <= kTileRows && seq.steps > 1;
-  }
-  __device__ __forceinline__ void cut(const TcParams& p, int64_t now, int64_t stop) {
-    tile0 = (int)max(now - at - kOver, (int64_t)0);
-    const int end = (int)max(min((int64_t)seq.steps, stop - at - kOver), (int64_t)tile0);
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int last = min((x + 1) * kTileRows, rows) - 1;
-      const int keys = last >= x * kTileRows || dual ? max(limit(p, min(last, rows - 1)), 0) : 0;
-      tiles[x] = max(min((keys + kKeys - 1) / kKeys, end) - tile0, 0);
-    }
-    n = max(tiles[0], tiles[1]);
-  }
-  __device__ __forceinline__ bool empty(int64_t stop) const { return stop <= at + kOver; }
-  // the keys that row r sees
-  __device__ __forceinline__ int limit(const TcParams& p, int r) const {
-    return r < rows ? min((int)((uint32_t)(block * kUnitRows + r) / (uint32_t)p.group) + 1 + seq.len - seq.lq,
-                          seq.len)
-                    : 0;
-  }
-  __device__ __forceinline__ int64_t token(const TcParams& p, int r, int* head) const {
-    const uint32_t i = block * kUnitRows + r;  // (a call has less than 2^31 rows)
-    const uint32_t tok = i / (uint32_t)p.group;
-    *head = kvh * p.group + (int)(i - tok * (uint32_t)p.group);
-    return seq.q0 + tok;
-  }
-  template <int BYTES>
-  __device__ __forceinline__ uint8_t* slot(const TcParams& p, int part) const {
-    return p.slots + (int64_t)(2 * (cta0 + part) + (part == 0 ? 1 : 0)) * BYTES;
-  }
-};
-
-__device__ __forceinline__ float load_if(bool on, const float* p) {
-  float v;
-  asm volatile(
-      "{\n\t.reg .pred on;\n\tsetp.ne.u32 on, %2, 0;\n\tmov.f32 %0, 0f00000000;\n\t"
-      "@on ld.global.nc.f32 %0, [%1];\n\t}"
-      : "=&f"(v)
-      : "l"(p), "r"((uint32_t)on));
-  return v;
+template <int BYTES>
+__device__ __forceinline__ uint8_t* slot_of(const TcParams& p, const TileUnit& u, int part) {
+  return p.slots + (int64_t)(2 * (u.cta0 + part) + (part == 0 ? 1 : 0)) * BYTES;
 }
 
 template <typename T, int DP, int HALVES>
@@ -198,7 +129,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const PlanHead head = *p.head;
-  const int64_t share = tc_share(p);
+  const int64_t share = tile_share(p);
   const int64_t begin = blockIdx.x * share, stop = min(begin + share, head.places);
   // rows in front of the first and behind the last sequence become zero
   if (p.zero_rows) {
@@ -260,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr int kPass = kKeys / kStep;
       const int ct = tid - kConvWarp * 32;
       const int piece = ct % kLanes, row0 = ct / kLanes;
-      TcUnit u;
+      TileUnit u;
       u.s = plan_find(p.seq, p.seqs, begin);
       int st = 0, use = 0;
       for (int64_t now = begin; now < stop; now = u.at + u.seq.steps + kOver) {
@@ -299,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         prefetch_tensormap(&map_k);
         prefetch_tensormap(&map_v);
       }
-      TcUnit u;
+      TileUnit u;
       u.s = plan_find(p.seq, p.seqs, begin);
       for (int64_t now = begin; now < stop && ok; now = u.at + u.seq.steps + kOver) {
         u.find(p, now, share);
@@ -434,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         ++p_uses;
       };
-      TcUnit u;
+      TileUnit u;
       u.s = plan_find(p.seq, p.seqs, begin);
       for (int64_t now = begin; now < stop && ok; now = u.at + u.seq.steps + kOver) {
         u.find(p, now, share);
@@ -510,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* q_tile = smem + C::kOffQ + x * HALVES * C::kTileBytes;
     const auto meet = [&]() { named_barrier(2 + x, 128); };
     int s_uses = 0, o_uses = 0;
-    TcUnit u;
+    TileUnit u;
     u.s = plan_find(p.seq, p.seqs, begin);
     for (int64_t now = begin; now < stop; now = u.at + u.seq.steps + kOver) {
       u.find(p, now, share);
@@ -828,7 +759,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool whole = u.parts == 1;
       const bool stores = !dual || x == 0;
       const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-      uint8_t* slot = u.slot<S::kBytes>(p, (int)blockIdx.x - u.cta0);
+      uint8_t* slot = slot_of<S::kBytes>(p, u, (int)blockIdx.x - u.cta0);
       const int rows = min(kTileRows, u.rows - r0);
       // 32 channels at a time through shared memory, so that they leave in whole lines
 #pragma unroll 1
@@ -902,11 +833,11 @@ __global__ void __launch_bounds__(256) join_tc_kernel(const TcParams p) {
   using S = TcSlot<DP>;
   constexpr int kBatch = 4;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t share = tc_share(p);
+  const int64_t share = tile_share(p);
   // the unit at the end of the CTA's share, if it begins there
   const int64_t place = (int64_t)(blockIdx.x + 1) * share - 1;
   if (place >= p.head->places) return;
-  TcUnit u;
+  TileUnit u;
   u.s = plan_find(p.seq, p.seqs, place);
   u.find(p, place, share);
   if (u.cta0 != (int)blockIdx.x || u.parts == 1) return;
@@ -920,7 +851,7 @@ __global__ void __launch_bounds__(256) join_tc_kernel(const TcParams p) {
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
         const bool there = i + b < u.parts;
-        const uint8_t* from = u.slot<S::kBytes>(p, there ? i + b : i);
+        const uint8_t* from = slot_of<S::kBytes>(p, u, there ? i + b : i);
         ml[b] = there ? __ldcg(reinterpret_cast<const float2*>(from + S::kMl) + r)
                       : make_float2(-INFINITY, 0.0f);
         v[b] = in ? __ldcg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(from) + r * DP + lane * 4))
@@ -1002,13 +933,8 @@ int launch_tc(const ChunkArgs& a, PlanHead* head, PlanSeq* seq, uint8_t* ws, boo
   p.width = a.width;
   p.qk_scale = a.sm_scale * kLog2e;
   p.zero_rows = zero_rows ? 1 : 0;
-  // no more CTAs than have their least share of the longest that the batch can be
-  const int64_t units =
-      (a.total_q * p.group / kUnitRows + std::min<int64_t>(a.seqs, a.total_q) + 1) * a.kv_heads;
-  const int64_t steps = ((int64_t)a.width * a.block_size + kKeys - 1) / kKeys + 1 + kOver;
-  const int64_t ctas = std::min<int64_t>(
-      kChunkTcCtas, units >= (int64_t)kChunkTcCtas * kLeast ? kChunkTcCtas : (units * steps + kLeast - 1) / kLeast);
-  p.ctas = (int)ctas;
+  const int ctas = chunk_tc_ctas(a);
+  p.ctas = ctas;
   auto kern = chunk_tc_kernel<T, DP, HALVES>;
   static std::atomic<uint64_t> done{0};
   allow_shared_memory(reinterpret_cast<const void*>(kern), C::kSmemBytes, done);
@@ -1025,8 +951,14 @@ int launch_tc(const ChunkArgs& a, PlanHead* head, PlanSeq* seq, uint8_t* ws, boo
 
 }  // namespace
 
-bool chunk_tc_takes(const ChunkArgs& a) {
-  return a.v_cache != nullptr && a.dim <= 128 && a.block_size % 16 == 0;
+bool chunk_tc_takes(const ChunkArgs& a) { return a.dim <= 128 && a.block_size % 16 == 0; }
+
+int chunk_tc_ctas(const ChunkArgs& a) {
+  const int64_t units = (a.total_q * (a.heads / a.kv_heads) / kUnitRows +
+                         std::min<int64_t>(a.seqs, a.total_q) + 1) * a.kv_heads;
+  const int64_t steps = ((int64_t)a.width * a.block_size + kKeys - 1) / kKeys + 1 + kOver;
+  return (int)std::min<int64_t>(
+      kChunkTcCtas, units >= (int64_t)kChunkTcCtas * kLeast ? kChunkTcCtas : (units * steps + kLeast - 1) / kLeast);
 }
 
 PlanArgs chunk_tc_plan(const PlanArgs& base) {

@@ -185,6 +185,15 @@ int launch_shared_prefix(const SharedPrefixArgs& a, void* workspace, size_t work
                          cudaStream_t stream);
 
 // ---- chunk.cu --------------------------------------------------------------
+// Words of the tables' pages that become zero beside a call's plan (sums null: none).
+struct ZeroArgs {
+  const int32_t* tables = nullptr;
+  const int32_t* lens = nullptr;
+  unsigned long long* sums = nullptr;  // [num_blocks, block_size]
+  int64_t num_blocks = 0;
+  int seqs = 0, block_size = 0, width = 0;
+};
+
 struct ChunkArgs {
   const void* q;
   int dtype;  // 0 fp32, 1 fp16, 2 bf16: of q and out
@@ -198,6 +207,7 @@ struct ChunkArgs {
   void* out;
   float* lse;  // nullable
   float* logits = nullptr;  // with lse alone: also the scores, [total_q * heads][width * block_size]
+  ZeroArgs zero;
   int64_t total_q, num_blocks;
   int64_t q_token_stride, q_head_stride;  // elements, of 16 bytes
   int seqs, heads, kv_heads, dim, block_size, width;

@@ -3,14 +3,15 @@
 //   weights[page(j), offset(j)] += 1/H sum over the call's tokens i and heads h of
 //                                  exp(scale q[i, h] . k_j - lse[i, h]),  j <= i + L - Lq
 //
-// with lse as the attention gave it, or taken first by the attention's own kernel
-// without its second product.
+// with lse as the attention gave it, or taken first by the attention's own kernels.
 //
-//   gather_kernel   an item is (sequence, KV head, 256 keys, at most 1,024 query rows).
-//                   A warp keeps 32 keys as fragments in registers and lets the rows
-//                   pass, 16 at a time, from shared memory; each lane sums its keys'
-//                   columns over the rows.
-//   spread_kernel   adds the sums to the weights.
+//   gather_tc_kernel  (weights_tc.cu) pages of a multiple of 16 tokens, head_dim up to 128;
+//   gather_kernel     the others: an item is (sequence, KV head, 256 keys, at most 1,024
+//                     query rows); a warp keeps 32 keys as fragments in registers and lets
+//                     the rows pass, 16 at a time, from shared memory;
+//   finish_kernel     few rows a sequence without lse: from the scores of the attention's
+//                     pass;
+//   spread_kernel     adds the sums to the weights.
 //
 // Sums of several items, and of sequences that share pages, meet as integers of 2^-38
 // in a workspace, so that the order of their arrival changes nothing.
@@ -20,8 +21,8 @@
 #include <string>
 #include <type_traits>
 
-#include "cache_mma.cuh"
-#include "pkv_internal.h"
+#include "chunk.h"
+#include "weights.h"
 
 namespace pkv {
 namespace {
@@ -31,9 +32,6 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kWarpKeys = 32;
 constexpr int kKeys = kWarps * kWarpKeys;  // of an item
 constexpr int kItemRows = 1024;            // fp32 sums of 64 values a lane, then exact
-constexpr float kUnit = 274877906944.0f;   // 2^38: 2^25 of weight before bit 63
-constexpr unsigned long long kNotFinite = 1ull << 63;
-
 struct GatherParams {
   const void* q;
   const int8_t* k_cache;
@@ -174,21 +172,39 @@ __global__ void __launch_bounds__(kThreads, DP > 128 ? 1 : 2) gather_kernel(cons
         sum[n][r] += __shfl_xor_sync(0xffffffffu, sum[n][r], 2);
         const uint32_t slot = __shfl_sync(0xffffffffu, at, n * 16 + r * 8 + g);
         if (t == 0 && slot != 0xffffffffu && r_begin < r_end) {
-          const float v = sum[n][r];
-          if (v < 33554432.0f) {
-            const unsigned long long u = __float2ull_rn(v * kUnit);
-            if (u != 0) atomicAdd(p.sums + slot, u);
-          } else {
-            atomicOr(p.sums + slot, kNotFinite);  // NaN, or lse of other tokens
-          }
+          add_weight(p.sums + slot, sum[n][r]);
         }
       }
   }
 }
 
-// The workspace of the tables' pages becomes zero, or is added to the weights.  A page
-// may be in several tables: whoever comes first takes its sum and leaves a zero.
-template <bool ADD>
+// The scores that the attention's kernel left (in powers of two), to weights: a thread per
+// cached token.  For calls of few rows, whose scores are a small part of the keys' bytes.
+__global__ void __launch_bounds__(256) finish_kernel(const GatherParams p, const float* logits,
+                                                     int64_t slots) {
+  const int64_t per_seq = (int64_t)p.width * p.bs;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < slots; i += gridDim.x * 256ll) {
+    const int64_t s = i / per_seq;
+    const int at = (int)(i - s * per_seq);
+    const PlanSeq seq = p.seq[s];
+    if (at >= seq.len || seq.lq == 0) continue;
+    const int page = at / p.bs, phys = p.tables[s * p.width + page];
+    if (phys < 0 || (int64_t)phys >= p.num_blocks) continue;
+    // the first token that sees this one
+    const int first = max(at - (seq.len - seq.lq), 0);
+    const int64_t r1 = (int64_t)(seq.q0 + seq.lq) * p.heads;
+    float sum = 0.0f;
+#pragma unroll 8
+    for (int64_t r = (int64_t)(seq.q0 + first) * p.heads; r < r1; ++r) {
+      const float lse = p.lse[r];
+      sum += lse == -INFINITY ? 0.0f : ex2(fmaf(-lse, kLog2e, logits[r * per_seq + at]));
+    }
+    add_weight(p.sums + (int64_t)phys * p.bs + (at - page * p.bs), sum);
+  }
+}
+
+// Adds the sums to the weights.  A page may be in several tables: whoever comes first
+// takes its sum and leaves a zero.
 __global__ void __launch_bounds__(256) spread_kernel(const int32_t* tables, const int32_t* lens,
                                                      unsigned long long* sums, float* weights,
                                                      int64_t num_blocks, int bs, int width,
@@ -201,19 +217,38 @@ __global__ void __launch_bounds__(256) spread_kernel(const int32_t* tables, cons
     const int page = at / bs, phys = tables[s * width + page];
     if (phys < 0 || (int64_t)phys >= num_blocks) continue;
     const int64_t slot = (int64_t)phys * bs + (at - page * bs);
-    if constexpr (ADD) {
-      const unsigned long long u = atomicExch(sums + slot, 0ull);
-      if (u != 0)
-        weights[slot] += u & kNotFinite ? __int_as_float(0x7fffffff)
-                                        : (float)((double)u * (1.0 / (double)kUnit)) * inv_heads;
-    } else {
-      sums[slot] = 0ull;
-    }
+    const unsigned long long u = atomicExch(sums + slot, 0ull);
+    if (u != 0)
+      weights[slot] += u & kNotFinite ? __int_as_float(0x7fffffff)
+                                      : (float)((double)u * (1.0 / (double)kWeightUnit)) * inv_heads;
   }
 }
 
+// How a call's denominators and scores come.  Calls of few rows a sequence (decode) whose
+// log denominators are not given leave their scores too, so that the keys are read once
+// (64 sequences of 2,050 tokens, 32 / 8 heads: 131 MB of keys, 34 MB of scores written and
+// read); the others' come from a pass of the attention (its V the keys', where that is the
+// tensor-memory kernel).
+constexpr int64_t kMostScores = 128ll << 20;  // bytes
+bool by_scores(const ChunkArgs& a) {
+  const int64_t pitch = (int64_t)a.width * a.block_size;
+  return a.lse == nullptr && a.total_q * (a.heads / a.kv_heads) <= 8 * (int64_t)a.seqs &&
+         pitch <= kMostScores / 4 / (a.total_q * a.heads);
+}
+// The call that gives lse.
+ChunkArgs inner_call(const ChunkArgs& a, float* lse, float* logits, void* out) {
+  ChunkArgs b = a;
+  b.lse = lse;
+  b.logits = logits;
+  b.out = out;
+  const bool all = !by_scores(a) && chunk_tc_takes(a);
+  b.v_cache = all ? (a.num_blocks > 0 ? a.k_cache : reinterpret_cast<const int8_t*>(16)) : nullptr;
+  b.v_scale = all ? a.k_scale : nullptr;
+  return b;
+}
+
 struct Layout {
-  size_t head, seq, lse, sums, inner, total;
+  size_t head, seq, lse, sums, logits, out, inner, total;
 };
 
 Layout layout(const ChunkArgs& a) {
@@ -224,24 +259,21 @@ Layout layout(const ChunkArgs& a) {
     at += (bytes + 255) / 256 * 256;
     return here;
   };
+  const bool scores = by_scores(a), inner = a.lse == nullptr;
+  const size_t rows = (size_t)a.total_q * a.heads;
   l.head = take(sizeof(PlanHead));
   l.seq = take(sizeof(PlanSeq) * (size_t)a.seqs);
   l.sums = take((size_t)a.num_blocks * a.block_size * 8);
-  l.lse = take(a.lse == nullptr ? (size_t)a.total_q * a.heads * 4 : 0);
+  l.lse = take(inner ? rows * 4 : 0);
+  l.logits = take(scores ? rows * a.width * a.block_size * 4 : 0);
+  l.out = take(inner && !scores && chunk_tc_takes(a) ? rows * a.dim * (a.dtype == 0 ? 4 : 2) : 0);
   l.inner = at;
-  if (a.lse == nullptr) {
-    ChunkArgs b = a;
-    b.v_cache = nullptr;
-    at += chunk_workspace_size(b);
-  }
+  if (inner) at += chunk_workspace_size(inner_call(a, nullptr, nullptr, nullptr));
   l.total = at + 256;
   return l;
 }
 
-template <typename T, int DP>
-void launch_gather(const ChunkArgs& a, const float* lse, uint8_t* ws, const Layout& lay, int* err,
-                   cudaStream_t stream) {
-  constexpr int HALVES = sizeof(T) == 4 ? 2 : 1;
+GatherParams gather_params(const ChunkArgs& a, const float* lse, uint8_t* ws, const Layout& lay) {
   GatherParams p;
   p.q = a.q;
   p.k_cache = a.k_cache;
@@ -262,6 +294,12 @@ void launch_gather(const ChunkArgs& a, const float* lse, uint8_t* ws, const Layo
   p.bs = a.block_size;
   p.width = a.width;
   p.qk_scale = a.sm_scale * kLog2e * kCodeUnit;
+  return p;
+}
+
+template <typename T, int DP>
+void launch_gather(const ChunkArgs& a, const GatherParams& p, int* err, cudaStream_t stream) {
+  constexpr int HALVES = sizeof(T) == 4 ? 2 : 1;
   const int64_t parts = ((int64_t)a.width * a.block_size + kKeys - 1) / kKeys;
   const int64_t chunks = a.total_q * p.group / kItemRows + std::min<int64_t>(a.seqs, a.total_q);
   const int64_t most = 148 * (DP > 128 ? 1 : 2);
@@ -288,51 +326,71 @@ int launch_accumulate(const ChunkArgs& a, float* weights, void* workspace, size_
   uint8_t* ws = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 255) &
                                            ~(uintptr_t)255);
   int* err = device_error_word();
+  auto* sums = reinterpret_cast<unsigned long long*>(ws + lay.sums);
+  const int64_t slots = (int64_t)a.seqs * a.width * a.block_size;
+  ZeroArgs zero;
+  zero.tables = a.tables;
+  zero.lens = a.lens;
+  zero.sums = sums;
+  zero.num_blocks = a.num_blocks;
+  zero.seqs = a.seqs;
+  zero.block_size = a.block_size;
+  zero.width = a.width;
   const float* lse = a.lse;
+  const bool scores = by_scores(a);
   if (lse == nullptr) {
-    ChunkArgs b = a;
-    b.v_cache = nullptr;
-    b.lse = reinterpret_cast<float*>(ws + lay.lse);
+    float* logits = reinterpret_cast<float*>(ws + lay.logits);
+    ChunkArgs b = inner_call(a, reinterpret_cast<float*>(ws + lay.lse), scores ? logits : nullptr,
+                             ws + lay.out);
+    if (scores) b.zero = zero;
     lse = b.lse;
     const int rc = launch_chunk(b, ws + lay.inner, chunk_workspace_size(b), stream);
     if (rc != kOk) return rc;
+    if (scores) {
+      GatherParams p = gather_params(a, lse, ws, lay);
+      p.seq = chunk_plan(b, ws + lay.inner);
+      const unsigned grid = (unsigned)std::min<int64_t>((slots + 255) / 256, 148 * 8);
+      finish_kernel<<<grid, 256, 0, stream>>>(p, logits, slots);
+    }
   }
-  PlanArgs plan;
-  plan.cu = a.cu;
-  plan.lens = a.lens;
-  plan.seqs = a.seqs;
-  plan.total_q = (int)a.total_q;
-  plan.group = a.heads / a.kv_heads;
-  plan.kv_heads = a.kv_heads;
-  plan.block_size = a.block_size;
-  plan.width = a.width;
-  plan.rows = kItemRows;
-  plan.step = kKeys;
-  plan.over = 0;
-  plan.from = 0;
-  plan.to = INT64_MAX;
-  plan.head = reinterpret_cast<PlanHead*>(ws + lay.head);
-  plan.seq = reinterpret_cast<PlanSeq*>(ws + lay.seq);
-  plan.counters = nullptr;
-  plan.counts = 0;
-  const int rc = launch_plan(plan, nullptr, err, stream);
-  if (rc != kOk) return rc;
-  auto* sums = reinterpret_cast<unsigned long long*>(ws + lay.sums);
-  const int64_t slots = (int64_t)a.seqs * a.width * a.block_size;
+  if (!scores) {
+    PlanArgs plan;
+    plan.cu = a.cu;
+    plan.lens = a.lens;
+    plan.seqs = a.seqs;
+    plan.total_q = (int)a.total_q;
+    plan.group = a.heads / a.kv_heads;
+    plan.kv_heads = a.kv_heads;
+    plan.block_size = a.block_size;
+    plan.width = a.width;
+    plan.rows = kItemRows;
+    plan.step = kKeys;
+    plan.over = 0;
+    plan.which = kPlanAll;
+    plan.few_rows = plan.few_steps = 0;
+    plan.head = reinterpret_cast<PlanHead*>(ws + lay.head);
+    plan.seq = reinterpret_cast<PlanSeq*>(ws + lay.seq);
+    plan.counters = nullptr;
+    plan.counts = 0;
+    const bool tc = chunk_tc_takes(a);
+    int rc = launch_plan(tc ? chunk_tc_plan(plan) : plan, nullptr, zero, err, stream);
+    if (rc != kOk) return rc;
+    const GatherParams p = gather_params(a, lse, ws, lay);
+    const auto with_dim = [&](auto t) {
+      using T = decltype(t);
+      if (a.dim <= 64) launch_gather<T, 64>(a, p, err, stream);
+      else if (a.dim <= 128) launch_gather<T, 128>(a, p, err, stream);
+      else launch_gather<T, 256>(a, p, err, stream);
+    };
+    if (tc) rc = launch_gather_tc(a, lse, plan.head, plan.seq, sums, stream);
+    else if (a.dtype == 0) with_dim(0.0f);
+    else if (a.dtype == 1) with_dim(__half());
+    else with_dim(__nv_bfloat16());
+    if (rc != kOk) return rc;
+  }
   const unsigned grid = (unsigned)std::min<int64_t>((slots + 255) / 256, 148 * 8);
-  spread_kernel<false><<<grid, 256, 0, stream>>>(a.tables, a.lens, sums, weights, a.num_blocks,
-                                                 a.block_size, a.width, slots, 0.0f);
-  const auto with_dim = [&](auto t) {
-    using T = decltype(t);
-    if (a.dim <= 64) launch_gather<T, 64>(a, lse, ws, lay, err, stream);
-    else if (a.dim <= 128) launch_gather<T, 128>(a, lse, ws, lay, err, stream);
-    else launch_gather<T, 256>(a, lse, ws, lay, err, stream);
-  };
-  if (a.dtype == 0) with_dim(0.0f);
-  else if (a.dtype == 1) with_dim(__half());
-  else with_dim(__nv_bfloat16());
-  spread_kernel<true><<<grid, 256, 0, stream>>>(a.tables, a.lens, sums, weights, a.num_blocks,
-                                                a.block_size, a.width, slots, 1.0f / a.heads);
+  spread_kernel<<<grid, 256, 0, stream>>>(a.tables, a.lens, sums, weights, a.num_blocks, a.block_size,
+                                          a.width, slots, 1.0f / a.heads);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) {
     set_error(std::string("accumulate launch failed: ") + cudaGetErrorString(e));
