@@ -178,23 +178,33 @@ __device__ __forceinline__ void stage_queries(uint2* frag, float* factor, float*
 }
 
 // One row of queries in the four lanes t of a lane group g, as operands of 8 columns:
-// channels p * 64 + t * 16 + w * 4 + 0..3 for step p * 4 + w.  `from` is row g's first
-// channel or null.  factor and start, as above, are those of rows 2 t and 2 t + 1.
-template <typename T, int DP, int HALVES>
-__device__ __forceinline__ void load_queries(const T* from, int dim, uint2 (&frag)[HALVES][DP / 16],
-                                             float (&factor)[2], float (&start)[2]) {
-  const int lane = threadIdx.x & 31, t = lane & 3;
-  float4 v[DP / 16];
-  float big = 0.0f;
+// channels p * 64 + t * 16 + w * 4 + 0..3 for step p * 4 + w.  First the loads: `from` is
+// row g's first channel or null.
+template <typename T>
+using Raw4 = std::conditional_t<sizeof(T) == 4, uint4, uint2>;
+template <typename T, int DP>
+__device__ __forceinline__ void load_queries(const T* from, int dim, Raw4<T> (&raw)[DP / 16]) {
+  const int t = threadIdx.x & 3;
 #pragma unroll
   for (int p = 0; p < DP / 64; ++p) {
     const int c = p * 64 + t * 16;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      float4& x = v[p * 4 + w];
-      x = from != nullptr && c < dim ? load4(from + c + w * 4) : make_float4(0, 0, 0, 0);
+      raw[p * 4 + w] = Raw4<T>{};
+      if (from != nullptr && c < dim)
+        raw[p * 4 + w] = *reinterpret_cast<const Raw4<T>*>(from + c + w * 4);
     }
   }
+}
+// Then the operands.  factor and start, as above, are those of rows 2 t and 2 t + 1.
+template <typename T, int DP, int HALVES>
+__device__ __forceinline__ void split_queries(const Raw4<T> (&raw)[DP / 16], uint2 (&frag)[HALVES][DP / 16],
+                                              float (&factor)[2], float (&start)[2]) {
+  const int t = threadIdx.x & 3;
+  float4 v[DP / 16];
+  float big = 0.0f;
+#pragma unroll
+  for (int k = 0; k < DP / 16; ++k) v[k] = load4(reinterpret_cast<const T*>(&raw[k]));
 #pragma unroll
   for (int k = 0; k < DP / 16; ++k)
     big = fmaxf(big, fmaxf(fmaxf(fabsf(v[k].x), fabsf(v[k].y)), fmaxf(fabsf(v[k].z), fabsf(v[k].w))));
@@ -255,17 +265,28 @@ constexpr float kCodeUnit = 16777216.0f;  // 2^24: what codes_plus_128 divides b
 // sequence block by block, the KV heads of a block next to one another.  A plan has all
 // sequences, or those of few rows of a KV head (at most few_rows, or so short that blocks
 // of 8 rows have no more than few_steps steps of 16 keys), or the others.
+//
+// With `workers`, each of which takes a share of the places, the plan says how large it is:
+// equal shares of all places (at least `least`), in which units follow each other and are
+// cut anywhere; or, where the call is so small that kPartSteps or twice as many steps a worker
+// do, parts of a unit of so many, a worker each (`over` is 0 then).
 enum PlanWhich { kPlanAll = 0, kPlanFew = 1, kPlanMany = 2 };
+constexpr int kPartSteps = 4;
 struct PlanSeq {
   int64_t first;  // places in front of the sequence's
   int q0, lq;     // its rows in the packed queries
   int len;        // its cached tokens, the new ones among them
   int steps;      // of a unit
+  int pitch;      // places of a unit
+  int unused;
 };
 
 struct PlanHead {
   int64_t places;      // in all
   int q_begin, q_end;  // rows of all sequences
+  int64_t share;       // places of a worker
+  int over;            // places in front of a unit's steps
+  int most_parts;      // no unit is cut into more
 };
 
 struct PlanArgs {
@@ -274,6 +295,7 @@ struct PlanArgs {
   int seqs, total_q;
   int group, kv_heads, block_size, width;
   int rows, step, over;
+  int workers, least;
   int which, few_rows, few_steps;
   PlanHead* head;
   PlanSeq* seq;   // [seqs]

@@ -97,7 +97,16 @@ __global__ void __launch_bounds__(kPlanThreads)
   int end = min(max(first, 0), p.total_q);
   const int q_begin = end;
   bool bad = first < 0 || first > p.total_q, longer = false;
-  int64_t base = 0;
+  // units of a sequence that this plan has
+  const auto units_of = [&](const PlanSeq& q) {
+    const int64_t rows = q.lq * (int64_t)p.group;
+    const bool few = rows <= p.few_rows ||
+                     (rows + 7) / 8 * p.kv_heads * (int64_t)((q.len + 15) / 16) <= p.few_steps;
+    return p.which == kPlanAll || few == (p.which == kPlanFew) ? (rows + p.rows - 1) / p.rows * p.kv_heads : 0;
+  };
+  int64_t in_shares = 0, in_parts[2] = {};  // places
+  int longest = 0;
+  PlanSeq q = {};
   for (int s0 = 0; s0 < p.seqs; s0 += kPlanThreads) {
     const int s = s0 + tid;
     int q1 = 0, len = 0;
@@ -112,34 +121,58 @@ __global__ void __launch_bounds__(kPlanThreads)
     const int incl = max(scan_max(q1, s_max, &most), end);
     s_end[tid] = incl;
     __syncthreads();
-    const int before = tid > 0 ? s_end[tid - 1] : end;
-    const int lq = incl - before;
-    const int steps = max((len + p.step - 1) / p.step, 1);
-    const int64_t rows = lq * (int64_t)p.group;
-    const bool few = rows <= p.few_rows ||
-                     (rows + 7) / 8 * p.kv_heads * (int64_t)((len + 15) / 16) <= p.few_steps;
-    const bool ours = s < p.seqs && (p.which == kPlanAll || few == (p.which == kPlanFew));
-    const int64_t mine =
-        ours ? (rows + p.rows - 1) / p.rows * p.kv_heads * (steps + p.over) : 0;
-    int64_t all;
-    const int64_t at = scan_sum(mine, s_sum, &all);
+    q.q0 = tid > 0 ? s_end[tid - 1] : end;
+    q.lq = incl - q.q0;
+    q.len = len;
+    q.steps = max((len + p.step - 1) / p.step, 1);
+    q.pitch = q.steps + p.over;
     if (s < p.seqs) {
-      PlanSeq q;
-      q.first = base + at - mine;
-      q.q0 = before;
-      q.lq = lq;
-      q.len = len;
-      q.steps = steps;
       p.seq[s] = q;
+      const int64_t units = units_of(q);
+      in_shares += units * q.pitch;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        in_parts[i] += units * ((q.steps + (kPartSteps << i) - 1) & -(kPartSteps << i));
+      if (units > 0) longest = max(longest, q.steps);
     }
-    base += all;
     end = max(end, most);
+    __syncthreads();
+  }
+  PlanHead h = {};
+  int part = 0;  // steps
+  if (p.workers > 0) {
+    int64_t all, parts[2];
+    scan_sum(in_shares, s_sum, &all);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      scan_sum(in_parts[i], s_sum, &parts[i]);
+      __syncthreads();
+    }
+    scan_max(longest, s_max, &longest);
+    __syncthreads();
+    part = parts[0] <= (int64_t)p.workers * kPartSteps       ? kPartSteps
+           : parts[1] <= (int64_t)p.workers * 2 * kPartSteps ? 2 * kPartSteps
+                                                             : 0;
+    h.share = part > 0 ? part : max((all + p.workers - 1) / p.workers, (int64_t)p.least);
+    h.over = part > 0 ? 0 : p.over;
+    h.most_parts = (int)((longest - 1) / h.share) + (part > 0 ? 1 : 2);
+  }
+  int64_t base = 0;
+  for (int s0 = 0; s0 < p.seqs; s0 += kPlanThreads) {
+    const int s = s0 + tid;
+    if (p.seqs > kPlanThreads && s < p.seqs) q = p.seq[s];
+    if (part > 0) q.pitch = (q.steps + part - 1) & -part;  // (a power of two)
+    const int64_t mine = s < p.seqs ? units_of(q) * q.pitch : 0;
+    int64_t all;
+    q.first = base + scan_sum(mine, s_sum, &all) - mine;
+    if (s < p.seqs) p.seq[s] = q;
+    base += all;
     __syncthreads();
   }
   if (bad) record_error(err, kDevBadSeqlens);
   if (longer) record_error(err, kDevSeqTooLong);
   if (tid == 0) {
-    PlanHead h;
     h.places = base;
     h.q_begin = q_begin;
     h.q_end = end;
@@ -166,7 +199,7 @@ constexpr int kStep = 16;      // keys of a step
 constexpr int kRows = 8;
 constexpr int kRowWarps = 8;   // of a CTA
 constexpr int kOver = 6;       // steps that a unit's start and end cost
-constexpr int kLeast = 16;     // places of a warp's share
+constexpr int kLeast = 2 * kPartSteps;  // places of a warp's share
 constexpr int kJoinHere = 8;   // parts that the last of them joins; more are left to join_kernel
 // A row's maximum moves when a step exceeds it by more than 2^kLazy, and p is kept times
 // 2^kPShift, at most 2^15 in fp16, times its key's V scale over a power of two above the
@@ -235,31 +268,31 @@ struct RowsUnit {
   int rows;
   int warp0, parts; // the warps that have steps of it
 
-  __device__ __forceinline__ void find(const RowsParams& p, int64_t place, int64_t share) {
+  __device__ __forceinline__ void find(const RowsParams& p, const PlanHead& plan, int64_t place) {
     for (;;) {  // (sequences that are not this kernel's have no places)
       seq = p.seq[s];
       const int64_t all = (seq.lq * (int64_t)p.group + kRows - 1) / kRows * p.kv_heads;
-      unit = (int)min((place - seq.first) / (seq.steps + kOver), all);
-      const int64_t next = s + 1 < p.seqs ? p.seq[s + 1].first : p.head->places;
+      unit = (int)min((place - seq.first) / seq.pitch, all);
+      const int64_t next = s + 1 < p.seqs ? p.seq[s + 1].first : plan.places;
       if (place < next) break;
       ++s;
     }
-    at = seq.first + (int64_t)unit * (seq.steps + kOver);
+    at = seq.first + (int64_t)unit * seq.pitch;
     kvh = unit % p.kv_heads;
     block = unit / p.kv_heads;
     rows = (int)min((int64_t)kRows, seq.lq * (int64_t)p.group - (int64_t)block * kRows);
-    warp0 = (int)((at + kOver) / share);
-    parts = (int)((at + kOver + seq.steps - 1) / share) - warp0 + 1;
+    warp0 = (int)((at + plan.over) / plan.share);
+    parts = (int)((at + plan.over + seq.steps - 1) / plan.share) - warp0 + 1;
   }
   // the keys that row r sees: those below its token's place, counted from the end
   __device__ __forceinline__ int limit(const RowsParams& p, int r) const {
-    return r < rows ? (int)((block * (int64_t)kRows + r) / p.group) + 1 + seq.len - seq.lq : 0;
+    return r < rows ? (int)((uint32_t)(block * kRows + r) / (uint32_t)p.group) + 1 + seq.len - seq.lq : 0;
   }
   // row r as (token, head) of the packed tensors
   __device__ __forceinline__ int64_t token(const RowsParams& p, int r, int* head) const {
-    const int64_t i = block * (int64_t)kRows + r;
-    const int tok = (int)(i / p.group);
-    *head = kvh * p.group + (int)(i - (int64_t)tok * p.group);
+    const uint32_t i = block * kRows + r;  // (a call has less than 2^31 rows)
+    const uint32_t tok = i / (uint32_t)p.group;
+    *head = kvh * p.group + (int)(i - tok * (uint32_t)p.group);
     return seq.q0 + tok;
   }
   template <int BYTES>
@@ -267,10 +300,6 @@ struct RowsUnit {
     return p.slots + (int64_t)(2 * (warp0 + part) + (part == 0 ? 1 : 0)) * BYTES;
   }
 };
-
-__device__ __forceinline__ int64_t rows_share(const RowsParams& p) {
-  return max((p.head->places + p.warps - 1) / p.warps, (int64_t)kLeast);
-}
 
 __device__ __forceinline__ float row_scale(float l) { return l > 0.0f || l != l ? 1.0f / l : 0.0f; }
 __device__ __forceinline__ float row_lse(float m, float l) {
@@ -297,7 +326,6 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, PV, WHOLE>::kCtas)
   extern __shared__ __align__(1024) uint8_t smem[];
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int in_cta = threadIdx.x >> 5;
-  const int warp = blockIdx.x * kRowWarps + in_cta;  // of the grid
   uint8_t* ring = smem + in_cta * C::kRingBytes;
   uint8_t* ring_scale = smem + C::kOffScale + in_cta * kStages * C::kScaleBytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBar) + in_cta * kStages;
@@ -314,12 +342,18 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, PV, WHOLE>::kCtas)
     hold = l2_policy_evict_first();
   }
 
-  // rows in front of the first and behind the last sequence become zero
   const PlanHead head = *p.head;
+  // Of the grid.  Where there is work for few warps they are on all SMs; neighbours in
+  // the plan, which read other heads of the same pages, are in the same CTA (64 sequences
+  // of 2,050 tokens: 67 us where they were not).
+  const int busy = (int)((head.places + head.share - 1) / head.share);
+  const int of_cta = min(max((busy + (int)gridDim.x - 1) / (int)gridDim.x, 1), kRowWarps);
+  const int warp = in_cta < of_cta ? (int)blockIdx.x * of_cta + in_cta : p.warps;
+  // rows in front of the first and behind the last sequence become zero
   const int64_t front = (int64_t)head.q_begin * p.heads;
   const int64_t behind = (int64_t)head.q_end * p.heads;
   const int64_t outside = front + (int64_t)p.total_q * p.heads - behind;
-  for (int64_t i = warp; i < outside; i += p.warps) {
+  for (int64_t i = blockIdx.x * kRowWarps + in_cta; i < outside; i += p.warps) {
     const int64_t r = i < front ? i : behind + i - front;
     for (int c = lane * 4; PV && c < p.dim; c += 128)
       store4(static_cast<T*>(p.out) + r * p.dim + c, make_float4(0, 0, 0, 0));
@@ -344,15 +378,14 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, PV, WHOLE>::kCtas)
   };
   const uint32_t v_at[2] = {v_place(kv0), v_place(kv1)};
 
-  const int64_t share = rows_share(p);
-  int64_t now = warp * share;
-  const int64_t stop = min(now + share, head.places);
+  int64_t now = warp * head.share;
+  const int64_t stop = min(now + head.share, head.places);
   RowsUnit u;
   if (now < stop) u.s = plan_find(p.seq, p.seqs, now);
-  for (; now < stop; now = u.at + u.seq.steps + kOver) {
-    u.find(p, now, share);
-    const int first_step = (int)max(now - u.at - kOver, (int64_t)0);
-    const int end_step = (int)min((int64_t)u.seq.steps, stop - u.at - kOver);
+  for (; now < stop; now = u.at + u.seq.pitch) {
+    u.find(p, head, now);
+    const int first_step = (int)max(now - u.at - head.over, (int64_t)0);
+    const int end_step = (int)min((int64_t)u.seq.steps, stop - u.at - head.over);
     if (end_step <= first_step) continue;  // none of its steps
     const int kvh = u.kvh, rows = u.rows;
     const int k0 = first_step * kStep;
@@ -430,18 +463,19 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, PV, WHOLE>::kCtas)
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) issue();
 
-    // a lane's rows are 2 t and 2 t + 1
-    uint2 qr[HALVES][kSteps];
-    float f[2], start[2];
+    Raw4<T> raw[kSteps];  // row g's queries, on their way
     {
       int h;
       const int64_t tok = u.token(p, g, &h);
-      load_queries<T, DP, HALVES>(
-          g < rows ? static_cast<const T*>(p.q) + tok * p.q_tok + h * p.q_head : nullptr, p.dim, qr,
-          f, start);
-      f[0] *= p.qk_scale;
-      f[1] *= p.qk_scale;
+      load_queries<T, DP>(g < rows ? static_cast<const T*>(p.q) + tok * p.q_tok + h * p.q_head : nullptr,
+                          p.dim, raw);
     }
+    // a lane's rows are 2 t and 2 t + 1
+    uint2 qr[HALVES][kSteps];
+    float f[2], start[2];
+    split_queries<T, DP, HALVES>(raw, qr, f, start);
+    f[0] *= p.qk_scale;
+    f[1] *= p.qk_scale;
     const int limit0 = u.limit(p, 2 * t), limit1 = u.limit(p, 2 * t + 1);
     const int clear = min(u.limit(p, 0), k1);  // every row sees the keys below
     float* logit[2] = {nullptr, nullptr};
@@ -692,8 +726,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, PV, WHOLE>::kCtas)
     int last = 0;
     if (lane == 0) last = atomic_add_acq_rel_gpu(&p.counters[u.warp0], 1) == u.parts - 1;
     if (!__shfl_sync(0xffffffffu, last, 0)) continue;
-    // the last part to end joins all of them, in order: lane r the rows' factors,
-    // then a row at a time
+    // The last part to end joins all of them, in order: lane r has row r's factors, then a
+    // lane four channels of all rows, so that a part's loads are under way together.
     float by[kJoinHere] = {}, m = -INFINITY, sum = 0.0f;
     {
       float2 ml[kJoinHere];
@@ -710,36 +744,44 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, PV, WHOLE>::kCtas)
         sum += ml[i].y * by[i];
       }
     }
-    for (int r = 0; r < rows; ++r) {
-      int h;
-      const int64_t tok = u.token(p, r, &h);
-      const float mr = __shfl_sync(0xffffffffu, m, r), lr = __shfl_sync(0xffffffffu, sum, r);
-      if constexpr (PV) {
+    int h = 0;
+    const int64_t tok = lane < rows ? u.token(p, lane, &h) : 0;
+    if (lane < rows && p.lse != nullptr) p.lse[tok * p.heads + h] = row_lse(m, sum);
+    if constexpr (PV) {
+      const int64_t place = (tok * p.heads + h) * p.dim;
 #pragma unroll
-        for (int c = 0; c < (DP + 127) / 128; ++c) {
-          const int at = c * 128 + lane * 4;
-          float4 v[kJoinHere], acc = make_float4(0, 0, 0, 0);
+      for (int c = 0; c < (DP + 127) / 128; ++c) {
+        const int at = c * 128 + lane * 4;
+        float4 acc[kRows];
 #pragma unroll
-          for (int i = 0; i < kJoinHere; ++i) {
-            v[i] = make_float4(0, 0, 0, 0);
-            if (i < u.parts && at < DP)
-              v[i] = __ldcg(reinterpret_cast<const float4*>(
-                  reinterpret_cast<const float*>(u.slot<S::kBytes>(p, i)) + r * DP + at));
+        for (int r = 0; r < kRows; ++r) acc[r] = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < kJoinHere; ++i) {
+          if (i >= u.parts) break;
+          const float* from = reinterpret_cast<const float*>(u.slot<S::kBytes>(p, i)) + at;
+          float4 v[kRows];
+#pragma unroll
+          for (int r = 0; r < kRows; ++r) {
+            v[r] = make_float4(0, 0, 0, 0);
+            if (r < rows && at < DP) v[r] = __ldcg(reinterpret_cast<const float4*>(from + r * DP));
           }
 #pragma unroll
-          for (int i = 0; i < kJoinHere; ++i) {
+          for (int r = 0; r < kRows; ++r) {
             const float k = __shfl_sync(0xffffffffu, by[i], r);
             if (k == 0.0f) continue;
-            acc.x += v[i].x * k, acc.y += v[i].y * k, acc.z += v[i].z * k, acc.w += v[i].w * k;
+            acc[r].x += v[r].x * k, acc[r].y += v[r].y * k, acc[r].z += v[r].z * k, acc[r].w += v[r].w * k;
           }
-          const float inv = row_scale(lr);
-          if (at < p.dim)
-            store4(static_cast<T*>(p.out) + (tok * p.heads + h) * p.dim + at,
-                   lr == 0.0f ? make_float4(0, 0, 0, 0)
-                              : make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+        }
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+          const float l = __shfl_sync(0xffffffffu, sum, r), inv = row_scale(l);
+          const int64_t to = __shfl_sync(0xffffffffu, place, r);
+          if (r < rows && at < p.dim)
+            store4(static_cast<T*>(p.out) + to + at,
+                   l == 0.0f ? make_float4(0, 0, 0, 0)
+                             : make_float4(acc[r].x * inv, acc[r].y * inv, acc[r].z * inv, acc[r].w * inv));
         }
       }
-      if (lane == 0 && p.lse != nullptr) p.lse[tok * p.heads + h] = row_lse(mr, lr);
     }
   }
 }
@@ -755,14 +797,15 @@ __global__ void __launch_bounds__(1024, 1) join_kernel(const RowsParams p) {
   __shared__ float2 s_ml[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r = warp & 7, quarter = warp >> 3;
-  const int64_t share = rows_share(p);
+  const PlanHead head = *p.head;
+  if (head.most_parts <= kJoinHere) return;
   // the unit at the end of the eight shares, if it begins in them
   static_assert(kJoinHere >= kRowWarps, "one unit of more parts in so many warps");
-  const int64_t place = (int64_t)(blockIdx.x + 1) * kRowWarps * share - 1;
-  if (place >= p.head->places) return;
+  const int64_t place = (int64_t)(blockIdx.x + 1) * kRowWarps * head.share - 1;
+  if (place >= head.places) return;
   RowsUnit u;
   u.s = plan_find(p.seq, p.seqs, place);
-  u.find(p, place, share);
+  u.find(p, head, place);
   if (u.warp0 / kRowWarps != (int)blockIdx.x || u.parts <= kJoinHere) return;
   const int each = (u.parts + 3) / 4, i0 = quarter * each, i1 = min(i0 + each, u.parts);
   float m = -INFINITY, l = 0.0f;
@@ -915,6 +958,16 @@ ChunkLayout chunk_layout(const ChunkArgs& a) {
   return l;
 }
 
+// CTAs of a launch: no more warps than have their least part of the longest that the batch
+// can be.
+int64_t rows_ctas(const ChunkArgs& a, int per_sm) {
+  const int64_t units =
+      (a.total_q * (a.heads / a.kv_heads) / kRows + std::min<int64_t>(a.seqs, a.total_q) + 1) * a.kv_heads;
+  const int64_t parts = ((int64_t)a.width * a.block_size + kStep * kPartSteps - 1) / (kStep * kPartSteps) + 1;
+  const int64_t most = 148 * per_sm;
+  return std::min(most, units >= most * kRowWarps ? most : (units * parts + kRowWarps - 1) / kRowWarps);
+}
+
 template <typename T, int DP, bool PV, bool WHOLE>
 int launch_rows(const ChunkArgs& a, uint8_t* ws, cudaStream_t stream) {
   constexpr int HALVES = sizeof(T) == 4 ? 2 : 1;
@@ -950,12 +1003,7 @@ int launch_rows(const ChunkArgs& a, uint8_t* ws, cudaStream_t stream) {
   auto kern = rows_kernel<T, DP, HALVES, PV, WHOLE>;
   static std::atomic<uint64_t> done{0};
   allow_shared_memory(reinterpret_cast<const void*>(kern), C::kSmemBytes, done);
-  // no more warps than have their least share of the longest that the batch can be
-  const int64_t units = (a.total_q * p.group / kRows + std::min<int64_t>(a.seqs, a.total_q) + 1) * a.kv_heads;
-  const int64_t steps = ((int64_t)a.width * a.block_size + kStep - 1) / kStep + 1 + kOver;
-  const int64_t most = 148 * C::kCtas;
-  const int64_t each = (int64_t)kRowWarps * kLeast;
-  const int64_t ctas = std::min(most, units >= most * each ? most : (units * steps + each - 1) / each);
+  const int64_t ctas = rows_ctas(a, C::kCtas);
   p.warps = (int)ctas * kRowWarps;
   CUtensorMap map_k = {}, map_v = {};
   if (WHOLE && (!cache_map(&map_k, a.k_cache, a, DP, kStep, true) ||
@@ -966,7 +1014,7 @@ int launch_rows(const ChunkArgs& a, uint8_t* ws, cudaStream_t stream) {
   kern<<<(unsigned)ctas, kRowWarps * 32, C::kSmemBytes, stream>>>(map_k, map_v, p,
                                                                   device_error_word());
   // a unit of so many parts needs so many steps
-  if ((steps - kOver) > (int64_t)kLeast * (kJoinHere - 1))
+  if (((int64_t)a.width * a.block_size + kStep - 1) / kStep > (int64_t)kPartSteps * kJoinHere)
     join_kernel<T, DP, PV><<<(unsigned)ctas, 1024, 0, stream>>>(p);
   return kOk;
 }
@@ -1018,6 +1066,8 @@ int launch_chunk(const ChunkArgs& a, void* workspace, size_t workspace_bytes, cu
   plan.rows = kRows;
   plan.step = kStep;
   plan.over = kOver;
+  plan.workers = (int)rows_ctas(a, a.v_cache != nullptr && a.dim > 128 ? 1 : 2) * kRowWarps;
+  plan.least = kLeast;
   plan.which = d.tc ? kPlanFew : kPlanAll;
   plan.few_rows = kFewRows;
   plan.few_steps = d.rows ? kFewSteps : 0;

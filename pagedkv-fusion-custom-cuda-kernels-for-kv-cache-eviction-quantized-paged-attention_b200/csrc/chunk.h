@@ -97,6 +97,91 @@ __device__ __forceinline__ float load_if(bool on, const float* p) {
   return v;
 }
 
+// Query rows of a unit, as tcgen05 operands in shared memory: boxes of 64 fp16 channels,
+// rows of 128 bytes in the 128-byte swizzle, BOX bytes from one to the next; for fp32
+// queries boxes of hi, then of lo.  They arrive as they are, a warp its 32 rows, all on
+// their way at once (a quarter of them at a time through registers took 18,000 clocks of
+// a call's first unit, 5 us each), in the places that the row's own thread then writes:
+// of 4-byte channels, 32 a box, those 32 i .. are box i / 2, or (odd i) DP / 64 further.
+// `mine` is the lane's row, count how many of the warp's there are; the others, and
+// channels behind dim, are zero.
+template <typename T, int DP, int BOX>
+__device__ __forceinline__ void copy_query_rows(uint32_t tile, int row0, const T* any, const T* mine,
+                                                int count, int dim) {
+  constexpr int kPieces = DP * (int)sizeof(T) / 16;  // of 16 bytes, of a row
+  constexpr int kEach = 32 / kPieces;                // rows at once
+  const int lane = threadIdx.x & 31, piece = lane % kPieces;
+  const int c = piece * (16 / (int)sizeof(T)), box = piece / 8;
+  const uint32_t to = tile + (sizeof(T) == 4 ? box / 2 + box % 2 * (DP / 64) : box) * BOX;
+#pragma unroll 4
+  for (int i = 0; i < kPieces; ++i) {
+    const int r = i * kEach + lane / kPieces;
+    const T* from = reinterpret_cast<const T*>(
+        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), r));
+    const bool on = r < count && c < dim;
+    copy16_if(on, to + sw128_offset(row0 + r, piece % 8 * 16), on ? from + c : any);
+  }
+  copies_commit();
+  copies_wait<0>();
+  __syncwarp();
+}
+// The largest magnitude of a row's (infinity or NaN where there is one); nothing for fp16.
+template <typename T, int DP, int BOX>
+__device__ __forceinline__ float query_row_most(const uint8_t* tile, int row) {
+  uint32_t most = 0;
+#pragma unroll 4
+  for (int i = 0; i < DP * (int)sizeof(T) / 16; ++i) {
+    const uint4 w = *reinterpret_cast<const uint4*>(tile + i / 8 * BOX + sw128_offset(row, i % 8 * 16));
+    if constexpr (sizeof(T) == 4) {
+      constexpr uint32_t kAbs = 0x7fffffffu;
+      most = max(most, max(max(w.x & kAbs, w.y & kAbs), max(w.z & kAbs, w.w & kAbs)));
+    } else {
+      constexpr uint32_t kAbs = 0x7fff7fffu;
+      most = __vmaxu2(most, __vmaxu2(__vmaxu2(w.x & kAbs, w.y & kAbs), __vmaxu2(w.z & kAbs, w.w & kAbs)));
+    }
+  }
+  return __uint_as_float(sizeof(T) == 4 ? most : max(most << 16, most & 0xffff0000u));
+}
+// A row times the power of two `up`, in place (fp16 is as it is).
+template <typename T, int DP, int BOX>
+__device__ __forceinline__ void split_query_row(uint8_t* tile, int row, float up) {
+  const auto at = [&](int box, int piece) {
+    return reinterpret_cast<uint4*>(tile + box * BOX + sw128_offset(row, piece * 16));
+  };
+#pragma unroll 1
+  for (int b = 0; b < DP / 64; ++b) {
+    if constexpr (sizeof(T) == 4) {
+      uint4 w[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i] = *at(b + i / 8 * (DP / 64), i % 8);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint4 x = w[2 * i + e / 2];
+          const float f0 = __uint_as_float(e & 1 ? x.z : x.x) * up, f1 = __uint_as_float(e & 1 ? x.w : x.y) * up;
+          const __half2 a = __floats2half2_rn(f0, f1);
+          const float2 back = __half22float2(a);
+          h[e] = word_of(a);
+          l[e] = word_of(__floats2half2_rn(f0 - back.x, f1 - back.y));
+        }
+        *at(b, i) = make_uint4(h[0], h[1], h[2], h[3]);
+        *at(b + DP / 64, i) = make_uint4(l[0], l[1], l[2], l[3]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint4 x = *at(b, i);
+        const auto scaled = [&](uint32_t v) {
+          return word_of(__floats2half2_rn(__uint_as_float(v << 16) * up, __uint_as_float(v & 0xffff0000u) * up));
+        };
+        *at(b, i) = make_uint4(scaled(x.x), scaled(x.y), scaled(x.z), scaled(x.w));
+      }
+    }
+  }
+}
+
 constexpr int kChunkTcCtas = 148;  // one per SM
 
 // Whether the tensor-memory kernel takes this call's shapes.

@@ -459,61 +459,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int first_masked = max(u.limit(p, r - lane), 0) / kKeys - u.tile0;
       float rf = 1.0f;  // power of two that the row was divided by
       if (first < nt) {
-        // The warp takes its 32 rows one after the other, a lane per 4 channels; eight loads
-        // first, each row's address from the lane of the row.  A row's largest magnitude is
-        // scaled to [2^10, 2^11): exact, and lo's steps stay far below hi's.  (fp16 queries
-        // are as they are.)
-        constexpr int kBatch = 8;  // (a rolled loop: the code of more is fetched for longer)
-        const T* mine = nullptr;
+        // A row's largest magnitude is scaled to [2^10, 2^11): exact, and lo's steps stay far
+        // below hi's.  (fp16 queries are as they are.)
+        const T* any = static_cast<const T*>(p.q);
+        const T* mine = any;
         if (valid) {
           int h;
           const int64_t tok = u.token(p, r, &h);
-          mine = static_cast<const T*>(p.q) + tok * p.q_tok + h * p.q_head;
+          mine += tok * p.q_tok + h * p.q_head;
         }
-        const int count = min(u.rows - (r - lane), 32);  // of the warp's rows (or none)
-        const bool in = lane * 4 < p.dim;
-#pragma unroll 1
-        for (int i0 = 0; i0 < 32; i0 += kBatch) {
-          using Raw = std::conditional_t<sizeof(T) == 4, uint4, uint2>;
-          Raw raw[kBatch];
-#pragma unroll
-          for (int e = 0; e < kBatch; ++e) {
-            const T* from = reinterpret_cast<const T*>(
-                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), i0 + e));
-            raw[e] = Raw{};
-            if (i0 + e < count && in) raw[e] = *reinterpret_cast<const Raw*>(from + lane * 4);
-          }
-#pragma unroll
-          for (int e8 = 0; e8 < kBatch; ++e8) {
-            const int i = i0 + e8;
-            const float4 v = load4(reinterpret_cast<const T*>(&raw[e8]));
-            float up = 1.0f;
-            if constexpr (!std::is_same<T, __half>::value) {
-              float big = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
-              big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
-              const int e = row_exponent(big);
-              up = power_of_two(e);
-              if (lane == i) rf = power_of_two(-e);
-            }
-            const float f[4] = {v.x * up, v.y * up, v.z * up, v.w * up};
-            uint32_t hi[2], lo[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const __half2 h = __floats2half2_rn(f[2 * e], f[2 * e + 1]);
-              hi[e] = word_of(h);
-              if constexpr (HALVES == 2) {
-                const float2 b = __half22float2(h);
-                lo[e] = word_of(__floats2half2_rn(f[2 * e] - b.x, f[2 * e + 1] - b.y));
-              }
-            }
-            if (lane * 4 < DP) {
-              const uint32_t off = (lane / 16) * (kTileRows * 128) +
-                                   sw128_offset((warp & 3) * 32 + i, (lane % 16) * 8);
-              *reinterpret_cast<uint2*>(q_tile + off) = make_uint2(hi[0], hi[1]);
-              if constexpr (HALVES == 2)
-                *reinterpret_cast<uint2*>(q_tile + C::kTileBytes + off) = make_uint2(lo[0], lo[1]);
-            }
-          }
+        constexpr int kBox = kTileRows * 128;
+        copy_query_rows<T, DP, kBox>(smem_u32(q_tile), row - lane, any, mine, u.rows - (r - lane), p.dim);
+        if constexpr (!std::is_same<T, __half>::value) {
+          const int e = row_exponent(query_row_most<T, DP, kBox>(q_tile, row));
+          rf = power_of_two(-e);
+          split_query_row<T, DP, kBox>(q_tile, row, power_of_two(e));
         }
         fence_proxy_async_smem();  // an MMA operand
         mbar_arrive(&q_full[x]);
@@ -761,7 +721,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
       uint8_t* slot = slot_of<S::kBytes>(p, u, (int)blockIdx.x - u.cta0);
       const int rows = min(kTileRows, u.rows - r0);
-      // 32 channels at a time through shared memory, so that they leave in whole lines
+      // 32 channels at a time; whole units' through shared memory, so that they leave in
+      // whole lines, parts as [4 channels][row]
+      int to[8];  // the (token, head) of rows that this thread stores
+      if (whole && stores) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          int h;
+          const int64_t tok = u.token(p, r0 + min((row >> 3) + 16 * i, rows - 1), &h);
+          to[i] = (int)(tok * p.heads + h);
+        }
+      }
 #pragma unroll 1
       for (int c = 0; c < DP; c += 32) {
         float f[32];
@@ -784,26 +754,29 @@ __global__ void __launch_bounds__(kThreads, 1)
           named_barrier(4, 256);
         }
         if (!stores) continue;
-        const bool none = whole && l == 0.0f;
+        if (!whole) {
+          if (ok && valid)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float k = whole ? inv : 1.0f;
+            for (int e = 0; e < 8; ++e)
+              reinterpret_cast<float4*>(slot)[(c / 4 + e) * kUnitRows + r] =
+                  make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
+          continue;
+        }
+        const bool none = l == 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
           *reinterpret_cast<float4*>(stage + row * 128 + ((e ^ (row & 7)) * 16)) =
               none ? make_float4(0, 0, 0, 0)
-                   : make_float4(f[4 * e] * k, f[4 * e + 1] * k, f[4 * e + 2] * k, f[4 * e + 3] * k);
-        }
+                   : make_float4(f[4 * e] * inv, f[4 * e + 1] * inv, f[4 * e + 2] * inv, f[4 * e + 3] * inv);
         meet();
         const int piece = row & 7, at = c + piece * 4;
         if (ok && at < p.dim)
-          for (int i = row >> 3; i < rows; i += 16) {
-            const float4 v = *reinterpret_cast<const float4*>(stage + i * 128 + ((piece ^ (i & 7)) * 16));
-            if (whole) {
-              int h;
-              const int64_t tok = u.token(p, r0 + i, &h);
-              store4(static_cast<T*>(p.out) + (tok * p.heads + h) * p.dim + at, v);
-            } else {
-              *reinterpret_cast<float4*>(reinterpret_cast<float*>(slot) + (r0 + i) * DP + at) = v;
-            }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int from = (row >> 3) + 16 * i;
+            if (from < rows)
+              store4(static_cast<T*>(p.out) + (int64_t)to[i] * p.dim + at,
+                     *reinterpret_cast<const float4*>(stage + from * 128 + ((piece ^ (from & 7)) * 16)));
           }
         meet();  // the buffer is free
       }
@@ -826,12 +799,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
 }
 
-// Units that were cut: a warp per row, all parts in order.
-constexpr int kJoinRows = 32;  // of a CTA
+// Units that were cut: a CTA has 32 rows, lane = row, a warp every eighth 4 channels of
+// all parts in order; the rows leave through shared memory.
+constexpr int kJoinRows = 32, kJoinWarps = 8;
 template <typename T, int DP>
-__global__ void __launch_bounds__(256) join_tc_kernel(const TcParams p) {
+__global__ void __launch_bounds__(kJoinWarps * 32) join_tc_kernel(const TcParams p) {
   using S = TcSlot<DP>;
-  constexpr int kBatch = 4;
+  constexpr int kBatch = 4, kEach = DP / 4 / kJoinWarps;
+  __shared__ float4 s_out[kJoinRows][DP / 4 + 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t share = tile_share(p);
   // the unit at the end of the CTA's share, if it begins there
@@ -840,43 +815,60 @@ __global__ void __launch_bounds__(256) join_tc_kernel(const TcParams p) {
   TileUnit u;
   u.s = plan_find(p.seq, p.seqs, place);
   u.find(p, place, share);
-  if (u.cta0 != (int)blockIdx.x || u.parts == 1) return;
-  for (int r = blockIdx.y * kJoinRows + warp; r < min(u.rows, (int)(blockIdx.y + 1) * kJoinRows); r += 8) {
-    float m = -INFINITY, l = 0.0f;
-    float4 acc = make_float4(0, 0, 0, 0);
-    const bool in = lane * 4 < p.dim;
-    for (int i = 0; i < u.parts; i += kBatch) {
-      float2 ml[kBatch];
-      float4 v[kBatch];
+  const int row0 = blockIdx.y * kJoinRows, r = row0 + lane;
+  if (u.cta0 != (int)blockIdx.x || u.parts == 1 || row0 >= u.rows) return;
+  const bool valid = r < u.rows;
+  float m = -INFINITY, l = 0.0f;
+  float4 acc[kEach];
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
-        const bool there = i + b < u.parts;
-        const uint8_t* from = slot_of<S::kBytes>(p, u, there ? i + b : i);
-        ml[b] = there ? __ldcg(reinterpret_cast<const float2*>(from + S::kMl) + r)
-                      : make_float2(-INFINITY, 0.0f);
-        v[b] = in ? __ldcg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(from) + r * DP + lane * 4))
-                  : make_float4(0, 0, 0, 0);
-      }
+  for (int c = 0; c < kEach; ++c) acc[c] = make_float4(0, 0, 0, 0);
+#pragma unroll 1
+  for (int i = 0; i < u.parts; i += kBatch) {
+    float2 ml[kBatch];
+    float4 v[kBatch][kEach];
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
-        if (ml[b].x == -INFINITY) continue;
-        const float big = fmaxf(m, ml[b].x);
-        const float f = m == -INFINITY ? 0.0f : ex2(m - big), k = ex2(ml[b].x - big);
-        m = big;
-        l = l * f + ml[b].y * k;
-        acc.x = acc.x * f + v[b].x * k, acc.y = acc.y * f + v[b].y * k;
-        acc.z = acc.z * f + v[b].z * k, acc.w = acc.w * f + v[b].w * k;
+    for (int b = 0; b < kBatch; ++b) {
+      const bool there = valid && i + b < u.parts;
+      const uint8_t* from = slot_of<S::kBytes>(p, u, i + b < u.parts ? i + b : i);
+      ml[b] = there ? __ldcg(reinterpret_cast<const float2*>(from + S::kMl) + r)
+                    : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+      for (int c = 0; c < kEach; ++c)
+        v[b][c] = there ? __ldcg(reinterpret_cast<const float4*>(from) + (warp + c * kJoinWarps) * kUnitRows + r)
+                        : make_float4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      if (ml[b].x == -INFINITY) continue;
+      const float big = fmaxf(m, ml[b].x);
+      const float f = m == -INFINITY ? 0.0f : ex2(m - big), k = ex2(ml[b].x - big);
+      m = big;
+      l = l * f + ml[b].y * k;
+#pragma unroll
+      for (int c = 0; c < kEach; ++c) {
+        acc[c].x = acc[c].x * f + v[b][c].x * k, acc[c].y = acc[c].y * f + v[b][c].y * k;
+        acc[c].z = acc[c].z * f + v[b][c].z * k, acc[c].w = acc[c].w * f + v[b][c].w * k;
       }
     }
+  }
+  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+#pragma unroll
+  for (int c = 0; c < kEach; ++c)
+    s_out[lane][warp + c * kJoinWarps] =
+        l == 0.0f ? make_float4(0, 0, 0, 0)
+                  : make_float4(acc[c].x * inv, acc[c].y * inv, acc[c].z * inv, acc[c].w * inv);
+  if (warp == 0 && valid && p.lse != nullptr) {
     int h;
     const int64_t tok = u.token(p, r, &h);
-    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    if (in)
-      store4(static_cast<T*>(p.out) + (tok * p.heads + h) * p.dim + lane * 4,
-             l == 0.0f ? make_float4(0, 0, 0, 0)
-                       : make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
-    if (lane == 0 && p.lse != nullptr)
-      p.lse[tok * p.heads + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * (1.0f / kLog2e);
+    p.lse[tok * p.heads + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * (1.0f / kLog2e);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = warp; i < kJoinRows; i += kJoinWarps) {
+    if (row0 + i >= u.rows || lane * 4 >= p.dim) continue;
+    int h;
+    const int64_t tok = u.token(p, row0 + i, &h);
+    store4(static_cast<T*>(p.out) + (tok * p.heads + h) * p.dim + lane * 4, s_out[i][lane]);
   }
 }
 
@@ -945,7 +937,7 @@ int launch_tc(const ChunkArgs& a, PlanHead* head, PlanSeq* seq, uint8_t* ws, boo
   }
   kern<<<(unsigned)ctas, kThreads, C::kSmemBytes, stream>>>(map_k, map_v, p, device_error_word());
   if (ctas > 1)
-    join_tc_kernel<T, DP><<<dim3((unsigned)ctas, kUnitRows / kJoinRows), 256, 0, stream>>>(p);
+    join_tc_kernel<T, DP><<<dim3((unsigned)ctas, kUnitRows / kJoinRows), kJoinWarps * 32, 0, stream>>>(p);
   return kOk;
 }
 
@@ -966,6 +958,7 @@ PlanArgs chunk_tc_plan(const PlanArgs& base) {
   p.rows = kUnitRows;
   p.step = kKeys;
   p.over = kOver;
+  p.workers = p.least = 0;
   p.counters = nullptr;
   p.counts = 0;
   return p;

@@ -366,6 +366,7 @@ int launch_accumulate(const ChunkArgs& a, float* weights, void* workspace, size_
     plan.rows = kItemRows;
     plan.step = kKeys;
     plan.over = 0;
+    plan.workers = plan.least = 0;
     plan.which = kPlanAll;
     plan.few_rows = plan.few_steps = 0;
     plan.head = reinterpret_cast<PlanHead*>(ws + lay.head);

@@ -271,83 +271,35 @@ __global__ void __launch_bounds__(kThreads, 1)
       named_barrier(2, 256);  // both warpgroups have seen every product of the last segment
       float down = 1.0f;      // what the products are multiplied by, for the power of two
       {
-        // thread = row for its denominator and how far it sees; a warp its 32 rows' queries,
-        // a lane per 4 channels, eight loads first
+        // thread = row: its denominator, how far it sees, and its queries
         const int r = tid;
-        const T* mine = nullptr;
+        const T* any = static_cast<const T*>(p.q);
+        const T* mine = any;
         float lse2 = INFINITY;  // rows that are not there, or see nothing, add nothing
         if (r < u.rows) {
           int h;
           const int64_t tok = u.token(p, r, &h);
-          mine = static_cast<const T*>(p.q) + tok * p.q_tok + h * p.q_head;
+          mine += tok * p.q_tok + h * p.q_head;
           const float v = p.lse[tok * p.heads + h];
           if (v != -INFINITY) lse2 = v * kLog2e;
         }
         s_lse[r] = lse2;
         s_limit[r] = u.limit(p, r);
-        const int count = u.rows - (r - lane);
-        const bool in = lane * 4 < p.dim;
-        using Raw = std::conditional_t<sizeof(T) == 4, uint4, uint2>;
-        const auto load8 = [&](int i0, Raw (&raw)[8]) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const T* from = reinterpret_cast<const T*>(
-                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), i0 + e));
-            raw[e] = Raw{};
-            if (i0 + e < count && in) raw[e] = *reinterpret_cast<const Raw*>(from + lane * 4);
-          }
-        };
-        float up = 1.0f;
+        constexpr int kBox = kRows * 128;
+        uint8_t* tile = smem + C::kOffQ;
+        copy_query_rows<T, DP, kBox>(smem_u32(tile), r - lane, any, mine, u.rows - (r - lane), p.dim);
         if constexpr (!std::is_same<T, __half>::value) {
           // the largest of the unit is scaled to [2^10, 2^11): what rows of smaller ones lose
           // is below 2^-36 of it
-          float big = 0.0f;
-#pragma unroll 1
-          for (int i0 = 0; i0 < 32 && i0 < count; i0 += 8) {
-            Raw raw[8];
-            load8(i0, raw);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float4 v = load4(reinterpret_cast<const T*>(&raw[e]));
-              const float a = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
-              big = fmaxf(big, a <= 3.0e38f ? a : 0.0f);
-            }
-          }
+          float big = query_row_most<T, DP, kBox>(tile, r);
+          big = big <= 3.0e38f ? big : 0.0f;  // (the row's weights are NaN anyway)
           big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
           if (lane == 0) s_big[warp] = big;
           named_barrier(2, 256);
           for (int w = 0; w < 8; ++w) big = fmaxf(big, s_big[w]);
           const int e = row_exponent(big);
-          up = power_of_two(e);
           down = power_of_two(-e);
-        }
-        uint8_t* tile = smem + C::kOffQ;
-#pragma unroll 1
-        for (int i0 = 0; i0 < 32; i0 += 8) {
-          Raw raw[8];
-          load8(i0, raw);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float4 v = load4(reinterpret_cast<const T*>(&raw[e]));
-            const float f[4] = {v.x * up, v.y * up, v.z * up, v.w * up};
-            uint32_t hi[2], lo[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const __half2 h = __floats2half2_rn(f[2 * k], f[2 * k + 1]);
-              hi[k] = word_of(h);
-              if constexpr (HALVES == 2) {
-                const float2 b = __half22float2(h);
-                lo[k] = word_of(__floats2half2_rn(f[2 * k] - b.x, f[2 * k + 1] - b.y));
-              }
-            }
-            if (lane * 4 < DP) {
-              const uint32_t off = (lane / 16) * (kRows * 128) +
-                                   sw128_offset(warp * 32 + i0 + e, (lane % 16) * 8);
-              *reinterpret_cast<uint2*>(tile + off) = make_uint2(hi[0], hi[1]);
-              if constexpr (HALVES == 2)
-                *reinterpret_cast<uint2*>(tile + C::kQBytes + off) = make_uint2(lo[0], lo[1]);
-            }
-          }
+          split_query_row<T, DP, kBox>(tile, r, power_of_two(e));
         }
         fence_proxy_async_smem();  // an MMA operand
         mbar_arrive(q_full);
