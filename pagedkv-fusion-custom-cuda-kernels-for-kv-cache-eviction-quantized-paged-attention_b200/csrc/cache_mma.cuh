@@ -17,6 +17,31 @@ namespace pkv {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// A kernel that may be launched while the one in front of it in the stream still runs
+// (programmatic dependent launch): it sets up what needs nothing of that one, and waits
+// for its end, and so for everything earlier, in behind_the_last().  Every thread of every
+// kernel of such a row calls that before it reads or writes global memory, and the kernels
+// in front let the next be launched at their start.  (A call is a row of two to six kernels of
+// 2 us and more.)
+__device__ __forceinline__ void behind_the_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void launch_the_next() { asm volatile("griddepcontrol.launch_dependents;"); }
+
+template <typename... Params, typename... Args>
+inline void launch_behind(void (*kernel)(Params...), dim3 grid, int threads, size_t shared,
+                          cudaStream_t stream, Args... args) {
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3((unsigned)threads);
+  config.dynamicSmemBytes = shared;
+  config.stream = stream;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  cudaLaunchKernelEx(&config, kernel, Params(args)...);  // (errors: cudaGetLastError, as after <<<>>>)
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -72,6 +72,7 @@ __device__ __forceinline__ int64_t scan_sum(int64_t v, int64_t* shared, int64_t*
 __global__ void __launch_bounds__(kPlanThreads)
     plan_kernel(const PlanArgs first_plan, const PlanArgs second_plan, int plans, const ZeroArgs z,
                 int* err) {
+  launch_the_next();
   if ((int)blockIdx.x >= plans) {
     const int64_t per_seq = (int64_t)z.width * z.block_size, slots = per_seq * z.seqs;
     const int64_t step = (int64_t)(gridDim.x - plans) * kPlanThreads;
@@ -342,6 +343,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, PV, WHOLE>::kCtas)
     hold = l2_policy_evict_first();
   }
 
+  launch_the_next();
+  behind_the_last();
   const PlanHead head = *p.head;
   // Of the grid.  Where there is work for few warps they are on all SMs; neighbours in
   // the plan, which read other heads of the same pages, are in the same CTA (64 sequences
@@ -797,6 +800,8 @@ __global__ void __launch_bounds__(1024, 1) join_kernel(const RowsParams p) {
   __shared__ float2 s_ml[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r = warp & 7, quarter = warp >> 3;
+  launch_the_next();
+  behind_the_last();
   const PlanHead head = *p.head;
   if (head.most_parts <= kJoinHere) return;
   // the unit at the end of the eight shares, if it begins in them
@@ -1011,11 +1016,11 @@ int launch_rows(const ChunkArgs& a, uint8_t* ws, cudaStream_t stream) {
     set_error("cuTensorMapEncodeTiled failed for the caches");
     return kCudaError;
   }
-  kern<<<(unsigned)ctas, kRowWarps * 32, C::kSmemBytes, stream>>>(map_k, map_v, p,
-                                                                  device_error_word());
+  launch_behind(kern, dim3((unsigned)ctas), kRowWarps * 32, C::kSmemBytes, stream, map_k, map_v, p,
+                device_error_word());
   // a unit of so many parts needs so many steps
   if (((int64_t)a.width * a.block_size + kStep - 1) / kStep > (int64_t)kPartSteps * kJoinHere)
-    join_kernel<T, DP, PV><<<(unsigned)ctas, 1024, 0, stream>>>(p);
+    launch_behind(join_kernel<T, DP, PV>, dim3((unsigned)ctas), 1024, 0, stream, p);
   return kOk;
 }
 

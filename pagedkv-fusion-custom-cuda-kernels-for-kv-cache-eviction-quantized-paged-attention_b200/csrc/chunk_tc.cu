@@ -128,23 +128,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const PlanHead head = *p.head;
-  const int64_t share = tile_share(p);
-  const int64_t begin = blockIdx.x * share, stop = min(begin + share, head.places);
-  // rows in front of the first and behind the last sequence become zero
-  if (p.zero_rows) {
-    const int64_t front = (int64_t)head.q_begin * p.heads;
-    const int64_t behind = (int64_t)head.q_end * p.heads;
-    const int64_t outside = front + (int64_t)p.total_q * p.heads - behind;
-    for (int64_t i = blockIdx.x * (kThreads / 32) + warp; i < outside; i += gridDim.x * (kThreads / 32)) {
-      const int64_t r = i < front ? i : behind + i - front;
-      for (int c = lane * 4; c < p.dim; c += 128)
-        store4(static_cast<T*>(p.out) + r * p.dim + c, make_float4(0, 0, 0, 0));
-      if (lane == 0 && p.lse != nullptr) p.lse[r] = -INFINITY;
-    }
-  }
-  if (begin >= stop) return;
-
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&kv_full[i], 128);
@@ -163,6 +146,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(mma_done, 2);
     mbar_fence_init();
   }
+  launch_the_next();
+  behind_the_last();
+  const PlanHead head = *p.head;
+  const int64_t share = tile_share(p);
+  const int64_t begin = blockIdx.x * share, stop = min(begin + share, head.places);
+  // rows in front of the first and behind the last sequence become zero
+  if (p.zero_rows) {
+    const int64_t front = (int64_t)head.q_begin * p.heads;
+    const int64_t behind = (int64_t)head.q_end * p.heads;
+    const int64_t outside = front + (int64_t)p.total_q * p.heads - behind;
+    for (int64_t i = blockIdx.x * (kThreads / 32) + warp; i < outside; i += gridDim.x * (kThreads / 32)) {
+      const int64_t r = i < front ? i : behind + i - front;
+      for (int c = lane * 4; c < p.dim; c += 128)
+        store4(static_cast<T*>(p.out) + r * p.dim + c, make_float4(0, 0, 0, 0));
+      if (lane == 0 && p.lse != nullptr) p.lse[r] = -INFINITY;
+    }
+  }
+  if (begin >= stop) return;
+
   if (warp == kMmaWarp) tmem_alloc(s_tmem, 512);
   tmem_fence_before_sync();
   __syncthreads();
@@ -808,6 +810,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_tc_kernel(const TcParams
   constexpr int kBatch = 4, kEach = DP / 4 / kJoinWarps;
   __shared__ float4 s_out[kJoinRows][DP / 4 + 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  launch_the_next();
+  behind_the_last();
   const int64_t share = tile_share(p);
   // the unit at the end of the CTA's share, if it begins there
   const int64_t place = (int64_t)(blockIdx.x + 1) * share - 1;
@@ -935,9 +939,11 @@ int launch_tc(const ChunkArgs& a, PlanHead* head, PlanSeq* seq, uint8_t* ws, boo
     set_error("cuTensorMapEncodeTiled failed for the caches");
     return kCudaError;
   }
-  kern<<<(unsigned)ctas, kThreads, C::kSmemBytes, stream>>>(map_k, map_v, p, device_error_word());
+  launch_behind(kern, dim3((unsigned)ctas), kThreads, C::kSmemBytes, stream, map_k, map_v, p,
+                device_error_word());
   if (ctas > 1)
-    join_tc_kernel<T, DP><<<dim3((unsigned)ctas, kUnitRows / kJoinRows), kJoinWarps * 32, 0, stream>>>(p);
+    launch_behind(join_tc_kernel<T, DP>, dim3((unsigned)ctas, kUnitRows / kJoinRows), kJoinWarps * 32, 0,
+                  stream, p);
   return kOk;
 }
 

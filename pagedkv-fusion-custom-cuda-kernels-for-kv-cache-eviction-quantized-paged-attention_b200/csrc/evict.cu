@@ -7,7 +7,7 @@
 // was smaller, and move as they are else.  The weights move along; the slots behind the
 // last token that were in use get weight 0.
 //
-//   pick_kernel   a CTA per sequence: the weights' sort keys, the key that the last
+//   pick_kernel   a CTA or a cluster per sequence: the weights' sort keys, the key that the last
 //                 kept token has (radix, 8 bits a pass), the kept tokens in order;
 //   move_kernel   a cluster per (sequence, K or V, KV head), and one per sequence for
 //                 the weights.
@@ -21,6 +21,7 @@
 #include <algorithm>
 #include <string>
 
+#include "cache_mma.cuh"
 #include "pkv_common.cuh"
 #include "pkv_internal.h"
 
@@ -62,20 +63,28 @@ __device__ __forceinline__ int2 before_me(int2 v, int2* shared, int2* all) {
   return make_int2(front.x + incl.x - v.x, front.y + incl.y - v.y);
 }
 
+// A cluster of `ctas` CTAs per sequence, each with a part of its tokens in their order: of
+// long sequences where there are few (one of 32,768 tokens: 30 us in one CTA).
 template <bool ON_CHIP>
-__global__ void __launch_bounds__(kPickThreads) pick_kernel(const PickParams p, int* err) {
+__global__ void __launch_bounds__(kPickThreads) pick_kernel(const PickParams p, int ctas, int* err) {
   extern __shared__ uint32_t s_keys[];  // ON_CHIP: key i at i + i / 32
-  __shared__ int s_count[256];
-  __shared__ int2 s_scan[kPickThreads / 32];
+  __shared__ int s_count[2][256], s_sum[256];
+  __shared__ int2 s_scan[kPickThreads / 32], s_all;
   __shared__ int s_bad, s_digit, s_above;
-  const int tid = threadIdx.x, s = blockIdx.x;
+  launch_the_next();
+  const int tid = threadIdx.x, s = blockIdx.x / ctas, rank = blockIdx.x % ctas;
+  auto cluster = cooperative_groups::this_cluster();
+  const auto meet = [&]() {
+    if (ctas > 1) cluster.sync();
+    else __syncthreads();
+  };
   const int32_t* table = p.tables + (int64_t)s * p.width;
   const int64_t room = (int64_t)p.width * p.bs;
   const int given = max(p.lens[s], 0);
   const int len = (int)min((int64_t)given, room);
   if (tid == 0) {
     s_bad = 0;
-    if (given > len) record_error(err, kDevSeqTooLong);
+    if (given > len && rank == 0) record_error(err, kDevSeqTooLong);
   }
   __syncthreads();
   int32_t* kept = p.kept + (int64_t)s * p.keep;
@@ -87,7 +96,8 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const PickParams p, 
     }
   }
   __syncthreads();
-  if (len <= p.keep || s_bad) {  // stays as it is
+  if (len <= p.keep || s_bad) {  // stays as it is (a cluster's CTAs all see that)
+    if (rank > 0) return;
     if (tid == 0) {
       p.lens_out[s] = len;
       if (s_bad) record_error(err, kDevBadBlockId);
@@ -95,39 +105,55 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const PickParams p, 
     for (int i = tid; i < p.keep; i += kPickThreads) kept[i] = !s_bad && i < len ? i : -1;
     return;
   }
-  // Tokens [sinks, sinks + n) compete for `want` places; the largest key wins.
+  // Tokens [sinks, sinks + n) compete for `want` places; the largest key wins.  This CTA
+  // has `mine` of them from `from` on.
   const int n = len - p.sinks - p.recent, want = p.keep - p.sinks - p.recent;
+  const int each = (n + ctas - 1) / ctas;
+  const int from = min(rank * each, n), mine = min(each, n - from);
   const auto key_of = [&](int i) {
-    const int at = p.sinks + i, page = at / p.bs;
-    return orderable_key(p.weights[(int64_t)table[page] * p.bs + (at - page * p.bs)]);
+    const int at = p.sinks + from + i, page = at / p.bs;
+    return orderable_key(__ldg(p.weights + (int64_t)__ldg(table + page) * p.bs + (at - page * p.bs)));
   };
   const auto key_at = [&](int i) { return ON_CHIP ? s_keys[i + i / 32] : key_of(i); };
-  if (ON_CHIP)
-    for (int i = tid; i < n; i += kPickThreads) s_keys[i + i / 32] = key_of(i);
+  if (ON_CHIP) {
+#pragma unroll 8
+    for (int i = tid; i < mine; i += kPickThreads) s_keys[i + i / 32] = key_of(i);
+  }
   uint32_t prefix = 0;  // of the key that the last kept token has
   int left = want;      // places for keys that begin with prefix
   for (int shift = 24; shift >= 0 && want > 0; shift -= 8) {
+    // (two buffers: the others may still read the last pass's)
+    int* count = s_count[shift / 8 & 1];
     __syncthreads();
-    if (tid < 256) s_count[tid] = 0;
+    if (tid < 256) count[tid] = 0;
     __syncthreads();
-    for (int i = tid; i < n; i += kPickThreads) {
+    for (int i = tid; i < mine; i += kPickThreads) {
       const uint32_t k = key_at(i);
-      if (shift == 24 || (k ^ prefix) >> (shift + 8) == 0) atomicAdd(&s_count[k >> shift & 255u], 1);
+      if (shift == 24 || (k ^ prefix) >> (shift + 8) == 0) atomicAdd(&count[k >> shift & 255u], 1);
     }
-    __syncthreads();
+    meet();
+    if (ctas > 1) {
+      if (tid < 256) {
+        int sum = 0;
+        for (int c = 0; c < ctas; ++c) sum += cluster.map_shared_rank(count, c)[tid];
+        s_sum[tid] = sum;
+      }
+      __syncthreads();
+      count = s_sum;
+    }
     if (tid < 32) {  // from the top: 8 digits a lane
-      int mine = 0;
-      for (int d = 0; d < 8; ++d) mine += s_count[255 - (tid * 8 + d)];
-      int incl = mine;
+      int here = 0;
+      for (int d = 0; d < 8; ++d) here += count[255 - (tid * 8 + d)];
+      int incl = here;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int x = __shfl_up_sync(0xffffffffu, incl, o);
         if (tid >= o) incl += x;
       }
-      int above = incl - mine;
+      int above = incl - here;
       if (above < left && incl >= left) {
         int d = 0;
-        while (above + s_count[255 - (tid * 8 + d)] < left) above += s_count[255 - (tid * 8 + d++)];
+        while (above + count[255 - (tid * 8 + d)] < left) above += count[255 - (tid * 8 + d++)];
         s_digit = 255 - (tid * 8 + d);
         s_above = above;
       }
@@ -138,8 +164,8 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const PickParams p, 
   }
   __syncthreads();
   // Each thread has a run of tokens: how many of them are above the key, and at it.
-  const int run = (n + kPickThreads - 1) / kPickThreads;
-  const int i0 = min(tid * run, n), i1 = min(i0 + run, n);
+  const int run = (mine + kPickThreads - 1) / kPickThreads;
+  const int i0 = min(tid * run, mine), i1 = min(i0 + run, mine);
   int2 v = make_int2(0, 0);
   if (want > 0)
     for (int i = i0; i < i1; ++i) {
@@ -148,18 +174,30 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const PickParams p, 
       v.y += k == prefix;
     }
   int2 all;
-  const int2 front = before_me(v, s_scan, &all);
+  int2 front = before_me(v, s_scan, &all);
+  if (ctas > 1) {  // and of the parts in front
+    if (tid == 0) s_all = all;
+    cluster.sync();
+    for (int c = 0; c < rank; ++c) {
+      const int2 x = *cluster.map_shared_rank(&s_all, c);
+      front.x += x.x;
+      front.y += x.y;
+    }
+    cluster.sync();  // nobody leaves while the others read
+  }
   if (want > 0) {
     int equal = front.y, to = p.sinks + front.x + min(front.y, left);
     for (int i = i0; i < i1; ++i) {
       const uint32_t k = key_at(i);
-      if (k > prefix || (k == prefix && equal < left)) kept[to++] = p.sinks + i;
+      if (k > prefix || (k == prefix && equal < left)) kept[to++] = p.sinks + from + i;
       equal += k == prefix;
     }
   }
-  for (int i = tid; i < p.sinks; i += kPickThreads) kept[i] = i;
-  for (int i = tid; i < p.recent; i += kPickThreads) kept[p.keep - p.recent + i] = len - p.recent + i;
-  if (tid == 0) p.lens_out[s] = p.keep;
+  const int step = ctas * kPickThreads;
+  for (int i = rank * kPickThreads + tid; i < p.sinks; i += step) kept[i] = i;
+  for (int i = rank * kPickThreads + tid; i < p.recent; i += step)
+    kept[p.keep - p.recent + i] = len - p.recent + i;
+  if (tid == 0 && rank == 0) p.lens_out[s] = p.keep;
 }
 
 // ---------------------------------------------------------------------------
@@ -167,8 +205,8 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const PickParams p, 
 // ---------------------------------------------------------------------------
 
 constexpr int kMoveThreads = 256;
-constexpr int kRound = 128;  // at most so many tokens of a CTA in a round
-constexpr int kHeld = 4;     // pieces that a thread holds
+constexpr int kIndex = 1024;  // tokens of a CTA whose places are looked up at once
+constexpr int kHeld = 4;      // pieces that a thread holds
 
 struct MoveParams {
   int8_t* cache;
@@ -192,15 +230,18 @@ struct Piece<4> { using T = uint32_t; };
 template <>
 struct Piece<1> { using T = uint8_t; };
 
+// rint(code ratio) of four codes.  A byte in the low mantissa of 2^23 is a number, and a
+// number at 1.5 2^23 is rounded to an integer, to even as rint, whose low byte is there: the
+// conversion instructions, 16 a clock and SM, would take 90 us of the 64 sequences' move.
 __device__ __forceinline__ uint32_t shrink4(uint32_t w, float ratio) {
-  uint32_t r = 0;
+  const uint32_t u = w ^ 0x80808080u;
+  uint32_t x[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float x = (float)(int8_t)(w >> (8 * i)) * ratio;
-    const int c = (int)fminf(fmaxf(rintf(x), -127.0f), 127.0f);
-    r |= (uint32_t)(c & 255) << (8 * i);
+    const float code = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + i)) - 8388736.0f;
+    x[i] = __float_as_uint(fminf(fmaxf(code * ratio, -127.0f), 127.0f) + 12582912.0f);
   }
-  return r;
+  return __byte_perm(__byte_perm(x[0], x[1], 0x0040), __byte_perm(x[2], x[3], 0x0040), 0x5410);
 }
 __device__ __forceinline__ uint4 shrink(uint4 v, float f) {
   return make_uint4(shrink4(v.x, f), shrink4(v.y, f), shrink4(v.z, f), shrink4(v.w, f));
@@ -211,8 +252,9 @@ __device__ __forceinline__ uint8_t shrink(uint8_t v, float f) { return (uint8_t)
 template <int VEC>
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const MoveParams p, int ctas) {
   using V = typename Piece<VEC>::T;
-  __shared__ int64_t s_from[kRound], s_to[kRound];  // token slots of the cache
-  __shared__ float s_old[kRound], s_new[kRound];
+  __shared__ int s_from[kIndex], s_to[kIndex];  // token slots of the cache
+  __shared__ float s_old[kIndex], s_new[kIndex];
+  behind_the_last();
   const int tid = threadIdx.x;
   const int rank = blockIdx.x % ctas;
   const int chain = blockIdx.x / ctas;
@@ -230,14 +272,14 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const MoveParams p, 
   };
   const auto slot_of = [&](int at) {
     const int page = at / p.bs;
-    return (int64_t)table[page] * p.bs + (at - page * p.bs);
+    return table[page] * p.bs + (at - page * p.bs);
   };
   if (kind == 2 * p.kv_heads) {  // the weights
     const int round = kMoveThreads * ctas;
     for (int r0 = 0; r0 < kept_n; r0 += round) {
       const int i = r0 + rank * kMoveThreads + tid;
       float w = 0.0f;
-      int64_t to = 0;
+      int to = 0;
       if (i < kept_n) {
         w = p.weights[slot_of(kept[i])];
         to = slot_of(i);
@@ -255,74 +297,105 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const MoveParams p, 
   const int64_t token_bytes = (int64_t)p.kv_heads * p.dim;
   const int pieces = p.dim / VEC;
   // Whole pages a round, as many tokens as the threads hold, in several passes over the
-  // channels where that is less than a page.
-  const int fit = min(kRound, kMoveThreads * kHeld / pieces);
+  // channels where that is less than a page.  The rounds' places and scales are looked up
+  // many at a time: a round that began with its own took 14 us (kept, table, scale and codes
+  // one behind the other).
+  const int fit = min(kIndex, kMoveThreads * kHeld / pieces);
   const int round = max(fit / p.bs, 1) * p.bs;
   const int per = min(pieces, kMoveThreads * kHeld / round);
-  for (int r0 = rank * round; r0 - rank * round < kept_n; r0 += round * ctas) {
-    const int n = max(min(round, kept_n - r0), 0);
-    for (int i = tid; i < n; i += kMoveThreads) {
-      const int at = kept[r0 + i], page = at / p.bs;
-      s_from[i] = (int64_t)table[page] * p.bs + (at - page * p.bs);
-      s_to[i] = slot_of(r0 + i);
-      s_old[i] = scales[(int64_t)table[page] * p.kv_heads];
+  const int rounds = (kept_n + round * ctas - 1) / (round * ctas), at_once = kIndex / round;
+  for (int g0 = 0; g0 < rounds; g0 += at_once) {
+    const int some = min(at_once, rounds - g0);
+    // the place among the kept ones of the CTA's i-th token of these rounds
+    const auto token_of = [&](int i) {
+      const int g = i / round;
+      return ((g0 + g) * ctas + rank) * round + i - g * round;
+    };
+#pragma unroll 4
+    for (int i = tid; i < some * round; i += kMoveThreads) {
+      const int t = token_of(i);
+      if (t < kept_n) {
+        const int at = kept[t], page = at / p.bs, phys = table[page];
+        s_from[i] = phys * p.bs + (at - page * p.bs);
+        s_to[i] = slot_of(t);
+        s_old[i] = scales[(int64_t)phys * p.kv_heads];
+      }
     }
     __syncthreads();
-    for (int i = tid * p.bs; i < n; i += kMoveThreads * p.bs) {
+    for (int i = tid * p.bs; i < some * round; i += kMoveThreads * p.bs) {
+      const int n = min(p.bs, kept_n - token_of(i));
+      if (n <= 0) continue;
       float most = s_old[i];
-      const int end = min(i + p.bs, n);
-      for (int j = i + 1; j < end; ++j) {
-        const float x = s_old[j];
+      for (int j = 1; j < n; ++j) {
+        const float x = s_old[i + j];
         asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(x));
       }
-      for (int j = i; j < end; ++j) s_new[j] = most;
+      s_new[i / p.bs] = most;
+      // what the codes are multiplied by; 1: they move as they are
+      for (int j = 0; j < n; ++j) s_old[i + j] = s_old[i + j] < most ? s_old[i + j] / most : 1.0f;
     }
-    for (int c0 = 0; c0 < pieces; c0 += per) {
-      const int m = min(per, pieces - c0);
-      V held[kHeld];
+    __syncthreads();
+    for (int g = 0; g < some; ++g) {
+      const int base = g * round;
+      const int n = max(min(round, kept_n - token_of(base)), 0);
+      for (int c0 = 0; c0 < pieces; c0 += per) {
+        const int m = min(per, pieces - c0);
+        V held[kHeld];
 #pragma unroll
-      for (int u = 0; u < kHeld; ++u) {
-        const int x = u * kMoveThreads + tid, i = x / m;
-        if (i < n)
-          held[u] = *reinterpret_cast<const V*>(cache + s_from[i] * token_bytes +
-                                                (c0 + x - i * m) * VEC);
-      }
-      meet();
+        for (int u = 0; u < kHeld; ++u) {
+          const int x = u * kMoveThreads + tid, i = x / m;
+          if (i < n)
+            held[u] = *reinterpret_cast<const V*>(cache + s_from[base + i] * token_bytes +
+                                                  (c0 + x - i * m) * VEC);
+        }
+        meet();
 #pragma unroll
-      for (int u = 0; u < kHeld; ++u) {
-        const int x = u * kMoveThreads + tid, i = x / m;
-        if (i < n) {
-          const float old = s_old[i], now = s_new[i];
-          V c = held[u];
-          if (old < now) c = shrink(c, old / now);
-          *reinterpret_cast<V*>(cache + s_to[i] * token_bytes + (c0 + x - i * m) * VEC) = c;
+        for (int u = 0; u < kHeld; ++u) {
+          const int x = u * kMoveThreads + tid, i = x / m;
+          if (i < n) {
+            const float ratio = s_old[base + i];
+            V c = held[u];
+            if (ratio != 1.0f) c = shrink(c, ratio);
+            *reinterpret_cast<V*>(cache + s_to[base + i] * token_bytes + (c0 + x - i * m) * VEC) = c;
+          }
         }
       }
     }
-    for (int i = tid * p.bs; i < n; i += kMoveThreads * p.bs)
-      scales[s_to[i] / p.bs * p.kv_heads] = s_new[i];
+    // (every CTA of the cluster has met since it read its scales of these rounds)
+    for (int i = tid * p.bs; i < some * round; i += kMoveThreads * p.bs)
+      if (token_of(i) < kept_n) scales[(int64_t)(s_to[i] / p.bs) * p.kv_heads] = s_new[i / p.bs];
     __syncthreads();
   }
 }
 
+// (errors: cudaGetLastError, as after <<<>>>)
+template <typename... Params, typename... Args>
+void launch_clusters(void (*kernel)(Params...), int64_t grid, int threads, int ctas, size_t shared,
+                     bool behind, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)grid);
+  config.blockDim = dim3((unsigned)threads);
+  config.dynamicSmemBytes = shared;
+  config.stream = stream;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ctas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attr;
+  config.numAttrs = behind ? 2 : 1;
+  cudaLaunchKernelEx(&config, kernel, Params(args)...);
+}
+
 template <int VEC>
-int launch_move(const MoveParams& p, cudaStream_t stream) {
+void launch_move(const MoveParams& p, cudaStream_t stream) {
   const int64_t chains = (int64_t)p.seqs * (2 * p.kv_heads + 1);
   // A cluster of more CTAs where there are few chains.
   int ctas = 1;
   while (ctas < 8 && chains * ctas * 2 <= 148 * 4) ctas *= 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(chains * ctas));
-  cfg.blockDim = dim3(kMoveThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = ctas > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, move_kernel<VEC>, p, ctas) == cudaSuccess ? kOk : kCudaError;
+  launch_clusters(move_kernel<VEC>, chains * ctas, kMoveThreads, ctas, 0, true, stream, p, ctas);
 }
 
 }  // namespace
@@ -343,15 +416,17 @@ int launch_evict(const EvictArgs& a, cudaStream_t stream) {
   k.sinks = a.sinks;
   k.recent = a.recent;
   const int64_t most = (int64_t)a.width * a.block_size;
-  if (most <= kKeysOnChip) {
-    const int bytes = (int)(most + most / 32 + 1) * 4;
-    static std::atomic<uint64_t> done{0};
-    allow_shared_memory(reinterpret_cast<const void*>(pick_kernel<true>),
-                        (kKeysOnChip + kKeysOnChip / 32 + 1) * 4, done);
-    pick_kernel<true><<<a.seqs, kPickThreads, bytes, stream>>>(k, err);
-  } else {
-    pick_kernel<false><<<a.seqs, kPickThreads, 0, stream>>>(k, err);
-  }
+  // more CTAs a sequence where that leaves each of them some keys a thread
+  int ctas = 1;
+  while (ctas < 8 && a.seqs * ctas * 2 <= 148 && most > 4 * kPickThreads * ctas) ctas *= 2;
+  const int64_t part = (most + ctas - 1) / ctas;
+  const bool on_chip = part <= kKeysOnChip;
+  const auto kern = on_chip ? pick_kernel<true> : pick_kernel<false>;
+  static std::atomic<uint64_t> done{0};
+  allow_shared_memory(reinterpret_cast<const void*>(pick_kernel<true>),
+                      (kKeysOnChip + kKeysOnChip / 32 + 1) * 4, done);
+  launch_clusters(kern, (int64_t)a.seqs * ctas, kPickThreads, ctas, on_chip ? (size_t)(part + part / 32 + 1) * 4 : 0,
+                  false, stream, k, ctas, err);
   MoveParams m;
   m.cache = a.cache;
   m.scales = a.scales;
@@ -368,11 +443,11 @@ int launch_evict(const EvictArgs& a, cudaStream_t stream) {
   m.width = a.width;
   m.keep = a.keep;
   const bool aligned = reinterpret_cast<uintptr_t>(a.cache) % 16 == 0;
-  const int rc = a.dim % 16 == 0 && aligned ? launch_move<16>(m, stream)
-                 : a.dim % 4 == 0 && aligned ? launch_move<4>(m, stream)
-                                             : launch_move<1>(m, stream);
+  if (a.dim % 16 == 0 && aligned) launch_move<16>(m, stream);
+  else if (a.dim % 4 == 0 && aligned) launch_move<4>(m, stream);
+  else launch_move<1>(m, stream);
   const cudaError_t e = cudaGetLastError();
-  if (rc != kOk || e != cudaSuccess) {
+  if (e != cudaSuccess) {
     set_error(std::string("evict launch failed: ") + cudaGetErrorString(e));
     return kCudaError;
   }

@@ -56,6 +56,8 @@ __global__ void __launch_bounds__(kThreads, DP > 128 ? 1 : 2) gather_kernel(cons
   __shared__ float s_factor[kPass], s_start[kPass], s_lse[kPass];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
+  launch_the_next();
+  behind_the_last();
   const int64_t items = p.head->places;
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const int s = plan_find(p.seq, p.seqs, item);
@@ -182,6 +184,8 @@ __global__ void __launch_bounds__(kThreads, DP > 128 ? 1 : 2) gather_kernel(cons
 // cached token.  For calls of few rows, whose scores are a small part of the keys' bytes.
 __global__ void __launch_bounds__(256) finish_kernel(const GatherParams p, const float* logits,
                                                      int64_t slots) {
+  launch_the_next();
+  behind_the_last();
   const int64_t per_seq = (int64_t)p.width * p.bs;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < slots; i += gridDim.x * 256ll) {
     const int64_t s = i / per_seq;
@@ -209,6 +213,7 @@ __global__ void __launch_bounds__(256) spread_kernel(const int32_t* tables, cons
                                                      unsigned long long* sums, float* weights,
                                                      int64_t num_blocks, int bs, int width,
                                                      int64_t slots, float inv_heads) {
+  behind_the_last();
   const int64_t per_seq = (int64_t)width * bs;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < slots; i += gridDim.x * 256ll) {
     const int64_t s = i / per_seq;
@@ -304,7 +309,7 @@ void launch_gather(const ChunkArgs& a, const GatherParams& p, int* err, cudaStre
   const int64_t chunks = a.total_q * p.group / kItemRows + std::min<int64_t>(a.seqs, a.total_q);
   const int64_t most = 148 * (DP > 128 ? 1 : 2);
   const int64_t grid = std::min(most, std::min(most, parts) * chunks * a.kv_heads);
-  gather_kernel<T, DP, HALVES><<<(unsigned)grid, kThreads, 0, stream>>>(p, err);
+  launch_behind(gather_kernel<T, DP, HALVES>, dim3((unsigned)grid), kThreads, 0, stream, p, err);
 }
 
 }  // namespace
@@ -350,7 +355,7 @@ int launch_accumulate(const ChunkArgs& a, float* weights, void* workspace, size_
       GatherParams p = gather_params(a, lse, ws, lay);
       p.seq = chunk_plan(b, ws + lay.inner);
       const unsigned grid = (unsigned)std::min<int64_t>((slots + 255) / 256, 148 * 8);
-      finish_kernel<<<grid, 256, 0, stream>>>(p, logits, slots);
+      launch_behind(finish_kernel, dim3(grid), 256, 0, stream, p, logits, slots);
     }
   }
   if (!scores) {
@@ -390,8 +395,8 @@ int launch_accumulate(const ChunkArgs& a, float* weights, void* workspace, size_
     if (rc != kOk) return rc;
   }
   const unsigned grid = (unsigned)std::min<int64_t>((slots + 255) / 256, 148 * 8);
-  spread_kernel<<<grid, 256, 0, stream>>>(a.tables, a.lens, sums, weights, a.num_blocks, a.block_size,
-                                          a.width, slots, 1.0f / a.heads);
+  launch_behind(spread_kernel, dim3(grid), 256, 0, stream, a.tables, a.lens, sums, weights, a.num_blocks,
+                a.block_size, a.width, slots, 1.0f / a.heads);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) {
     set_error(std::string("accumulate launch failed: ") + cudaGetErrorString(e));

@@ -85,9 +85,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   float* s_big = reinterpret_cast<float*>(smem + C::kOffMisc + 16);  // of each staging warp
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int64_t share = tile_share(p);
-  const int64_t begin = blockIdx.x * share, stop = min(begin + share, p.head->places);
-  if (begin >= stop) return;
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&kv_full[i], 128);
@@ -103,6 +100,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(mma_done, 1);
     mbar_fence_init();
   }
+  launch_the_next();
+  behind_the_last();
+  const int64_t share = tile_share(p);
+  const int64_t begin = blockIdx.x * share, stop = min(begin + share, p.head->places);
+  if (begin >= stop) return;
   if (warp == kMmaWarp) tmem_alloc(s_tmem, 512);
   tmem_fence_before_sync();
   __syncthreads();
@@ -400,7 +402,7 @@ int launch_gather_tc_t(const ChunkArgs& a, const float* lse, PlanHead* head, Pla
   auto kern = gather_tc_kernel<T, DP, HALVES>;
   static std::atomic<uint64_t> done{0};
   allow_shared_memory(reinterpret_cast<const void*>(kern), C::kSmemBytes, done);
-  kern<<<(unsigned)p.ctas, kThreads, C::kSmemBytes, stream>>>(map_k, p, device_error_word());
+  launch_behind(kern, dim3((unsigned)p.ctas), kThreads, C::kSmemBytes, stream, map_k, p, device_error_word());
   return kOk;
 }
 
