@@ -180,30 +180,61 @@ __global__ void __launch_bounds__(kThreads, DP > 128 ? 1 : 2) gather_kernel(cons
   }
 }
 
-// The scores that the attention's kernel left (in powers of two), to weights: a thread per
-// cached token.  For calls of few rows, whose scores are a small part of the keys' bytes.
+// The scores that the attention's kernel left (in powers of two), to weights, for calls of few
+// rows, whose scores are a small part of the keys' bytes.  A lane has N cached tokens next to
+// one another (4 where a table's tokens are a multiple of it: 16 bytes a load), a warp every
+// eighth row: what bounds it is how many loads are under way (a thread for a token and all
+// rows took 16 us for the 34 MB of 64 sequences).
+template <int N>
 __global__ void __launch_bounds__(256) finish_kernel(const GatherParams p, const float* logits,
                                                      int64_t slots) {
+  __shared__ float s_sum[8][32 * N];
   launch_the_next();
   behind_the_last();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t per_seq = (int64_t)p.width * p.bs;
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < slots; i += gridDim.x * 256ll) {
-    const int64_t s = i / per_seq;
-    const int at = (int)(i - s * per_seq);
-    const PlanSeq seq = p.seq[s];
-    if (at >= seq.len || seq.lq == 0) continue;
-    const int page = at / p.bs, phys = p.tables[s * p.width + page];
-    if (phys < 0 || (int64_t)phys >= p.num_blocks) continue;
-    // the first token that sees this one
-    const int first = max(at - (seq.len - seq.lq), 0);
-    const int64_t r1 = (int64_t)(seq.q0 + seq.lq) * p.heads;
-    float sum = 0.0f;
-#pragma unroll 8
-    for (int64_t r = (int64_t)(seq.q0 + first) * p.heads; r < r1; ++r) {
-      const float lse = p.lse[r];
-      sum += lse == -INFINITY ? 0.0f : ex2(fmaf(-lse, kLog2e, logits[r * per_seq + at]));
+  for (int64_t i0 = blockIdx.x * (32ll * N); i0 < slots; i0 += gridDim.x * (32ll * N)) {
+    const int64_t i = i0 + lane * N;
+    float sum[N] = {};
+    if (i < slots) {
+      const int s = slots <= 0x7fffffff ? (int)i / (int)per_seq : (int)(i / per_seq);
+      const int at = (int)(i - s * per_seq);
+      const PlanSeq seq = p.seq[s];
+      if (at < seq.len) {
+        // the token's rows, and of those the first that sees each of the N (rows are below 2^25)
+        const int r0 = seq.q0 * p.heads, r1 = r0 + seq.lq * p.heads;
+        int from[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          from[e] = (int)min((int64_t)r0 + max(at + e - (seq.len - seq.lq), 0) * (int64_t)p.heads, (int64_t)r1);
+#pragma unroll 4
+        for (int r = from[0] + warp; r < r1; r += 8) {
+          const float lse = p.lse[r], base = lse * kLog2e;
+          float x[N];
+          if constexpr (N == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(logits + r * per_seq + at);
+          else x[0] = logits[r * per_seq + at];
+#pragma unroll
+          for (int e = 0; e < N; ++e) sum[e] += r >= from[e] && lse != -INFINITY ? ex2(x[e] - base) : 0.0f;
+        }
+      }
     }
-    add_weight(p.sums + (int64_t)phys * p.bs + (at - page * p.bs), sum);
+#pragma unroll
+    for (int e = 0; e < N; ++e) s_sum[warp][lane * N + e] = sum[e];
+    __syncthreads();
+    const int64_t mine = i0 + threadIdx.x;
+    if (threadIdx.x < 32 * N && mine < slots) {
+      const int64_t s = mine / per_seq;
+      const int at = (int)(mine - s * per_seq);
+      const PlanSeq seq = p.seq[s];
+      const int page = at / p.bs, phys = at < seq.len && seq.lq > 0 ? p.tables[s * p.width + page] : -1;
+      if (phys >= 0 && (int64_t)phys < p.num_blocks) {
+        float all = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) all += s_sum[w][threadIdx.x];
+        add_weight(p.sums + (int64_t)phys * p.bs + (at - page * p.bs), all);
+      }
+    }
+    __syncthreads();
   }
 }
 
@@ -354,8 +385,9 @@ int launch_accumulate(const ChunkArgs& a, float* weights, void* workspace, size_
     if (scores) {
       GatherParams p = gather_params(a, lse, ws, lay);
       p.seq = chunk_plan(b, ws + lay.inner);
-      const unsigned grid = (unsigned)std::min<int64_t>((slots + 255) / 256, 148 * 8);
-      launch_behind(finish_kernel, dim3(grid), 256, 0, stream, p, logits, slots);
+      const int n = (int64_t)a.width * a.block_size % 4 == 0 ? 4 : 1;
+      const unsigned grid = (unsigned)std::min<int64_t>((slots + 32 * n - 1) / (32 * n), 148 * 8);
+      launch_behind(n == 4 ? finish_kernel<4> : finish_kernel<1>, dim3(grid), 256, 0, stream, p, logits, slots);
     }
   }
   if (!scores) {
