@@ -74,6 +74,12 @@ struct TcCfg {
   static_assert(256 * (kSoftRegs + kOtherRegs) <= 65536, "registers");
 };
 
+// The unit that begins in a CTA's share and goes on behind it, for the kernel that joins.
+struct CutUnit {
+  int parts;  // 0: there is none
+  int rows, kvh, block, q0;
+};
+
 struct TcParams : TileWork {
   const void* q;
   const int8_t* k_cache;
@@ -83,6 +89,7 @@ struct TcParams : TileWork {
   const int32_t* tables;
   void* out;
   float* lse;  // nullable
+  CutUnit* cuts;   // per CTA
   uint8_t* slots;  // per CTA two: of the unit that it begins with, and that it ends with
   float4* sums;    // per CTA and row tile: [DP / 4][128 rows], O of earlier tiles
   int64_t q_tok, q_head;
@@ -148,6 +155,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   launch_the_next();
   behind_the_last();
+  if (tid == 0) p.cuts[blockIdx.x].parts = 0;
   const PlanHead head = *p.head;
   const int64_t share = tile_share(p);
   const int64_t begin = blockIdx.x * share, stop = min(begin + share, head.places);
@@ -449,6 +457,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       u.find(p, now, share);
       if (u.empty(stop)) continue;
       u.cut(p, now, stop);
+      if (tid == 0 && u.parts > 1 && u.cta0 == (int)blockIdx.x)
+        p.cuts[blockIdx.x] = CutUnit{u.parts, u.rows, u.kvh, u.block, u.seq.q0};
       const bool dual = u.dual;
       const int first = dual ? x : 0, by = dual ? 2 : 1;
       const int nt = dual ? u.n : (x ? u.tiles[1] : u.tiles[0]);  // its tiles: first, first + by, ... < nt
@@ -802,25 +812,24 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Units that were cut: a CTA has 32 rows, lane = row, a warp every eighth 4 channels of
-// all parts in order; the rows leave through shared memory.
+// all parts in order; the rows leave through shared memory.  Most of the CTAs have none:
+// what counts is how soon they see that, and how many there are at a time (the search of
+// the plan and 110 registers a thread took 12.6 us for 64 units in 148 CTAs).
 constexpr int kJoinRows = 32, kJoinWarps = 8;
 template <typename T, int DP>
-__global__ void __launch_bounds__(kJoinWarps * 32) join_tc_kernel(const TcParams p) {
+__global__ void __launch_bounds__(kJoinWarps * 32, 4) join_tc_kernel(const TcParams p) {
   using S = TcSlot<DP>;
-  constexpr int kBatch = 4, kEach = DP / 4 / kJoinWarps;
+  constexpr int kBatch = 2, kEach = DP / 4 / kJoinWarps;
   __shared__ float4 s_out[kJoinRows][DP / 4 + 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   launch_the_next();
   behind_the_last();
-  const int64_t share = tile_share(p);
-  // the unit at the end of the CTA's share, if it begins there
-  const int64_t place = (int64_t)(blockIdx.x + 1) * share - 1;
-  if (place >= p.head->places) return;
-  TileUnit u;
-  u.s = plan_find(p.seq, p.seqs, place);
-  u.find(p, place, share);
+  const CutUnit cut = p.cuts[blockIdx.x];
   const int row0 = blockIdx.y * kJoinRows, r = row0 + lane;
-  if (u.cta0 != (int)blockIdx.x || u.parts == 1 || row0 >= u.rows) return;
+  if (cut.parts == 0 || row0 >= cut.rows) return;
+  TileUnit u;
+  u.cta0 = blockIdx.x, u.parts = cut.parts, u.rows = cut.rows;
+  u.kvh = cut.kvh, u.block = cut.block, u.seq.q0 = cut.q0;
   const bool valid = r < u.rows;
   float m = -INFINITY, l = 0.0f;
   float4 acc[kEach];
@@ -877,7 +886,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_tc_kernel(const TcParams
 }
 
 struct TcLayout {
-  size_t slots, sums, total;
+  size_t cuts, slots, sums, total;
 };
 
 TcLayout tc_layout(const ChunkArgs& a) {
@@ -891,6 +900,7 @@ TcLayout tc_layout(const ChunkArgs& a) {
     at += (bytes + 255) / 256 * 256;
     return here;
   };
+  l.cuts = take(sizeof(CutUnit) * kChunkTcCtas);
   l.slots = take((size_t)2 * kChunkTcCtas * (dp == 64 ? TcSlot<64>::kBytes : TcSlot<128>::kBytes));
   l.sums = take(dp == 128 && tiles > flush ? (size_t)kChunkTcCtas * 2 * kTileRows * dp * 4 : 0);
   l.total = at;
@@ -914,6 +924,7 @@ int launch_tc(const ChunkArgs& a, PlanHead* head, PlanSeq* seq, uint8_t* ws, boo
   p.lse = a.lse;
   p.head = head;
   p.seq = seq;
+  p.cuts = reinterpret_cast<CutUnit*>(ws + lay.cuts);
   p.slots = ws + lay.slots;
   p.sums = reinterpret_cast<float4*>(ws + lay.sums);
   p.q_tok = a.q_token_stride;
