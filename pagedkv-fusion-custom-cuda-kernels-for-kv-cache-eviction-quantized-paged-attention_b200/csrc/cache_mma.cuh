@@ -311,7 +311,7 @@ struct PlanHead {
   int q_begin, q_end;  // rows of all sequences
   int64_t share;       // places of a worker
   int over;            // places in front of a unit's steps
-  int most_parts;      // no unit is cut into more
+  int unused;
 };
 
 struct PlanArgs {

@@ -106,7 +106,6 @@ __global__ void __launch_bounds__(kPlanThreads)
     return p.which == kPlanAll || few == (p.which == kPlanFew) ? (rows + p.rows - 1) / p.rows * p.kv_heads : 0;
   };
   int64_t in_shares = 0, in_parts[2] = {};  // places
-  int longest = 0;
   PlanSeq q = {};
   for (int s0 = 0; s0 < p.seqs; s0 += kPlanThreads) {
     const int s = s0 + tid;
@@ -134,7 +133,6 @@ __global__ void __launch_bounds__(kPlanThreads)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         in_parts[i] += units * ((q.steps + (kPartSteps << i) - 1) & -(kPartSteps << i));
-      if (units > 0) longest = max(longest, q.steps);
     }
     end = max(end, most);
     __syncthreads();
@@ -150,14 +148,11 @@ __global__ void __launch_bounds__(kPlanThreads)
       scan_sum(in_parts[i], s_sum, &parts[i]);
       __syncthreads();
     }
-    scan_max(longest, s_max, &longest);
-    __syncthreads();
     part = parts[0] <= (int64_t)p.workers * kPartSteps       ? kPartSteps
            : parts[1] <= (int64_t)p.workers * 2 * kPartSteps ? 2 * kPartSteps
                                                              : 0;
     h.share = part > 0 ? part : max((all + p.workers - 1) / p.workers, (int64_t)p.least);
     h.over = part > 0 ? 0 : p.over;
-    h.most_parts = (int)((longest - 1) / h.share) + (part > 0 ? 1 : 2);
   }
   int64_t base = 0;
   for (int s0 = 0; s0 < p.seqs; s0 += kPlanThreads) {
@@ -252,6 +247,7 @@ struct RowsParams {
   const PlanHead* head;
   const PlanSeq* seq;
   int* counters;   // per warp: of the unit that begins in it and goes on behind it
+  CutUnit* cuts;   // per eight warps: the unit of more than kJoinHere parts that begins in them
   uint8_t* slots;  // per warp two: of the unit that it begins with, and that it ends with
   int64_t q_tok, q_head;  // strides, elements
   int64_t num_blocks;
@@ -724,7 +720,11 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, PV, WHOLE>::kCtas)
         reinterpret_cast<float2*>(slot + S::kMl)[2 * t + r] = make_float2(m, l[r]);
       }
     }
-    if (u.parts > kJoinHere) continue;
+    if (u.parts > kJoinHere) {
+      if (lane == 0 && warp == u.warp0)
+        p.cuts[warp / kRowWarps] = CutUnit{u.parts, u.rows, u.kvh, u.block, u.seq.q0, u.warp0};
+      continue;
+    }
     __syncwarp();
     int last = 0;
     if (lane == 0) last = atomic_add_acq_rel_gpu(&p.counters[u.warp0], 1) == u.parts - 1;
@@ -789,30 +789,25 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, PV, WHOLE>::kCtas)
   }
 }
 
-// Units of many parts (few long sequences): a CTA for each eight warps, in which no more
-// than one begins, a row for every four of its own, each of which takes a quarter of the
-// parts.
+// Units of many parts (few long sequences): two CTAs for each eight warps, in which no more
+// than one begins, each for 4 rows, of which a warp takes every fourth part.
+constexpr int kJoinRows = 4, kJoinWarps = 16;
+static_assert(kJoinHere >= kRowWarps, "one unit of more parts in so many warps");
 template <typename T, int DP, bool PV>
-__global__ void __launch_bounds__(1024, 1) join_kernel(const RowsParams p) {
+__global__ void __launch_bounds__(kJoinWarps * 32, 2) join_kernel(const RowsParams p) {
   using S = Slot<DP, PV>;
-  constexpr int kWide = (DP + 127) / 128;
-  __shared__ float4 s_o[32][kWide * 32];
-  __shared__ float2 s_ml[32];
+  constexpr int kWide = (DP + 127) / 128, kSlices = kJoinWarps / kJoinRows;
+  __shared__ float4 s_o[kJoinWarps][kWide * 32];
+  __shared__ float2 s_ml[kJoinWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int r = warp & 7, quarter = warp >> 3;
+  const int r = blockIdx.y * kJoinRows + warp % kJoinRows, slice = warp / kJoinRows;
   launch_the_next();
   behind_the_last();
-  const PlanHead head = *p.head;
-  if (head.most_parts <= kJoinHere) return;
-  // the unit at the end of the eight shares, if it begins in them
-  static_assert(kJoinHere >= kRowWarps, "one unit of more parts in so many warps");
-  const int64_t place = (int64_t)(blockIdx.x + 1) * kRowWarps * head.share - 1;
-  if (place >= head.places) return;
+  const CutUnit cut = p.cuts[blockIdx.x];
+  if (cut.parts == 0 || (int)blockIdx.y * kJoinRows >= cut.rows) return;
   RowsUnit u;
-  u.s = plan_find(p.seq, p.seqs, place);
-  u.find(p, head, place);
-  if (u.warp0 / kRowWarps != (int)blockIdx.x || u.parts <= kJoinHere) return;
-  const int each = (u.parts + 3) / 4, i0 = quarter * each, i1 = min(i0 + each, u.parts);
+  u.warp0 = cut.first, u.parts = cut.parts, u.rows = cut.rows;
+  u.kvh = cut.kvh, u.block = cut.block, u.seq.q0 = cut.q0;
   float m = -INFINITY, l = 0.0f;
   float4 acc[kWide];
 #pragma unroll
@@ -830,13 +825,13 @@ __global__ void __launch_bounds__(1024, 1) join_kernel(const RowsParams p) {
   };
   constexpr int kBatch = DP > 128 ? 2 : 4;
   if (r < u.rows)
-    for (int i = i0; i < i1; i += kBatch) {
+    for (int i = slice; i < u.parts; i += kBatch * kSlices) {
       float2 ml[kBatch];
       float4 v[kBatch][kWide];
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
-        const bool there = i + b < i1;
-        const uint8_t* from = u.slot<S::kBytes>(p, there ? i + b : i);
+        const bool there = i + b * kSlices < u.parts;
+        const uint8_t* from = u.slot<S::kBytes>(p, there ? i + b * kSlices : i);
         ml[b] = there ? __ldcg(reinterpret_cast<const float2*>(from + S::kMl) + r)
                       : make_float2(-INFINITY, 0.0f);
 #pragma unroll
@@ -854,8 +849,8 @@ __global__ void __launch_bounds__(1024, 1) join_kernel(const RowsParams p) {
   for (int c = 0; c < kWide; ++c) s_o[warp][c * 32 + lane] = acc[c];
   if (lane == 0) s_ml[warp] = make_float2(m, l);
   __syncthreads();
-  if (quarter > 0 || r >= u.rows) return;
-  for (int w = warp + 8; w < 32; w += 8) {
+  if (slice > 0 || r >= u.rows) return;
+  for (int w = warp + kJoinRows; w < kJoinWarps; w += kJoinRows) {
     float4 v[kWide];
 #pragma unroll
     for (int c = 0; c < kWide; ++c) v[c] = s_o[w][c * 32 + lane];
@@ -954,7 +949,8 @@ ChunkLayout chunk_layout(const ChunkArgs& a) {
   const Division d = division_of(a);
   l.head = take(sizeof(PlanHead));
   l.seq = take(sizeof(PlanSeq) * (size_t)a.seqs);
-  l.counters = take(d.rows ? sizeof(int) * kMostWarps : 0);
+  // (the counters and the cut units are zeroed together)
+  l.counters = take(d.rows ? sizeof(int) * kMostWarps + sizeof(CutUnit) * (kMostWarps / kRowWarps) : 0);
   l.slots = take(d.rows ? (size_t)2 * kMostWarps * ((a.v_cache != nullptr ? kRows * dp * 4 : 0) + kRows * 8) : 0);
   l.head2 = take(d.tc ? sizeof(PlanHead) : 0);
   l.seq2 = take(d.tc ? sizeof(PlanSeq) * (size_t)a.seqs : 0);
@@ -992,6 +988,7 @@ int launch_rows(const ChunkArgs& a, uint8_t* ws, cudaStream_t stream) {
   p.head = reinterpret_cast<PlanHead*>(ws + lay.head);
   p.seq = reinterpret_cast<PlanSeq*>(ws + lay.seq);
   p.counters = reinterpret_cast<int*>(ws + lay.counters);
+  p.cuts = reinterpret_cast<CutUnit*>(p.counters + kMostWarps);
   p.slots = ws + lay.slots;
   p.q_tok = a.q_token_stride;
   p.q_head = a.q_head_stride;
@@ -1020,7 +1017,7 @@ int launch_rows(const ChunkArgs& a, uint8_t* ws, cudaStream_t stream) {
                 device_error_word());
   // a unit of so many parts needs so many steps
   if (((int64_t)a.width * a.block_size + kStep - 1) / kStep > (int64_t)kPartSteps * kJoinHere)
-    launch_behind(join_kernel<T, DP, PV>, dim3((unsigned)ctas), 1024, 0, stream, p);
+    launch_behind(join_kernel<T, DP, PV>, dim3((unsigned)ctas, kRows / kJoinRows), kJoinWarps * 32, 0, stream, p);
   return kOk;
 }
 
@@ -1079,7 +1076,7 @@ int launch_chunk(const ChunkArgs& a, void* workspace, size_t workspace_bytes, cu
   plan.head = reinterpret_cast<PlanHead*>(ws + lay.head);
   plan.seq = reinterpret_cast<PlanSeq*>(ws + lay.seq);
   plan.counters = reinterpret_cast<int*>(ws + lay.counters);
-  plan.counts = kMostWarps;
+  plan.counts = kMostWarps + (int)sizeof(CutUnit) / 4 * (kMostWarps / kRowWarps);
   PlanArgs plan2 = chunk_tc_plan(plan);
   plan2.which = d.rows ? kPlanMany : kPlanAll;
   plan2.head = reinterpret_cast<PlanHead*>(ws + lay.head2);

@@ -17,6 +17,13 @@ bool cache_map(CUtensorMap* map, const int8_t* cache, const ChunkArgs& a, int ch
 // Where launch_chunk left the sequences' rows and lengths (of calls without a V cache).
 const PlanSeq* chunk_plan(const ChunkArgs& a, void* workspace);
 
+// A unit that was cut, for the kernel that joins its parts.
+struct CutUnit {
+  int parts;  // 0: there is none
+  int rows, kvh, block, q0;
+  int first;  // of the workers that have parts
+};
+
 constexpr int kTileUnitRows = 256;
 constexpr int kTileKeys = 128;
 constexpr int kTileOver = 3;   // tiles that a unit's start and end cost

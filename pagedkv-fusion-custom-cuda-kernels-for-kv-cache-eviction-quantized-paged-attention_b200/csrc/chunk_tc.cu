@@ -74,12 +74,6 @@ struct TcCfg {
   static_assert(256 * (kSoftRegs + kOtherRegs) <= 65536, "registers");
 };
 
-// The unit that begins in a CTA's share and goes on behind it, for the kernel that joins.
-struct CutUnit {
-  int parts;  // 0: there is none
-  int rows, kvh, block, q0;
-};
-
 struct TcParams : TileWork {
   const void* q;
   const int8_t* k_cache;
@@ -458,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (u.empty(stop)) continue;
       u.cut(p, now, stop);
       if (tid == 0 && u.parts > 1 && u.cta0 == (int)blockIdx.x)
-        p.cuts[blockIdx.x] = CutUnit{u.parts, u.rows, u.kvh, u.block, u.seq.q0};
+        p.cuts[blockIdx.x] = CutUnit{u.parts, u.rows, u.kvh, u.block, u.seq.q0, u.cta0};
       const bool dual = u.dual;
       const int first = dual ? x : 0, by = dual ? 2 : 1;
       const int nt = dual ? u.n : (x ? u.tiles[1] : u.tiles[0]);  // its tiles: first, first + by, ... < nt
