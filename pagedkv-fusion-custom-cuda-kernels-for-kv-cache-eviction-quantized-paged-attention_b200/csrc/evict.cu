@@ -233,14 +233,23 @@ struct Piece<1> { using T = uint8_t; };
 // rint(code ratio) of four codes.  A byte in the low mantissa of 2^23 is a number, and a
 // number at 1.5 2^23 is rounded to an integer, to even as rint, whose low byte is there: the
 // conversion instructions, 16 a clock and SM, would take 90 us of the 64 sequences' move.
+// (Only a scale of the other sign can take a code out of its range.)
 __device__ __forceinline__ uint32_t shrink4(uint32_t w, float ratio) {
   const uint32_t u = w ^ 0x80808080u;
   uint32_t x[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float code = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + i)) - 8388736.0f;
-    x[i] = __float_as_uint(fminf(fmaxf(code * ratio, -127.0f), 127.0f) + 12582912.0f);
+  for (int i = 0; i < 4; i += 2) {
+    const uint64_t code = add_f32x2(f32x2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + i)),
+                                          __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441 + i))),
+                                    f32x2(-8388736.0f, -8388736.0f));
+    const float2 c = unpack_f32x2(code);  // (products rounded apart from the sums behind them)
+    x[i] = __float_as_uint(__fadd_rn(__fmul_rn(c.x, ratio), 12582912.0f));
+    x[i + 1] = __float_as_uint(__fadd_rn(__fmul_rn(c.y, ratio), 12582912.0f));
   }
+  if (ratio < -1.0f)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      x[i] = __float_as_uint(fminf(fmaxf(__uint_as_float(x[i]), 12582912.0f - 127.0f), 12582912.0f + 127.0f));
   return __byte_perm(__byte_perm(x[0], x[1], 0x0040), __byte_perm(x[2], x[3], 0x0040), 0x5410);
 }
 __device__ __forceinline__ uint4 shrink(uint4 v, float f) {
@@ -340,24 +349,25 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const MoveParams p, 
       const int n = max(min(round, kept_n - token_of(base)), 0);
       for (int c0 = 0; c0 < pieces; c0 += per) {
         const int m = min(per, pieces - c0);
+        const uint32_t over_m = ((1u << 20) + m - 1) / m;  // exact for x m below 2^20
         V held[kHeld];
+        int token[kHeld], at[kHeld];
 #pragma unroll
         for (int u = 0; u < kHeld; ++u) {
-          const int x = u * kMoveThreads + tid, i = x / m;
-          if (i < n)
-            held[u] = *reinterpret_cast<const V*>(cache + s_from[base + i] * token_bytes +
-                                                  (c0 + x - i * m) * VEC);
+          const int x = u * kMoveThreads + tid;
+          token[u] = (int)(x * over_m >> 20);
+          at[u] = (c0 + x - token[u] * m) * VEC;
+          if (token[u] < n)
+            held[u] = *reinterpret_cast<const V*>(cache + s_from[base + token[u]] * token_bytes + at[u]);
         }
         meet();
 #pragma unroll
         for (int u = 0; u < kHeld; ++u) {
-          const int x = u * kMoveThreads + tid, i = x / m;
-          if (i < n) {
-            const float ratio = s_old[base + i];
-            V c = held[u];
-            if (ratio != 1.0f) c = shrink(c, ratio);
-            *reinterpret_cast<V*>(cache + s_to[base + i] * token_bytes + (c0 + x - i * m) * VEC) = c;
-          }
+          if (token[u] >= n) continue;
+          const float ratio = s_old[base + token[u]];
+          V c = held[u];
+          if (ratio != 1.0f) c = shrink(c, ratio);
+          *reinterpret_cast<V*>(cache + s_to[base + token[u]] * token_bytes + at[u]) = c;
         }
       }
     }

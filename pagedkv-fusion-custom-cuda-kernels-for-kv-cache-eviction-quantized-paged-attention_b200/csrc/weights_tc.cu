@@ -335,7 +335,12 @@ __global__ void __launch_bounds__(kThreads, 1)
               z[e + 1] = unpack_f32x2(fma_f32x2(
                   f32x2(__uint_as_float(w[2 * e + 2]), __uint_as_float(w[2 * e + 3])), k2, f32x2(-b.z, -b.w)));
             }
-            if (c + 32 < columns) tmem_load<32>(s_at + c + 32, w);  // on its way meanwhile
+            if (c + 32 < columns) {
+              tmem_load<32>(s_at + c + 32, w);  // on its way meanwhile
+            } else {  // the next products can come
+              tmem_fence_before_sync();
+              mbar_arrive(&s_empty[x]);
+            }
 #pragma unroll
             for (int e = 0; e < 16; ++e)
               sum[e & 1] = add_f32x2(sum[e & 1], f32x2(ex2(z[e].x), ex2(z[e].y)));
@@ -354,9 +359,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           sum[0] = f32x2(total, 0.0f);
+          tmem_fence_before_sync();
+          mbar_arrive(&s_empty[x]);
         }
-        tmem_fence_before_sync();
-        mbar_arrive(&s_empty[x]);
         const float2 a = unpack_f32x2(add_f32x2(sum[0], sum[1]));
         if (ok && group != kNoRow && key < u.seq.len) add_weight(p.sums + group + row % 16, a.x + a.y);
       }
