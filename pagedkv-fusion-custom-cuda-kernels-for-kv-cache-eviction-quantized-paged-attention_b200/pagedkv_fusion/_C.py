@@ -753,6 +753,8 @@ def shared_prefix_attention(q, k_cache_q, k_scale, v_cache_q, v_scale, prefix_ta
 def _query_rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` ``[tokens, heads, D]`` itself where its rows can be read in pieces of
     16 bytes (contiguous channels, strides and address of 16 bytes), else a copy."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:  # (D is a multiple of 16 bytes)
+        return t
     a, b, c = t.stride()
     n = 16 // t.element_size()
     if t.numel() == 0 or (c == 1 and a % n == 0 and b % n == 0 and t.data_ptr() % 16 == 0):
@@ -770,14 +772,16 @@ def _cached_size(cache: dict, fn, key: tuple) -> int:
 
 
 def _check_chunk(q, k_cache_q, k_scale, block_tables, seq_lens, cu_seqlens):
-    """Shapes and types of new tokens over an INT8 paged cache."""
-    if q.dim() != 3 or q.dtype not in _DTYPE_CODE:
+    """Shapes and types of new tokens over an INT8 paged cache; the sizes
+    ``(T, H, D, NB, bs, Hkv, S, M)``."""
+    shape, cache = q.shape, k_cache_q.shape
+    if len(shape) != 3 or q.dtype not in _DTYPE_CODE:
         raise RuntimeError("q must be [total_q, num_heads, head_dim] float32, float16 or bfloat16")
-    if k_cache_q.dim() != 4 or k_cache_q.dtype is not torch.int8:
+    if len(cache) != 4 or k_cache_q.dtype is not torch.int8:
         raise RuntimeError("the caches must be int8 [NB, bs, Hkv, D]")
-    NB, bs, Hkv, D = k_cache_q.shape
-    H = q.shape[1]
-    if D != q.shape[2]:
+    T, H, D = shape
+    NB, bs, Hkv, cache_dim = cache
+    if cache_dim != D:
         raise RuntimeError("cache head_dim must match q")
     if Hkv == 0 or H == 0 or H % Hkv:
         raise RuntimeError("num_heads must be a multiple of num_kv_heads")
@@ -785,20 +789,21 @@ def _check_chunk(q, k_cache_q, k_scale, block_tables, seq_lens, cu_seqlens):
         raise RuntimeError("supports head_dim % 32 == 0, <= 256")
     if not 0 < bs <= 64:
         raise RuntimeError("supports block_size <= 64")
-    if k_scale.dtype is not _F32 or tuple(k_scale.shape) != (NB, Hkv):
+    if k_scale.dtype is not _F32 or k_scale.shape != (NB, Hkv):
         raise RuntimeError("scales must be float32 [num_blocks, num_kv_heads]")
-    _check_tables(block_tables, seq_lens)
-    if cu_seqlens.dtype is not torch.int32 or cu_seqlens.dim() != 1 or \
-            cu_seqlens.shape[0] != block_tables.shape[0] + 1:
+    S, M = _check_tables(block_tables, seq_lens)
+    if cu_seqlens.dtype is not torch.int32 or cu_seqlens.shape != (S + 1,):
         raise RuntimeError("cu_seqlens must be int32 [num_seqs + 1]")
+    return T, H, D, NB, bs, Hkv, S, M
 
 
 def _check_tables(block_tables, seq_lens):
-    if block_tables.dtype is not torch.int32 or block_tables.dim() != 2:
+    shape = block_tables.shape
+    if block_tables.dtype is not torch.int32 or len(shape) != 2:
         raise RuntimeError("block_tables must be int32 [num_seqs, max_blocks_per_seq]")
-    if seq_lens.dtype not in _INTS or seq_lens.dim() != 1 or \
-            seq_lens.shape[0] != block_tables.shape[0]:
+    if seq_lens.dtype not in _INTS or seq_lens.shape != shape[:1]:
         raise RuntimeError("seq_lens must be int32 or int64 [num_seqs]")
+    return shape
 
 
 def chunk_attention(q, k_cache_q, k_scale, v_cache_q, v_scale, block_tables, seq_lens, cu_seqlens,
@@ -807,32 +812,31 @@ def chunk_attention(q, k_cache_q, k_scale, v_cache_q, v_scale, block_tables, seq
     (and, with ``return_lse``, the float32 ``[total_q, H]`` log denominators)."""
     dev = _check_inputs(q, k_cache_q, k_scale, v_cache_q, v_scale, block_tables, seq_lens,
                         cu_seqlens)
-    _check_chunk(q, k_cache_q, k_scale, block_tables, seq_lens, cu_seqlens)
+    T, H, D, NB, bs, Hkv, S, M = _check_chunk(q, k_cache_q, k_scale, block_tables, seq_lens,
+                                              cu_seqlens)
     if v_cache_q.dtype is not torch.int8 or v_cache_q.shape != k_cache_q.shape:
         raise RuntimeError("v_cache_q must be int8, shaped like k_cache_q")
     if v_scale.dtype is not _F32 or v_scale.shape != k_scale.shape:
         raise RuntimeError("scales must be float32 [num_blocks, num_kv_heads]")
-    T, H, D = q.shape
-    NB, bs, Hkv, _ = k_cache_q.shape
-    S, M = block_tables.shape
     qc, kc, vc = _query_rows(q), _aligned(k_cache_q), _aligned(v_cache_q)
-    ks, vs = _as_contiguous(k_scale, _F32), _as_contiguous(v_scale, _F32)
-    bt, sl = _as_contiguous(block_tables, torch.int32), _as_contiguous(seq_lens, torch.int32)
+    ks, vs = k_scale.contiguous(), v_scale.contiguous()
+    bt, sl = block_tables.contiguous(), _as_contiguous(seq_lens, torch.int32)
     cu = cu_seqlens.contiguous()
-    out = _like(q)
-    lse = torch.empty((T, H), dtype=_F32, device=q.device) if return_lse else None
+    # (new_empty: the type and device are not looked up by name)
+    out = qc.new_empty((T, H, D))
+    lse = ks.new_empty((T, H)) if return_lse else None
     nbytes = _cached_size(_CHUNK_WS_CACHE, _chunk_ws, (T, S, H, Hkv, D, bs, M))
-    ws, wp = _workspace(nbytes, q.device)
+    ws = kc.new_empty(nbytes)
     qt, qh, _ = qc.stride()
     _call(_fast.chunk_attention, dev, qc.data_ptr(), _DTYPE_CODE[q.dtype], kc.data_ptr(),
           ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), bt.data_ptr(), sl.data_ptr(), cu.data_ptr(),
           out.data_ptr(), None if lse is None else lse.data_ptr(), T, S, H, Hkv, D, bs, NB, M, qt,
-          qh, float(sm_scale), wp, nbytes, _raw_stream(dev))
+          qh, float(sm_scale), ws.data_ptr(), nbytes, _raw_stream(dev))
     return (out, lse) if return_lse else out
 
 
 def _check_weights(weights, num_blocks: int, block_size: int):
-    if weights.dtype is not _F32 or tuple(weights.shape) != (num_blocks, block_size):
+    if weights.dtype is not _F32 or weights.shape != (num_blocks, block_size):
         raise RuntimeError("weights must be float32 [num_blocks, block_size]")
     if not weights.is_contiguous():
         raise RuntimeError("weights must be contiguous (they are written in place)")
@@ -842,26 +846,23 @@ def accumulate_attention(weights, q, k_cache_q, k_scale, block_tables, seq_lens,
                          sm_scale, lse=None):
     """Adds the attention weights of packed new tokens to ``weights`` ``[NB, bs]``."""
     dev = _check_inputs(weights, q, k_cache_q, k_scale, block_tables, seq_lens, cu_seqlens, lse)
-    _check_chunk(q, k_cache_q, k_scale, block_tables, seq_lens, cu_seqlens)
-    T, H, D = q.shape
-    NB, bs, Hkv, _ = k_cache_q.shape
-    S, M = block_tables.shape
+    T, H, D, NB, bs, Hkv, S, M = _check_chunk(q, k_cache_q, k_scale, block_tables, seq_lens,
+                                              cu_seqlens)
     _check_weights(weights, NB, bs)
-    if lse is not None and (lse.dtype is not _F32 or tuple(lse.shape) != (T, H)):
+    if lse is not None and (lse.dtype is not _F32 or lse.shape != (T, H)):
         raise RuntimeError("lse must be float32 [total_q, num_heads]")
-    qc, kc = _query_rows(q), _aligned(k_cache_q)
-    ks = _as_contiguous(k_scale, _F32)
-    bt, sl = _as_contiguous(block_tables, torch.int32), _as_contiguous(seq_lens, torch.int32)
+    qc, kc, ks = _query_rows(q), _aligned(k_cache_q), k_scale.contiguous()
+    bt, sl = block_tables.contiguous(), _as_contiguous(seq_lens, torch.int32)
     cu = cu_seqlens.contiguous()
     given = None if lse is None else lse.contiguous()
     nbytes = _cached_size(_CHUNK_WS_CACHE, _accumulate_ws,
                           (T, S, H, Hkv, D, bs, NB, M, 0 if lse is None else 1))
-    ws, wp = _workspace(nbytes, q.device)
+    ws = kc.new_empty(nbytes)
     qt, qh, _ = qc.stride()
     _call(_fast.accumulate_attention, dev, weights.data_ptr(), qc.data_ptr(), _DTYPE_CODE[q.dtype],
           kc.data_ptr(), ks.data_ptr(), bt.data_ptr(), sl.data_ptr(), cu.data_ptr(),
           None if given is None else given.data_ptr(), T, S, H, Hkv, D, bs, NB, M, qt, qh,
-          float(sm_scale), wp, nbytes, _raw_stream(dev))
+          float(sm_scale), ws.data_ptr(), nbytes, _raw_stream(dev))
 
 
 def evict_tokens(kv_cache_int8, scale_cache, weights, block_tables, seq_lens, keep: int,
@@ -878,17 +879,15 @@ def evict_tokens(kv_cache_int8, scale_cache, weights, block_tables, seq_lens, ke
         raise RuntimeError("supports block_size <= 64")
     if not 0 < D <= 256:
         raise RuntimeError("head_dim must be 1 to 256")
-    if scale_cache.dtype is not _F32 or tuple(scale_cache.shape) != (2, NB, Hkv):
+    if scale_cache.dtype is not _F32 or scale_cache.shape != (2, NB, Hkv):
         raise RuntimeError("scale_cache must be float32 [2, NB, Hkv]")
     _check_weights(weights, NB, bs)
-    _check_tables(block_tables, seq_lens)
+    S, M = _check_tables(block_tables, seq_lens)
     keep, sinks, recent = int(keep), int(sinks), int(recent)
     if keep < 1 or sinks < 0 or recent < 0 or sinks + recent > keep:
         raise RuntimeError("keep must be positive and hold sinks and recent")
-    S, M = block_tables.shape
-    bt, sl = _as_contiguous(block_tables, torch.int32), _as_contiguous(seq_lens, torch.int32)
-    lens = torch.empty(S, dtype=torch.int32, device=sl.device)
-    kept = torch.empty((S, keep), dtype=torch.int32, device=sl.device)
+    bt, sl = block_tables.contiguous(), _as_contiguous(seq_lens, torch.int32)
+    lens, kept = sl.new_empty((S,)), sl.new_empty((S, keep))
     _call(_fast.evict_tokens, dev, kv_cache_int8.data_ptr(), scale_cache.data_ptr(),
           weights.data_ptr(), bt.data_ptr(), sl.data_ptr(), lens.data_ptr(), kept.data_ptr(), S, NB,
           bs, Hkv, D, M, keep, sinks, recent, _raw_stream(dev))
