@@ -7,12 +7,12 @@
 // in fp16; the products run on the tensor cores with fp32 sums, the K scales on the
 // scores and the V scales on the probabilities.
 //
-//   plan_kernel   one CTA: the sequences' rows and lengths, checked, and where in all of
-//                 the work each sequence's begins;
+//   plan_kernel   one CTA (one more for chunk_tc.cu's units): the sequences' rows and
+//                 lengths, checked, and where in all of the work each sequence's begins;
 //   rows_kernel   a unit is 8 query rows of a KV head and its sequence's keys; each
 //                 warp takes an equal share of the units' steps of 16 keys;
 //   join_kernel   units that more than 8 warps share.
-// Sequences of more rows than 8 go to chunk_tc.cu.
+// Sequences of many rows go to chunk_tc.cu (kFewRows).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -186,10 +186,19 @@ __global__ void __launch_bounds__(kPlanThreads)
 // the fragment; movmatrix turns the probabilities for the second product.
 //
 // Warps work alone, each with a ring of stages of 16 keys that is filled two steps ahead
-// (by TMA, two boxes a step; by cp.async where steps are not within a page): each has the same share of all units' steps, so that they end together, and
-// while one of them waits for the first pages of its next unit the others go on.  (CTAs
-// of 8 warps on one unit met at its start and end and took 94 us for 64 sequences of
-// 2,050 tokens, 75 us with equal shares.)
+// (by TMA, two boxes a step; by cp.async where steps are not within a page).  Each has the
+// same share of all units' steps, so that they end together, and while one of them waits
+// for the first pages of its next unit the others go on.  (CTAs of 8 warps on one unit met
+// at its start and end and took 94 us for 64 sequences of 2,050 tokens, 75 us with equal
+// shares.)  Calls of few steps are cut into parts of 4 or 8 steps, a warp each, since a
+// warp alone takes about 2,000 clocks a step (7 sequences of 40 to 4,000 tokens: 28 us in
+// shares of 16, 12 us in parts of 4).
+//
+// What bounds it: instructions, 440 a step, a third of them the codes' way to fp16, at 0.55
+// a clock and scheduler with 16 warps an SM, and what warps wait for at their start, 14,000
+// clocks of 115,000.  64 sequences of 2,050 tokens, 32 / 8 heads (260 MB): 62 us, 4.2 TB/s;
+// 24 sequences of 1 to 8 tokens behind 100 to 4,000: 60 us.  (Units of 16 rows, 8 warps an
+// SM: 78 us for the latter.)
 
 constexpr int kStep = 16;      // keys of a step
 constexpr int kRows = 8;
@@ -915,9 +924,9 @@ constexpr int kMostWarps = 148 * 2 * kRowWarps;
 
 // Which kernels a call's sequences go to: those of few rows to the warps of rows_kernel,
 // the others to chunk_tc.cu, where it takes the shapes.  (24 sequences of 1 to 8 tokens in
-// groups of 4: 63 us by the warps; split at 8 rows 76 us and 33 us, since a unit there
-// costs 10 to 15 us to start and end.)  The lengths are on the device, so a call launches
-// both unless its sizes tell.
+// groups of 4: 60 us by the warps; 66 us by chunk_tc.cu, or 54 us there for those above 16
+// rows and 28 us by the warps for the rest, since a unit there costs about 10 us to start
+// and end.)  The lengths are on the device, so a call launches both unless its sizes tell.
 constexpr int kFewRows = 32, kFewSteps = 4096;
 struct Division {
   bool rows, tc;

@@ -12,6 +12,11 @@
 //   move_kernel   a cluster per (sequence, K or V, KV head), and one per sequence for
 //                 the weights.
 //
+// 64 sequences of 1,500 to 2,600 tokens cut to 1,024, 8 heads of 128: pick 10 us, move 73
+// us (268 MB, 3.7 TB/s): pieces of 128 bytes, read and written in turns, and 150
+// instructions for 16 codes (issue slots 61% busy).  32,768 tokens to 4,096: pick 16 us, a
+// cluster's passes one behind the other, move 18 us.
+//
 // A kept token never moves back: those of the new pages [a, b) come from token a * bs
 // or later.  The cluster therefore takes the new pages in rounds, reads all of a round's
 // tokens, meets, and writes them: nothing that a later round reads is overwritten.

