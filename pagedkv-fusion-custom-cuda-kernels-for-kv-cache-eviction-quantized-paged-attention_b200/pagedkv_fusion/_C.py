@@ -753,8 +753,6 @@ def shared_prefix_attention(q, k_cache_q, k_scale, v_cache_q, v_scale, prefix_ta
 def _query_rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` ``[tokens, heads, D]`` itself where its rows can be read in pieces of
     16 bytes (contiguous channels, strides and address of 16 bytes), else a copy."""
-    if t.is_contiguous() and t.data_ptr() % 16 == 0:  # (D is a multiple of 16 bytes)
-        return t
     a, b, c = t.stride()
     n = 16 // t.element_size()
     if t.numel() == 0 or (c == 1 and a % n == 0 and b % n == 0 and t.data_ptr() % 16 == 0):

@@ -321,6 +321,23 @@ def test_strides_alignment_and_integer_types(cuda):
         assert torch.equal(ops.chunk_attention(**more), want)
 
 
+def test_strides_of_single_rows(cuda):
+    """Dimensions of one have whatever stride their view left them: contiguous, but not to step by."""
+    from pagedkv_fusion import ops
+    for q_lens, lens, heads, kv_heads in (([1], [50], 8, 2), ([5], [70], 1, 1), ([1], [9], 1, 1)):
+        p = problem(18, q_lens, lens, heads, kv_heads, 64, 16, "bf16")
+        want = ops.chunk_attention(**p)
+        q = p["q"].as_strided(p["q"].shape, (p["q"].stride(0) if len(p["q"]) > 1 else 7,
+                                             p["q"].stride(1) if heads > 1 else 13, 1))
+        assert torch.equal(q, p["q"]) and torch.equal(ops.chunk_attention(**dict(p, q=q)), want)
+        weights = torch.zeros(p["k_cache_q"].shape[:2], device="cuda")
+        same = weights.clone()
+        args = {k: v for k, v in p.items() if not k.startswith("v_") and k != "q"}
+        ops.accumulate_attention(weights, p["q"], **args)
+        ops.accumulate_attention(same, q, **args)
+        assert torch.equal(weights, same)
+
+
 def test_large_cache_offsets(cuda):
     """Pages more than 2^32 bytes apart."""
     from pagedkv_fusion import ops
