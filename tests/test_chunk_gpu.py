@@ -12,9 +12,11 @@ channels, steps 2^-23 (two half steps of fp32, since tensor cores cut sums):
 * p times its V scale is one fp16 number for 16-bit queries (2^-11), two for fp32 (2^-20);
   below the smallest step of fp16 it is off by half of that, which is 2^-30 of the largest p
   and the largest V scale;
-* the result is rounded to its type (2^-11 fp16, 2^-8 bf16, 2^-24 fp32).
+* the result is rounded to its type (2^-11 fp16, 2^-8 bf16, 2^-24 fp32), or, below the
+  type's smallest normal number, where the step no longer shrinks, by half of that step,
+  r_sub: fp16's is 2^-24 below 2^-14, so 2^-25.
 
-|got - want| <= A (2 t + 2^-18 + 2 n 2^-23 + r_p) + 2^-30 n max(p) max|v| + r_out |want|
+|got - want| <= A (2 t + 2^-18 + 2 n 2^-23 + r_p) + 2^-30 n max(p) max|v| + r_out |want| + r_sub
 
 The log denominator is off by t + 2^-19 + n 2^-23 and the steps of its own 2^-22 |lse|.
 """
@@ -65,6 +67,7 @@ def reference(p, lost=None):
     lse = q.new_full(q.shape[:2], -math.inf)
     lse_tol, parts = torch.zeros_like(lse), []
     half = torch.finfo(p["q"].dtype).eps / 2
+    sub = torch.finfo(p["q"].dtype).tiny * half
     r_p = 2.0 ** -20 if p["q"].dtype == torch.float32 else 2.0 ** -11
     cu = p["cu_seqlens"].tolist()
     for i, n in enumerate(p["seq_lens"].tolist()):
@@ -93,7 +96,7 @@ def reference(p, lost=None):
                 w = torch.softmax(s, 1).nan_to_num(0.0)
                 want[a:b, j] = w @ v
                 tol[a:b, j] = (w @ v.abs()) * (2 * t + 2.0 ** -18 + 2 * n * 2.0 ** -23 + r_p)[:, None] + \
-                    2.0 ** -30 * n * (w.amax(1) * v.abs().max())[:, None] + half * want[a:b, j].abs()
+                    2.0 ** -30 * n * (w.amax(1) * v.abs().max())[:, None] + half * want[a:b, j].abs() + sub
                 lse_tol[a:b, j] = t + 2.0 ** -19 + n * 2.0 ** -23 + 2.0 ** -22 * lse[a:b, j].abs().nan_to_num(0, 0, 0)
                 parts.append((i, j, slice(a, b), n, w, t))
     return want, tol, lse, lse_tol, parts
