@@ -661,6 +661,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // (NaN moves nothing, and makes the row NaN)
           move = valid && t > m && (m == -INFINITY || (t - m) * rf > kRoom);
           if (!__any_sync(0xffffffffu, move)) break;
+          tmem_wait_store();  // O and P of this pass are there before the next one's accesses
           big = 0.0f;
         }
         next = (t - m) * rf > kLazy ? t : m;
