@@ -64,7 +64,7 @@ struct TcCfg {
   static constexpr int kOffKV = 2 * HALVES * kTileBytes;
   static constexpr int kOffScale = kOffKV + kStages * kTileBytes;  // [slot][k, v][8 groups]
   static constexpr int kOffMask = kOffScale + kSlots * 64;  // [slot]: bits of the groups that count, K scales
-                                                            // that are negative or not finite
+                                                            // times sm_scale negative or not finite
   static constexpr int kOffMax = kOffMask + kSlots * 4;     // [slot]: the largest V scale
   // (base, l) of the rows of a row tile: behind the results in its query tile, or apart
   static constexpr int kOffMl = DP == 128 ? kOffQ + 16384 : kOffMax + kSlots * 4;
@@ -274,10 +274,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
             if (kind == 0) {
               // (what the slot held is used: three tiles at most are in flight)
-              if (lane < 16) s_scale[slot * 16 + lane] = lane < 8 ? scale * p.qk_scale : scale;
+              const float factor = lane < 8 ? scale * p.qk_scale : scale;
+              if (lane < 16) s_scale[slot * 16 + lane] = factor;
               // groups behind the length are hidden by the rows' limits
               const unsigned count = boxes | __ballot_sync(0xffffffffu, token >= len);
-              const bool odd = __any_sync(0xffffffffu, lane < 8 && !(scale >= 0.0f && scale <= 3.0e38f));
+              // (a negative sm_scale turns the order around as a negative K scale does)
+              const bool odd = __any_sync(0xffffffffu, lane < 8 && !(factor >= 0.0f && factor <= 3.0e38f));
               // the largest V scale; infinity where one is not finite
               const float a = fabsf(scale);
               const uint32_t big = __reduce_max_sync(

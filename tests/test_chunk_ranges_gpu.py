@@ -31,3 +31,19 @@ def test_rising_v_scales_beside_rising_scores(cuda, dtype, q_lens, lens, heads, 
     check(p)
     p["v_scale"][pages] *= 1.7 ** -step * 2.0 ** -(step % 3)  # and falling again
     check(p)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("q_lens,lens,heads,kv_heads,dim,bs", [
+    ([1, 2], [900, 333], 8, 2, 128, 16), ([200], [1500], 8, 2, 128, 16), ([90, 1], [1500, 40], 8, 2, 64, 32),
+    ([16], [5000], 8, 1, 128, 16), ([1, 40], [300, 90], 8, 2, 160, 5),
+])
+def test_scale_of_any_sign(cuda, dtype, q_lens, lens, heads, kv_heads, dim, bs):
+    """A negative sm_scale turns the scores' order around, for all keys or (with negative K scales)
+    for some; the scores spread over tens of powers of two.  With 0 all keys weigh the same."""
+    for spread, factor in ((0.1, -1.0), (0.5, -1.0), (0.5, -4.0), (0.5, 0.0)):
+        p = problem(32, q_lens, lens, heads, kv_heads, dim, bs, dtype, spread=spread)
+        p["sm_scale"] *= factor
+        check(p)
+        p["k_scale"][::3] *= -1
+        check(p)
