@@ -211,6 +211,13 @@ constexpr int kJoinHere = 8;   // parts that the last of them joins; more are le
 // warp's largest: fp16's smallest step, 2^-24, is then 2^-37 of the row's largest p.
 constexpr float kLazy = 2.0f;
 constexpr float kPShift = 13.0f;
+// The tensor cores cut the bits that an fp32 sum cannot hold, and a sum of many exponentials drops
+// those below its last place: V of one sign lost 1.5e-4 to 2.3e-4 over 32,768 keys of a warp, the
+// log denominator up to 4e-5.  Every so many keys a warp's O and l therefore join those of the
+// keys before, rounded to nearest, which wait in its slot: 3.3e-6 and 1e-5 at any length, and with
+// 16-bit queries 2.2e-5 of O, a tenth of the results' rounding to fp16.  (fp32, 64 sequences of
+// 8,192 tokens, 8 heads: 216 -> 224 us; of 2,050, 32 / 8 heads: 71.8 -> 73.5.  16 bits: no change.)
+constexpr int kSumKeysF32 = 512, kSumKeys16 = 4096;
 
 template <int DP, bool PV, bool WHOLE>
 struct RowsCfg {
@@ -329,6 +336,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, PV, WHOLE>::kCtas)
   constexpr int kV = kStep * DP;                // V of a stage
   constexpr int kRun = DP >= 128 ? 16 : 8;      // consecutive channels of a lane's results
   constexpr int kRuns = (DP + 127) / 128;
+  constexpr int kSumKeys = HALVES == 2 ? kSumKeysF32 : kSumKeys16;
   extern __shared__ __align__(1024) uint8_t smem[];
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int in_cta = threadIdx.x >> 5;
@@ -508,8 +516,73 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, PV, WHOLE>::kCtas)
     // times scale stays in fp16
     float unit_v = 0.0f, inv_v = 0.0f;
 
+    // channels c * 128 + g * kRun + 4 x on of row 2 t + r
+    const auto result = [&](int r, int c, int x, float by) {
+      const int at = c * 8 + 2 * x;
+      return make_float4(o[at][r] * by, o[at][r + 2] * by, o[at + 1][r] * by, o[at + 1][r + 2] * by);
+    };
+    const auto sum_over_lanes = [&]() {  // l of all the lanes of a row
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], x);
+    };
+    // The sums of earlier keys, in the slot as a part's: rows of O, then (base, l).
+    uint8_t* slot = u.slot<S::kBytes>(p, warp - u.warp0);
+    bool summed = false;
+    const auto join_sums = [&](bool keep) {
+      if (summed) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float2 was = reinterpret_cast<const float2*>(slot + S::kMl)[2 * t + r];
+          const float f = was.y == 0.0f ? 0.0f : ex2(was.x - base[r]);
+          if (g == 0) l[r] += was.y * f;
+          if constexpr (PV) {
+            const float* from = reinterpret_cast<const float*>(slot) + (2 * t + r) * DP;
+            const float by = f * inv_v;
+#pragma unroll
+            for (int c = 0; c < kRuns; ++c)
+#pragma unroll
+              for (int x = 0; x < kRun / 4; ++x) {
+                const float4 v = *reinterpret_cast<const float4*>(from + c * 128 + g * kRun + 4 * x);
+                const int at = c * 8 + 2 * x;
+                o[at][r] += v.x * by, o[at][r + 2] += v.y * by;
+                o[at + 1][r] += v.z * by, o[at + 1][r + 2] += v.w * by;
+              }
+          }
+        }
+        __syncwarp();  // (base, l) are read
+      }
+      sum_over_lanes();
+      if (!keep) return;
+      summed = true;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        if constexpr (PV) {
+          float* to = reinterpret_cast<float*>(slot) + (2 * t + r) * DP;
+#pragma unroll
+          for (int c = 0; c < kRuns; ++c)
+#pragma unroll
+            for (int x = 0; x < kRun / 4; ++x)
+              *reinterpret_cast<float4*>(to + c * 128 + g * kRun + 4 * x) = result(r, c, x, unit_v);
+        }
+        if (g == 0) reinterpret_cast<float2*>(slot + S::kMl)[2 * t + r] = make_float2(base[r], l[r]);
+        l[r] = 0.0f;
+      }
+      if constexpr (PV) {
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
+      }
+      __syncwarp();
+    };
+
     int used = 0;  // the stage
-    for (int key_now = k0; key_now < k1; key_now += kStep) {
+    for (int key_now = k0;; key_now += kStep) {
+      const bool end = key_now >= k1;
+      if (end || (key_now > k0 && (key_now - k0) % kSumKeys == 0)) join_sums(!end);
+      if (end) break;
       copies_wait<kStages - 2>();
       __syncwarp();
       issue();
@@ -681,15 +754,6 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, PV, WHOLE>::kCtas)
     }
     copies_wait<0>();
     __syncwarp();
-#pragma unroll
-    for (int r = 0; r < 2; ++r)
-#pragma unroll
-      for (int x = 4; x < 32; x <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], x);
-    // channels c * 128 + g * kRun + 4 x on of row 2 t + r
-    const auto result = [&](int r, int c, int x, float by) {
-      const int at = c * 8 + 2 * x;
-      return make_float4(o[at][r] * by, o[at][r + 2] * by, o[at + 1][r] * by, o[at + 1][r + 2] * by);
-    };
     if (u.parts == 1) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
@@ -711,7 +775,6 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, PV, WHOLE>::kCtas)
       }
       continue;
     }
-    uint8_t* slot = u.slot<S::kBytes>(p, warp - u.warp0);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       if (2 * t + r >= rows) continue;
