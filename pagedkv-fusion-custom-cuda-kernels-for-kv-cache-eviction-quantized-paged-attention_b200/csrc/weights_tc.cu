@@ -5,7 +5,8 @@
 // of 128 keys; one CTA per SM takes an equal share of all units' tiles.  The keys are the
 // products' M and the rows their N:
 //   S^T = K Q^T   tcgen05 kind::f16, 128 x (rows), K's codes as exact fp16 and Q as fp16
-//                 times a power of two of the unit (two numbers for fp32 queries)
+//                 times a power of two (two numbers for fp32 queries): of the unit, or, for
+//                 rows much smaller than its largest, of the row
 // so that a thread has a key and its sum over the rows crosses no lanes.  Q stays in
 // shared memory for the segment, the K tiles pass, and their products have two buffers
 // in tensor memory, each read by a warpgroup of its own.
@@ -32,6 +33,10 @@ constexpr int kKeys = kTileKeys;
 constexpr int kThreads = 512;
 constexpr int kConvWarp = 8, kMmaWarp = 12, kLoadWarp = 14;
 constexpr int kSlots = 8;  // scales of so many tiles
+// Rows whose largest query is within 2^kNear of the unit's share its power of two: their
+// operands keep 2^-26 of the row's largest.  Units with other rows take the masked tiles' loop,
+// where each row has its own.
+constexpr int kNear = 8;
 
 template <int DP, int HALVES>
 struct GatherCfg {
@@ -44,7 +49,8 @@ struct GatherCfg {
   static constexpr int kOffLimit = kOffLse + kRows * 4;
   static constexpr int kOffScale = kOffLimit + kRows * 4;       // [slot][8 groups]
   static constexpr int kOffRow = kOffScale + kSlots * 32;       // [slot][8 groups]: cache rows
-  static constexpr int kOffBar = kOffRow + kSlots * 32;
+  static constexpr int kOffPower = kOffRow + kSlots * 32;       // [row]: exponents, 8 bits
+  static constexpr int kOffBar = kOffPower + kRows;
   static constexpr int kBars = 3 * kStages + kSlots + 1 + 2 + 2 + 1;
   static constexpr int kOffMisc = kOffBar + kBars * 8;
   static constexpr int kSmemBytes = kOffMisc + 16 + 32;
@@ -83,7 +89,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* s_full = q_full + 1;   // per buffer, as the next
   uint64_t* s_empty = s_full + 2;
   uint64_t* mma_done = s_empty + 2;
+  int8_t* s_power = reinterpret_cast<int8_t*>(smem + C::kOffPower);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
+  uint8_t* s_apart = smem + C::kOffMisc + 8;  // of each staging warp
   float* s_big = reinterpret_cast<float*>(smem + C::kOffMisc + 16);  // of each staging warp
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -274,6 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (u.n == 0) continue;
       named_barrier(2, 256);  // both warpgroups have seen every product of the last segment
       float down = 1.0f;      // what the products are multiplied by, for the power of two
+      bool apart = false;     // rows have their own, s_power's
       {
         // thread = row: its denominator, how far it sees, and its queries
         const int r = tid;
@@ -293,28 +302,35 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint8_t* tile = smem + C::kOffQ;
         copy_query_rows<T, DP, kBox>(smem_u32(tile), r - lane, any, mine, u.rows - (r - lane), p.dim);
         if constexpr (!std::is_same<T, __half>::value) {
-          // the largest of the unit is scaled to [2^10, 2^11): what rows of smaller ones lose
-          // is below 2^-36 of it
-          float big = query_row_most<T, DP, kBox>(tile, r);
-          big = big <= 3.0e38f ? big : 0.0f;  // (the row's weights are NaN anyway)
-          big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
+          // the largest magnitude is scaled to [2^10, 2^11); infinity and NaN are no matter,
+          // since they take their row's weights with them
+          const float row_big = query_row_most<T, DP, kBox>(tile, r);
+          const bool finite = row_big <= 3.402823466e38f;
+          float big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(finite ? row_big : 0.0f)));
           if (lane == 0) s_big[warp] = big;
           named_barrier(2, 256);
           for (int w = 0; w < 8; ++w) big = fmaxf(big, s_big[w]);
-          const int e = row_exponent(big);
-          down = power_of_two(-e);
+          const int unit_e = row_exponent(big), own_e = row_exponent(row_big);
+          const bool far = finite && row_big != 0.0f && own_e - unit_e > kNear;
+          const int e = far ? own_e : unit_e;
+          down = power_of_two(-unit_e);
+          s_power[r] = (int8_t)-e;
+          apart = __any_sync(0xffffffffu, far);
+          if (lane == 0) s_apart[warp] = apart;
           split_query_row<T, DP, kBox>(tile, r, power_of_two(e));
         }
         fence_proxy_async_smem();  // an MMA operand
         mbar_arrive(q_full);
         named_barrier(2, 256);  // all denominators are there
+        if constexpr (!std::is_same<T, __half>::value)
+          for (int w = 0; w < 8; ++w) apart |= s_apart[w] != 0;
       }
-      const int clear = s_limit[0];  // every row sees the keys below
+      const int clear = apart ? 0 : s_limit[0];  // every row sees the keys below
       const int columns = (u.rows + 31) / 32 * 32;
       for (int j = (before & 1) == x ? 0 : 1; j < u.n; j += 2) {
         const int jj = before + j, slot = jj % kSlots;
         wait(&sc_full[slot], jj / kSlots);
-        const float k = s_scale[slot * 8 + row / 16] * down;
+        const float k_scale = s_scale[slot * 8 + row / 16], k = k_scale * down;
         const uint32_t group = s_row[slot * 8 + row / 16];
         const int key = (u.tile0 + j) * kKeys + row;
         wait(&s_full[x], jj / 2);
@@ -348,18 +364,23 @@ __global__ void __launch_bounds__(kThreads, 1)
               sum[e & 1] = add_f32x2(sum[e & 1], f32x2(ex2(z[e].x), ex2(z[e].y)));
           }
         } else {
-          // tiles with keys that some row does not see
+          // tiles with keys that some row does not see, or rows with powers of their own
           float total = 0.0f;
+          const auto masked = [&](auto own) {
 #pragma unroll 1
-          for (int c = 0; c < columns; c += 32) {
-            tmem_load<32>(s_at + c, w);
-            tmem_wait_load();
+            for (int c = 0; c < columns; c += 32) {
+              tmem_load<32>(s_at + c, w);
+              tmem_wait_load();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const float z = ex2(fmaf(__uint_as_float(w[e]), k, -s_lse[c + e]));
-              total += key < s_limit[c + e] ? z : 0.0f;
+              for (int e = 0; e < 32; ++e) {
+                const float by = decltype(own)::value ? k_scale * power_of_two(s_power[c + e]) : k;
+                const float z = ex2(fmaf(__uint_as_float(w[e]), by, -s_lse[c + e]));
+                total += key < s_limit[c + e] ? z : 0.0f;
+              }
             }
-          }
+          };
+          if (std::is_same<T, __half>::value || !apart) masked(std::false_type{});
+          else masked(std::true_type{});
           sum[0] = f32x2(total, 0.0f);
           tmem_fence_before_sync();
           mbar_arrive(&s_empty[x]);
