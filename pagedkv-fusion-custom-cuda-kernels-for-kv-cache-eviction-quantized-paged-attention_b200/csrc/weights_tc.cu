@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* mma_done = s_empty + 2;
   int8_t* s_power = reinterpret_cast<int8_t*>(smem + C::kOffPower);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
-  uint8_t* s_apart = smem + C::kOffMisc + 8;  // of each staging warp
+  uint8_t* s_rows = smem + C::kOffMisc + 8;  // of each staging warp: 1: far rows, 2: idle ones
   float* s_big = reinterpret_cast<float*>(smem + C::kOffMisc + 16);  // of each staging warp
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -282,22 +282,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (u.n == 0) continue;
       named_barrier(2, 256);  // both warpgroups have seen every product of the last segment
       float down = 1.0f;      // what the products are multiplied by, for the power of two
-      bool apart = false;     // rows have their own, s_power's
       {
         // thread = row: its denominator, how far it sees, and its queries
         const int r = tid;
         const T* any = static_cast<const T*>(p.q);
         const T* mine = any;
-        float lse2 = INFINITY;  // rows that are not there, or see nothing, add nothing
+        float lse2 = INFINITY;  // rows that are not there, or have no denominator, add nothing
+        bool idle = false, far = false;
         if (r < u.rows) {
           int h;
           const int64_t tok = u.token(p, r, &h);
           mine += tok * p.q_tok + h * p.q_head;
           const float v = p.lse[tok * p.heads + h];
-          if (v != -INFINITY) lse2 = v * kLog2e;
+          idle = v == -INFINITY;
+          if (!idle) lse2 = v * kLog2e;
         }
         s_lse[r] = lse2;
-        s_limit[r] = u.limit(p, r);
+        s_limit[r] = idle ? 0 : u.limit(p, r);  // (their queries may be NaN)
         constexpr int kBox = kRows * 128;
         uint8_t* tile = smem + C::kOffQ;
         copy_query_rows<T, DP, kBox>(smem_u32(tile), r - lane, any, mine, u.rows - (r - lane), p.dim);
@@ -311,21 +312,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           named_barrier(2, 256);
           for (int w = 0; w < 8; ++w) big = fmaxf(big, s_big[w]);
           const int unit_e = row_exponent(big), own_e = row_exponent(row_big);
-          const bool far = finite && row_big != 0.0f && own_e - unit_e > kNear;
+          far = finite && row_big != 0.0f && own_e - unit_e > kNear;
           const int e = far ? own_e : unit_e;
           down = power_of_two(-unit_e);
           s_power[r] = (int8_t)-e;
-          apart = __any_sync(0xffffffffu, far);
-          if (lane == 0) s_apart[warp] = apart;
           split_query_row<T, DP, kBox>(tile, r, power_of_two(e));
         }
+        // (rows that see no key anyway are not the point)
+        const int odd = (__any_sync(0xffffffffu, far) ? 1 : 0) |
+                        (__any_sync(0xffffffffu, idle && u.limit(p, r) > 0) ? 2 : 0);
+        if (lane == 0) s_rows[warp] = (uint8_t)odd;
         fence_proxy_async_smem();  // an MMA operand
         mbar_arrive(q_full);
         named_barrier(2, 256);  // all denominators are there
-        if constexpr (!std::is_same<T, __half>::value)
-          for (int w = 0; w < 8; ++w) apart |= s_apart[w] != 0;
       }
-      const int clear = apart ? 0 : s_limit[0];  // every row sees the keys below
+      int odd_rows = 0;
+      for (int w = 0; w < 8; ++w) odd_rows |= s_rows[w];
+      const bool apart = odd_rows & 1;                   // rows have their own power, s_power's
+      const int clear = odd_rows != 0 ? 0 : s_limit[0];  // every row sees, and counts for, the keys below
       const int columns = (u.rows + 31) / 32 * 32;
       for (int j = (before & 1) == x ? 0 : 1; j < u.n; j += 2) {
         const int jj = before + j, slot = jj % kSlots;
@@ -364,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               sum[e & 1] = add_f32x2(sum[e & 1], f32x2(ex2(z[e].x), ex2(z[e].y)));
           }
         } else {
-          // tiles with keys that some row does not see, or rows with powers of their own
+          // tiles with keys that some row does not see, or with odd rows
           float total = 0.0f;
           const auto masked = [&](auto own) {
 #pragma unroll 1

@@ -79,3 +79,17 @@ def test_negative_scale(cuda, dtype, q_lens, lens, bs):
     p["sm_scale"] *= -3
     for given in (False, True):
         check(p, given)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("q_lens,lens,bs", SHAPES)
+def test_rows_without_denominator_add_nothing(cuda, dtype, q_lens, lens, bs):
+    """Whatever their queries hold."""
+    from pagedkv_fusion import ops
+    p = problem(43, q_lens, lens, 8, 2, 128, bs, dtype)
+    lse = ops.chunk_attention(**p, return_lse=True)[1]
+    some = torch.rand(lse.shape, device="cuda") < 0.7
+    want = rows_alone(p, some, lse)
+    for bad in (math.nan, math.inf):
+        broken = dict(p, q=torch.where(some[..., None], p["q"], bad))
+        assert torch.equal(rows_alone(broken, some, lse), want)
