@@ -472,7 +472,7 @@ int pkv_chunk_attention(const void *q, int32_t dtype, const int8_t *k_cache,
  * call returned, or NULL: then it is computed first.  A row whose lse is -inf adds
  * nothing; NaN reaches the weights of the keys that its row sees.  Pages may be in
  * several tables; the result does not depend on the order of execution (sums meet as
- * integers, in steps of 2^-38).  total_q * num_heads <= 2^25.
+ * integers, in steps of 2^-37).  total_q * num_heads <= 2^25.
  */
 size_t pkv_accumulate_attention_workspace_size(
     int64_t total_q, int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,

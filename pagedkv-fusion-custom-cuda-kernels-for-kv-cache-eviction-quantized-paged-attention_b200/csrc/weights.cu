@@ -13,9 +13,9 @@
 //                     pass;
 //   spread_kernel     adds the sums to the weights.
 //
-// Sums of several items, and of sequences that share pages, meet as integers of 2^-38
+// Sums of several items, and of sequences that share pages, meet as integers of 2^-37
 // in a workspace, so that the order of their arrival changes nothing: a weight is then off
-// by half a step for each of them, 2^-39.
+// by half a step for each of them, 2^-38.
 #include <cuda_runtime.h>
 
 #include <algorithm>

@@ -6,9 +6,10 @@
 
 namespace pkv {
 
-// Weights meet as integers of 2^-38, so that the order of their arrival changes nothing;
-// 2^25 of weight before bit 63, which says that a sum was not finite.
-constexpr float kWeightUnit = 274877906944.0f;
+// Weights meet as integers of 2^-37, so that the order of their arrival changes nothing;
+// the 2^25 rows that a call may have give a token up to 2^62, with the roundings of their
+// exponentials, and bit 63 says that a sum was not finite.
+constexpr float kWeightUnit = 137438953472.0f;
 constexpr unsigned long long kNotFinite = 1ull << 63;
 
 __device__ __forceinline__ void add_weight(unsigned long long* sum, float v) {

@@ -93,3 +93,19 @@ def test_rows_without_denominator_add_nothing(cuda, dtype, q_lens, lens, bs):
     for bad in (math.nan, math.inf):
         broken = dict(p, q=torch.where(some[..., None], p["q"], bad))
         assert torch.equal(rows_alone(broken, some, lse), want)
+
+
+@pytest.mark.parametrize("bs", [16, 5])
+def test_the_largest_sum(cuda, bs):
+    """2^25 rows, the most of a call, with all their weight on one token: 2^22 sequences of 8 heads
+    that share a page and have one token each."""
+    S, H, D = 1 << 22, 8, 32
+    q = torch.zeros(S, H, D, dtype=torch.float16, device="cuda")
+    k = torch.zeros(2, bs, 1, D, dtype=torch.int8, device="cuda")
+    args = dict(q=q, k_cache_q=k, k_scale=torch.ones(2, 1, device="cuda"),
+                block_tables=torch.ones(S, 1, dtype=torch.int32, device="cuda"),
+                seq_lens=torch.ones(S, dtype=torch.int32, device="cuda"),
+                cu_seqlens=torch.arange(S + 1, dtype=torch.int32, device="cuda"), sm_scale=1.0)
+    got = call(args, torch.zeros(2, bs, device="cuda"), torch.zeros(S, H, device="cuda"))
+    assert float(got[1, 0]) == S and float(got.sum()) == S
+    assert cuda.read_device_error() == 0
