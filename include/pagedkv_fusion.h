@@ -498,12 +498,13 @@ int pkv_accumulate_attention(float *weights, const void *q, int32_t dtype,
  * num_kv_heads, head_dim], scale_cache fp32 [2, num_blocks, num_kv_heads] and weights
  * fp32 [num_blocks, block_size].  A page's new scale is the largest old scale of the
  * tokens it now holds, per KV head, K and V apart; codes become rint(code * (old /
- * new)) where old < new.  The slots that the sequence no longer uses keep their codes
- * and get weight 0.  lens_out int32 [num_seqs] receives the new lengths, kept int32
+ * new)) where old < new, clamped to -127 .. 127 where old is negative.  The slots
+ * that the sequence no longer uses keep their codes and get weight 0.  lens_out int32 [num_seqs] receives the new lengths, kept int32
  * [num_seqs, keep] the old places of the tokens that stay, ascending, then -1.
  * Sequences of at most `keep` tokens stay as they are, and so do those with a page
  * outside the cache (PKV_DEVERR_BAD_BLOCK_ID; their row of kept is -1).  The pages of a
- * sequence that is cut must not be in another sequence's table.  keep >= 1,
+ * sequence that is cut must not be in another sequence's table, nor twice in its own.
+ * keep >= 1,
  * sinks + recent <= keep, block_size <= 64, head_dim <= 256.
  */
 int pkv_evict_tokens(int8_t *kv_cache, float *scale_cache, float *weights,

@@ -4,8 +4,8 @@
 // the heaviest of the others (of equal weights the earlier), `keep` in all, in order, at
 // the front of its pages.  A page's new scale is the largest of its tokens' old ones, per
 // KV head and for K and V apart; codes become rint(code (old / new)) where the old scale
-// was smaller, and move as they are else.  The weights move along; the slots behind the
-// last token that were in use get weight 0.
+// was smaller (clamped to -127 .. 127 where it was negative), and move as they are else.  The
+// weights move along; the slots behind the last token that were in use get weight 0.
 //
 //   pick_kernel   a CTA or a cluster per sequence: the weights' sort keys, the key that the last
 //                 kept token has (radix, 8 bits a pass), the kept tokens in order;
@@ -238,7 +238,7 @@ struct Piece<1> { using T = uint8_t; };
 // rint(code ratio) of four codes.  A byte in the low mantissa of 2^23 is a number, and a
 // number at 1.5 2^23 is rounded to an integer, to even as rint, whose low byte is there: the
 // conversion instructions, 16 a clock and SM, would take 90 us of the 64 sequences' move.
-// (Only a scale of the other sign can take a code out of its range.)
+// (Only where the old scale is negative can a code leave its range: the ratio is not 0 to 1 then.)
 __device__ __forceinline__ uint32_t shrink4(uint32_t w, float ratio) {
   const uint32_t u = w ^ 0x80808080u;
   uint32_t x[4];
@@ -251,7 +251,7 @@ __device__ __forceinline__ uint32_t shrink4(uint32_t w, float ratio) {
     x[i] = __float_as_uint(__fadd_rn(__fmul_rn(c.x, ratio), 12582912.0f));
     x[i + 1] = __float_as_uint(__fadd_rn(__fmul_rn(c.y, ratio), 12582912.0f));
   }
-  if (ratio < -1.0f)
+  if (!(ratio >= 0.0f && ratio <= 1.0f))
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       x[i] = __float_as_uint(fminf(fmaxf(__uint_as_float(x[i]), 12582912.0f - 127.0f), 12582912.0f + 127.0f));

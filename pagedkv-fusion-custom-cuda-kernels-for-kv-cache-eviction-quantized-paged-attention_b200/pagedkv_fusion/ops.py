@@ -529,7 +529,7 @@ def evict_tokens(kv_cache_int8, scale_cache, weights, block_tables, seq_lens, ke
     Returns ``(lens, kept)``: the new lengths, int32 ``[S]``, and the old places of
     the tokens that stayed, int32 ``[S, keep]``, ascending, then -1.  The pages
     behind the new lengths are free.  A sequence that is cut must not share pages
-    with another one.  CUDA tensors only.
+    with another one, nor have one twice.  CUDA tensors only.
     """
     return _lib().evict_tokens(kv_cache_int8, scale_cache, weights, block_tables, seq_lens, keep,
                                sinks, recent)
