@@ -1,4 +1,5 @@
-"""evict_tokens: scales of both signs and infinite ones, by the rule."""
+"""evict_tokens: scales of both signs and infinite ones, by the rule; long sequences whose sort
+keys are read from the weights again and again."""
 
 from __future__ import annotations
 
@@ -6,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_evict_tokens_gpu import problem, run
+from test_evict_tokens_gpu import check, problem, run
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +52,25 @@ def test_scales_of_both_signs(cuda, dim):
     by_the_rule(p, 80, 3, 5)
     p["scale_cache"] = -p["scale_cache"].abs()  # all negative: the one nearest to zero is the largest
     by_the_rule(p, 80, 3, 5)
+
+
+def test_infinite_scales(cuda):
+    """A page with a token of infinite scale takes it: codes of finite scales become 0, the others
+    stay."""
+    p = problem(22, [200, 150], 2, 64, 16)
+    p["scale_cache"][0, ::3] = float("inf")
+    p["scale_cache"][1, 1::4] = float("inf")
+    got, _, kept = by_the_rule(p, 60, 2, 2)
+    page = got["kv_cache_int8"][0, p["block_tables"][0, 0].long()]
+    old = p["scale_cache"][0, p["block_tables"][0, kept[0, :16].long() // 16].long(), 0]
+    if bool(old.isinf().any()):
+        assert bool((page[~old.isinf(), 0] == 0).all()) and bool((page[old.isinf(), 0] != 0).any())
+
+
+@pytest.mark.parametrize("long,others,keep", [(50000, 75, 20000), (98304, 74, 98303), (49153, 148, 3)])
+def test_keys_that_do_not_fit_on_chip(cuda, long, others, keep):
+    """One long sequence beside so many that each has one CTA."""
+    p = problem(23, [long] + [40] * others, 1, 32, 16)
+    check(p, keep, min(keep, 2) - 1, 1)
+    p["weights"].copy_(torch.round(p["weights"] * 4) / 4)  # few values: the earlier token stays
+    check(p, keep, 0, 0)
