@@ -842,8 +842,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, PV, WHOLE>::kCtas)
           }
 #pragma unroll
           for (int r = 0; r < kRows; ++r) {
-            const float k = __shfl_sync(0xffffffffu, by[i], r);
-            if (k == 0.0f) continue;
+            const float k = __shfl_sync(0xffffffffu, by[i], r);  // (of a part of little weight 0: NaN stays)
             acc[r].x += v[r].x * k, acc[r].y += v[r].y * k, acc[r].z += v[r].z * k, acc[r].w += v[r].w * k;
           }
         }

@@ -47,3 +47,23 @@ def test_scale_of_any_sign(cuda, dtype, q_lens, lens, heads, kv_heads, dim, bs):
         check(p)
         p["k_scale"][::3] *= -1
         check(p)
+
+
+def test_values_that_are_not_finite_reach_rows_that_see_them(cuda):
+    """However little weight they have there, and in whichever part of the keys they are."""
+    from pagedkv_fusion import ops
+    for q_lens, lens, heads, kv_heads in (([1], [60], 8, 2), ([1], [300], 8, 2), ([1, 2], [900, 200], 8, 2),
+                                          ([1], [9000], 8, 2), ([300], [900], 8, 2), ([16], [6000], 8, 1)):
+        p = problem(33, q_lens, lens, heads, kv_heads, 128, 16, "f32", spread=0.0)
+        p["q"].abs_().add_(0.5).mul_(4)  # 200 nats from page to page
+        p["k_cache_q"].fill_(-100)
+        p["k_cache_q"][p["block_tables"][0, 0].long()] = 100  # the first page has all of the weight
+        want = ops.chunk_attention(**p)
+        assert bool(torch.isfinite(want).all())
+        for page in sorted({1, lens[0] // 32, (lens[0] - q_lens[0]) // 16 - 1} - {0}):
+            for bad in (float("inf"), float("nan")):
+                broken = dict(p, v_scale=p["v_scale"].clone())
+                broken["v_scale"][p["block_tables"][0, page].long()] = bad
+                out = ops.chunk_attention(**broken)
+                assert not bool(torch.isfinite(out[:q_lens[0]]).any()), (lens, page, bad)
+                assert torch.equal(out[q_lens[0]:], want[q_lens[0]:])
