@@ -347,8 +347,10 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowsCfg<DP, PV, WHOLE>::kCtas)
   uint64_t hold = 0;
   if constexpr (WHOLE) {
     if (lane == 0) {
-      prefetch_tensormap(&map_k);
-      if (PV) prefetch_tensormap(&map_v);
+      if (p.num_blocks > 0) {  // (an empty cache has no maps)
+        prefetch_tensormap(&map_k);
+        if (PV) prefetch_tensormap(&map_v);
+      }
       for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1);
       mbar_fence_init();
     }

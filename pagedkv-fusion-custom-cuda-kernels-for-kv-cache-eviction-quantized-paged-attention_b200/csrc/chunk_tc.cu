@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // loaded two tiles ahead, its scales (K: lanes 0-7, V: 8-15) one.
       const uint64_t hold = l2_policy_evict_last();
       const float* scales = lane < 8 ? p.k_scale : p.v_scale;
-      if (lane == 0) {
+      if (lane == 0 && p.num_blocks > 0) {  // (an empty cache has no maps)
         prefetch_tensormap(&map_k);
         prefetch_tensormap(&map_v);
       }

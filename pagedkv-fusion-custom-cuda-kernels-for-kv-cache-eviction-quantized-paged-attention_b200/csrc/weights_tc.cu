@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Lane l has the tile's group l & 7 of 16 tokens, which is on one page: its entry is
     // loaded two tiles ahead, its scale one.
     const uint64_t hold = l2_policy_evict_first();
-    if (lane == 0) prefetch_tensormap(&map_k);
+    if (lane == 0 && p.num_blocks > 0) prefetch_tensormap(&map_k);  // (an empty cache has no map)
     int loaded = 0;
     for (int64_t now = begin; now < stop && ok; now = u.at + u.seq.steps + kTileOver) {
       u.find(p, now, share);

@@ -67,3 +67,21 @@ def test_values_that_are_not_finite_reach_rows_that_see_them(cuda):
                 out = ops.chunk_attention(**broken)
                 assert not bool(torch.isfinite(out[:q_lens[0]]).any()), (lens, page, bad)
                 assert torch.equal(out[q_lens[0]:], want[q_lens[0]:])
+
+
+def test_cache_without_pages(cuda):
+    """Nothing is cached: every row is zero; lengths and table entries all the same are errors."""
+    from pagedkv_fusion import ops
+    for q_lens, lens, kv_heads, bs in (([1, 2], [0, 0], 2, 16), ([300, 40], [0, 0], 2, 16), ([300], [600], 1, 16),
+                                       ([2], [40], 2, 16), ([40], [60], 2, 5)):
+        p = problem(34, q_lens, lens, 8, kv_heads, 128, bs, "bf16", wide=1)
+        for name in ("k_cache_q", "v_cache_q", "k_scale", "v_scale"):
+            p[name] = p[name][:0].clone()
+        out, lse = ops.chunk_attention(**p, return_lse=True)
+        assert bool((out == 0).all()) and bool((lse == -float("inf")).all())
+        assert cuda.read_device_error() == (1 if max(lens) else 0)
+        args = {k: v for k, v in p.items() if not k.startswith("v_")}
+        weights = torch.zeros(0, bs, device="cuda")
+        for given in (lse, None):
+            ops.accumulate_attention(weights, **args, lse=given)
+        assert cuda.read_device_error() in ((0, 1) if max(lens) else (0,))
