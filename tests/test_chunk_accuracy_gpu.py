@@ -97,3 +97,22 @@ def test_mean_of_16_bit_results(cuda, q_lens, keys, heads, kv_heads, dim, bs):
     want = exact(p)[0]
     mean = float((ops.chunk_attention(**p).double() - want).mean() / want.mean())
     assert abs(mean) <= 6e-5, mean
+
+
+@pytest.mark.parametrize("dtype,q_lens,keys,heads,kv_heads,dim,bs,more", [
+    # few rows: P as two fp16 numbers for fp16 results, as one for bf16 ones
+    ("f16", [1] * 60, 4096, 40, 40, 128, 16, 1.03), ("f16", [4, 1, 8], 3000, 32, 8, 64, 24, 1.03),
+    ("f16", [1, 3], 5000, 8, 2, 256, 16, 1.03),
+    ("bf16", [1] * 60, 4096, 40, 40, 128, 16, 1.015), ("bf16", [4, 1, 8], 3000, 32, 8, 64, 24, 1.015),
+    # many: one number
+    ("f16", [512], 4096, 8, 2, 128, 16, 1.5), ("bf16", [512], 4096, 8, 2, 128, 16, 1.015),
+])
+def test_error_beside_the_rounding_of_results(cuda, dtype, q_lens, keys, heads, kv_heads, dim, bs, more):
+    """V of either sign: the error is at most `more` times what rounding the exact result leaves.
+    A rounding of P to fp16 is like the result's own to fp16 (sqrt(2) of it together) and an eighth
+    of one to bf16 (1.008)."""
+    from pagedkv_fusion import ops
+    p = accuracy_problem(q_lens, keys, heads, kv_heads, dim, bs, dtype)
+    p["v_cache_q"].random_(-127, 128)
+    want = exact(p)[0]
+    assert error(ops.chunk_attention(**p), want) <= more * error(want.to(p["q"].dtype), want)
