@@ -499,13 +499,13 @@ int pkv_accumulate_attention(float *weights, const void *q, int32_t dtype,
  * fp32 [num_blocks, block_size].  A page's new scale is the largest old scale of the
  * tokens it now holds, per KV head, K and V apart; codes become rint(code * (old /
  * new)) where old < new, clamped to -127 .. 127 where old is negative.  The slots
- * that the sequence no longer uses keep their codes and get weight 0.  lens_out int32 [num_seqs] receives the new lengths, kept int32
- * [num_seqs, keep] the old places of the tokens that stay, ascending, then -1.
+ * that the sequence no longer uses keep their codes and get weight 0.  lens_out int32
+ * [num_seqs] (not seq_lens itself: both are read at the end) receives the new lengths,
+ * kept int32 [num_seqs, keep] the old places of the tokens that stay, ascending, then -1.
  * Sequences of at most `keep` tokens stay as they are, and so do those with a page
  * outside the cache (PKV_DEVERR_BAD_BLOCK_ID; their row of kept is -1).  The pages of a
  * sequence that is cut must not be in another sequence's table, nor twice in its own.
- * keep >= 1,
- * sinks + recent <= keep, block_size <= 64, head_dim <= 256.
+ * keep >= 1, sinks + recent <= keep, block_size <= 64, head_dim <= 256.
  */
 int pkv_evict_tokens(int8_t *kv_cache, float *scale_cache, float *weights,
                      const int32_t *block_tables, const int32_t *seq_lens,

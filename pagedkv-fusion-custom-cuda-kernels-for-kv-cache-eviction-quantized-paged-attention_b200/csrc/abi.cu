@@ -787,6 +787,8 @@ int pkv_evict_tokens(int8_t* kv_cache, float* scale_cache, float* weights,
   if (num_seqs > 0 && (!seq_lens || !lens_out || !kept || (max_blocks_per_seq > 0 && !block_tables) ||
                        (num_blocks > 0 && (!kv_cache || !scale_cache || !weights))))
     return fail(PKV_ERR_INVALID_ARGUMENT, "null input or output pointer");
+  if (num_seqs > 0 && lens_out == seq_lens)
+    return fail(PKV_ERR_INVALID_ARGUMENT, "lens_out must not be seq_lens, which is read behind it");
   pkv::EvictArgs a;
   a.cache = kv_cache;
   a.scales = scale_cache;
