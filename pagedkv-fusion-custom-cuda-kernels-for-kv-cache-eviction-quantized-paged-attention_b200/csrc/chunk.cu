@@ -194,10 +194,10 @@ __global__ void __launch_bounds__(kPlanThreads)
 // warp alone takes about 2,000 clocks a step (7 sequences of 40 to 4,000 tokens: 28 us in
 // shares of 16, 12 us in parts of 4).
 //
-// What bounds it: instructions, 440 a step, a third of them the codes' way to fp16, at 0.55
-// a clock and scheduler with 16 warps an SM, and what warps wait for at their start, 14,000
-// clocks of 115,000.  64 sequences of 2,050 tokens, 32 / 8 heads (260 MB): 62 us, 4.2 TB/s;
-// 24 sequences of 1 to 8 tokens behind 100 to 4,000: 60 us.  (Units of 16 rows, 8 warps an
+// What bounds it: instructions, 440 a step, a third of them the codes' way to fp16, and their
+// latencies (0.55 a clock and scheduler, 3.6 warps each), and what warps wait for at their
+// start, 14,000 clocks of 115,000.  64 sequences of 2,050 tokens, 32 / 8 heads (260 MB): 60 us,
+// 4.3 TB/s; 24 sequences of 1 to 8 tokens behind 100 to 4,000: 61 us.  (Units of 16 rows, 8 warps an
 // SM: 78 us for the latter.)
 
 constexpr int kStep = 16;      // keys of a step
@@ -994,7 +994,10 @@ constexpr int kMostWarps = 148 * 2 * kRowWarps;
 // the others to chunk_tc.cu, where it takes the shapes.  (24 sequences of 1 to 8 tokens in
 // groups of 4: 60 us by the warps; 66 us by chunk_tc.cu, or 54 us there for those above 16
 // rows and 28 us by the warps for the rest, since a unit there costs about 10 us to start
-// and end.)  The lengths are on the device, so a call launches both unless its sizes tell.
+// and end.  What a unit costs does not grow with the keys: 24 sequences of 8 tokens, 32 rows,
+// take the warps 55, 152, 603 and 1,160 us behind 1,000, 4,000, 16,000 and 32,000 keys, and
+// chunk_tc.cu 55, 118, 325 and 621; of 4 tokens, 16 rows, 41, 88, 281 and 607 against 41, 89, 323 and
+// 617.)  The lengths are on the device, so a call launches both unless its sizes tell.
 constexpr int kFewRows = 32, kFewSteps = 4096;
 struct Division {
   bool rows, tc;

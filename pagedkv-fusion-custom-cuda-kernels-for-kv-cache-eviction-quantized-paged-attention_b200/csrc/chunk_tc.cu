@@ -18,7 +18,7 @@
 // What bounds it: the softmax warps, 3,900 clocks a pair of row tiles and 128 keys (2,048 of
 // them exponentials) and 1,300 in which they wait for the products between them, against
 // 2,050 of products; the tensor pipe is 37% busy.  2,048 tokens behind 14,336, 32 / 8 heads:
-// 638 us, 807 TFLOP/s.  A unit costs about 10 us to start and end (512 tokens behind 2,800:
+// 636 us, 810 TFLOP/s.  A unit costs about 10 us to start and end (512 tokens behind 2,800:
 // 61 us, 430 TFLOP/s).  Steps of 64 keys with two buffers of S took 720 us.
 //
 // Roles: two softmax warpgroups (thread = row), a loading warp (16 tokens of a page a

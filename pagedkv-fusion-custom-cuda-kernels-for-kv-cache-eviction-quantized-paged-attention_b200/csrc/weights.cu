@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(256) spread_kernel(const int32_t* tables, cons
 // log denominators are not given leave their scores too, so that the keys are read once
 // (64 sequences of 2,050 tokens, 32 / 8 heads: 131 MB of keys, 34 MB of scores written and
 // read); the others' come from a pass of the attention (its V the keys', where that is the
-// tensor-memory kernel).
+// tensor-memory kernel: 512 tokens over 4,096 take 113 us, with their denominators 43).
 constexpr int64_t kMostScores = 128ll << 20;  // bytes
 bool by_scores(const ChunkArgs& a) {
   const int64_t pitch = (int64_t)a.width * a.block_size;

@@ -502,7 +502,10 @@ def accumulate_attention(weights, q, k_cache_q, k_scale, block_tables, seq_lens,
     spreads a weight of 1.
 
     Arguments as in :func:`chunk_attention`; ``lse`` are the log denominators that
-    it returned for the same tokens, computed first where they are not given.  The
+    it returned for the same tokens, computed first where they are not given: by a
+    whole pass of attention for chunks (512 tokens over 4,096: 113 us instead of 43),
+    beside the weights for decode, which is faster without them (64 sequences of
+    2,050 tokens: 50 us instead of 70).  At most 2^25 rows (tokens times heads).  The
     result feeds :func:`eviction_scores` as ``attn_weights`` (whole blocks) and
     :func:`evict_tokens` (single tokens); to let old weight fade, scale
     ``weights`` between calls.  A page in several tables gathers from all of them.
