@@ -10,10 +10,11 @@
 //   P = exp2(...) times the key's V scale, fp16 (again two for fp32), written over S;
 //   O += P V     V's codes as fp16 read MN-major.
 // With 16-bit queries P is one fp16 number, whose 2^-11 adds 0.8% to the error of bf16 results
-// and 43% to that of fp16 ones (3.0e-4 instead of 2.1e-4 of their root mean square): with two, 2,048
-// tokens behind 14,336 take 892 us instead of 647, 512 beside 7 decoding 100 instead of 80.
-// The row tiles take turns on the tensor cores as in prefill.cu; a unit of at most 128 rows has its even key tiles taken by
-// the one and its odd ones by the other, joined at its end.
+// and 43% to that of fp16 ones (3.0e-4 instead of 2.1e-4 of their root mean square): with two,
+// 2,048 tokens behind 14,336 take 892 us instead of 647, 512 beside 7 decoding 100 instead of
+// 80.  The row tiles take turns on the tensor cores as in prefill.cu; a unit of at most 128
+// rows has its even key tiles taken by the one and its odd ones by the other, joined at its
+// end.
 //
 // What bounds it: the softmax warps, 3,900 clocks a pair of row tiles and 128 keys (2,048 of
 // them exponentials) and 1,300 in which they wait for the products between them, against
